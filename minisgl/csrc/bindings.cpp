@@ -437,6 +437,129 @@ void moe_combine(at::Tensor out, at::Tensor y, at::Tensor w, at::Tensor inv, int
                    out.size(1), topk, y.size(0), stream());
 }
 
+// ----- router and 4-bit weights. These allocate their outputs, so that a call costs one crossing of the
+// binding, and run on the tensors' own device and its current stream.
+std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, int64_t topk, bool sigmoid,
+                                                 c10::optional<at::Tensor> bias, int64_t groups, int64_t kept,
+                                                 bool top2, bool renorm, double scale) {
+  check_cuda(logits, "logits");
+  const bool f32 = logits.scalar_type() == at::kFloat;
+  CHECK(f32 || logits.scalar_type() == at::kBFloat16, "logits must be fp32 or bf16");
+  CHECK(logits.dim() == 2, "logits must be [tokens, experts]");
+  const int64_t T = logits.size(0), E = logits.size(1);
+  CHECK(E >= 1 && E <= 512, "route_experts: 1 to 512 experts, got ", E);
+  CHECK(groups >= 1 && groups <= 256 && E % groups == 0, "route_experts: ", E, " experts do not split into ", groups,
+        " groups (at most 256)");
+  CHECK(kept >= 1 && kept <= groups, "route_experts: top_groups must be in [1, ", groups, "], got ", kept);
+  CHECK(topk >= 1 && topk <= 32 && topk <= kept * (E / groups), "route_experts: top_k must be in [1, 32] and at most the ",
+        kept * (E / groups), " experts of the kept groups, got ", topk);
+  CHECK(!top2 || groups == 1 || E / groups >= 2, "route_experts: group_score 'top2' needs two experts per group");
+  CHECK(T < (1ll << 31), "route_experts: too many tokens");
+  const float* b = nullptr;
+  if (bias.has_value()) {
+    check_cuda(*bias, "bias"); check_dtype(*bias, at::kFloat, "bias"); check_contig(*bias, "bias");
+    CHECK(bias->numel() == E && bias->device() == logits.device(), "bias must be [experts] on the logits' device");
+    b = bias->data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  if (logits.stride(1) != 1 && E > 1) logits = logits.contiguous();
+  at::Tensor weights = at::empty({T, topk}, logits.options().dtype(at::kFloat));
+  at::Tensor ids = at::empty({T, topk}, logits.options().dtype(at::kInt));
+  const int rc = msgl_route_experts(logits.data_ptr(), f32, logits.stride(0), b, T, E, topk, sigmoid, groups, kept, top2,
+                                    renorm, scale, weights.data_ptr<float>(), ids.data_ptr<int32_t>(), stream());
+  CHECK(rc == 0, "route_experts failed (code ", rc, ")");
+  return {weights, ids};
+}
+
+// the packed arrays of one 4-bit weight, with the sizes that W4Weight keeps beside them
+MsglW4 w4_of(const at::Tensor& q, const at::Tensor& s, const c10::optional<at::Tensor>& z, int64_t n, int64_t k,
+             int64_t group, bool gated, const at::Device& dev, const char* name) {
+  CHECK(q.is_cuda() && q.device() == dev, name, " must be on the activations' device");
+  check_dtype(q, at::kByte, name); check_contig(q, name); check_contig(s, name);
+  CHECK(q.dim() == 4 && q.size(3) == 512 && s.dim() == 4 && s.size(3) == 16, name, " is not a packed 4-bit weight");
+  CHECK(s.scalar_type() == at::kBFloat16 || s.scalar_type() == at::kHalf, name, " scales must be bf16 or fp16");
+  const int64_t E = q.size(0), tiles = q.size(1), kb = q.size(2), kg = s.size(2);
+  CHECK(group == 32 || group == 64 || group == 128, name, " groups must be 32, 64 or 128 inputs");
+  CHECK(s.device() == dev && s.size(0) == E && s.size(1) == tiles && kg * group >= kb * 64, name, " scales' shape");
+  CHECK(k > 0 && k % 32 == 0 && k <= kb * 64 && kb * 64 - k < 128, name, " inputs do not match its blocks");
+  CHECK(n > 0 && (gated ? n % 2 == 0 && n / 2 <= tiles * 8 : n <= tiles * 16), name, " rows do not match its tiles");
+  CHECK(n < (1ll << 30) && k < (1ll << 30) && tiles * E < (1ll << 31), name, " is too large");
+  if (z.has_value()) {
+    check_dtype(*z, at::kByte, name); check_contig(*z, name);
+    CHECK(z->device() == dev && z->sizes() == s.sizes(), name, " zero points' shape");
+  }
+  CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0 &&
+            reinterpret_cast<uintptr_t>(opt_ptr(z)) % 16 == 0, name, " must be 16-byte aligned");
+  return {q.data_ptr(), s.data_ptr(), opt_ptr(z), (int)tiles, (int)kb, (int)kg, (int)group, (int)n, (int)k,
+          s.scalar_type() == at::kHalf};
+}
+
+// rows as the kernels read them: unit inner stride, every row on a 16-byte boundary (else a copy)
+at::Tensor w4_rows(const at::Tensor& x, int64_t k) {
+  check_bf16(x, "x");
+  CHECK(x.dim() == 2 && x.size(1) == k, "x must be [tokens, ", k, "], got ", x.sizes());
+  if (x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
+    return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+
+at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, c10::optional<at::Tensor> z, int64_t n, int64_t k,
+                     int64_t group, c10::optional<at::Tensor> bias) {
+  check_cuda(x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  const MsglW4 w = w4_of(q, s, z, n, k, group, false, x.device(), "weight");
+  CHECK(q.size(0) == 1, "linear_w4 takes one matrix, not ", q.size(0), " experts");
+  at::Tensor xr = w4_rows(x, k);
+  if (bias.has_value()) {
+    check_bf16(*bias, "bias"); check_contig(*bias, "bias");
+    CHECK(bias->numel() == n && bias->device() == x.device(), "bias size");
+  }
+  const int64_t M = x.size(0);
+  CHECK(M < (1ll << 31), "too many tokens");
+  at::Tensor out = at::empty({M, n}, x.options());
+  const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
+  CHECK(rc == 0, "linear_w4 failed (code ", rc, ")");
+  return out;
+}
+
+at::Tensor experts_w4(at::Tensor x, at::Tensor q1, at::Tensor s1, c10::optional<at::Tensor> z1, int64_t n1, int64_t k1,
+                      int64_t group1, at::Tensor q2, at::Tensor s2, c10::optional<at::Tensor> z2, int64_t n2, int64_t k2,
+                      int64_t group2, at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0,
+                      c10::optional<at::Tensor> b1, c10::optional<at::Tensor> b2) {
+  check_cuda(x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  const MsglW4 w1 = w4_of(q1, s1, z1, n1, k1, group1, true, x.device(), "w1");
+  const MsglW4 w2 = w4_of(q2, s2, z2, n2, k2, group2, false, x.device(), "w2");
+  const int64_t E = q1.size(0), T = x.size(0);
+  CHECK(q2.size(0) == E, "w1 has ", E, " experts, w2 ", q2.size(0));
+  CHECK(k2 == n1 / 2, "w2 takes ", k2, " inputs, w1 gives ", n1 / 2);
+  at::Tensor xr = w4_rows(x, k1);
+  check_i32(ids, "ids"); check_cuda(weights, "weights"); check_dtype(weights, at::kFloat, "weights");
+  check_contig(weights, "weights");
+  CHECK(ids.dim() == 2 && ids.size(0) == T && ids.size(1) >= 1 && weights.sizes() == ids.sizes() &&
+            ids.device() == x.device() && weights.device() == x.device(),
+        "weights and ids must be [tokens, top_k] on the activations' device");
+  CHECK(act >= 0 && act <= 2, "activation must be 0 (silu), 1 (gelu) or 2 (swiglu_oai)");
+  const int64_t topk = ids.size(1);
+  CHECK(T * topk < (1ll << 24), "experts_w4: too many tokens for one call");
+  CHECK(e0 >= 0 && e0 < (1ll << 30), "expert_offset out of range");
+  if (b1.has_value()) {
+    check_bf16(*b1, "w1_bias"); check_contig(*b1, "w1_bias");
+    CHECK(b1->numel() == E * n1 && b1->device() == x.device(), "w1_bias must be [E, 2 I]");
+  }
+  if (b2.has_value()) {
+    check_bf16(*b2, "w2_bias"); check_contig(*b2, "w2_bias");
+    CHECK(b2->numel() == E * n2 && b2->device() == x.device(), "w2_bias must be [E, H]");
+  }
+  at::Tensor out = at::empty({T, n2}, x.options());
+  at::Tensor ws = at::empty({msgl_w4_experts_workspace(T, topk, &w1, &w2)}, x.options().dtype(at::kByte));
+  const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0,
+                                 weights.data_ptr<float>(), ids.data_ptr<int32_t>(), opt_ptr(b1), opt_ptr(b2), act,
+                                 ws.data_ptr(), stream());
+  CHECK(rc == 0, "experts_w4 failed (code ", rc, ")");
+  return out;
+}
+
 // ----- peer-memory collectives
 int64_t peer_alloc(int64_t bytes) {
   void* p = msgl_peer_alloc(bytes);
@@ -567,6 +690,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_decode", &attention_decode);
   m.def("get_error", &get_error);
   m.def("gemm_grouped", &gemm_grouped);
+  m.def("route_experts", &route_experts);
+  m.def("linear_w4", &linear_w4);
+  m.def("experts_w4", &experts_w4);
 
   m.def("moe_route", &moe_route);
   m.def("moe_align", &moe_align, py::arg("ids"), py::arg("E"), py::arg("bn"), py::arg("perm"), py::arg("inv"),

@@ -91,6 +91,29 @@ void msgl_moe_act(void* out, const void* y, int rows, int inter, int act, const 
 void msgl_moe_combine(void* out, const void* y, const float* w, const int32_t* inv, int T, int H, int topk,
                       int y_rows, cudaStream_t s);
 
+// Router with softmax / sigmoid scores, bias, expert groups and top-k (see route.cu): logits fp32 or
+// bf16 [n_tok, E] with a row stride. Returns 0, 3 on unsupported sizes, 4 if the launch failed.
+int msgl_route_experts(const void* logits, int is_fp32, int64_t stride, const float* bias, int n_tok, int E, int topk,
+                       int sigmoid, int groups, int kept, int top2, int renorm, float scale, float* weights,
+                       int32_t* ids, cudaStream_t s);
+
+// ----- 4-bit weights with group scales (layout in w4.cu)
+typedef struct {
+  const void* q;  // [E][tiles][kb][512] bytes
+  const void* s;  // [E][tiles][kg][8][2] 16-bit scales
+  const void* z;  // [E][tiles][kg][8][2] bytes, or null (zero points of 8)
+  int tiles, kb, kg, group, n, k, fp16;
+} MsglW4;
+// out [M, n] = x [M, k] w^T (+ bias). Returns 0, 3 on unsupported sizes, 4 if a launch failed.
+int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
+                   cudaStream_t s);
+// out [T, w2.n] = sum_j weights[t, j] * w2[e] act(w1[e] x[t]), e = ids[t, j] - e0 in [0, E) (others add
+// nothing); w1 gated. Scratch of msgl_w4_experts_workspace bytes, written before it is read.
+int64_t msgl_w4_experts_workspace(int T, int topk, const MsglW4* w1, const MsglW4* w2);
+int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1, const MsglW4* w2,
+                    int E, int e0, const float* weights, const int32_t* ids, const void* b1, const void* b2, int act,
+                    void* workspace, cudaStream_t s);
+
 // ----- paged attention (bf16 q/kv, fp32 softmax)
 void msgl_attention_prefill(void* o, const void* q, const void* k_cache, const void* v_cache,
                             const int32_t* page_table, int64_t pt_stride, const int32_t* rows,

@@ -12,7 +12,9 @@ import torch
 from minisgl._native import cuda as _cuda
 
 from . import reference as ref
+from .moe import route_experts
 from .reference import GATE_UP_BLOCK, deinterleave_gate_up, interleave_gate_up
+from .w4 import W4Weight, experts_w4, linear_w4, quantize_w4
 
 
 def _on_gpu(t: torch.Tensor) -> bool:
@@ -161,5 +163,10 @@ __all__ = [
     "store_kv",
     "argmax",
     "sample",
+    "route_experts",
+    "W4Weight",
+    "quantize_w4",
+    "linear_w4",
+    "experts_w4",
     "ref",
 ]

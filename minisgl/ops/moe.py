@@ -16,6 +16,8 @@ import torch
 
 from minisgl._native import cuda as _cuda
 
+from . import reference as ref
+
 _ACT = {"silu": 0, "gelu": 1, "swiglu_oai": 2}
 _GATED_EPI = {"silu": 1, "gelu": 2, "swiglu_oai": 4}  # grouped-GEMM epilogue applying the activation
 
@@ -54,6 +56,38 @@ def interleave_experts(w1: torch.Tensor, w2: torch.Tensor, b1: torch.Tensor | No
             part[:, :inter] = b1[:, half * inter : (half + 1) * inter]
             vb[:, :, half] = part.view(E, nb, GATE_UP_BLOCK)
     return w1n, w2n, b1n
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: torch.Tensor | None = None,
+                  num_groups: int = 1, top_groups: int = 1, group_score: str = "max", renormalize: bool = True,
+                  scale: float = 1.0):
+    """Experts of every token: (weights fp32 ``[T, top_k]``, ids int32 ``[T, top_k]``, best first).
+
+    ``logits`` (fp32 or bf16 ``[T, E]``, E <= 512, rows may be strided) become scores by ``scoring``,
+    ``softmax`` or ``sigmoid``. Experts are chosen by score + ``bias`` (fp32 ``[E]``, a balancing bias
+    that moves the choice but not the weights), without a bias by their logit; equal ones go to the
+    lowest id, and the order is that of 64-bit arithmetic. With ``num_groups`` > 1 the experts form that
+    many groups of consecutive ids, and only those of the ``top_groups`` best are chosen from: a
+    group counts by its best expert (``group_score="max"``) or by the sum of the two best scores
+    (plus bias) in it (``"top2"``). The weights are the chosen scores, divided by their sum with
+    ``renormalize``, times ``scale``.
+
+    A NaN logit counts as -inf and +inf as the largest fp32 value; a row without a finite logit has
+    softmax scores of zero, and weights whose sum is zero stay zero. NaN biases count as the lowest fp32
+    value, infinite ones as the largest or lowest."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"scoring must be softmax or sigmoid, got {scoring!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(f"group_score must be max or top2, got {group_score!r}")
+    if not logits.is_cuda:
+        T, E = logits.shape
+        if E % num_groups or not 1 <= top_groups <= num_groups or not 1 <= top_k <= min(32, top_groups * (E // num_groups)):
+            raise ValueError(f"cannot choose {top_k} of {E} experts in {top_groups} of {num_groups} groups")
+        if group_score == "top2" and num_groups > 1 and E // num_groups < 2:
+            raise ValueError("group_score 'top2' needs two experts per group")
+        return ref.route_experts(logits, top_k, scoring, bias, num_groups, top_groups, group_score, renormalize, scale)
+    return _cuda().route_experts(logits, top_k, scoring == "sigmoid", bias, num_groups, top_groups,
+                                 group_score == "top2", renormalize, scale)
 
 
 def pick_bn(pairs: int, experts: int) -> int:

@@ -257,6 +257,64 @@ def sample(
     return (out, vals.to(logits.device)) if with_values else out
 
 
+def route_experts(logits, top_k: int, scoring: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1,
+                  group_score: str = "max", renormalize: bool = True, scale: float = 1.0):
+    """See ``ops.route_experts``; scores in 64 bits."""
+    big = torch.finfo(torch.float32).max
+    x = logits.float().nan_to_num(nan=float("-inf"), posinf=big, neginf=float("-inf")).double()
+    T, E = x.shape
+    if scoring == "softmax":
+        mx = x.amax(-1, keepdim=True)
+        e = torch.where(x == float("-inf"), torch.zeros_like(x), torch.exp(x - mx.clamp(min=-big)))
+        p = e / e.sum(-1, keepdim=True).clamp(min=1e-300)
+    else:
+        p = torch.sigmoid(x)
+    if bias is None:
+        v = x.clamp(min=-2.0 * big)  # the order of the scores, and every value finite
+    else:
+        v = p + bias.float().nan_to_num(nan=-big, posinf=big, neginf=-big).double()
+    if num_groups > 1:
+        per = E // num_groups
+        of = p if bias is None and group_score == "top2" else v
+        best = torch.sort(of.view(T, num_groups, per), dim=-1, descending=True).values
+        rank = best[..., 0] if group_score == "max" else best[..., :2].sum(-1)
+        order = torch.sort(rank, dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        keep = torch.zeros(T, num_groups, dtype=torch.bool, device=x.device).scatter_(1, order, True)
+        v = v.masked_fill(~keep.repeat_interleave(per, dim=1), float("-inf"))
+    ids = torch.sort(v, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    w = p.gather(1, ids)
+    if renormalize:
+        total = w.sum(-1, keepdim=True)
+        w = torch.where(total > 0, w / total, torch.zeros_like(w))
+    return (w * scale).float(), ids.to(torch.int32)
+
+
+def linear_w4(x, w, bias=None):
+    y = x.float() @ w.dequant().t()
+    return (y if bias is None else y + bias.float()).to(x.dtype)
+
+
+def experts_w4(x, w1, w2, weights, ids, activation="silu", expert_offset: int = 0, w1_bias=None, w2_bias=None):
+    """See ``ops.experts_w4``; the activated values are rounded once, at the end."""
+    from minisgl.moe.grouped import expert_act
+
+    m1, m2 = w1.dequant(), w2.dequant()
+    out = torch.zeros(x.shape[0], w2.n, dtype=torch.float32, device=x.device)
+    local = ids.long() - expert_offset
+    for e in range(m1.shape[0]):
+        tok, slot = torch.nonzero(local == e, as_tuple=True)
+        if tok.numel() == 0:
+            continue
+        y = x[tok].float() @ m1[e].t()
+        if w1_bias is not None:
+            y = y + w1_bias[e].float()
+        z = expert_act(y, activation) @ m2[e].t()
+        if w2_bias is not None:
+            z = z + w2_bias[e].float()
+        out.index_add_(0, tok, z * weights[tok, slot, None])
+    return out.to(x.dtype)
+
+
 def rope_cos_sin(max_pos: int, rotary_dim: int, inv_freq: torch.Tensor) -> torch.Tensor:
     t = torch.arange(max_pos, dtype=torch.float32)
     f = torch.outer(t, inv_freq.float())

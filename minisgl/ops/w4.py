@@ -1,0 +1,194 @@
+"""4-bit weights with group scales: a linear product and the routed experts of an MoE layer.
+
+``W4Weight`` holds one weight matrix ``[N, K]``, or the matrices ``[E, N, K]`` of a layer's experts,
+whose values are ``(code - zero) * scale``: a code 0..15 per value, and per row and group of 32, 64 or
+128 inputs one bf16 or fp16 scale and optionally a zero point 0..15 (without them every zero point is
+8). ``W4Weight.pack`` takes them as checkpoints hold them and lays them out once in the order in which
+the kernels read them (``csrc/kernels/w4.cu``); ``quantize_w4`` makes them from bf16 weights.
+
+    w = ops.W4Weight.pack(q, scales, zeros)               # q [N, K/2] uint8, scales / zeros [N, K/group]
+    y = ops.linear_w4(x, w, bias)                         # [M, K] bf16 -> [M, N] bf16
+
+    w1 = ops.W4Weight.pack(q1, s1, gated=True)            # [E, 2I, H]: gate rows, then up rows
+    w2 = ops.W4Weight.pack(q2, s2)                        # [E, H, I]
+    weights, ids = ops.route_experts(router_logits, top_k)
+    y = ops.experts_w4(x, w1, w2, weights, ids)
+
+CUDA tensors run the sm_100a kernels, CPU tensors the plain form in ``ops.reference``. Calls may be
+captured in CUDA graphs; they keep no state of their own, so calls on several streams are independent.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+import torch.nn.functional as F
+
+from minisgl._native import cuda as _cuda
+
+from . import reference as ref
+
+GROUP_SIZES = (32, 64, 128)
+_ACT = {"silu": 0, "gelu": 1, "swiglu_oai": 2}
+
+
+@dataclass
+class W4Weight:
+    q: torch.Tensor           # uint8 [E, Nt, KB, 512]: tiles of 16 rows x 64 inputs
+    s: torch.Tensor           # bf16 / fp16 [E, Nt, KG, 16]: (row g, row g + 8) pairs
+    z: torch.Tensor | None    # uint8 like s, or None: 8 everywhere
+    n: int                    # rows
+    k: int                    # inputs
+    group: int                # inputs per scale
+    gated: bool               # tiles of 8 gate rows and the 8 up rows of the same outputs
+    experts: bool             # [E, N, K] rather than one [N, K]
+
+    @property
+    def shape(self):
+        return (self.q.shape[0], self.n, self.k) if self.experts else (self.n, self.k)
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.q.is_cuda
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def nbytes(self) -> int:
+        z = 0 if self.z is None else self.z.numel()
+        return self.q.numel() + self.s.numel() * self.s.element_size() + z
+
+    def to(self, device) -> "W4Weight":
+        z = None if self.z is None else self.z.to(device)
+        return W4Weight(self.q.to(device), self.s.to(device), z, self.n, self.k, self.group, self.gated, self.experts)
+
+    @classmethod
+    def pack(cls, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+             gated: bool = False) -> "W4Weight":
+        """``q`` uint8 ``[(E,) N, K/2]``, two codes a byte along the inputs, the low nibble first;
+        ``scales`` bf16 / fp16 and ``zeros`` uint8 (0..15) ``[(E,) N, K/group]``. ``gated``: the rows
+        are ``[gate; up]`` halves, as in the first matrix of a gated MLP."""
+        if q.dtype != torch.uint8 or q.dim() not in (2, 3):
+            raise ValueError(f"4-bit codes must be uint8 [N, K/2] or [E, N, K/2], got {q.dtype} {tuple(q.shape)}")
+        experts = q.dim() == 3
+        if scales.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"4-bit scales must be bf16 or fp16, got {scales.dtype}")
+        if scales.dim() != q.dim() or scales.shape[:-1] != q.shape[:-1] or scales.shape[-1] == 0 or q.numel() == 0:
+            raise ValueError(f"4-bit codes {tuple(q.shape)} / scales {tuple(scales.shape)} mismatch")
+        k = 2 * q.shape[-1]
+        group = k // scales.shape[-1]
+        if group not in GROUP_SIZES or group * scales.shape[-1] != k:
+            raise ValueError(f"{k} inputs over {scales.shape[-1]} scales a row: groups must be 32, 64 or 128 inputs")
+        if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+            raise ValueError(f"4-bit zero points must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
+        n = q.shape[-2]
+        if gated and n % 2:
+            raise ValueError(f"a gated weight has as many gate as up rows, got {n} rows")
+        if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+            raise ValueError("4-bit zero points must be 0..15")
+        if any(t is not None and t.device != q.device for t in (scales, zeros)):
+            raise ValueError("4-bit codes, scales and zero points must be on one device")
+        if not experts:
+            q, scales, zeros = q[None], scales[None], None if zeros is None else zeros[None]
+        E = q.shape[0]
+        nt = -(-(n // 2) // 8) if gated else -(-n // 16)
+        kb = -(-k // 64)
+        kg = -(-kb * 64 // group)
+
+        def tiles(t: torch.Tensor, cols: int) -> torch.Tensor:
+            """[E, N, c] -> [E, Nt, 2, 8, cols]: the rows g and g + 8 of every tile, zeros beyond the end"""
+            t = F.pad(t, (0, cols - t.shape[-1]))
+            if gated:
+                t = F.pad(t.unflatten(1, (2, n // 2)), (0, 0, 0, nt * 8 - n // 2))
+                return t.unflatten(2, (nt, 8)).transpose(1, 2)
+            return F.pad(t, (0, 0, 0, nt * 16 - n)).unflatten(1, (nt, 2, 8))
+
+        # bytes of a row by (block, half h, lane column t, word j, byte i): codes 2i (low) and 2i + 1
+        b = tiles(q, kb * 32).unflatten(-1, (kb, 2, 4, 2, 2))
+        lo, hi = b[:, :, 0], b[:, :, 1]  # rows g, rows g + 8: [E, Nt, 8, KB, 2, 4, 2, 2]
+        out = torch.empty(E, nt, kb, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=q.device)
+        perm = (0, 1, 3, 2, 5, 4, 6, 7)  # -> [E, Nt, KB, g, t, h, j, i]
+        out[..., 0, :] = ((lo & 15) | (hi << 4)).permute(perm)
+        out[..., 1, :] = ((lo >> 4) | (hi & 0xF0)).permute(perm)
+        s = tiles(scales, kg).permute(0, 1, 4, 3, 2).reshape(E, nt, kg, 16)
+        z = None if zeros is None else tiles(zeros, kg).permute(0, 1, 4, 3, 2).reshape(E, nt, kg, 16).contiguous()
+        return cls(out.view(E, nt, kb, 512), s.contiguous(), z, n, k, group, gated, experts)
+
+    def codes(self):
+        """(q, scales, zeros) as ``pack`` took them."""
+        E, nt, kb, _ = self.q.shape
+        c = self.q.view(E, nt, kb, 8, 4, 2, 2, 2, 2).permute(0, 1, 3, 2, 5, 4, 6, 7, 8)  # [E, Nt, g, KB, h, t, j, c, i]
+        even, odd = c[..., 0, :], c[..., 1, :]
+        b = torch.stack([(even & 15) | ((odd & 15) << 4), (even >> 4) | (odd & 0xF0)], dim=2)  # [E, Nt, 2, g, KB, h, t, j, i]
+
+        def rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+            t = t.flatten(4)[..., :cols]
+            if self.gated:
+                return t.transpose(1, 2).flatten(2, 3)[:, :, : self.n // 2].flatten(1, 2).contiguous()
+            return t.flatten(1, 3)[:, : self.n].contiguous()
+
+        side = lambda t: rows(t.view(E, nt, -1, 8, 2).permute(0, 1, 4, 3, 2), self.k // self.group)  # noqa: E731
+        got = (rows(b, self.k // 2), side(self.s), None if self.z is None else side(self.z))
+        return got if self.experts else tuple(t if t is None else t[0] for t in got)
+
+    def dequant(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The ``[(E,) N, K]`` weights that the codes stand for."""
+        q, s, z = self.codes()
+        v = torch.stack([q & 15, q >> 4], dim=-1).flatten(-2).float().unflatten(-1, (-1, self.group))
+        zero = 8.0 if z is None else z.float().unsqueeze(-1)
+        return ((v - zero) * s.float().unsqueeze(-1)).flatten(-2).to(dtype)
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, scale_dtype: torch.dtype = torch.bfloat16):
+    """Rounds ``w [(E,) N, K]`` to 4 bits, per group of ``group`` inputs: (q, scales, zeros) for
+    ``W4Weight.pack``. Symmetric: the largest magnitude becomes 7 steps around a zero point of 8
+    (``zeros`` is None); otherwise the group's range, widened to hold 0, is cut into 15 steps."""
+    if group not in GROUP_SIZES or w.shape[-1] % group:
+        raise ValueError(f"{w.shape[-1]} inputs do not split into groups of {group} (32, 64 or 128)")
+    v = w.float().unflatten(-1, (-1, group))
+    if symmetric:
+        s = (v.abs().amax(-1) / 7).to(scale_dtype)
+        z = None
+        zero = 8.0
+    else:
+        lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
+        s = ((hi - lo) / 15).to(scale_dtype)
+        step = s.float()
+        z = torch.where(step > 0, torch.round(-lo / step), torch.zeros_like(lo)).clamp(0, 15)
+        zero = z.unsqueeze(-1)
+        z = z.to(torch.uint8)
+    step = s.float().unsqueeze(-1)
+    code = torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)) + zero
+    code = code.clamp(0, 15).to(torch.uint8).flatten(-2)
+    return (code[..., 0::2] | (code[..., 1::2] << 4)).contiguous(), s, z
+
+
+def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ w^T (+ bias)`` for bf16 ``x [M, K]`` and a 4-bit ``w [N, K]``; bf16 ``[M, N]``. Sums are
+    held in fp32. Rows of ``x`` may be strided."""
+    if w.experts or w.gated:
+        raise ValueError("linear_w4 takes one ungated matrix")
+    if not x.is_cuda:
+        return ref.linear_w4(x, w, bias)
+    return _cuda().linear_w4(x, w.q, w.s, w.z, w.n, w.k, w.group, bias)
+
+
+def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tensor, ids: torch.Tensor, *,
+               activation: str = "silu", expert_offset: int = 0, w1_bias: torch.Tensor | None = None,
+               w2_bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * (w2[e] act(w1[e] x[t]))`` with ``e = ids[t, j] - expert_offset``.
+
+    ``w1 [E, 2I, H]`` is packed with ``gated=True``, ``w2 [E, H, I]`` without; ``weights`` fp32 and
+    ``ids`` int32 ``[T, k]`` come from ``route_experts``. Ids of experts that are not here (expert
+    parallelism) add nothing. ``activation``: ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``.
+    The activated values between the two products are held in bf16, sums in fp32."""
+    if not (w1.experts and w1.gated and w2.experts and not w2.gated):
+        raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")
+    if activation not in _ACT:
+        raise ValueError(f"activation must be one of {sorted(_ACT)}, got {activation!r}")
+    if not x.is_cuda:
+        return ref.experts_w4(x, w1, w2, weights, ids, activation, expert_offset, w1_bias, w2_bias)
+    return _cuda().experts_w4(x, w1.q, w1.s, w1.z, w1.n, w1.k, w1.group, w2.q, w2.s, w2.z, w2.n, w2.k, w2.group,
+                              weights, ids, _ACT[activation], expert_offset, w1_bias, w2_bias)
