@@ -1,239 +1,208 @@
-// Products with 4-bit weights and group scales: w[n, k] = (code - zero) * scale(row n, group of k).
+// The 4-bit linear product out [M, N] = x [M, K] w^T (+ bias); see w4.cuh for the weights' layout and
+// the streaming product.
 //
-// Packed weights (ops/w4.py lays them out once): tiles of 16 rows by 64 inputs, 512 bytes each, in the
-// order of the tensor core's A fragments, so that a warp's 16-byte loads are one tile:
-//   q [E][Nt][KB][32 lanes][4 words], lane = 4 g + t. Word 2h + j holds, for k = 64 kb + 32 h + 8 t + 4 j,
-//     row g     codes k, k+1, k+2, k+3 in nibbles 0, 4, 2, 6
-//     row g + 8 codes k, k+1, k+2, k+3 in nibbles 1, 5, 3, 7
-//   s [E][Nt][KG][8][2] 16-bit scales of rows g and g + 8, z likewise in bytes (none: 8).
-// Rows and inputs are padded to whole tiles with scales of zero. In a gated weight rows 0-7 of a tile
-// are gate rows 8 i .. 8 i + 7 and rows 8-15 the up rows of the same outputs.
-#include <cuda_fp16.h>
-
+// Few tokens: persistent CTAs of 16 warps, one per SM. With `splits` > 1 a cluster of that many CTAs
+// shares its tiles and cuts the inputs: each CTA reads its share of the activations only, and the sums
+// meet through distributed shared memory. The split is the one whose largest share of weights, plus the
+// activations that every CTA reads, is smallest (plan()).
 #include <algorithm>
+#include <mutex>
 
-#include "api.h"
-#include "common.cuh"
+#include "w4.cuh"
 
 using namespace msgl;
 
 namespace {
 
-struct W4Tensor {
-  const uint4* q;
-  const uint32_t* s;  // two 16-bit scales
-  const uint16_t* z;  // two zero points, or null
-  int tiles, kb, kg, group, n, k, fp16;
+struct LinearArgs {
+  W4Tensor w;
+  const __nv_bfloat16* x;
+  int64_t x_stride;
+  int M;
+  const __nv_bfloat16* bias;
+  __nv_bfloat16* out;
+  int splits, max_tiles;
 };
 
-__device__ __forceinline__ float2 scale2(uint32_t v, int fp16) {
-  if (fp16) return __half22float2(*reinterpret_cast<__half2*>(&v));
-  return make_float2(bf16_lo(v), bf16_hi(v));
-}
+template <int NT, int G, bool Z>
+__global__ void __launch_bounds__(kW4Threads, 1) w4_linear_kernel(const __grid_constant__ LinearArgs p) {
+  using C = W4Chunk<G>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int clusters = gridDim.x / p.splits, cl = blockIdx.x / p.splits, rank = blockIdx.x % p.splits;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int t0 = (int)((int64_t)p.w.tiles * cl / clusters), t1 = (int)((int64_t)p.w.tiles * (cl + 1) / clusters);
+  const int chunks = p.w.kb / C::kUnits;
+  const int c0 = chunks * rank / p.splits, nc = chunks * (rank + 1) / p.splits - c0;
+  float4* part = reinterpret_cast<float4*>(smem);
+  float4* sums = reinterpret_cast<float4*>(smem + w4_part_bytes<NT>());  // [max_tiles][NT][32] with splits
+  const int sum_bytes = p.splits > 1 ? p.max_tiles * NT * 512 : 0;
+  uint8_t* xs = smem + w4_part_bytes<NT>() + sum_bytes;
+  const int kn = nc * C::kUnits * 64, pitch = w4_pitch(kn);
 
-// acc[m][0/1] += rows g and g + 8 of tile (e, nt) times x[m] over 64-input blocks kb0, kb0 + step, ...
-template <int MT>
-__device__ __forceinline__ void tile_dot(const W4Tensor& w, int64_t tile, const __nv_bfloat16* const (&x)[MT], int kb0,
-                                         int step, float (&acc)[MT][2]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint4* q = w.q + tile * w.kb * 32 + lane;
-  const uint32_t* s = w.s + tile * w.kg * 8 + g;
-  const uint16_t* z = w.z == nullptr ? nullptr : w.z + tile * w.kg * 8 + g;
-  for (int kb = kb0; kb < w.kb; kb += step) {
-    const uint4 v = q[(int64_t)kb * 32];
-    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+  pdl_launch();
+  // the weights do not depend on earlier kernels' results, but may have been written by one: they may be
+  // brought into L2 before the wait, not read
+  if (lane == 0 && t1 > t0) {
+    const int64_t total = (int64_t)(t1 - t0) * nc;
+    const int a = (int)(total * warp / kW4Warps), b = (int)(total * (warp + 1) / kW4Warps);
+    const int n = min(min(b - a, nc - a % nc), C::kDepth * 2);
+    if (n > 0)
+      prefetch_l2(p.w.q + ((int64_t)(t0 + a / nc) * p.w.kb + (c0 + a % nc) * C::kUnits) * 32, n * C::kUnits * 512);
+  }
+  pdl_wait();
+  if (t1 == t0) return;  // the same for every CTA of a cluster
+
+  const auto store = [&](int tile, const float (&acc)[NT][4]) {
+    const int n = (t0 + tile) * 16 + g;
+    const float b0 = p.bias != nullptr && n < p.w.n ? __bfloat162float(p.bias[n]) : 0.f;
+    const float b1 = p.bias != nullptr && n + 8 < p.w.n ? __bfloat162float(p.bias[n + 8]) : 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = kb * 64 + h * 32 + t * 8;
-      const int grp = (kb * 64 + h * 32) / w.group;
-      const float2 sc = scale2(s[grp * 8], w.fp16);
-      const uint32_t zz = z == nullptr ? 0x0808u : z[grp * 8];
-      const float z0 = (float)(zz & 255), z1 = (float)(zz >> 8);
-      if (k >= w.k) continue;
-      float a[8], b[8];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t u = words[2 * h + j];
-        constexpr int pos[4] = {0, 4, 2, 6};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[4 * j + i] = (float)((u >> (4 * pos[i])) & 15) - z0;
-          b[4 * j + i] = (float)((u >> (4 * pos[i] + 4)) & 15) - z1;
-        }
+      for (int c = 0; c < 2; ++c) {
+        const int m = nt * 8 + 2 * t + c;
+        if (m >= p.M) continue;
+        __nv_bfloat16* o = p.out + (int64_t)m * p.w.n + n;
+        if (n < p.w.n) o[0] = __float2bfloat16(acc[nt][c] + b0);
+        if (n + 8 < p.w.n) o[8] = __float2bfloat16(acc[nt][2 + c] + b1);
       }
+  };
+  const auto load = [&] {
+    load_rows(xs, pitch, p.M, c0 * C::kUnits * 64, kn, p.w.k, [&](int r) { return p.x + (int64_t)r * p.x_stride; });
+  };
+  if (p.splits == 1) {
+    run_tiles<NT, G, Z>(p.w, t0, t1 - t0, c0, nc, xs, pitch, p.M, part, load, store);
+    return;
+  }
+  run_tiles<NT, G, Z>(p.w, t0, t1 - t0, c0, nc, xs, pitch, p.M, part, load, [&](int tile, const float (&acc)[NT][4]) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4 xv = *reinterpret_cast<const uint4*>(x[m] + k);
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-        float da = 0.f, db = 0.f;
+    for (int nt = 0; nt < NT; ++nt)
+      sums[(tile * NT + nt) * 32 + lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+  });
+  cluster_sync();
+  for (int tile = rank * kW4Warps + warp; tile < t1 - t0; tile += p.splits * kW4Warps) {
+    float acc[NT][4] = {};
+    for (int r = 0; r < p.splits; ++r) {
+      const uint32_t from = dsmem_addr(smem_u32(sums + (tile * NT) * 32 + lane), r);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x0 = bf16_lo(xw[i]), x1 = bf16_hi(xw[i]);
-          da += a[2 * i] * x0 + a[2 * i + 1] * x1;
-          db += b[2 * i] * x0 + b[2 * i + 1] * x1;
-        }
-        acc[m][0] += da * sc.x;
-        acc[m][1] += db * sc.y;
+      for (int nt = 0; nt < NT; ++nt) {
+        const float4 v = ld_dsmem_v4(from + nt * 512);
+        acc[nt][0] += v.x, acc[nt][1] += v.y, acc[nt][2] += v.z, acc[nt][3] += v.w;
       }
     }
+    store(tile, acc);
   }
+  cluster_sync();  // the other CTAs of the cluster read this one's shared memory
 }
 
-// number of an expert among those from e0 on; wraps to a large number for one that is not here
-__device__ __forceinline__ unsigned local_expert(int32_t id, int e0) { return (unsigned)id - (unsigned)e0; }
+constexpr int kSmemMax = 227 * 1024;
 
-constexpr int kDotWarps = 4;
+struct Plan {
+  int splits, grid, max_tiles, smem;
+};
 
-// sums a tile's 16 rows over the lanes and warps of the CTA into red[row][m]
-template <int MT>
-__device__ __forceinline__ void tile_reduce(float (&acc)[MT][2], float (*red)[16][MT]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float v = acc[m][r];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if ((lane & 3) == 0) red[warp][(lane >> 2) + 8 * r][m] = v;
+// CTAs of a cluster of `splits` that run at once, in whole clusters (148 SMs, not all in groups of 8)
+template <auto Kernel>
+int resident_ctas(int splits) {
+  static std::mutex mu;
+  static int known[64][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> guard(mu);
+  int& k = known[dev][splits];
+  if (k != 0) return k;
+  if (splits == 1) return k = msgl_num_sms();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits);
+  cfg.blockDim = dim3(kW4Threads);
+  cfg.dynamicSmemBytes = kSmemMax;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  return k = n * splits;
+}
+
+// The split of the inputs with the least estimated time: the largest CTA's weight bytes at an SM's
+// share of the memory rate (43 B/ns), its activations at the L2's (four times that), and 1.5 us for the
+// exchange. Returns splits = 0 if the rows do not fit.
+template <auto Kernel, int NT, int G>
+Plan plan(const W4Tensor& w, int M) {
+  const int chunks = w.kb / W4Chunk<G>::kUnits;
+  Plan best = {0, 0, 0, 0};
+  double best_ns = 1e30;
+  for (int s = 1; s <= 8; s *= 2) {
+    if (s > chunks) break;
+    const int clusters = std::min(resident_ctas<Kernel>(s) / s, w.tiles);
+    if (clusters < 1) continue;
+    const int tiles = (w.tiles + clusters - 1) / clusters;
+    const int kn = (chunks + s - 1) / s * W4Chunk<G>::kUnits * 64;
+    const int64_t smem = w4_part_bytes<NT>() + (s > 1 ? (int64_t)tiles * NT * 512 : 0) + (int64_t)M * w4_pitch(kn);
+    if (smem > kSmemMax) continue;
+    const double ns = tiles * (kn / 64) * 512.0 / 43 + M * kn * 2.0 / 172 + (s > 1 ? 1500 : 0);
+    if (ns < best_ns) {
+      best_ns = ns;
+      best = {s, clusters * s, tiles, (int)smem};
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * MT; i += blockDim.x) {
-    float v = 0.f;
-    for (int w = 0; w < kDotWarps; ++w) v += red[w][i / MT][i % MT];
-    red[0][i / MT][i % MT] = v;
   }
-  __syncthreads();
+  return best;
 }
 
-constexpr int kLinM = 4;
+template <int NT, int G, bool Z>
+int launch_linear(LinearArgs p, cudaStream_t s) {
+  constexpr auto kernel = w4_linear_kernel<NT, G, Z>;
+  if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
+  const Plan pl = plan<kernel, NT, G>(p.w, p.M);
+  if (pl.splits == 0) return 3;
+  p.splits = pl.splits;
+  p.max_tiles = pl.max_tiles;
+  return msgl_launch(kernel, dim3(pl.grid), dim3(kW4Threads), pl.smem, s, pl.splits, p) == cudaSuccess ? 0 : 4;
+}
 
-__global__ void __launch_bounds__(kDotWarps * 32)
-w4_linear_kernel(W4Tensor w, const __nv_bfloat16* __restrict__ x, int64_t x_stride, int M,
-                 const __nv_bfloat16* __restrict__ bias, __nv_bfloat16* __restrict__ out) {
-  pdl_wait();
-  pdl_launch();
-  __shared__ float red[kDotWarps][16][kLinM];
-  const int tile = blockIdx.x, m0 = blockIdx.y * kLinM;
-  const __nv_bfloat16* rows[kLinM];
-#pragma unroll
-  for (int m = 0; m < kLinM; ++m) rows[m] = x + (int64_t)min(m0 + m, M - 1) * x_stride;
-  float acc[kLinM][2] = {};
-  tile_dot<kLinM>(w, tile, rows, threadIdx.x >> 5, kDotWarps, acc);
-  tile_reduce<kLinM>(acc, red);
-  for (int i = threadIdx.x; i < 16 * kLinM; i += blockDim.x) {
-    const int m = i >> 4, n = tile * 16 + (i & 15);
-    if (m0 + m < M && n < w.n) {
-      const float b = bias == nullptr ? 0.f : __bfloat162float(bias[n]);
-      out[(int64_t)(m0 + m) * w.n + n] = __float2bfloat16(red[0][i & 15][m] + b);
-    }
+template <int NT>
+int launch_linear_nt(const LinearArgs& p, cudaStream_t s) {
+  const bool z = p.w.z != nullptr;
+  switch (p.w.group) {
+    case 32: return z ? launch_linear<NT, 32, true>(p, s) : launch_linear<NT, 32, false>(p, s);
+    case 64: return z ? launch_linear<NT, 64, true>(p, s) : launch_linear<NT, 64, false>(p, s);
+    default: return z ? launch_linear<NT, 128, true>(p, s) : launch_linear<NT, 128, false>(p, s);
   }
 }
 
-__device__ __forceinline__ float gated_act(float g, float u, int act) {
-  if (act == 0) return g / (1.f + __expf(-g)) * u;
-  if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-  g = fminf(g, 7.f);
-  u = fminf(fmaxf(u, -7.f), 7.f);
-  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
-}
-
-// a[pair] = act(gate) * up of the pair's expert; zeros for an expert that is not here
-__global__ void __launch_bounds__(kDotWarps * 32)
-w4_gate_up_kernel(W4Tensor w, int E, int e0, const __nv_bfloat16* __restrict__ x, int64_t x_stride, int topk,
-                  const int32_t* __restrict__ ids, const __nv_bfloat16* __restrict__ bias, int act,
-                  __nv_bfloat16* __restrict__ a, int a_stride) {
-  pdl_wait();
-  pdl_launch();
-  __shared__ float red[kDotWarps][16][1];
-  const int tile = blockIdx.x, pair = blockIdx.y, inter = w.n / 2;
-  const unsigned e = local_expert(ids[pair], e0);
-  if (e >= (unsigned)E) return;
-  const __nv_bfloat16* rows[1] = {x + (int64_t)(pair / topk) * x_stride};
-  float acc[1][2] = {};
-  tile_dot<1>(w, (int64_t)e * w.tiles + tile, rows, threadIdx.x >> 5, kDotWarps, acc);
-  tile_reduce<1>(acc, red);
-  const int i = threadIdx.x, n = tile * 8 + i;
-  if (i < 8 && n < inter) {
-    float g = red[0][i][0], u = red[0][i + 8][0];
-    if (bias != nullptr) {
-      g += __bfloat162float(bias[(int64_t)e * w.n + n]);
-      u += __bfloat162float(bias[(int64_t)e * w.n + inter + n]);
-    }
-    a[(int64_t)pair * a_stride + n] = __float2bfloat16(gated_act(g, u, act));
-  }
-}
-
-__global__ void __launch_bounds__(kDotWarps * 32)
-w4_down_kernel(W4Tensor w, int E, int e0, const __nv_bfloat16* __restrict__ a, int a_stride,
-               const int32_t* __restrict__ ids, const __nv_bfloat16* __restrict__ bias, float* __restrict__ y) {
-  pdl_wait();
-  pdl_launch();
-  __shared__ float red[kDotWarps][16][1];
-  const int tile = blockIdx.x, pair = blockIdx.y;
-  const unsigned e = local_expert(ids[pair], e0);
-  if (e >= (unsigned)E) return;
-  const __nv_bfloat16* rows[1] = {a + (int64_t)pair * a_stride};
-  float acc[1][2] = {};
-  tile_dot<1>(w, (int64_t)e * w.tiles + tile, rows, threadIdx.x >> 5, kDotWarps, acc);
-  tile_reduce<1>(acc, red);
-  const int n = tile * 16 + threadIdx.x;
-  if (threadIdx.x < 16 && n < w.n)
-    y[(int64_t)pair * w.n + n] =
-        red[0][threadIdx.x][0] + (bias == nullptr ? 0.f : __bfloat162float(bias[(int64_t)e * w.n + n]));
-}
-
-__global__ void w4_combine_kernel(const float* __restrict__ y, const float* __restrict__ weights,
-                                  const int32_t* __restrict__ ids, int E, int e0, int topk, int H,
-                                  __nv_bfloat16* __restrict__ out) {
-  pdl_wait();
-  pdl_launch();
-  const int t = blockIdx.x;
-  for (int c = threadIdx.x; c < H; c += blockDim.x) {
-    float v = 0.f;
-    for (int j = 0; j < topk; ++j) {
-      if (local_expert(ids[(int64_t)t * topk + j], e0) < (unsigned)E) v += weights[(int64_t)t * topk + j] * y[((int64_t)t * topk + j) * H + c];
-    }
-    out[(int64_t)t * H + c] = __float2bfloat16(v);
-  }
-}
-
-W4Tensor tensor_of(const MsglW4* w) {
-  return {(const uint4*)w->q, (const uint32_t*)w->s, (const uint16_t*)w->z, w->tiles, w->kb, w->kg, w->group,
-          w->n, w->k, w->fp16};
+// rows in one launch if their activations fit into shared memory, else in halves
+int linear_rows(const LinearArgs& p, cudaStream_t s) {
+  const int rc = p.M <= 8 ? launch_linear_nt<1>(p, s) : p.M <= 16 ? launch_linear_nt<2>(p, s) : launch_linear_nt<4>(p, s);
+  if (rc != 3 || p.M == 1) return rc;
+  LinearArgs a = p, b = p;
+  a.M = p.M > 16 ? 16 : p.M > 8 ? 8 : p.M / 2;
+  b.M = p.M - a.M;
+  b.x += a.M * p.x_stride;
+  b.out += (int64_t)a.M * p.w.n;
+  const int ra = linear_rows(a, s);
+  return ra != 0 ? ra : linear_rows(b, s);
 }
 
 }  // namespace
 
 extern "C" int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
                               cudaStream_t s) {
-  if (M == 0 || w->n == 0) return 0;
-  const cudaError_t e =
-      msgl_launch(w4_linear_kernel, dim3(w->tiles, (M + kLinM - 1) / kLinM), dim3(kDotWarps * 32), 0, s, 1,
-                  tensor_of(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias, (__nv_bfloat16*)out);
-  return e == cudaSuccess ? 0 : 4;
-}
-
-extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, const MsglW4* w1, const MsglW4* w2) {
-  const int64_t pairs = (int64_t)T * topk;
-  return pairs * w2->kb * 64 * 2 + pairs * w2->n * 4;
-}
-
-extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
-                               const MsglW4* w2, int E, int e0, const float* weights, const int32_t* ids,
-                               const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
-  if (T == 0) return 0;
-  const int pairs = T * topk, a_stride = w2->kb * 64;
-  __nv_bfloat16* a = (__nv_bfloat16*)workspace;
-  float* y = (float*)((uint8_t*)workspace + (int64_t)pairs * a_stride * 2);
-  cudaError_t e = msgl_launch(w4_gate_up_kernel, dim3(w1->tiles, pairs), dim3(kDotWarps * 32), 0, s, 1, tensor_of(w1),
-                              E, e0, (const __nv_bfloat16*)x, x_stride, topk, ids, (const __nv_bfloat16*)b1, act, a,
-                              a_stride);
-  if (e == cudaSuccess)
-    e = msgl_launch(w4_down_kernel, dim3(w2->tiles, pairs), dim3(kDotWarps * 32), 0, s, 1, tensor_of(w2), E, e0,
-                    (const __nv_bfloat16*)a, a_stride, ids, (const __nv_bfloat16*)b2, y);
-  if (e == cudaSuccess)
-    e = msgl_launch(w4_combine_kernel, dim3(T), dim3(256), 0, s, 1, (const float*)y, weights, ids, E, e0, topk, w2->n,
-                    (__nv_bfloat16*)out);
-  return e == cudaSuccess ? 0 : 4;
+  if (M == 0) return 0;
+  LinearArgs p = {w4_tensor(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias, (__nv_bfloat16*)out,
+                  1, 0};
+  for (int m = 0; m < M; m += 32) {
+    LinearArgs a = p;
+    a.M = std::min(32, M - m);
+    a.x += m * x_stride;
+    a.out += (int64_t)m * w->n;
+    const int rc = linear_rows(a, s);
+    if (rc != 0) return rc;
+  }
+  return 0;
 }

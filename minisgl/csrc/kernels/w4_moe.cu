@@ -1,0 +1,241 @@
+// The experts' products of an MoE layer with 4-bit weights (layout and streaming product in w4.cuh):
+//   a[p] = act(w1[e] x[token]) for every (token, choice) pair p, y[p] = w2[e] a[p], out = sum of weight * y.
+//
+// Few tokens: the chosen experts' tiles, one after another, are cut into equal runs, one per SM. Every CTA
+// counts the pairs per expert itself (they are few) instead of waiting for a kernel that would, so a
+// layer is three launches; the counting of the second product overlaps the end of the first. The
+// activated values between the products are bf16, as the second product's operands are; y is fp32 and
+// the sum over a token's experts runs in the order of its choices, so results do not vary.
+#include <algorithm>
+
+#include "w4.cuh"
+
+using namespace msgl;
+
+namespace {
+
+constexpr int kMoeMaxPairs = 4096;  // pairs of one launch: the list of an expert's pairs is in shared memory
+constexpr int kMoeMaxExperts = 1024;
+constexpr int kSmemMax = 227 * 1024;
+
+// number of an expert among those from e0 on; wraps to a large number for one that is not here
+MSGL_DEVICE unsigned local_expert(int32_t id, int e0) { return (unsigned)id - (unsigned)e0; }
+
+MSGL_DEVICE float gated_act(float g, float u, int act) {
+  if (act == 0) return g / (1.f + __expf(-g)) * u;
+  if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
+  g = fminf(g, 7.f);
+  u = fminf(fmaxf(u, -7.f), 7.f);
+  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
+}
+
+struct ExpertArgs {
+  W4Tensor w;
+  int E, e0, pairs, topk;
+  const int32_t* ids;
+  const __nv_bfloat16* in;  // rows of x (gated: token pair / topk) or of the activated values (pair)
+  int64_t in_stride;
+  const __nv_bfloat16* bias;  // [E, n]
+  __nv_bfloat16* a;           // gated: [pairs, a_stride]
+  float* y;                   // else: [pairs, n]
+  int a_stride, act, rows;    // rows: tokens of one pass
+};
+
+template <int NT, int G, bool Z, bool GATED>
+__global__ void __launch_bounds__(kW4Threads, 1) w4_experts_kernel(const __grid_constant__ ExpertArgs p) {
+  using C = W4Chunk<G>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float4* part = reinterpret_cast<float4*>(smem);
+  int* count = reinterpret_cast<int*>(smem + w4_part_bytes<NT>());  // [E] pairs of every expert
+  int* hit = count + p.E;                                           // the experts that have any
+  int* list = hit + p.E;                                            // [pairs] pairs of one expert
+  uint8_t* xs = reinterpret_cast<uint8_t*>(list) + (p.pairs * 4 + 15) / 16 * 16 + (p.E * 8 % 16);
+  __shared__ int n_hit, n_list;
+
+  // The second product's ids were complete before the first product's kernel began its work, which is
+  // before this kernel could start (it triggers its dependents after its own wait).
+  if constexpr (GATED) pdl_wait();
+  pdl_launch();
+  for (int e = threadIdx.x; e < p.E; e += kW4Threads) count[e] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.pairs; i += kW4Threads) {
+    const unsigned e = local_expert(p.ids[i], p.e0);
+    if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int n = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const bool any = e0 + lane < p.E && count[e0 + lane] > 0;
+      const unsigned m = __ballot_sync(0xffffffffu, any);
+      if (any) hit[n + __popc(m & ((1u << lane) - 1))] = e0 + lane;
+      n += __popc(m);
+    }
+    if (lane == 0) n_hit = n;
+  }
+  __syncthreads();
+  const int64_t all = (int64_t)n_hit * p.w.tiles;
+  int64_t pos = all * blockIdx.x / gridDim.x;
+  const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
+  const int chunks = p.w.kb / C::kUnits, pitch = w4_pitch(p.w.kb * 64);
+  if constexpr (!GATED) {
+    // bring the run's first weights into L2 while the first product ends
+    if (lane == 0 && pos < end) {
+      const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
+      const int64_t total = (int64_t)nt * chunks;
+      const int a = (int)(total * warp / kW4Warps), b = (int)(total * (warp + 1) / kW4Warps);
+      const int n = min(b - a, C::kDepth * 2);
+      const int64_t tile = (int64_t)hit[pos / p.w.tiles] * p.w.tiles + ta;
+      if (n > 0) prefetch_l2(p.w.q + (tile * p.w.kb + (int64_t)a * C::kUnits) * 32, n * C::kUnits * 512);
+    }
+    pdl_wait();
+  }
+
+  while (pos < end) {
+    const int e = hit[pos / p.w.tiles];
+    const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
+    __syncthreads();  // the previous expert's list is done with
+    if (threadIdx.x == 0) n_list = 0;
+    __syncthreads();
+    // in any order: a token's sums do not depend on its place
+    for (int i = threadIdx.x; i < p.pairs; i += kW4Threads)
+      if (local_expert(p.ids[i], p.e0) == (unsigned)e) list[atomicAdd(&n_list, 1)] = i;
+    __syncthreads();
+    const int ne = n_list;
+    for (int m0 = 0; m0 < ne; m0 += p.rows) {
+      const int nx = min(p.rows, ne - m0);
+      const int* mine = list + m0;
+      const auto load = [&] {
+        load_rows(xs, pitch, nx, 0, p.w.kb * 64, p.w.k, [&](int r) {
+          return p.in + (int64_t)(GATED ? mine[r] / p.topk : mine[r]) * p.in_stride;
+        });
+      };
+      const auto emit = [&](int tile, const float (&acc)[NT][4]) {
+        if constexpr (GATED) {
+          const int inter = p.w.n / 2, i = (ta + tile) * 8 + g;
+          if (i >= inter) return;
+          const float bg = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + i]);
+          const float bu = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + inter + i]);
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int m = q * 8 + 2 * t + c;
+              if (m < nx)
+                p.a[(int64_t)mine[m] * p.a_stride + i] =
+                    __float2bfloat16(gated_act(acc[q][c] + bg, acc[q][2 + c] + bu, p.act));
+            }
+        } else {
+          const int n = (ta + tile) * 16 + g;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (n + 8 * r >= p.w.n) continue;
+            const float b = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + n + 8 * r]);
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int m = q * 8 + 2 * t + c;
+                if (m < nx) p.y[(int64_t)mine[m] * p.w.n + n + 8 * r] = acc[q][2 * r + c] + b;
+              }
+          }
+        }
+      };
+      run_tiles<NT, G, Z>(p.w, (int64_t)e * p.w.tiles + ta, nt, 0, chunks, xs, pitch, nx, part, load, emit);
+    }
+    pos += nt;
+  }
+}
+
+// out[t] = sum over a token's choices, in their order, of weight * y; four columns a thread
+__global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict__ y, const float* __restrict__ weights,
+                                                         const int32_t* __restrict__ ids, int E, int e0, int topk, int H,
+                                                         __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_launch();
+  const int64_t t = blockIdx.x;
+  const int c = (blockIdx.y * 128 + threadIdx.x) * 4;
+  if (c >= H) return;
+  float v[4] = {};
+  for (int j = 0; j < topk; ++j) {
+    const int64_t p = t * topk + j;
+    if (local_expert(ids[p], e0) >= (unsigned)E) continue;
+    const float w = weights[p];
+    if (H % 4 == 0) {
+      const float4 f = *reinterpret_cast<const float4*>(y + p * H + c);
+      v[0] += w * f.x, v[1] += w * f.y, v[2] += w * f.z, v[3] += w * f.w;
+    } else {
+      for (int i = 0; i < 4 && c + i < H; ++i) v[i] += w * y[p * H + c + i];
+    }
+  }
+  if (H % 4 == 0) {
+    *reinterpret_cast<uint2*>(out + t * H + c) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  } else {
+    for (int i = 0; i < 4 && c + i < H; ++i) out[t * H + c + i] = __float2bfloat16(v[i]);
+  }
+}
+
+template <int NT, int G, bool Z, bool GATED>
+int launch_experts(ExpertArgs p, int fixed, cudaStream_t s) {
+  constexpr auto kernel = w4_experts_kernel<NT, G, Z, GATED>;
+  if (msgl_set_smem<kernel>(kSmemMax - 64) != cudaSuccess) return 4;
+  const int pitch = w4_pitch(p.w.kb * 64);
+  p.rows = std::min(NT * 8, (kSmemMax - 64 - fixed - w4_part_bytes<NT>()) / pitch);
+  if (p.rows < 1) return 3;
+  const int smem = w4_part_bytes<NT>() + fixed + p.rows * pitch;
+  const int64_t most = (int64_t)std::min(p.E, p.pairs) * p.w.tiles;
+  const int grid = (int)std::min<int64_t>(msgl_num_sms(), most);
+  return msgl_launch(kernel, dim3(grid), dim3(kW4Threads), smem, s, 1, p) == cudaSuccess ? 0 : 4;
+}
+
+template <bool GATED, int NT>
+int launch_experts_nt(const ExpertArgs& p, int fixed, cudaStream_t s) {
+  const bool z = p.w.z != nullptr;
+  switch (p.w.group) {
+    case 32: return z ? launch_experts<NT, 32, true, GATED>(p, fixed, s) : launch_experts<NT, 32, false, GATED>(p, fixed, s);
+    case 64: return z ? launch_experts<NT, 64, true, GATED>(p, fixed, s) : launch_experts<NT, 64, false, GATED>(p, fixed, s);
+    default:
+      return z ? launch_experts<NT, 128, true, GATED>(p, fixed, s) : launch_experts<NT, 128, false, GATED>(p, fixed, s);
+  }
+}
+
+// One product. Token columns per pass: 8 while an expert has at most 4 tokens on average (its tokens then
+// rarely exceed 8), else 16; a second pass reads the expert's weights again, from L2.
+template <bool GATED>
+int experts_product(const ExpertArgs& p, cudaStream_t s) {
+  const int fixed = 8 * p.E + 16 + (p.pairs * 4 + 15) / 16 * 16;
+  return p.pairs <= 4 * p.E ? launch_experts_nt<GATED, 1>(p, fixed, s) : launch_experts_nt<GATED, 2>(p, fixed, s);
+}
+
+}  // namespace
+
+extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, const MsglW4* w1, const MsglW4* w2) {
+  const int64_t pairs = (int64_t)T * topk;
+  return pairs * w2->kb * 64 * 2 + pairs * w2->n * 4;
+}
+
+extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
+                               const MsglW4* w2, int E, int e0, const float* weights, const int32_t* ids,
+                               const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
+  if (T == 0) return 0;
+  if (E > kMoeMaxExperts || topk > kMoeMaxPairs) return 3;
+  const int a_stride = w2->kb * 64, most = kMoeMaxPairs / topk;
+  for (int t0 = 0; t0 < T; t0 += most) {
+    const int n = std::min(most, T - t0), pairs = n * topk;
+    __nv_bfloat16* a = (__nv_bfloat16*)workspace;
+    float* y = (float*)((uint8_t*)workspace + (int64_t)pairs * a_stride * 2);
+    const int32_t* id = ids + (int64_t)t0 * topk;
+    ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, id, (const __nv_bfloat16*)x + t0 * x_stride, x_stride,
+                     (const __nv_bfloat16*)b1, a, nullptr, a_stride, act, 0};
+    ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, id, a, a_stride, (const __nv_bfloat16*)b2, nullptr, y, 0, 0, 0};
+    int rc = experts_product<true>(p1, s);
+    if (rc == 0) rc = experts_product<false>(p2, s);
+    if (rc != 0) return rc;
+    if (msgl_launch(w4_combine_kernel, dim3(n, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)y,
+                    weights + (int64_t)t0 * topk, id, E, e0, topk, w2->n, (__nv_bfloat16*)out + (int64_t)t0 * w2->n) !=
+        cudaSuccess)
+      return 4;
+  }
+  return 0;
+}
