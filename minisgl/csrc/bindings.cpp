@@ -471,27 +471,25 @@ std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, int64_t topk
   return {weights, ids};
 }
 
-// the packed arrays of one 4-bit weight, with the sizes that W4Weight keeps beside them
-MsglW4 w4_of(const at::Tensor& q, const at::Tensor& s, const c10::optional<at::Tensor>& z, int64_t n, int64_t k,
-             int64_t group, bool gated, const at::Device& dev, const char* name) {
-  CHECK(q.is_cuda() && q.device() == dev, name, " must be on the activations' device");
-  check_dtype(q, at::kByte, name); check_contig(q, name); check_contig(s, name);
-  CHECK(q.dim() == 4 && q.size(3) == 512 && s.dim() == 4 && s.size(3) == 16, name, " is not a packed 4-bit weight");
-  CHECK(s.scalar_type() == at::kBFloat16 || s.scalar_type() == at::kHalf, name, " scales must be bf16 or fp16");
-  const int64_t E = q.size(0), tiles = q.size(1), kb = q.size(2), kg = s.size(2);
-  CHECK(group == 32 || group == 64 || group == 128, name, " groups must be 32, 64 or 128 inputs");
-  CHECK(s.device() == dev && s.size(0) == E && s.size(1) == tiles && kg * group >= kb * 64, name, " scales' shape");
-  CHECK(k > 0 && k % 32 == 0 && k <= kb * 64 && kb * 64 - k < 128, name, " inputs do not match its blocks");
-  CHECK(n > 0 && (gated ? n % 2 == 0 && n / 2 <= tiles * 8 : n <= tiles * 16), name, " rows do not match its tiles");
-  CHECK(n < (1ll << 30) && k < (1ll << 30) && tiles * E < (1ll << 31), name, " is too large");
-  if (z.has_value()) {
-    check_dtype(*z, at::kByte, name); check_contig(*z, name);
-    CHECK(z->device() == dev && z->sizes() == s.sizes(), name, " zero points' shape");
-  }
-  CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0 &&
-            reinterpret_cast<uintptr_t>(opt_ptr(z)) % 16 == 0, name, " must be 16-byte aligned");
-  return {q.data_ptr(), s.data_ptr(), opt_ptr(z), (int)tiles, (int)kb, (int)kg, (int)group, (int)n, (int)k,
-          s.scalar_type() == at::kHalf};
+// one packed 4-bit weight: its records, and the sizes that W4Weight keeps beside them
+struct W4Args {
+  at::Tensor data;
+  int64_t n, k, group;
+  bool zeros, fp16;
+};
+
+MsglW4 w4_of(const W4Args& a, bool gated, const at::Device& dev, const char* name) {
+  CHECK(a.data.is_cuda() && a.data.device() == dev, name, " must be on the activations' device");
+  check_dtype(a.data, at::kByte, name); check_contig(a.data, name);
+  CHECK(a.group == 32 || a.group == 64 || a.group == 128, name, " groups must be 32, 64 or 128 inputs");
+  const int64_t bytes = 2048 + (128 / a.group) * (a.zeros ? 96 : 64);
+  CHECK(a.data.dim() == 4 && a.data.size(3) == bytes, name, " is not a packed 4-bit weight");
+  const int64_t E = a.data.size(0), tiles = a.data.size(1), kc = a.data.size(2), n = a.n, k = a.k;
+  CHECK(k > 0 && k % 32 == 0 && k <= kc * 128 && kc * 128 - k < 128, name, " inputs do not match its records");
+  CHECK(n > 0 && (gated ? n % 2 == 0 && n / 2 <= tiles * 16 : n <= tiles * 32), name, " rows do not match its tiles");
+  CHECK(n < (1ll << 30) && k < (1ll << 24) && tiles * E < (1ll << 31), name, " is too large");
+  CHECK(reinterpret_cast<uintptr_t>(a.data.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
+  return {a.data.data_ptr(), (int)tiles, (int)kc, (int)a.group, (int)n, (int)k, a.zeros, a.fp16};
 }
 
 // rows as the kernels read them: unit inner stride, every row on a 16-byte boundary (else a copy)
@@ -503,12 +501,12 @@ at::Tensor w4_rows(const at::Tensor& x, int64_t k) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
-at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, c10::optional<at::Tensor> z, int64_t n, int64_t k,
-                     int64_t group, c10::optional<at::Tensor> bias) {
+at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_t group, bool zeros, bool fp16,
+                     c10::optional<at::Tensor> bias) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
-  const MsglW4 w = w4_of(q, s, z, n, k, group, false, x.device(), "weight");
-  CHECK(q.size(0) == 1, "linear_w4 takes one matrix, not ", q.size(0), " experts");
+  const MsglW4 w = w4_of({data, n, k, group, zeros, fp16}, false, x.device(), "weight");
+  CHECK(data.size(0) == 1, "linear_w4 takes one matrix, not ", data.size(0), " experts");
   at::Tensor xr = w4_rows(x, k);
   if (bias.has_value()) {
     check_bf16(*bias, "bias"); check_contig(*bias, "bias");
@@ -517,21 +515,22 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, c10::optional<at:
   const int64_t M = x.size(0);
   CHECK(M < (1ll << 31), "too many tokens");
   at::Tensor out = at::empty({M, n}, x.options());
+  if (M == 0) return out;
   const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
   CHECK(rc == 0, "linear_w4 failed (code ", rc, ")");
   return out;
 }
 
-at::Tensor experts_w4(at::Tensor x, at::Tensor q1, at::Tensor s1, c10::optional<at::Tensor> z1, int64_t n1, int64_t k1,
-                      int64_t group1, at::Tensor q2, at::Tensor s2, c10::optional<at::Tensor> z2, int64_t n2, int64_t k2,
-                      int64_t group2, at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0,
+at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, int64_t group1, bool zeros1, bool fp16_1,
+                      at::Tensor data2, int64_t n2, int64_t k2, int64_t group2, bool zeros2, bool fp16_2,
+                      at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0,
                       c10::optional<at::Tensor> b1, c10::optional<at::Tensor> b2) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
-  const MsglW4 w1 = w4_of(q1, s1, z1, n1, k1, group1, true, x.device(), "w1");
-  const MsglW4 w2 = w4_of(q2, s2, z2, n2, k2, group2, false, x.device(), "w2");
-  const int64_t E = q1.size(0), T = x.size(0);
-  CHECK(q2.size(0) == E, "w1 has ", E, " experts, w2 ", q2.size(0));
+  const MsglW4 w1 = w4_of({data1, n1, k1, group1, zeros1, fp16_1}, true, x.device(), "w1");
+  const MsglW4 w2 = w4_of({data2, n2, k2, group2, zeros2, fp16_2}, false, x.device(), "w2");
+  const int64_t E = data1.size(0), T = x.size(0);
+  CHECK(data2.size(0) == E && E <= 1024, "w1 has ", E, " experts (at most 1024), w2 ", data2.size(0));
   CHECK(k2 == n1 / 2, "w2 takes ", k2, " inputs, w1 gives ", n1 / 2);
   at::Tensor xr = w4_rows(x, k1);
   check_i32(ids, "ids"); check_cuda(weights, "weights"); check_dtype(weights, at::kFloat, "weights");

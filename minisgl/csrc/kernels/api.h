@@ -97,12 +97,10 @@ int msgl_route_experts(const void* logits, int is_fp32, int64_t stride, const fl
                        int sigmoid, int groups, int kept, int top2, int renorm, float scale, float* weights,
                        int32_t* ids, cudaStream_t s);
 
-// ----- 4-bit weights with group scales (layout in w4.cu)
+// ----- 4-bit weights with group scales (layout in w4.cuh)
 typedef struct {
-  const void* q;  // [E][tiles][kb][512] bytes
-  const void* s;  // [E][tiles][kg][8][2] 16-bit scales
-  const void* z;  // [E][tiles][kg][8][2] bytes, or null (zero points of 8)
-  int tiles, kb, kg, group, n, k, fp16;
+  const void* data;  // [E][tiles][kc] records
+  int tiles, kc, group, n, k, zeros, fp16;
 } MsglW4;
 // out [M, n] = x [M, k] w^T (+ bias). Returns 0, 3 on unsupported sizes, 4 if a launch failed.
 int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,

@@ -1,23 +1,29 @@
 // Products with 4-bit weights and group scales: w[n, k] = (code - zero) * scale(row n, group of k).
 //
-// Packed weights (ops/w4.py lays them out once): tiles of 16 rows by 64 inputs, 512 bytes each, in the
-// order of the tensor core's A fragments, so that a warp's 16-byte loads are one tile:
-//   q [E][Nt][KB][32 lanes][4 words], lane = 4 g + t. Word 2h + j holds, for k = 64 kb + 32 h + 8 t + 4 j,
-//     row g     codes k, k+1, k+2, k+3 in nibbles 0, 4, 2, 6
-//     row g + 8 codes k, k+1, k+2, k+3 in nibbles 1, 5, 3, 7
-//   s [E][Nt][KG][8][2] 16-bit scales of rows g and g + 8, z likewise in bytes (none: 8).
-// Rows and inputs are padded to whole tiles with scales of zero. In a gated weight rows 0-7 of a tile
-// are gate rows 8 i .. 8 i + 7 and rows 8-15 the up rows of the same outputs.
+// Packed weights (ops/w4.py lays them out once) are records of 32 rows by 128 inputs, [E][Nt][KC][bytes]:
+//   2048 bytes of codes: two halves of 16 rows, of each two blocks of 64 inputs in the order of the tensor
+//     core's A fragments: lane 4 g + t has 16 bytes = 4 words of a block. Word 2h + j holds, for
+//     k = 64 block + 32 h + 8 t + 4 j,
+//       row g     codes k, k+1, k+2, k+3 in nibbles 0, 4, 2, 6
+//       row g + 8 codes k, k+1, k+2, k+3 in nibbles 1, 5, 3, 7
+//   per group of inputs 64 bytes of 16-bit scales, [8 g][half][row g, row g + 8]
+//   per group 32 bytes of zero points, likewise (none: 8)
+// Rows and inputs are padded to whole records with scales of zero. In a gated weight rows g of half i of a
+// tile are gate rows 16 tile + 8 i + g, and rows g + 8 the up rows of the same outputs.
 //
-// This header is the streaming product for few tokens (the weight bytes bound it): every warp of a
-// CTA takes an equal, contiguous run of the CTA's weight tiles and keeps kDepth of them in flight in
-// registers; a word of eight codes becomes one A fragment with two logic instructions and one exact
-// subtraction per pair (a code c under the exponent of 128 is the bf16 value 128 + c), the group's
-// products go through mma.sync into fp32, and the group's scale multiplies the fp32 sums. So nothing
-// is rounded before the result. The inputs' order inside a block of 32 is the same permutation on both
-// sides, which is why no shuffle is needed.
+// This header is the streaming product for few tokens, which the weights' bytes bound. Every warp of a
+// CTA takes an equal, contiguous run of the CTA's records and keeps the next two on their way into a ring
+// of its own with bulk copies, issued by one lane once the warp has read the slot. (At 1 x 34816 x 5120 a
+// producer warp for all rings measured 38 us, cp.async by every lane 27 us, bulk copies of 16-row records
+// 25 us: what is left of an SM's issue slots beside the conversion decides.) A word of eight codes
+// becomes one A fragment with two logic instructions and one exact subtraction per pair (a code c under
+// the exponent of 128 is the bf16 value 128 + c), the group's products go through mma.sync into fp32, and
+// the group's scale multiplies the fp32 sums: nothing is rounded before the result. The inputs' order
+// inside a block of 32 is the same permutation on both sides, which is why no shuffle is needed.
 #pragma once
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "api.h"
 #include "common.cuh"
@@ -25,41 +31,50 @@
 namespace msgl {
 
 struct W4Tensor {
-  const uint4* q;
-  const uint32_t* s;  // two 16-bit scales
-  const uint16_t* z;  // two zero points, or null
-  int tiles, kb, kg, group, n, k, fp16;
+  const uint8_t* data;
+  int tiles, kc, n, k;
 };
 
-inline W4Tensor w4_tensor(const MsglW4* w) {
-  return {(const uint4*)w->q, (const uint32_t*)w->s, (const uint16_t*)w->z, w->tiles, w->kb, w->kg, w->group,
-          w->n, w->k, w->fp16};
-}
+inline W4Tensor w4_tensor(const MsglW4* w) { return {(const uint8_t*)w->data, w->tiles, w->kc, w->n, w->k}; }
 
-constexpr int kW4Warps = 16;
-constexpr int kW4Threads = kW4Warps * 32;
-constexpr int kW4Depth = 8;  // tiles of 512 bytes that a warp has in flight: 64 KB per SM
+constexpr int kW4Slots = 2;  // records of a warp's ring: 50 to 100 KB in flight per SM
 
-// a chunk is the least number of whole tiles and whole groups along the inputs
-template <int G>
-struct W4Chunk {
-  static constexpr int kUnits = G == 128 ? 2 : 1;
-  static constexpr int kScales = G == 32 ? 2 : 1;
-  static constexpr int kDepth = kW4Depth / kUnits;
+template <int G, bool Z>
+struct W4Record {
+  static constexpr int kGroups = 128 / G;
+  static constexpr int kScales = 2048;
+  static constexpr int kZeros = kScales + kGroups * 64;
+  static constexpr int kBytes = kZeros + (Z ? kGroups * 32 : 0);
+  static constexpr int kRing = kW4Slots * kBytes;  // of one warp
 };
 
-// shared memory of run_tiles for the warps' partial tiles
+// warps by the number of 8-token columns: as many as the registers of their sums allow
 template <int NT>
-constexpr int w4_part_bytes() { return kW4Warps * 2 * NT * 32 * 16; }
+constexpr int w4_warps() { return NT == 1 ? 24 : NT == 2 ? 16 : 12; }
+template <int NT>
+constexpr int w4_threads() { return w4_warps<NT>() * 32; }
+
+// shared memory of the runs: rings, partial tiles, barriers
+template <int NT, int G, bool Z>
+constexpr int w4_run_bytes() { return w4_warps<NT>() * (W4Record<G, Z>::kRing + NT * 1024 + kW4Slots * 8) + 16; }
 
 // bytes between the rows of the activations in shared memory: 64 more than a whole number of 128, so
 // that the eight 16-byte reads of a quarter warp (two rows, four columns) fall into different banks
 __host__ __device__ inline int w4_pitch(int inputs) { return inputs * 2 + 64; }
 
-MSGL_DEVICE uint4 ld_stream(const uint4* p) {
+MSGL_DEVICE uint4 lds128(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+MSGL_DEVICE uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+MSGL_DEVICE uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 
@@ -68,11 +83,39 @@ MSGL_DEVICE void prefetch_l2(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-MSGL_DEVICE void mma_bf16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// mbarrier operations and bulk_load on shared-memory addresses
+MSGL_DEVICE bool mbar_try_wait_a(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+MSGL_DEVICE void mbar_expect_tx_a(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+MSGL_DEVICE void bulk_load_a(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+MSGL_DEVICE void mma_bf16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+  if (first) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
 }
 
 // two codes (bits 0-3 and 16-19 of v) minus a zero point (given as 128 + zero in both halves), exactly
@@ -83,200 +126,244 @@ MSGL_DEVICE uint32_t codes_bf16x2(uint32_t v, uint32_t zero) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-MSGL_DEVICE float2 w4_scales(uint32_t v, int fp16) {
-  if (fp16) return __half22float2(*reinterpret_cast<__half2*>(&v));
+template <bool F>
+MSGL_DEVICE float2 w4_scales(uint32_t v) {
+  if constexpr (F) return __half22float2(*reinterpret_cast<__half2*>(&v));
   return make_float2(bf16_lo(v), bf16_hi(v));
 }
 
-// A warp's run of chunks, fetched ahead in registers. Chunks are numbered tile by tile.
-template <int G, bool Z>
-struct W4Stream {
-  using C = W4Chunk<G>;
-  uint4 q[C::kDepth][C::kUnits];
-  uint32_t s[C::kDepth][C::kScales];
-  uint32_t z[Z ? C::kDepth : 1][C::kScales];
-  const uint4* qp;
-  const uint32_t* sp;
-  const uint16_t* zp;
-  int c, nc;            // next chunk of its tile, chunks per tile
-  int q_skip, s_skip;   // from the end of a tile's chunks to the next tile's first
-
-  MSGL_DEVICE void start(const W4Tensor& w, int64_t tile, int c0, int c_, int nc_) {
-    const int lane = threadIdx.x & 31;
-    const int64_t chunk = c0 + c_;
-    c = c_;
-    nc = nc_;
-    qp = w.q + (tile * w.kb + chunk * C::kUnits) * 32 + lane;
-    sp = w.s + (tile * w.kg + chunk * C::kScales) * 8 + (lane >> 2);
-    zp = Z ? w.z + (tile * w.kg + chunk * C::kScales) * 8 + (lane >> 2) : nullptr;
-    q_skip = (w.kb - nc * C::kUnits) * 32;
-    s_skip = (w.kg - nc * C::kScales) * 8;
-  }
-  MSGL_DEVICE void fetch(int d) {
-#pragma unroll
-    for (int i = 0; i < C::kUnits; ++i) q[d][i] = ld_stream(qp + i * 32);
-#pragma unroll
-    for (int i = 0; i < C::kScales; ++i) {
-      s[d][i] = __ldg(sp + i * 8);
-      if constexpr (Z) z[d][i] = __ldg(zp + i * 8);
+// a wait that did not succeed at once
+static __noinline__ __device__ bool w4_wait(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait_a(bar, parity)) {
+    if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+      report_error(kErrMbarTimeout, 400);
+      return false;
     }
-    qp += C::kUnits * 32;
-    sp += C::kScales * 8;
-    if constexpr (Z) zp += C::kScales * 8;
-    if (++c == nc) {
-      c = 0;
-      qp += q_skip;
-      sp += s_skip;
-      if constexpr (Z) zp += s_skip;
+  }
+  return true;
+}
+
+// The runs of a CTA: its shared memory and how far the ring of this thread's warp has turned. F: fp16 scales.
+template <int NT, int G, bool Z, bool F>
+struct W4Runs {
+  using R = W4Record<G, Z>;
+  static constexpr int kWarps = w4_warps<NT>();
+  static_assert(NT * 1024 <= R::kRing && R::kRing % 16 == 0, "a tile's sums fit into a ring");
+  uint8_t* mem;
+  uint32_t it = 0;    // records that the warp has read
+  uint32_t runs = 0;  // runs so far: the phase of the activations' barrier
+  bool ok = true;
+
+  MSGL_DEVICE uint32_t ring(int warp) const { return smem_u32(mem) + warp * R::kRing; }
+  // sums of a tile that the warp shares with earlier warps, and (in its ring, once that is read) with later ones
+  MSGL_DEVICE float4* head(int warp) const { return reinterpret_cast<float4*>(mem + kWarps * R::kRing) + warp * NT * 64; }
+  MSGL_DEVICE float4* tail(int warp) const { return reinterpret_cast<float4*>(mem + warp * R::kRing); }
+  MSGL_DEVICE uint64_t* full(int warp) const {
+    return reinterpret_cast<uint64_t*>(mem + kWarps * (R::kRing + NT * 1024)) + warp * kW4Slots;
+  }
+
+  MSGL_DEVICE uint32_t xbar() const { return smem_u32(mem + w4_run_bytes<NT, G, Z>() - 16); }
+
+  // before the first run; a barrier must follow
+  MSGL_DEVICE void init() {
+    if (threadIdx.x < kWarps)
+      for (int i = 0; i < kW4Slots; ++i) mbar_init(full(threadIdx.x) + i, 1);
+    if (threadIdx.x == 0) mbar_init(reinterpret_cast<uint64_t*>(mem + w4_run_bytes<NT, G, Z>() - 16), 1);
+    if (threadIdx.x < 32) fence_barrier_init();
+  }
+
+  // first record of warp i's run, of `total` records
+  static MSGL_DEVICE int bound(int total, int i) { return total / kWarps * i + min(i, total % kWarps); }
+
+  // Products of `ntiles` tiles (absolute number tile0 on) over records [c0, c0 + nc) of each with the nx rows
+  // rows row(r), r < nx <= 32, of w.k bf16 each, which are brought to xs (pitch bytes apart, column 0 = record
+  // c0's first input). emit(tile, acc) gets every tile's sums, from one warp: acc[half][nt][0..3] = rows g,
+  // g, g + 8, g + 8 of the half, of tokens 8 nt + 2 t, + 1, + 0, + 1. Tiles that several warps share are
+  // summed through shared memory, in the order of the warps. Ends without a barrier: xs is free, the runs'
+  // memory is for the next run only. SPLIT: nc is less than all of a tile's records.
+  template <bool SPLIT, class Row, class Emit>
+  MSGL_DEVICE void run(const W4Tensor& w, int64_t tile0, int ntiles, int c0, int nc, uint8_t* xs, int pitch, int nx,
+                       Row row, Emit emit) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int total = ntiles * nc, a = bound(total, warp), b = bound(total, warp + 1);
+    // the rows first: behind the weights' copies they would wait for these
+    const int kn = min(nc * 128, w.k - c0 * 128), pad = nc * 128 - kn;
+    if (warp == 0) {
+      if (lane == 0) mbar_expect_tx_a(xbar(), nx * kn * 2);
+      __syncwarp();
+      if (lane < nx) bulk_load_a(smem_u32(xs) + lane * pitch, row(lane) + c0 * 128, kn * 2, xbar());
+    }
+    int tile = a / nc, cc = a - tile * nc;
+    const uint32_t ring0 = ring(warp), bars = smem_u32(full(warp));
+    const uint8_t* src = w.data + ((tile0 + tile) * w.kc + c0 + cc) * R::kBytes;  // next record to copy
+    const int64_t skip = (int64_t)(w.kc - nc) * R::kBytes;
+    int fc = cc;  // its number in its tile
+    const auto fetch = [&](uint32_t slot, uint32_t bar) {
+      if (lane == 0) {
+        mbar_expect_tx_a(bar, R::kBytes);
+        bulk_load_a(slot, src, R::kBytes, bar);
+      }
+      src += R::kBytes;
+      if constexpr (SPLIT) {
+        if (++fc == nc) {
+          fc = 0;
+          src += skip;
+        }
+      }
+    };
+    // the ring goes on where the previous run left it (whose sums this warp may have put there)
+    fence_async_smem();
+    __syncwarp();
+    uint32_t slot = ring0 + (it % kW4Slots) * R::kBytes, bar = bars + (it % kW4Slots) * 8;
+    constexpr uint32_t kOther = R::kBytes;
+    static_assert(kW4Slots == 2, "the slots alternate");
+    if (a < b) fetch(slot, bar);
+    if (a + 1 < b) fetch(2 * ring0 + kOther - slot, 2 * bars + 8 - bar);
+    // zeros behind the last input (pad is less than 128)
+    for (int i = threadIdx.x; i < nx * (pad / 8); i += w4_threads<NT>())
+      *reinterpret_cast<uint4*>(xs + i / (pad / 8) * pitch + kn * 2 + i % (pad / 8) * 16) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if (ok) ok = w4_wait(xbar(), runs & 1);
+    ++runs;
+
+    uint32_t xrow[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      xrow[nt] = smem_u32(xs) + (uint32_t)(min(nt * 8 + g, nx - 1) * pitch + t * 16);
+    const uint32_t mine = lane * 16, side = R::kScales + g * 8, zside = R::kZeros + g * 4;
+    float acc[2][NT][4];
+    for (int i = a; i < b;) {
+      const int from = i - cc;            // the tile's first record
+      const int end = min(from + nc, b);  // one past its last one here
+      uint32_t xoff = cc * 256;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[0][nt][r] = acc[1][nt][r] = 0.f;
+      for (; i < end; ++i) {
+        if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
+          if (ok) ok = w4_wait(bar, (it >> 1) & 1);
+        }
+        ++it;
+        uint4 q[2][2];
+        uint2 s[R::kGroups];
+        uint32_t z[R::kGroups];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r >> 1][r & 1] = lds128(slot + mine + r * 512);
+#pragma unroll
+        for (int j = 0; j < R::kGroups; ++j) {
+          s[j] = lds64(slot + side + j * 64);
+          if constexpr (Z) z[j] = lds32(slot + zside + j * 32);
+        }
+        __syncwarp();  // every lane has read the slot
+        if (i + 2 < b) fetch(slot, bar);
+        slot = 2 * ring0 + kOther - slot;
+        bar = 2 * bars + 8 - bar;
+
+        float tmp[2][NT][4];
+#pragma unroll
+        for (int quarter = 0; quarter < 4; ++quarter) {  // 32 inputs
+          constexpr int per = G / 32;                    // quarters per group
+          const int j = quarter / per;
+          uint32_t fr[2][2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t z0 = Z ? 0x43004300u + ((z[j] >> (16 * h)) & 15u) * 0x10001u : 0x43084308u;
+            const uint32_t z1 = Z ? 0x43004300u + ((z[j] >> (16 * h + 8)) & 15u) * 0x10001u : 0x43084308u;
+            const uint4 v4 = q[h][quarter >> 1];
+            const uint32_t words[2] = {quarter & 1 ? v4.z : v4.x, quarter & 1 ? v4.w : v4.y};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              fr[h][e][0] = codes_bf16x2(words[e], z0);
+              fr[h][e][1] = codes_bf16x2(words[e] >> 4, z1);
+              fr[h][e][2] = codes_bf16x2(words[e] >> 8, z0);
+              fr[h][e][3] = codes_bf16x2(words[e] >> 12, z1);
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 xv = lds128(xrow[nt] + xoff + quarter * 64);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mma_bf16_16816(tmp[h][nt], fr[h][0], xv.x, xv.y, quarter % per == 0);
+              mma_bf16_16816(tmp[h][nt], fr[h][1], xv.z, xv.w, false);
+            }
+          }
+          if (quarter % per == per - 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 sc = w4_scales<F>(h == 0 ? s[j].x : s[j].y);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                acc[h][nt][0] += tmp[h][nt][0] * sc.x;
+                acc[h][nt][1] += tmp[h][nt][1] * sc.x;
+                acc[h][nt][2] += tmp[h][nt][2] * sc.y;
+                acc[h][nt][3] += tmp[h][nt][3] * sc.y;
+              }
+            }
+          }
+        }
+        xoff += 256;
+      }
+      if (from >= a && from + nc <= b) {
+        emit(tile, acc);
+      } else if (from < a) {
+        put(head(warp) + lane, acc);
+      } else {
+        __syncwarp();
+        put(tail(warp) + lane, acc);
+      }
+      cc = 0;
+      ++tile;
+    }
+    __syncthreads();
+    // a tile that starts in this warp's run and ends in a later warp's: sum their parts in order
+    if (a < b) {
+      const int last = (b - 1) / nc, from = last * nc, to = from + nc;
+      if (a <= from && b < to) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[0][nt][r] = acc[1][nt][r] = 0.f;
+        add(acc, tail(warp) + lane);
+        for (int v = warp + 1; v < kWarps && bound(total, v) < min(to, total); ++v) add(acc, head(v) + lane);
+        emit(last, acc);
+      }
+    }
+  }
+
+  // one lane's sums of a tile, 32 lanes apart
+  static MSGL_DEVICE void put(float4* p, const float (&acc)[2][NT][4]) {
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const float(&v)[4] = acc[i / NT][i % NT];
+      p[i * 32] = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  static MSGL_DEVICE void add(float (&acc)[2][NT][4], const float4* p) {
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const float4 v = p[i * 32];
+      float(&o)[4] = acc[i / NT][i % NT];
+      o[0] += v.x, o[1] += v.y, o[2] += v.z, o[3] += v.w;
     }
   }
 };
 
-// Products of `ntiles` tiles (absolute number tile0 on) over chunks [c0, c0 + nc) with the nx rows in
-// xs (pitch bytes apart, column 0 = chunk c0's first input). load() brings the rows into xs once the
-// first weights are on their way; emit(tile, acc) gets every tile's sums, from one warp: acc[nt][0..3] =
-// rows g, g, g + 8, g + 8 of tokens 8 nt + 2 t, + 1, + 0, + 1. Tiles that several warps share are summed
-// through `part`, in the order of the warps. Ends without a barrier: xs is free, part is not until the
-// next barrier.
-template <int NT, int G, bool Z, class Load, class Emit>
-MSGL_DEVICE void run_tiles(const W4Tensor& w, int64_t tile0, int ntiles, int c0, int nc, const uint8_t* xs, int pitch,
-                           int nx, float4* part, Load load, Emit emit) {
-  using C = W4Chunk<G>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t total = (int64_t)ntiles * nc;
-  const auto bound = [&](int i) { return (int)(total * i / kW4Warps); };
-  const int a = bound(warp), b = bound(warp + 1);
-  int tile = a / nc, cc = a - tile * nc;
-  const int tile_first = tile;
-  W4Stream<G, Z> ws;
-  ws.start(w, tile0 + tile, c0, cc, nc);
-#pragma unroll
-  for (int d = 0; d < C::kDepth; ++d)
-    if (a + d < b) ws.fetch(d);
-  load();
-  __syncthreads();
-
-  const uint8_t* xrow[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) xrow[nt] = xs + (size_t)min(nt * 8 + g, nx - 1) * pitch + t * 16;
-  float acc[NT][4] = {};
-  bool whole = cc == 0;  // the warp's part of this tile began at the tile's first chunk
-  for (int i = a; i < b;) {
-#pragma unroll
-    for (int d = 0; d < C::kDepth; ++d) {
-      if (i >= b) break;
-      uint4 q[C::kUnits];
-      uint32_t s[C::kScales], z[C::kScales];
-#pragma unroll
-      for (int u = 0; u < C::kUnits; ++u) q[u] = ws.q[d][u];
-#pragma unroll
-      for (int u = 0; u < C::kScales; ++u) {
-        s[u] = ws.s[d][u];
-        z[u] = Z ? ws.z[d][u] : 0x0808u;
-      }
-      if (i + C::kDepth < b) ws.fetch(d);
-      float tmp[NT][4];
-#pragma unroll
-      for (int u = 0; u < C::kUnits; ++u) {
-        const uint32_t words[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int si = C::kScales == 2 ? h : 0;
-          const uint32_t z0 = Z ? 0x43004300u + (z[si] & 15u) * 0x10001u : 0x43084308u;
-          const uint32_t z1 = Z ? 0x43004300u + ((z[si] >> 8) & 15u) * 0x10001u : 0x43084308u;
-          if (G == 32 || (h == 0 && u == 0)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) tmp[nt][r] = 0.f;
-          }
-          uint32_t fr[2][4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t v = words[2 * h + j];
-            fr[j][0] = codes_bf16x2(v, z0);
-            fr[j][1] = codes_bf16x2(v >> 4, z1);
-            fr[j][2] = codes_bf16x2(v >> 8, z0);
-            fr[j][3] = codes_bf16x2(v >> 12, z1);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(xrow[nt] + (cc * C::kUnits + u) * 128 + h * 64);
-            mma_bf16_16816(tmp[nt], fr[0], xv.x, xv.y);
-            mma_bf16_16816(tmp[nt], fr[1], xv.z, xv.w);
-          }
-          if (G == 32 || (h == 1 && u == C::kUnits - 1)) {
-            const float2 sc = w4_scales(s[si], w.fp16);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][0] += tmp[nt][0] * sc.x;
-              acc[nt][1] += tmp[nt][1] * sc.x;
-              acc[nt][2] += tmp[nt][2] * sc.y;
-              acc[nt][3] += tmp[nt][3] * sc.y;
-            }
-          }
-        }
-      }
-      ++i;
-      ++cc;
-      if (cc == nc || i == b) {
-        if (cc == nc && whole) {
-          emit(tile, acc);
-        } else {
-          float4* p = part + ((warp * 2 + (tile == tile_first ? 0 : 1)) * NT) * 32 + lane;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) p[nt * 32] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[nt][r] = 0.f;
-        whole = true;
-        if (cc == nc) {
-          cc = 0;
-          ++tile;
-        }
-      }
-    }
-  }
-  __syncthreads();
-  // a tile that starts in this warp's run and ends in a later warp's: sum their parts in order
-  if (a < b) {
-    const int last = (b - 1) / nc;
-    const int64_t from = (int64_t)last * nc, to = from + nc;
-    if (a <= from && b < to) {
-      const float4* p = part + ((warp * 2 + (last == tile_first ? 0 : 1)) * NT) * 32 + lane;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float4 v = p[nt * 32];
-        acc[nt][0] = v.x, acc[nt][1] = v.y, acc[nt][2] = v.z, acc[nt][3] = v.w;
-      }
-      for (int v = warp + 1; v < kW4Warps && bound(v) < to; ++v) {
-        if (bound(v) == bound(v + 1)) continue;
-        const float4* o = part + (v * 2 * NT) * 32 + lane;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float4 f = o[nt * 32];
-          acc[nt][0] += f.x, acc[nt][1] += f.y, acc[nt][2] += f.z, acc[nt][3] += f.w;
-        }
-      }
-      emit(last, acc);
-    }
-  }
-}
-
-// rows of bf16 activations into shared memory: row(r) gives row r's address; inputs [k0, k0 + kn) of k,
-// zeros beyond k
-template <class Row>
-MSGL_DEVICE void load_rows(uint8_t* xs, int pitch, int nx, int k0, int kn, int k, Row row) {
-  const int vec = kn / 8;
-  for (int r = threadIdx.x >> 5; r < nx; r += kW4Warps) {
-    const __nv_bfloat16* src = row(r) + k0;
-    for (int i = threadIdx.x & 31; i < vec; i += 32) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (k0 + i * 8 < k) v = *reinterpret_cast<const uint4*>(src + i * 8);
-      *reinterpret_cast<uint4*>(xs + (size_t)r * pitch + i * 16) = v;
-    }
+// calls fn(group, zeros, fp16) with the weight's form as constants
+template <class Fn>
+int w4_dispatch(const MsglW4* w, Fn fn) {
+  const auto form = [&](auto g) {
+    using std::false_type, std::true_type;
+    if (w->zeros) return w->fp16 ? fn(g, true_type{}, true_type{}) : fn(g, true_type{}, false_type{});
+    return w->fp16 ? fn(g, false_type{}, true_type{}) : fn(g, false_type{}, false_type{});
+  };
+  switch (w->group) {
+    case 32: return form(std::integral_constant<int, 32>{});
+    case 64: return form(std::integral_constant<int, 64>{});
+    default: return form(std::integral_constant<int, 128>{});
   }
 }
 

@@ -41,25 +41,27 @@ struct ExpertArgs {
   int a_stride, act, rows;    // rows: tokens of one pass
 };
 
-template <int NT, int G, bool Z, bool GATED>
-__global__ void __launch_bounds__(kW4Threads, 1) w4_experts_kernel(const __grid_constant__ ExpertArgs p) {
-  using C = W4Chunk<G>;
+template <int NT, int G, bool Z, bool F, bool GATED>
+__global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const __grid_constant__ ExpertArgs p) {
+  using R = W4Record<G, Z>;
+  constexpr int kWarps = w4_warps<NT>(), kThreads = w4_threads<NT>();
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float4* part = reinterpret_cast<float4*>(smem);
-  int* count = reinterpret_cast<int*>(smem + w4_part_bytes<NT>());  // [E] pairs of every expert
-  int* hit = count + p.E;                                           // the experts that have any
-  int* list = hit + p.E;                                            // [pairs] pairs of one expert
+  int* count = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());  // [E] pairs of every expert
+  int* hit = count + p.E;                                               // the experts that have any
+  int* list = hit + p.E;                                                // [pairs] pairs of one expert
   uint8_t* xs = reinterpret_cast<uint8_t*>(list) + (p.pairs * 4 + 15) / 16 * 16 + (p.E * 8 % 16);
   __shared__ int n_hit, n_list;
+  W4Runs<NT, G, Z, F> runs{smem};
+  runs.init();
 
   // The second product's ids were complete before the first product's kernel began its work, which is
   // before this kernel could start (it triggers its dependents after its own wait).
   if constexpr (GATED) pdl_wait();
   pdl_launch();
-  for (int e = threadIdx.x; e < p.E; e += kW4Threads) count[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += kThreads) count[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < p.pairs; i += kW4Threads) {
+  for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
     const unsigned e = local_expert(p.ids[i], p.e0);
     if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
   }
@@ -78,16 +80,14 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_experts_kernel(const __grid_
   const int64_t all = (int64_t)n_hit * p.w.tiles;
   int64_t pos = all * blockIdx.x / gridDim.x;
   const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
-  const int chunks = p.w.kb / C::kUnits, pitch = w4_pitch(p.w.kb * 64);
+  const int pitch = w4_pitch(p.w.kc * 128);
   if constexpr (!GATED) {
     // bring the run's first weights into L2 while the first product ends
     if (lane == 0 && pos < end) {
       const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
-      const int64_t total = (int64_t)nt * chunks;
-      const int a = (int)(total * warp / kW4Warps), b = (int)(total * (warp + 1) / kW4Warps);
-      const int n = min(b - a, C::kDepth * 2);
       const int64_t tile = (int64_t)hit[pos / p.w.tiles] * p.w.tiles + ta;
-      if (n > 0) prefetch_l2(p.w.q + (tile * p.w.kb + (int64_t)a * C::kUnits) * 32, n * C::kUnits * 512);
+      const int a = runs.bound(nt * p.w.kc, warp), n = min(runs.bound(nt * p.w.kc, warp + 1) - a, kW4Slots);
+      if (n > 0) prefetch_l2(p.w.data + (tile * p.w.kc + a) * R::kBytes, n * R::kBytes);
     }
     pdl_wait();
   }
@@ -99,50 +99,37 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_experts_kernel(const __grid_
     if (threadIdx.x == 0) n_list = 0;
     __syncthreads();
     // in any order: a token's sums do not depend on its place
-    for (int i = threadIdx.x; i < p.pairs; i += kW4Threads)
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads)
       if (local_expert(p.ids[i], p.e0) == (unsigned)e) list[atomicAdd(&n_list, 1)] = i;
     __syncthreads();
     const int ne = n_list;
     for (int m0 = 0; m0 < ne; m0 += p.rows) {
       const int nx = min(p.rows, ne - m0);
       const int* mine = list + m0;
-      const auto load = [&] {
-        load_rows(xs, pitch, nx, 0, p.w.kb * 64, p.w.k, [&](int r) {
-          return p.in + (int64_t)(GATED ? mine[r] / p.topk : mine[r]) * p.in_stride;
-        });
-      };
-      const auto emit = [&](int tile, const float (&acc)[NT][4]) {
-        if constexpr (GATED) {
-          const int inter = p.w.n / 2, i = (ta + tile) * 8 + g;
-          if (i >= inter) return;
-          const float bg = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + i]);
-          const float bu = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + inter + i]);
+      const auto row = [&](int r) { return p.in + (int64_t)(GATED ? mine[r] / p.topk : mine[r]) * p.in_stride; };
+      const auto emit = [&](int tile, const float (&acc)[2][NT][4]) {
+#pragma unroll
+        for (int r = 0; r < (GATED ? 2 : 4); ++r) {
+          const int n = (ta + tile) * (GATED ? 16 : 32) + r * 8 + g;
+          if (n >= (GATED ? p.w.n / 2 : p.w.n)) continue;
+          const __nv_bfloat16* b = p.bias == nullptr ? nullptr : p.bias + (int64_t)e * p.w.n + n;
+          const float b0 = b == nullptr ? 0.f : __bfloat162float(b[0]);
+          const float b1 = !GATED || b == nullptr ? 0.f : __bfloat162float(b[p.w.n / 2]);
 #pragma unroll
           for (int q = 0; q < NT; ++q)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const int m = q * 8 + 2 * t + c;
-              if (m < nx)
-                p.a[(int64_t)mine[m] * p.a_stride + i] =
-                    __float2bfloat16(gated_act(acc[q][c] + bg, acc[q][2 + c] + bu, p.act));
+              if (m >= nx) continue;
+              if constexpr (GATED)
+                p.a[(int64_t)mine[m] * p.a_stride + n] =
+                    __float2bfloat16(gated_act(acc[r][q][c] + b0, acc[r][q][2 + c] + b1, p.act));
+              else
+                p.y[(int64_t)mine[m] * p.w.n + n] = acc[r >> 1][q][2 * (r & 1) + c] + b0;
             }
-        } else {
-          const int n = (ta + tile) * 16 + g;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (n + 8 * r >= p.w.n) continue;
-            const float b = p.bias == nullptr ? 0.f : __bfloat162float(p.bias[(int64_t)e * p.w.n + n + 8 * r]);
-#pragma unroll
-            for (int q = 0; q < NT; ++q)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const int m = q * 8 + 2 * t + c;
-                if (m < nx) p.y[(int64_t)mine[m] * p.w.n + n + 8 * r] = acc[q][2 * r + c] + b;
-              }
-          }
         }
       };
-      run_tiles<NT, G, Z>(p.w, (int64_t)e * p.w.tiles + ta, nt, 0, chunks, xs, pitch, nx, part, load, emit);
+      runs.template run<false>(p.w, (int64_t)e * p.w.tiles + ta, nt, 0, p.w.kc, xs, pitch, nx, row, emit);
     }
     pos += nt;
   }
@@ -176,43 +163,39 @@ __global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict
   }
 }
 
-template <int NT, int G, bool Z, bool GATED>
+template <int NT, int G, bool Z, bool F, bool GATED>
 int launch_experts(ExpertArgs p, int fixed, cudaStream_t s) {
-  constexpr auto kernel = w4_experts_kernel<NT, G, Z, GATED>;
+  constexpr auto kernel = w4_experts_kernel<NT, G, Z, F, GATED>;
   if (msgl_set_smem<kernel>(kSmemMax - 64) != cudaSuccess) return 4;
-  const int pitch = w4_pitch(p.w.kb * 64);
-  p.rows = std::min(NT * 8, (kSmemMax - 64 - fixed - w4_part_bytes<NT>()) / pitch);
+  const int pitch = w4_pitch(p.w.kc * 128);
+  constexpr int kRun = w4_run_bytes<NT, G, Z>();
+  p.rows = std::min(NT * 8, (kSmemMax - 64 - fixed - kRun) / pitch);
   if (p.rows < 1) return 3;
-  const int smem = w4_part_bytes<NT>() + fixed + p.rows * pitch;
+  const int smem = kRun + fixed + p.rows * pitch;
   const int64_t most = (int64_t)std::min(p.E, p.pairs) * p.w.tiles;
   const int grid = (int)std::min<int64_t>(msgl_num_sms(), most);
-  return msgl_launch(kernel, dim3(grid), dim3(kW4Threads), smem, s, 1, p) == cudaSuccess ? 0 : 4;
+  return msgl_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
 }
 
 template <bool GATED, int NT>
-int launch_experts_nt(const ExpertArgs& p, int fixed, cudaStream_t s) {
-  const bool z = p.w.z != nullptr;
-  switch (p.w.group) {
-    case 32: return z ? launch_experts<NT, 32, true, GATED>(p, fixed, s) : launch_experts<NT, 32, false, GATED>(p, fixed, s);
-    case 64: return z ? launch_experts<NT, 64, true, GATED>(p, fixed, s) : launch_experts<NT, 64, false, GATED>(p, fixed, s);
-    default:
-      return z ? launch_experts<NT, 128, true, GATED>(p, fixed, s) : launch_experts<NT, 128, false, GATED>(p, fixed, s);
-  }
+int launch_experts_nt(const ExpertArgs& p, const MsglW4* w, int fixed, cudaStream_t s) {
+  return w4_dispatch(w, [&](auto g, auto z, auto f) { return launch_experts<NT, g(), z(), f(), GATED>(p, fixed, s); });
 }
 
 // One product. Token columns per pass: 8 while an expert has at most 4 tokens on average (its tokens then
 // rarely exceed 8), else 16; a second pass reads the expert's weights again, from L2.
 template <bool GATED>
-int experts_product(const ExpertArgs& p, cudaStream_t s) {
+int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
   const int fixed = 8 * p.E + 16 + (p.pairs * 4 + 15) / 16 * 16;
-  return p.pairs <= 4 * p.E ? launch_experts_nt<GATED, 1>(p, fixed, s) : launch_experts_nt<GATED, 2>(p, fixed, s);
+  return p.pairs <= 4 * p.E ? launch_experts_nt<GATED, 1>(p, w, fixed, s)
+                             : launch_experts_nt<GATED, 2>(p, w, fixed, s);
 }
 
 }  // namespace
 
 extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, const MsglW4* w1, const MsglW4* w2) {
   const int64_t pairs = (int64_t)T * topk;
-  return pairs * w2->kb * 64 * 2 + pairs * w2->n * 4;
+  return pairs * w2->kc * 128 * 2 + pairs * w2->n * 4;
 }
 
 extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
@@ -220,7 +203,7 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
                                const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
   if (T == 0) return 0;
   if (E > kMoeMaxExperts || topk > kMoeMaxPairs) return 3;
-  const int a_stride = w2->kb * 64, most = kMoeMaxPairs / topk;
+  const int a_stride = w2->kc * 128, most = kMoeMaxPairs / topk;
   for (int t0 = 0; t0 < T; t0 += most) {
     const int n = std::min(most, T - t0), pairs = n * topk;
     __nv_bfloat16* a = (__nv_bfloat16*)workspace;
@@ -229,8 +212,8 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
     ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, id, (const __nv_bfloat16*)x + t0 * x_stride, x_stride,
                      (const __nv_bfloat16*)b1, a, nullptr, a_stride, act, 0};
     ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, id, a, a_stride, (const __nv_bfloat16*)b2, nullptr, y, 0, 0, 0};
-    int rc = experts_product<true>(p1, s);
-    if (rc == 0) rc = experts_product<false>(p2, s);
+    int rc = experts_product<true>(p1, w1, s);
+    if (rc == 0) rc = experts_product<false>(p2, w2, s);
     if (rc != 0) return rc;
     if (msgl_launch(w4_combine_kernel, dim3(n, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)y,
                     weights + (int64_t)t0 * topk, id, E, e0, topk, w2->n, (__nv_bfloat16*)out + (int64_t)t0 * w2->n) !=
@@ -239,3 +222,5 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   }
   return 0;
 }
+
+MSGL_ERROR_ACCESSOR(msgl_err_w4_moe)

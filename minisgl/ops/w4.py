@@ -4,7 +4,7 @@
 whose values are ``(code - zero) * scale``: a code 0..15 per value, and per row and group of 32, 64 or
 128 inputs one bf16 or fp16 scale and optionally a zero point 0..15 (without them every zero point is
 8). ``W4Weight.pack`` takes them as checkpoints hold them and lays them out once in the order in which
-the kernels read them (``csrc/kernels/w4.cu``); ``quantize_w4`` makes them from bf16 weights.
+the kernels read them (``csrc/kernels/w4.cuh``); ``quantize_w4`` makes them from bf16 weights.
 
     w = ops.W4Weight.pack(q, scales, zeros)               # q [N, K/2] uint8, scales / zeros [N, K/group]
     y = ops.linear_w4(x, w, bias)                         # [M, K] bf16 -> [M, N] bf16
@@ -20,7 +20,7 @@ captured in CUDA graphs; they keep no state of their own, so calls on several st
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 import torch.nn.functional as F
@@ -35,34 +35,32 @@ _ACT = {"silu": 0, "gelu": 1, "swiglu_oai": 2}
 
 @dataclass
 class W4Weight:
-    q: torch.Tensor           # uint8 [E, Nt, KB, 512]: tiles of 16 rows x 64 inputs
-    s: torch.Tensor           # bf16 / fp16 [E, Nt, KG, 16]: (row g, row g + 8) pairs
-    z: torch.Tensor | None    # uint8 like s, or None: 8 everywhere
-    n: int                    # rows
-    k: int                    # inputs
-    group: int                # inputs per scale
-    gated: bool               # tiles of 8 gate rows and the 8 up rows of the same outputs
-    experts: bool             # [E, N, K] rather than one [N, K]
+    data: torch.Tensor         # uint8 [E, Nt, KC, bytes]: records of 32 rows x 128 inputs
+    n: int                     # rows
+    k: int                     # inputs
+    group: int                 # inputs per scale
+    zeros: bool                # zero points are stored (else 8)
+    scale_dtype: torch.dtype   # bf16 / fp16
+    gated: bool                # tiles of 16 gate rows and the up rows of the same outputs
+    experts: bool              # [E, N, K] rather than one [N, K]
 
     @property
     def shape(self):
-        return (self.q.shape[0], self.n, self.k) if self.experts else (self.n, self.k)
+        return (self.data.shape[0], self.n, self.k) if self.experts else (self.n, self.k)
 
     @property
     def is_cuda(self) -> bool:
-        return self.q.is_cuda
+        return self.data.is_cuda
 
     @property
     def device(self) -> torch.device:
-        return self.q.device
+        return self.data.device
 
     def nbytes(self) -> int:
-        z = 0 if self.z is None else self.z.numel()
-        return self.q.numel() + self.s.numel() * self.s.element_size() + z
+        return self.data.numel()
 
     def to(self, device) -> "W4Weight":
-        z = None if self.z is None else self.z.to(device)
-        return W4Weight(self.q.to(device), self.s.to(device), z, self.n, self.k, self.group, self.gated, self.experts)
+        return replace(self, data=self.data.to(device))
 
     @classmethod
     def pack(cls, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
@@ -93,44 +91,54 @@ class W4Weight:
         if not experts:
             q, scales, zeros = q[None], scales[None], None if zeros is None else zeros[None]
         E = q.shape[0]
-        nt = -(-(n // 2) // 8) if gated else -(-n // 16)
-        kb = -(-k // 64)
-        kg = -(-kb * 64 // group)
+        nt = -(-(n // 2) // 16) if gated else -(-n // 32)
+        kc = -(-k // 128)
+        per = 128 // group  # groups of a record
 
         def tiles(t: torch.Tensor, cols: int) -> torch.Tensor:
-            """[E, N, c] -> [E, Nt, 2, 8, cols]: the rows g and g + 8 of every tile, zeros beyond the end"""
-            t = F.pad(t, (0, cols - t.shape[-1]))
+            """[E, N, c] -> [E, Nt, half, 2, 8, KC, cols]: rows g and g + 8 of every half, zeros beyond the end"""
+            t = F.pad(t, (0, kc * cols - t.shape[-1]))
             if gated:
-                t = F.pad(t.unflatten(1, (2, n // 2)), (0, 0, 0, nt * 8 - n // 2))
-                return t.unflatten(2, (nt, 8)).transpose(1, 2)
-            return F.pad(t, (0, 0, 0, nt * 16 - n)).unflatten(1, (nt, 2, 8))
+                t = F.pad(t.unflatten(1, (2, n // 2)), (0, 0, 0, nt * 16 - n // 2))
+                t = t.unflatten(2, (nt, 2, 8)).permute(0, 2, 3, 1, 4, 5)
+            else:
+                t = F.pad(t, (0, 0, 0, nt * 32 - n)).unflatten(1, (nt, 2, 2, 8))
+            return t.unflatten(-1, (kc, cols))
 
-        # bytes of a row by (block, half h, lane column t, word j, byte i): codes 2i (low) and 2i + 1
-        b = tiles(q, kb * 32).unflatten(-1, (kb, 2, 4, 2, 2))
-        lo, hi = b[:, :, 0], b[:, :, 1]  # rows g, rows g + 8: [E, Nt, 8, KB, 2, 4, 2, 2]
-        out = torch.empty(E, nt, kb, 8, 4, 2, 2, 2, 2, dtype=torch.uint8, device=q.device)
-        perm = (0, 1, 3, 2, 5, 4, 6, 7)  # -> [E, Nt, KB, g, t, h, j, i]
+        data = torch.empty(E, nt, kc, 2048 + per * (64 if zeros is None else 96), dtype=torch.uint8, device=q.device)
+        # bytes of a row by (block, h, lane column t, word j, byte i): codes 2i (low) and 2i + 1
+        b = tiles(q, 64).unflatten(-1, (2, 2, 4, 2, 2))
+        lo, hi = b[:, :, :, 0], b[:, :, :, 1]  # rows g, rows g + 8: [E, Nt, half, 8, KC, 2, 2, 4, 2, 2]
+        perm = (0, 1, 4, 2, 5, 3, 7, 6, 8, 9)  # -> [E, Nt, KC, half, block, g, t, h, j, i]
+        out = data[..., :2048].unflatten(-1, (2, 2, 8, 4, 2, 2, 2, 2))
         out[..., 0, :] = ((lo & 15) | (hi << 4)).permute(perm)
         out[..., 1, :] = ((lo >> 4) | (hi & 0xF0)).permute(perm)
-        s = tiles(scales, kg).permute(0, 1, 4, 3, 2).reshape(E, nt, kg, 16)
-        z = None if zeros is None else tiles(zeros, kg).permute(0, 1, 4, 3, 2).reshape(E, nt, kg, 16).contiguous()
-        return cls(out.view(E, nt, kb, 512), s.contiguous(), z, n, k, group, gated, experts)
+        side = lambda t: tiles(t, per).permute(0, 1, 5, 6, 4, 2, 3).reshape(E, nt, kc, per * 32)  # noqa: E731
+        data[..., 2048 : 2048 + per * 64] = side(scales.view(torch.int16)).view(torch.uint8)
+        if zeros is not None:
+            data[..., 2048 + per * 64 :] = side(zeros)
+        return cls(data, n, k, group, zeros is not None, scales.dtype, gated, experts)
 
     def codes(self):
         """(q, scales, zeros) as ``pack`` took them."""
-        E, nt, kb, _ = self.q.shape
-        c = self.q.view(E, nt, kb, 8, 4, 2, 2, 2, 2).permute(0, 1, 3, 2, 5, 4, 6, 7, 8)  # [E, Nt, g, KB, h, t, j, c, i]
-        even, odd = c[..., 0, :], c[..., 1, :]
-        b = torch.stack([(even & 15) | ((odd & 15) << 4), (even >> 4) | (odd & 0xF0)], dim=2)  # [E, Nt, 2, g, KB, h, t, j, i]
+        E, nt, kc, _ = self.data.shape
+        per = 128 // self.group
 
         def rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-            t = t.flatten(4)[..., :cols]
+            """[E, Nt, half, 2, 8, ...] -> [E, N, cols]"""
+            t = t.flatten(5)[..., :cols]
             if self.gated:
-                return t.transpose(1, 2).flatten(2, 3)[:, :, : self.n // 2].flatten(1, 2).contiguous()
-            return t.flatten(1, 3)[:, : self.n].contiguous()
+                return t.permute(0, 3, 1, 2, 4, 5).flatten(2, 4)[:, :, : self.n // 2].flatten(1, 2).contiguous()
+            return t.flatten(1, 4)[:, : self.n].contiguous()
 
-        side = lambda t: rows(t.view(E, nt, -1, 8, 2).permute(0, 1, 4, 3, 2), self.k // self.group)  # noqa: E731
-        got = (rows(b, self.k // 2), side(self.s), None if self.z is None else side(self.z))
+        c = self.data[..., :2048].unflatten(-1, (2, 2, 8, 4, 2, 2, 2, 2))  # [E, Nt, KC, half, block, g, t, h, j, c, i]
+        c = c.permute(0, 1, 3, 5, 2, 4, 7, 6, 8, 9, 10)  # [E, Nt, half, g, KC, block, h, t, j, c, i]
+        even, odd = c[..., 0, :], c[..., 1, :]
+        q = torch.stack([(even & 15) | ((odd & 15) << 4), (even >> 4) | (odd & 0xF0)], dim=3)
+        side = lambda t: rows(t.view(E, nt, kc, per, 8, 2, 2).permute(0, 1, 5, 6, 4, 2, 3), self.k // self.group)  # noqa: E731
+        s = side(self.data[..., 2048 : 2048 + per * 64].contiguous().view(torch.int16)).view(self.scale_dtype)
+        z = side(self.data[..., 2048 + per * 64 :].contiguous()) if self.zeros else None
+        got = (rows(q, self.k // 2), s, z)
         return got if self.experts else tuple(t if t is None else t[0] for t in got)
 
     def dequant(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -165,6 +173,10 @@ def quantize_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, scale
     return (code[..., 0::2] | (code[..., 1::2] << 4)).contiguous(), s, z
 
 
+def _args(w: W4Weight):
+    return w.data, w.n, w.k, w.group, w.zeros, w.scale_dtype == torch.float16
+
+
 def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ w^T (+ bias)`` for bf16 ``x [M, K]`` and a 4-bit ``w [N, K]``; bf16 ``[M, N]``. Sums are
     held in fp32. Rows of ``x`` may be strided."""
@@ -172,7 +184,7 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) ->
         raise ValueError("linear_w4 takes one ungated matrix")
     if not x.is_cuda:
         return ref.linear_w4(x, w, bias)
-    return _cuda().linear_w4(x, w.q, w.s, w.z, w.n, w.k, w.group, bias)
+    return _cuda().linear_w4(x, *_args(w), bias)
 
 
 def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tensor, ids: torch.Tensor, *,
@@ -190,5 +202,5 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
         raise ValueError(f"activation must be one of {sorted(_ACT)}, got {activation!r}")
     if not x.is_cuda:
         return ref.experts_w4(x, w1, w2, weights, ids, activation, expert_offset, w1_bias, w2_bias)
-    return _cuda().experts_w4(x, w1.q, w1.s, w1.z, w1.n, w1.k, w1.group, w2.q, w2.s, w2.z, w2.n, w2.k, w2.group,
-                              weights, ids, _ACT[activation], expert_offset, w1_bias, w2_bias)
+    return _cuda().experts_w4(x, *_args(w1), *_args(w2), weights, ids, _ACT[activation], expert_offset, w1_bias,
+                              w2_bias)

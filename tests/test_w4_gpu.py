@@ -7,6 +7,8 @@ with the weights rounded to bf16 (many tokens) are off by another 2^-8 of the su
 most, and by far less in the 2-norm: there one rounding is 2^-8 / sqrt(3) at most.
 """
 
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -395,8 +397,8 @@ def test_refusals():
     w1, w2 = _packed(c1, c2)
     wt, ids = torch.rand(4, 2, device=DEV), torch.zeros(4, 2, device=DEV, dtype=torch.int32)
     logits = torch.randn(4, 8, device=DEV)
-    short = ops.W4Weight(w.q, w.s, w.z, 500, w.k, w.group, False, False)
-    wrong_group = ops.W4Weight(w.q, w.s, w.z, w.n, w.k, 16, False, False)
+    short = replace(w, n=500)
+    wrong_group = replace(w, group=16)
     for bad in (
         lambda: ops.linear_w4(x.float(), w),
         lambda: ops.linear_w4(x[:, :64], w),
