@@ -8,7 +8,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "w4.cuh"
+#include "w4_gemm.cuh"
 
 using namespace msgl;
 
@@ -165,14 +165,15 @@ int launch_linear_nt(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   return w4_dispatch(w, [&](auto g, auto z, auto f) { return launch_linear<NT, g(), z(), f()>(p, s); });
 }
 
+// Tokens up to which the streaming product is taken (one or two columns of 8).
+constexpr int kStreamTokens = 16;
+
 // rows in one launch if their activations fit into shared memory, else in parts
 int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
-  const int rc = p.M <= 8    ? launch_linear_nt<1>(p, w, s)
-                 : p.M <= 16 ? launch_linear_nt<2>(p, w, s)
-                             : launch_linear_nt<4>(p, w, s);
+  const int rc = p.M <= 8 ? launch_linear_nt<1>(p, w, s) : launch_linear_nt<2>(p, w, s);
   if (rc != 3 || p.M == 1) return rc;
   LinearArgs a = p, b = p;
-  a.M = p.M > 16 ? 16 : p.M > 8 ? 8 : p.M / 2;
+  a.M = p.M > 8 ? 8 : p.M / 2;
   b.M = p.M - a.M;
   b.x += a.M * p.x_stride;
   b.out += (int64_t)a.M * p.w.n;
@@ -180,21 +181,35 @@ int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   return ra != 0 ? ra : linear_rows(b, w, s);
 }
 
+// many tokens: tiles of 128 rows by up to 256 tokens; where these leave SMs idle a cluster cuts the inputs
+int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
+  W4GemmArgs p = {};
+  p.w = a.w;
+  p.group = w->group, p.zeros = w->zeros, p.fp16 = w->fp16;
+  p.in = a.x, p.in_stride = a.x_stride;
+  p.bias = a.bias;
+  p.out = a.out, p.out_stride = w->n;
+  p.M = a.M;
+  p.m_tiles = (a.M + 255) / 256;
+  p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
+  p.m_tiles = (a.M + p.bn - 1) / p.bn;
+  p.n_tiles = (a.w.tiles + 3) / 4;
+  const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
+  if (units >= (1ll << 31)) return 3;
+  const int sms = msgl_num_sms();
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / units, 8, (int64_t)a.w.kc}));
+  if (p.splits > 1) return w4_gemm_launch<kW4Dense, true>(p, (int)units * p.splits, s);
+  return w4_gemm_launch<kW4Dense, false>(p, (int)std::min<int64_t>(units, sms), s);
+}
+
 }  // namespace
 
 extern "C" int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
                               cudaStream_t s) {
-  LinearArgs p = {w4_tensor(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias, (__nv_bfloat16*)out,
-                  1, 0};
-  for (int m = 0; m < M; m += 32) {
-    LinearArgs a = p;
-    a.M = std::min(32, M - m);
-    a.x += m * x_stride;
-    a.out += (int64_t)m * w->n;
-    const int rc = linear_rows(a, w, s);
-    if (rc != 0) return rc;
-  }
-  return 0;
+  if (M == 0) return 0;
+  const LinearArgs p = {w4_tensor(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias,
+                        (__nv_bfloat16*)out, 1, 0};
+  return M <= kStreamTokens ? linear_rows(p, w, s) : linear_tiles(p, w, s);
 }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4)

@@ -50,7 +50,7 @@ struct W4Record {
 
 // warps by the number of 8-token columns: as many as the registers of their sums allow
 template <int NT>
-constexpr int w4_warps() { return NT == 1 ? 24 : NT == 2 ? 16 : 12; }
+constexpr int w4_warps() { return NT == 1 ? 24 : 16; }
 template <int NT>
 constexpr int w4_threads() { return w4_warps<NT>() * 32; }
 
