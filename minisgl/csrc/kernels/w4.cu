@@ -193,13 +193,22 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   p.m_tiles = (a.M + 255) / 256;
   p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
   p.m_tiles = (a.M + p.bn - 1) / p.bn;
-  p.n_tiles = (a.w.tiles + 3) / 4;
+  const int sms = msgl_num_sms();
+  // 256-row tiles unless these, their inputs cut in eight, would use less than half the SMs
+  const int64_t wide = (int64_t)((a.w.tiles + 7) / 8) * p.m_tiles;
+  const bool two = wide * std::min(8, a.w.kc) >= sms / 2;
+  p.n_tiles = two ? (a.w.tiles + 7) / 8 : (a.w.tiles + 3) / 4;
   const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
   if (units >= (1ll << 31)) return 3;
-  const int sms = msgl_num_sms();
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / units, 8, (int64_t)a.w.kc}));
-  if (p.splits > 1) return w4_gemm_launch<kW4Dense, true>(p, (int)units * p.splits, s);
-  return w4_gemm_launch<kW4Dense, false>(p, (int)std::min<int64_t>(units, sms), s);
+  const int grid = (int)std::min<int64_t>(units * p.splits, sms);
+  if (p.splits > 1) {
+    const int rc = two ? w4_gemm_launch<kW4Dense, 2, true>(p, grid, s) : w4_gemm_launch<kW4Dense, 1, true>(p, grid, s);
+    if (rc != 3) return rc;
+    p.splits = 1;  // the fp32 tile does not fit
+  }
+  return two ? w4_gemm_launch<kW4Dense, 2, false>(p, (int)std::min<int64_t>(units, sms), s)
+             : w4_gemm_launch<kW4Dense, 1, false>(p, (int)std::min<int64_t>(units, sms), s);
 }
 
 }  // namespace

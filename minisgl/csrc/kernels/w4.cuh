@@ -132,16 +132,17 @@ MSGL_DEVICE float2 w4_scales(uint32_t v) {
   return make_float2(bf16_lo(v), bf16_hi(v));
 }
 
-// a wait that did not succeed at once
+// A wait that did not succeed at once. NS > 0: the warp sleeps between its looks, so that it does not take
+// issue slots from the others (a look every 40 ns by each of 26 warps took most of an SM's). Bounded to a
+// few seconds; false when they are over.
+template <int NS>
 static __noinline__ __device__ bool w4_wait(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait_a(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
-      report_error(kErrMbarTimeout, 400);
-      return false;
-    }
+  for (int i = 0; i < (NS > 0 ? 1 << 24 : 1 << 26); ++i) {
+    if (mbar_try_wait_a(bar, parity)) return true;
+    if constexpr (NS > 0) __nanosleep(NS);
   }
-  return true;
+  report_error(kErrMbarTimeout, 400);
+  return false;
 }
 
 // The runs of a CTA: its shared memory and how far the ring of this thread's warp has turned. F: fp16 scales.
@@ -225,7 +226,7 @@ struct W4Runs {
     for (int i = threadIdx.x; i < nx * (pad / 8); i += w4_threads<NT>())
       *reinterpret_cast<uint4*>(xs + i / (pad / 8) * pitch + kn * 2 + i % (pad / 8) * 16) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (ok) ok = w4_wait(xbar(), runs & 1);
+    if (ok) ok = w4_wait<20>(xbar(), runs & 1);
     ++runs;
 
     uint32_t xrow[NT];
@@ -244,7 +245,7 @@ struct W4Runs {
         for (int r = 0; r < 4; ++r) acc[0][nt][r] = acc[1][nt][r] = 0.f;
       for (; i < end; ++i) {
         if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
-          if (ok) ok = w4_wait(bar, (it >> 1) & 1);
+          if (ok) ok = w4_wait<20>(bar, (it >> 1) & 1);
         }
         ++it;
         uint4 q[2][2];

@@ -1,16 +1,21 @@
 // 4-bit products for many tokens, on the 5th-generation tensor core (layout of the weights in w4.cuh).
 //
-// A tile is 128 weight rows (the MMA's M) by up to 256 tokens (its N, a multiple of 16 that follows the
-// number of tokens), 128 inputs per step. Roles of a CTA's 26 warps, one CTA per SM, persistent over tiles:
+// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 256 tokens (their N, a multiple of 16
+// that follows the number of tokens), 64 inputs per step. Roles of a CTA's 26 warps, one CTA per SM,
+// persistent over tiles:
 //   warps 0-3    epilogue, one TMEM lane quadrant each
 //   warps 4-7    the tokens' rows, gathered with cp.async into a ring of 128-byte-swizzled K-major tiles
-//   warp 8       bulk copies of the four records of a step into a ring of their own
-//   warp 9       MMA issuer: D[128 x N] += A[128 x 128] B[N x 128]^T, fp32 in TMEM, two accumulators
-//   warps 10-25  records -> bf16 A tiles: the codes become bf16 as in w4.cuh, times the group's scale
+//   warp 8       bulk copies of the tile's records of 128 inputs (two steps) into a ring of their own
+//   warp 9       MMA issuer: D_h[128 x N] += A_h[128 x 64] B[N x 64]^T, fp32 in TMEM, two sets if they fit
+//   warps 10-25  records -> bf16 A tiles: the codes become bf16 as in w4.cuh, times the group's scale. Half of
+//                them take the even steps, half the odd ones: one half converts while the other waits for
+//                its barriers and its stores' fence.
 // Rounding (code - zero) * scale to bf16 is a choice: an fp32 scale applied to the sums would need the
 // accumulator to be read back once per group. It adds half a step of bf16 per weight, independent from
-// weight to weight, about what the result's own rounding does. The conversion bounds the kernel (11
-// instructions per 8 codes, and 8 for scales and stores) up to about 128 tokens, then the tensor core.
+// weight to weight, about what the result's own rounding does.
+//
+// 256 rows per tile (H = 2) because the tokens' rows come from L2 once per tile: with 128 rows 200 tokens x
+// 34816 x 5120 read 560 MB of them, 145 us. H = 1 where 256-row tiles would leave SMs idle.
 //
 // SPLIT: the CTAs of a cluster cut the inputs of one tile; each leaves its fp32 tile in its drained rings
 // and sums its share of the tokens over the cluster through distributed shared memory.
@@ -35,18 +40,14 @@ struct W4GemmArgs {
   const int4* work;
   const int* sorted;
   int topk, act;
-  int stages;
+  int stages, slots, raw_bytes;  // rings: operand tiles, records of two steps
 };
 
 constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
-constexpr int kGwRaw = 4 * W4Record<32, true>::kBytes, kGwRawSlots = 2;
-constexpr int kGwA = 128 * 128 * 2;
+constexpr int kGwMaxSlots = 8, kGwMaxStages = 4;
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
-__host__ __device__ constexpr int w4_gemm_stage(int bn) { return kGwA + bn * 256; }
-__host__ __device__ constexpr int w4_gemm_smem(int bn, int stages) {
-  return 1024 + stages * w4_gemm_stage(bn) + kGwRawSlots * kGwRaw + kGwMisc;
-}
+__host__ __device__ constexpr int w4_gemm_stage(int h, int bn) { return h * 128 * 128 + bn * 128; }
 
 MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
   if (act == 0) return g / (1.f + __expf(-g)) * u;
@@ -57,34 +58,49 @@ MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
 }
 
 // pair of exact integers (bf16x2) times a scale, rounded once
-MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale, bool fp16) {
-  if (fp16) return pack_bf16(bf16_lo(v) * scale, bf16_hi(v) * scale);
+template <bool F>
+MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale) {
+  if constexpr (F) return pack_bf16(bf16_lo(v) * scale, bf16_hi(v) * scale);
   const __nv_bfloat162 p = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&scale2));
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-template <int MODE, bool SPLIT>
+MSGL_DEVICE void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// a role's wait: true once the phase is complete, false if it never is
+template <int NS>
+MSGL_DEVICE bool w4_await(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  return mbar_try_wait_a(a, parity) || w4_wait<NS>(a, parity);
+}
+
+template <int MODE, int H, bool SPLIT, bool F>
 __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_constant__ W4GemmArgs p) {
+  static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
+  constexpr int kRecs = 4 * H, kA = H * 128 * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int S = p.stages, stage_bytes = w4_gemm_stage(p.bn);
+  const int S = p.stages, stage_bytes = w4_gemm_stage(H, p.bn);
   uint8_t* raw = smem + S * stage_bytes;
-  int* rows = reinterpret_cast<int*>(raw + kGwRawSlots * kGwRaw);
+  int* rows = reinterpret_cast<int*>(raw + p.slots * p.raw_bytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(rows + 256);
-  uint64_t *raw_full = bars, *raw_empty = bars + kGwRawSlots, *a_full = raw_empty + kGwRawSlots, *b_full = a_full + 4,
-           *ab_empty = b_full + 4, *tfull = ab_empty + 4, *tempty = tfull + 2;
+  uint64_t *raw_full = bars, *raw_empty = bars + kGwMaxSlots, *a_full = raw_empty + kGwMaxSlots,
+           *b_full = a_full + kGwMaxStages, *ab_empty = b_full + kGwMaxStages, *tfull = ab_empty + kGwMaxStages,
+           *tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = SPLIT ? (int)cluster_ctarank() : 0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kGwRawSlots; ++i) {
+    for (int i = 0; i < p.slots; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], kGwConv);
     }
     for (int i = 0; i < S; ++i) {
-      mbar_init(&a_full[i], kGwConv);
-      mbar_init(&b_full[i], kGwLoad);
+      mbar_init(&a_full[i], kGwConv / 2);
+      mbar_init(&b_full[i], kGwLoad * 32);
       mbar_init(&ab_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -93,9 +109,11 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     }
     fence_barrier_init();
   }
-  const int acc_cols = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
+  // accumulators: H x half_cols columns a set, two sets if TMEM's 512 columns hold them
+  const int half_cols = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
+  const int sets = 2 * H * half_cols <= 512 ? 2 : 1, tmem_cols = sets * H * half_cols;
   if (warp == 9) {
-    tmem_alloc(tmem_slot, 2 * acc_cols);
+    tmem_alloc(tmem_slot, tmem_cols);
     tmem_relinquish();
   }
   pdl_launch();
@@ -129,6 +147,9 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     t.cols = (t.n + 15) & ~15;
     return t;
   };
+  // set and phase of the n-th tile of this CTA
+  const auto set_of = [&](int n) { return sets == 2 ? n & 1 : 0; };
+  const auto set_phase = [&](int n) { return (uint32_t)(sets == 2 ? n >> 1 : n) & 1; };
 
   bool ok = true;
   if (warp < kGwEpi) {
@@ -136,38 +157,39 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     int use = 0;
     for (int u = u_first; u < units && ok && !SPLIT; u += u_step, ++use) {
       const Tile tl = tile_of(u);
-      const int acc = use & 1;
-      if (!(ok = mbar_wait(&tfull[acc], (use >> 1) & 1, 410))) break;
+      const int set = set_of(use);
+      if (!(ok = w4_await<200>(&tfull[set], set_phase(use)))) break;
       tc_fence_after();
-      const uint32_t d = tmem + acc * acc_cols + ((uint32_t)(warp * 32) << 16);
+      const uint32_t d = tmem + set * H * half_cols + ((uint32_t)(warp * 32) << 16);
       const __nv_bfloat16* bias = p.bias == nullptr ? nullptr : p.bias + (int64_t)tl.e * p.w.n;
       for (int c0 = 0; c0 < tl.cols; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(d + c0, r);
-        tc_wait_ld();
         const int cn = min(16, tl.n - c0);
-        if constexpr (MODE == kW4GateUp) {
-          // even rows are gates, odd rows their ups: even lanes finish even tokens, odd lanes odd ones
-          const int inter = p.w.n / 2, i = tl.nt * 64 + warp * 16 + (lane >> 1), odd = lane & 1;
-          const float bg = bias != nullptr && i < inter ? __bfloat162float(bias[i]) : 0.f;
-          const float bu = bias != nullptr && i < inter ? __bfloat162float(bias[inter + i]) : 0.f;
+        uint32_t r[H][16];
 #pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const float v0 = __uint_as_float(r[c]), v1 = __uint_as_float(r[c + 1]);
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
-            const float gate = odd ? got : v0, up = odd ? v1 : got;
-            if (c + odd < cn && i < inter)
-              reinterpret_cast<__nv_bfloat16*>(p.out)[(int64_t)(tl.row0 + c0 + c + odd) * p.out_stride + i] =
-                  __float2bfloat16(w4_gated_act(gate + bg, up + bu, p.act));
+        for (int h = 0; h < H; ++h) tmem_ld_32x32b_x16(d + h * half_cols + c0, r[h]);
+        tc_wait_ld();
+        if constexpr (MODE == kW4GateUp) {
+          const int inter = p.w.n / 2, i = tl.nt * 128 + warp * 32 + lane;
+          if (i < inter) {
+            const float bg = bias != nullptr ? __bfloat162float(bias[i]) : 0.f;
+            const float bu = bias != nullptr ? __bfloat162float(bias[inter + i]) : 0.f;
+            __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(tl.row0 + c0) * p.out_stride + i;
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (c < cn)
+                o[c * p.out_stride] = __float2bfloat16(
+                    w4_gated_act(__uint_as_float(r[0][c]) + bg, __uint_as_float(r[H - 1][c]) + bu, p.act));
           }
         } else {
-          const int n = tl.nt * 128 + warp * 32 + lane;
-          if (n < p.w.n) {
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            const int n = (tl.nt * H + h) * 128 + warp * 32 + lane;
+            if (n >= p.w.n) continue;
             const float b = bias == nullptr ? 0.f : __bfloat162float(bias[n]);
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
               if (c >= cn) break;
-              const float v = __uint_as_float(r[c]) + b;
+              const float v = __uint_as_float(r[h][c]) + b;
               if constexpr (MODE == kW4Dense)
                 reinterpret_cast<__nv_bfloat16*>(p.out)[(int64_t)(tl.row0 + c0 + c) * p.out_stride + n] = __float2bfloat16(v);
               else
@@ -178,29 +200,31 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[acc]);
+      if (lane == 0) mbar_arrive(&tempty[set]);
     }
     if constexpr (SPLIT) {
-      // one tile per cluster: leave it as fp32 [token][128 rows] in the drained rings
+      // one tile per cluster: leave it as fp32 [token][128 H rows] in the drained rings
       const Tile tl = tile_of(u_first);
-      if (ok) ok = mbar_wait(&tfull[0], 0, 411);
+      if (ok) ok = w4_await<200>(&tfull[0], 0);
       tc_fence_after();
       float* dump = reinterpret_cast<float*>(smem);
-      for (int c0 = 0; c0 < tl.cols; c0 += 16) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(tmem + ((uint32_t)(warp * 32) << 16) + c0, r);
-        tc_wait_ld();
+      for (int c0 = 0; c0 < tl.cols; c0 += 16)
 #pragma unroll
-        for (int c = 0; c < 16; ++c) dump[(c0 + c) * 128 + warp * 32 + lane] = __uint_as_float(r[c]);
-      }
+        for (int h = 0; h < H; ++h) {
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(tmem + ((uint32_t)(warp * 32) << 16) + h * half_cols + c0, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 16; ++c) dump[((c0 + c) * H + h) * 128 + warp * 32 + lane] = __uint_as_float(r[c]);
+        }
       tc_fence_before();
     }
   } else if (warp < kGwEpi + kGwLoad) {
     // ------------------------------------------------------------------ tokens' rows
-    const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 15, r0 = lt >> 4;
+    const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 7, r0 = lt >> 3;
+    constexpr int kRows = kGwLoad * 4;  // rows of one pass
     int stage = 0;
     uint32_t phase = 0;
-    int before = -1;  // stage of the previous step, whose copies have not been waited for
     for (int u = u_first; u < units && ok; u += u_step) {
       const Tile tl = tile_of(u);
       if constexpr (MODE == kW4GateUp) {
@@ -208,52 +232,41 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
         for (int r = lt; r < tl.cols; r += kGwLoad * 32) rows[r] = p.sorted[tl.row0 + min(r, tl.n - 1)] / p.topk;
         named_bar_sync(1, kGwLoad * 32);
       }
-      for (int kb = k0; kb < k1; ++kb) {
-        if (!(ok = mbar_wait(&ab_empty[stage], phase ^ 1, 412))) break;
-        const uint32_t dst = smem_u32(smem + stage * stage_bytes + kGwA) + (chunk >> 3) * tl.cols * 128;
-        const int k = kb * 128 + chunk * 8;
+      for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
+        if (!(ok = w4_await<50>(&ab_empty[stage], phase ^ 1))) break;
+        // a thread's rows are 16 apart, so their swizzle is the same
+        uint32_t dst = smem_u32(smem) + stage * stage_bytes + kA + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+        const int k = ks * 64 + chunk * 8;
         const uint32_t bytes = k < p.w.k ? 16 : 0;  // zeros beyond the last input
-        const int kk = min(k, p.w.k - 8);
-        for (int r = r0; r < tl.cols; r += kGwLoad * 2) {
+        const __nv_bfloat16* src = p.in + min(k, p.w.k - 8);
+        for (int r = r0; r < tl.cols; r += kRows, dst += kRows * 128) {
           const int row = MODE == kW4GateUp ? rows[r] : tl.row0 + min(r, tl.n - 1);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)),
-                       "l"(p.in + (int64_t)row * p.in_stride + kk), "r"(bytes)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src + (int64_t)row * p.in_stride),
+                       "r"(bytes)
                        : "memory");
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (before >= 0) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b_full[before]);
-        }
-        before = stage;
+        // counts on the barrier when this thread's copies have landed; the MMA thread fences the proxies
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&b_full[stage])) : "memory");
         if (++stage == S) stage = 0, phase ^= 1;
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (before >= 0) {
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b_full[before]);
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 8) {
     // ------------------------------------------------------------------ records
-    const int bytes = W4Record<128, false>::kScales + 128 / p.group * (p.zeros ? 96 : 64);
+    const int bytes = p.raw_bytes / kRecs;
     if (lane == 0) {
       int slot = 0;
       uint32_t phase = 0;
       for (int u = u_first; u < units && ok; u += u_step) {
         const Tile tl = tile_of(u);
-        const int n = min(4, p.w.tiles - tl.nt * 4);
-        const uint8_t* src = p.w.data + ((int64_t)tl.e * p.w.tiles + tl.nt * 4) * p.w.kc * bytes;
+        const int n = min(kRecs, p.w.tiles - tl.nt * kRecs);
+        const uint8_t* src = p.w.data + ((int64_t)tl.e * p.w.tiles + tl.nt * kRecs) * p.w.kc * bytes;
         for (int kb = k0; kb < k1; ++kb) {
-          if (!(ok = mbar_wait(&raw_empty[slot], phase ^ 1, 413))) break;
+          if (!(ok = w4_await<100>(&raw_empty[slot], phase ^ 1))) break;
           mbar_expect_tx(&raw_full[slot], n * bytes);
           for (int i = 0; i < n; ++i)
-            bulk_load(raw + slot * kGwRaw + i * bytes, src + ((int64_t)i * p.w.kc + kb) * bytes, bytes, &raw_full[slot]);
-          if (++slot == kGwRawSlots) slot = 0, phase ^= 1;
+            bulk_load(raw + slot * p.raw_bytes + i * bytes, src + ((int64_t)i * p.w.kc + kb) * bytes, bytes, &raw_full[slot]);
+          if (++slot == p.slots) slot = 0, phase ^= 1;
         }
       }
     }
@@ -264,89 +277,95 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
       uint32_t phase = 0;
       for (int u = u_first; u < units && ok; u += u_step, ++use) {
         const Tile tl = tile_of(u);
-        const uint32_t idesc = idesc_bf16_f32(128, tl.cols), d = tmem + (use & 1) * acc_cols;
-        if (!(ok = mbar_wait(&tempty[use & 1], ((use >> 1) & 1) ^ 1, 414))) break;
+        const uint32_t idesc = idesc_bf16_f32(128, tl.cols), d = tmem + set_of(use) * H * half_cols;
+        if (!(ok = w4_await<20>(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
         tc_fence_after();
-        for (int kb = k0; kb < k1; ++kb) {
-          if (!(ok = mbar_wait(&b_full[stage], phase, 415) && mbar_wait(&a_full[stage], phase, 416))) break;
+        for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
+          if (!(ok = w4_await<0>(&b_full[stage], phase) && w4_await<0>(&a_full[stage], phase))) break;
+          fence_async_smem();
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + kGwA;
+          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + kA;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            tc_mma_f16(d, smem_desc_sw128(a + (j >> 2) * (128 * 128) + (j & 3) * 32),
-                       smem_desc_sw128(b + (j >> 2) * tl.cols * 128 + (j & 3) * 32), idesc, kb > k0 || j > 0);
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+              tc_mma_f16(d + h * half_cols, smem_desc_sw128(a + h * (128 * 128) + j * 32), smem_desc_sw128(b + j * 32),
+                         idesc, ks > 2 * k0 || j > 0);
           tc_commit(&ab_empty[stage]);
           if (++stage == S) stage = 0, phase ^= 1;
         }
-        tc_commit(&tfull[use & 1]);
+        tc_commit(&tfull[set_of(use)]);
       }
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ records -> A tile
-    // a warp's part of a step: 16 rows by 64 inputs of one record
-    const int cw = warp - kGwEpi - kGwLoad - 2, ti = cw >> 2, half = (cw >> 1) & 1, block = cw & 1;
-    const int g = lane >> 2, t = lane & 3;
-    const int bytes = W4Record<128, false>::kScales + 128 / p.group * (p.zeros ? 96 : 64);
+    // a warp's part of a step: 64 inputs of 16 H rows of a record (H = 1: two warps share a record)
+    const int cw = warp - kGwEpi - kGwLoad - 2, block = cw & 1, m = cw >> 1;
+    const int ti = H == 2 ? m : m >> 1, g = lane >> 2, t = lane & 3;
+    const int bytes = p.raw_bytes / kRecs;
     const int shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;  // quarters of a record per group
     const int zoff = W4Record<128, false>::kScales + 128 / p.group * 64;
-    // rows of the A tile: as in the records, or (gated) gate and up rows in turn
-    const int ra = MODE == kW4GateUp ? 2 * (ti * 16 + half * 8 + g) : ti * 32 + half * 16 + g;
-    const int rb = MODE == kW4GateUp ? ra + 1 : ra + 8;
-    int stage = 0, slot = 0;
+    const uint32_t raw0 = smem_u32(raw), ops0 = smem_u32(smem);
+    int stage = block, slot = 0;
     uint32_t phase = 0, rphase = 0;
     for (int u = u_first; u < units && ok; u += u_step) {
       const Tile tl = tile_of(u);
-      const bool there = tl.nt * 4 + ti < p.w.tiles;
+      const bool there = tl.nt * kRecs + ti < p.w.tiles;
       for (int kb = k0; kb < k1; ++kb) {
-        if (!(ok = mbar_wait(&raw_full[slot], rphase, 417))) break;
-        const uint32_t rec = smem_u32(raw + slot * kGwRaw) + ti * bytes;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        uint32_t s[2] = {0, 0}, z[2] = {0x0808, 0x0808};
+        if (!(ok = w4_await<20>(&raw_full[slot], rphase))) break;
+        const uint32_t rec = raw0 + slot * p.raw_bytes + ti * bytes;
+        uint4 q[H] = {};
+        uint2 s[2] = {};
+        uint32_t z[2] = {0x08080808u, 0x08080808u};
         if (there) {
-          q = lds128(rec + (half * 2 + block) * 512 + lane * 16);
+#pragma unroll
+          for (int i = 0; i < H; ++i) q[i] = lds128(rec + ((H == 2 ? i : m & 1) * 2 + block) * 512 + lane * 16);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int grp = (block * 2 + h) >> shift;
-            s[h] = lds32(rec + W4Record<128, false>::kScales + grp * 64 + g * 8 + half * 4);
-            if (p.zeros) z[h] = lds32(rec + zoff + grp * 32 + g * 4) >> (16 * half);
+            const int grp = (2 * block + h) >> shift;
+            s[h] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
+            if (p.zeros) z[h] = lds32(rec + zoff + grp * 32 + g * 4);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[slot]);
-        if (++slot == kGwRawSlots) slot = 0, rphase ^= 1;
-        if (!(ok = mbar_wait(&ab_empty[stage], phase ^ 1, 418))) break;
+        if (++slot == p.slots) slot = 0, rphase ^= 1;
+        if (!(ok = w4_await<50>(&ab_empty[stage], phase ^ 1))) break;
         if (there) {
-          uint8_t* sub = smem + stage * stage_bytes + block * (128 * 128);
-          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            // neighbouring rows start with different halves of their 128 bytes: the stores of a quarter
-            // warp (two rows, four chunks) then fall into different banks
-            const int h = hh ^ (g & 1);
-            const uint32_t w0 = h ? words[2] : words[0], w1 = h ? words[3] : words[1];
-            const uint32_t sv = h ? s[1] : s[0], zv = h ? z[1] : z[0];
-            const uint32_t z0 = 0x43004300u + (zv & 15u) * 0x10001u, z1 = 0x43004300u + ((zv >> 8) & 15u) * 0x10001u;
-            const uint32_t sa2 = (sv & 0xffffu) * 0x10001u, sb2 = (sv >> 16) * 0x10001u;
-            float2 sf = make_float2(0.f, 0.f);
-            if (p.fp16) sf = w4_scales<true>(sv);
-            uint32_t oa[4], ob[4];
-            oa[0] = w4_times(codes_bf16x2(w0, z0), sa2, sf.x, p.fp16);
-            oa[1] = w4_times(codes_bf16x2(w0 >> 8, z0), sa2, sf.x, p.fp16);
-            oa[2] = w4_times(codes_bf16x2(w1, z0), sa2, sf.x, p.fp16);
-            oa[3] = w4_times(codes_bf16x2(w1 >> 8, z0), sa2, sf.x, p.fp16);
-            ob[0] = w4_times(codes_bf16x2(w0 >> 4, z1), sb2, sf.y, p.fp16);
-            ob[1] = w4_times(codes_bf16x2(w0 >> 12, z1), sb2, sf.y, p.fp16);
-            ob[2] = w4_times(codes_bf16x2(w1 >> 4, z1), sb2, sf.y, p.fp16);
-            ob[3] = w4_times(codes_bf16x2(w1 >> 12, z1), sb2, sf.y, p.fp16);
-            *reinterpret_cast<uint4*>(sub + ra * 128 + (((4 * h + t) ^ (ra & 7)) << 4)) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-            *reinterpret_cast<uint4*>(sub + rb * 128 + (((4 * h + t) ^ (rb & 7)) << 4)) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+          for (int i = 0; i < H; ++i) {
+            const int half = H == 2 ? i : m & 1;
+            // rows of the A tile: as in the records, or (gated) gate rows in one half and up rows in the other
+            const int row = MODE == kW4GateUp ? ti * 16 + half * 8 + g : (ti * 32 + half * 16 + g) & 127;
+            const uint32_t a = ops0 + stage * stage_bytes + row * 128 + (MODE != kW4GateUp ? (ti >> 2) * (128 * 128) : 0);
+            const uint32_t b = a + (MODE == kW4GateUp ? 128 * 128 : 8 * 128);
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              // neighbouring rows start with different halves of their 128 bytes: the stores of a quarter
+              // warp (two rows, four chunks) then fall into different banks
+              const int h = (hh ^ g) & 1;
+              const uint32_t w0 = h ? q[i].z : q[i].x, w1 = h ? q[i].w : q[i].y;
+              const uint2 s2 = h ? s[1] : s[0];
+              const uint32_t sv = half ? s2.y : s2.x, zv = (h ? z[1] : z[0]) >> (16 * half);
+              const uint32_t z0 = 0x43004300u + (zv & 15u) * 0x10001u, z1 = 0x43004300u + ((zv >> 8) & 15u) * 0x10001u;
+              const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
+              float2 sf = make_float2(0.f, 0.f);
+              if constexpr (F) sf = w4_scales<true>(sv);
+              const uint32_t at = ((4 * h + t) ^ (g & 7)) << 4;  // every row here is g modulo 8
+              sts128(a + at, w4_times<F>(codes_bf16x2(w0, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w0 >> 8, z0), sa2, sf.x),
+                     w4_times<F>(codes_bf16x2(w1, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w1 >> 8, z0), sa2, sf.x));
+              sts128(b + at, w4_times<F>(codes_bf16x2(w0 >> 4, z1), sb2, sf.y),
+                     w4_times<F>(codes_bf16x2(w0 >> 12, z1), sb2, sf.y), w4_times<F>(codes_bf16x2(w1 >> 4, z1), sb2, sf.y),
+                     w4_times<F>(codes_bf16x2(w1 >> 12, z1), sb2, sf.y));
+            }
           }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&a_full[stage]);
-        if (++stage == S) stage = 0, phase ^= 1;
+        stage += 2;  // the other half takes the step between; there are at least two stages
+        if (stage >= S) stage -= S, phase ^= 1;
       }
     }
   }
@@ -354,13 +373,13 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
   if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync();
-    // this CTA's share of the tokens: a warp per token, four rows a lane
+    // this CTA's share of the tokens: a warp per token and 128 rows, four rows a lane
     const Tile tl = tile_of(u_first);
-    const int n = tl.nt * 128 + lane * 4;
     const int from = tl.n * rank / p.splits, to = tl.n * (rank + 1) / p.splits;
-    for (int c = from + warp; c < to; c += kGwThreads / 32) {
+    for (int ch = from * H + warp; ch < to * H; ch += kGwThreads / 32) {
+      const int c = ch / H, n = (tl.nt * H + ch % H) * 128 + lane * 4;
       float v[4] = {};
-      const uint32_t at = smem_u32(smem) + (c * 128 + lane * 4) * 4;
+      const uint32_t at = smem_u32(smem) + (ch * 128 + lane * 4) * 4;
       for (int r = 0; r < p.splits; ++r) {
         const float4 f = ld_dsmem_v4(dsmem_addr(at, r));
         v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
@@ -383,20 +402,29 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * acc_cols);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
-template <int MODE, bool SPLIT>
-int w4_gemm_launch(W4GemmArgs p, int grid, cudaStream_t s) {
-  constexpr auto kernel = w4_gemm_kernel<MODE, SPLIT>;
+template <int MODE, int H, bool SPLIT, bool F>
+int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
+  constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, F>;
   constexpr int kMax = 227 * 1024;
   if (msgl_set_smem<kernel>(kMax) != cudaSuccess) return 4;
-  p.stages = std::min(4, (kMax - w4_gemm_smem(p.bn, 0)) / w4_gemm_stage(p.bn));
-  return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), w4_gemm_smem(p.bn, p.stages), s, SPLIT ? p.splits : 1, p) ==
-                 cudaSuccess
-             ? 0
-             : 4;
+  // Records of two pairs of steps at least (a copy takes about 1 us), two to four operand stages, then the
+  // rest for records again. With `splits` the rings also hold the fp32 tile.
+  p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (p.zeros ? 96 : 64));
+  const int room = kMax - 1024 - kGwMisc, stage = w4_gemm_stage(H, p.bn);
+  p.stages = std::max(2, std::min(kGwMaxStages, (room - 2 * p.raw_bytes) / stage));
+  p.slots = std::min(kGwMaxSlots, (room - p.stages * stage) / p.raw_bytes);
+  if (SPLIT && p.bn * H * 512 > p.stages * stage + p.slots * p.raw_bytes) return 3;
+  const int smem = 1024 + kGwMisc + p.stages * stage + p.slots * p.raw_bytes;
+  return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p) == cudaSuccess ? 0 : 4;
+}
+
+template <int MODE, int H, bool SPLIT>
+int w4_gemm_launch(const W4GemmArgs& p, int grid, cudaStream_t s) {
+  return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, true>(p, grid, s) : w4_gemm_launch_as<MODE, H, SPLIT, false>(p, grid, s);
 }
 
 }  // namespace msgl
