@@ -4,7 +4,8 @@
 // that follows the number of tokens), 64 inputs per step. Roles of a CTA's 26 warps, one CTA per SM,
 // persistent over tiles:
 //   warps 0-3    epilogue, one TMEM lane quadrant each
-//   warps 4-7    the tokens' rows, gathered with cp.async into a ring of 128-byte-swizzled K-major tiles
+//   warps 4-7    the tokens' rows into a ring of 128-byte-swizzled K-major tiles: one TMA copy per step (dense),
+//                one per 16 rows (down), or gathered by token with cp.async (gate_up)
 //   warp 8       bulk copies of the tile's records of 128 inputs (two steps) into a ring of their own
 //   warp 9       MMA issuer: D_h[128 x N] += A_h[128 x 64] B[N x 64]^T, fp32 in TMEM, two sets if they fit
 //   warps 10-25  records -> bf16 A tiles: the codes become bf16 as in w4.cuh, times the group's scale. Half of
@@ -20,6 +21,8 @@
 // SPLIT: the CTAs of a cluster cut the inputs of one tile; each leaves its fp32 tile in its drained rings
 // and sums its share of the tokens over the cluster through distributed shared memory.
 #pragma once
+#include <mutex>
+
 #include "w4.cuh"
 
 namespace msgl {
@@ -76,8 +79,9 @@ MSGL_DEVICE bool w4_await(uint64_t* bar, uint32_t parity) {
   return mbar_try_wait_a(a, parity) || w4_wait<NS>(a, parity);
 }
 
-template <int MODE, int H, bool SPLIT, bool F>
-__global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_constant__ W4GemmArgs p) {
+template <int MODE, int H, bool SPLIT, bool Z, bool F>
+__global__ void __launch_bounds__(kGwThreads, 1)
+w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUtensorMap rows_map) {
   static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
   constexpr int kRecs = 4 * H, kA = H * 128 * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     }
     for (int i = 0; i < S; ++i) {
       mbar_init(&a_full[i], kGwConv / 2);
-      mbar_init(&b_full[i], kGwLoad * 32);
+      mbar_init(&b_full[i], MODE == kW4GateUp ? kGwLoad : 1);
       mbar_init(&ab_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -108,6 +112,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
       mbar_init(&tempty[i], kGwEpi);
     }
     fence_barrier_init();
+    if constexpr (MODE != kW4GateUp) prefetch_tmap(&rows_map);
   }
   // accumulators: H x half_cols columns a set, two sets if TMEM's 512 columns hold them
   const int half_cols = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     for (int u = u_first; u < units && ok && !SPLIT; u += u_step, ++use) {
       const Tile tl = tile_of(u);
       const int set = set_of(use);
-      if (!(ok = w4_await<200>(&tfull[set], set_phase(use)))) break;
+      if (!(ok = w4_await<500>(&tfull[set], set_phase(use)))) break;
       tc_fence_after();
       const uint32_t d = tmem + set * H * half_cols + ((uint32_t)(warp * 32) << 16);
       const __nv_bfloat16* bias = p.bias == nullptr ? nullptr : p.bias + (int64_t)tl.e * p.w.n;
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     if constexpr (SPLIT) {
       // one tile per cluster: leave it as fp32 [token][128 H rows] in the drained rings
       const Tile tl = tile_of(u_first);
-      if (ok) ok = w4_await<200>(&tfull[0], 0);
+      if (ok) ok = w4_await<500>(&tfull[0], 0);
       tc_fence_after();
       float* dump = reinterpret_cast<float*>(smem);
       for (int c0 = 0; c0 < tl.cols; c0 += 16)
@@ -221,36 +226,65 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     }
   } else if (warp < kGwEpi + kGwLoad) {
     // ------------------------------------------------------------------ tokens' rows
-    const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 7, r0 = lt >> 3;
-    constexpr int kRows = kGwLoad * 4;  // rows of one pass
     int stage = 0;
     uint32_t phase = 0;
-    for (int u = u_first; u < units && ok; u += u_step) {
-      const Tile tl = tile_of(u);
-      if constexpr (MODE == kW4GateUp) {
+    if constexpr (MODE != kW4GateUp) {
+      if (warp == kGwEpi && lane == 0) {
+        for (int u = u_first; u < units && ok; u += u_step) {
+          const Tile tl = tile_of(u);
+          for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
+            if (!(ok = w4_await<100>(&ab_empty[stage], phase ^ 1))) break;
+            uint8_t* dst = smem + stage * stage_bytes + kA;
+            // rows beyond the last one and inputs beyond the last one arrive as zeros, and count
+            if constexpr (MODE == kW4Dense) {
+              mbar_expect_tx(&b_full[stage], p.bn * 128);
+              tma_load_2d(dst, &rows_map, &b_full[stage], ks * 64, tl.row0);
+            } else {
+              mbar_expect_tx(&b_full[stage], tl.cols * 128);
+              for (int r = 0; r < tl.cols; r += 16) tma_load_2d(dst + r * 128, &rows_map, &b_full[stage], ks * 64, tl.row0 + r);
+            }
+            if (++stage == S) stage = 0, phase ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+    } else {
+      const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 7, r0 = lt >> 3;
+      constexpr int kRows = kGwLoad * 4;  // rows of one pass
+      int before = -1;                    // stage of the previous step, whose copies are not announced yet
+      const auto announce = [&] {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_full[before]);
+      };
+      for (int u = u_first; u < units && ok; u += u_step) {
+        const Tile tl = tile_of(u);
         named_bar_sync(1, kGwLoad * 32);  // the previous tile's numbers are no longer needed
         for (int r = lt; r < tl.cols; r += kGwLoad * 32) rows[r] = p.sorted[tl.row0 + min(r, tl.n - 1)] / p.topk;
         named_bar_sync(1, kGwLoad * 32);
-      }
-      for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-        if (!(ok = w4_await<50>(&ab_empty[stage], phase ^ 1))) break;
-        // a thread's rows are 16 apart, so their swizzle is the same
-        uint32_t dst = smem_u32(smem) + stage * stage_bytes + kA + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
-        const int k = ks * 64 + chunk * 8;
-        const uint32_t bytes = k < p.w.k ? 16 : 0;  // zeros beyond the last input
-        const __nv_bfloat16* src = p.in + min(k, p.w.k - 8);
-        for (int r = r0; r < tl.cols; r += kRows, dst += kRows * 128) {
-          const int row = MODE == kW4GateUp ? rows[r] : tl.row0 + min(r, tl.n - 1);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src + (int64_t)row * p.in_stride),
-                       "r"(bytes)
-                       : "memory");
+        for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
+          if (!(ok = w4_await<100>(&ab_empty[stage], phase ^ 1))) break;
+          // a thread's rows are 16 apart, so their swizzle is the same
+          uint32_t dst = smem_u32(smem) + stage * stage_bytes + kA + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+          const int k = ks * 64 + chunk * 8;
+          const uint32_t bytes = k < p.w.k ? 16 : 0;  // zeros beyond the last input
+          const __nv_bfloat16* src = p.in + min(k, p.w.k - 8);
+          for (int r = r0; r < tl.cols; r += kRows, dst += kRows * 128)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                         "l"(src + (int64_t)rows[r] * p.in_stride), "r"(bytes)
+                         : "memory");
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (before >= 0) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            announce();
+          }
+          before = stage;
+          if (++stage == S) stage = 0, phase ^= 1;
         }
-        // counts on the barrier when this thread's copies have landed; the MMA thread fences the proxies
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&b_full[stage])) : "memory");
-        if (++stage == S) stage = 0, phase ^= 1;
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (before >= 0) announce();
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 8) {
     // ------------------------------------------------------------------ records
     const int bytes = p.raw_bytes / kRecs;
@@ -262,7 +296,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
         const int n = min(kRecs, p.w.tiles - tl.nt * kRecs);
         const uint8_t* src = p.w.data + ((int64_t)tl.e * p.w.tiles + tl.nt * kRecs) * p.w.kc * bytes;
         for (int kb = k0; kb < k1; ++kb) {
-          if (!(ok = w4_await<100>(&raw_empty[slot], phase ^ 1))) break;
+          if (!(ok = w4_await<200>(&raw_empty[slot], phase ^ 1))) break;
           mbar_expect_tx(&raw_full[slot], n * bytes);
           for (int i = 0; i < n; ++i)
             bulk_load(raw + slot * p.raw_bytes + i * bytes, src + ((int64_t)i * p.w.kc + kb) * bytes, bytes, &raw_full[slot]);
@@ -282,15 +316,13 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
         tc_fence_after();
         for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
           if (!(ok = w4_await<0>(&b_full[stage], phase) && w4_await<0>(&a_full[stage], phase))) break;
-          fence_async_smem();
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + stage * stage_bytes), b = a + kA;
+          const uint64_t a = smem_desc_sw128(smem_u32(smem) + stage * stage_bytes), b = a + (kA >> 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int h = 0; h < H; ++h)
-              tc_mma_f16(d + h * half_cols, smem_desc_sw128(a + h * (128 * 128) + j * 32), smem_desc_sw128(b + j * 32),
-                         idesc, ks > 2 * k0 || j > 0);
+              tc_mma_f16(d + h * half_cols, a + (h * (128 * 128) + j * 32) / 16, b + j * 2, idesc, ks > 2 * k0 || j > 0);
           tc_commit(&ab_empty[stage]);
           if (++stage == S) stage = 0, phase ^= 1;
         }
@@ -307,6 +339,13 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
     const int shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;  // quarters of a record per group
     const int zoff = W4Record<128, false>::kScales + 128 / p.group * 64;
     const uint32_t raw0 = smem_u32(raw), ops0 = smem_u32(smem);
+    // rows g (and g + 8, kRowB behind) of a record's half in the A tile: as in the records, or (gated) gate rows
+    // in one half of the tile and up rows in the other
+    constexpr uint32_t kRowB = MODE == kW4GateUp ? 128 * 128 : 8 * 128;
+    const uint32_t row0 = (MODE == kW4GateUp ? ti * 16 + g : ti * 32 + g) * 128;
+    // neighbouring rows start with different halves of their 128 bytes: the stores of a quarter warp (two
+    // rows, four chunks) then fall into different banks
+    const uint32_t at0 = ((4 * (g & 1) + t) ^ g) << 4, at1 = ((4 * (~g & 1) + t) ^ g) << 4;
     int stage = block, slot = 0;
     uint32_t phase = 0, rphase = 0;
     for (int u = u_first; u < units && ok; u += u_step) {
@@ -315,17 +354,16 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
       for (int kb = k0; kb < k1; ++kb) {
         if (!(ok = w4_await<20>(&raw_full[slot], rphase))) break;
         const uint32_t rec = raw0 + slot * p.raw_bytes + ti * bytes;
-        uint4 q[H] = {};
-        uint2 s[2] = {};
+        uint2 q[H][2] = {}, s[2] = {};
         uint32_t z[2] = {0x08080808u, 0x08080808u};
         if (there) {
 #pragma unroll
-          for (int i = 0; i < H; ++i) q[i] = lds128(rec + ((H == 2 ? i : m & 1) * 2 + block) * 512 + lane * 16);
+          for (int e = 0; e < 2; ++e) {
+            const int h = (e ^ g) & 1, grp = (2 * block + h) >> shift;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int grp = (2 * block + h) >> shift;
-            s[h] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
-            if (p.zeros) z[h] = lds32(rec + zoff + grp * 32 + g * 4);
+            for (int i = 0; i < H; ++i) q[i][e] = lds64(rec + ((H == 2 ? i : m & 1) * 2 + block) * 512 + lane * 16 + h * 8);
+            s[e] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
+            if constexpr (Z) z[e] = lds32(rec + zoff + grp * 32 + g * 4);
           }
         }
         __syncwarp();
@@ -336,26 +374,19 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
 #pragma unroll
           for (int i = 0; i < H; ++i) {
             const int half = H == 2 ? i : m & 1;
-            // rows of the A tile: as in the records, or (gated) gate rows in one half and up rows in the other
-            const int row = MODE == kW4GateUp ? ti * 16 + half * 8 + g : (ti * 32 + half * 16 + g) & 127;
-            const uint32_t a = ops0 + stage * stage_bytes + row * 128 + (MODE != kW4GateUp ? (ti >> 2) * (128 * 128) : 0);
-            const uint32_t b = a + (MODE == kW4GateUp ? 128 * 128 : 8 * 128);
+            const uint32_t a = ops0 + stage * stage_bytes + row0 + half * (MODE == kW4GateUp ? 8 * 128 : 16 * 128);
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              // neighbouring rows start with different halves of their 128 bytes: the stores of a quarter
-              // warp (two rows, four chunks) then fall into different banks
-              const int h = (hh ^ g) & 1;
-              const uint32_t w0 = h ? q[i].z : q[i].x, w1 = h ? q[i].w : q[i].y;
-              const uint2 s2 = h ? s[1] : s[0];
-              const uint32_t sv = half ? s2.y : s2.x, zv = (h ? z[1] : z[0]) >> (16 * half);
-              const uint32_t z0 = 0x43004300u + (zv & 15u) * 0x10001u, z1 = 0x43004300u + ((zv >> 8) & 15u) * 0x10001u;
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t w0 = q[i][e].x, w1 = q[i][e].y, sv = half ? s[e].y : s[e].x, zv = z[e] >> (16 * half);
+              const uint32_t z0 = Z ? 0x43004300u + (zv & 15u) * 0x10001u : 0x43084308u;
+              const uint32_t z1 = Z ? 0x43004300u + ((zv >> 8) & 15u) * 0x10001u : 0x43084308u;
               const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
               float2 sf = make_float2(0.f, 0.f);
               if constexpr (F) sf = w4_scales<true>(sv);
-              const uint32_t at = ((4 * h + t) ^ (g & 7)) << 4;  // every row here is g modulo 8
-              sts128(a + at, w4_times<F>(codes_bf16x2(w0, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w0 >> 8, z0), sa2, sf.x),
+              const uint32_t at = a + (e ? at1 : at0);
+              sts128(at, w4_times<F>(codes_bf16x2(w0, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w0 >> 8, z0), sa2, sf.x),
                      w4_times<F>(codes_bf16x2(w1, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w1 >> 8, z0), sa2, sf.x));
-              sts128(b + at, w4_times<F>(codes_bf16x2(w0 >> 4, z1), sb2, sf.y),
+              sts128(at + kRowB, w4_times<F>(codes_bf16x2(w0 >> 4, z1), sb2, sf.y),
                      w4_times<F>(codes_bf16x2(w0 >> 12, z1), sb2, sf.y), w4_times<F>(codes_bf16x2(w1 >> 4, z1), sb2, sf.y),
                      w4_times<F>(codes_bf16x2(w1 >> 12, z1), sb2, sf.y));
             }
@@ -406,25 +437,56 @@ __global__ void __launch_bounds__(kGwThreads, 1) w4_gemm_kernel(const __grid_con
   }
 }
 
-template <int MODE, int H, bool SPLIT, bool F>
+typedef CUresult (*W4EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// bf16 rows [rows, cols] with boxes of 64 columns x box_rows, 128-byte swizzle; false if it cannot be encoded
+inline bool w4_rows_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
+  static W4EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<W4EncodeFn>(ptr);
+  });
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, ones,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MODE, int H, bool SPLIT, bool Z, bool F>
 int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
-  constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, F>;
+  constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, Z, F>;
   constexpr int kMax = 227 * 1024;
   if (msgl_set_smem<kernel>(kMax) != cudaSuccess) return 4;
   // Records of two pairs of steps at least (a copy takes about 1 us), two to four operand stages, then the
   // rest for records again. With `splits` the rings also hold the fp32 tile.
-  p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (p.zeros ? 96 : 64));
+  p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
   const int room = kMax - 1024 - kGwMisc, stage = w4_gemm_stage(H, p.bn);
   p.stages = std::max(2, std::min(kGwMaxStages, (room - 2 * p.raw_bytes) / stage));
   p.slots = std::min(kGwMaxSlots, (room - p.stages * stage) / p.raw_bytes);
   if (SPLIT && p.bn * H * 512 > p.stages * stage + p.slots * p.raw_bytes) return 3;
+  CUtensorMap map = {};
+  if (MODE != kW4GateUp &&
+      !w4_rows_map(&map, p.in, p.M, p.w.k, p.M == 1 ? (int64_t)p.w.k : p.in_stride, MODE == kW4Dense ? p.bn : 16))
+    return 2;
   const int smem = 1024 + kGwMisc + p.stages * stage + p.slots * p.raw_bytes;
-  return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p) == cudaSuccess ? 0 : 4;
+  return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
 }
 
 template <int MODE, int H, bool SPLIT>
 int w4_gemm_launch(const W4GemmArgs& p, int grid, cudaStream_t s) {
-  return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, true>(p, grid, s) : w4_gemm_launch_as<MODE, H, SPLIT, false>(p, grid, s);
+  if (p.zeros)
+    return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, true, true>(p, grid, s)
+                  : w4_gemm_launch_as<MODE, H, SPLIT, true, false>(p, grid, s);
+  return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, false, true>(p, grid, s)
+                : w4_gemm_launch_as<MODE, H, SPLIT, false, false>(p, grid, s);
 }
 
 }  // namespace msgl
