@@ -181,7 +181,7 @@ int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   return ra != 0 ? ra : linear_rows(b, w, s);
 }
 
-// many tokens: tiles of 128 rows by up to 256 tokens; where these leave SMs idle a cluster cuts the inputs
+// many tokens: tiles of 128 or 256 rows by up to 192 tokens; where these leave SMs idle a cluster cuts the inputs
 int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   W4GemmArgs p = {};
   p.w = a.w;
@@ -190,7 +190,7 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   p.bias = a.bias;
   p.out = a.out, p.out_stride = w->n;
   p.M = a.M;
-  p.m_tiles = (a.M + 255) / 256;
+  p.m_tiles = (a.M + kGwMaxTokens - 1) / kGwMaxTokens;
   p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
   p.m_tiles = (a.M + p.bn - 1) / p.bn;
   const int sms = msgl_num_sms();

@@ -2,8 +2,8 @@
 //
 // Packed weights (ops/w4.py lays them out once) are records of 32 rows by 128 inputs, [E][Nt][KC][bytes]:
 //   2048 bytes of codes: two halves of 16 rows, of each two blocks of 64 inputs in the order of the tensor
-//     core's A fragments: lane 4 g + t has 16 bytes = 4 words of a block. Word 2h + j holds, for
-//     k = 64 block + 32 h + 8 t + 4 j,
+//     core's A fragments: lane 4 g + t has 16 bytes = 4 words of a block. Word b holds, for
+//     k = 64 block + 16 b + 4 t,
 //       row g     codes k, k+1, k+2, k+3 in nibbles 0, 4, 2, 6
 //       row g + 8 codes k, k+1, k+2, k+3 in nibbles 1, 5, 3, 7
 //   per group of inputs 64 bytes of 16-bit scales, [8 g][half][row g, row g + 8]
@@ -19,7 +19,7 @@
 // becomes one A fragment with two logic instructions and one exact subtraction per pair (a code c under
 // the exponent of 128 is the bf16 value 128 + c), the group's products go through mma.sync into fp32, and
 // the group's scale multiplies the fp32 sums: nothing is rounded before the result. The inputs' order
-// inside a block of 32 is the same permutation on both sides, which is why no shuffle is needed.
+// inside 16 is the same permutation on both sides, which is why no shuffle is needed.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -58,9 +58,9 @@ constexpr int w4_threads() { return w4_warps<NT>() * 32; }
 template <int NT, int G, bool Z>
 constexpr int w4_run_bytes() { return w4_warps<NT>() * (W4Record<G, Z>::kRing + NT * 1024 + kW4Slots * 8) + 16; }
 
-// bytes between the rows of the activations in shared memory: 64 more than a whole number of 128, so
-// that the eight 16-byte reads of a quarter warp (two rows, four columns) fall into different banks
-__host__ __device__ inline int w4_pitch(int inputs) { return inputs * 2 + 64; }
+// bytes between the rows of the activations in shared memory: 32 more than a whole number of 128, so
+// that the sixteen 8-byte reads of a half warp (four rows, four columns) fall into different banks
+__host__ __device__ inline int w4_pitch(int inputs) { return inputs * 2 + 32; }
 
 MSGL_DEVICE uint4 lds128(uint32_t a) {
   uint4 v;
@@ -232,7 +232,7 @@ struct W4Runs {
     uint32_t xrow[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-      xrow[nt] = smem_u32(xs) + (uint32_t)(min(nt * 8 + g, nx - 1) * pitch + t * 16);
+      xrow[nt] = smem_u32(xs) + (uint32_t)(min(nt * 8 + g, nx - 1) * pitch + t * 8);
     const uint32_t mine = lane * 16, side = R::kScales + g * 8, zside = R::kZeros + g * 4;
     float acc[2][NT][4];
     for (int i = a; i < b;) {
@@ -285,11 +285,11 @@ struct W4Runs {
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint4 xv = lds128(xrow[nt] + xoff + quarter * 64);
+            const uint2 x0 = lds64(xrow[nt] + xoff + quarter * 64), x1 = lds64(xrow[nt] + xoff + quarter * 64 + 32);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              mma_bf16_16816(tmp[h][nt], fr[h][0], xv.x, xv.y, quarter % per == 0);
-              mma_bf16_16816(tmp[h][nt], fr[h][1], xv.z, xv.w, false);
+              mma_bf16_16816(tmp[h][nt], fr[h][0], x0.x, x0.y, quarter % per == 0);
+              mma_bf16_16816(tmp[h][nt], fr[h][1], x1.x, x1.y, false);
             }
           }
           if (quarter % per == per - 1) {

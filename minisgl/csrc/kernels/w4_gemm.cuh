@@ -1,6 +1,6 @@
 // 4-bit products for many tokens, on the 5th-generation tensor core (layout of the weights in w4.cuh).
 //
-// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 256 tokens (their N, a multiple of 16
+// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 192 tokens (their N, a multiple of 16
 // that follows the number of tokens), 64 inputs per step. Roles of a CTA's 26 warps, one CTA per SM,
 // persistent over tiles:
 //   warps 0-3    epilogue, one TMEM lane quadrant each
@@ -8,9 +8,11 @@
 //                one per 16 rows (down), or gathered by token with cp.async (gate_up)
 //   warp 8       bulk copies of the tile's records of 128 inputs (two steps) into a ring of their own
 //   warp 9       MMA issuer: D_h[128 x N] += A_h[128 x 64] B[N x 64]^T, fp32 in TMEM, two sets if they fit
-//   warps 10-25  records -> bf16 A tiles: the codes become bf16 as in w4.cuh, times the group's scale. Half of
-//                them take the even steps, half the odd ones: one half converts while the other waits for
-//                its barriers and its stores' fence.
+//   warps 10-25  records -> bf16 A tiles in tensor memory: the codes become bf16 as in w4.cuh, times the group's
+//                scale. Half of them take the even steps, half the odd ones: one half converts while the other
+//                waits for its barriers and its stores.
+// A comes from tensor memory because shared memory's 128 bytes a clock were the limit with A tiles there
+// (200 tokens: 143 KB a step, of which A written and read 64): 72 us at 200 x 34816 x 5120.
 // Rounding (code - zero) * scale to bf16 is a choice: an fp32 scale applied to the sums would need the
 // accumulator to be read back once per group. It adds half a step of bf16 per weight, independent from
 // weight to weight, about what the result's own rounding does.
@@ -43,14 +45,16 @@ struct W4GemmArgs {
   const int4* work;
   const int* sorted;
   int topk, act;
-  int stages, slots, raw_bytes;  // rings: operand tiles, records of two steps
+  int sets, half_cols;           // accumulators: sets of H x half_cols columns
+  int stages, b_stages, slots, raw_bytes;  // rings: A, tokens' rows, records of two steps
+  int ring_bytes;                // all of them, or the fp32 tile if that is larger
 };
 
 constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
 constexpr int kGwMaxSlots = 8, kGwMaxStages = 4;
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
-__host__ __device__ constexpr int w4_gemm_stage(int h, int bn) { return h * 128 * 128 + bn * 128; }
+constexpr int kGwMaxTokens = 192;    // of a tile: two stages of A then fit beside the accumulators
 
 MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
   if (act == 0) return g / (1.f + __expf(-g)) * u;
@@ -68,8 +72,14 @@ MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-MSGL_DEVICE void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+// 16 lanes x 32 columns of tensor memory from the warp's registers: r[4i], r[4i + 1] are columns 8i + 2t,
+// 8i + 2t + 1 of lane g, r[4i + 2], r[4i + 3] those of lane g + 8 (thread 4 g + t)
+MSGL_DEVICE void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 // a role's wait: true once the phase is complete, false if it never is
@@ -83,16 +93,16 @@ template <int MODE, int H, bool SPLIT, bool Z, bool F>
 __global__ void __launch_bounds__(kGwThreads, 1)
 w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUtensorMap rows_map) {
   static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
-  constexpr int kRecs = 4 * H, kA = H * 128 * 128;
+  constexpr int kRecs = 4 * H;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int S = p.stages, stage_bytes = w4_gemm_stage(H, p.bn);
-  uint8_t* raw = smem + S * stage_bytes;
-  int* rows = reinterpret_cast<int*>(raw + p.slots * p.raw_bytes);
+  const int S = p.stages, SB = p.b_stages, stage_bytes = p.bn * 128;
+  uint8_t* raw = smem + SB * stage_bytes;
+  int* rows = reinterpret_cast<int*>(smem + p.ring_bytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(rows + 256);
   uint64_t *raw_full = bars, *raw_empty = bars + kGwMaxSlots, *a_full = raw_empty + kGwMaxSlots,
-           *b_full = a_full + kGwMaxStages, *ab_empty = b_full + kGwMaxStages, *tfull = ab_empty + kGwMaxStages,
-           *tempty = tfull + 2;
+           *a_empty = a_full + kGwMaxStages, *b_full = a_empty + kGwMaxStages, *b_empty = b_full + kGwMaxStages,
+           *tfull = b_empty + kGwMaxStages, *tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = SPLIT ? (int)cluster_ctarank() : 0;
@@ -104,8 +114,11 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     }
     for (int i = 0; i < S; ++i) {
       mbar_init(&a_full[i], kGwConv / 2);
+      mbar_init(&a_empty[i], 1);
+    }
+    for (int i = 0; i < SB; ++i) {
       mbar_init(&b_full[i], MODE == kW4GateUp ? kGwLoad : 1);
-      mbar_init(&ab_empty[i], 1);
+      mbar_init(&b_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
@@ -114,11 +127,10 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     fence_barrier_init();
     if constexpr (MODE != kW4GateUp) prefetch_tmap(&rows_map);
   }
-  // accumulators: H x half_cols columns a set, two sets if TMEM's 512 columns hold them
-  const int half_cols = p.bn <= 32 ? 32 : p.bn <= 64 ? 64 : p.bn <= 128 ? 128 : 256;
-  const int sets = 2 * H * half_cols <= 512 ? 2 : 1, tmem_cols = sets * H * half_cols;
+  // tensor memory: accumulators from column 0, A stages of H x 32 columns at the end
+  const int sets = p.sets, half_cols = p.half_cols;
   if (warp == 9) {
-    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   pdl_launch();
@@ -126,7 +138,10 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // all of tensor memory was allocated, so it begins at column 0
+  constexpr uint32_t tmem = 0;
+  const uint32_t tmem_a = 512 - S * H * 32;
+  if (*tmem_slot != 0 && threadIdx.x == 0) report_error(kErrBounds, 420);
 
   const int units = p.n_tiles * (MODE == kW4Dense ? p.m_tiles : *p.count);
   const int u_first = SPLIT ? blockIdx.x / p.splits : blockIdx.x, u_step = SPLIT ? units : gridDim.x;
@@ -233,8 +248,8 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         for (int u = u_first; u < units && ok; u += u_step) {
           const Tile tl = tile_of(u);
           for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-            if (!(ok = w4_await<100>(&ab_empty[stage], phase ^ 1))) break;
-            uint8_t* dst = smem + stage * stage_bytes + kA;
+            if (!(ok = w4_await<100>(&b_empty[stage], phase ^ 1))) break;
+            uint8_t* dst = smem + stage * stage_bytes;
             // rows beyond the last one and inputs beyond the last one arrive as zeros, and count
             if constexpr (MODE == kW4Dense) {
               mbar_expect_tx(&b_full[stage], p.bn * 128);
@@ -243,7 +258,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
               mbar_expect_tx(&b_full[stage], tl.cols * 128);
               for (int r = 0; r < tl.cols; r += 16) tma_load_2d(dst + r * 128, &rows_map, &b_full[stage], ks * 64, tl.row0 + r);
             }
-            if (++stage == S) stage = 0, phase ^= 1;
+            if (++stage == SB) stage = 0, phase ^= 1;
           }
         }
       }
@@ -263,9 +278,9 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         for (int r = lt; r < tl.cols; r += kGwLoad * 32) rows[r] = p.sorted[tl.row0 + min(r, tl.n - 1)] / p.topk;
         named_bar_sync(1, kGwLoad * 32);
         for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-          if (!(ok = w4_await<100>(&ab_empty[stage], phase ^ 1))) break;
+          if (!(ok = w4_await<100>(&b_empty[stage], phase ^ 1))) break;
           // a thread's rows are 16 apart, so their swizzle is the same
-          uint32_t dst = smem_u32(smem) + stage * stage_bytes + kA + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+          uint32_t dst = smem_u32(smem) + stage * stage_bytes + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
           const int k = ks * 64 + chunk * 8;
           const uint32_t bytes = k < p.w.k ? 16 : 0;  // zeros beyond the last input
           const __nv_bfloat16* src = p.in + min(k, p.w.k - 8);
@@ -279,7 +294,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             announce();
           }
           before = stage;
-          if (++stage == S) stage = 0, phase ^= 1;
+          if (++stage == SB) stage = 0, phase ^= 1;
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -306,46 +321,49 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA
-    if (lane == 0) {
-      int stage = 0, use = 0;
-      uint32_t phase = 0;
-      for (int u = u_first; u < units && ok; u += u_step, ++use) {
-        const Tile tl = tile_of(u);
-        const uint32_t idesc = idesc_bf16_f32(128, tl.cols), d = tmem + set_of(use) * H * half_cols;
-        if (!(ok = w4_await<20>(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
+    // the whole warp runs the loop, so that the descriptors stay in uniform registers; one lane issues
+    int stage = 0, bstage = 0, use = 0;
+    uint32_t phase = 0, bphase = 0;
+    for (int u = u_first; u < units && ok; u += u_step, ++use) {
+      const Tile tl = tile_of(u);
+      const uint32_t idesc = idesc_bf16_f32(128, tl.cols), d = set_of(use) * H * half_cols;
+      if (!(ok = w4_await<20>(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
+      tc_fence_after();
+      for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
+        if (!(ok = w4_await<0>(&b_full[bstage], bphase) && w4_await<0>(&a_full[stage], phase))) break;
         tc_fence_after();
-        for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-          if (!(ok = w4_await<0>(&b_full[stage], phase) && w4_await<0>(&a_full[stage], phase))) break;
-          tc_fence_after();
-          const uint64_t a = smem_desc_sw128(smem_u32(smem) + stage * stage_bytes), b = a + (kA >> 4);
+        const uint64_t b = smem_desc_sw128(smem_u32(smem) + bstage * stage_bytes);
+        const uint32_t a = 512 - (S - stage) * H * 32;
+        if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int h = 0; h < H; ++h)
-              tc_mma_f16(d + h * half_cols, a + (h * (128 * 128) + j * 32) / 16, b + j * 2, idesc, ks > 2 * k0 || j > 0);
-          tc_commit(&ab_empty[stage]);
-          if (++stage == S) stage = 0, phase ^= 1;
+              tc_mma_f16_ts(d + h * half_cols, a + h * 32 + j * 8, b + j * 2, idesc, ks > 2 * k0 || j > 0);
+          tc_commit(&a_empty[stage]);
+          tc_commit(&b_empty[bstage]);
         }
-        tc_commit(&tfull[set_of(use)]);
+        __syncwarp();
+        if (++stage == S) stage = 0, phase ^= 1;
+        if (++bstage == SB) bstage = 0, bphase ^= 1;
       }
+      if (elect_one()) tc_commit(&tfull[set_of(use)]);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------------ records -> A tile
-    // a warp's part of a step: 64 inputs of 16 H rows of a record (H = 1: two warps share a record)
-    const int cw = warp - kGwEpi - kGwLoad - 2, block = cw & 1, m = cw >> 1;
-    const int ti = H == 2 ? m : m >> 1, g = lane >> 2, t = lane & 3;
+    // A warp's part of a step: 64 inputs of 16 H rows of a record (H = 1: two warps share a record). It writes
+    // the 32 lanes that its number modulo 4 gives it: records go to the rows of the tile in their order, or
+    // (gated) their gate rows to one half of the tile and their up rows to the other, 16 lanes each.
+    const int cw = warp - kGwEpi - kGwLoad - 2, quad = warp & 3, other = cw >> 2;  // four warps of each quadrant
+    const int block = other & 1, m = other >> 1;
+    const int ti = MODE == kW4GateUp ? quad * 2 + m : H == 2 ? quad + 4 * m : quad;
+    const int g = lane >> 2, t = lane & 3;
     const int bytes = p.raw_bytes / kRecs;
     const int shift = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;  // quarters of a record per group
     const int zoff = W4Record<128, false>::kScales + 128 / p.group * 64;
-    const uint32_t raw0 = smem_u32(raw), ops0 = smem_u32(smem);
-    // rows g (and g + 8, kRowB behind) of a record's half in the A tile: as in the records, or (gated) gate rows
-    // in one half of the tile and up rows in the other
-    constexpr uint32_t kRowB = MODE == kW4GateUp ? 128 * 128 : 8 * 128;
-    const uint32_t row0 = (MODE == kW4GateUp ? ti * 16 + g : ti * 32 + g) * 128;
-    // neighbouring rows start with different halves of their 128 bytes: the stores of a quarter warp (two
-    // rows, four chunks) then fall into different banks
-    const uint32_t at0 = ((4 * (g & 1) + t) ^ g) << 4, at1 = ((4 * (~g & 1) + t) ^ g) << 4;
+    const uint32_t raw0 = smem_u32(raw);
+    const uint32_t lanes = (uint32_t)(quad * 32 + (MODE == kW4GateUp ? m * 16 : 0)) << 16;
     int stage = block, slot = 0;
     uint32_t phase = 0, rphase = 0;
     for (int u = u_first; u < units && ok; u += u_step) {
@@ -354,14 +372,15 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       for (int kb = k0; kb < k1; ++kb) {
         if (!(ok = w4_await<20>(&raw_full[slot], rphase))) break;
         const uint32_t rec = raw0 + slot * p.raw_bytes + ti * bytes;
-        uint2 q[H][2] = {}, s[2] = {};
+        uint4 q[H] = {};
+        uint2 s[2] = {};
         uint32_t z[2] = {0x08080808u, 0x08080808u};
         if (there) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int h = (e ^ g) & 1, grp = (2 * block + h) >> shift;
+          for (int i = 0; i < H; ++i) q[i] = lds128(rec + ((H == 2 ? i : m) * 2 + block) * 512 + lane * 16);
 #pragma unroll
-            for (int i = 0; i < H; ++i) q[i][e] = lds64(rec + ((H == 2 ? i : m & 1) * 2 + block) * 512 + lane * 16 + h * 8);
+          for (int e = 0; e < 2; ++e) {
+            const int grp = (2 * block + e) >> shift;
             s[e] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
             if constexpr (Z) z[e] = lds32(rec + zoff + grp * 32 + g * 4);
           }
@@ -369,30 +388,45 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[slot]);
         if (++slot == p.slots) slot = 0, rphase ^= 1;
-        if (!(ok = w4_await<50>(&ab_empty[stage], phase ^ 1))) break;
-        if (there) {
+        // the bf16 values: [row g, row g + 8 of a half][word][pair of inputs]
+        uint32_t v[H][2][4][2];
 #pragma unroll
-          for (int i = 0; i < H; ++i) {
-            const int half = H == 2 ? i : m & 1;
-            const uint32_t a = ops0 + stage * stage_bytes + row0 + half * (MODE == kW4GateUp ? 8 * 128 : 16 * 128);
+        for (int i = 0; i < H; ++i) {
+          const int half = H == 2 ? i : m;
+          const uint32_t words[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t w0 = q[i][e].x, w1 = q[i][e].y, sv = half ? s[e].y : s[e].x, zv = z[e] >> (16 * half);
-              const uint32_t z0 = Z ? 0x43004300u + (zv & 15u) * 0x10001u : 0x43084308u;
-              const uint32_t z1 = Z ? 0x43004300u + ((zv >> 8) & 15u) * 0x10001u : 0x43084308u;
-              const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
-              float2 sf = make_float2(0.f, 0.f);
-              if constexpr (F) sf = w4_scales<true>(sv);
-              const uint32_t at = a + (e ? at1 : at0);
-              sts128(at, w4_times<F>(codes_bf16x2(w0, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w0 >> 8, z0), sa2, sf.x),
-                     w4_times<F>(codes_bf16x2(w1, z0), sa2, sf.x), w4_times<F>(codes_bf16x2(w1 >> 8, z0), sa2, sf.x));
-              sts128(at + kRowB, w4_times<F>(codes_bf16x2(w0 >> 4, z1), sb2, sf.y),
-                     w4_times<F>(codes_bf16x2(w0 >> 12, z1), sb2, sf.y), w4_times<F>(codes_bf16x2(w1 >> 4, z1), sb2, sf.y),
-                     w4_times<F>(codes_bf16x2(w1 >> 12, z1), sb2, sf.y));
-            }
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t sv = half ? s[b >> 1].y : s[b >> 1].x, zv = z[b >> 1] >> (16 * half);
+            const uint32_t z0 = Z ? 0x43004300u + (zv & 15u) * 0x10001u : 0x43084308u;
+            const uint32_t z1 = Z ? 0x43004300u + ((zv >> 8) & 15u) * 0x10001u : 0x43084308u;
+            const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
+            float2 sf = make_float2(0.f, 0.f);
+            if constexpr (F) sf = w4_scales<true>(sv);
+            v[i][0][b][0] = w4_times<F>(codes_bf16x2(words[b], z0), sa2, sf.x);
+            v[i][1][b][0] = w4_times<F>(codes_bf16x2(words[b] >> 4, z1), sb2, sf.y);
+            v[i][0][b][1] = w4_times<F>(codes_bf16x2(words[b] >> 8, z0), sa2, sf.x);
+            v[i][1][b][1] = w4_times<F>(codes_bf16x2(words[b] >> 12, z1), sb2, sf.y);
           }
         }
-        fence_async_smem();
+        if (!(ok = w4_await<50>(&a_empty[stage], phase ^ 1))) break;
+        tc_fence_after();
+        const uint32_t dst = tmem_a + lanes + stage * H * 32;
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          uint32_t r[16];
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              // gated: the gate rows (i = 0) or up rows (i = 1) of both halves
+              r[4 * b + c] = MODE == kW4GateUp ? v[0][i][b][c] : v[i][0][b][c];
+              r[4 * b + 2 + c] = MODE == kW4GateUp ? v[H - 1][i][b][c] : v[i][1][b][c];
+            }
+          if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x4(dst + i * 32, r);
+          else tmem_st_16x256b_x4(dst + (H == 2 ? m * 32 : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r);
+        }
+        tc_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&a_full[stage]);
         stage += 2;  // the other half takes the step between; there are at least two stages
@@ -433,7 +467,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -465,18 +499,25 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, Z, F>;
   constexpr int kMax = 227 * 1024;
   if (msgl_set_smem<kernel>(kMax) != cudaSuccess) return 4;
-  // Records of two pairs of steps at least (a copy takes about 1 us), two to four operand stages, then the
-  // rest for records again. With `splits` the rings also hold the fp32 tile.
+  // Tensor memory's 512 columns: two sets of accumulators if three stages of A fit beside them, else one and
+  // up to four stages. Shared memory: the tokens' stages, and up to eight steps' records (a copy takes about
+  // 1 us).
+  p.half_cols = (p.bn + 31) / 32 * 32;
+  p.sets = 512 - 2 * H * p.half_cols >= 3 * H * 32 ? 2 : 1;
+  p.stages = std::min(kGwMaxStages, (512 - p.sets * H * p.half_cols) / (H * 32));
+  if (p.stages < 2) return 3;
   p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
-  const int room = kMax - 1024 - kGwMisc, stage = w4_gemm_stage(H, p.bn);
-  p.stages = std::max(2, std::min(kGwMaxStages, (room - 2 * p.raw_bytes) / stage));
-  p.slots = std::min(kGwMaxSlots, (room - p.stages * stage) / p.raw_bytes);
-  if (SPLIT && p.bn * H * 512 > p.stages * stage + p.slots * p.raw_bytes) return 3;
+  const int room = kMax - 1024 - kGwMisc, stage = p.bn * 128;
+  p.b_stages = kGwMaxStages;
+  p.slots = std::min(kGwMaxSlots, (room - p.b_stages * stage) / p.raw_bytes);
+  p.ring_bytes = p.b_stages * stage + p.slots * p.raw_bytes;
+  if (SPLIT) p.ring_bytes = std::max(p.ring_bytes, p.bn * H * 512);
+  if (p.ring_bytes > room) return 3;
   CUtensorMap map = {};
   if (MODE != kW4GateUp &&
       !w4_rows_map(&map, p.in, p.M, p.w.k, p.M == 1 ? (int64_t)p.w.k : p.in_stride, MODE == kW4Dense ? p.bn : 16))
     return 2;
-  const int smem = 1024 + kGwMisc + p.stages * stage + p.slots * p.raw_bytes;
+  const int smem = 1024 + kGwMisc + p.ring_bytes;
   return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
 }
 

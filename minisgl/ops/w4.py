@@ -106,11 +106,11 @@ class W4Weight:
             return t.unflatten(-1, (kc, cols))
 
         data = torch.empty(E, nt, kc, 2048 + per * (64 if zeros is None else 96), dtype=torch.uint8, device=q.device)
-        # bytes of a row by (block, h, lane column t, word j, byte i): codes 2i (low) and 2i + 1
-        b = tiles(q, 64).unflatten(-1, (2, 2, 4, 2, 2))
-        lo, hi = b[:, :, :, 0], b[:, :, :, 1]  # rows g, rows g + 8: [E, Nt, half, 8, KC, 2, 2, 4, 2, 2]
-        perm = (0, 1, 4, 2, 5, 3, 7, 6, 8, 9)  # -> [E, Nt, KC, half, block, g, t, h, j, i]
-        out = data[..., :2048].unflatten(-1, (2, 2, 8, 4, 2, 2, 2, 2))
+        # bytes of a row by (block, word, lane column t, byte i): codes 2i (low) and 2i + 1
+        b = tiles(q, 64).unflatten(-1, (2, 4, 4, 2))
+        lo, hi = b[:, :, :, 0], b[:, :, :, 1]  # rows g, rows g + 8: [E, Nt, half, 8, KC, block, word, t, i]
+        perm = (0, 1, 4, 2, 5, 3, 7, 6, 8)  # -> [E, Nt, KC, half, block, g, t, word, i]
+        out = data[..., :2048].unflatten(-1, (2, 2, 8, 4, 4, 2, 2))
         out[..., 0, :] = ((lo & 15) | (hi << 4)).permute(perm)
         out[..., 1, :] = ((lo >> 4) | (hi & 0xF0)).permute(perm)
         side = lambda t: tiles(t, per).permute(0, 1, 5, 6, 4, 2, 3).reshape(E, nt, kc, per * 32)  # noqa: E731
@@ -131,8 +131,8 @@ class W4Weight:
                 return t.permute(0, 3, 1, 2, 4, 5).flatten(2, 4)[:, :, : self.n // 2].flatten(1, 2).contiguous()
             return t.flatten(1, 4)[:, : self.n].contiguous()
 
-        c = self.data[..., :2048].unflatten(-1, (2, 2, 8, 4, 2, 2, 2, 2))  # [E, Nt, KC, half, block, g, t, h, j, c, i]
-        c = c.permute(0, 1, 3, 5, 2, 4, 7, 6, 8, 9, 10)  # [E, Nt, half, g, KC, block, h, t, j, c, i]
+        c = self.data[..., :2048].unflatten(-1, (2, 2, 8, 4, 4, 2, 2))  # [E, Nt, KC, half, block, g, t, word, c, i]
+        c = c.permute(0, 1, 3, 5, 2, 4, 7, 6, 8, 9)  # [E, Nt, half, g, KC, block, word, t, c, i]
         even, odd = c[..., 0, :], c[..., 1, :]
         q = torch.stack([(even & 15) | ((odd & 15) << 4), (even >> 4) | (odd & 0xF0)], dim=3)
         side = lambda t: rows(t.view(E, nt, kc, per, 8, 2, 2).permute(0, 1, 5, 6, 4, 2, 3), self.k // self.group)  # noqa: E731

@@ -47,7 +47,7 @@ def test_pack_keeps_the_weights(shape, zeros, gated):
 def test_pack_layout():
     """The documented place of one code: tile, block, lane, word and nibble."""
     q = torch.zeros(64, 128, dtype=torch.uint8)
-    row, k = 59, 239  # tile 1, half 1, row 11 = g 3 of its upper 8; record 1, block 1, h 1, t 1, j 1, last code
+    row, k = 59, 239  # tile 1, half 1, row 11 = g 3 of its upper 8; record 1, block 1, word 2, t 3, last code
     q[row, k // 2] = 0xD0
     s = torch.zeros(64, 8, dtype=torch.bfloat16)
     s[row, k // 32] = 1.0
@@ -57,8 +57,8 @@ def test_pack_layout():
     assert w.data.shape == (1, 2, 2, 2048 + 4 * 96) and w.data.count_nonzero() == 4  # 0xD, 1.0 = 0x3F80, 5
     rec = w.data[0, 1, 1]
     words = rec[:2048].view(torch.int32).view(2, 2, 32, 4)
-    g, t, h, j, nibble = 3, 1, 1, 1, 7
-    assert (int(words[1, 1, 4 * g + t, 2 * h + j]) >> (4 * nibble)) & 15 == 0xD
+    g, t, word, nibble = 3, 3, 2, 7
+    assert (int(words[1, 1, 4 * g + t, word]) >> (4 * nibble)) & 15 == 0xD
     assert rec[2048:2304].view(torch.bfloat16).view(4, 8, 2, 2)[3, g, 1, 1] == 1.0
     assert rec[2304:].view(4, 8, 2, 2)[3, g, 1, 1] == 5
 
