@@ -1,6 +1,6 @@
 // 4-bit products for many tokens, on the 5th-generation tensor core (layout of the weights in w4.cuh).
 //
-// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 192 tokens (their N, a multiple of 16
+// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 224 tokens (their N, a multiple of 16
 // that follows the number of tokens), 64 inputs per step. Roles of a CTA's 26 warps, one CTA per SM,
 // persistent over tiles:
 //   warps 0-3    epilogue, one TMEM lane quadrant each
@@ -46,15 +46,15 @@ struct W4GemmArgs {
   const int* sorted;
   int topk, act;
   int sets, half_cols;           // accumulators: sets of H x half_cols columns
-  int stages, b_stages, slots, raw_bytes;  // rings: A, tokens' rows, records of two steps
+  int stages, slots, raw_bytes;  // rings: A, records of two steps
   int ring_bytes;                // all of them, or the fp32 tile if that is larger
 };
 
 constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
-constexpr int kGwMaxSlots = 8, kGwMaxStages = 4;
+constexpr int kGwMaxSlots = 8, kGwMaxA = 8, kGwB = 4;  // most stages of the rings
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
-constexpr int kGwMaxTokens = 192;    // of a tile: two stages of A then fit beside the accumulators
+constexpr int kGwMaxTokens = 224;    // of a tile: two stages of A then fit beside the accumulators
 
 MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
   if (act == 0) return g / (1.f + __expf(-g)) * u;
@@ -72,14 +72,12 @@ MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// 16 lanes x 32 columns of tensor memory from the warp's registers: r[4i], r[4i + 1] are columns 8i + 2t,
+// 16 lanes x 16 columns of tensor memory from the warp's registers: r[4i], r[4i + 1] are columns 8i + 2t,
 // 8i + 2t + 1 of lane g, r[4i + 2], r[4i + 3] those of lane g + 8 (thread 4 g + t)
-MSGL_DEVICE void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+MSGL_DEVICE void tmem_st_16x256b_x2(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // a role's wait: true once the phase is complete, false if it never is
@@ -89,20 +87,23 @@ MSGL_DEVICE bool w4_await(uint64_t* bar, uint32_t parity) {
   return mbar_try_wait_a(a, parity) || w4_wait<NS>(a, parity);
 }
 
-template <int MODE, int H, bool SPLIT, bool Z, bool F>
+template <int MODE, int H, bool SPLIT, bool FINE, bool Z, bool F>
 __global__ void __launch_bounds__(kGwThreads, 1)
 w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUtensorMap rows_map) {
   static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
   constexpr int kRecs = 4 * H;
+  // Columns of a half in a stage of A. FINE: a stage is half a step, so that three fit beside the accumulators of
+  // more than 192 tokens; the MMA warp then waits and commits twice a step, which small tiles would feel.
+  constexpr int kCols = FINE ? 16 : 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int S = p.stages, SB = p.b_stages, stage_bytes = p.bn * 128;
-  uint8_t* raw = smem + SB * stage_bytes;
+  const int S = p.stages, stage_bytes = p.bn * 128;
+  uint8_t* raw = smem + kGwB * stage_bytes;
   int* rows = reinterpret_cast<int*>(smem + p.ring_bytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(rows + 256);
   uint64_t *raw_full = bars, *raw_empty = bars + kGwMaxSlots, *a_full = raw_empty + kGwMaxSlots,
-           *a_empty = a_full + kGwMaxStages, *b_full = a_empty + kGwMaxStages, *b_empty = b_full + kGwMaxStages,
-           *tfull = b_empty + kGwMaxStages, *tempty = tfull + 2;
+           *a_empty = a_full + kGwMaxA, *b_full = a_empty + kGwMaxA, *b_empty = b_full + kGwB, *tfull = b_empty + kGwB,
+           *tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = SPLIT ? (int)cluster_ctarank() : 0;
@@ -116,7 +117,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       mbar_init(&a_full[i], kGwConv / 2);
       mbar_init(&a_empty[i], 1);
     }
-    for (int i = 0; i < SB; ++i) {
+    for (int i = 0; i < kGwB; ++i) {
       mbar_init(&b_full[i], MODE == kW4GateUp ? kGwLoad : 1);
       mbar_init(&b_empty[i], 1);
     }
@@ -127,7 +128,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     fence_barrier_init();
     if constexpr (MODE != kW4GateUp) prefetch_tmap(&rows_map);
   }
-  // tensor memory: accumulators from column 0, A stages of H x 32 columns at the end
+  // tensor memory: accumulators from column 0, A stages of H x kCols columns at the end
   const int sets = p.sets, half_cols = p.half_cols;
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
@@ -140,7 +141,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
   tc_fence_after();
   // all of tensor memory was allocated, so it begins at column 0
   constexpr uint32_t tmem = 0;
-  const uint32_t tmem_a = 512 - S * H * 32;
+  const uint32_t tmem_a = 512 - S * H * kCols;
   if (*tmem_slot != 0 && threadIdx.x == 0) report_error(kErrBounds, 420);
 
   const int units = p.n_tiles * (MODE == kW4Dense ? p.m_tiles : *p.count);
@@ -258,7 +259,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
               mbar_expect_tx(&b_full[stage], tl.cols * 128);
               for (int r = 0; r < tl.cols; r += 16) tma_load_2d(dst + r * 128, &rows_map, &b_full[stage], ks * 64, tl.row0 + r);
             }
-            if (++stage == SB) stage = 0, phase ^= 1;
+            if (++stage == kGwB) stage = 0, phase ^= 1;
           }
         }
       }
@@ -294,7 +295,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             announce();
           }
           before = stage;
-          if (++stage == SB) stage = 0, phase ^= 1;
+          if (++stage == kGwB) stage = 0, phase ^= 1;
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -303,20 +304,24 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
   } else if (warp == 8) {
     // ------------------------------------------------------------------ records
     const int bytes = p.raw_bytes / kRecs;
-    if (lane == 0) {
-      int slot = 0;
-      uint32_t phase = 0;
-      for (int u = u_first; u < units && ok; u += u_step) {
-        const Tile tl = tile_of(u);
-        const int n = min(kRecs, p.w.tiles - tl.nt * kRecs);
-        const uint8_t* src = p.w.data + ((int64_t)tl.e * p.w.tiles + tl.nt * kRecs) * p.w.kc * bytes;
-        for (int kb = k0; kb < k1; ++kb) {
-          if (!(ok = w4_await<200>(&raw_empty[slot], phase ^ 1))) break;
-          mbar_expect_tx(&raw_full[slot], n * bytes);
-          for (int i = 0; i < n; ++i)
-            bulk_load(raw + slot * p.raw_bytes + i * bytes, src + ((int64_t)i * p.w.kc + kb) * bytes, bytes, &raw_full[slot]);
-          if (++slot == p.slots) slot = 0, phase ^= 1;
+    const uint32_t raw0 = smem_u32(raw), full0 = smem_u32(raw_full);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int u = u_first; u < units && ok; u += u_step) {
+      const Tile tl = tile_of(u);
+      const int n = min(kRecs, p.w.tiles - tl.nt * kRecs);
+      const uint8_t* src = p.w.data + (((int64_t)tl.e * p.w.tiles + tl.nt * kRecs) * p.w.kc + k0) * bytes;
+      for (int kb = k0; kb < k1; ++kb, src += bytes) {
+        if (!(ok = w4_await<100>(&raw_empty[slot], phase ^ 1))) break;
+        if (elect_one()) {
+          mbar_expect_tx_a(full0 + slot * 8, n * bytes);
+#pragma unroll
+          for (int i = 0; i < kRecs; ++i)
+            if (i < n)
+              bulk_load_a(raw0 + slot * p.raw_bytes + i * bytes, src + (int64_t)i * p.w.kc * bytes, bytes, full0 + slot * 8);
         }
+        __syncwarp();
+        if (++slot == p.slots) slot = 0, phase ^= 1;
       }
     }
   } else if (warp == 9) {
@@ -330,22 +335,32 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       if (!(ok = w4_await<20>(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
       tc_fence_after();
       for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-        if (!(ok = w4_await<0>(&b_full[bstage], bphase) && w4_await<0>(&a_full[stage], phase))) break;
-        tc_fence_after();
+        if (!(ok = w4_await<0>(&b_full[bstage], bphase))) break;
         const uint64_t b = smem_desc_sw128(smem_u32(smem) + bstage * stage_bytes);
-        const uint32_t a = 512 - (S - stage) * H * 32;
-        if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+        for (int e = 0; e < 2; ++e) {
+          if (FINE || e == 0) {
+            if (ok) ok = w4_await<0>(&a_full[stage], phase);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          const uint32_t a = 512 - (S - stage) * H * kCols;
+          if (elect_one()) {
 #pragma unroll
-            for (int h = 0; h < H; ++h)
-              tc_mma_f16_ts(d + h * half_cols, a + h * 32 + j * 8, b + j * 2, idesc, ks > 2 * k0 || j > 0);
-          tc_commit(&a_empty[stage]);
-          tc_commit(&b_empty[bstage]);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int h = 0; h < H; ++h)
+                tc_mma_f16_ts(d + h * half_cols, a + h * kCols + (FINE ? 0 : e * 16) + j * 8, b + e * 4 + j * 2, idesc,
+                              ks > 2 * k0 || e > 0 || j > 0);
+            if (FINE || e == 1) tc_commit(&a_empty[stage]);
+            if (e == 1) tc_commit(&b_empty[bstage]);
+          }
+          __syncwarp();
+          if (FINE || e == 1)
+            if (++stage == S) stage = 0, phase ^= 1;
         }
-        __syncwarp();
-        if (++stage == S) stage = 0, phase ^= 1;
-        if (++bstage == SB) bstage = 0, bphase ^= 1;
+        if (!ok) break;
+        if (++bstage == kGwB) bstage = 0, bphase ^= 1;
       }
       if (elect_one()) tc_commit(&tfull[set_of(use)]);
       __syncwarp();
@@ -364,8 +379,13 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     const int zoff = W4Record<128, false>::kScales + 128 / p.group * 64;
     const uint32_t raw0 = smem_u32(raw);
     const uint32_t lanes = (uint32_t)(quad * 32 + (MODE == kW4GateUp ? m * 16 : 0)) << 16;
-    int stage = block, slot = 0;
+    int stage = 0, slot = 0;  // stage of the step of both halves that comes next
     uint32_t phase = 0, rphase = 0;
+    const auto advance = [&](int n) {
+      for (stage += n; stage >= S; stage -= S) phase ^= 1;
+    };
+    constexpr int kStages = FINE ? 2 : 1;  // of a step
+    if (block == 1) advance(kStages);
     for (int u = u_first; u < units && ok; u += u_step) {
       const Tile tl = tile_of(u);
       const bool there = tl.nt * kRecs + ti < p.w.tiles;
@@ -408,29 +428,38 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             v[i][1][b][1] = w4_times<F>(codes_bf16x2(words[b] >> 12, z1), sb2, sf.y);
           }
         }
-        if (!(ok = w4_await<50>(&a_empty[stage], phase ^ 1))) break;
-        tc_fence_after();
-        const uint32_t dst = tmem_a + lanes + stage * H * 32;
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          uint32_t r[16];
+        for (int e = 0; e < 2; ++e) {  // 32 inputs
+          if (FINE || e == 0) {
+            if (ok) ok = w4_await<50>(&a_empty[stage], phase ^ 1);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          const uint32_t dst = tmem_a + lanes + stage * H * kCols + (FINE ? 0 : e * 16);
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+          for (int i = 0; i < H; ++i) {
+            uint32_t r[8];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              // gated: the gate rows (i = 0) or up rows (i = 1) of both halves
-              r[4 * b + c] = MODE == kW4GateUp ? v[0][i][b][c] : v[i][0][b][c];
-              r[4 * b + 2 + c] = MODE == kW4GateUp ? v[H - 1][i][b][c] : v[i][1][b][c];
-            }
-          if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x4(dst + i * 32, r);
-          else tmem_st_16x256b_x4(dst + (H == 2 ? m * 32 : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r);
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                // gated: the gate rows (i = 0) or up rows (i = 1) of both halves
+                r[4 * b + c] = MODE == kW4GateUp ? v[0][i][2 * e + b][c] : v[i][0][2 * e + b][c];
+                r[4 * b + 2 + c] = MODE == kW4GateUp ? v[H - 1][i][2 * e + b][c] : v[i][1][2 * e + b][c];
+              }
+            if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x2(dst + i * kCols, r);
+            else tmem_st_16x256b_x2(dst + (H == 2 ? m * kCols : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r);
+          }
+          if (FINE || e == 1) {
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[stage]);
+            advance(1);
+          }
         }
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[stage]);
-        stage += 2;  // the other half takes the step between; there are at least two stages
-        if (stage >= S) stage -= S, phase ^= 1;
+        if (!ok) break;
+        advance(kStages);  // the other warps' step
       }
     }
   }
@@ -494,23 +523,23 @@ inline bool w4_rows_map(CUtensorMap* m, const void* base, int64_t rows, int64_t 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE, int H, bool SPLIT, bool Z, bool F>
+template <int MODE, int H, bool SPLIT, bool FINE, bool Z, bool F>
 int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
-  constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, Z, F>;
+  constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, FINE, Z, F>;
   constexpr int kMax = 227 * 1024;
   if (msgl_set_smem<kernel>(kMax) != cudaSuccess) return 4;
-  // Tensor memory's 512 columns: two sets of accumulators if three stages of A fit beside them, else one and
-  // up to four stages. Shared memory: the tokens' stages, and up to eight steps' records (a copy takes about
-  // 1 us).
-  p.half_cols = (p.bn + 31) / 32 * 32;
-  p.sets = 512 - 2 * H * p.half_cols >= 3 * H * 32 ? 2 : 1;
-  p.stages = std::min(kGwMaxStages, (512 - p.sets * H * p.half_cols) / (H * 32));
+  // Tensor memory's 512 columns: two sets of accumulators if two steps of A fit beside them, else one and up to
+  // eight stages. Shared memory: four stages of the tokens' rows, and up to eight steps' records (a copy
+  // takes about 1 us).
+  constexpr int kA = H * (FINE ? 16 : 32);
+  p.half_cols = p.bn;
+  p.sets = 512 - 2 * H * p.half_cols >= 2 * H * 32 ? 2 : 1;
+  p.stages = std::min(kGwMaxA, (512 - p.sets * H * p.half_cols) / kA);
   if (p.stages < 2) return 3;
   p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
   const int room = kMax - 1024 - kGwMisc, stage = p.bn * 128;
-  p.b_stages = kGwMaxStages;
-  p.slots = std::min(kGwMaxSlots, (room - p.b_stages * stage) / p.raw_bytes);
-  p.ring_bytes = p.b_stages * stage + p.slots * p.raw_bytes;
+  p.slots = std::min(kGwMaxSlots, (room - kGwB * stage) / p.raw_bytes);
+  p.ring_bytes = kGwB * stage + p.slots * p.raw_bytes;
   if (SPLIT) p.ring_bytes = std::max(p.ring_bytes, p.bn * H * 512);
   if (p.ring_bytes > room) return 3;
   CUtensorMap map = {};
@@ -521,13 +550,21 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
 }
 
+template <int MODE, int H, bool SPLIT, bool FINE>
+int w4_gemm_launch_form(const W4GemmArgs& p, int grid, cudaStream_t s) {
+  if (p.zeros)
+    return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, FINE, true, true>(p, grid, s)
+                  : w4_gemm_launch_as<MODE, H, SPLIT, FINE, true, false>(p, grid, s);
+  return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, FINE, false, true>(p, grid, s)
+                : w4_gemm_launch_as<MODE, H, SPLIT, FINE, false, false>(p, grid, s);
+}
+
 template <int MODE, int H, bool SPLIT>
 int w4_gemm_launch(const W4GemmArgs& p, int grid, cudaStream_t s) {
-  if (p.zeros)
-    return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, true, true>(p, grid, s)
-                  : w4_gemm_launch_as<MODE, H, SPLIT, true, false>(p, grid, s);
-  return p.fp16 ? w4_gemm_launch_as<MODE, H, SPLIT, false, true>(p, grid, s)
-                : w4_gemm_launch_as<MODE, H, SPLIT, false, false>(p, grid, s);
+  if constexpr (MODE == kW4Dense && H == 2) {
+    if (p.bn > 192) return w4_gemm_launch_form<MODE, H, SPLIT, true>(p, grid, s);
+  }
+  return w4_gemm_launch_form<MODE, H, SPLIT, false>(p, grid, s);
 }
 
 }  // namespace msgl
