@@ -439,6 +439,11 @@ void moe_combine(at::Tensor out, at::Tensor y, at::Tensor w, at::Tensor inv, int
 
 // ----- router and 4-bit weights. These allocate their outputs, so that a call costs one crossing of the
 // binding, and run on the tensors' own device and its current stream.
+void check_launch(int rc, const char* op) {
+  CHECK(rc != 3, op, ": these sizes are not supported");
+  CHECK(rc == 0, op, " failed (code ", rc, ": ", cudaGetErrorString(cudaGetLastError()), ")");
+}
+
 std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, int64_t topk, bool sigmoid,
                                                  c10::optional<at::Tensor> bias, int64_t groups, int64_t kept,
                                                  bool top2, bool renorm, double scale) {
@@ -467,7 +472,7 @@ std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, int64_t topk
   at::Tensor ids = at::empty({T, topk}, logits.options().dtype(at::kInt));
   const int rc = msgl_route_experts(logits.data_ptr(), f32, logits.stride(0), b, T, E, topk, sigmoid, groups, kept, top2,
                                     renorm, scale, weights.data_ptr<float>(), ids.data_ptr<int32_t>(), stream());
-  CHECK(rc == 0, "route_experts failed (code ", rc, ")");
+  check_launch(rc, "route_experts");
   return {weights, ids};
 }
 
@@ -517,7 +522,7 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
   at::Tensor out = at::empty({M, n}, x.options());
   if (M == 0) return out;
   const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
-  CHECK(rc == 0, "linear_w4 failed (code ", rc, ")");
+  check_launch(rc, "linear_w4");
   return out;
 }
 
@@ -551,11 +556,12 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
     CHECK(b2->numel() == E * n2 && b2->device() == x.device(), "w2_bias must be [E, H]");
   }
   at::Tensor out = at::empty({T, n2}, x.options());
-  at::Tensor ws = at::empty({msgl_w4_experts_workspace(T, topk, &w1, &w2)}, x.options().dtype(at::kByte));
+  at::Tensor ws = at::empty({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, x.options().dtype(at::kByte));
+  if (T == 0) return out;
   const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0,
                                  weights.data_ptr<float>(), ids.data_ptr<int32_t>(), opt_ptr(b1), opt_ptr(b2), act,
                                  ws.data_ptr(), stream());
-  CHECK(rc == 0, "experts_w4 failed (code ", rc, ")");
+  check_launch(rc, "experts_w4");
   return out;
 }
 

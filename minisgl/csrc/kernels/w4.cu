@@ -6,7 +6,6 @@
 // meet through distributed shared memory. The split is the one whose largest share of weights, plus the
 // activations that every CTA reads, is smallest (plan()).
 #include <algorithm>
-#include <mutex>
 
 #include "w4_gemm.cuh"
 
@@ -97,35 +96,6 @@ struct Plan {
   int splits, grid, max_tiles, smem;
 };
 
-// clusters of `splits` CTAs that run at once, one CTA per SM (148 SMs, not all in groups of 8)
-template <auto Kernel>
-int resident_clusters(int splits, int threads) {
-  static std::mutex mu;
-  static int known[64][9] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (splits == 1) return msgl_num_sms();
-  std::lock_guard<std::mutex> guard(mu);
-  int& k = known[dev][splits];
-  if (k != 0) return k;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = kSmemMax;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = splits;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    n = 1;
-  }
-  return k = n;
-}
-
 // The split of the inputs with the least estimated time: the largest CTA's weight bytes at an SM's
 // share of the memory rate (43 B/ns), its activations at the L2's (four times that), and 1.5 us for the
 // exchange. Returns splits = 0 if the rows do not fit.
@@ -134,7 +104,7 @@ Plan plan(const W4Tensor& w, int M) {
   Plan best = {0, 0, 0, 0};
   double best_ns = 1e30;
   for (int s = 1; s <= 8 && s <= w.kc; s *= 2) {
-    const int clusters = std::min(resident_clusters<Kernel>(s, w4_threads<NT>()), w.tiles);
+    const int clusters = std::min(w4_resident_clusters<Kernel>(s, w4_threads<NT>()), w.tiles);
     if (clusters < 1) continue;
     const int tiles = (w.tiles + clusters - 1) / clusters;
     const int records = (w.kc + s - 1) / s, kn = records * 128;
@@ -193,22 +163,32 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   p.m_tiles = (a.M + kGwMaxTokens - 1) / kGwMaxTokens;
   p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
   p.m_tiles = (a.M + p.bn - 1) / p.bn;
-  const int sms = msgl_num_sms();
-  // 256-row tiles unless these, their inputs cut in eight, would use less than half the SMs
-  const int64_t wide = (int64_t)((a.w.tiles + 7) / 8) * p.m_tiles;
-  const bool two = wide * std::min(8, a.w.kc) >= sms / 2;
-  p.n_tiles = two ? (a.w.tiles + 7) / 8 : (a.w.tiles + 3) / 4;
-  const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
-  if (units >= (1ll << 31)) return 3;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / units, 8, (int64_t)a.w.kc}));
-  const int grid = (int)std::min<int64_t>(units * p.splits, sms);
-  if (p.splits > 1) {
-    const int rc = two ? w4_gemm_launch<kW4Dense, 2, true>(p, grid, s) : w4_gemm_launch<kW4Dense, 1, true>(p, grid, s);
-    if (rc != 3) return rc;
-    p.splits = 1;  // the fp32 tile does not fit
+  // Halves of a tile and cuts of the inputs with the least estimated time, in clocks per 128 inputs of a tile:
+  // conversion 450 a half (measured), the tensor core 4 a token and half, the tokens' rows from L2 5 a token;
+  // the exchange 2000 and 20 a token and half.
+  double best = 1e30;
+  int halves = 1;
+  for (int h = 1; h <= 2; ++h) {
+    const int64_t units = (int64_t)((a.w.tiles + 4 * h - 1) / (4 * h)) * p.m_tiles;
+    if (units >= (1ll << 31)) return 3;
+    for (int s = 1; s <= std::min(8, a.w.kc); ++s) {
+      if (s > 1 && p.bn * h * 512 > kGwRoom) continue;  // the fp32 tile does not fit
+      const int at_once = h == 2 ? w4_gemm_clusters<2>(s) : w4_gemm_clusters<1>(s);
+      if (at_once < 1) continue;
+      const double waves = (double)((units + at_once - 1) / at_once), records = (a.w.kc + s - 1) / s;
+      const double per = std::max({450.0 * h, 4.0 * p.bn * h, 5.0 * p.bn});
+      const double t = waves * (records * per + 1500) + (s > 1 ? 2000 + 20.0 * p.bn * h : 0);
+      if (t < best) best = t, halves = h, p.splits = s;
+    }
   }
-  return two ? w4_gemm_launch<kW4Dense, 2, false>(p, (int)std::min<int64_t>(units, sms), s)
-             : w4_gemm_launch<kW4Dense, 1, false>(p, (int)std::min<int64_t>(units, sms), s);
+  p.n_tiles = (a.w.tiles + 4 * halves - 1) / (4 * halves);
+  const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
+  if (p.splits > 1) {
+    const int grid = (int)(units * p.splits);
+    return halves == 2 ? w4_gemm_launch<kW4Dense, 2, true>(p, grid, s) : w4_gemm_launch<kW4Dense, 1, true>(p, grid, s);
+  }
+  const int grid = (int)std::min<int64_t>(units, msgl_num_sms());
+  return halves == 2 ? w4_gemm_launch<kW4Dense, 2, false>(p, grid, s) : w4_gemm_launch<kW4Dense, 1, false>(p, grid, s);
 }
 
 }  // namespace

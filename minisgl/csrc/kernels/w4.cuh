@@ -23,6 +23,7 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "api.h"
@@ -352,6 +353,36 @@ struct W4Runs {
     }
   }
 };
+
+// clusters of `splits` CTAs that run at once, one CTA per SM (148 SMs, in groups that are no multiples of 8)
+template <auto Kernel>
+int w4_resident_clusters(int splits, int threads) {
+  static std::mutex mu;
+  static int known[64][9] = {};
+  if (splits == 1) return msgl_num_sms();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> guard(mu);
+  int& k = known[dev][splits];
+  if (k != 0) return k;
+  if (msgl_set_smem<Kernel>(227 * 1024) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = 227 * 1024;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  return k = n;
+}
 
 // calls fn(group, zeros, fp16) with the weight's form as constants
 template <class Fn>

@@ -54,6 +54,7 @@ constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
 constexpr int kGwMaxSlots = 8, kGwMaxA = 8, kGwB = 4;  // most stages of the rings
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
+constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
 constexpr int kGwMaxTokens = 224;    // of a tile: two stages of A then fit beside the accumulators
 
 MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
@@ -537,7 +538,7 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   p.stages = std::min(kGwMaxA, (512 - p.sets * H * p.half_cols) / kA);
   if (p.stages < 2) return 3;
   p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
-  const int room = kMax - 1024 - kGwMisc, stage = p.bn * 128;
+  const int room = kGwRoom, stage = p.bn * 128;
   p.slots = std::min(kGwMaxSlots, (room - kGwB * stage) / p.raw_bytes);
   p.ring_bytes = kGwB * stage + p.slots * p.raw_bytes;
   if (SPLIT) p.ring_bytes = std::max(p.ring_bytes, p.bn * H * 512);
@@ -549,6 +550,10 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   const int smem = 1024 + kGwMisc + p.ring_bytes;
   return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
 }
+
+// clusters of s CTAs of the dense form that run at once
+template <int H>
+int w4_gemm_clusters(int s) { return w4_resident_clusters<w4_gemm_kernel<kW4Dense, H, true, false, false, false>>(s, kGwThreads); }
 
 template <int MODE, int H, bool SPLIT, bool FINE>
 int w4_gemm_launch_form(const W4GemmArgs& p, int grid, cudaStream_t s) {

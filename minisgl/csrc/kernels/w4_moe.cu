@@ -6,9 +6,12 @@
 // layer is three launches; the counting of the second product overlaps the end of the first. The
 // activated values between the products are bf16, as the second product's operands are; y is fp32 and
 // the sum over a token's experts runs in the order of its choices, so results do not vary.
+//
+// Many tokens: a kernel sorts the pairs by expert and lists tiles of up to 96 of an expert's pairs; the products
+// run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
 #include <algorithm>
 
-#include "w4.cuh"
+#include "w4_gemm.cuh"
 
 using namespace msgl;
 
@@ -20,14 +23,6 @@ constexpr int kSmemMax = 227 * 1024;
 
 // number of an expert among those from e0 on; wraps to a large number for one that is not here
 MSGL_DEVICE unsigned local_expert(int32_t id, int e0) { return (unsigned)id - (unsigned)e0; }
-
-MSGL_DEVICE float gated_act(float g, float u, int act) {
-  if (act == 0) return g / (1.f + __expf(-g)) * u;
-  if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-  g = fminf(g, 7.f);
-  u = fminf(fmaxf(u, -7.f), 7.f);
-  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
-}
 
 struct ExpertArgs {
   W4Tensor w;
@@ -47,11 +42,12 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   constexpr int kWarps = w4_warps<NT>(), kThreads = w4_threads<NT>();
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  int* count = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());  // [E] pairs of every expert
-  int* hit = count + p.E;                                               // the experts that have any
-  int* list = hit + p.E;                                                // [pairs] pairs of one expert
+  int* const n_hit = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());
+  int* const n_list = n_hit + 1;
+  int* count = n_hit + 4;    // [E] pairs of every expert
+  int* hit = count + p.E;    // the experts that have any
+  int* list = hit + p.E;     // [pairs] pairs of one expert
   uint8_t* xs = reinterpret_cast<uint8_t*>(list) + (p.pairs * 4 + 15) / 16 * 16 + (p.E * 8 % 16);
-  __shared__ int n_hit, n_list;
   W4Runs<NT, G, Z, F> runs{smem};
   runs.init();
 
@@ -74,10 +70,10 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
       if (any) hit[n + __popc(m & ((1u << lane) - 1))] = e0 + lane;
       n += __popc(m);
     }
-    if (lane == 0) n_hit = n;
+    if (lane == 0) *n_hit = n;
   }
   __syncthreads();
-  const int64_t all = (int64_t)n_hit * p.w.tiles;
+  const int64_t all = (int64_t)*n_hit * p.w.tiles;
   int64_t pos = all * blockIdx.x / gridDim.x;
   const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
   const int pitch = w4_pitch(p.w.kc * 128);
@@ -96,13 +92,13 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
     const int e = hit[pos / p.w.tiles];
     const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
     __syncthreads();  // the previous expert's list is done with
-    if (threadIdx.x == 0) n_list = 0;
+    if (threadIdx.x == 0) *n_list = 0;
     __syncthreads();
     // in any order: a token's sums do not depend on its place
     for (int i = threadIdx.x; i < p.pairs; i += kThreads)
-      if (local_expert(p.ids[i], p.e0) == (unsigned)e) list[atomicAdd(&n_list, 1)] = i;
+      if (local_expert(p.ids[i], p.e0) == (unsigned)e) list[atomicAdd(n_list, 1)] = i;
     __syncthreads();
-    const int ne = n_list;
+    const int ne = *n_list;
     for (int m0 = 0; m0 < ne; m0 += p.rows) {
       const int nx = min(p.rows, ne - m0);
       const int* mine = list + m0;
@@ -123,7 +119,7 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
               if (m >= nx) continue;
               if constexpr (GATED)
                 p.a[(int64_t)mine[m] * p.a_stride + n] =
-                    __float2bfloat16(gated_act(acc[r][q][c] + b0, acc[r][q][2 + c] + b1, p.act));
+                    __float2bfloat16(w4_gated_act(acc[r][q][c] + b0, acc[r][q][2 + c] + b1, p.act));
               else
                 p.y[(int64_t)mine[m] * p.w.n + n] = acc[r >> 1][q][2 * (r & 1) + c] + b0;
             }
@@ -166,10 +162,10 @@ __global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict
 template <int NT, int G, bool Z, bool F, bool GATED>
 int launch_experts(ExpertArgs p, int fixed, cudaStream_t s) {
   constexpr auto kernel = w4_experts_kernel<NT, G, Z, F, GATED>;
-  if (msgl_set_smem<kernel>(kSmemMax - 64) != cudaSuccess) return 4;
+  if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
   const int pitch = w4_pitch(p.w.kc * 128);
   constexpr int kRun = w4_run_bytes<NT, G, Z>();
-  p.rows = std::min(NT * 8, (kSmemMax - 64 - fixed - kRun) / pitch);
+  p.rows = std::min(NT * 8, (kSmemMax - fixed - kRun) / pitch);
   if (p.rows < 1) return 3;
   const int smem = kRun + fixed + p.rows * pitch;
   const int64_t most = (int64_t)std::min(p.E, p.pairs) * p.w.tiles;
@@ -186,41 +182,147 @@ int launch_experts_nt(const ExpertArgs& p, const MsglW4* w, int fixed, cudaStrea
 // rarely exceed 8), else 16; a second pass reads the expert's weights again, from L2.
 template <bool GATED>
 int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
-  const int fixed = 8 * p.E + 16 + (p.pairs * 4 + 15) / 16 * 16;
+  const int fixed = 8 * p.E + 32 + (p.pairs * 4 + 15) / 16 * 16;
   return p.pairs <= 4 * p.E ? launch_experts_nt<GATED, 1>(p, w, fixed, s)
                              : launch_experts_nt<GATED, 2>(p, w, fixed, s);
 }
 
+constexpr int kTileTokens = 96;  // of a tile: two sets of accumulators then fit into tensor memory
+
+// Sorts the pairs by expert (in any order within one: a pair's result does not depend on its place) and cuts
+// every expert's into equal tiles. One CTA.
+__global__ void __launch_bounds__(1024) w4_plan_kernel(const int32_t* __restrict__ ids, int pairs, int E, int e0,
+                                                       int32_t* __restrict__ sorted, int4* __restrict__ work,
+                                                       int32_t* __restrict__ count) {
+  __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], sums[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch();
+  cnt[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < pairs; i += 1024) {
+    const unsigned e = local_expert(ids[i], e0);
+    if (e < (unsigned)E) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  // running sums of the pairs and tiles over the experts, one a thread
+  const int c = cnt[tid], tiles = (c + kTileTokens - 1) / kTileTokens;
+  int a = c, b = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += x, b += y;
+  }
+  if (lane == 31) sums[0][warp] = a, sums[1][warp] = b;
+  __syncthreads();
+  if (warp == 0) {
+    int x = sums[0][lane], y = sums[1][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) x += u, y += v;
+    }
+    sums[0][lane] = x, sums[1][lane] = y;
+    if (lane == 31) *count = y;
+  }
+  __syncthreads();
+  const int start = a - c + (warp > 0 ? sums[0][warp - 1] : 0), first = b - tiles + (warp > 0 ? sums[1][warp - 1] : 0);
+  at[tid] = start;
+  for (int i = 0; i < tiles; ++i) {
+    const int from = (int)((int64_t)c * i / tiles), to = (int)((int64_t)c * (i + 1) / tiles);
+    work[first + i] = make_int4(tid, start + from, to - from, 0);
+  }
+  __syncthreads();
+  for (int i = tid; i < pairs; i += 1024) {
+    const unsigned e = local_expert(ids[i], e0);
+    if (e < (unsigned)E) sorted[atomicAdd(&at[e], 1)] = i;
+  }
+}
+
+// scratch of a call: activated rows, results of the pairs, and for many tokens the sorted pairs and tiles
+struct Scratch {
+  int64_t a, y, sorted, work, count, bytes;
+};
+Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
+  const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  Scratch s;
+  s.a = 0;
+  s.y = up(pairs * w2->kc * 128 * 2);
+  s.sorted = s.y + up(pairs * w2->n * 4);
+  s.work = s.sorted + up(pairs * 4);
+  s.count = s.work + up((E + pairs / kTileTokens) * 16);
+  s.bytes = s.count + 256;
+  return s;
+}
+
+// Pairs per expert up to which the streaming product is taken.
+constexpr int kStreamPairs = 8;
+
+int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
+                  const int32_t* ids, const void* b1, const void* b2, int act, uint8_t* ws, const Scratch& sc,
+                  cudaStream_t s) {
+  int32_t *sorted = (int32_t*)(ws + sc.sorted), *count = (int32_t*)(ws + sc.count);
+  int4* work = (int4*)(ws + sc.work);
+  if (msgl_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, work, count) != cudaSuccess)
+    return 4;
+  W4GemmArgs p = {};
+  p.bn = std::min(kTileTokens, (pairs + 15) / 16 * 16);
+  p.splits = 1;
+  p.count = count, p.work = work, p.sorted = sorted;
+  p.topk = topk, p.act = act;
+  const int64_t tiles = std::min<int64_t>(E + pairs / kTileTokens, pairs);
+  W4GemmArgs q = p;
+  p.w = w4_tensor(w1);
+  p.group = w1->group, p.zeros = w1->zeros, p.fp16 = w1->fp16;
+  p.in = (const __nv_bfloat16*)x, p.in_stride = x_stride;
+  p.bias = (const __nv_bfloat16*)b1;
+  p.out = ws + sc.a, p.out_stride = w2->kc * 128;
+  p.n_tiles = (w1->tiles + 7) / 8;
+  q.w = w4_tensor(w2);
+  q.group = w2->group, q.zeros = w2->zeros, q.fp16 = w2->fp16;
+  q.in = (const __nv_bfloat16*)(ws + sc.a), q.in_stride = w2->kc * 128;
+  q.M = pairs;
+  q.bias = (const __nv_bfloat16*)b2;
+  q.out = ws + sc.y, q.out_stride = w2->n;
+  q.n_tiles = (w2->tiles + 7) / 8;
+  const int64_t most = tiles * std::max(p.n_tiles, q.n_tiles);
+  if (most >= (1ll << 31)) return 3;
+  const int sms = msgl_num_sms();
+  const int rc = w4_gemm_launch<kW4GateUp, 2, false>(p, (int)std::min<int64_t>(sms, tiles * p.n_tiles), s);
+  return rc != 0 ? rc : w4_gemm_launch<kW4Down, 2, false>(q, (int)std::min<int64_t>(sms, tiles * q.n_tiles), s);
+}
+
 }  // namespace
 
-extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, const MsglW4* w1, const MsglW4* w2) {
-  const int64_t pairs = (int64_t)T * topk;
-  return pairs * w2->kc * 128 * 2 + pairs * w2->n * 4;
+extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, int E, const MsglW4* w1, const MsglW4* w2) {
+  return scratch_of((int64_t)T * topk, E, w2).bytes;
 }
 
 extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
                                const MsglW4* w2, int E, int e0, const float* weights, const int32_t* ids,
                                const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
   if (T == 0) return 0;
-  if (E > kMoeMaxExperts || topk > kMoeMaxPairs) return 3;
-  const int a_stride = w2->kc * 128, most = kMoeMaxPairs / topk;
-  for (int t0 = 0; t0 < T; t0 += most) {
-    const int n = std::min(most, T - t0), pairs = n * topk;
-    __nv_bfloat16* a = (__nv_bfloat16*)workspace;
-    float* y = (float*)((uint8_t*)workspace + (int64_t)pairs * a_stride * 2);
-    const int32_t* id = ids + (int64_t)t0 * topk;
-    ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, id, (const __nv_bfloat16*)x + t0 * x_stride, x_stride,
-                     (const __nv_bfloat16*)b1, a, nullptr, a_stride, act, 0};
-    ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, id, a, a_stride, (const __nv_bfloat16*)b2, nullptr, y, 0, 0, 0};
-    int rc = experts_product<true>(p1, w1, s);
+  if (E > kMoeMaxExperts) return 3;
+  const int pairs = T * topk, a_stride = w2->kc * 128;
+  uint8_t* ws = (uint8_t*)workspace;
+  const Scratch sc = scratch_of(pairs, E, w2);
+  int rc;
+  if (pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs) {
+    __nv_bfloat16* a = (__nv_bfloat16*)(ws + sc.a);
+    ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, ids, (const __nv_bfloat16*)x, x_stride, (const __nv_bfloat16*)b1,
+                     a, nullptr, a_stride, act, 0};
+    ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, ids, a, a_stride, (const __nv_bfloat16*)b2, nullptr,
+                     (float*)(ws + sc.y), 0, 0, 0};
+    rc = experts_product<true>(p1, w1, s);
     if (rc == 0) rc = experts_product<false>(p2, w2, s);
-    if (rc != 0) return rc;
-    if (msgl_launch(w4_combine_kernel, dim3(n, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)y,
-                    weights + (int64_t)t0 * topk, id, E, e0, topk, w2->n, (__nv_bfloat16*)out + (int64_t)t0 * w2->n) !=
-        cudaSuccess)
-      return 4;
+  } else {
+    rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, ids, b1, b2, act, ws, sc, s);
   }
-  return 0;
+  if (rc != 0) return rc;
+  return msgl_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),
+                     weights, ids, E, e0, topk, w2->n, (__nv_bfloat16*)out) == cudaSuccess
+             ? 0
+             : 4;
 }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4_moe)
