@@ -17,12 +17,17 @@ using namespace msgl;
 
 namespace {
 
-constexpr int kMoeMaxPairs = 4096;  // pairs of one launch: the list of an expert's pairs is in shared memory
+constexpr int kMoeMaxPairs = 4096;  // of the streaming product: their experts are kept in shared memory
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kSmemMax = 227 * 1024;
 
 // number of an expert among those from e0 on; wraps to a large number for one that is not here
 MSGL_DEVICE unsigned local_expert(int32_t id, int e0) { return (unsigned)id - (unsigned)e0; }
+
+// shared memory of the lists behind the runs', a multiple of 16
+__host__ __device__ inline int prelude_bytes(int E, int pairs, int rows) {
+  return (4 + 16 + 32 + 2 * E + pairs / rows + pairs + 3) / 4 * 16;
+}
 
 struct ExpertArgs {
   W4Tensor w;
@@ -42,12 +47,14 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   constexpr int kWarps = w4_warps<NT>(), kThreads = w4_threads<NT>();
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  int* const n_hit = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());
-  int* const n_list = n_hit + 1;
-  int* count = n_hit + 4;    // [E] pairs of every expert
-  int* hit = count + p.E;    // the experts that have any
-  int* list = hit + p.E;     // [pairs] pairs of one expert
-  uint8_t* xs = reinterpret_cast<uint8_t*>(list) + (p.pairs * 4 + 15) / 16 * 16 + (p.E * 8 % 16);
+  // units: up to p.rows of an expert's pairs
+  int* const n_units = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());
+  int* const list = n_units + 4;                          // [16] pairs of the unit at hand
+  int* const seen = list + 16;                            // [32] warps' counts
+  int* const count = seen + 32;                           // [E] pairs of every expert
+  int* const units = count + p.E;                         // [E + pairs / rows] expert, number of the unit in it
+  uint32_t* const lid = reinterpret_cast<uint32_t*>(units + p.E + p.pairs / p.rows);  // [pairs] experts here
+  uint8_t* xs = smem + (w4_run_bytes<NT, G, Z>() + prelude_bytes(p.E, p.pairs, p.rows));
   W4Runs<NT, G, Z, F> runs{smem};
   runs.init();
 
@@ -59,49 +66,68 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   __syncthreads();
   for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
     const unsigned e = local_expert(p.ids[i], p.e0);
+    lid[i] = e;
     if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
   }
   __syncthreads();
   if (warp == 0) {
     int n = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const bool any = e0 + lane < p.E && count[e0 + lane] > 0;
-      const unsigned m = __ballot_sync(0xffffffffu, any);
-      if (any) hit[n + __popc(m & ((1u << lane) - 1))] = e0 + lane;
-      n += __popc(m);
+    for (int b = 0; b < p.E; b += 32) {
+      const int e = b + lane, mine = e < p.E ? (count[e] + p.rows - 1) / p.rows : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      for (int i = 0; i < mine; ++i) units[n + sum - mine + i] = e | i << 16;
+      n += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) *n_hit = n;
+    if (lane == 0) *n_units = n;
   }
   __syncthreads();
-  const int64_t all = (int64_t)*n_hit * p.w.tiles;
-  int64_t pos = all * blockIdx.x / gridDim.x;
-  const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
+  // this CTA's run of the units' tiles: an equal share, whichever experts it falls on
+  const int all = *n_units * p.w.tiles, share = all / (int)gridDim.x, rest = all % (int)gridDim.x;
+  int pos = (int)blockIdx.x * share + min((int)blockIdx.x, rest);
+  const int end = pos + share + ((int)blockIdx.x < rest ? 1 : 0);
   const int pitch = w4_pitch(p.w.kc * 128);
   if constexpr (!GATED) {
     // bring the run's first weights into L2 while the first product ends
     if (lane == 0 && pos < end) {
-      const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
-      const int64_t tile = (int64_t)hit[pos / p.w.tiles] * p.w.tiles + ta;
+      const int ta = pos % p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
+      const int64_t tile = (int64_t)(units[pos / p.w.tiles] & 0xffff) * p.w.tiles + ta;
       const int a = runs.bound(nt * p.w.kc, warp), n = min(runs.bound(nt * p.w.kc, warp + 1) - a, kW4Slots);
       if (n > 0) prefetch_l2(p.w.data + (tile * p.w.kc + a) * R::kBytes, n * R::kBytes);
     }
     pdl_wait();
   }
 
+  // the pairs are looked through by all warps, a run of whole 32s each
+  const int per = ((p.pairs + 31) / 32 + kWarps - 1) / kWarps * 32;
   while (pos < end) {
-    const int e = hit[pos / p.w.tiles];
-    const int ta = (int)(pos % p.w.tiles), nt = (int)min((int64_t)(p.w.tiles - ta), end - pos);
-    __syncthreads();  // the previous expert's list is done with
-    if (threadIdx.x == 0) *n_list = 0;
+    const int unit = units[pos / p.w.tiles], e = unit & 0xffff, i0 = unit >> 16;
+    const int ta = pos % p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
+    // the expert's pairs are cut into equal units; every CTA finds the same ones in the same order
+    const int c = count[e], cuts = (c + p.rows - 1) / p.rows, m0 = c * i0 / cuts, nx = c * (i0 + 1) / cuts - m0;
+    __syncthreads();  // the previous unit's list is done with
+    int found = 0;
+    for (int i = warp * per + lane; i < (warp + 1) * per; i += 32)
+      found += __popc(__ballot_sync(0xffffffffu, i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e));
+    if (lane == 0) seen[warp] = found;
     __syncthreads();
-    // in any order: a token's sums do not depend on its place
-    for (int i = threadIdx.x; i < p.pairs; i += kThreads)
-      if (local_expert(p.ids[i], p.e0) == (unsigned)e) list[atomicAdd(n_list, 1)] = i;
+    int at = -m0;
+    for (int w = 0; w < warp; ++w) at += seen[w];
+    if (found > 0)
+      for (int i = warp * per + lane; i < (warp + 1) * per; i += 32) {
+        const bool is = i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e;
+        const unsigned m = __ballot_sync(0xffffffffu, is);
+        const int k = at + __popc(m & ((1u << lane) - 1));
+        if (is && k >= 0 && k < nx) list[k] = i;
+        at += __popc(m);
+      }
     __syncthreads();
-    const int ne = *n_list;
-    for (int m0 = 0; m0 < ne; m0 += p.rows) {
-      const int nx = min(p.rows, ne - m0);
-      const int* mine = list + m0;
+    const int* mine = list;
+    {
       const auto row = [&](int r) { return p.in + (int64_t)(GATED ? mine[r] / p.topk : mine[r]) * p.in_stride; };
       const auto emit = [&](int tile, const float (&acc)[2][NT][4]) {
 #pragma unroll
@@ -160,31 +186,27 @@ __global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict
 }
 
 template <int NT, int G, bool Z, bool F, bool GATED>
-int launch_experts(ExpertArgs p, int fixed, cudaStream_t s) {
+int launch_experts(ExpertArgs p, cudaStream_t s) {
   constexpr auto kernel = w4_experts_kernel<NT, G, Z, F, GATED>;
   if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
-  const int pitch = w4_pitch(p.w.kc * 128);
   constexpr int kRun = w4_run_bytes<NT, G, Z>();
-  p.rows = std::min(NT * 8, (kSmemMax - fixed - kRun) / pitch);
+  const int pitch = w4_pitch(p.w.kc * 128);
+  p.rows = std::min(NT * 8, (kSmemMax - kRun - prelude_bytes(p.E, p.pairs, 1)) / pitch);
   if (p.rows < 1) return 3;
-  const int smem = kRun + fixed + p.rows * pitch;
-  const int64_t most = (int64_t)std::min(p.E, p.pairs) * p.w.tiles;
+  const int64_t most = (int64_t)(std::min(p.E, p.pairs) + p.pairs / p.rows) * p.w.tiles;
+  if (most * 2 >= (1ll << 31)) return 3;
+  const int smem = kRun + prelude_bytes(p.E, p.pairs, p.rows) + p.rows * pitch;
   const int grid = (int)std::min<int64_t>(msgl_num_sms(), most);
   return msgl_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
 }
 
-template <bool GATED, int NT>
-int launch_experts_nt(const ExpertArgs& p, const MsglW4* w, int fixed, cudaStream_t s) {
-  return w4_dispatch(w, [&](auto g, auto z, auto f) { return launch_experts<NT, g(), z(), f(), GATED>(p, fixed, s); });
-}
-
 // One product. Token columns per pass: 8 while an expert has at most 4 tokens on average (its tokens then
-// rarely exceed 8), else 16; a second pass reads the expert's weights again, from L2.
+// rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2.
 template <bool GATED>
 int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
-  const int fixed = 8 * p.E + 32 + (p.pairs * 4 + 15) / 16 * 16;
-  return p.pairs <= 4 * p.E ? launch_experts_nt<GATED, 1>(p, w, fixed, s)
-                             : launch_experts_nt<GATED, 2>(p, w, fixed, s);
+  return w4_dispatch(w, [&](auto g, auto z, auto f) {
+    return p.pairs <= 4 * p.E ? launch_experts<1, g(), z(), f(), GATED>(p, s) : launch_experts<2, g(), z(), f(), GATED>(p, s);
+  });
 }
 
 constexpr int kTileTokens = 96;  // of a tile: two sets of accumulators then fit into tensor memory
