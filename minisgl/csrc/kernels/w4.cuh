@@ -215,9 +215,7 @@ struct W4Runs {
         }
       }
     };
-    // the ring goes on where the previous run left it (whose sums this warp may have put there)
-    fence_async_smem();
-    __syncwarp();
+    // the ring goes on where the previous run left it
     uint32_t slot = ring0 + (it % kW4Slots) * R::kBytes, bar = bars + (it % kW4Slots) * 8;
     constexpr uint32_t kOther = R::kBytes;
     static_assert(kW4Slots == 2, "the slots alternate");
@@ -236,106 +234,111 @@ struct W4Runs {
       xrow[nt] = smem_u32(xs) + (uint32_t)(min(nt * 8 + g, nx - 1) * pitch + t * 8);
     const uint32_t mine = lane * 16, side = R::kScales + g * 8, zside = R::kZeros + g * 4;
     float acc[2][NT][4];
-    for (int i = a; i < b;) {
-      const int from = i - cc;            // the tile's first record
-      const int end = min(from + nc, b);  // one past its last one here
-      uint32_t xoff = cc * 256;
+    // One place gives sums away, for the size of the code: a launch of a few microseconds is mostly its first
+    // execution. First the warp's own tiles, then, behind the barrier, one that it shares with later warps.
+    for (int i = a;;) {
+      int give = tile;
+      if (i < b) {
+        const int from = i - cc;            // the tile's first record
+        const int end = min(from + nc, b);  // one past its last one here
+        uint32_t xoff = cc * 256;
+        clear(acc);
+        for (; i < end; ++i) {
+          if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
+            if (ok) ok = w4_wait<20>(bar, (it >> 1) & 1);
+          }
+          ++it;
+          uint4 q[2][2];
+          uint2 s[R::kGroups];
+          uint32_t z[R::kGroups];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+          for (int r = 0; r < 4; ++r) q[r >> 1][r & 1] = lds128(slot + mine + r * 512);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[0][nt][r] = acc[1][nt][r] = 0.f;
-      for (; i < end; ++i) {
-        if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
-          if (ok) ok = w4_wait<20>(bar, (it >> 1) & 1);
-        }
-        ++it;
-        uint4 q[2][2];
-        uint2 s[R::kGroups];
-        uint32_t z[R::kGroups];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) q[r >> 1][r & 1] = lds128(slot + mine + r * 512);
-#pragma unroll
-        for (int j = 0; j < R::kGroups; ++j) {
-          s[j] = lds64(slot + side + j * 64);
-          if constexpr (Z) z[j] = lds32(slot + zside + j * 32);
-        }
-        __syncwarp();  // every lane has read the slot
-        if (i + 2 < b) fetch(slot, bar);
-        slot = 2 * ring0 + kOther - slot;
-        bar = 2 * bars + 8 - bar;
+          for (int j = 0; j < R::kGroups; ++j) {
+            s[j] = lds64(slot + side + j * 64);
+            if constexpr (Z) z[j] = lds32(slot + zside + j * 32);
+          }
+          __syncwarp();  // every lane has read the slot
+          if (i + 2 < b) fetch(slot, bar);
+          slot = 2 * ring0 + kOther - slot;
+          bar = 2 * bars + 8 - bar;
 
-        float tmp[2][NT][4];
+          float tmp[2][NT][4];
 #pragma unroll
-        for (int quarter = 0; quarter < 4; ++quarter) {  // 32 inputs
-          constexpr int per = G / 32;                    // quarters per group
-          const int j = quarter / per;
-          uint32_t fr[2][2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t z0 = Z ? 0x43004300u + ((z[j] >> (16 * h)) & 15u) * 0x10001u : 0x43084308u;
-            const uint32_t z1 = Z ? 0x43004300u + ((z[j] >> (16 * h + 8)) & 15u) * 0x10001u : 0x43084308u;
-            const uint4 v4 = q[h][quarter >> 1];
-            const uint32_t words[2] = {quarter & 1 ? v4.z : v4.x, quarter & 1 ? v4.w : v4.y};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              fr[h][e][0] = codes_bf16x2(words[e], z0);
-              fr[h][e][1] = codes_bf16x2(words[e] >> 4, z1);
-              fr[h][e][2] = codes_bf16x2(words[e] >> 8, z0);
-              fr[h][e][3] = codes_bf16x2(words[e] >> 12, z1);
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint2 x0 = lds64(xrow[nt] + xoff + quarter * 64), x1 = lds64(xrow[nt] + xoff + quarter * 64 + 32);
+          for (int quarter = 0; quarter < 4; ++quarter) {  // 32 inputs
+            constexpr int per = G / 32;                    // quarters per group
+            const int j = quarter / per;
+            uint32_t fr[2][2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              mma_bf16_16816(tmp[h][nt], fr[h][0], x0.x, x0.y, quarter % per == 0);
-              mma_bf16_16816(tmp[h][nt], fr[h][1], x1.x, x1.y, false);
+              const uint32_t z0 = Z ? 0x43004300u + ((z[j] >> (16 * h)) & 15u) * 0x10001u : 0x43084308u;
+              const uint32_t z1 = Z ? 0x43004300u + ((z[j] >> (16 * h + 8)) & 15u) * 0x10001u : 0x43084308u;
+              const uint4 v4 = q[h][quarter >> 1];
+              const uint32_t words[2] = {quarter & 1 ? v4.z : v4.x, quarter & 1 ? v4.w : v4.y};
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                fr[h][e][0] = codes_bf16x2(words[e], z0);
+                fr[h][e][1] = codes_bf16x2(words[e] >> 4, z1);
+                fr[h][e][2] = codes_bf16x2(words[e] >> 8, z0);
+                fr[h][e][3] = codes_bf16x2(words[e] >> 12, z1);
+              }
             }
-          }
-          if (quarter % per == per - 1) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 sc = w4_scales<F>(h == 0 ? s[j].x : s[j].y);
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint2 x0 = lds64(xrow[nt] + xoff + quarter * 64), x1 = lds64(xrow[nt] + xoff + quarter * 64 + 32);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                acc[h][nt][0] += tmp[h][nt][0] * sc.x;
-                acc[h][nt][1] += tmp[h][nt][1] * sc.x;
-                acc[h][nt][2] += tmp[h][nt][2] * sc.y;
-                acc[h][nt][3] += tmp[h][nt][3] * sc.y;
+              for (int h = 0; h < 2; ++h) {
+                mma_bf16_16816(tmp[h][nt], fr[h][0], x0.x, x0.y, quarter % per == 0);
+                mma_bf16_16816(tmp[h][nt], fr[h][1], x1.x, x1.y, false);
+              }
+            }
+            if (quarter % per == per - 1) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 sc = w4_scales<F>(h == 0 ? s[j].x : s[j].y);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  acc[h][nt][0] += tmp[h][nt][0] * sc.x;
+                  acc[h][nt][1] += tmp[h][nt][1] * sc.x;
+                  acc[h][nt][2] += tmp[h][nt][2] * sc.y;
+                  acc[h][nt][3] += tmp[h][nt][3] * sc.y;
+                }
               }
             }
           }
+          xoff += 256;
         }
-        xoff += 256;
-      }
-      if (from >= a && from + nc <= b) {
-        emit(tile, acc);
-      } else if (from < a) {
-        put(head(warp) + lane, acc);
+        cc = 0;
+        ++tile;
+        if (from < a || from + nc > b) {
+          if (from < a) {
+            put(head(warp) + lane, acc);
+          } else {
+            __syncwarp();
+            put(tail(warp) + lane, acc);
+            fence_async_smem();  // before the next run's copies
+          }
+          continue;
+        }
       } else {
-        __syncwarp();
-        put(tail(warp) + lane, acc);
-      }
-      cc = 0;
-      ++tile;
-    }
-    __syncthreads();
-    // a tile that starts in this warp's run and ends in a later warp's: sum their parts in order
-    if (a < b) {
-      const int last = (b - 1) / nc, from = last * nc, to = from + nc;
-      if (a <= from && b < to) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[0][nt][r] = acc[1][nt][r] = 0.f;
+        if (i == b) __syncthreads();
+        // a tile that starts in this warp's run and ends in a later warp's: sum their parts in order
+        const int last = (b - 1) / nc, from = last * nc, to = from + nc;
+        if (i > b || a == b || a > from || b >= to) break;
+        i = b + 1;
+        give = last;
+        clear(acc);
         add(acc, tail(warp) + lane);
         for (int v = warp + 1; v < kWarps && bound(total, v) < min(to, total); ++v) add(acc, head(v) + lane);
-        emit(last, acc);
       }
+      emit(give, acc);
     }
   }
 
+  static MSGL_DEVICE void clear(float (&acc)[2][NT][4]) {
+#pragma unroll
+    for (int i = 0; i < 8 * NT; ++i) acc[i / (4 * NT)][i / 4 % NT][i % 4] = 0.f;
+  }
   // one lane's sums of a tile, 32 lanes apart
   static MSGL_DEVICE void put(float4* p, const float (&acc)[2][NT][4]) {
 #pragma unroll
@@ -353,6 +356,15 @@ struct W4Runs {
     }
   }
 };
+
+// a call and not inlined: several copies of it would lengthen a short launch by their first execution
+static __noinline__ __device__ float w4_gated_act(float g, float u, int act) {
+  if (act == 0) return g / (1.f + __expf(-g)) * u;
+  if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
+  g = fminf(g, 7.f);
+  u = fminf(fmaxf(u, -7.f), 7.f);
+  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
+}
 
 // clusters of `splits` CTAs that run at once, one CTA per SM (148 SMs, in groups that are no multiples of 8)
 template <auto Kernel>

@@ -57,14 +57,6 @@ constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
 constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
 constexpr int kGwMaxTokens = 224;    // of a tile: two stages of A then fit beside the accumulators
 
-MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
-  if (act == 0) return g / (1.f + __expf(-g)) * u;
-  if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-  g = fminf(g, 7.f);
-  u = fminf(fmaxf(u, -7.f), 7.f);
-  return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
-}
-
 // pair of exact integers (bf16x2) times a scale, rounded once
 template <bool F>
 MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale) {

@@ -26,7 +26,7 @@ MSGL_DEVICE unsigned local_expert(int32_t id, int e0) { return (unsigned)id - (u
 
 // shared memory of the lists behind the runs', a multiple of 16
 __host__ __device__ inline int prelude_bytes(int E, int pairs, int rows) {
-  return (4 + 16 + 32 + 2 * E + pairs / rows + pairs + 3) / 4 * 16;
+  return (16 + 32 + 2 * E + pairs / rows + pairs + 3) / 4 * 16;
 }
 
 struct ExpertArgs {
@@ -48,8 +48,7 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // units: up to p.rows of an expert's pairs
-  int* const n_units = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());
-  int* const list = n_units + 4;                          // [16] pairs of the unit at hand
+  int* const list = reinterpret_cast<int*>(smem + w4_run_bytes<NT, G, Z>());  // [16] pairs of the unit at hand
   int* const seen = list + 16;                            // [32] warps' counts
   int* const count = seen + 32;                           // [E] pairs of every expert
   int* const units = count + p.E;                         // [E + pairs / rows] expert, number of the unit in it
@@ -70,24 +69,28 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
     if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  if (warp == 0) {
-    int n = 0;
-    for (int b = 0; b < p.E; b += 32) {
-      const int e = b + lane, mine = e < p.E ? (count[e] + p.rows - 1) / p.rows : 0;
-      int sum = mine;
+  // the units, expert by expert: sums of 32 experts a warp, then of the warps
+  int n_units = 0;
+  for (int b = 0; b < p.E; b += kThreads) {
+    const int e = b + (int)threadIdx.x, mine = e < p.E ? (count[e] + p.rows - 1) / p.rows : 0;
+    int sum = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      for (int i = 0; i < mine; ++i) units[n + sum - mine + i] = e | i << 16;
-      n += __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
     }
-    if (lane == 0) *n_units = n;
+    if (lane == 31) seen[warp] = sum;
+    __syncthreads();
+    int before = lane < kWarps ? seen[lane] : 0;
+    const int all = __reduce_add_sync(0xffffffffu, before);
+    before = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0);
+    for (int i = 0; i < mine; ++i) units[n_units + before + sum - mine + i] = e | i << 16;
+    n_units += all;
+    if (b + kThreads < p.E) __syncthreads();  // seen is used again
   }
   __syncthreads();
   // this CTA's run of the units' tiles: an equal share, whichever experts it falls on
-  const int all = *n_units * p.w.tiles, share = all / (int)gridDim.x, rest = all % (int)gridDim.x;
+  const int all = n_units * p.w.tiles, share = all / (int)gridDim.x, rest = all % (int)gridDim.x;
   int pos = (int)blockIdx.x * share + min((int)blockIdx.x, rest);
   const int end = pos + share + ((int)blockIdx.x < rest ? 1 : 0);
   const int pitch = w4_pitch(p.w.kc * 128);
@@ -105,18 +108,18 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   // the pairs are looked through by all warps, a run of whole 32s each
   const int per = ((p.pairs + 31) / 32 + kWarps - 1) / kWarps * 32;
   while (pos < end) {
-    const int unit = units[pos / p.w.tiles], e = unit & 0xffff, i0 = unit >> 16;
-    const int ta = pos % p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
+    const int un = pos / p.w.tiles, unit = units[un], e = unit & 0xffff, i0 = unit >> 16;
+    const int ta = pos - un * p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
     // the expert's pairs are cut into equal units; every CTA finds the same ones in the same order
-    const int c = count[e], cuts = (c + p.rows - 1) / p.rows, m0 = c * i0 / cuts, nx = c * (i0 + 1) / cuts - m0;
+    const int c = count[e], cuts = c <= p.rows ? 1 : (c + p.rows - 1) / p.rows;
+    const int m0 = cuts == 1 ? 0 : c * i0 / cuts, nx = (cuts == 1 ? c : c * (i0 + 1) / cuts) - m0;
     __syncthreads();  // the previous unit's list is done with
     int found = 0;
     for (int i = warp * per + lane; i < (warp + 1) * per; i += 32)
       found += __popc(__ballot_sync(0xffffffffu, i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e));
     if (lane == 0) seen[warp] = found;
     __syncthreads();
-    int at = -m0;
-    for (int w = 0; w < warp; ++w) at += seen[w];
+    int at = (int)__reduce_add_sync(0xffffffffu, lane < warp ? seen[lane] : 0) - m0;
     if (found > 0)
       for (int i = warp * per + lane; i < (warp + 1) * per; i += 32) {
         const bool is = i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e;
