@@ -9,7 +9,16 @@
 //
 // A NaN logit counts as -inf and +inf as the largest float; a row without a finite logit has scores of
 // zero, and weights whose sum is zero stay zero. Biases are held to the floats' finite range (NaN: the
-// lowest), so every v is finite and the order is total.
+// lowest), so every v is finite and the order is total: that of 64-bit arithmetic.
+//
+// One warp per token. The choice is made in fp32, with a bound on its errors: where two values that the
+// choice depends on are nearer than that (about one row in a thousand), the row is done again in 64 bits;
+// without a bias the logits themselves decide and nothing is near. Doing every row in 64 bits took 65 us
+// at 16384 x 256 with groups.
+//
+// Top k: the (k + 1)-th largest of the lanes' maxima (a sort of 32 keys across the warp) bounds the
+// (k + 1)-th largest value from below; the few values at or above it are gathered, a lane each, and ranked by
+// comparing each with each. Rows with more than 32 of them (many equal values) pick one after another.
 #include <cfloat>
 
 #include "api.h"
@@ -22,6 +31,16 @@ namespace {
 constexpr int kRouteWarps = 4;
 constexpr int kRouteMaxE = 512;
 
+struct RouteArgs {
+  const void* logits;
+  int64_t stride;
+  const float* bias;
+  int n_tok, E, topk, sigmoid, groups, kept, top2, renorm;
+  float scale;
+  float* weights;
+  int32_t* ids;
+};
+
 template <typename T>
 __device__ __forceinline__ float logit_of(const T* p);
 template <>
@@ -29,7 +48,8 @@ __device__ __forceinline__ float logit_of<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float logit_of<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+// (+ 0.f: -0 and 0 are equal, and so are their keys)
+__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX) + 0.f; }
 __device__ __forceinline__ float clean_bias(float b) { return b != b ? -FLT_MAX : fmaxf(fminf(b, FLT_MAX), -FLT_MAX); }
 
 // largest value of the warp's lanes, then the lowest index that has it
@@ -42,22 +62,12 @@ __device__ __forceinline__ void warp_best(double& v, int& i) {
   }
 }
 
-// One warp per token, everything in 64 bits.
+// One token in 64 bits, with 2 E doubles of scratch.
 template <typename T>
-__global__ void __launch_bounds__(kRouteWarps * 32)
-route_experts_kernel(const T* __restrict__ logits, int64_t stride, const float* __restrict__ bias, int n_tok, int E,
-                     int topk, int sigmoid, int groups, int kept, int top2, int renorm, float scale,
-                     float* __restrict__ weights, int32_t* __restrict__ ids) {
-  pdl_wait();
-  pdl_launch();
-  extern __shared__ double route_sm[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * kRouteWarps + warp;
-  if (t >= n_tok) return;
-  double* p = route_sm + (size_t)warp * 2 * E;  // scores
-  double* v = p + E;                            // what the choice goes by
-  const T* row = logits + (int64_t)t * stride;
-  const bool by_logit = bias == nullptr;
+__device__ __noinline__ void route_exact(const RouteArgs& a, const T* row, int t, double* p) {
+  const int lane = threadIdx.x & 31, E = a.E, topk = a.topk, groups = a.groups;
+  double* v = p + E;  // what the choice goes by
+  const bool by_logit = a.bias == nullptr;
 
   double mx = -INFINITY;
   for (int e = lane; e < E; e += 32) {
@@ -71,16 +81,16 @@ route_experts_kernel(const T* __restrict__ logits, int64_t stride, const float* 
   for (int e = lane; e < E; e += 32) {
     const double x = p[e];
     double s;
-    if (sigmoid) s = 1.0 / (1.0 + exp(-x));
+    if (a.sigmoid) s = 1.0 / (1.0 + exp(-x));
     else s = mx == -INFINITY ? 0.0 : exp(x - mx);
-    v[e] = by_logit ? fmax(x, -(double)FLT_MAX * 2) : (double)clean_bias(bias[e]);
+    v[e] = by_logit ? fmax(x, -(double)FLT_MAX * 2) : (double)clean_bias(a.bias[e]);
     p[e] = s;
     sum += s;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   for (int e = lane; e < E; e += 32) {
-    if (!sigmoid) p[e] = sum > 0.0 ? p[e] / sum : 0.0;
+    if (!a.sigmoid) p[e] = sum > 0.0 ? p[e] / sum : 0.0;
     if (!by_logit) v[e] += p[e];
   }
   __syncwarp();
@@ -93,15 +103,15 @@ route_experts_kernel(const T* __restrict__ logits, int64_t stride, const float* 
     for (int i = 0; i < 8; ++i) {
       const int g = lane + 32 * i;
       if (g >= groups) { rank[i] = -INFINITY; continue; }
-      double a = -INFINITY, b = -INFINITY;
+      double c = -INFINITY, d = -INFINITY;
       for (int j = 0; j < per; ++j) {
-        const double x = (by_logit && top2) ? p[g * per + j] : v[g * per + j];
-        if (x > a) { b = a; a = x; } else if (x > b) b = x;
+        const double x = (by_logit && a.top2) ? p[g * per + j] : v[g * per + j];
+        if (x > c) { d = c; c = x; } else if (x > d) d = x;
       }
-      rank[i] = top2 ? a + b : a;
+      rank[i] = a.top2 ? c + d : c;
     }
     unsigned keep = 0;  // bit i: this lane's group lane + 32 i stays
-    for (int n = 0; n < kept; ++n) {
+    for (int n = 0; n < a.kept; ++n) {
       double bv = -INFINITY;
       int bi = 0x7fffffff;
 #pragma unroll
@@ -130,15 +140,234 @@ route_experts_kernel(const T* __restrict__ logits, int64_t stride, const float* 
     warp_best(bv, bi);
     total += p[bi];
     if (lane == 0) {
-      ids[(int64_t)t * topk + n] = bi;
+      a.ids[(int64_t)t * topk + n] = bi;
       v[bi] = -INFINITY;
     }
     __syncwarp();
   }
   if (lane < topk) {
-    const double w = p[ids[(int64_t)t * topk + lane]];
-    weights[(int64_t)t * topk + lane] = (float)((renorm ? (total > 0.0 ? w / total : 0.0) : w) * (double)scale);
+    const double w = p[a.ids[(int64_t)t * topk + lane]];
+    a.weights[(int64_t)t * topk + lane] = (float)((a.renorm ? (total > 0.0 ? w / total : 0.0) : w) * (double)a.scale);
   }
+}
+
+// unsigned keys in the order of the floats; 0 is below all of them
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
+
+__device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
+
+// lane i's place among the first n lanes' keys, largest first, equal ones by lane
+__device__ __forceinline__ int place_of(uint32_t key, int n) {
+  const int lane = threadIdx.x & 31;
+  int r = 0;
+  for (int j = 0; j < n; ++j) {
+    const uint32_t o = __shfl_sync(0xffffffffu, key, j);
+    r += o > key || (o == key && j < lane);
+  }
+  return r;
+}
+
+// PER: experts of a lane, e = lane + 32 i
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const __grid_constant__ RouteArgs a) {
+  pdl_wait();
+  pdl_launch();
+  extern __shared__ double route_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = a.E;
+  const int t = blockIdx.x * kRouteWarps + warp;
+  if (t >= a.n_tok) return;
+  double* scratch = route_sm + (size_t)warp * (2 * E + 32);
+  const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)t * a.stride;
+  const bool by_logit = a.bias == nullptr, sums = a.groups > 1 && a.top2;
+
+  float x[PER];
+  uint32_t key[PER];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    x[i] = e < E ? clean_logit(logit_of(row + e)) : -INFINITY;
+    key[i] = e < E ? key_of(x[i]) : 0u;
+    mx = fmaxf(mx, x[i]);
+  }
+  float inv = 0.f, top_p = 1.f;  // softmax: 1 / the sum of the exponentials; no score is above top_p
+  if (!a.sigmoid) {
+    mx = warp_max(mx);
+    if (!by_logit || sums || !a.renorm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum += mx == -INFINITY ? 0.f : expf(x[i] - mx);
+      sum = warp_sum(sum);
+      inv = top_p = sum > 0.f ? 1.f / sum : 0.f;
+    }
+  }
+  const auto score = [&](float l) {
+    return a.sigmoid ? sigmoid_of(l) : mx == -INFINITY ? 0.f : expf(l - mx) * inv;
+  };
+  // Errors: a sigmoid is off by a few roundings (2^-21 of it at most), a softmax score by the roundings of its
+  // sum too (32 at most: 2^-19), p + bias by another rounding. Values further apart than `near` are in order.
+  const float rel = a.sigmoid ? 0x1p-21f : 0x1p-19f;
+  float most = 0.f;  // largest |v|
+  if (!by_logit || sums) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = lane + 32 * i;
+      if (e >= E) continue;
+      float v = score(x[i]);
+      if (!by_logit) {
+        v += clean_bias(a.bias[e]);
+        key[i] = key_of(v);
+      }
+      most = fmaxf(most, fabsf(v));
+      x[i] = v;  // the groups' sums are of these
+    }
+    most = warp_max(most);
+  }
+  const float near = 2.f * (rel * top_p + 0x1p-23f * most);
+  bool exact = !(most < 0x1p100f);  // sums of such would overflow
+
+  if (a.groups > 1 && a.groups <= 32 && !exact) {
+    const int per = E / a.groups;
+    uint32_t* gk = reinterpret_cast<uint32_t*>(scratch);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < E) gk[lane + 32 * i] = sums ? key_of(x[i]) : key[i];
+    __syncwarp();
+    uint32_t rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      uint32_t c = 0, d = 0;  // the lane's two largest
+      for (int j = lane; j < per; j += 32) {
+        const uint32_t o = gk[g * per + j];
+        d = max(d, min(c, o));
+        c = max(c, o);
+      }
+      uint32_t m = __reduce_max_sync(0xffffffffu, c);
+      if (a.top2) {
+        const int first = __ffs(__ballot_sync(0xffffffffu, c == m)) - 1;
+        const uint32_t n = __reduce_max_sync(0xffffffffu, lane == first ? d : c);
+        m = key_of(of_key(m) + of_key(n));
+      }
+      if (lane == g) rank = m;
+    }
+    const int among = place_of(rank, a.groups), place = lane < a.groups ? among : 99;
+    const unsigned keep = __ballot_sync(0xffffffffu, place < a.kept);
+    if (a.kept < a.groups && (sums || !by_logit)) {
+      // the last group that stays and the first that does not
+      const int in = __ffs(__ballot_sync(0xffffffffu, place == a.kept - 1)) - 1;
+      const int out = __ffs(__ballot_sync(0xffffffffu, place == a.kept)) - 1;
+      const float u = of_key(__shfl_sync(0xffffffffu, rank, in)), w = of_key(__shfl_sync(0xffffffffu, rank, out));
+      exact = !(u - w > 2.f * near + 0x1p-22f * fabsf(u));
+    }
+    const int magic = ((1 << 20) + per - 1) / per;  // e / per for e < 512
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (!((keep >> (((lane + 32 * i) * magic) >> 20)) & 1)) key[i] = 0;
+    __syncwarp();
+  } else if (a.groups > 32) {
+    exact = true;
+  }
+  if (exact) {
+    route_exact<T>(a, row, t, scratch);
+    return;
+  }
+
+  // the (k + 1)-th largest of the lanes' maxima
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) top = max(top, key[i]);
+  uint32_t sorted = top;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, sorted, o);
+      const bool larger = ((lane & size) == 0) == ((lane & o) == 0);  // descending in the end
+      sorted = larger ? max(sorted, other) : min(sorted, other);
+    }
+  const uint32_t floor_key = a.topk < 32 ? max(__shfl_sync(0xffffffffu, sorted, a.topk & 31), 1u) : 1u;
+  uint32_t* ck = reinterpret_cast<uint32_t*>(scratch);
+  uint32_t* ce = ck + 32;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool in = key[i] >= floor_key;
+    const unsigned m = __ballot_sync(0xffffffffu, in);
+    const int at = n + __popc(m & ((1u << lane) - 1));
+    if (in && at < 32) ck[at] = key[i], ce[at] = lane + 32 * i;
+    n += __popc(m);
+  }
+  __syncwarp();
+  // chosen: lane r has the r-th
+  uint32_t ckey = 0;
+  int cid = 0;
+  if (n <= 32) {
+    const uint32_t mine = lane < n ? ck[lane] : 0u;
+    const int id = lane < n ? (int)ce[lane] : 0;
+    const int r = place_of(mine, n);
+    __syncwarp();
+    if (lane < n) ck[r] = mine, ce[r] = id;
+    __syncwarp();
+    if (lane < n) ckey = ck[lane], cid = (int)ce[lane];
+  } else {
+    for (int k = 0; k <= a.topk && k < 32; ++k) {
+      uint32_t b = 0;
+      int bi = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (key[i] > b) b = key[i], bi = i;
+      const uint32_t m = __reduce_max_sync(0xffffffffu, b);
+      const uint32_t e = __reduce_min_sync(0xffffffffu, b == m ? (uint32_t)(lane + 32 * bi) : 0xffffffffu);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if ((uint32_t)(lane + 32 * i) == e) key[i] = 0;
+      if (lane == k) ckey = m, cid = (int)e;
+    }
+  }
+  if (!by_logit) {
+    const float v = of_key(ckey), next = of_key(__shfl_down_sync(0xffffffffu, ckey, 1));
+    // the last candidate has nothing behind it; with 32 chosen the 33rd is not known
+    const bool behind = lane < a.topk && lane + 1 < min(n, 32);
+    const bool unsure = a.topk == 32 && E > 32;
+    if (unsure || __any_sync(0xffffffffu, behind && !(v - next > near))) {
+      __syncwarp();
+      route_exact<T>(a, row, t, scratch);
+      return;
+    }
+  }
+  float p = 0.f;
+  if (lane < a.topk) {
+    const float l = clean_logit(logit_of(row + cid));
+    p = a.sigmoid ? sigmoid_of(l) : mx == -INFINITY ? 0.f : expf(l - mx) * (inv > 0.f ? inv : 1.f);
+  }
+  if (a.renorm) {
+    const float total = warp_sum(p);
+    if (!(total > 0x1p-80f)) {  // scores at the end of fp32's range (or zero)
+      __syncwarp();
+      route_exact<T>(a, row, t, scratch);
+      return;
+    }
+    p /= total;
+  }
+  if (lane < a.topk) {
+    a.weights[(int64_t)t * a.topk + lane] = p * a.scale;
+    a.ids[(int64_t)t * a.topk + lane] = cid;
+  }
+}
+
+template <typename T>
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t s) {
+  const dim3 grid((a.n_tok + kRouteWarps - 1) / kRouteWarps), block(kRouteWarps * 32);
+  const size_t smem = (size_t)kRouteWarps * (2 * a.E + 32) * sizeof(double);
+  const int per = (a.E + 31) / 32;
+  if (per <= 1) return msgl_launch(route_experts_kernel<T, 1>, grid, block, smem, s, 1, a);
+  if (per <= 2) return msgl_launch(route_experts_kernel<T, 2>, grid, block, smem, s, 1, a);
+  if (per <= 4) return msgl_launch(route_experts_kernel<T, 4>, grid, block, smem, s, 1, a);
+  if (per <= 8) return msgl_launch(route_experts_kernel<T, 8>, grid, block, smem, s, 1, a);
+  return msgl_launch(route_experts_kernel<T, 16>, grid, block, smem, s, 1, a);
 }
 
 }  // namespace
@@ -148,13 +377,7 @@ extern "C" int msgl_route_experts(const void* logits, int is_fp32, int64_t strid
                                   float* weights, int32_t* ids, cudaStream_t s) {
   if (n_tok == 0) return 0;
   if (E < 1 || E > kRouteMaxE || topk < 1 || topk > 32 || groups < 1 || groups > 256 || E % groups != 0) return 3;
-  const dim3 grid((n_tok + kRouteWarps - 1) / kRouteWarps), block(kRouteWarps * 32);
-  const size_t smem = (size_t)kRouteWarps * 2 * E * sizeof(double);
-  const cudaError_t e =
-      is_fp32 ? msgl_launch(route_experts_kernel<float>, grid, block, smem, s, 1, (const float*)logits, stride, bias,
-                            n_tok, E, topk, sigmoid, groups, kept, top2, renorm, scale, weights, ids)
-              : msgl_launch(route_experts_kernel<__nv_bfloat16>, grid, block, smem, s, 1,
-                            (const __nv_bfloat16*)logits, stride, bias, n_tok, E, topk, sigmoid, groups, kept, top2,
-                            renorm, scale, weights, ids);
+  const RouteArgs a = {logits, stride, bias, n_tok, E, topk, sigmoid, groups, kept, top2, renorm, scale, weights, ids};
+  const cudaError_t e = is_fp32 ? launch_route<float>(a, s) : launch_route<__nv_bfloat16>(a, s);
   return e == cudaSuccess ? 0 : 4;
 }
