@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kRouteWarps = 4;
 constexpr int kRouteMaxE = 512;
+constexpr int kRouteCtas = 8;  // per SM: what the registers hold
 
 struct RouteArgs {
   const void* logits;
@@ -49,7 +50,8 @@ template <>
 __device__ __forceinline__ float logit_of<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
 // (+ 0.f: -0 and 0 are equal, and so are their keys)
-__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX) + 0.f; }
+// fmaxf takes the other operand of a NaN
+__device__ __forceinline__ float clean_logit(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX) + 0.f; }
 __device__ __forceinline__ float clean_bias(float b) { return b != b ? -FLT_MAX : fmaxf(fminf(b, FLT_MAX), -FLT_MAX); }
 
 // largest value of the warp's lanes, then the lowest index that has it
@@ -154,7 +156,7 @@ __device__ __noinline__ void route_exact(const RouteArgs& a, const T* row, int t
 // unsigned keys in the order of the floats; 0 is below all of them
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x);
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
@@ -171,27 +173,18 @@ __device__ __forceinline__ int place_of(uint32_t key, int n) {
   return r;
 }
 
-// PER: experts of a lane, e = lane + 32 i
-template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const __grid_constant__ RouteArgs a) {
-  pdl_wait();
-  pdl_launch();
-  extern __shared__ double route_sm[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = a.E;
-  const int t = blockIdx.x * kRouteWarps + warp;
-  if (t >= a.n_tok) return;
-  double* scratch = route_sm + (size_t)warp * (2 * E + 32);
-  const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)t * a.stride;
-  const bool by_logit = a.bias == nullptr, sums = a.groups > 1 && a.top2;
-
-  float x[PER];
+// One token. x: the lane's logits, of experts lane + 32 i; FULL: there are exactly 32 PER.
+template <typename T, int PER, bool GROUPS, bool FULL>
+__device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, int t, double* scratch, float (&x)[PER]) {
+  const int lane = threadIdx.x & 31, E = FULL ? 32 * PER : a.E;
+  const bool by_logit = a.bias == nullptr, sums = GROUPS && a.top2;
   uint32_t key[PER];
   float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int e = lane + 32 * i;
-    x[i] = e < E ? clean_logit(logit_of(row + e)) : -INFINITY;
-    key[i] = e < E ? key_of(x[i]) : 0u;
+    const bool in = FULL || lane + 32 * i < E;
+    x[i] = in ? clean_logit(x[i]) : -INFINITY;
+    key[i] = in ? key_of(x[i]) : 0u;
     mx = fmaxf(mx, x[i]);
   }
   float inv = 0.f, top_p = 1.f;  // softmax: 1 / the sum of the exponentials; no score is above top_p
@@ -216,7 +209,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = lane + 32 * i;
-      if (e >= E) continue;
+      if (!FULL && e >= E) continue;
       float v = score(x[i]);
       if (!by_logit) {
         v += clean_bias(a.bias[e]);
@@ -230,28 +223,52 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
   const float near = 2.f * (rel * top_p + 0x1p-23f * most);
   bool exact = !(most < 0x1p100f);  // sums of such would overflow
 
-  if (a.groups > 1 && a.groups <= 32 && !exact) {
+  if (GROUPS && a.groups > 32) exact = true;
+  if (GROUPS && !exact) {
     const int per = E / a.groups;
-    uint32_t* gk = reinterpret_cast<uint32_t*>(scratch);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i < E) gk[lane + 32 * i] = sums ? key_of(x[i]) : key[i];
-    __syncwarp();
     uint32_t rank = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      uint32_t c = 0, d = 0;  // the lane's two largest
-      for (int j = lane; j < per; j += 32) {
-        const uint32_t o = gk[g * per + j];
-        d = max(d, min(c, o));
-        c = max(c, o);
-      }
+    // c, d: the lane's two largest of a group
+    const auto rank_of = [&](uint32_t c, uint32_t d) {
       uint32_t m = __reduce_max_sync(0xffffffffu, c);
       if (a.top2) {
         const int first = __ffs(__ballot_sync(0xffffffffu, c == m)) - 1;
         const uint32_t n = __reduce_max_sync(0xffffffffu, lane == first ? d : c);
         m = key_of(of_key(m) + of_key(n));
       }
-      if (lane == g) rank = m;
+      return m;
+    };
+    if (per % 32 == 0) {  // whole registers
+      uint32_t c = 0, d = 0;
+      int g = 0, end = per;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t o = by_logit && sums ? key_of(x[i]) : key[i];
+        d = max(d, min(c, o));
+        c = max(c, o);
+        if (32 * (i + 1) == end) {
+          const uint32_t m = rank_of(c, d);
+          if (lane == g) rank = m;
+          ++g, end += per;
+          c = d = 0;
+        }
+      }
+    } else {
+      uint32_t* gk = reinterpret_cast<uint32_t*>(scratch);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (FULL || lane + 32 * i < E) gk[lane + 32 * i] = by_logit && sums ? key_of(x[i]) : key[i];
+      __syncwarp();
+      for (int g = 0; g < a.groups; ++g) {
+        uint32_t c = 0, d = 0;
+        for (int j = lane; j < per; j += 32) {
+          const uint32_t o = gk[g * per + j];
+          d = max(d, min(c, o));
+          c = max(c, o);
+        }
+        const uint32_t m = rank_of(c, d);
+        if (lane == g) rank = m;
+      }
+      __syncwarp();
     }
     const int among = place_of(rank, a.groups), place = lane < a.groups ? among : 99;
     const unsigned keep = __ballot_sync(0xffffffffu, place < a.kept);
@@ -266,9 +283,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (!((keep >> (((lane + 32 * i) * magic) >> 20)) & 1)) key[i] = 0;
-    __syncwarp();
-  } else if (a.groups > 32) {
-    exact = true;
   }
   if (exact) {
     route_exact<T>(a, row, t, scratch);
@@ -358,16 +372,54 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
   }
 }
 
+// PER: experts of a lane. The warps take the tokens in turn; a token's logits are on their way while the one before
+// it is done.
+template <typename T, int PER, bool GROUPS, bool FULL>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const __grid_constant__ RouteArgs a) {
+  pdl_wait();
+  pdl_launch();
+  extern __shared__ double route_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = FULL ? 32 * PER : a.E;
+  double* scratch = route_sm + (size_t)warp * (2 * E + 32);
+  const T* base = reinterpret_cast<const T*>(a.logits);
+  const int step = gridDim.x * kRouteWarps;
+  float next[PER];
+  const auto fetch = [&](int t) {
+    const T* row = base + (int64_t)t * a.stride + lane;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) next[i] = FULL || lane + 32 * i < E ? logit_of(row + 32 * i) : 0.f;
+  };
+  int t = blockIdx.x * kRouteWarps + warp;
+  if (t < a.n_tok) fetch(t);
+  for (; t < a.n_tok; t += step) {
+    float x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = next[i];
+    if (t + step < a.n_tok) fetch(t + step);
+    route_token<T, PER, GROUPS, FULL>(a, base + (int64_t)t * a.stride, t, scratch, x);
+    __syncwarp();
+  }
+}
+
+template <typename T, int PER>
+cudaError_t launch_route_per(const RouteArgs& a, cudaStream_t s) {
+  const size_t smem = (size_t)kRouteWarps * (2 * a.E + 32) * sizeof(double);
+  const int ctas = (a.n_tok + kRouteWarps - 1) / kRouteWarps, most = msgl_num_sms() * kRouteCtas;
+  const dim3 grid(ctas < most ? ctas : most), block(kRouteWarps * 32);
+  if (a.E == 32 * PER)
+    return a.groups > 1 ? msgl_launch(route_experts_kernel<T, PER, true, true>, grid, block, smem, s, 1, a)
+                        : msgl_launch(route_experts_kernel<T, PER, false, true>, grid, block, smem, s, 1, a);
+  return a.groups > 1 ? msgl_launch(route_experts_kernel<T, PER, true, false>, grid, block, smem, s, 1, a)
+                      : msgl_launch(route_experts_kernel<T, PER, false, false>, grid, block, smem, s, 1, a);
+}
+
 template <typename T>
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t s) {
-  const dim3 grid((a.n_tok + kRouteWarps - 1) / kRouteWarps), block(kRouteWarps * 32);
-  const size_t smem = (size_t)kRouteWarps * (2 * a.E + 32) * sizeof(double);
-  const int per = (a.E + 31) / 32;
-  if (per <= 1) return msgl_launch(route_experts_kernel<T, 1>, grid, block, smem, s, 1, a);
-  if (per <= 2) return msgl_launch(route_experts_kernel<T, 2>, grid, block, smem, s, 1, a);
-  if (per <= 4) return msgl_launch(route_experts_kernel<T, 4>, grid, block, smem, s, 1, a);
-  if (per <= 8) return msgl_launch(route_experts_kernel<T, 8>, grid, block, smem, s, 1, a);
-  return msgl_launch(route_experts_kernel<T, 16>, grid, block, smem, s, 1, a);
+  if (a.E <= 32) return launch_route_per<T, 1>(a, s);
+  if (a.E <= 64) return launch_route_per<T, 2>(a, s);
+  if (a.E <= 128) return launch_route_per<T, 4>(a, s);
+  if (a.E <= 256) return launch_route_per<T, 8>(a, s);
+  return launch_route_per<T, 16>(a, s);
 }
 
 }  // namespace
