@@ -37,6 +37,7 @@ struct RouteArgs {
   int64_t stride;
   const float* bias;
   int n_tok, E, topk, sigmoid, groups, kept, top2, renorm;
+  int per, magic;  // experts of a group, and 2^20 / per rounded up
   float scale;
   float* weights;
   int32_t* ids;
@@ -162,14 +163,20 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^
 
 __device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
 
-// lane i's place among the first n lanes' keys, largest first, equal ones by lane
+// e^x on the MUFU unit, for the choice: off by 2^-22 and the rounding of x log2 e, which |x| <= 16 makes 2^-20 of the
+// value at most and a smaller part of the largest score where |x| is larger
+__device__ __forceinline__ float exp_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
+// the lane's place among the first n lanes' keys, largest first, equal ones by lane; lanes from n on have 0
 __device__ __forceinline__ int place_of(uint32_t key, int n) {
-  const int lane = threadIdx.x & 31;
-  int r = 0;
-  for (int j = 0; j < n; ++j) {
-    const uint32_t o = __shfl_sync(0xffffffffu, key, j);
-    r += o > key || (o == key && j < lane);
-  }
+  int r = __popc(__match_any_sync(0xffffffffu, key) & ((1u << (threadIdx.x & 31)) - 1));
+  for (int j = 0; j < n; j += 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r += __shfl_sync(0xffffffffu, key, j + i) > key;
   return r;
 }
 
@@ -192,40 +199,46 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
     mx = warp_max(mx);
     if (!by_logit || sums || !a.renorm) {
       float sum = 0.f;
+      const float m = mx == -INFINITY ? 0.f : mx;  // then every exponential is zero
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += mx == -INFINITY ? 0.f : expf(x[i] - mx);
+      for (int i = 0; i < PER; ++i) sum += exp_fast(x[i] - m);
       sum = warp_sum(sum);
       inv = top_p = sum > 0.f ? 1.f / sum : 0.f;
     }
   }
-  const auto score = [&](float l) {
-    return a.sigmoid ? sigmoid_of(l) : mx == -INFINITY ? 0.f : expf(l - mx) * inv;
-  };
-  // Errors: a sigmoid is off by a few roundings (2^-21 of it at most), a softmax score by the roundings of its
-  // sum too (32 at most: 2^-19), p + bias by another rounding. Values further apart than `near` are in order.
-  const float rel = a.sigmoid ? 0x1p-21f : 0x1p-19f;
+  // Errors: a sigmoid is off by 2^-20 and a few roundings (2^-19 of the largest possible, 1), a softmax score by
+  // the roundings of its sum too (32 at most: 2^-18 of the largest, top_p), p + bias by another rounding. Values
+  // further apart than `near` are in order.
+  const float rel = a.sigmoid ? 0x1p-19f : 0x1p-18f;
   float most = 0.f;  // largest |v|
   if (!by_logit || sums) {
+    if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = lane + 32 * i;
-      if (!FULL && e >= E) continue;
-      float v = score(x[i]);
-      if (!by_logit) {
-        v += clean_bias(a.bias[e]);
-        key[i] = key_of(v);
-      }
-      most = fmaxf(most, fabsf(v));
-      x[i] = v;  // the groups' sums are of these
+      for (int i = 0; i < PER; ++i) x[i] = __fdividef(1.f, 1.f + exp_fast(-x[i]));
+    } else {
+      const float m = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = exp_fast(x[i] - m) * inv;
     }
-    most = warp_max(most);
+    if (!by_logit) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (FULL || lane + 32 * i < E) {
+          x[i] += clean_bias(__ldg(a.bias + lane + 32 * i));
+          key[i] = key_of(x[i]);
+          most = fmaxf(most, fabsf(x[i]));
+        }
+      most = warp_max(most);
+    } else {
+      most = top_p;
+    }
   }
   const float near = 2.f * (rel * top_p + 0x1p-23f * most);
   bool exact = !(most < 0x1p100f);  // sums of such would overflow
 
   if (GROUPS && a.groups > 32) exact = true;
   if (GROUPS && !exact) {
-    const int per = E / a.groups;
+    const int per = a.per;
     uint32_t rank = 0;
     // c, d: the lane's two largest of a group
     const auto rank_of = [&](uint32_t c, uint32_t d) {
@@ -247,7 +260,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
         c = max(c, o);
         if (32 * (i + 1) == end) {
           const uint32_t m = rank_of(c, d);
-          if (lane == g) rank = m;
+          if (lane == g && g < a.groups) rank = m;  // registers behind the last group hold nothing
           ++g, end += per;
           c = d = 0;
         }
@@ -279,10 +292,9 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
       const float u = of_key(__shfl_sync(0xffffffffu, rank, in)), w = of_key(__shfl_sync(0xffffffffu, rank, out));
       exact = !(u - w > 2.f * near + 0x1p-22f * fabsf(u));
     }
-    const int magic = ((1 << 20) + per - 1) / per;  // e / per for e < 512
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (!((keep >> (((lane + 32 * i) * magic) >> 20)) & 1)) key[i] = 0;
+    for (int i = 0; i < PER; ++i)  // a.magic: e / per for e < 512
+      if (!((keep >> (((lane + 32 * i) * a.magic) >> 20)) & 1)) key[i] = 0;
   }
   if (exact) {
     route_exact<T>(a, row, t, scratch);
@@ -303,15 +315,13 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
       sorted = larger ? max(sorted, other) : min(sorted, other);
     }
   const uint32_t floor_key = a.topk < 32 ? max(__shfl_sync(0xffffffffu, sorted, a.topk & 31), 1u) : 1u;
-  uint32_t* ck = reinterpret_cast<uint32_t*>(scratch);
-  uint32_t* ce = ck + 32;
+  uint2* cand = reinterpret_cast<uint2*>(scratch);  // {key, expert}, room for all of them
   int n = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const bool in = key[i] >= floor_key;
     const unsigned m = __ballot_sync(0xffffffffu, in);
-    const int at = n + __popc(m & ((1u << lane) - 1));
-    if (in && at < 32) ck[at] = key[i], ce[at] = lane + 32 * i;
+    if (in) cand[n + __popc(m & ((1u << lane) - 1))] = make_uint2(key[i], lane + 32 * i);
     n += __popc(m);
   }
   __syncwarp();
@@ -319,13 +329,12 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
   uint32_t ckey = 0;
   int cid = 0;
   if (n <= 32) {
-    const uint32_t mine = lane < n ? ck[lane] : 0u;
-    const int id = lane < n ? (int)ce[lane] : 0;
-    const int r = place_of(mine, n);
+    const uint2 mine = lane < n ? cand[lane] : make_uint2(0, 0);
+    const int r = place_of(mine.x, n);
     __syncwarp();
-    if (lane < n) ck[r] = mine, ce[r] = id;
+    if (lane < n) cand[r] = mine;
     __syncwarp();
-    if (lane < n) ckey = ck[lane], cid = (int)ce[lane];
+    if (lane < n) ckey = cand[lane].x, cid = (int)cand[lane].y;
   } else {
     for (int k = 0; k <= a.topk && k < 32; ++k) {
       uint32_t b = 0;
@@ -364,7 +373,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
       route_exact<T>(a, row, t, scratch);
       return;
     }
-    p /= total;
+    p = __fdividef(p, total);
   }
   if (lane < a.topk) {
     a.weights[(int64_t)t * a.topk + lane] = p * a.scale;
@@ -429,7 +438,9 @@ extern "C" int msgl_route_experts(const void* logits, int is_fp32, int64_t strid
                                   float* weights, int32_t* ids, cudaStream_t s) {
   if (n_tok == 0) return 0;
   if (E < 1 || E > kRouteMaxE || topk < 1 || topk > 32 || groups < 1 || groups > 256 || E % groups != 0) return 3;
-  const RouteArgs a = {logits, stride, bias, n_tok, E, topk, sigmoid, groups, kept, top2, renorm, scale, weights, ids};
+  const int per = E / groups;
+  const RouteArgs a = {logits, stride, bias, n_tok, E, topk, sigmoid, groups, kept, top2, renorm,
+                       per, ((1 << 20) + per - 1) / per, scale, weights, ids};
   const cudaError_t e = is_fp32 ? launch_route<float>(a, s) : launch_route<__nv_bfloat16>(a, s);
   return e == cudaSuccess ? 0 : 4;
 }
