@@ -30,14 +30,14 @@ namespace {
 
 constexpr int kRouteWarps = 4;
 constexpr int kRouteMaxE = 512;
-constexpr int kRouteCtas = 8;  // per SM: what the registers hold
+constexpr int kRouteCtas = 6;  // per SM: what the registers hold
 
 struct RouteArgs {
   const void* logits;
   int64_t stride;
   const float* bias;
   int n_tok, E, topk, sigmoid, groups, kept, top2, renorm;
-  int per, magic;  // experts of a group, and 2^20 / per rounded up
+  int per, lanes, log_lanes;  // experts of a group, lanes of a group and their logarithm
   float scale;
   float* weights;
   int32_t* ids;
@@ -180,9 +180,18 @@ __device__ __forceinline__ int place_of(uint32_t key, int n) {
   return r;
 }
 
+// what the lane's experts keep over the tokens: their biases, and with groups (e = lane + 32 i, g its group) the place
+// of their values in the scratch, e + g L, and the first of the group's lanes, g L
+template <int PER, bool GROUPS>
+struct LaneExperts {
+  float bias[PER];
+  int at[GROUPS ? PER : 1], first[GROUPS ? PER : 1];
+};
+
 // One token. x: the lane's logits, of experts lane + 32 i; FULL: there are exactly 32 PER.
 template <typename T, int PER, bool GROUPS, bool FULL>
-__device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, int t, double* scratch, float (&x)[PER]) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExperts<PER, GROUPS>& le, const T* row, int t, double* scratch,
+                                            float (&x)[PER]) {
   const int lane = threadIdx.x & 31, E = FULL ? 32 * PER : a.E;
   const bool by_logit = a.bias == nullptr, sums = GROUPS && a.top2;
   uint32_t key[PER];
@@ -224,7 +233,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
 #pragma unroll
       for (int i = 0; i < PER; ++i)
         if (FULL || lane + 32 * i < E) {
-          x[i] += clean_bias(__ldg(a.bias + lane + 32 * i));
+          x[i] += le.bias[i];
           key[i] = key_of(x[i]);
           most = fmaxf(most, fabsf(x[i]));
         }
@@ -238,63 +247,48 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
 
   if (GROUPS && a.groups > 32) exact = true;
   if (GROUPS && !exact) {
-    const int per = a.per;
-    uint32_t rank = 0;
-    // c, d: the lane's two largest of a group
-    const auto rank_of = [&](uint32_t c, uint32_t d) {
-      uint32_t m = __reduce_max_sync(0xffffffffu, c);
-      if (a.top2) {
-        const int first = __ffs(__ballot_sync(0xffffffffu, c == m)) - 1;
-        const uint32_t n = __reduce_max_sync(0xffffffffu, lane == first ? d : c);
-        m = key_of(of_key(m) + of_key(n));
-      }
-      return m;
-    };
-    if (per % 32 == 0) {  // whole registers
-      uint32_t c = 0, d = 0;
-      int g = 0, end = per;
+    // L lanes share a group: each keeps its two largest, and they merge. The groups lie L words further apart
+    // than their size, so that groups of 32 do not meet in the banks.
+    const int per = a.per, L = a.lanes;
+    uint32_t* gk = reinterpret_cast<uint32_t*>(scratch);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t o = by_logit && sums ? key_of(x[i]) : key[i];
+    for (int i = 0; i < PER; ++i) {
+      if (FULL || lane + 32 * i < E) gk[le.at[i]] = by_logit && sums ? key_of(x[i]) : key[i];
+    }
+    __syncwarp();
+    const int g = lane >> a.log_lanes, q = lane & (L - 1);
+    uint32_t c = 0, d = 0;
+    if (g < a.groups)
+#pragma unroll 4
+      for (int j = q; j < per; j += L) {
+        const uint32_t o = gk[g * (per + L) + j];
         d = max(d, min(c, o));
         c = max(c, o);
-        if (32 * (i + 1) == end) {
-          const uint32_t m = rank_of(c, d);
-          if (lane == g && g < a.groups) rank = m;  // registers behind the last group hold nothing
-          ++g, end += per;
-          c = d = 0;
-        }
       }
-    } else {
-      uint32_t* gk = reinterpret_cast<uint32_t*>(scratch);
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (FULL || lane + 32 * i < E) gk[lane + 32 * i] = by_logit && sums ? key_of(x[i]) : key[i];
-      __syncwarp();
-      for (int g = 0; g < a.groups; ++g) {
-        uint32_t c = 0, d = 0;
-        for (int j = lane; j < per; j += 32) {
-          const uint32_t o = gk[g * per + j];
-          d = max(d, min(c, o));
-          c = max(c, o);
-        }
-        const uint32_t m = rank_of(c, d);
-        if (lane == g) rank = m;
-      }
-      __syncwarp();
+    for (int o = 1; o < L; o <<= 1) {
+      const uint32_t c2 = __shfl_xor_sync(0xffffffffu, c, o), d2 = __shfl_xor_sync(0xffffffffu, d, o);
+      d = max(max(d, d2), min(c, c2));
+      c = max(c, c2);
     }
-    const int among = place_of(rank, a.groups), place = lane < a.groups ? among : 99;
-    const unsigned keep = __ballot_sync(0xffffffffu, place < a.kept);
+    // every lane of a group has its rank
+    const uint32_t rank = g >= a.groups ? 0u : a.top2 ? key_of(of_key(c) + of_key(d)) : c;
+    int place = 0;
+    for (int j = 0; j < a.groups; ++j) {
+      const uint32_t o = __shfl_sync(0xffffffffu, rank, j * L);
+      place += o > rank || (o == rank && j < g);
+    }
+    const unsigned stay = __ballot_sync(0xffffffffu, place < a.kept && g < a.groups);
     if (a.kept < a.groups && (sums || !by_logit)) {
       // the last group that stays and the first that does not
-      const int in = __ffs(__ballot_sync(0xffffffffu, place == a.kept - 1)) - 1;
-      const int out = __ffs(__ballot_sync(0xffffffffu, place == a.kept)) - 1;
+      const int in = __ffs(__ballot_sync(0xffffffffu, place == a.kept - 1 && g < a.groups)) - 1;
+      const int out = __ffs(__ballot_sync(0xffffffffu, place == a.kept && g < a.groups)) - 1;
       const float u = of_key(__shfl_sync(0xffffffffu, rank, in)), w = of_key(__shfl_sync(0xffffffffu, rank, out));
       exact = !(u - w > 2.f * near + 0x1p-22f * fabsf(u));
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i)  // a.magic: e / per for e < 512
-      if (!((keep >> (((lane + 32 * i) * a.magic) >> 20)) & 1)) key[i] = 0;
+    for (int i = 0; i < PER; ++i)
+      if (!((stay >> le.first[i]) & 1)) key[i] = 0;
+    __syncwarp();
   }
   if (exact) {
     route_exact<T>(a, row, t, scratch);
@@ -384,7 +378,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const T* row, in
 // PER: experts of a lane. The warps take the tokens in turn; a token's logits are on their way while the one before
 // it is done.
 template <typename T, int PER, bool GROUPS, bool FULL>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const __grid_constant__ RouteArgs a) {
+__global__ void __launch_bounds__(kRouteWarps * 32, PER <= 8 ? kRouteCtas : 3) route_experts_kernel(const __grid_constant__ RouteArgs a) {
   pdl_wait();
   pdl_launch();
   extern __shared__ double route_sm[];
@@ -393,6 +387,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
   const T* base = reinterpret_cast<const T*>(a.logits);
   const int step = gridDim.x * kRouteWarps;
   float next[PER];
+  LaneExperts<PER, GROUPS> le;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    le.bias[i] = a.bias != nullptr && e < E ? clean_bias(__ldg(a.bias + e)) : 0.f;
+    if constexpr (GROUPS) le.first[i] = e / a.per * a.lanes & 31, le.at[i] = e + e / a.per * a.lanes;
+  }
   const auto fetch = [&](int t) {
     const T* row = base + (int64_t)t * a.stride + lane;
 #pragma unroll
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_experts_kernel(const _
 #pragma unroll
     for (int i = 0; i < PER; ++i) x[i] = next[i];
     if (t + step < a.n_tok) fetch(t + step);
-    route_token<T, PER, GROUPS, FULL>(a, base + (int64_t)t * a.stride, t, scratch, x);
+    route_token<T, PER, GROUPS, FULL>(a, le, base + (int64_t)t * a.stride, t, scratch, x);
     __syncwarp();
   }
 }
@@ -439,8 +440,10 @@ extern "C" int msgl_route_experts(const void* logits, int is_fp32, int64_t strid
   if (n_tok == 0) return 0;
   if (E < 1 || E > kRouteMaxE || topk < 1 || topk > 32 || groups < 1 || groups > 256 || E % groups != 0) return 3;
   const int per = E / groups;
+  int log_lanes = 5;
+  while (log_lanes > 0 && (groups << log_lanes) > 32) --log_lanes;
   const RouteArgs a = {logits, stride, bias, n_tok, E, topk, sigmoid, groups, kept, top2, renorm,
-                       per, ((1 << 20) + per - 1) / per, scale, weights, ids};
+                       per, 1 << log_lanes, log_lanes, scale, weights, ids};
   const cudaError_t e = is_fp32 ? launch_route<float>(a, s) : launch_route<__nv_bfloat16>(a, s);
   return e == cudaSuccess ? 0 : 4;
 }
