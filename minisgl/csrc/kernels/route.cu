@@ -12,9 +12,10 @@
 // lowest), so every v is finite and the order is total: that of 64-bit arithmetic.
 //
 // One warp per token. The choice is made in fp32, with a bound on its errors: where two values that the
-// choice depends on are nearer than that (about one row in a thousand), the row is done again in 64 bits;
-// without a bias the logits themselves decide and nothing is near. Doing every row in 64 bits took 65 us
-// at 16384 x 256 with groups.
+// choice depends on are nearer than that (a few rows in a thousand), the candidates or the groups are looked at
+// again in 64 bits; without a bias the logits themselves decide and nothing is near. 16384 tokens x 256
+// experts, 8 of them, fp32 logits: 13 us softmax, 26 us with sigmoid scores, bias and groups, 700 to 1000
+// instructions a token, against 2.8 us for the bytes; every row in 64 bits took 65 us.
 //
 // Top k: the (k + 1)-th largest of the lanes' maxima (a sort of 32 keys across the warp) bounds the
 // (k + 1)-th largest value from below; the few values at or above it are gathered, a lane each, and ranked by
@@ -30,7 +31,8 @@ namespace {
 
 constexpr int kRouteWarps = 4;
 constexpr int kRouteMaxE = 512;
-constexpr int kRouteCtas = 6;  // per SM: what the registers hold
+// CTAs per SM: more would spill registers
+__host__ __device__ constexpr int route_ctas(bool groups) { return groups ? 4 : 6; }
 
 struct RouteArgs {
   const void* logits;
@@ -180,6 +182,53 @@ __device__ __forceinline__ int place_of(uint32_t key, int n) {
   return r;
 }
 
+// e^(l - mx) over a row, and an expert's score + bias, in 64 bits
+template <typename T>
+__device__ __noinline__ double sum_exact(const T* row, int E, float mx) {
+  double sum = 0.0;
+  if (mx != -INFINITY)
+    for (int e = threadIdx.x & 31; e < E; e += 32) sum += exp((double)clean_logit(logit_of(row + e)) - mx);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+template <typename T>
+__device__ __noinline__ double value_exact(const RouteArgs& a, const T* row, int e, float mx, double sum) {
+  const double l = clean_logit(logit_of(row + e));
+  const double p = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : sum > 0.0 ? exp(l - mx) / sum : 0.0;
+  return a.bias == nullptr ? p : p + clean_bias(a.bias[e]);
+}
+
+// The groups that stay (bit g << log_lanes), from scores in 64 bits; v: E doubles of scratch.
+template <typename T>
+__device__ __noinline__ unsigned groups_exact(const RouteArgs& a, const T* row, float mx, double* v) {
+  const int lane = threadIdx.x & 31, L = a.lanes, g = lane >> a.log_lanes;
+  const double sum = a.sigmoid ? 0.0 : sum_exact(row, a.E, mx);
+  __syncwarp();
+  for (int e = lane; e < a.E; e += 32) v[e] = value_exact(a, row, e, mx, sum);
+  __syncwarp();
+  double c = -INFINITY, d = -INFINITY;
+  if (g < a.groups)
+    for (int j = lane & (L - 1); j < a.per; j += L) {
+      const double o = v[g * a.per + j];
+      d = fmax(d, fmin(c, o));
+      c = fmax(c, o);
+    }
+  for (int o = 1; o < L; o <<= 1) {
+    const double c2 = __shfl_xor_sync(0xffffffffu, c, o), d2 = __shfl_xor_sync(0xffffffffu, d, o);
+    d = fmax(fmax(d, d2), fmin(c, c2));
+    c = fmax(c, c2);
+  }
+  const double rank = a.top2 ? c + d : c;
+  int place = 0;
+  for (int j = 0; j < a.groups; ++j) {
+    const double o = __shfl_sync(0xffffffffu, rank, j * L);
+    place += o > rank || (o == rank && j < g);
+  }
+  __syncwarp();
+  return __ballot_sync(0xffffffffu, place < a.kept && g < a.groups);
+}
+
 // what the lane's experts keep over the tokens: their biases, and with groups (e = lane + 32 i, g its group) the place
 // of their values in the scratch, e + g L, and the first of the group's lanes, g L
 template <int PER, bool GROUPS>
@@ -277,13 +326,13 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
       const uint32_t o = __shfl_sync(0xffffffffu, rank, j * L);
       place += o > rank || (o == rank && j < g);
     }
-    const unsigned stay = __ballot_sync(0xffffffffu, place < a.kept && g < a.groups);
+    unsigned stay = __ballot_sync(0xffffffffu, place < a.kept && g < a.groups);
     if (a.kept < a.groups && (sums || !by_logit)) {
       // the last group that stays and the first that does not
       const int in = __ffs(__ballot_sync(0xffffffffu, place == a.kept - 1 && g < a.groups)) - 1;
       const int out = __ffs(__ballot_sync(0xffffffffu, place == a.kept && g < a.groups)) - 1;
       const float u = of_key(__shfl_sync(0xffffffffu, rank, in)), w = of_key(__shfl_sync(0xffffffffu, rank, out));
-      exact = !(u - w > 2.f * near + 0x1p-22f * fabsf(u));
+      if (!(u - w > 2.f * near + 0x1p-22f * fabsf(u))) stay = groups_exact(a, row, mx, scratch);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -308,7 +357,9 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
       const bool larger = ((lane & size) == 0) == ((lane & o) == 0);  // descending in the end
       sorted = larger ? max(sorted, other) : min(sorted, other);
     }
-  const uint32_t floor_key = a.topk < 32 ? max(__shfl_sync(0xffffffffu, sorted, a.topk & 31), 1u) : 1u;
+  uint32_t floor_key = a.topk < 32 ? max(__shfl_sync(0xffffffffu, sorted, a.topk & 31), 1u) : 1u;
+  // what may be one of the k + 1 largest in truth
+  if (!by_logit && floor_key > 1u) floor_key = max(key_of(of_key(floor_key) - near), 1u);
   uint2* cand = reinterpret_cast<uint2*>(scratch);  // {key, expert}, room for all of them
   int n = 0;
 #pragma unroll
@@ -348,11 +399,24 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
     const float v = of_key(ckey), next = of_key(__shfl_down_sync(0xffffffffu, ckey, 1));
     // the last candidate has nothing behind it; with 32 chosen the 33rd is not known
     const bool behind = lane < a.topk && lane + 1 < min(n, 32);
-    const bool unsure = a.topk == 32 && E > 32;
-    if (unsure || __any_sync(0xffffffffu, behind && !(v - next > near))) {
+    if (__any_sync(0xffffffffu, behind && !(v - next > near)) || (a.topk == 32 && n > 32)) {
+      if (n > 32) {
+        __syncwarp();
+        route_exact<T>(a, row, t, scratch);
+        return;
+      }
+      // the candidates again in 64 bits, and their order
+      const double sum = a.sigmoid ? 0.0 : sum_exact(row, E, mx);
+      const double w = lane < n ? value_exact(a, row, cid, mx, sum) : -INFINITY;
+      int r = 0;
+      for (int k = 0; k < n; ++k) {
+        const double o = __shfl_sync(0xffffffffu, w, k);
+        const int e = __shfl_sync(0xffffffffu, cid, k);
+        r += o > w || (o == w && e < cid);
+      }
+      if (lane < n) cand[r] = make_uint2(ckey, cid);
       __syncwarp();
-      route_exact<T>(a, row, t, scratch);
-      return;
+      if (lane < n) cid = (int)cand[lane].y;
     }
   }
   float p = 0.f;
@@ -378,7 +442,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
 // PER: experts of a lane. The warps take the tokens in turn; a token's logits are on their way while the one before
 // it is done.
 template <typename T, int PER, bool GROUPS, bool FULL>
-__global__ void __launch_bounds__(kRouteWarps * 32, PER <= 8 ? kRouteCtas : 3) route_experts_kernel(const __grid_constant__ RouteArgs a) {
+__global__ void __launch_bounds__(kRouteWarps * 32, route_ctas(GROUPS)) route_experts_kernel(const __grid_constant__ RouteArgs a) {
   pdl_wait();
   pdl_launch();
   extern __shared__ double route_sm[];
@@ -414,7 +478,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, PER <= 8 ? kRouteCtas : 3) r
 template <typename T, int PER>
 cudaError_t launch_route_per(const RouteArgs& a, cudaStream_t s) {
   const size_t smem = (size_t)kRouteWarps * (2 * a.E + 32) * sizeof(double);
-  const int ctas = (a.n_tok + kRouteWarps - 1) / kRouteWarps, most = msgl_num_sms() * kRouteCtas;
+  const int ctas = (a.n_tok + kRouteWarps - 1) / kRouteWarps, most = msgl_num_sms() * route_ctas(a.groups > 1);
   const dim3 grid(ctas < most ? ctas : most), block(kRouteWarps * 32);
   if (a.E == 32 * PER)
     return a.groups > 1 ? msgl_launch(route_experts_kernel<T, PER, true, true>, grid, block, smem, s, 1, a)
