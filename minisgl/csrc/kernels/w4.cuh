@@ -357,13 +357,15 @@ struct W4Runs {
   }
 };
 
-// a call and not inlined: several copies of it would lengthen a short launch by their first execution
-static __noinline__ __device__ float w4_gated_act(float g, float u, int act) {
-  if (act == 0) return g / (1.f + __expf(-g)) * u;
+// The rarer activations are a call: inlined copies would lengthen a short launch by their first execution.
+static __noinline__ __device__ float w4_other_act(float g, float u, int act) {
   if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
   g = fminf(g, 7.f);
   u = fminf(fmaxf(u, -7.f), 7.f);
   return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
+}
+MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
+  return act == 0 ? __fdividef(g, 1.f + __expf(-g)) * u : w4_other_act(g, u, act);
 }
 
 // clusters of `splits` CTAs that run at once, one CTA per SM (148 SMs, in groups that are no multiples of 8)

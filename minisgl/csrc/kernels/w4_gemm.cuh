@@ -37,7 +37,7 @@ struct W4GemmArgs {
   const __nv_bfloat16* in;  // dense: [M]; gate_up: the tokens' rows; down: activated rows in sorted order
   int64_t in_stride;
   const __nv_bfloat16* bias;  // [n] of every expert
-  void* out;                  // dense: bf16 [M, n]; gate_up: bf16 rows in sorted order; down: fp32 [pairs, n]
+  void* out;                  // dense: bf16 [M, n]; gate_up: bf16, down: fp32 rows in sorted order
   int64_t out_stride;
   int M, bn, n_tiles, m_tiles, splits;
   // experts: tiles {expert, first sorted row, rows} of a device list, and the sorted rows' pairs
@@ -52,7 +52,9 @@ struct W4GemmArgs {
 
 constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
-constexpr int kGwMaxSlots = 8, kGwMaxA = 8, kGwB = 4;  // most stages of the rings
+constexpr int kGwMaxSlots = 8, kGwMaxA = 8;  // most stages of the rings
+constexpr int kGwB = 4;    // stages of the tokens' rows
+constexpr int kGwLag = 1;  // steps after which gathered rows are announced (3 with six stages measured no faster)
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
 constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
 constexpr int kGwMaxTokens = 224;    // of a tile: two stages of A then fit beside the accumulators
@@ -172,7 +174,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     for (int u = u_first; u < units && ok && !SPLIT; u += u_step, ++use) {
       const Tile tl = tile_of(u);
       const int set = set_of(use);
-      if (!(ok = w4_await<500>(&tfull[set], set_phase(use)))) break;
+      if (!(ok = w4_await<200>(&tfull[set], set_phase(use)))) break;
       tc_fence_after();
       const uint32_t d = tmem + set * H * half_cols + ((uint32_t)(warp * 32) << 16);
       const __nv_bfloat16* bias = p.bias == nullptr ? nullptr : p.bias + (int64_t)tl.e * p.w.n;
@@ -184,31 +186,32 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         tc_wait_ld();
         if constexpr (MODE == kW4GateUp) {
           const int inter = p.w.n / 2, i = tl.nt * 128 + warp * 32 + lane;
-          if (i < inter) {
-            const float bg = bias != nullptr ? __bfloat162float(bias[i]) : 0.f;
-            const float bu = bias != nullptr ? __bfloat162float(bias[inter + i]) : 0.f;
-            __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(tl.row0 + c0) * p.out_stride + i;
+          const float bg = bias != nullptr && i < inter ? __bfloat162float(bias[i]) : 0.f;
+          const float bu = bias != nullptr && i < inter ? __bfloat162float(bias[inter + i]) : 0.f;
+          float v[16];
+          if (p.act == 0) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[c] = w4_gated_act(__uint_as_float(r[0][c]) + bg, __uint_as_float(r[H - 1][c]) + bu, 0);
+          } else {
 #pragma unroll
             for (int c = 0; c < 16; ++c)
-              if (c < cn)
-                o[c * p.out_stride] = __float2bfloat16(
-                    w4_gated_act(__uint_as_float(r[0][c]) + bg, __uint_as_float(r[H - 1][c]) + bu, p.act));
+              v[c] = w4_other_act(__uint_as_float(r[0][c]) + bg, __uint_as_float(r[H - 1][c]) + bu, p.act);
           }
+          __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(tl.row0 + c0) * p.out_stride + i;
+#pragma unroll
+          for (int c = 0; c < 16; ++c, o += p.out_stride)
+            if (c < cn && i < inter) *o = __float2bfloat16(v[c]);
         } else {
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             const int n = (tl.nt * H + h) * 128 + warp * 32 + lane;
+            const float b = bias == nullptr || n >= p.w.n ? 0.f : __bfloat162float(bias[n]);
             if (n >= p.w.n) continue;
-            const float b = bias == nullptr ? 0.f : __bfloat162float(bias[n]);
+            using Out = std::conditional_t<MODE == kW4Dense, __nv_bfloat16, float>;
+            Out* o = reinterpret_cast<Out*>(p.out) + (int64_t)(tl.row0 + c0) * p.out_stride + n;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              if (c >= cn) break;
-              const float v = __uint_as_float(r[h][c]) + b;
-              if constexpr (MODE == kW4Dense)
-                reinterpret_cast<__nv_bfloat16*>(p.out)[(int64_t)(tl.row0 + c0 + c) * p.out_stride + n] = __float2bfloat16(v);
-              else
-                reinterpret_cast<float*>(p.out)[(int64_t)p.sorted[tl.row0 + c0 + c] * p.out_stride + n] = v;
-            }
+            for (int c = 0; c < 16; ++c, o += p.out_stride)
+              if (c < cn) *o = Out(__uint_as_float(r[h][c]) + b);
           }
         }
       }
@@ -260,11 +263,12 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     } else {
       const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 7, r0 = lt >> 3;
       constexpr int kRows = kGwLoad * 4;  // rows of one pass
-      int before = -1;                    // stage of the previous step, whose copies are not announced yet
+      int behind = 0, done = 0;           // steps whose copies are not announced yet, and the first one's stage
       const auto announce = [&] {
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b_full[before]);
+        if (lane == 0) mbar_arrive(&b_full[done]);
+        if (++done == kGwB) done = 0;
       };
       for (int u = u_first; u < units && ok; u += u_step) {
         const Tile tl = tile_of(u);
@@ -283,16 +287,16 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
                          "l"(src + (int64_t)rows[r] * p.in_stride), "r"(bytes)
                          : "memory");
           asm volatile("cp.async.commit_group;" ::: "memory");
-          if (before >= 0) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          if (++behind > kGwLag) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kGwLag) : "memory");
             announce();
+            --behind;
           }
-          before = stage;
           if (++stage == kGwB) stage = 0, phase ^= 1;
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (before >= 0) announce();
+      for (; behind > 0; --behind) announce();
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------------ records

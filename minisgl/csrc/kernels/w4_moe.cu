@@ -160,8 +160,10 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   }
 }
 
-// out[t] = sum over a token's choices, in their order, of weight * y; four columns a thread
-__global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict__ y, const float* __restrict__ weights,
+// out[t] = sum over a token's choices, in their order, of weight * y; four columns a thread. A pair's row of y is its
+// number, or its place[].
+__global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ place,
+                                                         const float* __restrict__ weights,
                                                          const int32_t* __restrict__ ids, int E, int e0, int topk, int H,
                                                          __nv_bfloat16* __restrict__ out) {
   pdl_wait();
@@ -174,11 +176,12 @@ __global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict
     const int64_t p = t * topk + j;
     if (local_expert(ids[p], e0) >= (unsigned)E) continue;
     const float w = weights[p];
+    const float* from = y + (place == nullptr ? p : (int64_t)place[p]) * H + c;
     if (H % 4 == 0) {
-      const float4 f = *reinterpret_cast<const float4*>(y + p * H + c);
+      const float4 f = *reinterpret_cast<const float4*>(from);
       v[0] += w * f.x, v[1] += w * f.y, v[2] += w * f.z, v[3] += w * f.w;
     } else {
-      for (int i = 0; i < 4 && c + i < H; ++i) v[i] += w * y[p * H + c + i];
+      for (int i = 0; i < 4 && c + i < H; ++i) v[i] += w * from[i];
     }
   }
   if (H % 4 == 0) {
@@ -217,7 +220,8 @@ constexpr int kTileTokens = 96;  // of a tile: two sets of accumulators then fit
 // Sorts the pairs by expert (in any order within one: a pair's result does not depend on its place) and cuts
 // every expert's into equal tiles. One CTA.
 __global__ void __launch_bounds__(1024) w4_plan_kernel(const int32_t* __restrict__ ids, int pairs, int E, int e0,
-                                                       int32_t* __restrict__ sorted, int4* __restrict__ work,
+                                                       int32_t* __restrict__ sorted, int32_t* __restrict__ place,
+                                                       int4* __restrict__ work,
                                                        int32_t* __restrict__ count) {
   __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -260,13 +264,17 @@ __global__ void __launch_bounds__(1024) w4_plan_kernel(const int32_t* __restrict
   __syncthreads();
   for (int i = tid; i < pairs; i += 1024) {
     const unsigned e = local_expert(ids[i], e0);
-    if (e < (unsigned)E) sorted[atomicAdd(&at[e], 1)] = i;
+    if (e < (unsigned)E) {
+      const int to = atomicAdd(&at[e], 1);
+      sorted[to] = i;
+      place[i] = to;
+    }
   }
 }
 
 // scratch of a call: activated rows, results of the pairs, and for many tokens the sorted pairs and tiles
 struct Scratch {
-  int64_t a, y, sorted, work, count, bytes;
+  int64_t a, y, sorted, place, work, count, bytes;
 };
 Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
   const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
@@ -274,7 +282,8 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
   s.a = 0;
   s.y = up(pairs * w2->kc * 128 * 2);
   s.sorted = s.y + up(pairs * w2->n * 4);
-  s.work = s.sorted + up(pairs * 4);
+  s.place = s.sorted + up(pairs * 4);
+  s.work = s.place + up(pairs * 4);
   s.count = s.work + up((E + pairs / kTileTokens) * 16);
   s.bytes = s.count + 256;
   return s;
@@ -288,7 +297,8 @@ int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const Ms
                   cudaStream_t s) {
   int32_t *sorted = (int32_t*)(ws + sc.sorted), *count = (int32_t*)(ws + sc.count);
   int4* work = (int4*)(ws + sc.work);
-  if (msgl_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, work, count) != cudaSuccess)
+  if (msgl_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, (int32_t*)(ws + sc.place), work,
+                  count) != cudaSuccess)
     return 4;
   W4GemmArgs p = {};
   p.bn = std::min(kTileTokens, (pairs + 15) / 16 * 16);
@@ -332,7 +342,8 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   uint8_t* ws = (uint8_t*)workspace;
   const Scratch sc = scratch_of(pairs, E, w2);
   int rc;
-  if (pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs) {
+  const bool stream = pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs;
+  if (stream) {
     __nv_bfloat16* a = (__nv_bfloat16*)(ws + sc.a);
     ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, ids, (const __nv_bfloat16*)x, x_stride, (const __nv_bfloat16*)b1,
                      a, nullptr, a_stride, act, 0};
@@ -345,7 +356,7 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   }
   if (rc != 0) return rc;
   return msgl_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),
-                     weights, ids, E, e0, topk, w2->n, (__nv_bfloat16*)out) == cudaSuccess
+                     stream ? (const int32_t*)nullptr : (const int32_t*)(ws + sc.place), weights, ids, E, e0, topk, w2->n, (__nv_bfloat16*)out) == cudaSuccess
              ? 0
              : 4;
 }
