@@ -38,10 +38,18 @@ class _CountingModule:
             return fn
         from minisgl.engine.counters import COUNTERS
 
-        def call(*args, **kwargs):
-            COUNTERS.launches += 2 if (name == "attention_decode" and args[-2] > 1) else 1
-            return fn(*args, **kwargs)
+        if name == "attention_decode":
+            def call(*args, **kwargs):
+                COUNTERS.launches += 2 if args[-2] > 1 else 1
+                return fn(*args, **kwargs)
+        else:
+            launches = 3 if name == "experts_w4" else 1  # (4 with many tokens)
 
+            def call(*args, **kwargs):
+                COUNTERS.launches += launches
+                return fn(*args, **kwargs)
+
+        setattr(self, name, call)  # looked up once: a small call's time is mostly the host's
         return call
 
 

@@ -1,6 +1,7 @@
 // Torch bindings for the sm_100a kernels: validate tensors (dtype / device / contiguity / shape),
 // take the current CUDA stream, and call the C ABI in kernels/api.h.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -439,6 +440,11 @@ void moe_combine(at::Tensor out, at::Tensor y, at::Tensor w, at::Tensor inv, int
 
 // ----- router and 4-bit weights. These allocate their outputs, so that a call costs one crossing of the
 // binding, and run on the tensors' own device and its current stream.
+// a device tensor without the dispatcher's way there (about 1 us of a small call's 5)
+at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt);
+}
+
 void check_launch(int rc, const char* op) {
   CHECK(rc != 3, op, ": these sizes are not supported");
   CHECK(rc == 0, op, " failed (code ", rc, ": ", cudaGetErrorString(cudaGetLastError()), ")");
@@ -468,8 +474,8 @@ std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, int64_t topk
   }
   c10::cuda::CUDAGuard guard(logits.device());
   if (logits.stride(1) != 1 && E > 1) logits = logits.contiguous();
-  at::Tensor weights = at::empty({T, topk}, logits.options().dtype(at::kFloat));
-  at::Tensor ids = at::empty({T, topk}, logits.options().dtype(at::kInt));
+  at::Tensor weights = new_cuda({T, topk}, at::kFloat, logits.device());
+  at::Tensor ids = new_cuda({T, topk}, at::kInt, logits.device());
   const int rc = msgl_route_experts(logits.data_ptr(), f32, logits.stride(0), b, T, E, topk, sigmoid, groups, kept, top2,
                                     renorm, scale, weights.data_ptr<float>(), ids.data_ptr<int32_t>(), stream());
   check_launch(rc, "route_experts");
@@ -519,7 +525,7 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
   }
   const int64_t M = x.size(0);
   CHECK(M < (1ll << 31), "too many tokens");
-  at::Tensor out = at::empty({M, n}, x.options());
+  at::Tensor out = new_cuda({M, n}, at::kBFloat16, x.device());
   if (M == 0) return out;
   const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
   check_launch(rc, "linear_w4");
@@ -555,8 +561,8 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
     check_bf16(*b2, "w2_bias"); check_contig(*b2, "w2_bias");
     CHECK(b2->numel() == E * n2 && b2->device() == x.device(), "w2_bias must be [E, H]");
   }
-  at::Tensor out = at::empty({T, n2}, x.options());
-  at::Tensor ws = at::empty({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, x.options().dtype(at::kByte));
+  at::Tensor out = new_cuda({T, n2}, at::kBFloat16, x.device());
+  at::Tensor ws = new_cuda({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, at::kByte, x.device());
   if (T == 0) return out;
   const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0,
                                  weights.data_ptr<float>(), ids.data_ptr<int32_t>(), opt_ptr(b1), opt_ptr(b2), act,
