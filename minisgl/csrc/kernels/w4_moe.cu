@@ -61,32 +61,50 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   // before this kernel could start (it triggers its dependents after its own wait).
   if constexpr (GATED) pdl_wait();
   pdl_launch();
-  for (int e = threadIdx.x; e < p.E; e += kThreads) count[e] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
-    const unsigned e = local_expert(p.ids[i], p.e0);
-    lid[i] = e;
-    if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
+  // Up to 32 pairs are a lane each: the lanes that hold an expert first stand for its unit, if none has more pairs
+  // than fit one (decoding a few tokens; the lists below cost 2 us there).
+  unsigned my_e = 0xffffffffu, same = 0, leaders = 0;
+  bool few = p.pairs <= 32;
+  if (few) {
+    if (lane < p.pairs) my_e = local_expert(p.ids[lane], p.e0);
+    same = __match_any_sync(0xffffffffu, my_e);
+    leaders = __ballot_sync(0xffffffffu, my_e < (unsigned)p.E && __ffs(same) == lane + 1);
+    few = !__any_sync(0xffffffffu, my_e < (unsigned)p.E && __popc(same) > p.rows);
   }
-  __syncthreads();
-  // the units, expert by expert: sums of 32 experts a warp, then of the warps
-  int n_units = 0;
-  for (int b = 0; b < p.E; b += kThreads) {
-    const int e = b + (int)threadIdx.x, mine = e < p.E ? (count[e] + p.rows - 1) / p.rows : 0;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (lane == 31) seen[warp] = sum;
+  // the lane that stands for unit `un`
+  const auto leader_of = [&](int un) {
+    const bool is = ((leaders >> lane) & 1) && __popc(leaders & ((1u << lane) - 1)) == un;
+    return __ffs(__ballot_sync(0xffffffffu, is)) - 1;
+  };
+  int n_units = __popc(leaders);
+  if (!few) {
+    n_units = 0;
+    for (int e = threadIdx.x; e < p.E; e += kThreads) count[e] = 0;
     __syncthreads();
-    int before = lane < kWarps ? seen[lane] : 0;
-    const int all = __reduce_add_sync(0xffffffffu, before);
-    before = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0);
-    for (int i = 0; i < mine; ++i) units[n_units + before + sum - mine + i] = e | i << 16;
-    n_units += all;
-    if (b + kThreads < p.E) __syncthreads();  // seen is used again
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
+      const unsigned e = local_expert(p.ids[i], p.e0);
+      lid[i] = e;
+      if (e < (unsigned)p.E) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    // the units, expert by expert: sums of 32 experts a warp, then of the warps
+    for (int b = 0; b < p.E; b += kThreads) {
+      const int e = b + (int)threadIdx.x, mine = e < p.E ? (count[e] + p.rows - 1) / p.rows : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (lane == 31) seen[warp] = sum;
+      __syncthreads();
+      int before = lane < kWarps ? seen[lane] : 0;
+      const int all = __reduce_add_sync(0xffffffffu, before);
+      before = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0);
+      for (int i = 0; i < mine; ++i) units[n_units + before + sum - mine + i] = e | i << 16;
+      n_units += all;
+      if (b + kThreads < p.E) __syncthreads();  // seen is used again
+    }
   }
   __syncthreads();
   // this CTA's run of the units' tiles: an equal share, whichever experts it falls on
@@ -96,9 +114,11 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   const int pitch = w4_pitch(p.w.kc * 128);
   if constexpr (!GATED) {
     // bring the run's first weights into L2 while the first product ends
+    const int un = pos / p.w.tiles;
+    const int e = pos >= end ? 0 : few ? (int)__shfl_sync(0xffffffffu, my_e, leader_of(un)) : units[un] & 0xffff;
     if (lane == 0 && pos < end) {
-      const int ta = pos % p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
-      const int64_t tile = (int64_t)(units[pos / p.w.tiles] & 0xffff) * p.w.tiles + ta;
+      const int ta = pos - un * p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
+      const int64_t tile = (int64_t)e * p.w.tiles + ta;
       const int a = runs.bound(nt * p.w.kc, warp), n = min(runs.bound(nt * p.w.kc, warp + 1) - a, kW4Slots);
       if (n > 0) prefetch_l2(p.w.data + (tile * p.w.kc + a) * R::kBytes, n * R::kBytes);
     }
@@ -108,26 +128,37 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
   // the pairs are looked through by all warps, a run of whole 32s each
   const int per = ((p.pairs + 31) / 32 + kWarps - 1) / kWarps * 32;
   while (pos < end) {
-    const int un = pos / p.w.tiles, unit = units[un], e = unit & 0xffff, i0 = unit >> 16;
-    const int ta = pos - un * p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
-    // the expert's pairs are cut into equal units; every CTA finds the same ones in the same order
-    const int c = count[e], cuts = c <= p.rows ? 1 : (c + p.rows - 1) / p.rows;
-    const int m0 = cuts == 1 ? 0 : c * i0 / cuts, nx = (cuts == 1 ? c : c * (i0 + 1) / cuts) - m0;
+    const int un = pos / p.w.tiles, ta = pos - un * p.w.tiles, nt = min(p.w.tiles - ta, end - pos);
+    int e, nx;
     __syncthreads();  // the previous unit's list is done with
-    int found = 0;
-    for (int i = warp * per + lane; i < (warp + 1) * per; i += 32)
-      found += __popc(__ballot_sync(0xffffffffu, i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e));
-    if (lane == 0) seen[warp] = found;
-    __syncthreads();
-    int at = (int)__reduce_add_sync(0xffffffffu, lane < warp ? seen[lane] : 0) - m0;
-    if (found > 0)
-      for (int i = warp * per + lane; i < (warp + 1) * per; i += 32) {
-        const bool is = i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e;
-        const unsigned m = __ballot_sync(0xffffffffu, is);
-        const int k = at + __popc(m & ((1u << lane) - 1));
-        if (is && k >= 0 && k < nx) list[k] = i;
-        at += __popc(m);
-      }
+    if (few) {
+      const int leader = leader_of(un);
+      const unsigned m = __shfl_sync(0xffffffffu, same, leader);
+      e = __shfl_sync(0xffffffffu, my_e, leader);
+      nx = __popc(m);
+      if (warp == 0 && ((m >> lane) & 1)) list[__popc(m & ((1u << lane) - 1))] = lane;
+    } else {
+      const int unit = units[un], i0 = unit >> 16;
+      e = unit & 0xffff;
+      // the expert's pairs are cut into equal units; every CTA finds the same ones in the same order
+      const int c = count[e], cuts = c <= p.rows ? 1 : (c + p.rows - 1) / p.rows;
+      const int m0 = cuts == 1 ? 0 : c * i0 / cuts;
+      nx = (cuts == 1 ? c : c * (i0 + 1) / cuts) - m0;
+      int found = 0;
+      for (int i = warp * per + lane; i < (warp + 1) * per; i += 32)
+        found += __popc(__ballot_sync(0xffffffffu, i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e));
+      if (lane == 0) seen[warp] = found;
+      __syncthreads();
+      int at = (int)__reduce_add_sync(0xffffffffu, lane < warp ? seen[lane] : 0) - m0;
+      if (found > 0)
+        for (int i = warp * per + lane; i < (warp + 1) * per; i += 32) {
+          const bool is = i < p.pairs && lid[min(i, p.pairs - 1)] == (unsigned)e;
+          const unsigned m = __ballot_sync(0xffffffffu, is);
+          const int k = at + __popc(m & ((1u << lane) - 1));
+          if (is && k >= 0 && k < nx) list[k] = i;
+          at += __popc(m);
+        }
+    }
     __syncthreads();
     const int* mine = list;
     {
