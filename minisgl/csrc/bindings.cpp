@@ -503,11 +503,13 @@ MsglW4 w4_of(const W4Args& a, bool gated, const at::Device& dev, const char* nam
   return {a.data.data_ptr(), (int)tiles, (int)kc, (int)a.group, (int)n, (int)k, a.zeros, a.fp16};
 }
 
-// rows as the kernels read them: unit inner stride, every row on a 16-byte boundary (else a copy)
+// rows as the kernels read them: unit inner stride, every row on a 16-byte boundary and behind the one before (a tensor
+// map takes no rows that overlap); else a copy
 at::Tensor w4_rows(const at::Tensor& x, int64_t k) {
   check_bf16(x, "x");
   CHECK(x.dim() == 2 && x.size(1) == k, "x must be [tokens, ", k, "], got ", x.sizes());
-  if (x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
+  if (x.stride(1) == 1 && (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= k)) &&
+      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
     return x;
   return x.clone(at::MemoryFormat::Contiguous);
 }
@@ -524,7 +526,7 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
     CHECK(bias->numel() == n && bias->device() == x.device(), "bias size");
   }
   const int64_t M = x.size(0);
-  CHECK(M < (1ll << 31), "too many tokens");
+  CHECK(M < (1ll << 30), "linear_w4: too many tokens for one call");
   at::Tensor out = new_cuda({M, n}, at::kBFloat16, x.device());
   if (M == 0) return out;
   const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());

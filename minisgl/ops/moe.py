@@ -80,7 +80,11 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     if group_score not in ("max", "top2"):
         raise ValueError(f"group_score must be max or top2, got {group_score!r}")
     if not logits.is_cuda:
+        if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"logits must be fp32 or bf16 [tokens, experts], got {logits.dtype} {tuple(logits.shape)}")
         T, E = logits.shape
+        if bias is not None and bias.shape != (E,):
+            raise ValueError(f"bias must be [{E}], got {tuple(bias.shape)}")
         if E % num_groups or not 1 <= top_groups <= num_groups or not 1 <= top_k <= min(32, top_groups * (E // num_groups)):
             raise ValueError(f"cannot choose {top_k} of {E} experts in {top_groups} of {num_groups} groups")
         if group_score == "top2" and num_groups > 1 and E // num_groups < 2:

@@ -155,3 +155,26 @@ def test_refusals():
     ):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_refusals_of_sizes():
+    gen = torch.Generator().manual_seed(3)
+    w = ops.W4Weight.pack(*_codes(gen, (32, 128), 64, False))
+    w1 = ops.W4Weight.pack(*_codes(gen, (4, 64, 128), 64, False), gated=True)
+    w2 = ops.W4Weight.pack(*_codes(gen, (4, 128, 32), 32, False))
+    x, wt, ids = torch.randn(4, 128), torch.rand(4, 2), torch.zeros(4, 2, dtype=torch.int32)
+    logits = torch.randn(4, 8)
+    for bad in (
+        lambda: ops.linear_w4(x[:, :64], w),
+        lambda: ops.linear_w4(x[0], w),
+        lambda: ops.linear_w4(x, w, torch.zeros(1)),
+        lambda: ops.experts_w4(x, w1, w2, wt[:3], ids),
+        lambda: ops.experts_w4(x, w1, w2, wt, ids[:, :1]),
+        lambda: ops.experts_w4(x[:, :64], w1, w2, wt, ids),
+        lambda: ops.experts_w4(x, w1, ops.W4Weight.pack(*_codes(gen, (3, 128, 32), 32, False)), wt, ids),
+        lambda: ops.route_experts(logits[0], 2),
+        lambda: ops.route_experts(logits.double(), 2),
+        lambda: ops.route_experts(logits, 2, bias=torch.zeros(1)),
+    ):
+        with pytest.raises(ValueError):
+            bad()
