@@ -151,7 +151,7 @@ int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   return ra != 0 ? ra : linear_rows(b, w, s);
 }
 
-// many tokens: tiles of 128 or 256 rows by up to 192 tokens; where these leave SMs idle a cluster cuts the inputs
+// many tokens: tiles of 128 or 256 rows by up to 208 tokens; where these leave SMs idle a cluster cuts the inputs
 int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   W4GemmArgs p = {};
   p.w = a.w;

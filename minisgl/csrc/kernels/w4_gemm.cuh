@@ -1,6 +1,6 @@
 // 4-bit products for many tokens, on the 5th-generation tensor core (layout of the weights in w4.cuh).
 //
-// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 224 tokens (their N, a multiple of 16
+// A tile is 128 H weight rows (H = 1 or 2 MMAs of M = 128) by up to 208 tokens (their N, a multiple of 16
 // that follows the number of tokens), 64 inputs per step. Roles of a CTA's 26 warps, one CTA per SM,
 // persistent over tiles:
 //   warps 0-3    epilogue, one TMEM lane quadrant each
@@ -57,7 +57,7 @@ constexpr int kGwB = 4;    // stages of the tokens' rows
 constexpr int kGwLag = 1;  // steps after which gathered rows are announced (3 with six stages measured no faster)
 constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
 constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
-constexpr int kGwMaxTokens = 224;    // of a tile: two stages of A then fit beside the accumulators
+constexpr int kGwMaxTokens = 208;    // of a tile: three half-step stages of A then fit beside the accumulators
 
 // pair of exact integers (bf16x2) times a scale, rounded once
 template <bool F>
@@ -532,7 +532,10 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   p.half_cols = p.bn;
   p.sets = 512 - 2 * H * p.half_cols >= 2 * H * 32 ? 2 : 1;
   p.stages = std::min(kGwMaxA, (512 - p.sets * H * p.half_cols) / kA);
-  if (p.stages < 2) return 3;
+  // A team of converters waits for a stage's turn by the parity of its phase, and takes every other step: its last wait
+  // must have shown that all but the latest of the stage's turns are over. That is so with two stages of a step, or
+  // three of half a step.
+  if (p.stages < (FINE ? 3 : 2)) return 3;
   p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
   const int room = kGwRoom, stage = p.bn * 128;
   p.slots = std::min(kGwMaxSlots, (room - kGwB * stage) / p.raw_bytes);

@@ -24,6 +24,15 @@ def test_linear_rows_overlap(M, step):
     assert torch.equal(ops.linear_w4(x, w), ops.linear_w4(x.clone(memory_format=torch.contiguous_format), w))
 
 
+@pytest.mark.parametrize("M,N,K", [(3001, 4000, 416), (700, 33, 256), (208, 2048, 1024), (224, 2048, 1024), (624, 34816, 256),
+                                   (1021, 64, 1152)])
+def test_linear_many_tiles(M, N, K):
+    q, s, z = _codes((N, K), 32, False)
+    x = torch.randn(M, K, device=DEV).to(torch.bfloat16)
+    bias = torch.randn(N, device=DEV).to(torch.bfloat16)
+    _check_linear(x, q, s, z, bias, ops.linear_w4(x, ops.W4Weight.pack(q, s, z), bias))
+
+
 @pytest.mark.parametrize("T,E,k", [(1, 1, 1), (20, 1, 1), (3, 1024, 6), (1100, 1024, 8), (4000, 4, 3)])
 def test_experts_few_and_many(T, E, k):
     """One expert, 1024 of them, many tiles a CTA."""
