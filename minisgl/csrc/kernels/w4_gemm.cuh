@@ -405,28 +405,31 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[slot]);
         if (++slot == p.slots) slot = 0, rphase ^= 1;
-        // the bf16 values: [row g, row g + 8 of a half][word][pair of inputs]
-        uint32_t v[H][2][4][2];
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          const int half = H == 2 ? i : m;
-          const uint32_t words[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+        for (int e = 0; e < 2; ++e) {  // 32 inputs
+          // a store's registers: two words by rows g (two pairs of inputs) and rows g + 8 of a half; gated: by the gate
+          // rows (first store) or the up rows (second) of both halves
+          uint32_t r[H][8];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const uint32_t sv = half ? s[b >> 1].y : s[b >> 1].x, zv = z[b >> 1] >> (16 * half);
+          for (int i = 0; i < H; ++i) {
+            const int half = H == 2 ? i : m;
+            const uint32_t sv = half ? s[e].y : s[e].x, zv = z[e] >> (16 * half);
             const uint32_t z0 = Z ? 0x43004300u + (zv & 15u) * 0x10001u : 0x43084308u;
             const uint32_t z1 = Z ? 0x43004300u + ((zv >> 8) & 15u) * 0x10001u : 0x43084308u;
             const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
             float2 sf = make_float2(0.f, 0.f);
             if constexpr (F) sf = w4_scales<true>(sv);
-            v[i][0][b][0] = w4_times<F>(codes_bf16x2(words[b], z0), sa2, sf.x);
-            v[i][1][b][0] = w4_times<F>(codes_bf16x2(words[b] >> 4, z1), sb2, sf.y);
-            v[i][0][b][1] = w4_times<F>(codes_bf16x2(words[b] >> 8, z0), sa2, sf.x);
-            v[i][1][b][1] = w4_times<F>(codes_bf16x2(words[b] >> 12, z1), sb2, sf.y);
-          }
-        }
+            const uint32_t words[2] = {e ? q[i].z : q[i].x, e ? q[i].w : q[i].y};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // 32 inputs
+            for (int b = 0; b < 2; ++b) {
+              uint32_t* const lo = MODE == kW4GateUp ? &r[0][4 * b + 2 * i] : &r[i][4 * b];
+              uint32_t* const hi = MODE == kW4GateUp ? &r[H - 1][4 * b + 2 * i] : &r[i][4 * b + 2];
+              lo[0] = w4_times<F>(codes_bf16x2(words[b], z0), sa2, sf.x);
+              hi[0] = w4_times<F>(codes_bf16x2(words[b] >> 4, z1), sb2, sf.y);
+              lo[1] = w4_times<F>(codes_bf16x2(words[b] >> 8, z0), sa2, sf.x);
+              hi[1] = w4_times<F>(codes_bf16x2(words[b] >> 12, z1), sb2, sf.y);
+            }
+          }
           if (FINE || e == 0) {
             if (ok) ok = w4_await<50>(&a_empty[stage], phase ^ 1);
             if (!ok) break;
@@ -435,17 +438,8 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
           const uint32_t dst = tmem_a + lanes + stage * H * kCols + (FINE ? 0 : e * 16);
 #pragma unroll
           for (int i = 0; i < H; ++i) {
-            uint32_t r[8];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                // gated: the gate rows (i = 0) or up rows (i = 1) of both halves
-                r[4 * b + c] = MODE == kW4GateUp ? v[0][i][2 * e + b][c] : v[i][0][2 * e + b][c];
-                r[4 * b + 2 + c] = MODE == kW4GateUp ? v[H - 1][i][2 * e + b][c] : v[i][1][2 * e + b][c];
-              }
-            if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x2(dst + i * kCols, r);
-            else tmem_st_16x256b_x2(dst + (H == 2 ? m * kCols : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r);
+            if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x2(dst + i * kCols, r[i]);
+            else tmem_st_16x256b_x2(dst + (H == 2 ? m * kCols : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r[i]);
           }
           if (FINE || e == 1) {
             tc_wait_st();
