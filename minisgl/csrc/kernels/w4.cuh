@@ -96,6 +96,18 @@ MSGL_DEVICE bool mbar_try_wait_a(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// the same; the hardware may hold the warp for `ns`
+MSGL_DEVICE bool mbar_try_wait_a(uint32_t bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
 MSGL_DEVICE void mbar_expect_tx_a(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -133,15 +145,11 @@ MSGL_DEVICE float2 w4_scales(uint32_t v) {
   return make_float2(bf16_lo(v), bf16_hi(v));
 }
 
-// A wait that did not succeed at once. NS > 0: the warp sleeps between its looks, so that it does not take
-// issue slots from the others (a look every 40 ns by each of 26 warps took most of an SM's). Bounded to a
-// few seconds; false when they are over.
-template <int NS>
+// A wait that did not succeed at once. The hardware may hold the warp until the phase is over or 2 us have passed (looks
+// 40 ns apart by each of 26 warps took most of an SM's issue slots). Bounded to a few seconds; false when they are over.
 static __noinline__ __device__ bool w4_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < (NS > 0 ? 1 << 24 : 1 << 26); ++i) {
-    if (mbar_try_wait_a(bar, parity)) return true;
-    if constexpr (NS > 0) __nanosleep(NS);
-  }
+  for (int i = 0; i < 1 << 21; ++i)
+    if (mbar_try_wait_a(bar, parity, 2000)) return true;
   report_error(kErrMbarTimeout, 400);
   return false;
 }
@@ -225,7 +233,7 @@ struct W4Runs {
     for (int i = threadIdx.x; i < nx * (pad / 8); i += w4_threads<NT>())
       *reinterpret_cast<uint4*>(xs + i / (pad / 8) * pitch + kn * 2 + i % (pad / 8) * 16) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (ok) ok = w4_wait<20>(xbar(), runs & 1);
+    if (ok) ok = w4_wait(xbar(), runs & 1);
     ++runs;
 
     uint32_t xrow[NT];
@@ -245,7 +253,7 @@ struct W4Runs {
         clear(acc);
         for (; i < end; ++i) {
           if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
-            if (ok) ok = w4_wait<20>(bar, (it >> 1) & 1);
+            if (ok) ok = w4_wait(bar, (it >> 1) & 1);
           }
           ++it;
           uint4 q[2][2];

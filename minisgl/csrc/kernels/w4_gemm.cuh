@@ -53,9 +53,10 @@ struct W4GemmArgs {
 constexpr int kGwEpi = 4, kGwLoad = 4, kGwConv = 16;
 constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
 constexpr int kGwMaxSlots = 8, kGwMaxA = 8;  // most stages of the rings
-constexpr int kGwB = 4;    // stages of the tokens' rows
-constexpr int kGwLag = 1;  // steps after which gathered rows are announced (3 with six stages measured no faster)
-constexpr int kGwMisc = 1024 + 512;  // row numbers, barriers
+constexpr int kGwMaxB = 8;
+constexpr int w4_row_stages(int mode) { return mode == kW4GateUp ? kGwMaxB : 4; }  // of the tokens' rows
+constexpr int kGwMaxGather = 96;  // gathered tokens of a tile
+constexpr int kGwMisc = kGwLoad * kGwMaxGather * 4 + 512;  // row numbers, barriers
 constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
 constexpr int kGwMaxTokens = 208;    // of a tile: three half-step stages of A then fit beside the accumulators
 
@@ -75,18 +76,22 @@ MSGL_DEVICE void tmem_st_16x256b_x2(uint32_t taddr, const uint32_t (&r)[8]) {
                : "memory");
 }
 
+// 16 bytes, or zeros if `bytes` is 0
+MSGL_DEVICE void cp_async_zfill(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 // a role's wait: true once the phase is complete, false if it never is
-template <int NS>
 MSGL_DEVICE bool w4_await(uint64_t* bar, uint32_t parity) {
   const uint32_t a = smem_u32(bar);
-  return mbar_try_wait_a(a, parity) || w4_wait<NS>(a, parity);
+  return mbar_try_wait_a(a, parity) || w4_wait(a, parity);
 }
 
 template <int MODE, int H, bool SPLIT, bool FINE, bool Z, bool F>
 __global__ void __launch_bounds__(kGwThreads, 1)
 w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUtensorMap rows_map) {
   static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
-  constexpr int kRecs = 4 * H;
+  constexpr int kRecs = 4 * H, kGwB = w4_row_stages(MODE);
   // Columns of a half in a stage of A. FINE: a stage is half a step, so that three fit beside the accumulators of
   // more than 192 tokens; the MMA warp then waits and commits twice a step, which small tiles would feel.
   constexpr int kCols = FINE ? 16 : 32;
@@ -95,9 +100,9 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
   const int S = p.stages, stage_bytes = p.bn * 128;
   uint8_t* raw = smem + kGwB * stage_bytes;
   int* rows = reinterpret_cast<int*>(smem + p.ring_bytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(rows + 256);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(rows + kGwLoad * kGwMaxGather);
   uint64_t *raw_full = bars, *raw_empty = bars + kGwMaxSlots, *a_full = raw_empty + kGwMaxSlots,
-           *a_empty = a_full + kGwMaxA, *b_full = a_empty + kGwMaxA, *b_empty = b_full + kGwB, *tfull = b_empty + kGwB,
+           *a_empty = a_full + kGwMaxA, *b_full = a_empty + kGwMaxA, *b_empty = b_full + kGwMaxB, *tfull = b_empty + kGwMaxB,
            *tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -113,7 +118,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       mbar_init(&a_empty[i], 1);
     }
     for (int i = 0; i < kGwB; ++i) {
-      mbar_init(&b_full[i], MODE == kW4GateUp ? kGwLoad : 1);
+      mbar_init(&b_full[i], 1);
       mbar_init(&b_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -174,7 +179,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     for (int u = u_first; u < units && ok && !SPLIT; u += u_step, ++use) {
       const Tile tl = tile_of(u);
       const int set = set_of(use);
-      if (!(ok = w4_await<200>(&tfull[set], set_phase(use)))) break;
+      if (!(ok = w4_await(&tfull[set], set_phase(use)))) break;
       tc_fence_after();
       const uint32_t d = tmem + set * H * half_cols + ((uint32_t)(warp * 32) << 16);
       const __nv_bfloat16* bias = p.bias == nullptr ? nullptr : p.bias + (int64_t)tl.e * p.w.n;
@@ -222,7 +227,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     if constexpr (SPLIT) {
       // one tile per cluster: leave it as fp32 [token][128 H rows] in the drained rings
       const Tile tl = tile_of(u_first);
-      if (ok) ok = w4_await<500>(&tfull[0], 0);
+      if (ok) ok = w4_await(&tfull[0], 0);
       tc_fence_after();
       float* dump = reinterpret_cast<float*>(smem);
       for (int c0 = 0; c0 < tl.cols; c0 += 16)
@@ -245,7 +250,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
         for (int u = u_first; u < units && ok; u += u_step) {
           const Tile tl = tile_of(u);
           for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-            if (!(ok = w4_await<100>(&b_empty[stage], phase ^ 1))) break;
+            if (!(ok = w4_await(&b_empty[stage], phase ^ 1))) break;
             uint8_t* dst = smem + stage * stage_bytes;
             // rows beyond the last one and inputs beyond the last one arrive as zeros, and count
             if constexpr (MODE == kW4Dense) {
@@ -261,42 +266,37 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       }
       __syncwarp();
     } else {
-      const int lt = threadIdx.x - kGwEpi * 32, chunk = lt & 7, r0 = lt >> 3;
-      constexpr int kRows = kGwLoad * 4;  // rows of one pass
-      int behind = 0, done = 0;           // steps whose copies are not announced yet, and the first one's stage
-      const auto announce = [&] {
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b_full[done]);
-        if (++done == kGwB) done = 0;
-      };
-      for (int u = u_first; u < units && ok; u += u_step) {
+      // A warp per step, in turn: a step's cost is mostly one chain of dependent instructions (four warps with a
+      // quarter of every step's rows each were the products' limit).
+      const int lw = warp - kGwEpi, chunk = lane & 7, r0 = lane >> 3;
+      int* const mine = rows + lw * kGwMaxGather;
+      const uint32_t even = r0 * 128 + ((chunk ^ r0) << 4), odd = even ^ 64;  // rows 8 i + r0, 8 i + r0 + 4 (swizzled)
+      int step = 0;
+      for (int u = u_first; u < units; u += u_step) {
         const Tile tl = tile_of(u);
-        named_bar_sync(1, kGwLoad * 32);  // the previous tile's numbers are no longer needed
-        for (int r = lt; r < tl.cols; r += kGwLoad * 32) rows[r] = p.sorted[tl.row0 + min(r, tl.n - 1)] / p.topk;
-        named_bar_sync(1, kGwLoad * 32);
-        for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-          if (!(ok = w4_await<100>(&b_empty[stage], phase ^ 1))) break;
-          // a thread's rows are 16 apart, so their swizzle is the same
-          uint32_t dst = smem_u32(smem) + stage * stage_bytes + r0 * 128 + ((chunk ^ (r0 & 7)) << 4);
+        __syncwarp();  // the previous tile's numbers are no longer needed
+        for (int r = lane; r < tl.cols; r += 32) mine[r] = p.sorted[tl.row0 + min(r, tl.n - 1)] / p.topk;
+        __syncwarp();
+        for (int ks = 2 * k0; ks < 2 * k1; ++ks, ++step) {
+          if (step % kGwLoad != lw) continue;
+          const int st = step % kGwB;
+          if (ok) ok = w4_await(&b_empty[st], (step / kGwB & 1) ^ 1);
+          __syncwarp();
+          uint32_t dst = smem_u32(smem) + st * stage_bytes;
           const int k = ks * 64 + chunk * 8;
           const uint32_t bytes = k < p.w.k ? 16 : 0;  // zeros beyond the last input
           const __nv_bfloat16* src = p.in + min(k, p.w.k - 8);
-          for (int r = r0; r < tl.cols; r += kRows, dst += kRows * 128)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                         "l"(src + (int64_t)rows[r] * p.in_stride), "r"(bytes)
-                         : "memory");
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (++behind > kGwLag) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kGwLag) : "memory");
-            announce();
-            --behind;
+#pragma unroll 2
+          for (int r = r0; r < tl.cols; r += 8, dst += 1024) {
+            cp_async_zfill(dst + even, src + (int64_t)mine[r] * p.in_stride, bytes);
+            cp_async_zfill(dst + 512 + odd, src + (int64_t)mine[r + 4] * p.in_stride, bytes);
           }
-          if (++stage == kGwB) stage = 0, phase ^= 1;
+          asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b_full[st]);
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      for (; behind > 0; --behind) announce();
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------------ records
@@ -309,7 +309,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       const int n = min(kRecs, p.w.tiles - tl.nt * kRecs);
       const uint8_t* src = p.w.data + (((int64_t)tl.e * p.w.tiles + tl.nt * kRecs) * p.w.kc + k0) * bytes;
       for (int kb = k0; kb < k1; ++kb, src += bytes) {
-        if (!(ok = w4_await<100>(&raw_empty[slot], phase ^ 1))) break;
+        if (!(ok = w4_await(&raw_empty[slot], phase ^ 1))) break;
         if (elect_one()) {
           mbar_expect_tx_a(full0 + slot * 8, n * bytes);
 #pragma unroll
@@ -329,34 +329,31 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     for (int u = u_first; u < units && ok; u += u_step, ++use) {
       const Tile tl = tile_of(u);
       const uint32_t idesc = idesc_bf16_f32(128, tl.cols), d = set_of(use) * H * half_cols;
-      if (!(ok = w4_await<20>(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
+      if (!(ok = w4_await(&tempty[set_of(use)], set_phase(use) ^ 1))) break;
       tc_fence_after();
+      bool acc = false;
       for (int ks = 2 * k0; ks < 2 * k1; ++ks) {
-        if (!(ok = w4_await<0>(&b_full[bstage], bphase))) break;
+        if (!(ok = w4_await(&b_full[bstage], bphase))) break;
         const uint64_t b = smem_desc_sw128(smem_u32(smem) + bstage * stage_bytes);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (FINE || e == 0) {
-            if (ok) ok = w4_await<0>(&a_full[stage], phase);
-            if (!ok) break;
-            tc_fence_after();
-          }
+        for (int e = 0; e < 2; e += FINE ? 1 : 2) {
+          if (!(ok = w4_await(&a_full[stage], phase))) break;
+          tc_fence_after();
           const uint32_t a = 512 - (S - stage) * H * kCols;
           if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < (FINE ? 2 : 4); ++j)
 #pragma unroll
               for (int h = 0; h < H; ++h)
-                tc_mma_f16_ts(d + h * half_cols, a + h * kCols + (FINE ? 0 : e * 16) + j * 8, b + e * 4 + j * 2, idesc,
-                              ks > 2 * k0 || e > 0 || j > 0);
-            if (FINE || e == 1) tc_commit(&a_empty[stage]);
-            if (e == 1) tc_commit(&b_empty[bstage]);
+                tc_mma_f16_ts(d + h * half_cols, a + h * kCols + j * 8, b + e * 4 + j * 2, idesc, acc || e > 0 || j > 0);
+            tc_commit(&a_empty[stage]);
+            if (!FINE || e == 1) tc_commit(&b_empty[bstage]);
           }
           __syncwarp();
-          if (FINE || e == 1)
-            if (++stage == S) stage = 0, phase ^= 1;
+          if (++stage == S) stage = 0, phase ^= 1;
         }
         if (!ok) break;
+        acc = true;
         if (++bstage == kGwB) bstage = 0, bphase ^= 1;
       }
       if (elect_one()) tc_commit(&tfull[set_of(use)]);
@@ -387,7 +384,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
       const Tile tl = tile_of(u);
       const bool there = tl.nt * kRecs + ti < p.w.tiles;
       for (int kb = k0; kb < k1; ++kb) {
-        if (!(ok = w4_await<20>(&raw_full[slot], rphase))) break;
+        if (!(ok = w4_await(&raw_full[slot], rphase))) break;
         const uint32_t rec = raw0 + slot * p.raw_bytes + ti * bytes;
         uint4 q[H] = {};
         uint2 s[2] = {};
@@ -431,7 +428,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             }
           }
           if (FINE || e == 0) {
-            if (ok) ok = w4_await<50>(&a_empty[stage], phase ^ 1);
+            if (ok) ok = w4_await(&a_empty[stage], phase ^ 1);
             if (!ok) break;
             tc_fence_after();
           }
@@ -517,7 +514,7 @@ inline bool w4_rows_map(CUtensorMap* m, const void* base, int64_t rows, int64_t 
 template <int MODE, int H, bool SPLIT, bool FINE, bool Z, bool F>
 int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   constexpr auto kernel = w4_gemm_kernel<MODE, H, SPLIT, FINE, Z, F>;
-  constexpr int kMax = 227 * 1024;
+  constexpr int kMax = 227 * 1024, kGwB = w4_row_stages(MODE);
   if (msgl_set_smem<kernel>(kMax) != cudaSuccess) return 4;
   // Tensor memory's 512 columns: two sets of accumulators if two steps of A fit beside them, else one and up to
   // eight stages. Shared memory: four stages of the tokens' rows, and up to eight steps' records (a copy
@@ -529,7 +526,7 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   // A team of converters waits for a stage's turn by the parity of its phase, and takes every other step: its last wait
   // must have shown that all but the latest of the stage's turns are over. That is so with two stages of a step, or
   // three of half a step.
-  if (p.stages < (FINE ? 3 : 2)) return 3;
+  if (p.stages < (FINE ? 3 : 2) || (MODE == kW4GateUp && p.bn > kGwMaxGather)) return 3;
   p.raw_bytes = 4 * H * (W4Record<128, false>::kScales + 128 / p.group * (Z ? 96 : 64));
   const int room = kGwRoom, stage = p.bn * 128;
   p.slots = std::min(kGwMaxSlots, (room - kGwB * stage) / p.raw_bytes);

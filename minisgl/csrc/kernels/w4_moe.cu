@@ -246,7 +246,7 @@ int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
   });
 }
 
-constexpr int kTileTokens = 96;  // of a tile: two sets of accumulators then fit into tensor memory
+constexpr int kTileTokens = kGwMaxGather;  // 96 of a tile: two sets of accumulators then fit into tensor memory
 
 // Sorts the pairs by expert (in any order within one: a pair's result does not depend on its place) and cuts
 // every expert's into equal tiles. One CTA.
