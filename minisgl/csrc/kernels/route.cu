@@ -294,7 +294,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
   const float near = 2.f * (rel * top_p + 0x1p-23f * most);
   bool exact = !(most < 0x1p100f);  // sums of such would overflow
 
-  if (GROUPS && a.groups > 32) exact = true;
+  if (GROUPS && a.groups > 32) exact = true;  // more groups than lanes
   if (GROUPS && !exact) {
     // L lanes share a group: each keeps its two largest, and they merge. The groups lie L words further apart
     // than their size, so that groups of 32 do not meet in the banks.

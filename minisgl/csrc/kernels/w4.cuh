@@ -20,6 +20,8 @@
 // the exponent of 128 is the bf16 value 128 + c), the group's products go through mma.sync into fp32, and
 // the group's scale multiplies the fp32 sums: nothing is rounded before the result. The inputs' order
 // inside 16 is the same permutation on both sides, which is why no shuffle is needed.
+// 1 x 34816 x 5120, groups of 128: 20.9 us, 4.4 TB/s, of which about 5 us are the launch, the first copies and the last
+// tiles; 16 x 34816 x 5120 27 us (twice the products a record: the issue slots bound it).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -145,8 +147,9 @@ MSGL_DEVICE float2 w4_scales(uint32_t v) {
   return make_float2(bf16_lo(v), bf16_hi(v));
 }
 
-// A wait that did not succeed at once. The hardware may hold the warp until the phase is over or 2 us have passed (looks
-// 40 ns apart by each of 26 warps took most of an SM's issue slots). Bounded to a few seconds; false when they are over.
+// A wait that did not succeed at once. try_wait may hold the warp until the phase is over or 2 us have passed (looks 20
+// to 40 ns apart by each of 26 warps took a third of an SM's issue slots). Bounded to a few seconds; false when they are
+// over.
 static __noinline__ __device__ bool w4_wait(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < 1 << 21; ++i)
     if (mbar_try_wait_a(bar, parity, 2000)) return true;

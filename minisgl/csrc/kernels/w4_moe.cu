@@ -9,6 +9,9 @@
 //
 // Many tokens: a kernel sorts the pairs by expert and lists tiles of up to 96 of an expert's pairs; the products
 // run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
+//
+// 128 experts of 2048 x 768, 8 a token, groups of 128, whole layer: 1 token 17.9 us (3.0 for the bytes; three launches
+// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 161 (48), 2048 tokens 336 (92).
 #include <algorithm>
 
 #include "w4_gemm.cuh"
@@ -238,7 +241,8 @@ int launch_experts(ExpertArgs p, cudaStream_t s) {
 }
 
 // One product. Token columns per pass: 8 while an expert has at most 4 tokens on average (its tokens then
-// rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2.
+// rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of
+// 2048 x 768: at 4 tokens 77 us with columns of 8 and 81 with 16, at 8 tokens 112 and 100.
 template <bool GATED>
 int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
   return w4_dispatch(w, [&](auto g, auto z, auto f) {
@@ -320,7 +324,8 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
   return s;
 }
 
-// Pairs per expert up to which the streaming product is taken.
+// Pairs per expert up to which the streaming product is taken (128 experts of 2048 x 768: at 8 a layer takes 100 us
+// streaming and 114 on the tensor core, at 16 it takes 138 and 134).
 constexpr int kStreamPairs = 8;
 
 int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
@@ -387,7 +392,8 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   }
   if (rc != 0) return rc;
   return msgl_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),
-                     stream ? (const int32_t*)nullptr : (const int32_t*)(ws + sc.place), weights, ids, E, e0, topk, w2->n, (__nv_bfloat16*)out) == cudaSuccess
+                     stream ? (const int32_t*)nullptr : (const int32_t*)(ws + sc.place), weights, ids, E, e0, topk, w2->n,
+                     (__nv_bfloat16*)out) == cudaSuccess
              ? 0
              : 4;
 }
