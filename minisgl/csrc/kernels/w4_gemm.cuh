@@ -12,7 +12,7 @@
 //                scale. Half of them take the even steps, half the odd ones: one half converts while the other
 //                waits for its barriers and its stores.
 // What bounds it is the conversion's issue slots (about 1000 warp instructions of a step's 2000) and, next to it, the
-// latency of one step through conversion, MMA and release: 640 clocks a step with few tokens, 17 x 34816 x 5120 34 us;
+// latency of one step through conversion, MMA and release: 640 clocks a step with few tokens, 17 x 34816 x 5120 33 us;
 // 200 x 34816 x 5120 57 us, 1.26 PFLOP/s, 75% of a measured bf16 product's rate; 1024 tokens 276 us, 79%.
 // A comes from tensor memory because shared memory's 128 bytes a clock were the limit with A tiles there
 // (200 tokens: 143 KB a step, of which A written and read 64): 72 us at 200 x 34816 x 5120.
@@ -386,23 +386,20 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
     constexpr int kStages = FINE ? 2 : 1;  // of a step
     if (block == 1) advance(kStages);
     for (int u = u_first; u < units && ok; u += u_step) {
-      const Tile tl = tile_of(u);
-      const bool there = tl.nt * kRecs + ti < p.w.tiles;
       for (int kb = k0; kb < k1; ++kb) {
         if (!(ok = w4_await(&raw_full[slot], rphase))) break;
+        // (records behind the weight's last one are whatever the slot holds: their rows of the result are not stored)
         const uint32_t rec = raw0 + slot * p.raw_bytes + ti * bytes;
-        uint4 q[H] = {};
-        uint2 s[2] = {};
-        uint32_t z[2] = {0x08080808u, 0x08080808u};
-        if (there) {
+        uint4 q[H];
+        uint2 s[2];
+        uint32_t z[2];
 #pragma unroll
-          for (int i = 0; i < H; ++i) q[i] = lds128(rec + ((H == 2 ? i : m) * 2 + block) * 512 + lane * 16);
+        for (int i = 0; i < H; ++i) q[i] = lds128(rec + ((H == 2 ? i : m) * 2 + block) * 512 + lane * 16);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int grp = (2 * block + e) >> shift;
-            s[e] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
-            if constexpr (Z) z[e] = lds32(rec + zoff + grp * 32 + g * 4);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int grp = (2 * block + e) >> shift;
+          s[e] = lds64(rec + W4Record<128, false>::kScales + grp * 64 + g * 8);
+          z[e] = Z ? lds32(rec + zoff + grp * 32 + g * 4) : 0x08080808u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[slot]);

@@ -11,7 +11,7 @@
 // run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
 //
 // 128 experts of 2048 x 768, 8 a token, groups of 128, whole layer: 1 token 17.9 us (3.0 for the bytes; three launches
-// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 161 (48), 2048 tokens 336 (92).
+// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 159 (48), 2048 tokens 332 (92).
 #include <algorithm>
 
 #include "w4_gemm.cuh"
@@ -325,7 +325,7 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
 }
 
 // Pairs per expert up to which the streaming product is taken (128 experts of 2048 x 768: at 8 a layer takes 100 us
-// streaming and 114 on the tensor core, at 16 it takes 138 and 134).
+// streaming and 114 on the tensor core, at 16 it takes 138 and 133).
 constexpr int kStreamPairs = 8;
 
 int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
