@@ -371,8 +371,9 @@ struct W4Runs {
 // The rarer activations are a call: inlined copies would lengthen a short launch by their first execution.
 static __noinline__ __device__ float w4_other_act(float g, float u, int act) {
   if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-  g = fminf(g, 7.f);
-  u = fminf(fmaxf(u, -7.f), 7.f);
+  // by comparison: fminf and fmaxf would drop a NaN
+  g = g > 7.f ? 7.f : g;
+  u = u > 7.f ? 7.f : u < -7.f ? -7.f : u;
   return g / (1.f + __expf(-1.702f * g)) * (u + 1.f);
 }
 MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
