@@ -464,13 +464,16 @@ __global__ void __launch_bounds__(kRouteWarps * 32, route_ctas(GROUPS)) route_ex
     for (int i = 0; i < PER; ++i) next[i] = FULL || lane + 32 * i < E ? logit_of(row + 32 * i) : 0.f;
   };
   int t = blockIdx.x * kRouteWarps + warp;
-  if (t < a.n_tok) fetch(t);
-  for (; t < a.n_tok; t += step) {
+  if (t >= a.n_tok) return;
+  fetch(t);
+  for (;; t += step) {
     float x[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) x[i] = next[i];
-    if (t + step < a.n_tok) fetch(t + step);
+    const bool more = a.n_tok - t > step;  // (t + step may be beyond 31 bits)
+    if (more) fetch(t + step);
     route_token<T, PER, GROUPS, FULL>(a, le, base + (int64_t)t * a.stride, t, scratch, x);
+    if (!more) return;
     __syncwarp();
   }
 }
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, route_ctas(GROUPS)) route_ex
 template <typename T, int PER>
 cudaError_t launch_route_per(const RouteArgs& a, cudaStream_t s) {
   const size_t smem = (size_t)kRouteWarps * (2 * a.E + 32) * sizeof(double);
-  const int ctas = (a.n_tok + kRouteWarps - 1) / kRouteWarps, most = msgl_num_sms() * route_ctas(a.groups > 1);
+  const int ctas = (a.n_tok - 1) / kRouteWarps + 1, most = msgl_num_sms() * route_ctas(a.groups > 1);
   const dim3 grid(ctas < most ? ctas : most), block(kRouteWarps * 32);
   if (a.E == 32 * PER)
     return a.groups > 1 ? msgl_launch(route_experts_kernel<T, PER, true, true>, grid, block, smem, s, 1, a)

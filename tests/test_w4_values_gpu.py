@@ -48,3 +48,13 @@ def test_infinite_factors_are_clamped(T):
     far = b1.clamp(-1e30, 1e30)
     assert torch.equal(ops.experts_w4(x, w1, w2, weights, ids, activation="swiglu_oai", w1_bias=b1),
                        ops.experts_w4(x, w1, w2, weights, ids, activation="swiglu_oai", w1_bias=far))
+
+
+def test_route_most_tokens():
+    """As many tokens as a call takes: the last ones' numbers plus a grid's warps are beyond 31 bits."""
+    T = 2 ** 31 - 1
+    weights, ids = ops.route_experts(torch.ones(1, 1, device=DEV, dtype=torch.bfloat16).expand(T, 1), 1)
+    assert ids.shape == (T, 1)
+    assert not bool(ids.any()) and bool((weights == 1).all())
+    with pytest.raises((RuntimeError, ValueError)):
+        ops.route_experts(torch.ones(1, 1, device=DEV).expand(T + 1, 1), 1)
