@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_linear_kernel(const __
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int m = nt * 8 + 2 * t + c;
-          if (m < p.M) p.out[(int64_t)m * p.w.n + n] = __float2bfloat16(acc[r >> 1][nt][2 * (r & 1) + c] + b);
+          if (m < p.M) p.out[(int64_t)m * p.w.n + n] = __float2bfloat16(acc[r >> 1][nt][2 * (r & 1) + c] * kW4Unit + b);
         }
     }
   };

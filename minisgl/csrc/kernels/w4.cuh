@@ -17,9 +17,11 @@
 // producer warp for all rings measured 38 us, cp.async by every lane 27 us, bulk copies of 16-row records
 // 25 us: what is left of an SM's issue slots beside the conversion decides.) A word of eight codes
 // becomes one A fragment with two logic instructions and one exact subtraction per pair (a code c under
-// the exponent of 128 is the bf16 value 128 + c), the group's products go through mma.sync into fp32, and
-// the group's scale multiplies the fp32 sums: nothing is rounded before the result. The inputs' order
-// inside 16 is the same permutation on both sides, which is why no shuffle is needed.
+// the exponent of 2^-4 is the bf16 value 2^-4 + c 2^-11), the group's products go through mma.sync into fp32, and
+// the group's scale multiplies the fp32 sums: nothing is rounded before the result. The sums are 2^-11 of the result
+// until they are given away, so that a group's 128 products with codes of up to 15 stay in range whatever finite value
+// the activations have. The inputs' order inside 16 is the same permutation on both sides, which is why no shuffle is
+// needed.
 // 1 x 34816 x 5120, groups of 128: 20.9 us, 4.4 TB/s, of which about 5 us are the launch, the first copies and the last
 // tiles; 16 x 34816 x 5120 27 us (twice the products a record: the issue slots bound it).
 #pragma once
@@ -133,10 +135,15 @@ MSGL_DEVICE void mma_bf16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t 
   }
 }
 
-// two codes (bits 0-3 and 16-19 of v) minus a zero point (given as 128 + zero in both halves), exactly
+// bf16 pairs whose last bit is a code's unit: 128 + code, and 2^-4 + code 2^-11
+constexpr uint32_t kW4Whole = 0x43004300u, kW4Small = 0x3d803d80u;
+constexpr float kW4Unit = 2048.f;  // of a code under kW4Small, inverted
+
+// two codes (bits 0-3 and 16-19 of v) under a base minus a zero point (base + zero in both halves), exactly
+template <uint32_t BASE>
 MSGL_DEVICE uint32_t codes_bf16x2(uint32_t v, uint32_t zero) {
   uint32_t c;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(c) : "r"(v));  // (v & 0x000f000f) | 0x43004300
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(c) : "r"(v), "n"(BASE));  // (v & 0x000f000f) | base
   const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&c), *reinterpret_cast<__nv_bfloat162*>(&zero));
   return *reinterpret_cast<const uint32_t*>(&d);
 }
@@ -191,7 +198,7 @@ struct W4Runs {
 
   // Products of `ntiles` tiles (absolute number tile0 on) over records [c0, c0 + nc) of each with the nx rows
   // rows row(r), r < nx <= 32, of w.k bf16 each, which are brought to xs (pitch bytes apart, column 0 = record
-  // c0's first input). emit(tile, acc) gets every tile's sums, from one warp: acc[half][nt][0..3] = rows g,
+  // c0's first input). emit(tile, acc) gets every tile's sums over kW4Unit, from one warp: acc[half][nt][0..3] = rows g,
   // g, g + 8, g + 8 of the half, of tokens 8 nt + 2 t, + 1, + 0, + 1. Tiles that several warps share are
   // summed through shared memory, in the order of the warps. Ends without a barrier: xs is free, the runs'
   // memory is for the next run only. SPLIT: nc is less than all of a tile's records.
@@ -282,16 +289,16 @@ struct W4Runs {
             uint32_t fr[2][2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t z0 = Z ? 0x43004300u + ((z[j] >> (16 * h)) & 15u) * 0x10001u : 0x43084308u;
-              const uint32_t z1 = Z ? 0x43004300u + ((z[j] >> (16 * h + 8)) & 15u) * 0x10001u : 0x43084308u;
+              const uint32_t z0 = kW4Small + (Z ? ((z[j] >> (16 * h)) & 15u) * 0x10001u : 0x00080008u);
+              const uint32_t z1 = kW4Small + (Z ? ((z[j] >> (16 * h + 8)) & 15u) * 0x10001u : 0x00080008u);
               const uint4 v4 = q[h][quarter >> 1];
               const uint32_t words[2] = {quarter & 1 ? v4.z : v4.x, quarter & 1 ? v4.w : v4.y};
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                fr[h][e][0] = codes_bf16x2(words[e], z0);
-                fr[h][e][1] = codes_bf16x2(words[e] >> 4, z1);
-                fr[h][e][2] = codes_bf16x2(words[e] >> 8, z0);
-                fr[h][e][3] = codes_bf16x2(words[e] >> 12, z1);
+                fr[h][e][0] = codes_bf16x2<kW4Small>(words[e], z0);
+                fr[h][e][1] = codes_bf16x2<kW4Small>(words[e] >> 4, z1);
+                fr[h][e][2] = codes_bf16x2<kW4Small>(words[e] >> 8, z0);
+                fr[h][e][3] = codes_bf16x2<kW4Small>(words[e] >> 12, z1);
               }
             }
 #pragma unroll

@@ -413,8 +413,8 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
           for (int i = 0; i < H; ++i) {
             const int half = H == 2 ? i : m;
             const uint32_t sv = half ? s[e].y : s[e].x, zv = z[e] >> (16 * half);
-            const uint32_t z0 = Z ? 0x43004300u + (zv & 15u) * 0x10001u : 0x43084308u;
-            const uint32_t z1 = Z ? 0x43004300u + ((zv >> 8) & 15u) * 0x10001u : 0x43084308u;
+            const uint32_t z0 = kW4Whole + (Z ? (zv & 15u) * 0x10001u : 0x00080008u);
+            const uint32_t z1 = kW4Whole + (Z ? ((zv >> 8) & 15u) * 0x10001u : 0x00080008u);
             const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
             float2 sf = make_float2(0.f, 0.f);
             if constexpr (F) sf = w4_scales<true>(sv);
@@ -423,10 +423,10 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             for (int b = 0; b < 2; ++b) {
               uint32_t* const lo = MODE == kW4GateUp ? &r[0][4 * b + 2 * i] : &r[i][4 * b];
               uint32_t* const hi = MODE == kW4GateUp ? &r[H - 1][4 * b + 2 * i] : &r[i][4 * b + 2];
-              lo[0] = w4_times<F>(codes_bf16x2(words[b], z0), sa2, sf.x);
-              hi[0] = w4_times<F>(codes_bf16x2(words[b] >> 4, z1), sb2, sf.y);
-              lo[1] = w4_times<F>(codes_bf16x2(words[b] >> 8, z0), sa2, sf.x);
-              hi[1] = w4_times<F>(codes_bf16x2(words[b] >> 12, z1), sb2, sf.y);
+              lo[0] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b], z0), sa2, sf.x);
+              hi[0] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 4, z1), sb2, sf.y);
+              lo[1] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 8, z0), sa2, sf.x);
+              hi[1] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 12, z1), sb2, sf.y);
             }
           }
           if (FINE || e == 0) {

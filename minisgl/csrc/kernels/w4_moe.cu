@@ -182,9 +182,9 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
               if (m >= nx) continue;
               if constexpr (GATED)
                 p.a[(int64_t)mine[m] * p.a_stride + n] =
-                    __float2bfloat16(w4_gated_act(acc[r][q][c] + b0, acc[r][q][2 + c] + b1, p.act));
+                    __float2bfloat16(w4_gated_act(acc[r][q][c] * kW4Unit + b0, acc[r][q][2 + c] * kW4Unit + b1, p.act));
               else
-                p.y[(int64_t)mine[m] * p.w.n + n] = acc[r >> 1][q][2 * (r & 1) + c] + b0;
+                p.y[(int64_t)mine[m] * p.w.n + n] = acc[r >> 1][q][2 * (r & 1) + c] * kW4Unit + b0;
             }
         }
       };

@@ -6,7 +6,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from minisgl import ops  # noqa: E402
-from test_w4_gpu import DEV, _codes, _cuda_only, _experts_case, _packed  # noqa: E402,F401
+from test_w4_gpu import (DEV, _check_experts, _check_linear, _codes, _cuda_only, _experts_case,  # noqa: E402,F401
+                         _experts_wide, _packed)
 
 
 # 12 and 16 pairs of 4 experts: the streaming product; 300: the tensor core
@@ -58,3 +59,42 @@ def test_route_most_tokens():
     assert not bool(ids.any()) and bool((weights == 1).all())
     with pytest.raises((RuntimeError, ValueError)):
         ops.route_experts(torch.ones(1, 1, device=DEV).expand(T + 1, 1), 1)
+
+
+def _check_finite(got):
+    assert bool(got.isfinite().all())
+
+
+# With codes of up to 15 a group's sum before its scale passes the end of fp32 where the result does not
+# come near it; at the other end a small unit of the codes must not lose a result that is still normal.
+@pytest.mark.parametrize("M", [1, 7, 12, 16, 40, 200])
+@pytest.mark.parametrize("power", [123, -110])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, False), (128, True)])
+def test_linear_at_the_ends_of_the_range(M, power, group, zeros):
+    q, s, z = _codes((160, 512), group, zeros)
+    x = (torch.randn(M, 512, device=DEV) * 2.0 ** power).to(torch.bfloat16)
+    got = ops.linear_w4(x, ops.W4Weight.pack(q, s, z))
+    _check_finite(got)
+    _check_linear(x, q, s, z, None, got)
+
+
+def test_linear_largest_activations():
+    """Every activation the largest bf16, every code 15 and its zero point 0; 2^-20 brings the result back."""
+    big = torch.finfo(torch.bfloat16).max
+    for M in (1, 9, 33):
+        q = torch.full((48, 64), 255, device=DEV, dtype=torch.uint8)
+        s = torch.full((48, 1), 2.0 ** -20, device=DEV, dtype=torch.bfloat16)
+        got = ops.linear_w4(torch.full((M, 128), big, device=DEV, dtype=torch.bfloat16),
+                            ops.W4Weight.pack(q, s, torch.zeros(48, 1, device=DEV, dtype=torch.uint8)))
+        # bf16 has 8 bits: 128 * 15 * big * 2^-20 is (2 - 2^-7) * 15 * 2^114, rounded once
+        assert bool((got == torch.tensor(128.0 * 15 * big * 2.0 ** -20, dtype=torch.float64).to(torch.bfloat16).item()).all())
+
+
+@pytest.mark.parametrize("T", [3, 8, 60])
+def test_experts_of_large_activations(T):
+    """Activated values of about 2^122, results below 2^127."""
+    x, c1, c2, weights, ids = _experts_case(T, 4, 2, 256, 256, 128, 128, False)
+    x = (x.float() * 2.0 ** 60).to(torch.bfloat16)
+    got = ops.experts_w4(x, *_packed(c1, c2), weights, ids)
+    _check_finite(got)
+    _check_experts(got, *_experts_wide(x, c1, c2, weights, ids))
