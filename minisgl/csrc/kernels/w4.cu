@@ -138,7 +138,7 @@ int launch_linear_nt(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
 // Tokens up to which the streaming product is taken (one or two columns of 8).
 constexpr int kStreamTokens = 16;
 
-// rows in one launch if their activations fit into shared memory, else in parts
+// rows in one launch if their activations fit into shared memory, else in parts; 3 if not one row does
 int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   const int rc = p.M <= 8 ? launch_linear_nt<1>(p, w, s) : launch_linear_nt<2>(p, w, s);
   if (rc != 3 || p.M == 1) return rc;
@@ -198,7 +198,8 @@ extern "C" int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M,
   if (M == 0) return 0;
   const LinearArgs p = {w4_tensor(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias,
                         (__nv_bfloat16*)out, 1, 0};
-  return M <= kStreamTokens ? linear_rows(p, w, s) : linear_tiles(p, w, s);
+  const int rc = M <= kStreamTokens ? linear_rows(p, w, s) : 3;
+  return rc == 3 ? linear_tiles(p, w, s) : rc;
 }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4)

@@ -225,16 +225,18 @@ __global__ void __launch_bounds__(128) w4_combine_kernel(const float* __restrict
   }
 }
 
+// 3 if not even one token's inputs fit beside the rings and lists; `launch` false: only says so
 template <int NT, int G, bool Z, bool F, bool GATED>
-int launch_experts(ExpertArgs p, cudaStream_t s) {
+int launch_experts(ExpertArgs p, bool launch, cudaStream_t s) {
   constexpr auto kernel = w4_experts_kernel<NT, G, Z, F, GATED>;
-  if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
   constexpr int kRun = w4_run_bytes<NT, G, Z>();
   const int pitch = w4_pitch(p.w.kc * 128);
   p.rows = std::min(NT * 8, (kSmemMax - kRun - prelude_bytes(p.E, p.pairs, 1)) / pitch);
   if (p.rows < 1) return 3;
   const int64_t most = (int64_t)(std::min(p.E, p.pairs) + p.pairs / p.rows) * p.w.tiles;
   if (most * 2 >= (1ll << 31)) return 3;
+  if (!launch) return 0;
+  if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
   const int smem = kRun + prelude_bytes(p.E, p.pairs, p.rows) + p.rows * pitch;
   const int grid = (int)std::min<int64_t>(msgl_num_sms(), most);
   return msgl_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
@@ -244,9 +246,10 @@ int launch_experts(ExpertArgs p, cudaStream_t s) {
 // rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of
 // 2048 x 768: at 4 tokens 77 us with columns of 8 and 81 with 16, at 8 tokens 112 and 100.
 template <bool GATED>
-int experts_product(const ExpertArgs& p, const MsglW4* w, cudaStream_t s) {
+int experts_product(const ExpertArgs& p, const MsglW4* w, bool launch, cudaStream_t s) {
   return w4_dispatch(w, [&](auto g, auto z, auto f) {
-    return p.pairs <= 4 * p.E ? launch_experts<1, g(), z(), f(), GATED>(p, s) : launch_experts<2, g(), z(), f(), GATED>(p, s);
+    return p.pairs <= 4 * p.E ? launch_experts<1, g(), z(), f(), GATED>(p, launch, s)
+                              : launch_experts<2, g(), z(), f(), GATED>(p, launch, s);
   });
 }
 
@@ -377,16 +380,18 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   const int pairs = T * topk, a_stride = w2->kc * 128;
   uint8_t* ws = (uint8_t*)workspace;
   const Scratch sc = scratch_of(pairs, E, w2);
+  __nv_bfloat16* a = (__nv_bfloat16*)(ws + sc.a);
+  const ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, ids, (const __nv_bfloat16*)x, x_stride, (const __nv_bfloat16*)b1,
+                         a, nullptr, a_stride, act, 0};
+  const ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, ids, a, a_stride, (const __nv_bfloat16*)b2, nullptr,
+                         (float*)(ws + sc.y), 0, 0, 0};
+  // (experts of some 20,000 inputs and more may not fit the streaming products)
+  const bool stream = pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs && experts_product<true>(p1, w1, false, s) == 0 &&
+                      experts_product<false>(p2, w2, false, s) == 0;
   int rc;
-  const bool stream = pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs;
   if (stream) {
-    __nv_bfloat16* a = (__nv_bfloat16*)(ws + sc.a);
-    ExpertArgs p1 = {w4_tensor(w1), E, e0, pairs, topk, ids, (const __nv_bfloat16*)x, x_stride, (const __nv_bfloat16*)b1,
-                     a, nullptr, a_stride, act, 0};
-    ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, ids, a, a_stride, (const __nv_bfloat16*)b2, nullptr,
-                     (float*)(ws + sc.y), 0, 0, 0};
-    rc = experts_product<true>(p1, w1, s);
-    if (rc == 0) rc = experts_product<false>(p2, w2, s);
+    rc = experts_product<true>(p1, w1, true, s);
+    if (rc == 0) rc = experts_product<false>(p2, w2, true, s);
   } else {
     rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, ids, b1, b2, act, ws, sc, s);
   }

@@ -1,0 +1,73 @@
+"""Every form of the 4-bit products for many tokens, against 64-bit sums of the same rounded weights.
+
+Above 16 tokens (experts: 8 pairs an expert) a weight is (code - zero) * scale rounded to bf16. That
+rounding is part of the form, so the oracle makes it too, and what is left is narrow: the sums' chains of at most
+K / 16 + 64 additions in fp32, 2^-23 of the sum of magnitudes each, and one rounding of the result, 2^-8.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from minisgl import ops  # noqa: E402
+from test_w4_gpu import A, DEV, R, _codes, _cuda_only, _near, _packed, _wide  # noqa: E402,F401
+
+
+def _check_tiles(x, q, s, z, bias, got):
+    m, xd = _wide(q, s, z).to(torch.bfloat16).double(), x.double()
+    want, size = xd @ m.t(), xd.abs() @ m.abs().t()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    assert got.shape == want.shape and got.dtype == torch.bfloat16
+    _near(got, want, R * want.abs() + (x.shape[1] / 16 + 64) * A * size)
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 20])
+def test_linear_of_very_wide_rows(M):
+    """Not even one row fits beside the streaming product's rings: the form for many tokens, whatever their number."""
+    q, s, z = _codes((33, 460800), 128, False)
+    x = torch.randn(M, 460800, device=DEV).to(torch.bfloat16)
+    _check_tiles(x, q, s, z, None, ops.linear_w4(x, ops.W4Weight.pack(q, s, z)))
+
+
+def _experts_rounded(x, c1, c2, weights, ids, offset=0):
+    """(result, bound) of silu experts as the form for many tokens computes them: weights and activated values
+    rounded to bf16. The fp32 sums move an activated value a little; where that reaches the middle between
+    two bf16 values it may become the other one, and the step goes through the second product."""
+    E, H, inter = c1[0].shape[0], c2[0].shape[1], c1[0].shape[1] // 2
+    out = torch.zeros(x.shape[0], H, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(out)
+    for e in range(E):
+        tok, slot = torch.nonzero(ids == e + offset, as_tuple=True)
+        if len(tok) == 0:
+            continue
+        m1, m2 = (_wide(*(None if t is None else t[e] for t in c)).to(torch.bfloat16).double() for c in (c1, c2))
+        xd = x[tok].double()
+        h, dh = xd @ m1.t(), (x.shape[1] / 16 + 64) * A * (xd.abs() @ m1.abs().t())
+        g, u, dg, du = h[:, :inter], h[:, inter:], dh[:, :inter], dh[:, inter:]
+        silu = g * torch.sigmoid(g)
+        a = silu * u
+        # silu's slope is at most 1.1; the fast exponential is off by 2 + 1.2 |g| steps of fp32 and the quotient by 2
+        # (and is zero where it would be below 2^-126)
+        off = 1.1 * dg * (u.abs() + du) + silu.abs() * du + (8 + 2 * g.abs()) * A * a.abs() + 1e-35
+        rounded = a.to(torch.bfloat16).double()
+        exponent = torch.frexp((a.abs() - off).clamp(min=2.0 ** -120))[1]
+        half = torch.ldexp(torch.ones_like(a), exponent - 9)  # of a step of bf16
+        moved = torch.where((a - rounded).abs() + off >= half, off + 2 * R * (a.abs() + off), torch.zeros_like(a))
+        w = weights[tok, slot, None].double()
+        out.index_add_(0, tok, w * (rounded @ m2.t()))
+        bound.index_add_(0, tok, w.abs() * (moved @ m2.abs().t()
+                                            + (inter / 16 + 64 + ids.shape[1]) * A * (rounded.abs() @ m2.abs().t())))
+    return out, R * out.abs() + bound
+
+
+@pytest.mark.parametrize("T,E,H,inter", [(1, 2, 65536, 32), (4, 2, 65536, 32), (3, 2, 64, 65536), (16, 2, 64, 65536)])
+def test_experts_of_very_wide_rows(T, E, H, inter):
+    c1, c2 = _codes((E, 2 * inter, H), 32, False), _codes((E, H, inter), 32, True)
+    c1[1].mul_(0.02)
+    x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
+    ids = torch.arange(T, device=DEV, dtype=torch.int32)[:, None] % E
+    weights = torch.rand(T, 1, device=DEV)
+    want, bound = _experts_rounded(x, c1, c2, weights, ids)
+    _near(ops.experts_w4(x, *_packed(c1, c2), weights, ids), want, bound)
