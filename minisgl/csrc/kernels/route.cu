@@ -265,10 +265,11 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
     }
   }
   // Errors: a sigmoid is off by 2^-20 and a few roundings (2^-19 of the largest possible, 1), a softmax score by
-  // the roundings of its sum too (32 at most: 2^-18 of the largest, top_p), p + bias by another rounding. Values
-  // further apart than `near` are in order.
-  const float rel = a.sigmoid ? 0x1p-19f : 0x1p-18f;
-  float most = 0.f;  // largest |v|
+  // the roundings of its sum too (32 at most: 2^-18 of the largest, top_p), p + bias by its own rounding too. Values
+  // further apart than near() of the larger magnitude are in order, and so is whatever lies beyond them: a value that
+  // is far away (a bias that masks an expert) has a larger error, but not one that brings it back.
+  const float err = (a.sigmoid ? 0x1p-19f : 0x1p-18f) * top_p;
+  const auto near = [err](float v) { return 2.f * err + 0x1p-22f * fabsf(v); };
   if (!by_logit || sums) {
     if (a.sigmoid) {
 #pragma unroll
@@ -284,17 +285,11 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
         if (FULL || lane + 32 * i < E) {
           x[i] += le.bias[i];
           key[i] = key_of(x[i]);
-          most = fmaxf(most, fabsf(x[i]));
         }
-      most = warp_max(most);
-    } else {
-      most = top_p;
     }
   }
-  const float near = 2.f * (rel * top_p + 0x1p-23f * most);
-  bool exact = !(most < 0x1p100f);  // sums of such would overflow
 
-  if (GROUPS && a.groups > 32) exact = true;  // more groups than lanes
+  const bool exact = GROUPS && a.groups > 32;  // more groups than lanes
   if (GROUPS && !exact) {
     // L lanes share a group: each keeps its two largest, and they merge. The groups lie L words further apart
     // than their size, so that groups of 32 do not meet in the banks.
@@ -319,8 +314,8 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
       d = max(max(d, d2), min(c, c2));
       c = max(c, c2);
     }
-    // every lane of a group has its rank
-    const uint32_t rank = g >= a.groups ? 0u : a.top2 ? key_of(of_key(c) + of_key(d)) : c;
+    // every lane of a group has its rank (a sum is held to the finite values: beyond them 64 bits decide)
+    const uint32_t rank = g >= a.groups ? 0u : a.top2 ? key_of(fmaxf(fminf(of_key(c) + of_key(d), FLT_MAX), -FLT_MAX)) : c;
     int place = 0;
     for (int j = 0; j < a.groups; ++j) {
       const uint32_t o = __shfl_sync(0xffffffffu, rank, j * L);
@@ -332,7 +327,11 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
       const int in = __ffs(__ballot_sync(0xffffffffu, place == a.kept - 1 && g < a.groups)) - 1;
       const int out = __ffs(__ballot_sync(0xffffffffu, place == a.kept && g < a.groups)) - 1;
       const float u = of_key(__shfl_sync(0xffffffffu, rank, in)), w = of_key(__shfl_sync(0xffffffffu, rank, out));
-      if (!(u - w > 2.f * near + 0x1p-22f * fabsf(u))) stay = groups_exact(a, row, mx, scratch);
+      // values of opposite signs leave a sum smaller than its errors: the most that any group's two cancel
+      // (lanes without a group have keys of NaN, which fmaxf drops)
+      float gone = 0.f;
+      if (a.top2) gone = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fminf(of_key(c), -of_key(d)), 0.f))));
+      if (!(u - w > 2.f * near(fmaxf(fabsf(u), fabsf(w))) + 0x1p-21f * gone)) stay = groups_exact(a, row, mx, scratch);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -359,7 +358,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
     }
   uint32_t floor_key = a.topk < 32 ? max(__shfl_sync(0xffffffffu, sorted, a.topk & 31), 1u) : 1u;
   // what may be one of the k + 1 largest in truth
-  if (!by_logit && floor_key > 1u) floor_key = max(key_of(of_key(floor_key) - near), 1u);
+  if (!by_logit && floor_key > 1u) floor_key = max(key_of(of_key(floor_key) - near(of_key(floor_key))), 1u);
   uint2* cand = reinterpret_cast<uint2*>(scratch);  // {key, expert}, room for all of them
   int n = 0;
 #pragma unroll
@@ -399,7 +398,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, const LaneExpert
     const float v = of_key(ckey), next = of_key(__shfl_down_sync(0xffffffffu, ckey, 1));
     // the last candidate has nothing behind it; with 32 chosen the 33rd is not known
     const bool behind = lane < a.topk && lane + 1 < min(n, 32);
-    if (__any_sync(0xffffffffu, behind && !(v - next > near)) || (a.topk == 32 && n > 32)) {
+    if (__any_sync(0xffffffffu, behind && !(v - next > near(fmaxf(fabsf(v), fabsf(next))))) || (a.topk == 32 && n > 32)) {
       if (n > 32) {
         __syncwarp();
         route_exact<T>(a, row, t, scratch);

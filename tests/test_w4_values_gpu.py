@@ -6,8 +6,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from minisgl import ops  # noqa: E402
-from test_w4_gpu import (DEV, _check_experts, _check_linear, _codes, _cuda_only, _experts_case,  # noqa: E402,F401
-                         _experts_wide, _packed)
+from test_w4_gpu import (DEV, _check_experts, _check_linear, _check_route, _codes, _cuda_only,  # noqa: E402,F401
+                         _experts_case, _experts_wide, _packed)
 
 
 # 12 and 16 pairs of 4 experts: the streaming product; 300: the tensor core
@@ -98,3 +98,36 @@ def test_experts_of_large_activations(T):
     got = ops.experts_w4(x, *_packed(c1, c2), weights, ids)
     _check_finite(got)
     _check_experts(got, *_experts_wide(x, c1, c2, weights, ids))
+
+
+@pytest.mark.parametrize("E,groups", [(32, 1), (96, 3), (256, 1), (256, 8), (512, 16), (300, 1)])
+@pytest.mark.parametrize("values", [[-1e9], [-float("inf")], [float("nan"), -3e38], [1e9], [1e9, -1e9], [3e38, -3e38, -1e30]])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_biases_far_apart(E, groups, values, scoring):
+    """Biases that mask experts or force them, for one expert, a few, most and all but three of them."""
+    for many in (1, E // 8, E - E // 8, E - 3):
+        bias = torch.randn(E, device=DEV) * 0.1
+        at = torch.randperm(E, device=DEV)[:many]
+        bias[at] = torch.tensor(values, device=DEV).repeat(many)[:many]
+        logits = torch.randn(150, E, device=DEV) * 1.5
+        for k in (1, 8):
+            _check_route(logits, k, scoring=scoring, bias=bias)
+            if groups > 1:
+                for group_score in ("max", "top2"):
+                    _check_route(logits, k, scoring=scoring, bias=bias, num_groups=groups, top_groups=max(1, groups // 2),
+                                 group_score=group_score)
+
+
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+def test_route_whole_groups_masked(group_score):
+    """Groups without an expert to choose are passed over, and chosen from when only they are left."""
+    for mask in (-1e9, -float("inf")):
+        bias = torch.randn(256, device=DEV) * 0.1
+        bias[32:160] = mask
+        for kept in (3, 4, 6):
+            logits = torch.randn(200, 256, device=DEV)
+            kw = dict(scoring="sigmoid", bias=bias, num_groups=8, top_groups=kept, group_score=group_score)
+            _check_route(logits, 8, **kw)
+            if kept <= 4:
+                ids = ops.route_experts(logits, 8, **kw)[1]
+                assert not bool(((ids >= 32) & (ids < 160)).any())
