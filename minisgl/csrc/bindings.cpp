@@ -536,7 +536,7 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
 
 at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, int64_t group1, bool zeros1, bool fp16_1,
                       at::Tensor data2, int64_t n2, int64_t k2, int64_t group2, bool zeros2, bool fp16_2,
-                      at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0,
+                      at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0, int64_t total,
                       c10::optional<at::Tensor> b1, c10::optional<at::Tensor> b2) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
@@ -555,6 +555,7 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
   const int64_t topk = ids.size(1);
   CHECK(T * topk < (1ll << 24), "experts_w4: too many tokens for one call");
   CHECK(e0 >= 0 && e0 < (1ll << 30), "expert_offset out of range");
+  CHECK(total >= E && total < (1ll << 31), "num_experts must be at least the ", E, " experts that are here, got ", total);
   if (b1.has_value()) {
     check_bf16(*b1, "w1_bias"); check_contig(*b1, "w1_bias");
     CHECK(b1->numel() == E * n1 && b1->device() == x.device(), "w1_bias must be [E, 2 I]");
@@ -566,7 +567,7 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
   at::Tensor out = new_cuda({T, n2}, at::kBFloat16, x.device());
   at::Tensor ws = new_cuda({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, at::kByte, x.device());
   if (T == 0) return out;
-  const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0,
+  const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0, total,
                                  weights.data_ptr<float>(), ids.data_ptr<int32_t>(), opt_ptr(b1), opt_ptr(b2), act,
                                  ws.data_ptr(), stream());
   check_launch(rc, "experts_w4");

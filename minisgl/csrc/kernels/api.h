@@ -106,11 +106,12 @@ typedef struct {
 int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
                    cudaStream_t s);
 // out [T, w2.n] = sum_j weights[t, j] * w2[e] act(w1[e] x[t]), e = ids[t, j] - e0 in [0, E) (others add
-// nothing); w1 gated. Scratch of msgl_w4_experts_workspace bytes, written before it is read.
+// nothing); w1 gated. The pairs spread over `total` >= E experts, those elsewhere included. Scratch of
+// msgl_w4_experts_workspace bytes, written before it is read.
 int64_t msgl_w4_experts_workspace(int T, int topk, int E, const MsglW4* w1, const MsglW4* w2);
 int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1, const MsglW4* w2,
-                    int E, int e0, const float* weights, const int32_t* ids, const void* b1, const void* b2, int act,
-                    void* workspace, cudaStream_t s);
+                    int E, int e0, int total, const float* weights, const int32_t* ids, const void* b1, const void* b2,
+                    int act, void* workspace, cudaStream_t s);
 
 // ----- paged attention (bf16 q/kv, fp32 softmax)
 void msgl_attention_prefill(void* o, const void* q, const void* k_cache, const void* v_cache,

@@ -242,13 +242,13 @@ int launch_experts(ExpertArgs p, bool launch, cudaStream_t s) {
   return msgl_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
 }
 
-// One product. Token columns per pass: 8 while an expert has at most 4 tokens on average (its tokens then
-// rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of
+// One product of experts out of `total`. Token columns per pass: 8 while an expert has at most 4 tokens on average (its
+// tokens then rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of
 // 2048 x 768: at 4 tokens 77 us with columns of 8 and 81 with 16, at 8 tokens 112 and 100.
 template <bool GATED>
-int experts_product(const ExpertArgs& p, const MsglW4* w, bool launch, cudaStream_t s) {
+int experts_product(const ExpertArgs& p, const MsglW4* w, int total, bool launch, cudaStream_t s) {
   return w4_dispatch(w, [&](auto g, auto z, auto f) {
-    return p.pairs <= 4 * p.E ? launch_experts<1, g(), z(), f(), GATED>(p, launch, s)
+    return p.pairs <= 4ll * total ? launch_experts<1, g(), z(), f(), GATED>(p, launch, s)
                               : launch_experts<2, g(), z(), f(), GATED>(p, launch, s);
   });
 }
@@ -328,7 +328,9 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
 }
 
 // Pairs per expert up to which the streaming product is taken (128 experts of 2048 x 768: at 8 a layer takes 100 us
-// streaming and 114 on the tensor core, at 16 it takes 138 and 133).
+// streaming and 114 on the tensor core, at 16 it takes 138 and 133). Where only a share of the experts is here, pairs
+// and experts of all ranks count: 8 of 64 experts of 2880 x 2880 at 32 tokens, 8 a token, 35 us streaming and 64 on the
+// tensor core; 32 of 256 of 4096 x 1024 at 128 tokens 62 and 88.
 constexpr int kStreamPairs = 8;
 
 int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
@@ -373,7 +375,7 @@ extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, int E, const MsglW
 }
 
 extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
-                               const MsglW4* w2, int E, int e0, const float* weights, const int32_t* ids,
+                               const MsglW4* w2, int E, int e0, int total, const float* weights, const int32_t* ids,
                                const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
   if (T == 0) return 0;
   if (E > kMoeMaxExperts) return 3;
@@ -386,12 +388,12 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   const ExpertArgs p2 = {w4_tensor(w2), E, e0, pairs, topk, ids, a, a_stride, (const __nv_bfloat16*)b2, nullptr,
                          (float*)(ws + sc.y), 0, 0, 0};
   // (experts of some 20,000 inputs and more may not fit the streaming products)
-  const bool stream = pairs <= kStreamPairs * E && pairs <= kMoeMaxPairs && experts_product<true>(p1, w1, false, s) == 0 &&
-                      experts_product<false>(p2, w2, false, s) == 0;
+  const bool stream = pairs <= (int64_t)kStreamPairs * total && pairs <= kMoeMaxPairs &&
+                      experts_product<true>(p1, w1, total, false, s) == 0 && experts_product<false>(p2, w2, total, false, s) == 0;
   int rc;
   if (stream) {
-    rc = experts_product<true>(p1, w1, true, s);
-    if (rc == 0) rc = experts_product<false>(p2, w2, true, s);
+    rc = experts_product<true>(p1, w1, total, true, s);
+    if (rc == 0) rc = experts_product<false>(p2, w2, total, true, s);
   } else {
     rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, ids, b1, b2, act, ws, sc, s);
   }

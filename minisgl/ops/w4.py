@@ -191,24 +191,29 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) ->
 
 
 def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tensor, ids: torch.Tensor, *,
-               activation: str = "silu", expert_offset: int = 0, w1_bias: torch.Tensor | None = None,
-               w2_bias: torch.Tensor | None = None) -> torch.Tensor:
+               activation: str = "silu", expert_offset: int = 0, num_experts: int | None = None,
+               w1_bias: torch.Tensor | None = None, w2_bias: torch.Tensor | None = None) -> torch.Tensor:
     """``out[t] = sum_j weights[t, j] * (w2[e] act(w1[e] x[t]))`` with ``e = ids[t, j] - expert_offset``.
 
     ``w1 [E, 2I, H]`` is packed with ``gated=True``, ``w2 [E, H, I]`` without; ``weights`` fp32 and
     ``ids`` int32 ``[T, k]`` come from ``route_experts``. Ids of experts that are not here (expert
-    parallelism) add nothing. ``activation``: ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU
-    a call takes up to 1024 experts and 2^24 pairs of a token and an expert.
+    parallelism) add nothing; ``num_experts`` then says how many experts the ids are of (default: those
+    here), by which the GPU estimates how many tokens an expert gets and chooses its form. ``activation``:
+    ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU a call takes up to 1024 experts and 2^24
+    pairs of a token and an expert.
     The activated values between the two products are held in bf16, sums in fp32."""
     if not (w1.experts and w1.gated and w2.experts and not w2.gated):
         raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")
     if activation not in _ACT:
         raise ValueError(f"activation must be one of {sorted(_ACT)}, got {activation!r}")
+    total = w1.shape[0] if num_experts is None else num_experts
+    if total < w1.shape[0]:
+        raise ValueError(f"num_experts must be at least the {w1.shape[0]} experts that are here, got {num_experts}")
     if not x.is_cuda:
         if x.dim() != 2 or x.shape[1] != w1.k or w2.k != w1.n // 2 or w1.shape[0] != w2.shape[0]:
             raise ValueError(f"experts_w4: x {tuple(x.shape)}, w1 {w1.shape} and w2 {w2.shape} do not match")
         if ids.dim() != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
             raise ValueError(f"experts_w4: weights {tuple(weights.shape)} and ids {tuple(ids.shape)} must be [tokens, top_k]")
         return ref.experts_w4(x, w1, w2, weights, ids, activation, expert_offset, w1_bias, w2_bias)
-    return _cuda().experts_w4(x, *_args(w1), *_args(w2), weights, ids, _ACT[activation], expert_offset, w1_bias,
-                              w2_bias)
+    return _cuda().experts_w4(x, *_args(w1), *_args(w2), weights, ids, _ACT[activation], expert_offset, total,
+                              w1_bias, w2_bias)

@@ -31,9 +31,9 @@ def test_linear_of_very_wide_rows(M):
     _check_tiles(x, q, s, z, None, ops.linear_w4(x, ops.W4Weight.pack(q, s, z)))
 
 
-def _experts_rounded(x, c1, c2, weights, ids, offset=0):
+def _experts_rounded(x, c1, c2, weights, ids, offset=0, exact_weights=False):
     """(result, bound) of silu experts as the form for many tokens computes them: weights and activated values
-    rounded to bf16. The fp32 sums move an activated value a little; where that reaches the middle between
+    rounded to bf16 (``exact_weights``: the form for few tokens, activated values only). The fp32 sums move an activated value a little; where that reaches the middle between
     two bf16 values it may become the other one, and the step goes through the second product."""
     E, H, inter = c1[0].shape[0], c2[0].shape[1], c1[0].shape[1] // 2
     out = torch.zeros(x.shape[0], H, dtype=torch.float64, device=DEV)
@@ -42,7 +42,9 @@ def _experts_rounded(x, c1, c2, weights, ids, offset=0):
         tok, slot = torch.nonzero(ids == e + offset, as_tuple=True)
         if len(tok) == 0:
             continue
-        m1, m2 = (_wide(*(None if t is None else t[e] for t in c)).to(torch.bfloat16).double() for c in (c1, c2))
+        m1, m2 = (_wide(*(None if t is None else t[e] for t in c)) for c in (c1, c2))
+        if not exact_weights:
+            m1, m2 = m1.to(torch.bfloat16).double(), m2.to(torch.bfloat16).double()
         xd = x[tok].double()
         h, dh = xd @ m1.t(), (x.shape[1] / 16 + 64) * A * (xd.abs() @ m1.abs().t())
         g, u, dg, du = h[:, :inter], h[:, inter:], dh[:, :inter], dh[:, inter:]
@@ -71,3 +73,33 @@ def test_experts_of_very_wide_rows(T, E, H, inter):
     weights = torch.rand(T, 1, device=DEV)
     want, bound = _experts_rounded(x, c1, c2, weights, ids)
     _near(ops.experts_w4(x, *_packed(c1, c2), weights, ids), want, bound)
+
+
+@pytest.mark.parametrize("T", [9, 17, 33, 64, 65])
+@pytest.mark.parametrize("spread", ["all ranks", "one expert", "elsewhere", "here"])
+def test_experts_of_a_share_choose_by_all(T, spread):
+    """4 experts of 64, 8 a token: up to 64 tokens an expert has 8 pairs if they spread over all ranks, and the form
+    for few tokens runs whatever they do. Its results have exact weights, so the bound tells the forms apart."""
+    E, total, k, H, inter, offset = 4, 64, 8, 256, 128, 20
+    c1, c2 = _codes((E, 2 * inter, H), 64, True), _codes((E, H, inter), 128, False)
+    x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
+    lo, hi = {"all ranks": (0, total), "one expert": (22, 23), "elsewhere": (24, total), "here": (20, 24)}[spread]
+    ids = torch.randint(lo, hi, (T, k), device=DEV, dtype=torch.int32)
+    weights = torch.rand(T, k, device=DEV)
+    w1, w2 = _packed(c1, c2)
+    got = ops.experts_w4(x, w1, w2, weights, ids, expert_offset=offset, num_experts=total)
+    want, bound = _experts_rounded(x, c1, c2, weights, ids, offset, exact_weights=T <= 64)
+    _near(got, want, bound)
+    if spread == "elsewhere":
+        assert not got.any()
+    for n in (E, total + 1000):  # whatever the estimate, the same experts' results
+        other = ops.experts_w4(x, w1, w2, weights, ids, expert_offset=offset, num_experts=n)
+        few = T * k <= min(8 * n, 4096)
+        _near(other, *_experts_rounded(x, c1, c2, weights, ids, offset, exact_weights=few))
+
+
+def test_experts_refuse_fewer_than_are_here():
+    c1, c2 = _codes((4, 64, 128), 64, False), _codes((4, 128, 32), 32, False)
+    x, ids = torch.randn(2, 128, device=DEV).to(torch.bfloat16), torch.zeros(2, 2, device=DEV, dtype=torch.int32)
+    with pytest.raises((RuntimeError, ValueError)):
+        ops.experts_w4(x, *_packed(c1, c2), torch.rand(2, 2, device=DEV), ids, num_experts=3)
