@@ -520,13 +520,13 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
   c10::cuda::CUDAGuard guard(x.device());
   const MsglW4 w = w4_of({data, n, k, group, zeros, fp16}, false, x.device(), "weight");
   CHECK(data.size(0) == 1, "linear_w4 takes one matrix, not ", data.size(0), " experts");
-  at::Tensor xr = w4_rows(x, k);
   if (bias.has_value()) {
     check_bf16(*bias, "bias"); check_contig(*bias, "bias");
     CHECK(bias->numel() == n && bias->device() == x.device(), "bias size");
   }
+  CHECK(x.dim() == 2 && x.size(0) < (1ll << 30), "linear_w4: x must be [tokens, ", k, "], of less than 2^30 tokens");
   const int64_t M = x.size(0);
-  CHECK(M < (1ll << 30), "linear_w4: too many tokens for one call");
+  at::Tensor xr = w4_rows(x, k);
   at::Tensor out = new_cuda({M, n}, at::kBFloat16, x.device());
   if (M == 0) return out;
   const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
@@ -542,10 +542,10 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
   c10::cuda::CUDAGuard guard(x.device());
   const MsglW4 w1 = w4_of({data1, n1, k1, group1, zeros1, fp16_1}, true, x.device(), "w1");
   const MsglW4 w2 = w4_of({data2, n2, k2, group2, zeros2, fp16_2}, false, x.device(), "w2");
+  CHECK(x.dim() == 2, "x must be [tokens, ", k1, "], got ", x.sizes());
   const int64_t E = data1.size(0), T = x.size(0);
   CHECK(data2.size(0) == E && E <= 1024, "w1 has ", E, " experts (at most 1024), w2 ", data2.size(0));
   CHECK(k2 == n1 / 2, "w2 takes ", k2, " inputs, w1 gives ", n1 / 2);
-  at::Tensor xr = w4_rows(x, k1);
   check_i32(ids, "ids"); check_cuda(weights, "weights"); check_dtype(weights, at::kFloat, "weights");
   check_contig(weights, "weights");
   CHECK(ids.dim() == 2 && ids.size(0) == T && ids.size(1) >= 1 && weights.sizes() == ids.sizes() &&
@@ -564,6 +564,7 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
     check_bf16(*b2, "w2_bias"); check_contig(*b2, "w2_bias");
     CHECK(b2->numel() == E * n2 && b2->device() == x.device(), "w2_bias must be [E, H]");
   }
+  at::Tensor xr = w4_rows(x, k1);
   at::Tensor out = new_cuda({T, n2}, at::kBFloat16, x.device());
   at::Tensor ws = new_cuda({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, at::kByte, x.device());
   if (T == 0) return out;

@@ -63,10 +63,10 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
                   scale: float = 1.0):
     """Experts of every token: (weights fp32 ``[T, top_k]``, ids int32 ``[T, top_k]``, best first).
 
-    ``logits`` (fp32 or bf16 ``[T, E]``, E <= 512, rows may be strided) become scores by ``scoring``,
-    ``softmax`` or ``sigmoid``. Experts are chosen by score + ``bias`` (fp32 ``[E]``, a balancing bias
+    ``logits`` (fp32 or bf16 ``[T, E]``, E <= 512, may be strided) become scores by ``scoring``,
+    ``softmax`` or ``sigmoid``. Up to 32 experts are chosen by score + ``bias`` (fp32 ``[E]``, a balancing bias
     that moves the choice but not the weights), without a bias by their logit; equal ones go to the
-    lowest id, and the order is that of 64-bit arithmetic. With ``num_groups`` > 1 the experts form that
+    lowest id, and the order is that of 64-bit arithmetic. With ``num_groups`` > 1 (at most 256) the experts form that
     many groups of consecutive ids, and only those of the ``top_groups`` best are chosen from: a
     group counts by its best expert (``group_score="max"``) or by the sum of the two best scores
     (plus bias) in it (``"top2"``). The weights are the chosen scores, divided by their sum with
@@ -79,14 +79,21 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
         raise ValueError(f"scoring must be softmax or sigmoid, got {scoring!r}")
     if group_score not in ("max", "top2"):
         raise ValueError(f"group_score must be max or top2, got {group_score!r}")
-    if not logits.is_cuda:
+    if not logits.is_cuda:  # (the kernel's binding checks the same)
         if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"logits must be fp32 or bf16 [tokens, experts], got {logits.dtype} {tuple(logits.shape)}")
         T, E = logits.shape
-        if bias is not None and bias.shape != (E,):
-            raise ValueError(f"bias must be [{E}], got {tuple(bias.shape)}")
-        if E % num_groups or not 1 <= top_groups <= num_groups or not 1 <= top_k <= min(32, top_groups * (E // num_groups)):
-            raise ValueError(f"cannot choose {top_k} of {E} experts in {top_groups} of {num_groups} groups")
+        if not 1 <= E <= 512 or T >= 2**31:
+            raise ValueError(f"route_experts: 1 to 512 experts and less than 2^31 tokens, got {tuple(logits.shape)}")
+        if bias is not None:
+            if bias.dtype != torch.float32 or bias.numel() != E or bias.is_cuda or not bias.is_contiguous():
+                raise ValueError(f"bias must be contiguous fp32 [{E}] on the logits' device, got {bias.dtype} "
+                                 f"{tuple(bias.shape)} on {bias.device}")
+            bias = bias.view(E)
+        if not 1 <= num_groups <= 256 or E % num_groups:
+            raise ValueError(f"{E} experts do not split into {num_groups} groups (at most 256)")
+        if not 1 <= top_groups <= num_groups or not 1 <= top_k <= min(32, top_groups * (E // num_groups)):
+            raise ValueError(f"cannot choose {top_k} of {E} experts in {top_groups} of {num_groups} groups (at most 32)")
         if group_score == "top2" and num_groups > 1 and E // num_groups < 2:
             raise ValueError("group_score 'top2' needs two experts per group")
         return ref.route_experts(logits, top_k, scoring, bias, num_groups, top_groups, group_score, renormalize, scale)

@@ -20,6 +20,7 @@ captured in CUDA graphs; they keep no state of their own, so calls on several st
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, replace
 
 import torch
@@ -177,16 +178,34 @@ def _args(w: W4Weight):
     return w.data, w.n, w.k, w.group, w.zeros, w.scale_dtype == torch.float16
 
 
+# What the kernels' bindings check, for tensors that do not go there.
+def _check_rows(op: str, x: torch.Tensor, *weights: W4Weight):
+    k = weights[0].k
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"{op}: x must be bf16 [tokens, {k}], got {x.dtype} {tuple(x.shape)}")
+    if any(w.is_cuda for w in weights):
+        raise ValueError(f"{op}: weights must be on the activations' device")
+
+
+def _bias(name: str, b: torch.Tensor | None, shape):
+    if b is None:
+        return None
+    if b.dtype != torch.bfloat16 or b.numel() != math.prod(shape) or b.is_cuda or not b.is_contiguous():
+        raise ValueError(f"{name} must be contiguous bf16 {list(shape)} on the activations' device, got {b.dtype} "
+                         f"{tuple(b.shape)} on {b.device}")
+    return b.view(shape)
+
+
 def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ w^T (+ bias)`` for bf16 ``x [M, K]`` and a 4-bit ``w [N, K]``; bf16 ``[M, N]``. Sums are
     held in fp32. Rows of ``x`` may be strided."""
     if w.experts or w.gated:
         raise ValueError("linear_w4 takes one ungated matrix")
     if not x.is_cuda:
-        if x.dim() != 2 or x.shape[1] != w.k or (bias is not None and bias.shape != (w.n,)):
-            raise ValueError(f"linear_w4: x must be [tokens, {w.k}] and a bias [{w.n}], got {tuple(x.shape)}"
-                             + ("" if bias is None else f" and {tuple(bias.shape)}"))
-        return ref.linear_w4(x, w, bias)
+        _check_rows("linear_w4", x, w)
+        if x.shape[0] >= 2**30:
+            raise ValueError("linear_w4: too many tokens for one call")
+        return ref.linear_w4(x, w, _bias("bias", bias, (w.n,)))
     return _cuda().linear_w4(x, *_args(w), bias)
 
 
@@ -210,10 +229,20 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
     if total < w1.shape[0]:
         raise ValueError(f"num_experts must be at least the {w1.shape[0]} experts that are here, got {num_experts}")
     if not x.is_cuda:
-        if x.dim() != 2 or x.shape[1] != w1.k or w2.k != w1.n // 2 or w1.shape[0] != w2.shape[0]:
-            raise ValueError(f"experts_w4: x {tuple(x.shape)}, w1 {w1.shape} and w2 {w2.shape} do not match")
-        if ids.dim() != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
+        _check_rows("experts_w4", x, w1, w2)
+        T, E = x.shape[0], w1.shape[0]
+        if w2.k != w1.n // 2 or w2.shape[0] != E or E > 1024:
+            raise ValueError(f"experts_w4: w1 {w1.shape} and w2 {w2.shape} do not match, or are more than 1024 experts")
+        if ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] < 1 or weights.shape != ids.shape:
             raise ValueError(f"experts_w4: weights {tuple(weights.shape)} and ids {tuple(ids.shape)} must be [tokens, top_k]")
-        return ref.experts_w4(x, w1, w2, weights, ids, activation, expert_offset, w1_bias, w2_bias)
+        for name, t, dtype in (("weights", weights, torch.float32), ("ids", ids, torch.int32)):
+            if t.dtype != dtype or t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"experts_w4: {name} must be contiguous {dtype} on the activations' device")
+        if ids.numel() >= 2**24:
+            raise ValueError("experts_w4: too many tokens for one call")
+        if not 0 <= expert_offset < 2**30:
+            raise ValueError("expert_offset out of range")
+        return ref.experts_w4(x, w1, w2, weights, ids, activation, expert_offset, _bias("w1_bias", w1_bias, (E, w1.n)),
+                              _bias("w2_bias", w2_bias, (E, w2.n)))
     return _cuda().experts_w4(x, *_args(w1), *_args(w2), weights, ids, _ACT[activation], expert_offset, total,
                               w1_bias, w2_bias)

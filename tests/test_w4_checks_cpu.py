@@ -22,3 +22,61 @@ def test_num_experts_is_an_estimate_only():
         assert torch.equal(ops.experts_w4(x, w1, w2, wt, ids, expert_offset=8, num_experts=n), want)
     with pytest.raises(ValueError, match="num_experts"):
         ops.experts_w4(x, w1, w2, wt, ids, num_experts=3)
+
+
+def bad_calls(dev):
+    """(name, call) of what both forms refuse, before anything is copied or launched"""
+    logits = torch.randn(2, 512, device=dev)
+    zeros = lambda *shape, dtype=torch.float32: torch.zeros(*shape, device=dev, dtype=dtype)  # noqa: E731
+    w, w1, w2 = (t.to(dev) for t in (_weight((32, 128)), _weight((4, 64, 128), gated=True), _weight((4, 128, 32))))
+    many1, many2 = _weight((1025, 64, 32), gated=True).to(dev), _weight((1025, 32, 32)).to(dev)
+    x, wt, ids = zeros(4, 128, dtype=torch.bfloat16), zeros(4, 2), zeros(4, 2, dtype=torch.int32)
+    long = zeros(2 ** 23, 2, dtype=torch.int32)
+    route, linear, experts = ops.route_experts, ops.linear_w4, ops.experts_w4
+    bf16 = torch.bfloat16
+    return [
+        ("513 experts", lambda: route(zeros(2, 513), 2)),
+        ("no experts", lambda: route(zeros(2, 0), 1)),
+        ("512 groups", lambda: route(logits, 2, num_groups=512, top_groups=2)),
+        ("no groups", lambda: route(logits, 2, num_groups=0)),
+        ("negative groups", lambda: route(logits, 2, num_groups=-2, top_groups=-2)),
+        ("no group kept", lambda: route(logits, 2, num_groups=4, top_groups=0)),
+        ("none chosen", lambda: route(logits, 0)),
+        ("33 chosen", lambda: route(logits, 33)),
+        ("a bias in 64 bits", lambda: route(logits, 2, bias=zeros(512, dtype=torch.float64))),
+        ("a strided bias", lambda: route(logits, 2, bias=zeros(1024)[::2])),
+        ("2^31 rows", lambda: route(zeros(1, 1).expand(2 ** 31, 1), 1)),
+        ("x in 32 bits", lambda: linear(x.float(), w)),
+        ("a linear bias in 32 bits", lambda: linear(x, w, zeros(32))),
+        ("a short linear bias", lambda: linear(x, w, zeros(31, dtype=bf16))),
+        ("a strided linear bias", lambda: linear(x, w, zeros(64, dtype=bf16)[::2])),
+        ("2^30 tokens", lambda: linear(x[:1].expand(2 ** 30, 128), w)),
+        ("experts' x in 32 bits", lambda: experts(x.float(), w1, w2, wt, ids)),
+        ("experts' x of one row", lambda: experts(x[0], w1, w2, wt, ids)),
+        ("weights in 64 bits", lambda: experts(x, w1, w2, wt.double(), ids)),
+        ("ids in 64 bits", lambda: experts(x, w1, w2, wt, ids.long())),
+        ("weights turned", lambda: experts(x, w1, w2, wt.t().contiguous().t(), ids)),
+        ("no choices", lambda: experts(x, w1, w2, wt[:, :0], ids[:, :0])),
+        ("a negative offset", lambda: experts(x, w1, w2, wt, ids, expert_offset=-1)),
+        ("w1_bias in 32 bits", lambda: experts(x, w1, w2, wt, ids, w1_bias=zeros(4, 64))),
+        ("a short w2_bias", lambda: experts(x, w1, w2, wt, ids, w2_bias=zeros(4, 32, dtype=bf16))),
+        ("1025 experts here", lambda: experts(x[:, :32].contiguous(), many1, many2, wt, ids)),
+        ("2^24 pairs", lambda: experts(x[:1].expand(2 ** 23, 128), w1, w2, long.float(), long)),
+        ("fewer in all than here", lambda: experts(x, w1, w2, wt, ids, num_experts=3)),
+    ]
+
+
+@pytest.mark.parametrize("name,call", bad_calls("cpu"), ids=lambda v: v if isinstance(v, str) else "")
+def test_refused(name, call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_at_the_limits():
+    logits = torch.randn(2, 512)
+    assert ops.route_experts(logits, 32, num_groups=256, top_groups=16, bias=torch.zeros(1, 512))[1].shape == (2, 32)
+    w1, w2 = _weight((1024, 64, 32), gated=True), _weight((1024, 32, 32))
+    ids = torch.tensor([[0, 1023]], dtype=torch.int32)
+    y = ops.experts_w4(torch.ones(1, 32, dtype=torch.bfloat16), w1, w2, torch.ones(1, 2), ids,
+                       w1_bias=torch.zeros(1024, 64, dtype=torch.bfloat16), w2_bias=torch.ones(1024, 32, dtype=torch.bfloat16))
+    assert y.shape == (1, 32) and bool(y.isfinite().all())

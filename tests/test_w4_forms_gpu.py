@@ -11,6 +11,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from minisgl import ops  # noqa: E402
+from test_w4_checks_cpu import bad_calls  # noqa: E402
 from test_w4_gpu import A, DEV, R, _codes, _cuda_only, _near, _packed, _wide  # noqa: E402,F401
 
 
@@ -98,8 +99,11 @@ def test_experts_of_a_share_choose_by_all(T, spread):
         _near(other, *_experts_rounded(x, c1, c2, weights, ids, offset, exact_weights=few))
 
 
-def test_experts_refuse_fewer_than_are_here():
-    c1, c2 = _codes((4, 64, 128), 64, False), _codes((4, 128, 32), 32, False)
-    x, ids = torch.randn(2, 128, device=DEV).to(torch.bfloat16), torch.zeros(2, 2, device=DEV, dtype=torch.int32)
-    with pytest.raises((RuntimeError, ValueError)):
-        ops.experts_w4(x, *_packed(c1, c2), torch.rand(2, 2, device=DEV), ids, num_experts=3)
+def test_refused_as_on_the_cpu():
+    before = torch.cuda.memory_allocated()
+    for name, call in bad_calls(DEV):
+        torch.cuda.reset_peak_memory_stats()
+        with pytest.raises((RuntimeError, ValueError)) as what:
+            call()
+        assert not isinstance(what.value, torch.OutOfMemoryError), name
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 30
