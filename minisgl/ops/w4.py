@@ -153,7 +153,10 @@ class W4Weight:
 def quantize_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, scale_dtype: torch.dtype = torch.bfloat16):
     """Rounds ``w [(E,) N, K]`` to 4 bits, per group of ``group`` inputs: (q, scales, zeros) for
     ``W4Weight.pack``. Symmetric: the largest magnitude becomes 7 steps around a zero point of 8
-    (``zeros`` is None); otherwise the group's range, widened to hold 0, is cut into 15 steps."""
+    (``zeros`` is None); otherwise the group's range, widened to hold 0, is cut into 15 steps. Weights
+    that are not finite, or whose scale is beyond ``scale_dtype``, are refused."""
+    if scale_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"4-bit scales must be bf16 or fp16, got {scale_dtype}")
     if group not in GROUP_SIZES or w.shape[-1] % group:
         raise ValueError(f"{w.shape[-1]} inputs do not split into groups of {group} (32, 64 or 128)")
     v = w.float().unflatten(-1, (-1, group))
@@ -168,6 +171,8 @@ def quantize_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, scale
         z = torch.where(step > 0, torch.round(-lo / step), torch.zeros_like(lo)).clamp(0, 15)
         zero = z.unsqueeze(-1)
         z = z.to(torch.uint8)
+    if not bool(s.isfinite().all()):
+        raise ValueError(f"weights of up to {float(v.abs().max()):.4g} have no finite scale in {scale_dtype}")
     step = s.float().unsqueeze(-1)
     code = torch.where(step > 0, torch.round(v / step), torch.zeros_like(v)) + zero
     code = code.clamp(0, 15).to(torch.uint8).flatten(-2)

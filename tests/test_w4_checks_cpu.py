@@ -80,3 +80,21 @@ def test_at_the_limits():
     y = ops.experts_w4(torch.ones(1, 32, dtype=torch.bfloat16), w1, w2, torch.ones(1, 2), ids,
                        w1_bias=torch.zeros(1024, 64, dtype=torch.bfloat16), w2_bias=torch.ones(1024, 32, dtype=torch.bfloat16))
     assert y.shape == (1, 32) and bool(y.isfinite().all())
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("scales", [torch.bfloat16, torch.float16])
+def test_quantize_refuses_scales_that_are_not_finite(symmetric, scales):
+    """An infinite scale would make every weight of its group an infinity or NaN."""
+    w = torch.randn(4, 128, generator=torch.Generator().manual_seed(7))
+    for bad in (float("inf"), -float("inf"), float("nan"), 1e7 if scales == torch.float16 else None):
+        if bad is None:
+            continue
+        v = w.clone()
+        v[2, 77] = bad
+        with pytest.raises(ValueError, match="scale"):
+            ops.quantize_w4(v, 64, symmetric, scales)
+    q, s, z = ops.quantize_w4(w * 1e4, 64, symmetric, scales)
+    assert bool(ops.W4Weight.pack(q, s, z).dequant().isfinite().all())
+    with pytest.raises(ValueError):
+        ops.quantize_w4(w, 64, symmetric, torch.float32)
