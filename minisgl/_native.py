@@ -29,6 +29,8 @@ class _CountingModule:
                    "ipc_handle", "ipc_open", "ipc_close", "peer_grid", "nvls_grid", "nvls_flag_bytes",
                    "nvls_state_words", "nvls_ticket_offset", "gemm_force_bn", "attention_prefill_trace"}
 
+    _COUNTED = {"linear_w4", "experts_w4"}  # return how many kernels they launched beside their result
+
     def __init__(self, mod):
         self._mod = mod
 
@@ -42,11 +44,14 @@ class _CountingModule:
             def call(*args, **kwargs):
                 COUNTERS.launches += 2 if args[-2] > 1 else 1
                 return fn(*args, **kwargs)
-        else:
-            launches = 3 if name == "experts_w4" else 1  # (4 with many tokens)
-
+        elif name in self._COUNTED:
             def call(*args, **kwargs):
+                out, launches = fn(*args, **kwargs)
                 COUNTERS.launches += launches
+                return out
+        else:
+            def call(*args, **kwargs):
+                COUNTERS.launches += 1
                 return fn(*args, **kwargs)
 
         setattr(self, name, call)  # looked up once: a small call's time is mostly the host's

@@ -514,8 +514,9 @@ at::Tensor w4_rows(const at::Tensor& x, int64_t k) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
-at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_t group, bool zeros, bool fp16,
-                     c10::optional<at::Tensor> bias) {
+// (result, kernels launched)
+std::tuple<at::Tensor, int> linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_t group, bool zeros, bool fp16,
+                                      c10::optional<at::Tensor> bias) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
   const MsglW4 w = w4_of({data, n, k, group, zeros, fp16}, false, x.device(), "weight");
@@ -528,16 +529,17 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor data, int64_t n, int64_t k, int64_
   const int64_t M = x.size(0);
   at::Tensor xr = w4_rows(x, k);
   at::Tensor out = new_cuda({M, n}, at::kBFloat16, x.device());
-  if (M == 0) return out;
-  const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), stream());
+  if (M == 0) return {out, 0};
+  int launches = 0;
+  const int rc = msgl_w4_linear(out.data_ptr(), xr.data_ptr(), xr.stride(0), M, &w, opt_ptr(bias), &launches, stream());
   check_launch(rc, "linear_w4");
-  return out;
+  return {out, launches};
 }
 
-at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, int64_t group1, bool zeros1, bool fp16_1,
-                      at::Tensor data2, int64_t n2, int64_t k2, int64_t group2, bool zeros2, bool fp16_2,
-                      at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0, int64_t total,
-                      c10::optional<at::Tensor> b1, c10::optional<at::Tensor> b2) {
+std::tuple<at::Tensor, int> experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, int64_t group1, bool zeros1,
+                                       bool fp16_1, at::Tensor data2, int64_t n2, int64_t k2, int64_t group2, bool zeros2,
+                                       bool fp16_2, at::Tensor weights, at::Tensor ids, int64_t act, int64_t e0,
+                                       int64_t total, c10::optional<at::Tensor> b1, c10::optional<at::Tensor> b2) {
   check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
   const MsglW4 w1 = w4_of({data1, n1, k1, group1, zeros1, fp16_1}, true, x.device(), "w1");
@@ -567,12 +569,13 @@ at::Tensor experts_w4(at::Tensor x, at::Tensor data1, int64_t n1, int64_t k1, in
   at::Tensor xr = w4_rows(x, k1);
   at::Tensor out = new_cuda({T, n2}, at::kBFloat16, x.device());
   at::Tensor ws = new_cuda({msgl_w4_experts_workspace(T, topk, E, &w1, &w2)}, at::kByte, x.device());
-  if (T == 0) return out;
+  if (T == 0) return {out, 0};
+  int launches = 0;
   const int rc = msgl_w4_experts(out.data_ptr(), xr.data_ptr(), xr.stride(0), T, topk, &w1, &w2, E, e0, total,
                                  weights.data_ptr<float>(), ids.data_ptr<int32_t>(), opt_ptr(b1), opt_ptr(b2), act,
-                                 ws.data_ptr(), stream());
+                                 ws.data_ptr(), &launches, stream());
   check_launch(rc, "experts_w4");
-  return out;
+  return {out, launches};
 }
 
 // ----- peer-memory collectives

@@ -102,8 +102,8 @@ typedef struct {
   const void* data;  // [E][tiles][kc] records
   int tiles, kc, group, n, k, zeros, fp16;
 } MsglW4;
-// out [M, n] = x [M, k] w^T (+ bias). Returns 0, 3 on unsupported sizes, 4 if a launch failed.
-int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
+// out [M, n] = x [M, k] w^T (+ bias). Returns 0, 3 on unsupported sizes, 4 if a launch failed; `launches`: kernels.
+int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias, int* launches,
                    cudaStream_t s);
 // out [T, w2.n] = sum_j weights[t, j] * w2[e] act(w1[e] x[t]), e = ids[t, j] - e0 in [0, E) (others add
 // nothing); w1 gated. The pairs spread over `total` >= E experts, those elsewhere included. Scratch of
@@ -111,7 +111,7 @@ int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const Msgl
 int64_t msgl_w4_experts_workspace(int T, int topk, int E, const MsglW4* w1, const MsglW4* w2);
 int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1, const MsglW4* w2,
                     int E, int e0, int total, const float* weights, const int32_t* ids, const void* b1, const void* b2,
-                    int act, void* workspace, cudaStream_t s);
+                    int act, void* workspace, int* launches, cudaStream_t s);
 
 // ----- paged attention (bf16 q/kv, fp32 softmax)
 void msgl_attention_prefill(void* o, const void* q, const void* k_cache, const void* v_cache,

@@ -127,7 +127,7 @@ int launch_linear(LinearArgs p, cudaStream_t s) {
   if (pl.splits == 0) return 3;
   p.splits = pl.splits;
   p.max_tiles = pl.max_tiles;
-  return msgl_launch(kernel, dim3(pl.grid), dim3(w4_threads<NT>()), pl.smem, s, pl.splits, p) == cudaSuccess ? 0 : 4;
+  return w4_launch(kernel, dim3(pl.grid), dim3(w4_threads<NT>()), pl.smem, s, pl.splits, p) == cudaSuccess ? 0 : 4;
 }
 
 template <int NT>
@@ -194,12 +194,15 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
 }  // namespace
 
 extern "C" int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias,
-                              cudaStream_t s) {
+                              int* launches, cudaStream_t s) {
+  *launches = w4_launched = 0;
   if (M == 0) return 0;
   const LinearArgs p = {w4_tensor(w), (const __nv_bfloat16*)x, x_stride, M, (const __nv_bfloat16*)bias,
                         (__nv_bfloat16*)out, 1, 0};
-  const int rc = M <= kStreamTokens ? linear_rows(p, w, s) : 3;
-  return rc == 3 ? linear_tiles(p, w, s) : rc;
+  int rc = M <= kStreamTokens ? linear_rows(p, w, s) : 3;
+  if (rc == 3) rc = linear_tiles(p, w, s);
+  *launches = w4_launched;
+  return rc;
 }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4)

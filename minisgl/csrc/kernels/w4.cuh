@@ -387,6 +387,15 @@ MSGL_DEVICE float w4_gated_act(float g, float u, int act) {
   return act == 0 ? __fdividef(g, 1.f + __expf(-g)) * u : w4_other_act(g, u, act);
 }
 
+// kernels that a call has launched so far, and their launches
+inline thread_local int w4_launched = 0;
+template <typename... KArgs, typename... Args>
+cudaError_t w4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, const Args&... args) {
+  const cudaError_t e = msgl_launch(kernel, grid, block, smem, s, cluster, args...);
+  if (e == cudaSuccess) ++w4_launched;
+  return e;
+}
+
 // clusters of `splits` CTAs that run at once, one CTA per SM (148 SMs, in groups that are no multiples of 8)
 template <auto Kernel>
 int w4_resident_clusters(int splits, int threads) {

@@ -540,7 +540,7 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
       !w4_rows_map(&map, p.in, p.M, p.w.k, p.M == 1 ? (int64_t)p.w.k : p.in_stride, MODE == kW4Dense ? p.bn : 16))
     return 2;
   const int smem = 1024 + kGwMisc + p.ring_bytes;
-  return msgl_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
+  return w4_launch(kernel, dim3(grid), dim3(kGwThreads), smem, s, SPLIT ? p.splits : 1, p, map) == cudaSuccess ? 0 : 4;
 }
 
 // clusters of s CTAs of the dense form that run at once

@@ -239,7 +239,7 @@ int launch_experts(ExpertArgs p, bool launch, cudaStream_t s) {
   if (msgl_set_smem<kernel>(kSmemMax) != cudaSuccess) return 4;
   const int smem = kRun + prelude_bytes(p.E, p.pairs, p.rows) + p.rows * pitch;
   const int grid = (int)std::min<int64_t>(msgl_num_sms(), most);
-  return msgl_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
+  return w4_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
 }
 
 // One product of experts out of `total`. Token columns per pass: 8 while an expert has at most 4 tokens on average (its
@@ -338,7 +338,7 @@ int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const Ms
                   cudaStream_t s) {
   int32_t *sorted = (int32_t*)(ws + sc.sorted), *count = (int32_t*)(ws + sc.count);
   int4* work = (int4*)(ws + sc.work);
-  if (msgl_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, (int32_t*)(ws + sc.place), work,
+  if (w4_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, (int32_t*)(ws + sc.place), work,
                   count) != cudaSuccess)
     return 4;
   W4GemmArgs p = {};
@@ -376,7 +376,9 @@ extern "C" int64_t msgl_w4_experts_workspace(int T, int topk, int E, const MsglW
 
 extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk, const MsglW4* w1,
                                const MsglW4* w2, int E, int e0, int total, const float* weights, const int32_t* ids,
-                               const void* b1, const void* b2, int act, void* workspace, cudaStream_t s) {
+                               const void* b1, const void* b2, int act, void* workspace, int* launches,
+                               cudaStream_t s) {
+  *launches = w4_launched = 0;
   if (T == 0) return 0;
   if (E > kMoeMaxExperts) return 3;
   const int pairs = T * topk, a_stride = w2->kc * 128;
@@ -397,12 +399,13 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
   } else {
     rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, ids, b1, b2, act, ws, sc, s);
   }
-  if (rc != 0) return rc;
-  return msgl_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),
-                     stream ? (const int32_t*)nullptr : (const int32_t*)(ws + sc.place), weights, ids, E, e0, topk, w2->n,
-                     (__nv_bfloat16*)out) == cudaSuccess
-             ? 0
-             : 4;
+  if (rc == 0 &&
+      w4_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),
+                stream ? (const int32_t*)nullptr : (const int32_t*)(ws + sc.place), weights, ids, E, e0, topk, w2->n,
+                (__nv_bfloat16*)out) != cudaSuccess)
+    rc = 4;
+  *launches = w4_launched;
+  return rc;
 }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4_moe)

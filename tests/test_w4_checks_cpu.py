@@ -98,3 +98,18 @@ def test_quantize_refuses_scales_that_are_not_finite(symmetric, scales):
     assert bool(ops.W4Weight.pack(q, s, z).dequant().isfinite().all())
     with pytest.raises(ValueError):
         ops.quantize_w4(w, 64, symmetric, torch.float32)
+
+
+def test_launch_counts_come_from_the_call():
+    from types import SimpleNamespace
+
+    from minisgl._native import _CountingModule
+    from minisgl.engine.counters import COUNTERS
+
+    mod = _CountingModule(SimpleNamespace(linear_w4=lambda m: ("y", m), experts_w4=lambda m: ("z", m + 2),
+                                          route_experts=lambda: "r"))
+    before = COUNTERS.launches
+    assert mod.linear_w4(2) == "y" and COUNTERS.launches == before + 2
+    assert mod.linear_w4(0) == "y" and COUNTERS.launches == before + 2
+    assert mod.experts_w4(2) == "z" and COUNTERS.launches == before + 6
+    assert mod.route_experts() == "r" and COUNTERS.launches == before + 7

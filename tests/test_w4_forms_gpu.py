@@ -107,3 +107,22 @@ def test_refused_as_on_the_cpu():
             call()
         assert not isinstance(what.value, torch.OutOfMemoryError), name
     assert torch.cuda.max_memory_allocated() - before < 2 ** 30
+
+
+def test_kernels_are_counted():
+    """One kernel a linear call, two where 16 rows of 33024 inputs run in halves; three for few tokens of experts,
+    four for many (a plan before them)."""
+    from minisgl.engine.counters import COUNTERS
+
+    def launched(call):
+        before = COUNTERS.launches
+        call()
+        return COUNTERS.launches - before
+
+    w = ops.W4Weight.pack(*_codes((64, 33024), 128, False))
+    x = torch.randn(40, 33024, device=DEV).to(torch.bfloat16)
+    assert [launched(lambda: ops.linear_w4(x[:m], w)) for m in (0, 1, 16, 40)] == [0, 1, 2, 1]
+    w1, w2 = _packed(_codes((4, 64, 128), 64, False), _codes((4, 128, 32), 32, False))
+    x = torch.randn(40, 128, device=DEV).to(torch.bfloat16)
+    ids, wt = torch.zeros(40, 2, device=DEV, dtype=torch.int32), torch.rand(40, 2, device=DEV)
+    assert [launched(lambda: ops.experts_w4(x[:t], w1, w2, wt[:t], ids[:t])) for t in (0, 1, 16, 40)] == [0, 3, 3, 4]
