@@ -210,7 +210,7 @@ struct W4Runs {
     const int total = ntiles * nc, a = bound(total, warp), b = bound(total, warp + 1);
     // the rows first: behind the weights' copies they would wait for these
     const int kn = min(nc * 128, w.k - c0 * 128), pad = nc * 128 - kn;
-    if (warp == 0) {
+    if (warp == 0 && ok) {
       if (lane == 0) mbar_expect_tx_a(xbar(), nx * kn * 2);
       __syncwarp();
       if (lane < nx) bulk_load_a(smem_u32(xs) + lane * pitch, row(lane) + c0 * 128, kn * 2, xbar());
@@ -237,13 +237,19 @@ struct W4Runs {
     uint32_t slot = ring0 + (it % kW4Slots) * R::kBytes, bar = bars + (it % kW4Slots) * 8;
     constexpr uint32_t kOther = R::kBytes;
     static_assert(kW4Slots == 2, "the slots alternate");
-    if (a < b) fetch(slot, bar);
-    if (a + 1 < b) fetch(2 * ring0 + kOther - slot, 2 * bars + 8 - bar);
+    // A wait that fails is the last one: no copy is started after it, and those under way get as long to land.
+    int most = ok ? b : 0;  // records up to here are fetched
+    if (a < most) fetch(slot, bar);
+    if (a + 1 < most) fetch(2 * ring0 + kOther - slot, 2 * bars + 8 - bar);
     // zeros behind the last input (pad is less than 128)
     for (int i = threadIdx.x; i < nx * (pad / 8); i += w4_threads<NT>())
       *reinterpret_cast<uint4*>(xs + i / (pad / 8) * pitch + kn * 2 + i % (pad / 8) * 16) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (ok) ok = w4_wait(xbar(), runs & 1);
+    if (ok && !(ok = w4_wait(xbar(), runs & 1))) {
+      most = 0;
+      if (a < b) w4_wait(bar, (it >> 1) & 1);
+      if (a + 1 < b) w4_wait(2 * bars + 8 - bar, ((it + 1) >> 1) & 1);
+    }
     ++runs;
 
     uint32_t xrow[NT];
@@ -263,7 +269,10 @@ struct W4Runs {
         clear(acc);
         for (; i < end; ++i) {
           if (!mbar_try_wait_a(bar, (it >> 1) & 1)) {
-            if (ok) ok = w4_wait(bar, (it >> 1) & 1);
+            if (ok && !(ok = w4_wait(bar, (it >> 1) & 1))) {
+              most = 0;
+              if (i + 1 < b) w4_wait(2 * bars + 8 - bar, ((it + 1) >> 1) & 1);
+            }
           }
           ++it;
           uint4 q[2][2];
@@ -277,7 +286,7 @@ struct W4Runs {
             if constexpr (Z) z[j] = lds32(slot + zside + j * 32);
           }
           __syncwarp();  // every lane has read the slot
-          if (i + 2 < b) fetch(slot, bar);
+          if (i + 2 < most) fetch(slot, bar);
           slot = 2 * ring0 + kOther - slot;
           bar = 2 * bars + 8 - bar;
 
