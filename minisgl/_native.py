@@ -27,7 +27,7 @@ class _CountingModule:
 
     _NON_LAUNCH = {"get_error", "num_sms", "gemm_splits", "peer_flag_bytes", "peer_alloc", "peer_free",
                    "ipc_handle", "ipc_open", "ipc_close", "peer_grid", "nvls_grid", "nvls_flag_bytes",
-                   "nvls_state_words", "nvls_ticket_offset", "gemm_force_bn", "attention_prefill_trace"}
+                   "nvls_state_words", "nvls_ticket_offset", "gemm_force_bn", "w4_force_form", "attention_prefill_trace"}
 
     _COUNTED = {"linear_w4", "experts_w4"}  # return how many kernels they launched beside their result
 

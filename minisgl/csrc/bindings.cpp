@@ -710,6 +710,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_grouped", &gemm_grouped);
   m.def("route_experts", &route_experts);
   m.def("linear_w4", &linear_w4);
+  m.def("w4_force_form", [](int halves, int splits) { msgl_w4_force_form(halves, splits); });
   m.def("experts_w4", &experts_w4);
 
   m.def("moe_route", &moe_route);

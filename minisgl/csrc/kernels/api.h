@@ -105,6 +105,9 @@ typedef struct {
 // out [M, n] = x [M, k] w^T (+ bias). Returns 0, 3 on unsupported sizes, 4 if a launch failed; `launches`: kernels.
 int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M, const MsglW4* w, const void* bias, int* launches,
                    cudaStream_t s);
+// Form of the product for many tokens, for tests: 128-row halves of a tile (1, 2) and cuts of the inputs (1 to 8);
+// 0, 0: by the estimate. A form that a call cannot take is an unsupported size.
+void msgl_w4_force_form(int halves, int splits);
 // out [T, w2.n] = sum_j weights[t, j] * w2[e] act(w1[e] x[t]), e = ids[t, j] - e0 in [0, E) (others add
 // nothing); w1 gated. The pairs spread over `total` >= E experts, those elsewhere included. Scratch of
 // msgl_w4_experts_workspace bytes, written before it is read.

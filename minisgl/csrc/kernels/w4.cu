@@ -6,6 +6,7 @@
 // meet through distributed shared memory. The split is the one whose largest share of weights, plus the
 // activations that every CTA reads, is smallest (plan()).
 #include <algorithm>
+#include <atomic>
 
 #include "w4_gemm.cuh"
 
@@ -151,6 +152,9 @@ int linear_rows(const LinearArgs& p, const MsglW4* w, cudaStream_t s) {
   return ra != 0 ? ra : linear_rows(b, w, s);
 }
 
+// Form override for tests (0, 0: by the estimate): halves of a tile and cuts of the inputs. Not for concurrent use.
+std::atomic<int> g_halves{0}, g_splits{0};
+
 // many tokens: tiles of 128 or 256 rows by up to 208 tokens; where these leave SMs idle a cluster cuts the inputs
 int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   W4GemmArgs p = {};
@@ -168,10 +172,13 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   // the exchange 2000 and 20 a token and half.
   double best = 1e30;
   int halves = 1;
+  const int only_h = g_halves.load(), only_s = g_splits.load();
   for (int h = 1; h <= 2; ++h) {
+    if (only_h != 0 && h != only_h) continue;
     const int64_t units = (int64_t)((a.w.tiles + 4 * h - 1) / (4 * h)) * p.m_tiles;
     if (units >= (1ll << 31)) return 3;
     for (int s = 1; s <= std::min(8, a.w.kc); ++s) {
+      if (only_s != 0 && s != only_s) continue;
       if (s > 1 && p.bn * h * 512 > kGwRoom) continue;  // the fp32 tile does not fit
       const int at_once = h == 2 ? w4_gemm_clusters<2>(s) : w4_gemm_clusters<1>(s);
       if (at_once < 1) continue;
@@ -181,6 +188,7 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
       if (t < best) best = t, halves = h, p.splits = s;
     }
   }
+  if (p.splits == 0) return 3;
   p.n_tiles = (a.w.tiles + 4 * halves - 1) / (4 * halves);
   const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
   if (p.splits > 1) {
@@ -204,5 +212,7 @@ extern "C" int msgl_w4_linear(void* out, const void* x, int64_t x_stride, int M,
   *launches = w4_launched;
   return rc;
 }
+
+extern "C" void msgl_w4_force_form(int halves, int splits) { g_halves.store(halves), g_splits.store(splits); }
 
 MSGL_ERROR_ACCESSOR(msgl_err_w4)

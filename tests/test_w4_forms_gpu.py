@@ -126,3 +126,101 @@ def test_kernels_are_counted():
     x = torch.randn(40, 128, device=DEV).to(torch.bfloat16)
     ids, wt = torch.zeros(40, 2, device=DEV, dtype=torch.int32), torch.rand(40, 2, device=DEV)
     assert [launched(lambda: ops.experts_w4(x[:t], w1, w2, wt[:t], ids[:t])) for t in (0, 1, 16, 40)] == [0, 3, 3, 4]
+
+
+# -------------------------------------------------------------------------- every form of the many-token product
+def _side(M, form):
+    """Scale types, zero points and inputs that end inside a record, another combination for each size and form."""
+    i = M + 3 * form[0] + 5 * form[1]
+    return (32, 64, 128)[i % 3], i % 2 == 0, (torch.bfloat16, torch.float16)[i // 2 % 2]
+
+
+def _forced(form, x, q, s, z, bias):
+    from minisgl._native import cuda
+
+    cuda().w4_force_form(*form)
+    try:
+        return ops.linear_w4(x, ops.W4Weight.pack(q, s, z), bias)
+    finally:
+        cuda().w4_force_form(0, 0)
+
+
+FORMS = [(1, 1), (1, 2), (1, 5), (1, 8), (2, 1), (2, 2), (2, 3), (2, 8)]
+
+
+# up to 192 tokens a tile: whole steps in a stage; 193 to 208: half steps with 256-row tiles; 300: two tiles of tokens
+@pytest.mark.parametrize("M", [17, 64, 96, 97, 130, 192, 193, 200, 208, 209, 300])
+@pytest.mark.parametrize("form", FORMS)
+def test_linear_every_form(M, form):
+    for shift in range(3):
+        group, zeros, dtype = _side(M + shift, form)
+        N, K = 530 + 13 * shift, {32: 1184, 64: 1088, 128: 1152}[group]  # 37 x 32, 17 x 64, 9 x 128
+        q, s, z = _codes((N, K), group, zeros, dtype)
+        x = torch.randn(M, K, device=DEV).to(torch.bfloat16)
+        bias = torch.randn(N, device=DEV).to(torch.bfloat16) if shift else None
+        _check_tiles(x, q, s, z, bias, _forced(form, x, q, s, z, bias))
+
+
+@pytest.mark.parametrize("M", [64, 130, 192, 200, 700])
+@pytest.mark.parametrize("form", [(1, 1), (2, 1)])
+@pytest.mark.parametrize("group,zeros,dtype", [(32, True, torch.float16), (64, False, torch.float16), (128, False, torch.bfloat16),
+                                               (128, True, torch.bfloat16)])
+def test_linear_many_tiles_a_block(M, form, group, zeros, dtype):
+    """More tiles than SMs: blocks go on to further tiles with their rings and phases where they are."""
+    q, s, z = _codes((39700, 640), group, zeros, dtype)
+    x = torch.randn(M, 640, device=DEV).to(torch.bfloat16)
+    _check_tiles(x, q, s, z, None, _forced(form, x, q, s, z, None))
+
+
+@pytest.mark.parametrize("form", [(2, 1), (2, 3), (1, 4)])
+@pytest.mark.parametrize("group,zeros,dtype", [(32, True, torch.float16), (128, False, torch.bfloat16)])
+def test_linear_long_inputs(form, group, zeros, dtype):
+    """Some hundred steps a tile: the rings turn many times."""
+    for M in (40, 200):
+        q, s, z = _codes((1000, 17408), group, zeros, dtype)
+        x = torch.randn(M, 17408, device=DEV).to(torch.bfloat16)
+        _check_tiles(x, q, s, z, None, _forced(form, x, q, s, z, None))
+
+
+def test_linear_form_that_does_not_fit():
+    q, s, z = _codes((64, 256), 64, False)
+    x = torch.randn(20, 256, device=DEV).to(torch.bfloat16)
+    with pytest.raises(RuntimeError, match="not supported"):
+        _forced((2, 3), x, q, s, z, None)  # two records of inputs cannot be cut in three
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 34816, 1024), (64, 34500, 640), (130, 10240, 5120), (192, 5120, 17408), (64, 5120, 17408),
+                                   (200, 34816, 1024), (256, 10240, 1024), (16384, 640, 512), (16385, 1001, 96)])
+def test_linear_of_real_sizes(M, N, K):
+    """Projections as models have them, at decode batches and prompts up to a whole chunk."""
+    q, s, z = _codes((N, K), 32 if K % 128 else 128, M % 2 == 0, torch.float16 if M in (64, 192) else torch.bfloat16)
+    x = torch.randn(M, K, device=DEV).to(torch.bfloat16)
+    _check_tiles(x, q, s, z, None, ops.linear_w4(x, ops.W4Weight.pack(q, s, z)))
+
+
+# ------------------------------------------------------------------------------------ the experts, element by element
+@pytest.mark.parametrize("T,E,k,H,inter,g1,g2", [(4, 8, 2, 256, 128, 64, 32), (16, 128, 8, 512, 192, 128, 64), (33, 4, 4, 96, 32, 32, 32),
+                                                (80, 3, 1, 2880, 160, 64, 32), (300, 32, 6, 384, 256, 32, 128),
+                                                (777, 5, 2, 160, 416, 32, 32), (100, 1, 1, 128, 64, 128, 64)])
+@pytest.mark.parametrize("zeros,dtype", [(False, torch.bfloat16), (True, torch.float16)])
+def test_experts_element_by_element(T, E, k, H, inter, g1, g2, zeros, dtype):
+    c1, c2 = _codes((E, 2 * inter, H), g1, zeros, dtype), _codes((E, H, inter), g2, zeros, dtype)
+    c1[1].mul_(0.3)
+    x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
+    weights, ids = ops.route_experts(torch.randn(T, E, device=DEV), k)
+    want, bound = _experts_rounded(x, c1, c2, weights, ids, exact_weights=T * k <= 8 * E)
+    _near(ops.experts_w4(x, *_packed(c1, c2), weights, ids), want, bound)
+
+
+@pytest.mark.parametrize("E,k,offset,all_experts", [(32, 8, 0, None), (16, 8, 48, 128)])
+def test_experts_of_a_whole_chunk(E, k, offset, all_experts):
+    """16384 tokens, uneven shares: an expert without any, one that a quarter of the pairs goes to."""
+    T, H, inter = 16384, 256, 128
+    c1, c2 = _codes((E, 2 * inter, H), 64, False), _codes((E, H, inter), 128, True)
+    x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
+    p = torch.randn(T, all_experts or E, device=DEV)
+    p[:, offset + 3] = -100.0
+    p[:, offset + 5] += 2.0
+    weights, ids = ops.route_experts(p, k)
+    got = ops.experts_w4(x, *_packed(c1, c2), weights, ids, expert_offset=offset, num_experts=all_experts)
+    _near(got, *_experts_rounded(x, c1, c2, weights, ids, offset))
