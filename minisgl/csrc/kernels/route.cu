@@ -14,8 +14,14 @@
 // One warp per token. The choice is made in fp32, with a bound on its errors: where two values that the
 // choice depends on are nearer than that (a few rows in a thousand), the candidates or the groups are looked at
 // again in 64 bits; without a bias the logits themselves decide and nothing is near. 16384 tokens x 256
-// experts, 8 of them, fp32 logits: 13 us softmax, 26 us with sigmoid scores, bias and groups, 700 to 1000
-// instructions a token, against 2.8 us for the bytes; every row in 64 bits took 65 us.
+// experts, 8 of them, fp32 logits: 13 us softmax (490 warp instructions a token), 26 us with sigmoid scores, bias and
+// groups (900), against 2.8 us for the bytes; every row in 64 bits took 65 us. What bounds both is waiting: with the 24
+// and 16 warps an SM that the registers leave, 65% and 55% of the issue slots are used, and the rest goes to chains of
+// dependent instructions, to shuffles and shared memory, and to the chosen logits' second read.
+//
+// The weights: an expf, over the sum of the row's fast exponentials (softmax without renormalising) or of the chosen
+// scores. The exponent's rounding counts |logit - largest| times 2^-24: down to scores of e^-32 of the largest a weight is
+// off by 2^-18 of its value at most, as a rule by 2^-23.
 //
 // Top k: the (k + 1)-th largest of the lanes' maxima (a sort of 32 keys across the warp) bounds the
 // (k + 1)-th largest value from below; the few values at or above it are gathered, a lane each, and ranked by
@@ -31,7 +37,8 @@ namespace {
 
 constexpr int kRouteWarps = 4;
 constexpr int kRouteMaxE = 512;
-// CTAs per SM: more would spill registers
+// CTAs per SM. At 6 (80 registers) the forms without groups spill 8 to 32 bytes for 128 and 256 experts, 140 between and
+// some 200 above them; with groups, at 4 (128 registers), only those above 256 experts do (about 110 bytes).
 __host__ __device__ constexpr int route_ctas(bool groups) { return groups ? 4 : 6; }
 
 struct RouteArgs {

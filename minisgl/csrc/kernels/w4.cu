@@ -99,7 +99,9 @@ struct Plan {
 
 // The split of the inputs with the least estimated time: the largest CTA's weight bytes at an SM's
 // share of the memory rate (43 B/ns), its activations at the L2's (four times that), and 1.5 us for the
-// exchange. Returns splits = 0 if the rows do not fit.
+// exchange. It ranks splits and is no forecast: the products' issue slots are not in it (16 x 5120 x 17408, groups of
+// 64 with zero points: 9.9 us estimated, 23 measured; there only a split in 8 has room for the rows). Returns splits = 0
+// if the rows do not fit.
 template <auto Kernel, int NT, int G, bool Z>
 Plan plan(const W4Tensor& w, int M) {
   Plan best = {0, 0, 0, 0};
@@ -168,7 +170,7 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
   p.m_tiles = (a.M + p.bn - 1) / p.bn;
   // Halves of a tile and cuts of the inputs with the least estimated time, in clocks per 128 inputs of a tile:
-  // conversion 450 a half (measured), the tensor core 4 a token and half, the tokens' rows from L2 5 a token;
+  // conversion 450 a half (measured with bf16 scales; fp16 ones take about a quarter longer), the tensor core 4 a token and half, the tokens' rows from L2 5 a token;
   // the exchange 2000 and 20 a token and half.
   double best = 1e30;
   int halves = 1;

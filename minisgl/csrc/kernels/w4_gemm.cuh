@@ -11,9 +11,11 @@
 //   warps 10-25  records -> bf16 A tiles in tensor memory: the codes become bf16 as in w4.cuh, times the group's
 //                scale. Half of them take the even steps, half the odd ones: one half converts while the other
 //                waits for its barriers and its stores.
-// What bounds it is the conversion's issue slots (about 1000 warp instructions of a step's 2000) and, next to it, the
-// latency of one step through conversion, MMA and release: 640 clocks a step with few tokens, 17 x 34816 x 5120 33 us;
-// 200 x 34816 x 5120 57 us, 1.26 PFLOP/s, 75% of a measured bf16 product's rate; 1024 tokens 276 us, 79%.
+// What bounds it is the conversion's issue slots (about 1000 warp instructions of a step's 1900; 64% of the slots are used
+// at 32 tokens, the tensor pipe 17% of the time) and, next to it, the latency of one step through conversion, MMA and
+// release: 640 clocks a step with few tokens, 17 x 34816 x 5120 33 us; 200 x 34816 x 5120 57 us, 1.26 PFLOP/s, 75% of a
+// measured bf16 product's rate; 1024 tokens 271 to 276 us, 79%. fp16 scales are multiplied in fp32 and cost more: 64
+// tokens 46 us (bf16 37), 200 tokens 65 (56), 1024 tokens 363 (271); zero points 1 to 8% with either.
 // A comes from tensor memory because shared memory's 128 bytes a clock were the limit with A tiles there
 // (200 tokens: 143 KB a step, of which A written and read 64): 72 us at 200 x 34816 x 5120.
 // Rounding (code - zero) * scale to bf16 is a choice: an fp32 scale applied to the sums would need the

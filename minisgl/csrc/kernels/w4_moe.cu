@@ -11,7 +11,8 @@
 // run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
 //
 // 128 experts of 2048 x 768, 8 a token, groups of 128, whole layer: 1 token 17.9 us (3.0 for the bytes; three launches
-// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 159 (48), 2048 tokens 332 (92).
+// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 160 (48), 2048 tokens 335 (92),
+// 16384 tokens 2128 (737), of which the one block that sorts the 131072 pairs takes 96 (15 at 2048 tokens, 7 at 512).
 #include <algorithm>
 
 #include "w4_gemm.cuh"

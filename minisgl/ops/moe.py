@@ -70,7 +70,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     many groups of consecutive ids, and only those of the ``top_groups`` best are chosen from: a
     group counts by its best expert (``group_score="max"``) or by the sum of the two best scores
     (plus bias) in it (``"top2"``). The weights are the chosen scores, divided by their sum with
-    ``renormalize``, times ``scale``.
+    ``renormalize``, times ``scale``, in fp32 (on the GPU off by at most 2^-18 of
+    the value, for scores down to e^-32 of the largest).
 
     A NaN logit counts as -inf and +inf as the largest fp32 value; a row without a finite logit has
     softmax scores of zero, and weights whose sum is zero stay zero. NaN biases count as the lowest fp32

@@ -3,8 +3,9 @@
 ``W4Weight`` holds one weight matrix ``[N, K]``, or the matrices ``[E, N, K]`` of a layer's experts,
 whose values are ``(code - zero) * scale``: a code 0..15 per value, and per row and group of 32, 64 or
 128 inputs one bf16 or fp16 scale and optionally a zero point 0..15 (without them every zero point is
-8). ``W4Weight.pack`` takes them as checkpoints hold them and lays them out once in the order in which
-the kernels read them (``csrc/kernels/w4.cuh``); ``quantize_w4`` makes them from bf16 weights.
+8). ``W4Weight.pack`` takes two codes a byte along the inputs, as many checkpoints hold them (other orders
+are the caller's to turn into this one), and lays them out once in the order in which the kernels read
+them (``csrc/kernels/w4.cuh``); ``quantize_w4`` makes them from bf16 weights.
 
     w = ops.W4Weight.pack(q, scales, zeros)               # q [N, K/2] uint8, scales / zeros [N, K/group]
     y = ops.linear_w4(x, w, bias)                         # [M, K] bf16 -> [M, N] bf16
@@ -16,6 +17,12 @@ the kernels read them (``csrc/kernels/w4.cuh``); ``quantize_w4`` makes them from
 
 CUDA tensors run the sm_100a kernels, CPU tensors the plain form in ``ops.reference``. Calls may be
 captured in CUDA graphs; they keep no state of their own, so calls on several streams are independent.
+
+What is rounded on the GPU: for few tokens (up to 16, experts: up to 8 pairs of a token and an expert per
+expert) nothing of a weight, its scale multiplies the fp32 sum of its group; for more tokens, and for
+rows too wide for that form's shared memory, every weight once to bf16, as in a bf16 copy of the weights.
+A token's result so moves a little, within what one rounding of the weights does, when a batch passes
+from the one to the other. Equal calls give equal results.
 """
 
 from __future__ import annotations
@@ -203,7 +210,8 @@ def _bias(name: str, b: torch.Tensor | None, shape):
 
 def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ w^T (+ bias)`` for bf16 ``x [M, K]`` and a 4-bit ``w [N, K]``; bf16 ``[M, N]``. Sums are
-    held in fp32. Rows of ``x`` may be strided."""
+    held in fp32; above 16 tokens every weight ``(code - zero) * scale`` is rounded to bf16 first. ``x`` may
+    be strided (rows that overlap or are off the 16-byte grid are copied), ``bias`` is bf16 ``[N]``."""
     if w.experts or w.gated:
         raise ValueError("linear_w4 takes one ungated matrix")
     if not x.is_cuda:
@@ -225,7 +233,9 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
     here), by which the GPU estimates how many tokens an expert gets and chooses its form. ``activation``:
     ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU a call takes up to 1024 experts and 2^24
     pairs of a token and an expert.
-    The activated values between the two products are held in bf16, sums in fp32."""
+    The activated values between the two products are held in bf16, sums in fp32; above 8 pairs per expert
+    every weight is rounded to bf16 first. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
+    ``w1_bias [E, 2I]`` and ``w2_bias [E, H]`` are contiguous."""
     if not (w1.experts and w1.gated and w2.experts and not w2.gated):
         raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")
     if activation not in _ACT:
