@@ -9,7 +9,7 @@
 //   warp 8       bulk copies of the tile's records of 128 inputs (two steps) into a ring of their own
 //   warp 9       MMA issuer: D_h[128 x N] += A_h[128 x 64] B[N x 64]^T, fp32 in TMEM, two sets if they fit
 //   warps 10-25  records -> bf16 A tiles in tensor memory: the codes become bf16 as in w4.cuh, times the group's
-//                scale. Half of them take the even steps, half the odd ones: one half converts while the other
+//                scale (experts: its two parts). Half of them take the even steps, half the odd ones: one half converts while the other
 //                waits for its barriers and its stores.
 // What bounds it is the conversion's issue slots (about 1000 warp instructions of a step's 1900; 64% of the slots are used
 // at 32 tokens, the tensor pipe 17% of the time) and, next to it, the latency of one step through conversion, MMA and
@@ -18,9 +18,15 @@
 // tokens 46 us (bf16 37), 200 tokens 65 (56), 1024 tokens 363 (271); zero points 1 to 8% with either.
 // A comes from tensor memory because shared memory's 128 bytes a clock were the limit with A tiles there
 // (200 tokens: 143 KB a step, of which A written and read 64): 72 us at 200 x 34816 x 5120.
-// Rounding (code - zero) * scale to bf16 is a choice: an fp32 scale applied to the sums would need the
-// accumulator to be read back once per group. It adds half a step of bf16 per weight, independent from
-// weight to weight, about what the result's own rounding does.
+// Rounding (code - zero) * scale to bf16 is a choice of the dense product: an fp32 scale applied to the sums would need
+// the accumulator to be read back once per group. It adds half a step of bf16 per weight, independent from weight to
+// weight, about what the result's own rounding does: 0.0022 off in the 2-norm where exact weights give 0.0017.
+// The experts' two products in a row would be 0.0033 to 0.0037 off. Their weights are exact: a scale is the sum of its
+// first four bits and the rest, a code times the first is exact in bf16, times the rest too (fp16 scales leave 7 bits: off
+// by half a step of bf16 of an eighth of the weight at most, 2^-12 of it), and both are tiles of A, multiplied one after
+// the other into the same sums: 0.0023, which is what the roundings of the activated values and of the result leave. The
+// price, 128 experts of 2048 x 768, 8 a token, beside rounded weights: 512 tokens 181 us and 160, 2048 tokens 408 and
+// 334; with fp16 scales 512 tokens 190 and 192.
 //
 // 256 rows per tile (H = 2) because the tokens' rows come from L2 once per tile: with 128 rows 200 tokens x
 // 34816 x 5120 read 560 MB of them, 145 us. H = 1 where 256-row tiles would leave SMs idle.
@@ -60,7 +66,10 @@ constexpr int kGwThreads = (kGwEpi + kGwLoad + 2 + kGwConv) * 32;
 constexpr int kGwMaxSlots = 8, kGwMaxA = 8;  // most stages of the rings
 constexpr int kGwMaxB = 8;
 constexpr int w4_row_stages(int mode) { return mode == kW4GateUp ? kGwMaxB : 4; }  // of the tokens' rows
-constexpr int kGwMaxGather = 96;  // gathered tokens of a tile
+// A tiles that a weight is given as. One: (code - zero) * scale rounded to bf16. Two: the products with the scale's
+// first four bits, which are exact in bf16, and with the rest of it, which are exact for bf16 scales.
+constexpr int w4_parts(int mode) { return mode == kW4Dense ? 1 : 2; }
+constexpr int kGwMaxGather = 128;  // gathered tokens of a tile
 constexpr int kGwMisc = kGwLoad * kGwMaxGather * 4 + 512;  // row numbers, barriers
 constexpr int kGwRoom = 227 * 1024 - 1024 - kGwMisc;  // of the rings
 constexpr int kGwMaxTokens = 208;    // of a tile: three half-step stages of A then fit beside the accumulators
@@ -71,6 +80,22 @@ MSGL_DEVICE uint32_t w4_times(uint32_t v, uint32_t scale2, float scale) {
   if constexpr (F) return pack_bf16(bf16_lo(v) * scale, bf16_hi(v) * scale);
   const __nv_bfloat162 p = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&scale2));
   return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// two scales as bf16 pairs that sum to them: their first four bits (the leading one among them), and the rest
+template <bool F>
+MSGL_DEVICE void w4_scale_parts(uint32_t scales, uint32_t (&part)[2]) {
+  if constexpr (F) {
+    uint32_t top = scales & 0xff80ff80u;
+    const __half2 rest = __hsub2(*reinterpret_cast<__half2*>(&scales), *reinterpret_cast<__half2*>(&top));
+    const float2 t = w4_scales<true>(top), r = __half22float2(rest);
+    part[0] = pack_bf16(t.x, t.y);
+    part[1] = pack_bf16(r.x, r.y);
+  } else {
+    part[0] = scales & 0xfff0fff0u;
+    const __nv_bfloat162 rest = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&scales), *reinterpret_cast<__nv_bfloat162*>(&part[0]));
+    part[1] = *reinterpret_cast<const uint32_t*>(&rest);
+  }
 }
 
 // 16 lanes x 16 columns of tensor memory from the warp's registers: r[4i], r[4i + 1] are columns 8i + 2t,
@@ -97,10 +122,10 @@ __global__ void __launch_bounds__(kGwThreads, 1)
 w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUtensorMap rows_map) {
   static_assert(MODE != kW4GateUp || H == 2, "gate rows in one half, up rows in the other");
   constexpr int kRecs = 4 * H, kGwB = w4_row_stages(MODE);
-  // Columns of a half in a stage of A. FINE: a stage is half a step, so that three fit beside the accumulators of
+  // Columns of a half in a stage of A, by parts. FINE: a stage is half a step, so that three fit beside the accumulators of
   // more than 192 tokens; the MMA warp then waits and commits twice a step, which small tiles would feel. (One issue
   // of a step's eight MMAs against two of four: 17 tokens 34.4 and 35.8 us, 256 tokens 87.8 and 84.7.)
-  constexpr int kCols = FINE ? 16 : 32;
+  constexpr int kPart = FINE ? 16 : 32, kCols = kPart * w4_parts(MODE);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int S = p.stages, stage_bytes = p.bn * 128;
@@ -352,7 +377,10 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             for (int j = 0; j < (FINE ? 2 : 4); ++j)
 #pragma unroll
               for (int h = 0; h < H; ++h)
-                tc_mma_f16_ts(d + h * half_cols, a + h * kCols + j * 8, b + e * 4 + j * 2, idesc, acc || e > 0 || j > 0);
+#pragma unroll
+                for (int q = 0; q < w4_parts(MODE); ++q)
+                  tc_mma_f16_ts(d + h * half_cols, a + h * kCols + q * kPart + j * 8, b + e * 4 + j * 2, idesc,
+                                acc || e > 0 || j > 0 || q > 0);
             tc_commit(&a_empty[stage]);
             if (!FINE || e == 1) tc_commit(&b_empty[bstage]);
           }
@@ -411,6 +439,7 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
           // a store's registers: two words by rows g (two pairs of inputs) and rows g + 8 of a half; gated: by the gate
           // rows (first store) or the up rows (second) of both halves
           uint32_t r[H][8];
+          uint32_t parts[H][2][2];  // by half, part and row: a scale in both halves of a register
 #pragma unroll
           for (int i = 0; i < H; ++i) {
             const int half = H == 2 ? i : m;
@@ -419,16 +448,31 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
             const uint32_t z1 = kW4Whole + (Z ? ((zv >> 8) & 15u) * 0x10001u : 0x00080008u);
             const uint32_t sa2 = __byte_perm(sv, 0, 0x1010), sb2 = __byte_perm(sv, 0, 0x3232);
             float2 sf = make_float2(0.f, 0.f);
-            if constexpr (F) sf = w4_scales<true>(sv);
+            if constexpr (w4_parts(MODE) == 2) {
+              uint32_t part[2];
+              w4_scale_parts<F>(sv, part);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                parts[i][k][0] = __byte_perm(part[k], 0, 0x1010);
+                parts[i][k][1] = __byte_perm(part[k], 0, 0x3232);
+              }
+            } else if constexpr (F) {
+              sf = w4_scales<true>(sv);
+            }
             const uint32_t words[2] = {e ? q[i].z : q[i].x, e ? q[i].w : q[i].y};
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               uint32_t* const lo = MODE == kW4GateUp ? &r[0][4 * b + 2 * i] : &r[i][4 * b];
               uint32_t* const hi = MODE == kW4GateUp ? &r[H - 1][4 * b + 2 * i] : &r[i][4 * b + 2];
-              lo[0] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b], z0), sa2, sf.x);
-              hi[0] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 4, z1), sb2, sf.y);
-              lo[1] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 8, z0), sa2, sf.x);
-              hi[1] = w4_times<F>(codes_bf16x2<kW4Whole>(words[b] >> 12, z1), sb2, sf.y);
+              // (two parts: the codes alone, times the parts of their scales below)
+              const auto value = [&](uint32_t word, uint32_t zero, uint32_t s2, float s) {
+                const uint32_t v = codes_bf16x2<kW4Whole>(word, zero);
+                return w4_parts(MODE) == 2 ? v : w4_times<F>(v, s2, s);
+              };
+              lo[0] = value(words[b], z0, sa2, sf.x);
+              hi[0] = value(words[b] >> 4, z1, sb2, sf.y);
+              lo[1] = value(words[b] >> 8, z0, sa2, sf.x);
+              hi[1] = value(words[b] >> 12, z1, sb2, sf.y);
             }
           }
           if (FINE || e == 0) {
@@ -439,8 +483,20 @@ w4_gemm_kernel(const __grid_constant__ W4GemmArgs p, const __grid_constant__ CUt
           const uint32_t dst = tmem_a + lanes + stage * H * kCols + (FINE ? 0 : e * 16);
 #pragma unroll
           for (int i = 0; i < H; ++i) {
-            if constexpr (MODE == kW4GateUp) tmem_st_16x256b_x2(dst + i * kCols, r[i]);
-            else tmem_st_16x256b_x2(dst + (H == 2 ? m * kCols : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16), r[i]);
+            const uint32_t to = MODE == kW4GateUp ? dst + i * kCols
+                                                  : dst + (H == 2 ? m * kCols : 0) + ((uint32_t)((H == 2 ? i : m) * 16) << 16);
+            if constexpr (w4_parts(MODE) == 1) {
+              tmem_st_16x256b_x2(to, r[i]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                uint32_t o[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  o[c] = w4_times<false>(r[i][c], MODE == kW4GateUp ? parts[c / 2 % 2][k][i] : parts[i][k][c / 2 % 2], 0.f);
+                tmem_st_16x256b_x2(to + k * kPart, o);
+              }
+            }
           }
           if (FINE || e == 1) {
             tc_wait_st();
@@ -523,9 +579,9 @@ int w4_gemm_launch_as(W4GemmArgs p, int grid, cudaStream_t s) {
   // Tensor memory's 512 columns: two sets of accumulators if two steps of A fit beside them, else one and up to
   // eight stages. Shared memory: four stages of the tokens' rows, and up to eight steps' records (a copy
   // takes about 1 us).
-  constexpr int kA = H * (FINE ? 16 : 32);
+  constexpr int kA = H * (FINE ? 16 : 32) * w4_parts(MODE);
   p.half_cols = p.bn;
-  p.sets = 512 - 2 * H * p.half_cols >= 2 * H * 32 ? 2 : 1;
+  p.sets = 512 - 2 * H * p.half_cols >= (FINE ? 3 : 2) * kA ? 2 : 1;
   p.stages = std::min(kGwMaxA, (512 - p.sets * H * p.half_cols) / kA);
   // A team of converters waits for a stage's turn by the parity of its phase, and takes every other step: its last wait
   // must have shown that all but the latest of the stage's turns are over. That is so with two stages of a step, or

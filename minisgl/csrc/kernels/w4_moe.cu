@@ -4,15 +4,16 @@
 // Few tokens: the chosen experts' tiles, one after another, are cut into equal runs, one per SM. Every CTA
 // counts the pairs per expert itself (they are few) instead of waiting for a kernel that would, so a
 // layer is three launches; the counting of the second product overlaps the end of the first. The
-// activated values between the products are bf16, as the second product's operands are; y is fp32 and
-// the sum over a token's experts runs in the order of its choices, so results do not vary.
+// activated values between the products are bf16, as the second product's operands are; weights are exact in both
+// forms; y is fp32 and the sum over a token's experts runs in the order of its choices, so results do not vary.
 //
-// Many tokens: a kernel sorts the pairs by expert and lists tiles of up to 96 of an expert's pairs; the products
+// Many tokens: a kernel sorts the pairs by expert and lists tiles of up to 64 or 128 of an expert's pairs; the products
 // run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
 //
 // 128 experts of 2048 x 768, 8 a token, groups of 128, whole layer: 1 token 17.9 us (3.0 for the bytes; three launches
-// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45); on the tensor core 512 tokens 160 (48), 2048 tokens 335 (92),
-// 16384 tokens 2128 (737), of which the one block that sorts the 131072 pairs takes 96 (15 at 2048 tokens, 7 at 512).
+// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45), 256 tokens 138 (47); on the tensor core 512 tokens 181 (48),
+// 2048 tokens 408 (92), 16384 tokens 2670 (737), of which the one block that sorts the 131072 pairs takes 96 (15 at 2048
+// tokens, 7 at 512).
 #include <algorithm>
 
 #include "w4_gemm.cuh"
@@ -254,14 +255,19 @@ int experts_product(const ExpertArgs& p, const MsglW4* w, int total, bool launch
   });
 }
 
-constexpr int kTileTokens = kGwMaxGather;  // 96 of a tile: two sets of accumulators then fit into tensor memory
+// Pairs of a tile. Up to 64 two sets of accumulators fit into tensor memory beside two stages of A, so that a tile's
+// results leave while the next one is multiplied; 128 fit once, and convert the weights half as often. 128 experts of
+// 2048 x 768, 8 a token, 64 and 128 a tile: 512 tokens (32 pairs an expert) 181 and 196 us, 1024 tokens 271 and 254, 2048
+// tokens 435 and 401, 16384 tokens 3135 and 2656. (80 and 96 lie between.)
+constexpr int kTileFew = 64, kTileMany = kGwMaxGather;
+inline int tile_tokens(int64_t pairs, int64_t total) { return pairs <= 40 * total ? kTileFew : kTileMany; }
 
 // Sorts the pairs by expert (in any order within one: a pair's result does not depend on its place) and cuts
 // every expert's into equal tiles. One CTA.
 __global__ void __launch_bounds__(1024) w4_plan_kernel(const int32_t* __restrict__ ids, int pairs, int E, int e0,
                                                        int32_t* __restrict__ sorted, int32_t* __restrict__ place,
                                                        int4* __restrict__ work,
-                                                       int32_t* __restrict__ count) {
+                                                       int32_t* __restrict__ count, int tile) {
   __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(1024) w4_plan_kernel(const int32_t* __restrict
   }
   __syncthreads();
   // running sums of the pairs and tiles over the experts, one a thread
-  const int c = cnt[tid], tiles = (c + kTileTokens - 1) / kTileTokens;
+  const int c = cnt[tid], tiles = (c + tile - 1) / tile;
   int a = c, b = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -323,31 +329,32 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
   s.sorted = s.y + up(pairs * w2->n * 4);
   s.place = s.sorted + up(pairs * 4);
   s.work = s.place + up(pairs * 4);
-  s.count = s.work + up((E + pairs / kTileTokens) * 16);
+  s.count = s.work + up((E + pairs / kTileFew) * 16);
   s.bytes = s.count + 256;
   return s;
 }
 
-// Pairs per expert up to which the streaming product is taken (128 experts of 2048 x 768: at 8 a layer takes 100 us
-// streaming and 114 on the tensor core, at 16 it takes 138 and 133). Where only a share of the experts is here, pairs
-// and experts of all ranks count: 8 of 64 experts of 2880 x 2880 at 32 tokens, 8 a token, 35 us streaming and 64 on the
-// tensor core; 32 of 256 of 4096 x 1024 at 128 tokens 62 and 88.
-constexpr int kStreamPairs = 8;
+// Pairs per expert up to which the streaming product is taken. 128 experts of 2048 x 768, streaming and on the tensor
+// core: at 16 a layer takes 138 and 156 us, at 20 156 and 165, at 24 176 and 171; 32 experts of 2880 x 2880, groups of 32
+// with zero points: at 16 193 and 205, at 25 254 and 228. Where only a share of the experts is here, pairs and experts of
+// all ranks count: 8 of 64 experts of 2880 x 2880 at 32 tokens, 8 a token, 35 us streaming and 64 on the tensor core.
+constexpr int kStreamPairs = 20;
 
 int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
-                  const int32_t* ids, const void* b1, const void* b2, int act, uint8_t* ws, const Scratch& sc,
+                  int total, const int32_t* ids, const void* b1, const void* b2, int act, uint8_t* ws, const Scratch& sc,
                   cudaStream_t s) {
   int32_t *sorted = (int32_t*)(ws + sc.sorted), *count = (int32_t*)(ws + sc.count);
   int4* work = (int4*)(ws + sc.work);
+  const int tile = tile_tokens(pairs, total);
   if (w4_launch(w4_plan_kernel, dim3(1), dim3(1024), 0, s, 1, ids, pairs, E, e0, sorted, (int32_t*)(ws + sc.place), work,
-                  count) != cudaSuccess)
+                  count, tile) != cudaSuccess)
     return 4;
   W4GemmArgs p = {};
-  p.bn = std::min(kTileTokens, (pairs + 15) / 16 * 16);
+  p.bn = std::min(tile, (pairs + 15) / 16 * 16);
   p.splits = 1;
   p.count = count, p.work = work, p.sorted = sorted;
   p.topk = topk, p.act = act;
-  const int64_t tiles = std::min<int64_t>(E + pairs / kTileTokens, pairs);
+  const int64_t tiles = std::min<int64_t>(E + pairs / tile, pairs);
   W4GemmArgs q = p;
   p.w = w4_tensor(w1);
   p.group = w1->group, p.zeros = w1->zeros, p.fp16 = w1->fp16;
@@ -398,7 +405,7 @@ extern "C" int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T
     rc = experts_product<true>(p1, w1, total, true, s);
     if (rc == 0) rc = experts_product<false>(p2, w2, total, true, s);
   } else {
-    rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, ids, b1, b2, act, ws, sc, s);
+    rc = experts_tiles(x, x_stride, pairs, topk, w1, w2, E, e0, total, ids, b1, b2, act, ws, sc, s);
   }
   if (rc == 0 &&
       w4_launch(w4_combine_kernel, dim3(T, (w2->n + 511) / 512), dim3(128), 0, s, 1, (const float*)(ws + sc.y),

@@ -18,11 +18,12 @@ them (``csrc/kernels/w4.cuh``); ``quantize_w4`` makes them from bf16 weights.
 CUDA tensors run the sm_100a kernels, CPU tensors the plain form in ``ops.reference``. Calls may be
 captured in CUDA graphs; they keep no state of their own, so calls on several streams are independent.
 
-What is rounded on the GPU: for few tokens (up to 16, experts: up to 8 pairs of a token and an expert per
-expert) nothing of a weight, its scale multiplies the fp32 sum of its group; for more tokens, and for
-rows too wide for that form's shared memory, every weight once to bf16, as in a bf16 copy of the weights.
-A token's result so moves a little, within what one rounding of the weights does, when a batch passes
-from the one to the other. Equal calls give equal results.
+What is rounded on the GPU: the linear product holds weights exactly for up to 16 tokens (their scale
+multiplies the fp32 sum of its group); for more tokens, and for rows too wide for that form's shared
+memory, every weight is rounded once to bf16, as in a bf16 copy of the weights. A token's result so moves
+a little, within what one rounding of the weights does, when a batch passes from the one to the other.
+The experts' products hold weights exactly for any number of tokens (for many tokens and fp16 scales: to
+2^-12). Equal calls give equal results.
 """
 
 from __future__ import annotations
@@ -74,7 +75,7 @@ class W4Weight:
     def pack(cls, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
              gated: bool = False) -> "W4Weight":
         """``q`` uint8 ``[(E,) N, K/2]``, two codes a byte along the inputs, the low nibble first;
-        ``scales`` bf16 / fp16 and ``zeros`` uint8 (0..15) ``[(E,) N, K/group]``. ``gated``: the rows
+        ``scales`` bf16 / fp16, finite, and ``zeros`` uint8 (0..15) ``[(E,) N, K/group]``. ``gated``: the rows
         are ``[gate; up]`` halves, as in the first matrix of a gated MLP."""
         if q.dtype != torch.uint8 or q.dim() not in (2, 3):
             raise ValueError(f"4-bit codes must be uint8 [N, K/2] or [E, N, K/2], got {q.dtype} {tuple(q.shape)}")
@@ -96,6 +97,8 @@ class W4Weight:
             raise ValueError("4-bit zero points must be 0..15")
         if any(t is not None and t.device != q.device for t in (scales, zeros)):
             raise ValueError("4-bit codes, scales and zero points must be on one device")
+        if not bool(scales.isfinite().all()):
+            raise ValueError("4-bit scales must be finite")
         if not experts:
             q, scales, zeros = q[None], scales[None], None if zeros is None else zeros[None]
         E = q.shape[0]
@@ -233,8 +236,8 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
     here), by which the GPU estimates how many tokens an expert gets and chooses its form. ``activation``:
     ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU a call takes up to 1024 experts and 2^24
     pairs of a token and an expert.
-    The activated values between the two products are held in bf16, sums in fp32; above 8 pairs per expert
-    every weight is rounded to bf16 first. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
+    The activated values between the two products are held in bf16, weights exactly (to 2^-12 of them with
+    fp16 scales and many tokens), sums in fp32. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
     ``w1_bias [E, 2I]`` and ``w2_bias [E, H]`` are contiguous."""
     if not (w1.experts and w1.gated and w2.experts and not w2.gated):
         raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")

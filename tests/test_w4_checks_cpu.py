@@ -113,3 +113,13 @@ def test_launch_counts_come_from_the_call():
     assert mod.linear_w4(0) == "y" and COUNTERS.launches == before + 2
     assert mod.experts_w4(2) == "z" and COUNTERS.launches == before + 6
     assert mod.route_experts() == "r" and COUNTERS.launches == before + 7
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pack_refuses_scales_that_are_not_finite(dtype):
+    q = torch.zeros(3, 64, dtype=torch.uint8)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        s = torch.ones(3, 4, dtype=dtype)
+        s[1, 2] = bad
+        with pytest.raises(ValueError, match="finite"):
+            ops.W4Weight.pack(q, s)

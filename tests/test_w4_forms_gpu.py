@@ -1,8 +1,9 @@
-"""Every form of the 4-bit products for many tokens, against 64-bit sums of the same rounded weights.
+"""Every form of the 4-bit products for many tokens, against 64-bit sums with their roundings made.
 
-Above 16 tokens (experts: 8 pairs an expert) a weight is (code - zero) * scale rounded to bf16. That
-rounding is part of the form, so the oracle makes it too, and what is left is narrow: the sums' chains of at most
-K / 16 + 64 additions in fp32, 2^-23 of the sum of magnitudes each, and one rounding of the result, 2^-8.
+Above 16 tokens a weight of the linear product is (code - zero) * scale rounded to bf16; the experts' weights are exact,
+their activated values rounded. These roundings are part of the forms, so the oracle makes them too, and what is left
+is narrow: the sums' chains of at most K / 16 + 64 additions in fp32, 2^-23 of the sum of magnitudes each
+(K / 8 where two parts of a weight are added one after the other), and one rounding of the result, 2^-8.
 """
 
 import pytest
@@ -12,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 from minisgl import ops  # noqa: E402
 from test_w4_checks_cpu import bad_calls  # noqa: E402
-from test_w4_gpu import A, DEV, R, _codes, _cuda_only, _near, _packed, _wide  # noqa: E402,F401
+from test_w4_gpu import A, DEV, R, _codes, _cuda_only, _experts_wide, _near, _packed, _wide  # noqa: E402,F401
 
 
 def _check_tiles(x, q, s, z, bias, got):
@@ -32,11 +33,13 @@ def test_linear_of_very_wide_rows(M):
     _check_tiles(x, q, s, z, None, ops.linear_w4(x, ops.W4Weight.pack(q, s, z)))
 
 
-def _experts_rounded(x, c1, c2, weights, ids, offset=0, exact_weights=False):
-    """(result, bound) of silu experts as the form for many tokens computes them: weights and activated values
-    rounded to bf16 (``exact_weights``: the form for few tokens, activated values only). The fp32 sums move an activated value a little; where that reaches the middle between
-    two bf16 values it may become the other one, and the step goes through the second product."""
+def _experts_bounded(x, c1, c2, weights, ids, offset=0):
+    """(result, bound) of silu experts with exact weights and activated values rounded to bf16. The fp32 sums move
+    an activated value a little; where that reaches the middle between two bf16 values it may become the other
+    one, and the step goes through the second product. An fp16 scale of 11 bits is its first four, whose product with a
+    code is exact, and seven more, an eighth of it at most, whose product is rounded to bf16: off by 2^-9 2^-3."""
     E, H, inter = c1[0].shape[0], c2[0].shape[1], c1[0].shape[1] // 2
+    w1_off, w2_off = (2.0 ** -12 if c[1].dtype == torch.float16 else 0.0 for c in (c1, c2))
     out = torch.zeros(x.shape[0], H, dtype=torch.float64, device=DEV)
     bound = torch.zeros_like(out)
     for e in range(E):
@@ -44,10 +47,8 @@ def _experts_rounded(x, c1, c2, weights, ids, offset=0, exact_weights=False):
         if len(tok) == 0:
             continue
         m1, m2 = (_wide(*(None if t is None else t[e] for t in c)) for c in (c1, c2))
-        if not exact_weights:
-            m1, m2 = m1.to(torch.bfloat16).double(), m2.to(torch.bfloat16).double()
         xd = x[tok].double()
-        h, dh = xd @ m1.t(), (x.shape[1] / 16 + 64) * A * (xd.abs() @ m1.abs().t())
+        h, dh = xd @ m1.t(), ((x.shape[1] / 8 + 64) * A + w1_off) * (xd.abs() @ m1.abs().t())
         g, u, dg, du = h[:, :inter], h[:, inter:], dh[:, :inter], dh[:, inter:]
         silu = g * torch.sigmoid(g)
         a = silu * u
@@ -61,7 +62,7 @@ def _experts_rounded(x, c1, c2, weights, ids, offset=0, exact_weights=False):
         w = weights[tok, slot, None].double()
         out.index_add_(0, tok, w * (rounded @ m2.t()))
         bound.index_add_(0, tok, w.abs() * (moved @ m2.abs().t()
-                                            + (inter / 16 + 64 + ids.shape[1]) * A * (rounded.abs() @ m2.abs().t())))
+                                            + ((inter / 8 + 64 + ids.shape[1]) * A + w2_off) * (rounded.abs() @ m2.abs().t())))
     return out, R * out.abs() + bound
 
 
@@ -72,15 +73,17 @@ def test_experts_of_very_wide_rows(T, E, H, inter):
     x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
     ids = torch.arange(T, device=DEV, dtype=torch.int32)[:, None] % E
     weights = torch.rand(T, 1, device=DEV)
-    want, bound = _experts_rounded(x, c1, c2, weights, ids)
+    want, bound = _experts_bounded(x, c1, c2, weights, ids)
     _near(ops.experts_w4(x, *_packed(c1, c2), weights, ids), want, bound)
 
 
-@pytest.mark.parametrize("T", [9, 17, 33, 64, 65])
+@pytest.mark.parametrize("T", [9, 17, 64, 160, 161])
 @pytest.mark.parametrize("spread", ["all ranks", "one expert", "elsewhere", "here"])
 def test_experts_of_a_share_choose_by_all(T, spread):
-    """4 experts of 64, 8 a token: up to 64 tokens an expert has 8 pairs if they spread over all ranks, and the form
-    for few tokens runs whatever they do. Its results have exact weights, so the bound tells the forms apart."""
+    """4 experts of 64, 8 a token: up to 160 tokens an expert has 20 pairs if they spread over all ranks, and the form
+    for few tokens runs whatever they do (three kernels; for many tokens there are four)."""
+    from minisgl.engine.counters import COUNTERS
+
     E, total, k, H, inter, offset = 4, 64, 8, 256, 128, 20
     c1, c2 = _codes((E, 2 * inter, H), 64, True), _codes((E, H, inter), 128, False)
     x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
@@ -88,15 +91,18 @@ def test_experts_of_a_share_choose_by_all(T, spread):
     ids = torch.randint(lo, hi, (T, k), device=DEV, dtype=torch.int32)
     weights = torch.rand(T, k, device=DEV)
     w1, w2 = _packed(c1, c2)
+    want, bound = _experts_bounded(x, c1, c2, weights, ids, offset)
+    before = COUNTERS.launches
     got = ops.experts_w4(x, w1, w2, weights, ids, expert_offset=offset, num_experts=total)
-    want, bound = _experts_rounded(x, c1, c2, weights, ids, offset, exact_weights=T <= 64)
+    assert COUNTERS.launches - before == (3 if T <= 160 else 4)
     _near(got, want, bound)
     if spread == "elsewhere":
         assert not got.any()
     for n in (E, total + 1000):  # whatever the estimate, the same experts' results
+        before = COUNTERS.launches
         other = ops.experts_w4(x, w1, w2, weights, ids, expert_offset=offset, num_experts=n)
-        few = T * k <= min(8 * n, 4096)
-        _near(other, *_experts_rounded(x, c1, c2, weights, ids, offset, exact_weights=few))
+        assert COUNTERS.launches - before == (3 if T * k <= min(20 * n, 4096) else 4)
+        _near(other, want, bound)
 
 
 def test_refused_as_on_the_cpu():
@@ -123,9 +129,9 @@ def test_kernels_are_counted():
     x = torch.randn(40, 33024, device=DEV).to(torch.bfloat16)
     assert [launched(lambda: ops.linear_w4(x[:m], w)) for m in (0, 1, 16, 40)] == [0, 1, 2, 1]
     w1, w2 = _packed(_codes((4, 64, 128), 64, False), _codes((4, 128, 32), 32, False))
-    x = torch.randn(40, 128, device=DEV).to(torch.bfloat16)
-    ids, wt = torch.zeros(40, 2, device=DEV, dtype=torch.int32), torch.rand(40, 2, device=DEV)
-    assert [launched(lambda: ops.experts_w4(x[:t], w1, w2, wt[:t], ids[:t])) for t in (0, 1, 16, 40)] == [0, 3, 3, 4]
+    x = torch.randn(41, 128, device=DEV).to(torch.bfloat16)
+    ids, wt = torch.zeros(41, 2, device=DEV, dtype=torch.int32), torch.rand(41, 2, device=DEV)
+    assert [launched(lambda: ops.experts_w4(x[:t], w1, w2, wt[:t], ids[:t])) for t in (0, 1, 40, 41)] == [0, 3, 3, 4]
 
 
 # -------------------------------------------------------------------------- every form of the many-token product
@@ -208,7 +214,7 @@ def test_experts_element_by_element(T, E, k, H, inter, g1, g2, zeros, dtype):
     c1[1].mul_(0.3)
     x = torch.randn(T, H, device=DEV).to(torch.bfloat16)
     weights, ids = ops.route_experts(torch.randn(T, E, device=DEV), k)
-    want, bound = _experts_rounded(x, c1, c2, weights, ids, exact_weights=T * k <= 8 * E)
+    want, bound = _experts_bounded(x, c1, c2, weights, ids)
     _near(ops.experts_w4(x, *_packed(c1, c2), weights, ids), want, bound)
 
 
@@ -223,4 +229,18 @@ def test_experts_of_a_whole_chunk(E, k, offset, all_experts):
     p[:, offset + 5] += 2.0
     weights, ids = ops.route_experts(p, k)
     got = ops.experts_w4(x, *_packed(c1, c2), weights, ids, expert_offset=offset, num_experts=all_experts)
-    _near(got, *_experts_rounded(x, c1, c2, weights, ids, offset))
+    _near(got, *_experts_bounded(x, c1, c2, weights, ids, offset))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k", [(40, 64, 2), (300, 8, 2), (700, 5, 3), (4000, 8, 2)])
+def test_experts_lose_no_bits_with_more_tokens(T, E, k, dtype):
+    """In the 2-norm: two roundings to bf16 and nothing else, of the activated values and of the result. A rounding
+    is even over half a step to either side, 2^-8 / sqrt(3) at most for values just above a power of two;
+    a hundredth more for fp32 sums and chance. (Rounded weights would add three more.)"""
+    c1, c2 = _codes((E, 512, 512), 64, True, dtype), _codes((E, 512, 256), 32, False, dtype)
+    x = torch.randn(T, 512, device=DEV).to(torch.bfloat16)
+    weights, ids = ops.route_experts(torch.randn(T, E, device=DEV), k)
+    want, _ = _experts_wide(x, c1, c2, weights, ids)
+    got = ops.experts_w4(x, *_packed(c1, c2), weights, ids)
+    assert (got.double() - want).norm() / want.norm() <= 1.01 * (2 * R ** 2 / 3) ** 0.5
