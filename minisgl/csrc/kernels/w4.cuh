@@ -384,6 +384,13 @@ struct W4Runs {
   }
 };
 
+// An activated value as the sum of two bf16 (16 bits of it): its upper half, and what is left. Infinities have nothing left.
+MSGL_DEVICE void w4_act_parts(float v, __nv_bfloat16& upper, __nv_bfloat16& rest) {
+  const float u = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  upper = __float2bfloat16(u);
+  rest = __float2bfloat16(v == u ? 0.f : v - u);
+}
+
 // The rarer activations are a call: inlined copies would lengthen a short launch by their first execution.
 static __noinline__ __device__ float w4_other_act(float g, float u, int act) {
   if (act == 1) return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;

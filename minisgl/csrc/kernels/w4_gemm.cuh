@@ -25,7 +25,7 @@
 // first four bits and the rest, a code times the first is exact in bf16, times the rest too (fp16 scales leave 7 bits: off
 // by half a step of bf16 of an eighth of the weight at most, 2^-12 of it), and both are tiles of A, multiplied one after
 // the other into the same sums: 0.0023, which is what the roundings of the activated values and of the result leave. The
-// price, 128 experts of 2048 x 768, 8 a token, beside rounded weights: 512 tokens 181 us and 160, 2048 tokens 408 and
+// price, 128 experts of 2048 x 768, 8 a token, beside rounded weights: 512 tokens 181 us and 160, 2048 tokens 400 and
 // 334; with fp16 scales 512 tokens 190 and 192.
 //
 // 256 rows per tile (H = 2) because the tokens' rows come from L2 once per tile: with 128 rows 200 tokens x

@@ -4,15 +4,16 @@
 // Few tokens: the chosen experts' tiles, one after another, are cut into equal runs, one per SM. Every CTA
 // counts the pairs per expert itself (they are few) instead of waiting for a kernel that would, so a
 // layer is three launches; the counting of the second product overlaps the end of the first. The
-// activated values between the products are bf16, as the second product's operands are; weights are exact in both
-// forms; y is fp32 and the sum over a token's experts runs in the order of its choices, so results do not vary.
+// activated values between the products are two bf16 each, 16 bits, whose columns are mostly there anyway (in one, their
+// rounding put the result 0.0024 off in the 2-norm, where its own rounding is 0.0017); y is fp32 and the sum over a
+// token's experts runs in the order of its choices, so results do not vary.
 //
 // Many tokens: a kernel sorts the pairs by expert and lists tiles of up to 64 or 128 of an expert's pairs; the products
 // run on the tensor core (w4_gemm.cuh), the first one gathering the tokens' rows, and the sum is the same.
 //
 // 128 experts of 2048 x 768, 8 a token, groups of 128, whole layer: 1 token 17.9 us (3.0 for the bytes; three launches
-// of 5 to 7 us), 16 tokens 49 (25), 128 tokens 100 (45), 256 tokens 138 (47); on the tensor core 512 tokens 181 (48),
-// 2048 tokens 408 (92), 16384 tokens 2670 (737), of which the one block that sorts the 131072 pairs takes 96 (15 at 2048
+// of 5 to 7 us), 16 tokens 51 (25), 128 tokens 113 (45); on the tensor core 256 tokens 156 (47), 512 tokens 181 (48),
+// 2048 tokens 400 (92), 16384 tokens 2640 (737), of which the one block that sorts the 131072 pairs takes 96 (15 at 2048
 // tokens, 7 at 512).
 #include <algorithm>
 
@@ -38,13 +39,17 @@ struct ExpertArgs {
   W4Tensor w;
   int E, e0, pairs, topk;
   const int32_t* ids;
-  const __nv_bfloat16* in;  // rows of x (gated: token pair / topk) or of the activated values (pair)
+  const __nv_bfloat16* in;  // rows of x (gated: token pair / topk) or of the activated values (pair; two planes, w4_act_parts)
   int64_t in_stride;
   const __nv_bfloat16* bias;  // [E, n]
-  __nv_bfloat16* a;           // gated: [pairs, a_stride]
+  __nv_bfloat16* a;           // gated: [2, pairs, a_stride]
   float* y;                   // else: [pairs, n]
-  int a_stride, act, rows;    // rows: tokens of one pass
+  int a_stride, act, rows;    // rows: pairs of one pass
 };
+
+// columns that a pair takes of the streaming product: the second product has its activated values in two parts, side by
+// side, and adds their sums
+constexpr int columns_of(bool gated) { return gated ? 1 : 2; }
 
 template <int NT, int G, bool Z, bool F, bool GATED>
 __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const __grid_constant__ ExpertArgs p) {
@@ -167,7 +172,9 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
     __syncthreads();
     const int* mine = list;
     {
-      const auto row = [&](int r) { return p.in + (int64_t)(GATED ? mine[r] / p.topk : mine[r]) * p.in_stride; };
+      const auto row = [&](int r) {
+        return p.in + (GATED ? mine[r] / p.topk : (int64_t)(r & 1) * p.pairs + mine[r >> 1]) * p.in_stride;
+      };
       const auto emit = [&](int tile, const float (&acc)[2][NT][4]) {
 #pragma unroll
         for (int r = 0; r < (GATED ? 2 : 4); ++r) {
@@ -177,20 +184,25 @@ __global__ void __launch_bounds__(w4_threads<NT>(), 1) w4_experts_kernel(const _
           const float b0 = b == nullptr ? 0.f : __bfloat162float(b[0]);
           const float b1 = !GATED || b == nullptr ? 0.f : __bfloat162float(b[p.w.n / 2]);
 #pragma unroll
-          for (int q = 0; q < NT; ++q)
+          for (int q = 0; q < NT; ++q) {
+            if constexpr (GATED) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int m = q * 8 + 2 * t + c;
-              if (m >= nx) continue;
-              if constexpr (GATED)
-                p.a[(int64_t)mine[m] * p.a_stride + n] =
-                    __float2bfloat16(w4_gated_act(acc[r][q][c] * kW4Unit + b0, acc[r][q][2 + c] * kW4Unit + b1, p.act));
-              else
-                p.y[(int64_t)mine[m] * p.w.n + n] = acc[r >> 1][q][2 * (r & 1) + c] * kW4Unit + b0;
+              for (int c = 0; c < 2; ++c) {
+                const int m = q * 8 + 2 * t + c;
+                if (m >= nx) continue;
+                __nv_bfloat16* a = p.a + (int64_t)mine[m] * p.a_stride + n;
+                w4_act_parts(w4_gated_act(acc[r][q][c] * kW4Unit + b0, acc[r][q][2 + c] * kW4Unit + b1, p.act), a[0],
+                             a[(int64_t)p.pairs * p.a_stride]);
+              }
+            } else {
+              const int m = q * 4 + t;
+              const float(&v)[4] = acc[r >> 1][q];
+              if (m < nx) p.y[(int64_t)mine[m] * p.w.n + n] = (v[2 * (r & 1)] + v[2 * (r & 1) + 1]) * kW4Unit + b0;
             }
+          }
         }
       };
-      runs.template run<false>(p.w, (int64_t)e * p.w.tiles + ta, nt, 0, p.w.kc, xs, pitch, nx, row, emit);
+      runs.template run<false>(p.w, (int64_t)e * p.w.tiles + ta, nt, 0, p.w.kc, xs, pitch, nx * columns_of(GATED), row, emit);
     }
     pos += nt;
   }
@@ -232,8 +244,8 @@ template <int NT, int G, bool Z, bool F, bool GATED>
 int launch_experts(ExpertArgs p, bool launch, cudaStream_t s) {
   constexpr auto kernel = w4_experts_kernel<NT, G, Z, F, GATED>;
   constexpr int kRun = w4_run_bytes<NT, G, Z>();
-  const int pitch = w4_pitch(p.w.kc * 128);
-  p.rows = std::min(NT * 8, (kSmemMax - kRun - prelude_bytes(p.E, p.pairs, 1)) / pitch);
+  const int pitch = w4_pitch(p.w.kc * 128) * columns_of(GATED);  // of a pair's rows
+  p.rows = std::min(NT * 8 / columns_of(GATED), (kSmemMax - kRun - prelude_bytes(p.E, p.pairs, 1)) / pitch);
   if (p.rows < 1) return 3;
   const int64_t most = (int64_t)(std::min(p.E, p.pairs) + p.pairs / p.rows) * p.w.tiles;
   if (most * 2 >= (1ll << 31)) return 3;
@@ -244,13 +256,13 @@ int launch_experts(ExpertArgs p, bool launch, cudaStream_t s) {
   return w4_launch(kernel, dim3(grid), dim3(w4_threads<NT>()), smem, s, 1, p) == cudaSuccess ? 0 : 4;
 }
 
-// One product of experts out of `total`. Token columns per pass: 8 while an expert has at most 4 tokens on average (its
-// tokens then rarely exceed 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of
-// 2048 x 768: at 4 tokens 77 us with columns of 8 and 81 with 16, at 8 tokens 112 and 100.
+// One product of experts out of `total`. Columns per pass: 8 while an expert has at most 4 on average (it then rarely has
+// more than 8), else 16; a second pass reads the expert's weights again, mostly from L2. 128 experts of 2048 x 768, both
+// products with one column a pair: at 4 pairs 77 us with columns of 8 and 81 with 16, at 8 pairs 112 and 100.
 template <bool GATED>
 int experts_product(const ExpertArgs& p, const MsglW4* w, int total, bool launch, cudaStream_t s) {
   return w4_dispatch(w, [&](auto g, auto z, auto f) {
-    return p.pairs <= 4ll * total ? launch_experts<1, g(), z(), f(), GATED>(p, launch, s)
+    return p.pairs * columns_of(GATED) <= 4ll * total ? launch_experts<1, g(), z(), f(), GATED>(p, launch, s)
                               : launch_experts<2, g(), z(), f(), GATED>(p, launch, s);
   });
 }
@@ -325,7 +337,7 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
   const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   Scratch s;
   s.a = 0;
-  s.y = up(pairs * w2->kc * 128 * 2);
+  s.y = up((pairs <= kMoeMaxPairs ? 2 : 1) * pairs * w2->kc * 128 * 2);  // (the streaming product's in two parts)
   s.sorted = s.y + up(pairs * w2->n * 4);
   s.place = s.sorted + up(pairs * 4);
   s.work = s.place + up(pairs * 4);
@@ -335,10 +347,10 @@ Scratch scratch_of(int64_t pairs, int E, const MsglW4* w2) {
 }
 
 // Pairs per expert up to which the streaming product is taken. 128 experts of 2048 x 768, streaming and on the tensor
-// core: at 16 a layer takes 138 and 156 us, at 20 156 and 165, at 24 176 and 171; 32 experts of 2880 x 2880, groups of 32
-// with zero points: at 16 193 and 205, at 25 254 and 228. Where only a share of the experts is here, pairs and experts of
-// all ranks count: 8 of 64 experts of 2880 x 2880 at 32 tokens, 8 a token, 35 us streaming and 64 on the tensor core.
-constexpr int kStreamPairs = 20;
+// core: at 12 a layer takes 140 and 146 us, at 14 151 and 153, at 16 163 and 156; 32 experts of 2880 x 2880, groups of 32
+// with zero points: at 12.5 both 198, at 16 231 and 205. Where only a share of the experts is here, pairs and experts of
+// all ranks count: 8 of 64 experts of 2880 x 2880 at 32 tokens, 8 a token, 38 us streaming and 74 on the tensor core.
+constexpr int kStreamPairs = 12;
 
 int experts_tiles(const void* x, int64_t x_stride, int pairs, int topk, const MsglW4* w1, const MsglW4* w2, int E, int e0,
                   int total, const int32_t* ids, const void* b1, const void* b2, int act, uint8_t* ws, const Scratch& sc,

@@ -23,7 +23,8 @@ multiplies the fp32 sum of its group); for more tokens, and for rows too wide fo
 memory, every weight is rounded once to bf16, as in a bf16 copy of the weights. A token's result so moves
 a little, within what one rounding of the weights does, when a batch passes from the one to the other.
 The experts' products hold weights exactly for any number of tokens (for many tokens and fp16 scales: to
-2^-12). Equal calls give equal results.
+2^-12), the activated values between them in 16 bits for few tokens (up to 12 pairs of a token and an
+expert per expert) and in bf16 for more. Equal calls give equal results.
 """
 
 from __future__ import annotations
@@ -236,8 +237,8 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
     here), by which the GPU estimates how many tokens an expert gets and chooses its form. ``activation``:
     ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU a call takes up to 1024 experts and 2^24
     pairs of a token and an expert.
-    The activated values between the two products are held in bf16, weights exactly (to 2^-12 of them with
-    fp16 scales and many tokens), sums in fp32. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
+    The activated values between the two products are held in 16 bits, in bf16 above 12 pairs per expert,
+    weights exactly (to 2^-12 of them with fp16 scales and many tokens), sums in fp32. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
     ``w1_bias [E, 2I]`` and ``w2_bias [E, H]`` are contiguous."""
     if not (w1.experts and w1.gated and w2.experts and not w2.gated):
         raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")
