@@ -170,8 +170,8 @@ int linear_tiles(const LinearArgs& a, const MsglW4* w, cudaStream_t s) {
   p.bn = ((a.M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
   p.m_tiles = (a.M + p.bn - 1) / p.bn;
   // Halves of a tile and cuts of the inputs with the least estimated time, in clocks per 128 inputs of a tile:
-  // conversion 450 a half (measured with bf16 scales; fp16 ones take about a quarter longer), the tensor core 4 a token and half, the tokens' rows from L2 5 a token;
-  // the exchange 2000 and 20 a token and half.
+  // conversion 450 a half (measured with bf16 scales; fp16 ones take about a quarter longer), the tensor core 4 a token and
+  // half, the tokens' rows from L2 5 a token; the exchange 2000 and 20 a token and half.
   double best = 1e30;
   int halves = 1;
   const int only_h = g_halves.load(), only_s = g_splits.load();

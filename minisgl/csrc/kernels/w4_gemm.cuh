@@ -9,8 +9,8 @@
 //   warp 8       bulk copies of the tile's records of 128 inputs (two steps) into a ring of their own
 //   warp 9       MMA issuer: D_h[128 x N] += A_h[128 x 64] B[N x 64]^T, fp32 in TMEM, two sets if they fit
 //   warps 10-25  records -> bf16 A tiles in tensor memory: the codes become bf16 as in w4.cuh, times the group's
-//                scale (experts: its two parts). Half of them take the even steps, half the odd ones: one half converts while the other
-//                waits for its barriers and its stores.
+//                scale (experts: its two parts). Half of them take the even steps, half the odd ones: one half
+//                converts while the other waits for its barriers and its stores.
 // What bounds it is the conversion's issue slots (about 1000 warp instructions of a step's 1900; 64% of the slots are used
 // at 32 tokens, the tensor pipe 17% of the time) and, next to it, the latency of one step through conversion, MMA and
 // release: 640 clocks a step with few tokens, 17 x 34816 x 5120 33 us; 200 x 34816 x 5120 57 us, 1.26 PFLOP/s, 75% of a

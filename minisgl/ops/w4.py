@@ -238,8 +238,9 @@ def experts_w4(x: torch.Tensor, w1: W4Weight, w2: W4Weight, weights: torch.Tenso
     ``silu``, ``gelu`` (tanh form) or ``swiglu_oai``. On the GPU a call takes up to 1024 experts and 2^24
     pairs of a token and an expert.
     The activated values between the two products are held in 16 bits, in bf16 above 12 pairs per expert,
-    weights exactly (to 2^-12 of them with fp16 scales and many tokens), sums in fp32. ``x`` may be strided; ``weights``, ``ids`` and the bf16 biases
-    ``w1_bias [E, 2I]`` and ``w2_bias [E, H]`` are contiguous."""
+    weights exactly (to 2^-12 of them with fp16 scales and many tokens), sums in fp32. ``x`` may be
+    strided; ``weights``, ``ids`` and the bf16 biases ``w1_bias [E, 2I]`` and ``w2_bias [E, H]`` are
+    contiguous."""
     if not (w1.experts and w1.gated and w2.experts and not w2.gated):
         raise ValueError("experts_w4 takes w1 [E, 2I, H] packed with gated=True and w2 [E, H, I] without")
     if activation not in _ACT:
