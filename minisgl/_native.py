@@ -29,7 +29,7 @@ class _CountingModule:
                    "ipc_handle", "ipc_open", "ipc_close", "peer_grid", "nvls_grid", "nvls_flag_bytes",
                    "nvls_state_words", "nvls_ticket_offset", "gemm_force_bn", "w4_force_form", "attention_prefill_trace"}
 
-    _COUNTED = {"linear_w4", "experts_w4"}  # return how many kernels they launched beside their result
+    _COUNTED = {"linear_w4", "experts_w4", "attention_kv8"}  # return how many kernels they launched beside their result
 
     def __init__(self, mod):
         self._mod = mod

@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -578,6 +579,141 @@ std::tuple<at::Tensor, int> experts_w4(at::Tensor x, at::Tensor data1, int64_t n
   return {out, launches};
 }
 
+// ----- 8-bit key/value cache
+struct Kv8Tensors {
+  at::Tensor k, v, k_scale, v_scale;
+};
+
+// the cache's tensors (ops.KV8Cache checks the same when it is made); returns whether the codes are e4m3
+bool kv8_check(const Kv8Tensors& c) {
+  check_cuda(c.k, "cache");
+  const bool fp8 = c.k.scalar_type() == at::kFloat8_e4m3fn;
+  CHECK(fp8 || c.k.scalar_type() == at::kChar, "8-bit cache codes must be int8 or float8_e4m3fn, got ", c.k.scalar_type());
+  CHECK(c.k.dim() == 3 && (c.k.size(2) == 64 || c.k.size(2) == 128) && c.k.size(0) > 0 && c.k.size(1) > 0 &&
+            c.k.size(1) % 16 == 0 && c.k.size(0) * c.k.size(1) < (1ll << 31),
+        "8-bit cache codes must be [kv heads, slots, 64 or 128] with pages of 16 slots, got ", c.k.sizes());
+  CHECK(c.v.sizes() == c.k.sizes() && c.v.scalar_type() == c.k.scalar_type(), "8-bit cache: value codes do not match the keys'");
+  for (const at::Tensor* t : {&c.k_scale, &c.v_scale})
+    CHECK(t->scalar_type() == at::kFloat && t->sizes() == c.k.sizes().slice(0, 2), "8-bit cache scales must be fp32 [kv heads, slots]");
+  for (const at::Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale})
+    CHECK(t->device() == c.k.device() && t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+          "8-bit cache: codes and scales must be contiguous, 16-byte aligned and on one device");
+  return fp8;
+}
+
+const int32_t* kv8_ids(const at::Tensor& t, int64_t n, const at::Device& dev, const char* name) {
+  CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.device() == dev, name,
+        " must be contiguous int32 [", n, "] on the cache's device, got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+  return t.data_ptr<int32_t>();
+}
+
+// rows of heads as the kernels read them: unit inner stride, every head's row on a 16-byte boundary; else a copy
+at::Tensor kv8_rows(const at::Tensor& x, int64_t heads, int64_t hd, const at::Device& dev, const char* name) {
+  CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 3 && (heads < 0 || x.size(1) == heads) && x.size(2) == hd && x.device() == dev,
+        name, " must be bf16 [tokens, heads, ", hd, "] on the cache's device, got ", x.scalar_type(), " ", x.sizes(), " on ", x.device());
+  if (x.stride(2) == 1 && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && (x.size(1) <= 1 || x.stride(1) % 8 == 0) &&
+      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
+    return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+
+void store_kv8(at::Tensor k, at::Tensor v, at::Tensor ck, at::Tensor cv, at::Tensor sk, at::Tensor sv, at::Tensor out_loc) {
+  const bool fp8 = kv8_check({ck, cv, sk, sv});
+  const at::Device dev = ck.device();
+  const int64_t nkv = ck.size(0), hd = ck.size(2), n = k.dim() ? k.size(0) : 0;
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor kr = kv8_rows(k, nkv, hd, dev, "store_kv8: k"), vr = kv8_rows(v, nkv, hd, dev, "store_kv8: v");
+  CHECK(v.size(0) == n && n < (1ll << 31), "store_kv8: k and v must be of the same tokens, less than 2^31");
+  const int32_t* slots = kv8_ids(out_loc, n, dev, "store_kv8: out_loc");
+  if (n == 0) return;
+  const Kv8Store p{kr.data_ptr(), vr.data_ptr(), kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1), ck.data_ptr(),
+                   cv.data_ptr(), sk.data_ptr<float>(), sv.data_ptr<float>(), slots, (int)n, (int)nkv, (int)ck.size(1)};
+  check_launch(msgl_kv8_store(&p, hd, fp8, stream()), "store_kv8");
+}
+
+std::tuple<at::Tensor, at::Tensor> load_kv8(at::Tensor ck, at::Tensor cv, at::Tensor sk, at::Tensor sv, at::Tensor slots) {
+  const bool fp8 = kv8_check({ck, cv, sk, sv});
+  const at::Device dev = ck.device();
+  const int64_t nkv = ck.size(0), hd = ck.size(2), n = slots.numel();
+  CHECK(n < (1ll << 31), "load_kv8: less than 2^31 slots");
+  const int32_t* at = kv8_ids(slots, n, dev, "load_kv8: slots");
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor k = new_cuda({n, nkv, hd}, at::kBFloat16, dev), v = new_cuda({n, nkv, hd}, at::kBFloat16, dev);
+  if (n == 0) return {k, v};
+  const Kv8Load p{k.data_ptr(), v.data_ptr(), ck.data_ptr(), cv.data_ptr(), sk.data_ptr<float>(), sv.data_ptr<float>(), at,
+                  (int)n, (int)nkv, (int)ck.size(1)};
+  check_launch(msgl_kv8_load(&p, hd, fp8, stream()), "load_kv8");
+  return {k, v};
+}
+
+// bytes that a tensor lies in
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
+  int64_t last = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {a, a + last * t.element_size()};
+}
+
+std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tensor cv, at::Tensor sk, at::Tensor sv,
+                                          at::Tensor page_table, at::Tensor rows, at::Tensor cu_q, at::Tensor kv_lens, int64_t page,
+                                          int64_t max_q_len, c10::optional<double> scale, int64_t window,
+                                          c10::optional<at::Tensor> sinks, c10::optional<at::Tensor> out) {
+  const bool fp8 = kv8_check({ck, cv, sk, sv});
+  const at::Device dev = ck.device();
+  const int64_t nkv = ck.size(0), hd = ck.size(2), B = rows.numel();
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor qr = kv8_rows(q, -1, hd, dev, "attention_kv8: q");
+  const int64_t T = q.size(0), nq = q.size(1);
+  CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 128, "attention_kv8: ", nq, " query heads over ", nkv, " kv heads (1 to 128 each)");
+  CHECK(T * nq < (1ll << 31) && B < (1ll << 24), "attention_kv8: too many queries for one call");
+  CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt && page_table.device() == dev &&
+            (page_table.numel() == 0 || page_table.stride(1) == 1 || page_table.size(1) == 1) && page_table.size(0) < (1ll << 31) &&
+            page_table.size(1) < (1ll << 31),
+        "attention_kv8: page_table must be int32 [rows, positions] with unit inner stride on the cache's device, got ",
+        page_table.scalar_type(), " ", page_table.sizes());
+  Kv8Attn p;
+  p.rows = kv8_ids(rows, B, dev, "attention_kv8: rows");
+  p.cu_q = kv8_ids(cu_q, B + 1, dev, "attention_kv8: cu_q");
+  p.kv_lens = kv8_ids(kv_lens, B, dev, "attention_kv8: kv_lens");
+  CHECK(page >= 16 && page % 16 == 0, "attention_kv8: pages must be a multiple of 16 slots, got ", page);
+  CHECK(max_q_len >= -1, "attention_kv8: max_q_len must not be negative");
+  CHECK(window == -1 || window >= 1, "attention_kv8: window must be positive, or -1 for none, got ", window);
+  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)hd);
+  CHECK(std::isfinite(sc), "attention_kv8: scale must be finite, got ", sc);
+  p.sinks = nullptr;
+  if (sinks.has_value()) {
+    CHECK(sinks->scalar_type() == at::kFloat && sinks->dim() == 1 && sinks->size(0) == nq && sinks->is_contiguous() &&
+              sinks->device() == dev, "attention_kv8: sinks must be contiguous fp32 [", nq, "] on the cache's device");
+    p.sinks = sinks->data_ptr<float>();
+  }
+  at::Tensor o;
+  if (out.has_value()) {
+    CHECK(out->scalar_type() == at::kBFloat16 && out->sizes() == q.sizes() && out->is_contiguous() && out->device() == dev &&
+              reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0,
+          "attention_kv8: out must be contiguous bf16 ", q.sizes(), ", 16-byte aligned, on the cache's device");
+    if (T > 0) {
+      const auto a = span_of(q), b = span_of(*out);
+      CHECK(a.second <= b.first || b.second <= a.first, "attention_kv8: out must not overlap q");
+    }
+    o = *out;
+  } else {
+    o = new_cuda({T, nq, hd}, at::kBFloat16, dev);
+  }
+  if (T == 0) return {o, 0};
+  p.o = o.data_ptr(); p.q = qr.data_ptr(); p.q_row = qr.stride(0); p.q_head = qr.stride(1);
+  p.ck = ck.data_ptr(); p.cv = cv.data_ptr(); p.sk = sk.data_ptr<float>(); p.sv = sv.data_ptr<float>();
+  p.page_table = page_table.data_ptr<int32_t>(); p.pt_stride = page_table.stride(0);
+  p.pt_rows = page_table.size(0); p.pt_width = page_table.size(1); p.num_slots = ck.size(1); p.num_reqs = B; p.total_q = T;
+  p.nq = nq; p.nkv = nkv;
+  p.page = page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
+  p.window = window >= p.pt_width ? -1 : (int)window;  // (one as long as the table hides no key)
+  p.zero_tail = !out.has_value();
+  p.scale = (float)sc;
+  int launches = 0;
+  check_launch(msgl_kv8_attention(&p, hd, fp8, max_q_len < 0 ? T : std::min<int64_t>(max_q_len, T), &launches, stream()), "attention_kv8");
+  return {o, launches};
+}
+
 // ----- peer-memory collectives
 int64_t peer_alloc(int64_t bytes) {
   void* p = msgl_peer_alloc(bytes);
@@ -712,6 +848,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_w4", &linear_w4);
   m.def("w4_force_form", [](int halves, int splits) { msgl_w4_force_form(halves, splits); });
   m.def("experts_w4", &experts_w4);
+  m.def("store_kv8", &store_kv8);
+  m.def("load_kv8", &load_kv8);
+  m.def("attention_kv8", &attention_kv8);
 
   m.def("moe_route", &moe_route);
   m.def("moe_align", &moe_align, py::arg("ids"), py::arg("E"), py::arg("bn"), py::arg("perm"), py::arg("inv"),

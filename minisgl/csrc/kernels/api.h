@@ -116,6 +116,43 @@ int msgl_w4_experts(void* out, const void* x, int64_t x_stride, int T, int topk,
                     int E, int e0, int total, const float* weights, const int32_t* ids, const void* b1, const void* b2,
                     int act, void* workspace, int* launches, cudaStream_t s);
 
+// ----- 8-bit key/value cache (layout in kv8.cu; fp8: e4m3 codes, else int8). Each returns 0, 2 if a tensor map could
+// not be encoded, 3 on unsupported sizes, 4 if a launch failed. Negative slots are skipped or read as zeros.
+typedef struct {
+  const void *k, *v;  // bf16 rows: [n] tokens x [nkv] heads, strides in elements (16-byte aligned)
+  int64_t k_row, k_head, v_row, v_head;
+  void *ck, *cv;  // codes [nkv][num_slots][hd]
+  float *sk, *sv;  // scales [nkv][num_slots]
+  const int32_t* slots;  // [n]
+  int n, nkv, num_slots;
+} Kv8Store;
+int msgl_kv8_store(const Kv8Store* p, int hd, int fp8, cudaStream_t s);
+typedef struct {
+  void *k, *v;  // bf16 [n][nkv][hd]
+  const void *ck, *cv;
+  const float *sk, *sv;
+  const int32_t* slots;
+  int n, nkv, num_slots;
+} Kv8Load;
+int msgl_kv8_load(const Kv8Load* p, int hd, int fp8, cudaStream_t s);
+// Ragged causal attention over the paged cache (kv8_attn.cu).
+typedef struct {
+  void* o;        // bf16 [total_q][nq][hd]
+  const void* q;  // bf16, strides in elements
+  int64_t q_row, q_head;
+  const void *ck, *cv;
+  const float *sk, *sv;
+  const int32_t* page_table;  // [pt_rows][pt_width], rows pt_stride apart
+  int64_t pt_stride;
+  const int32_t *rows, *cu_q, *kv_lens;
+  const float* sinks;  // [nq] or null
+  int pt_rows, pt_width, num_slots, num_reqs, total_q, nq, nkv, page;
+  int window;     // keys a query sees at most, -1: all up to its own
+  int zero_tail;  // rows behind the last request's are set to zero
+  float scale;
+} Kv8Attn;
+int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, int* launches, cudaStream_t s);
+
 // ----- paged attention (bf16 q/kv, fp32 softmax)
 void msgl_attention_prefill(void* o, const void* q, const void* k_cache, const void* v_cache,
                             const int32_t* page_table, int64_t pt_stride, const int32_t* rows,

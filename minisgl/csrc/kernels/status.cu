@@ -10,10 +10,12 @@ extern "C" int msgl_err_moe(int* info);
 extern "C" int msgl_err_plan(int* info);
 extern "C" int msgl_err_w4(int* info);
 extern "C" int msgl_err_w4_moe(int* info);
+extern "C" int msgl_err_kv8(int* info);
+extern "C" int msgl_err_kv8_attn(int* info);
 
 extern "C" int msgl_get_error(int* info) {
   int (*fns[])(int*) = {msgl_err_gemm, msgl_err_elementwise, msgl_err_attention, msgl_err_sampling, msgl_err_comm, msgl_err_moe, msgl_err_plan,
-                        msgl_err_w4, msgl_err_w4_moe};
+                        msgl_err_w4, msgl_err_w4_moe, msgl_err_kv8, msgl_err_kv8_attn};
   int first = 0;
   for (auto f : fns) {
     int inf = 0;

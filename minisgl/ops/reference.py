@@ -177,6 +177,74 @@ def paged_attention(
     return out
 
 
+def quantise_kv8(x: torch.Tensor, dtype: torch.dtype):
+    """Rows of ``x [..., hd]`` in 8 bits: (codes, fp32 scales ``[...]``). The quotients are taken in 64 bits, where a
+    16-bit value's is never rounded over a border."""
+    largest = 127.0 if dtype == torch.int8 else 448.0
+    top = x.float().abs().amax(-1, keepdim=True)
+    top = torch.where(x.float().isfinite().all(-1, keepdim=True), top, math.nan)
+    quot = torch.where(top > 0, x.double() * largest / top.double(), 0.0)
+    codes = quot.round().to(torch.int8) if dtype == torch.int8 else quot.float().to(dtype)
+    return codes, (top / largest).squeeze(-1)
+
+
+def store_kv8(k, v, cache, out_loc) -> None:
+    keep = out_loc >= 0
+    at = out_loc[keep].long()
+    for x, codes, scale in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        q, s = quantise_kv8(x[keep], codes.dtype)
+        codes.view(torch.uint8)[:, at] = q.view(torch.uint8).transpose(0, 1)
+        scale[:, at] = s.transpose(0, 1)
+
+
+def load_kv8(cache, slots):
+    at = slots.long().clamp(min=0)
+    keep = (slots >= 0).view(-1, 1, 1)
+    return tuple(torch.where(keep, (codes[:, at].float() * scale[:, at, None]).transpose(0, 1), 0.0).to(torch.bfloat16)
+                 for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+
+
+def attention_kv8(q, cache, page_table, rows, cu_q, kv_lens, page_size: int, scale: float, window: int, sinks, out=None):
+    """Plain form of ``ops.attention_kv8``."""
+    T, nq, hd = q.shape
+    g = nq // cache.num_kv_heads
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format) if out is None else out
+    ends, lens, rws = cu_q.tolist(), kv_lens.tolist(), rows.tolist()
+    if lens and (ends[0] != 0 or any(a > b for a, b in zip(ends, ends[1:])) or ends[-1] > T):
+        raise ValueError(f"attention_kv8: cu_q must rise from 0 to at most {T}")
+    for b, L in enumerate(lens):
+        s, e = ends[b], ends[b + 1]
+        if e == s:
+            continue
+        if not 0 <= rws[b] < page_table.shape[0] or not 0 <= L <= page_table.shape[1]:
+            raise ValueError(f"attention_kv8: row {rws[b]} and length {L} of a table {tuple(page_table.shape)}")
+        if L == 0:
+            out[s:e] = 0
+            continue
+        pos = torch.arange(L)
+        page = page_table[rws[b], torch.arange(0, L, page_size)].long()
+        if int(page.min()) < 0 or int(page.max()) > cache.num_slots - page_size or bool((page % page_size).any()):
+            raise ValueError("attention_kv8: a page is not in the cache")
+        at = page.repeat_interleave(page_size)[:L] + pos % page_size
+        kx = (cache.k[:, at].float() * cache.k_scale[:, at, None]).repeat_interleave(g, dim=0)
+        vx = (cache.v[:, at].float() * cache.v_scale[:, at, None]).repeat_interleave(g, dim=0)
+        scores = torch.einsum("qhd,hkd->hqk", q[s:e].float(), kx) * scale
+        mine = torch.arange(L - (e - s), L)[:, None]
+        seen = pos <= mine
+        if window > 0:
+            seen &= pos > mine - window
+        scores = scores.masked_fill(~seen, -math.inf)
+        if sinks is not None:
+            scores = torch.cat([scores, sinks.view(nq, 1, 1).expand(nq, e - s, 1)], dim=-1)
+        p = torch.softmax(scores, dim=-1)[..., :L]
+        # a hidden key's value does not count, whatever it is; a seen one that is no number makes the output none
+        lost = ~vx.isfinite().all(-1)
+        o = torch.einsum("hqk,hkd->qhd", p.where(seen, 0.0), vx.where(~lost.unsqueeze(-1), 0.0))
+        o = o.masked_fill((seen & lost.unsqueeze(1)).any(-1).t().unsqueeze(-1), math.nan)
+        out[s:e] = o.where(seen.any(-1).view(-1, 1, 1), 0.0).to(q.dtype)
+    return out
+
+
 def argmax(logits: torch.Tensor) -> torch.Tensor:
     return torch.argmax(logits.float(), dim=-1).to(torch.int32)
 
