@@ -709,8 +709,10 @@ std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tenso
   p.window = window >= p.pt_width ? -1 : (int)window;  // (one as long as the table hides no key)
   p.zero_tail = !out.has_value();
   p.scale = (float)sc;
+  const int most = max_q_len < 0 ? std::max<int64_t>(T - B + 1, 1) : std::min<int64_t>(max_q_len, T);  // (not told: a query each, one with the rest)
   int launches = 0;
-  check_launch(msgl_kv8_attention(&p, hd, fp8, max_q_len < 0 ? T : std::min<int64_t>(max_q_len, T), &launches, stream()), "attention_kv8");
+  at::Tensor ws = new_cuda({msgl_kv8_attention_workspace(&p, hd, most)}, at::kByte, dev);
+  check_launch(msgl_kv8_attention(&p, hd, fp8, most, ws.data_ptr(), &launches, stream()), "attention_kv8");
   return {o, launches};
 }
 

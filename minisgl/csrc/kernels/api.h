@@ -151,7 +151,8 @@ typedef struct {
   int zero_tail;  // rows behind the last request's are set to zero
   float scale;
 } Kv8Attn;
-int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, int* launches, cudaStream_t s);
+int64_t msgl_kv8_attention_workspace(const Kv8Attn* p, int hd, int max_q_len);  // bytes, written before they are read
+int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, void* workspace, int* launches, cudaStream_t s);
 
 // ----- paged attention (bf16 q/kv, fp32 softmax)
 void msgl_attention_prefill(void* o, const void* q, const void* k_cache, const void* v_cache,

@@ -23,4 +23,55 @@ MSGL_DEVICE float2 kv8_decode2(uint32_t pair) {
   }
 }
 
+// Four codes (one register) to two fp16 pairs, exactly: lo holds the first two values, hi the others. int8: the byte
+// with its sign bit turned is the low mantissa of 1024 + (code + 128), from which 1152 is taken.
+template <bool FP8>
+MSGL_DEVICE void kv8_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
+  } else {
+    const uint32_t u = codes ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+// 2^x, to 2^-22 of it (2^-126 and below: zero)
+MSGL_DEVICE float kv8_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+MSGL_DEVICE uint32_t pack_half(float a, float b) {
+  const __half2 t = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// The power of two that brings a row of queries with this largest magnitude to [2^14, 2^15), where fp16 holds them
+// exactly down to 2^-31 of the largest; 1 for rows of zeros and rows that are not finite.
+MSGL_DEVICE float kv8_q_factor(float top) {
+  if (!(top > 0.f) || !(top < INFINITY)) return 1.f;
+  const int e = (int)(__float_as_uint(top) >> 23);  // biased
+  return __uint_as_float((uint32_t)min(268 - e, 253) << 23);
+}
+MSGL_DEVICE float kv8_reciprocal(float power_of_two) { return __uint_as_float((254u << 23) - __float_as_uint(power_of_two)); }
+
+// A softmax weight times its value's scale is rounded to fp16, so it is that product which must lie in fp16's range, not
+// the probability: a token that takes nearly all of a softmax often has a value row of nearly nothing. So a row's
+// running offset m is the maximum of s_j + log2 s^v_j, less kKv8Top, not that of the logits s_j: products
+// 2^(s_j - m) s^v_j are at most 2^14, and 11 bits hold down to 2^-28 of the largest. The sum of the 2^(s_j - m) is fp32, with
+// the same m, and keeps its own range as long as a row's scales are between 2^-96 and 2^96; smaller ones (a row of zeros has
+// 0) are taken for 2^-96 in m, which leaves the products right but smaller.
+constexpr float kKv8Top = 14.f;
+MSGL_DEVICE float kv8_log_scale(float scale) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
+  return fminf(fmaxf(y, -96.f), 96.f);
+}
+
 }  // namespace msgl

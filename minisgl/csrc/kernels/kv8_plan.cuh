@@ -1,0 +1,251 @@
+// How attention over the 8-bit cache spreads its work, and how it joins what was cut.
+//
+// The rows of a request and kv head are its (token, head of the group) pairs, packed: row r is token r / G, head r % G,
+// so a key read once serves the whole group. A segment is a tile of R rows and the 64-key blocks that any of them
+// sees (at least one, empty or not). All segments' blocks, request by request, head by head, tile by tile, form one row
+// of units that is cut into P equal runs, one per CTA: lengths of any mixture balance without a work list from
+// the host, and a graph replays with new ones. A CTA finds its run by a scan over the requests (some 2 us). Whole
+// segments are written out at once; a run has at most one part of a segment at its start and one at its end, so there
+// are 2 P slots for parts whatever the lengths, and a second kernel joins each cut segment from its first part's header.
+// That kernel costs about 2 us; counters that let the last part's CTA do it would have to be zeroed by a launch
+// as well, or shared between calls.
+#pragma once
+#include "api.h"
+#include "common.cuh"
+
+namespace msgl {
+
+constexpr int kKv8Block = 64;  // keys per unit
+constexpr float kKv8Log2e = 1.4426950408889634f;
+
+// A request's queries and keys, with what is outside its tables taken out (and recorded).
+struct Kv8Req {
+  int q0, n, L, row;
+};
+MSGL_DEVICE Kv8Req kv8_request(const Kv8Attn& p, int b) {
+  Kv8Req r;
+  const int a = p.cu_q[b], e = p.cu_q[b + 1];
+  r.L = p.kv_lens[b];
+  r.row = p.rows[b];
+  r.q0 = min(max(a, 0), p.total_q);
+  r.n = min(max(e, r.q0), p.total_q) - r.q0;
+  const bool ok = r.q0 == a && r.q0 + r.n == e && r.L >= 0 && r.L <= p.pt_width && (r.L == 0 || (r.row >= 0 && r.row < p.pt_rows));
+  if (!ok) {
+    report_error(kErrBounds, kBcAttnRow);
+    r.L = 0;
+  }
+  return r;
+}
+
+// First slot of the page that holds position `pos` (a multiple of the page), or -1.
+MSGL_DEVICE int kv8_page(const Kv8Attn& p, int row, int pos) {
+  const int slot = p.page_table[(int64_t)row * p.pt_stride + pos];
+  if (slot < 0 || slot > p.num_slots - p.page || slot % p.page != 0) {
+    report_error(kErrBounds, kBcAttnSlot);
+    return -1;
+  }
+  return slot;
+}
+
+// Tile t of a request: rows [r0, r0 + nr), the positions of the first and the last of them, the keys [lo, kend)
+// that any of them sees and the blocks [blk0, blk0 + nblk) that hold those.
+struct Kv8Tile {
+  int r0, nr, pos0, pos1, lo, kend, blk0, nblk;
+};
+template <int R>
+MSGL_DEVICE Kv8Tile kv8_tile(const Kv8Attn& p, const Kv8Req& r, int G, int t) {
+  Kv8Tile k;
+  k.r0 = t * R;
+  k.nr = min(R, r.n * G - k.r0);
+  k.pos0 = r.L - r.n + k.r0 / G;
+  k.pos1 = r.L - r.n + (k.r0 + k.nr - 1) / G;
+  k.kend = max(0, k.pos1 + 1);
+  k.lo = p.window > 0 ? max(0, max(k.pos0, -1) - p.window + 1) : 0;
+  k.blk0 = k.lo / kKv8Block;
+  k.nblk = max(1, (k.kend > 0 ? (k.kend - 1) / kKv8Block + 1 : 0) - k.blk0);
+  return k;
+}
+template <int R>
+MSGL_DEVICE int kv8_tiles(const Kv8Req& r, int G) {
+  return (int)(((int64_t)r.n * G + R - 1) / R);
+}
+
+// A CTA's run of units [u0, u1), and the segment that u0 is in: tile t of head h of request b, from unit s0 on.
+struct Kv8Plan {
+  int64_t total, u0, u1, s0;
+  int ctas, b, h, t;
+};
+// the CTA whose run holds unit u: runs are [total c / P, total (c + 1) / P)
+MSGL_DEVICE int kv8_cta_of(const Kv8Plan& pl, int64_t u) { return (int)(((u + 1) * pl.ctas - 1) / pl.total); }
+
+// All NT threads of the CTA; `red` holds NT / 32 words. A run has at least `least` units.
+template <int R, int NT>
+MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.nq / p.nkv;
+  const int rounds = (p.num_reqs + NT - 1) / NT;
+  int64_t base = 0, v = 0, excl = 0, run0 = 0, run1 = 0;
+  // one round over the requests, NT at a time: v the units of request (round, tid), excl those before it
+  auto scan = [&](int c) {
+    const int b = c * NT + tid;
+    v = 0;
+    if (b < p.num_reqs) {
+      const Kv8Req r = kv8_request(p, b);
+      const int tiles = kv8_tiles<R>(r, G);
+      for (int t = 0; t < tiles; ++t) v += kv8_tile<R>(p, r, G, t).nblk;
+      v *= p.nkv;
+    }
+    int64_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) before += red[w];
+      all += red[w];
+    }
+    excl = base + before + incl - v;
+    base += all;
+  };
+  auto place = [&](int c) {
+    if (run0 < excl || run0 >= excl + v || run0 >= run1) return;
+    const int b = c * NT + tid;
+    const Kv8Req r = kv8_request(p, b);
+    const int64_t per = v / p.nkv;
+    int64_t rem = run0 - excl;
+    pl->b = b;
+    pl->h = (int)(rem / per);
+    rem -= pl->h * per;
+    for (int t = 0;; ++t) {
+      const int nblk = kv8_tile<R>(p, r, G, t).nblk;
+      if (rem < nblk) {
+        pl->t = t;
+        break;
+      }
+      rem -= nblk;
+    }
+    pl->s0 = run0 - rem;
+  };
+  for (int c = 0; c < rounds; ++c) scan(c);
+  const int64_t total = base;
+  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total / least));
+  const int c = blockIdx.x;
+  if (c < ctas) {
+    run0 = total * c / ctas;
+    run1 = total * (c + 1) / ctas;
+  }
+  if (tid == 0) {
+    pl->total = total;
+    pl->ctas = ctas;
+    pl->u0 = run0;
+    pl->u1 = run1;
+  }
+  if (rounds == 1) {
+    place(0);
+  } else {
+    base = 0;
+    for (int i = 0; i < rounds; ++i) {
+      scan(i);
+      place(i);
+    }
+  }
+  __syncthreads();
+}
+
+// Scratch of one call: a header per CTA (of the segment that its run ends in, if cut there and begun in it), and per
+// slot the rows' maxima and sums (the logits' log2 domain) and their sums of values.
+struct Kv8Part {
+  int parts, q0, r0, nr, h, pad[3];  // parts 0: nothing to join
+};
+struct Kv8Scratch {
+  Kv8Part* head;  // [ctas]
+  float2* ml;     // [2 ctas][R]
+  float* o;       // [2 ctas][R][HD]
+};
+template <int R, int HD>
+inline int64_t kv8_scratch_bytes(int ctas) {
+  return (int64_t)ctas * (sizeof(Kv8Part) + 2 * R * (sizeof(float2) + HD * sizeof(float)));
+}
+template <int R, int HD>
+inline Kv8Scratch kv8_scratch(void* ws, int ctas) {
+  Kv8Scratch s;
+  s.head = reinterpret_cast<Kv8Part*>(ws);
+  s.ml = reinterpret_cast<float2*>(s.head + ctas);
+  s.o = reinterpret_cast<float*>(s.ml + (int64_t)2 * ctas * R);
+  return s;
+}
+
+// Softmax factors with a sink: o / l becomes o * result.
+MSGL_DEVICE float kv8_norm(float m, float l, const float* sinks, int head) {
+  float f = 1.f;
+  if (sinks != nullptr && l != 0.f) {
+    const float sink = sinks[head] * kKv8Log2e, mn = fmaxf(m, sink);
+    f = exp2f(m - mn);
+    l = l * f + exp2f(sink - mn);
+  }
+  return l == 0.f ? 0.f : f / l;
+}
+
+// Rows behind the last request's.
+template <int HD>
+MSGL_DEVICE void kv8_zero_tail(const Kv8Attn& p, int tid, int threads) {
+  if (!p.zero_tail) return;
+  const int from = min(max(p.cu_q[p.num_reqs], 0), p.total_q);
+  const int64_t per = (int64_t)p.nq * HD / 8, end = p.total_q * per;
+  for (int64_t i = from * per + (int64_t)blockIdx.x * threads + tid; i < end; i += (int64_t)gridDim.x * threads)
+    reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Joins cut segments: grid (ctas, rows / 8), a warp per row.
+template <int R, int HD>
+__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) {
+  pdl_wait();
+  pdl_launch();
+  const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const Kv8Part hd = s.head[c];
+  if (hd.parts == 0 || i >= hd.nr) return;
+  const int G = p.nq / p.nkv, r = hd.r0 + i, head = hd.h * G + r % G;
+  // part 0 ends its CTA's run, the others begin theirs
+  auto row = [&](int part) { return (int64_t)(part == 0 ? 2 * c + 1 : 2 * (c + part)) * R + i; };
+  float m = -INFINITY;
+  for (int j = lane; j < hd.parts; j += 32) m = fmaxf(m, s.ml[row(j)].x);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  constexpr int E = HD / 32;
+  float l = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int j0 = 0; j0 < hd.parts; j0 += 32) {
+    float w = 0.f;
+    if (j0 + lane < hd.parts) {
+      const float2 ml = s.ml[row(j0 + lane)];
+      w = exp2f(ml.x - base);
+      l += w * ml.y;
+    }
+    const int n = min(32, hd.parts - j0);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float* src = s.o + row(j0 + j) * HD + lane * E;
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        acc[0] += wj * x.x, acc[1] += wj * x.y, acc[2] += wj * x.z, acc[3] += wj * x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        acc[0] += wj * x.x, acc[1] += wj * x.y;
+      }
+    }
+  }
+  l = warp_sum(l);
+  const float f = kv8_norm(m, l, p.sinks, head);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.o) + ((int64_t)(hd.q0 + r / G) * p.nq + head) * (HD / 2) + lane * (E / 2);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) dst[e / 2] = pack_bf16(acc[e] * f, acc[e + 1] * f);
+}
+
+}  // namespace msgl

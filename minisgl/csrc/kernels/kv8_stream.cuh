@@ -1,0 +1,448 @@
+// Attention over the 8-bit cache for few rows per request and kv head: decoded tokens, a few drafted ones.
+//
+// What bounds it is the cache's bytes, so the kernel is a stream of them: one CTA per SM, one warp that issues
+// copies of whole pages (codes swizzled by the tensor map, scales as they lie) into a ring of 64-key stages, and two
+// groups of four warps that take the stages in turn, 16 keys a warp. Codes go from shared memory to registers once,
+// 16 bytes a lane, in an order of head dims and keys that fits mma.sync without a transposition:
+//   S = Q K^T  (m16n8k16): lane (g, t) = (lane / 4, lane % 4) holds of key g the head dims [HD/4 t, HD/4 (t + 1)): four
+//     codes are the two registers of one step. The queries' fragments are loaded in the same order of head dims.
+//   O += P V: P's fragments are S's accumulators; lane (g, t) holds of keys 2t, 2t + 1, 2t + 8, 2t + 9 the HD / 8 head dims
+//     from HD/8 g on, and pairs of keys are made by byte permutes. So lane (g, t) ends up with HD / 4 head dims in a row.
+// Codes are exact in fp16, and the queries are, scaled by a power of two. Logits, sums and O are fp32.
+// A warp keeps its own maximum and sum; the eight are joined when a segment ends (see kv8_plan.cuh).
+#pragma once
+#include "kv8.cuh"
+#include "kv8_plan.cuh"
+
+namespace msgl {
+
+constexpr int kKsRows = 16;  // rows of a tile: M of the MMA
+constexpr int kKsWarps = 8;
+constexpr int kKsThreads = 32 * (kKsWarps + 1);
+constexpr int kKsDescs = 4;   // segments looked up ahead
+
+struct KsDesc {
+  int q0, h, r0, nr, row, pos0, pos1, L, n, lo, kend, blk, nb, slot, parts, valid;  // blocks [blk, blk + nb); slot -1: whole
+};
+
+template <int HD>
+struct KsCfg {
+  static constexpr int kTile = kKv8Block * HD;
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kStages = HD == 128 ? 8 : 16;
+  static constexpr int kScales = 2 * kKv8Block * 4;  // of a stage: keys', then values'
+  static constexpr int kMergeQ = HD / 4 + 4, kMergeRow = 4 * kMergeQ;  // floats of a lane's head dims and of a row (no bank conflicts)
+  static constexpr int kMerge = kKsWarps * kKsRows * kMergeRow * 4 + kKsWarps * kKsRows * 8;
+  static constexpr int kSmem = 1024 + kStages * (kStage + kScales) + kMerge + kKsDescs * (int)sizeof(KsDesc) + (int)sizeof(Kv8Plan) +
+                               8 * (kKsThreads / 32) + 8 * (2 * kStages + 2 * kKsDescs) + 16;
+};
+
+// byte of (row, 16-byte chunk) in a tile of HD-byte rows as the tensor map's swizzle lays it out
+template <int HD>
+MSGL_DEVICE uint32_t ks_swz(int row, int chunk) {
+  return HD == 128 ? (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+}
+MSGL_DEVICE uint4 ks_lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+MSGL_DEVICE uint2 ks_lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+MSGL_DEVICE float2 ks_lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+MSGL_DEVICE void ks_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The producer's copies of one 64-key block: the pages that hold keys of [.., kend), slots of which lanes `first`.. hold.
+// Returns after lane 0 has issued them; their bytes complete `bar`.
+template <int HD>
+MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tk, const CUtensorMap* tv, uint8_t* k, uint8_t* v, float* ks,
+                                float* vs, uint64_t* bar, int h, int slots, int first, int pages, int lane) {
+  const int page = p.page;
+  const unsigned lost = __ballot_sync(0xffffffffu, slots < 0) >> first & ((1u << pages) - 1);
+  if (lane == 0) {
+    if (lost) {  // pages that are not there: their codes lie outside the tensor and are filled with zeros, and so are their scales
+      for (int i = 0; i < pages; ++i)
+        if (lost >> i & 1)
+          for (int j = 0; j < page; ++j) ks[i * page + j] = 0.f, vs[i * page + j] = 0.f;
+      fence_async_smem();
+    }
+    mbar_expect_tx(bar, 2 * page * (pages * HD + (pages - __popc(lost)) * 4));
+  }
+  __syncwarp();
+  for (int i = 0; i < pages; ++i) {
+    const int slot = __shfl_sync(0xffffffffu, slots, first + i);
+    if (lane == 0) {
+      const int y = slot < 0 ? p.num_slots : slot;
+      tma_load_3d(k + i * page * HD, tk, bar, 0, y, h);
+      tma_load_3d(v + i * page * HD, tv, bar, 0, y, h);
+      if (slot >= 0) {
+        const int64_t at = (int64_t)h * p.num_slots + slot;
+        bulk_load(ks + i * page, p.sk + at, page * 4, bar);
+        bulk_load(vs + i * page, p.sv + at, page * 4, bar);
+      }
+    }
+  }
+}
+
+template <int HD, bool FP8>
+__global__ void __launch_bounds__(kKsThreads, 1)
+kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, Kv8Attn p, Kv8Scratch scratch) {
+  using C = KsCfg<HD>;
+  constexpr int NK = HD / 16;  // steps of Q K^T, and (twice as many) n-tiles of O
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  float* scales = reinterpret_cast<float*>(ring + C::kStages * C::kStage);
+  float* merge = scales + C::kStages * (C::kScales / 4);                       // [8][16][kMergeRow]
+  float2* merge_ml = reinterpret_cast<float2*>(merge + kKsWarps * kKsRows * C::kMergeRow);  // [8][16]
+  KsDesc* descs = reinterpret_cast<KsDesc*>(merge_ml + kKsWarps * kKsRows);
+  Kv8Plan* plan = reinterpret_cast<Kv8Plan*>(descs + kKsDescs);
+  int64_t* red = reinterpret_cast<int64_t*>(plan + 1);
+  uint64_t* full = reinterpret_cast<uint64_t*>(red + kKsThreads / 32);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* dfull = empty + C::kStages;
+  uint64_t* dempty = dfull + kKsDescs;
+  volatile int* abort_flag = reinterpret_cast<int*>(dempty + kKsDescs);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kKsWarps / 2);
+    }
+    for (int i = 0; i < kKsDescs; ++i) {
+      mbar_init(&dfull[i], 1);
+      mbar_init(&dempty[i], kKsWarps);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  pdl_wait();
+  pdl_launch();
+  if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
+  kv8_plan<kKsRows, kKsThreads>(p, 2, plan, red);  // (its barriers order the initialisation above as well)
+  const Kv8Plan pl = *plan;
+  const int G = p.nq / p.nkv;
+  kv8_zero_tail<HD>(p, threadIdx.x, kKsThreads);
+
+  if (warp == kKsWarps) {
+    // ------------------------------------------------------------------ segments and copies
+    const int gpb = kKv8Block / p.page, per_batch = 32 / gpb;  // pages of a block, blocks of a batch of slots
+    int b = pl.b, h = pl.h, t = pl.t, stage = 0, tiles = 0;
+    uint32_t phase = 0;
+    int64_t u = pl.u0, s0 = pl.s0;
+    bool ok = true;
+    Kv8Req r;
+    if (u < pl.u1) {
+      r = kv8_request(p, b);
+      tiles = kv8_tiles<kKsRows>(r, G);
+    }
+    for (int i = 0; ok; ++i) {
+      const int d = i % kKsDescs;
+      if (lane == 0) ok = mbar_wait(&dempty[d], ((i / kKsDescs) & 1) ^ 1, 700);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      if (u >= pl.u1) {
+        if (lane == 0) {
+          descs[d].valid = 0;
+          mbar_arrive(&dfull[d]);
+        }
+        break;
+      }
+      const Kv8Tile k = kv8_tile<kKsRows>(p, r, G, t);
+      const int from = (int)(u - s0), to = (int)min((int64_t)k.nblk, pl.u1 - s0);
+      const bool starts = from == 0, ends = to == k.nblk;
+      if (lane == 0) {
+        KsDesc& D = descs[d];
+        D.q0 = r.q0; D.h = h; D.r0 = k.r0; D.nr = k.nr; D.row = r.row; D.pos0 = k.pos0; D.pos1 = k.pos1; D.L = r.L; D.n = r.n;
+        D.lo = k.lo; D.kend = k.kend; D.blk = k.blk0 + from; D.nb = to - from; D.valid = 1;
+        D.slot = starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
+        D.parts = starts && !ends ? kv8_cta_of(pl, s0 + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
+        if (u + (to - from) >= pl.u1) {  // the run's last segment: what there is to join
+          Kv8Part& hd = scratch.head[blockIdx.x];
+          hd.parts = D.parts; hd.q0 = r.q0; hd.r0 = k.r0; hd.nr = k.nr; hd.h = h;
+        }
+        mbar_arrive(&dfull[d]);
+      }
+      // the blocks' pages, looked up 32 at a time and one batch ahead
+      const int page0 = (k.blk0 + from) * gpb, pages_end = k.kend > k.lo ? (k.kend - 1) / p.page + 1 : 0;
+      auto look_up = [&](int batch) {
+        const int g = page0 + batch * 32 + lane;
+        return g < pages_end && g < (k.blk0 + to) * gpb ? kv8_page(p, r.row, g * p.page) : -1;
+      };
+      int slots = look_up(0), next = -1;
+      for (int j = 0; j < to - from; ++j) {
+        const int at = j % per_batch;
+        if (at == 0) {
+          if (j > 0) slots = next;
+          if (j + per_batch < to - from) next = look_up(j / per_batch + 1);
+        }
+        if (lane == 0) ok = mbar_wait(&empty[stage], phase ^ 1, 701);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
+        uint8_t* st = ring + stage * C::kStage;
+        float* sc = scales + stage * (C::kScales / 4);
+        kv8_copy_block<HD>(p, &tk, &tv, st, st + C::kTile, sc, sc + kKv8Block, &full[stage], h, slots, at * gpb, pages, lane);
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+      }
+      // the next segment
+      u = s0 + to;
+      s0 += k.nblk;
+      if (u < pl.u1 && ++t == tiles) {
+        t = 0;
+        if (++h == p.nkv) {
+          h = 0;
+          do {
+            if (++b >= p.num_reqs) break;  // (never: units are left)
+            r = kv8_request(p, b);
+            tiles = kv8_tiles<kKsRows>(r, G);
+          } while (tiles == 0);
+          if (b >= p.num_reqs) u = pl.u1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // given up (and recorded): the copies in flight land before the CTA's memory goes
+      for (int i = 0; i < C::kStages; ++i) {
+        mbar_wait(&full[stage], phase ^ 1, 702);
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------------- products
+  const int g = lane >> 2, t = lane & 3, group = warp >> 2, key0 = (warp & 3) * 16;
+  const int ctid = threadIdx.x;
+  uint32_t seq = 0;  // stages gone through; this warp takes those of its group's parity
+  bool dead = false;
+  for (int i = 0;; ++i) {
+    const int d = i % kKsDescs;
+    if (!dead && !mbar_wait(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
+    if (!dead && !descs[d].valid) {
+      named_bar_sync(1, kKsWarps * 32);  // (pairs with the barrier below of a warp that has given up)
+      break;
+    }
+    const KsDesc D = descs[d];
+    __syncwarp();
+    if (!dead && lane == 0) mbar_arrive(&dempty[d]);
+
+    // queries: rows g and g + 8 in fragments, brought to fp16's range by a power of two each
+    uint32_t qf[NK][4];
+    float qs[2];
+    int qpos[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int rr = g + 8 * x, r = D.r0 + rr, tok = r / G;
+      const bool in = !dead && rr < D.nr;
+      uint4 u[HD / 32];
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) u[j] = make_uint4(0, 0, 0, 0);
+      if (in) {
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(p.q) + (D.q0 + tok) * p.q_row +
+                                   (int64_t)(D.h * G + r - tok * G) * p.q_head + t * (HD / 4);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      }
+      qpos[x] = in ? D.L - D.n + tok : -1;
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j)
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(u[j].x & 0x7fff7fffu, u[j].y & 0x7fff7fffu), __vmaxu2(u[j].z & 0x7fff7fffu, u[j].w & 0x7fff7fffu)));
+      m = max(m & 0xffffu, m >> 16);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const float f = kv8_q_factor(__uint_as_float(m << 16));
+      qs[x] = p.scale * kKv8Log2e * kv8_reciprocal(f);
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) {
+        const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // dims 8 j + 2 e and the next: step 2 j + e / 2
+          qf[2 * j + (e >> 1)][x + 2 * (e & 1)] = pack_half(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
+      }
+    }
+
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[2 * NK][4];
+#pragma unroll
+    for (int j = 0; j < 2 * NK; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+    for (int j = (int)((seq ^ group) & 1); j < D.nb && !dead; j += 2) {
+      const uint32_t at = seq + j, stage = at % C::kStages;
+      if (!mbar_wait(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
+      const uint32_t sk = smem_u32(ring + stage * C::kStage), sv = sk + C::kTile;
+      const uint32_t ssc = smem_u32(scales + stage * (C::kScales / 4)) + (key0 + 2 * t) * 4;
+      // S: keys key0 + 8 n + g
+      float s[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        uint32_t w[NK];
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+          const uint4 v = ks_lds128(sk + ks_swz<HD>(key0 + 8 * n + g, t * (HD / 64) + c));
+          w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          uint32_t b0, b1;
+          kv8_to_half<FP8>(w[kk], b0, b1);
+          ks_mma(s[n], qf[kk], b0, b1);
+        }
+      }
+      const float2 ks0 = ks_lds_f2(ssc), ks1 = ks_lds_f2(ssc + 32), vs0 = ks_lds_f2(ssc + 256), vs1 = ks_lds_f2(ssc + 288);
+      const float ksc[4] = {ks0.x, ks0.y, ks1.x, ks1.y};
+      float vsc[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
+      const int k0 = (D.blk + j) * kKv8Block + key0;
+      const bool inside = k0 + 16 <= D.pos0 + 1 && (p.window <= 0 || k0 >= D.pos1 - p.window + 1);  // every row sees all 16
+      uint32_t vw[4][NK / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 2 * t + (e & 1) + 8 * (e >> 1);
+        if constexpr (HD == 128) {
+          const uint4 v = ks_lds128(sv + ks_swz<HD>(key, g));
+          vw[e][0] = v.x; vw[e][1] = v.y; vw[e][2] = v.z; vw[e][3] = v.w;
+        } else {
+          const uint2 v = ks_lds64(sv + ks_swz<HD>(key, g >> 1) + (g & 1) * 8);
+          vw[e][0] = v.x; vw[e][1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= ksc[2 * n + (e & 1)] * qs[e >> 1];
+      if (!inside) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int kp = k0 + 8 * n + 2 * t + e;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const bool seen = kp <= qpos[x] && (p.window <= 0 || kp > qpos[x] - p.window);
+              s[n][2 * x + e] = seen ? s[n][2 * x + e] : -INFINITY;
+            }
+            // a key that no row of the tile sees may be no position at all: its codes and scale can be anything
+            if (kp < D.lo || kp >= D.kend) {
+              vsc[2 * n + e] = 0.f;
+#pragma unroll
+              for (int c = 0; c < NK / 2; ++c) vw[2 * n + e][c] = 0u;
+            }
+          }
+      }
+      float lv[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lv[e] = kv8_log_scale(vsc[e]);
+      float f[2];
+      uint32_t pf[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float mx = fmaxf(fmaxf(s[0][2 * x] + lv[0], s[0][2 * x + 1] + lv[1]), fmaxf(s[1][2 * x] + lv[2], s[1][2 * x + 1] + lv[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = fmaxf(mx - kKv8Top, m[x]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        f[x] = kv8_exp2(m[x] - base);
+        m[x] = mx;
+        float e[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) e[y] = kv8_exp2(s[y >> 1][2 * x + (y & 1)] - base);
+        l[x] = l[x] * f[x] + ((e[0] + e[1]) + (e[2] + e[3]));  // (of this lane's keys; joined over t at the end)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)  // (a hidden key's weight is zero whatever its scale)
+          e[y] = s[y >> 1][2 * x + (y & 1)] == -INFINITY ? 0.f : e[y] * vsc[y];
+        pf[x] = pack_half(e[0], e[1]);
+        pf[2 + x] = pack_half(e[2], e[3]);
+      }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < 2 * NK; ++n) {
+          o[n][0] *= f[0]; o[n][1] *= f[0]; o[n][2] *= f[1]; o[n][3] *= f[1];
+        }
+      }
+      // O: n-tile n holds head dim HD/8 g + n of every g
+#pragma unroll
+      for (int c = 0; c < NK / 2; ++c) {
+        uint32_t b[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t lo = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x5140), hi = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x7362);
+          kv8_to_half<FP8>(lo, b[x][0], b[x][1]);
+          kv8_to_half<FP8>(hi, b[x][2], b[x][3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ks_mma(o[4 * c + e], pf, b[0][e], b[1][e]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+    seq += D.nb;
+
+    // join the eight warps
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      const int rr = g + 8 * x;
+      if (rr < D.nr) {
+        if (t == 0) merge_ml[warp * kKsRows + rr] = make_float2(m[x], l[x]);
+        float* dst = merge + (warp * kKsRows + rr) * C::kMergeRow + t * C::kMergeQ;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)  // n-tile j, columns 2 t and 2 t + 1: head dims HD/4 t + j and HD/4 t + HD/8 + j
+#pragma unroll
+          for (int j = 0; j < HD / 8; j += 4)
+            *reinterpret_cast<float4*>(dst + n * (HD / 8) + j) = make_float4(o[j][2 * x + n], o[j + 1][2 * x + n], o[j + 2][2 * x + n], o[j + 3][2 * x + n]);
+      }
+    }
+    named_bar_sync(1, kKsWarps * 32);
+    if (*abort_flag) break;
+    for (int idx = ctid; idx < D.nr * (HD / 4); idx += kKsWarps * 32) {
+      const int rr = idx / (HD / 4), c4 = idx % (HD / 4);
+      float mx = -INFINITY;
+      float2 ml[kKsWarps];
+#pragma unroll
+      for (int w = 0; w < kKsWarps; ++w) {
+        ml[w] = merge_ml[w * kKsRows + rr];
+        mx = fmaxf(mx, ml[w].x);
+      }
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float ll = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kKsWarps; ++w) {
+        const float fw = kv8_exp2(ml[w].x - base);
+        ll += fw * ml[w].y;
+        const float4 v = *reinterpret_cast<const float4*>(merge + (w * kKsRows + rr) * C::kMergeRow + c4 / (HD / 16) * C::kMergeQ + c4 % (HD / 16) * 4);
+        acc.x += fw * v.x; acc.y += fw * v.y; acc.z += fw * v.z; acc.w += fw * v.w;
+      }
+      if (D.slot < 0) {
+        const int r = D.r0 + rr, tok = r / G, head = D.h * G + r - tok * G;
+        const float f = kv8_norm(mx, ll, p.sinks, head);
+        reinterpret_cast<uint2*>(p.o)[((int64_t)(D.q0 + tok) * p.nq + head) * (HD / 4) + c4] =
+            make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+      } else {
+        const int64_t row = (int64_t)D.slot * kKsRows + rr;
+        reinterpret_cast<float4*>(scratch.o)[row * (HD / 4) + c4] = acc;
+        if (c4 == 0) scratch.ml[row] = make_float2(mx, ll);
+      }
+    }
+    named_bar_sync(1, kKsWarps * 32);  // the merge scratch is free
+  }
+}
+
+}  // namespace msgl
