@@ -7,6 +7,31 @@
 
 namespace msgl {
 
+MSGL_DEVICE void kv8_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// mbar_wait for waits that a stream of data goes through: the clock, which takes long to read, is looked at now and then only.
+MSGL_DEVICE bool kv8_wait(uint64_t* bar, uint32_t parity, int where) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 0) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitTimeoutNs) {
+        report_error(kErrMbarTimeout, where);
+        return false;
+      }
+    }
+  }
+}
+
 // two values to two e4m3 codes, nearest, ties to even (the first one in the low byte)
 MSGL_DEVICE uint16_t kv8_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);

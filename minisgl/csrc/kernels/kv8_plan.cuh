@@ -37,9 +37,8 @@ MSGL_DEVICE Kv8Req kv8_request(const Kv8Attn& p, int b) {
   return r;
 }
 
-// First slot of the page that holds position `pos` (a multiple of the page), or -1.
-MSGL_DEVICE int kv8_page(const Kv8Attn& p, int row, int pos) {
-  const int slot = p.page_table[(int64_t)row * p.pt_stride + pos];
+// A page's first slot as the table has it, or -1 if there is no such page (recorded).
+MSGL_DEVICE int kv8_checked(const Kv8Attn& p, int slot) {
   if (slot < 0 || slot > p.num_slots - p.page || slot % p.page != 0) {
     report_error(kErrBounds, kBcAttnSlot);
     return -1;

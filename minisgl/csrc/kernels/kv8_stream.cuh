@@ -17,8 +17,9 @@
 namespace msgl {
 
 constexpr int kKsRows = 16;  // rows of a tile: M of the MMA
-constexpr int kKsWarps = 8;
-constexpr int kKsThreads = 32 * (kKsWarps + 1);
+constexpr int kKsWarps = 8;   // of products
+constexpr int kKsCopies = 4;  // warps that issue copies
+constexpr int kKsThreads = 32 * (kKsWarps + kKsCopies);
 constexpr int kKsDescs = 4;   // segments looked up ahead
 
 struct KsDesc {
@@ -64,41 +65,34 @@ MSGL_DEVICE void ks_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The producer's copies of one 64-key block: the pages that hold keys of [.., kend), slots of which lanes `first`.. hold.
-// Returns after lane 0 has issued them; their bytes complete `bar`.
+// Which of a page's two parts holds the keys' (0 or 1): the tensor maps' base is the lower of the two addresses.
+struct Kv8Order {
+  int codes, scales;
+};
+
+// The copies of one 64-key block, a page at a time: its keys' and values' codes with one instruction, its scales with
+// another (an instruction costs the warp some 100 cycles, whatever it copies). Lanes first .. first + pages - 1 hold the pages'
+// slots, -1 for a page that is not there: what lies outside the tensors is filled with zeros. A page's keys are
+// beside its values, codes and scales alike.
 template <int HD>
-MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tk, const CUtensorMap* tv, uint8_t* k, uint8_t* v, float* ks,
-                                float* vs, uint64_t* bar, int h, int slots, int first, int pages, int lane) {
+MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tc, const CUtensorMap* ts, uint8_t* codes, float* scales, uint64_t* bar,
+                                int h, int slots, int first, int pages, int lane) {
   const int page = p.page;
-  const unsigned lost = __ballot_sync(0xffffffffu, slots < 0) >> first & ((1u << pages) - 1);
-  if (lane == 0) {
-    if (lost) {  // pages that are not there: their codes lie outside the tensor and are filled with zeros, and so are their scales
-      for (int i = 0; i < pages; ++i)
-        if (lost >> i & 1)
-          for (int j = 0; j < page; ++j) ks[i * page + j] = 0.f, vs[i * page + j] = 0.f;
-      fence_async_smem();
-    }
-    mbar_expect_tx(bar, 2 * page * (pages * HD + (pages - __popc(lost)) * 4));
-  }
+  if (lane == 0) mbar_expect_tx(bar, 2 * page * pages * (HD + 4));
   __syncwarp();
   for (int i = 0; i < pages; ++i) {
-    const int slot = __shfl_sync(0xffffffffu, slots, first + i);
+    int slot = __shfl_sync(0xffffffffu, slots, first + i);
     if (lane == 0) {
-      const int y = slot < 0 ? p.num_slots : slot;
-      tma_load_3d(k + i * page * HD, tk, bar, 0, y, h);
-      tma_load_3d(v + i * page * HD, tv, bar, 0, y, h);
-      if (slot >= 0) {
-        const int64_t at = (int64_t)h * p.num_slots + slot;
-        bulk_load(ks + i * page, p.sk + at, page * 4, bar);
-        bulk_load(vs + i * page, p.sv + at, page * 4, bar);
-      }
+      if (slot < 0) slot = p.num_slots;
+      kv8_load_4d(codes + 2 * i * page * HD, tc, bar, 0, slot, h, 0);
+      tma_load_3d(scales + 2 * i * page, ts, bar, slot, h, 0);
     }
   }
 }
 
 template <int HD, bool FP8>
 __global__ void __launch_bounds__(kKsThreads, 1)
-kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, Kv8Attn p, Kv8Scratch scratch) {
+kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
   using C = KsCfg<HD>;
   constexpr int NK = HD / 16;  // steps of Q K^T, and (twice as many) n-tiles of O
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -128,8 +122,8 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     *abort_flag = 0;
     fence_barrier_init();
-    prefetch_tmap(&tk);
-    prefetch_tmap(&tv);
+    prefetch_tmap(&tc);
+    prefetch_tmap(&ts);
   }
   pdl_wait();
   pdl_launch();
@@ -139,11 +133,13 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   const int G = p.nq / p.nkv;
   kv8_zero_tail<HD>(p, threadIdx.x, kKsThreads);
 
-  if (warp == kKsWarps) {
+  if (warp >= kKsWarps) {
     // ------------------------------------------------------------------ segments and copies
-    const int gpb = kKv8Block / p.page, per_batch = 32 / gpb;  // pages of a block, blocks of a batch of slots
-    int b = pl.b, h = pl.h, t = pl.t, stage = 0, tiles = 0;
-    uint32_t phase = 0;
+    // Every copying warp goes through the run's segments and takes every fourth block; the first one publishes them.
+    const int me = warp - kKsWarps;
+    const int page = p.page, gpb = kKv8Block / page, mine = 32 / gpb;  // pages of a block, blocks whose slots the lanes hold
+    int b = pl.b, h = pl.h, t = pl.t, tiles = 0;
+    uint32_t seq = 0;
     int64_t u = pl.u0, s0 = pl.s0;
     bool ok = true;
     Kv8Req r;
@@ -151,55 +147,60 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       r = kv8_request(p, b);
       tiles = kv8_tiles<kKsRows>(r, G);
     }
-    for (int i = 0; ok; ++i) {
-      const int d = i % kKsDescs;
-      if (lane == 0) ok = mbar_wait(&dempty[d], ((i / kKsDescs) & 1) ^ 1, 700);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
-      if (u >= pl.u1) {
-        if (lane == 0) {
-          descs[d].valid = 0;
-          mbar_arrive(&dfull[d]);
-        }
-        break;
-      }
+    int i = 0, issued = 0;
+    uint32_t last = 0;
+    for (; ok && u < pl.u1; ++i) {
       const Kv8Tile k = kv8_tile<kKsRows>(p, r, G, t);
       const int from = (int)(u - s0), to = (int)min((int64_t)k.nblk, pl.u1 - s0);
-      const bool starts = from == 0, ends = to == k.nblk;
-      if (lane == 0) {
-        KsDesc& D = descs[d];
-        D.q0 = r.q0; D.h = h; D.r0 = k.r0; D.nr = k.nr; D.row = r.row; D.pos0 = k.pos0; D.pos1 = k.pos1; D.L = r.L; D.n = r.n;
-        D.lo = k.lo; D.kend = k.kend; D.blk = k.blk0 + from; D.nb = to - from; D.valid = 1;
-        D.slot = starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
-        D.parts = starts && !ends ? kv8_cta_of(pl, s0 + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
-        if (u + (to - from) >= pl.u1) {  // the run's last segment: what there is to join
-          Kv8Part& hd = scratch.head[blockIdx.x];
-          hd.parts = D.parts; hd.q0 = r.q0; hd.r0 = k.r0; hd.nr = k.nr; hd.h = h;
+      if (me == 0) {
+        const int d = i % kKsDescs;
+        if (lane == 0) {
+          ok = kv8_wait(&dempty[d], ((i / kKsDescs) & 1) ^ 1, 700);
+          if (ok) {
+            const bool starts = from == 0, ends = to == k.nblk;
+            KsDesc& D = descs[d];
+            D.q0 = r.q0; D.h = h; D.r0 = k.r0; D.nr = k.nr; D.row = r.row; D.pos0 = k.pos0; D.pos1 = k.pos1; D.L = r.L; D.n = r.n;
+            D.lo = k.lo; D.kend = k.kend; D.blk = k.blk0 + from; D.nb = to - from; D.valid = 1;
+            D.slot = starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
+            const int parts = starts && !ends ? kv8_cta_of(pl, s0 + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
+            if (parts > 0) {  // (the run's last segment)
+              Kv8Part& hd = scratch.head[blockIdx.x];
+              hd.q0 = r.q0; hd.r0 = k.r0; hd.nr = k.nr; hd.h = h; hd.parts = parts;
+            }
+            mbar_arrive(&dfull[d]);
+          }
         }
-        mbar_arrive(&dfull[d]);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
       }
-      // the blocks' pages, looked up 32 at a time and one batch ahead
-      const int page0 = (k.blk0 + from) * gpb, pages_end = k.kend > k.lo ? (k.kend - 1) / p.page + 1 : 0;
-      auto look_up = [&](int batch) {
-        const int g = page0 + batch * 32 + lane;
-        return g < pages_end && g < (k.blk0 + to) * gpb ? kv8_page(p, r.row, g * p.page) : -1;
+      // This warp's blocks j = j0, j0 + 4, ..: their pages' slots, a batch of `mine` blocks ahead. Looked up in one go, looked over
+      // when their turn comes, so that the loads' latency is not waited for.
+      const int page0 = (k.blk0 + from) * gpb, pages_end = k.kend > k.lo ? (k.kend - 1) / page + 1 : 0;
+      const int j0 = (int)((me - seq) & (kKsCopies - 1));
+      auto look_up = [&](int j) {
+        const int g = page0 + (j + lane / gpb * kKsCopies) * gpb + lane % gpb;
+        return g < pages_end && j + lane / gpb * kKsCopies < to - from ? p.page_table[(int64_t)r.row * p.pt_stride + (int64_t)g * page] : -1;
       };
-      int slots = look_up(0), next = -1;
-      for (int j = 0; j < to - from; ++j) {
-        const int at = j % per_batch;
-        if (at == 0) {
-          if (j > 0) slots = next;
-          if (j + per_batch < to - from) next = look_up(j / per_batch + 1);
+      int next = look_up(j0), slots = -1;
+      for (int j = j0, at = 0; j < to - from; j += kKsCopies, ++at) {
+        if (at % mine == 0) {
+          slots = next;
+          const int g = page0 + (j + lane / gpb * kKsCopies) * gpb + lane % gpb;
+          if (g < pages_end && j + lane / gpb * kKsCopies < to - from) slots = kv8_checked(p, slots);
+          if (j + mine * kKsCopies < to - from) next = look_up(j + mine * kKsCopies);
         }
-        if (lane == 0) ok = mbar_wait(&empty[stage], phase ^ 1, 701);
+        const uint32_t x = seq + j, stage = x % C::kStages;
+        if (lane == 0) ok = kv8_wait(&empty[stage], ((x / C::kStages) & 1) ^ 1, 701);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
-        uint8_t* st = ring + stage * C::kStage;
-        float* sc = scales + stage * (C::kScales / 4);
-        kv8_copy_block<HD>(p, &tk, &tv, st, st + C::kTile, sc, sc + kKv8Block, &full[stage], h, slots, at * gpb, pages, lane);
-        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+        kv8_copy_block<HD>(p, &tc, &ts, ring + stage * C::kStage, scales + stage * (C::kScales / 4), &full[stage], h, slots,
+                           at % mine * gpb, pages, lane);
+        last = x;
+        ++issued;
       }
+      if (!ok) break;
+      seq += to - from;
       // the next segment
       u = s0 + to;
       s0 += k.nblk;
@@ -216,10 +217,15 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
       }
     }
-    if (!ok && lane == 0) {  // given up (and recorded): the copies in flight land before the CTA's memory goes
-      for (int i = 0; i < C::kStages; ++i) {
-        mbar_wait(&full[stage], phase ^ 1, 702);
-        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+    if (ok) {
+      if (me == 0 && lane == 0 && kv8_wait(&dempty[i % kKsDescs], ((i / kKsDescs) & 1) ^ 1, 702)) {
+        descs[i % kKsDescs].valid = 0;
+        mbar_arrive(&dfull[i % kKsDescs]);
+      }
+    } else if (lane == 0) {  // given up (and recorded): this warp's copies in flight land before the CTA's memory goes
+      for (int n = 0; n < min(issued, C::kStages / kKsCopies); ++n) {
+        const uint32_t x = last - n * kKsCopies;
+        kv8_wait(&full[x % C::kStages], (x / C::kStages) & 1, 703);
       }
     }
     return;
@@ -228,11 +234,15 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   // -------------------------------------------------------------------- products
   const int g = lane >> 2, t = lane & 3, group = warp >> 2, key0 = (warp & 3) * 16;
   const int ctid = threadIdx.x;
+  // this warp's keys lie in one page: [keys' page][values' page] each
+  const int base = key0 + (key0 & ~(p.page - 1));
+  const uint32_t k_at = (uint32_t)(base + order.codes * p.page) * HD, v_at = (uint32_t)(base + (order.codes ^ 1) * p.page) * HD;
+  const uint32_t ks_at = (uint32_t)(base + order.scales * p.page + 2 * t) * 4, vs_at = (uint32_t)(base + (order.scales ^ 1) * p.page + 2 * t) * 4;
   uint32_t seq = 0;  // stages gone through; this warp takes those of its group's parity
   bool dead = false;
   for (int i = 0;; ++i) {
     const int d = i % kKsDescs;
-    if (!dead && !mbar_wait(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
+    if (!dead && !kv8_wait(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
     if (!dead && !descs[d].valid) {
       named_bar_sync(1, kKsWarps * 32);  // (pairs with the barrier below of a warp that has given up)
       break;
@@ -284,9 +294,9 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
     for (int j = (int)((seq ^ group) & 1); j < D.nb && !dead; j += 2) {
       const uint32_t at = seq + j, stage = at % C::kStages;
-      if (!mbar_wait(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
-      const uint32_t sk = smem_u32(ring + stage * C::kStage), sv = sk + C::kTile;
-      const uint32_t ssc = smem_u32(scales + stage * (C::kScales / 4)) + (key0 + 2 * t) * 4;
+      if (!kv8_wait(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
+      const uint32_t st = smem_u32(ring + stage * C::kStage), sk = st + k_at, sv = st + v_at;
+      const uint32_t ssc = smem_u32(scales + stage * (C::kScales / 4));
       // S: keys key0 + 8 n + g
       float s[2][4];
 #pragma unroll
@@ -295,7 +305,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         uint32_t w[NK];
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c) {
-          const uint4 v = ks_lds128(sk + ks_swz<HD>(key0 + 8 * n + g, t * (HD / 64) + c));
+          const uint4 v = ks_lds128(sk + ks_swz<HD>(8 * n + g, t * (HD / 64) + c));
           w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
         }
 #pragma unroll
@@ -305,7 +315,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           ks_mma(s[n], qf[kk], b0, b1);
         }
       }
-      const float2 ks0 = ks_lds_f2(ssc), ks1 = ks_lds_f2(ssc + 32), vs0 = ks_lds_f2(ssc + 256), vs1 = ks_lds_f2(ssc + 288);
+      const float2 ks0 = ks_lds_f2(ssc + ks_at), ks1 = ks_lds_f2(ssc + ks_at + 32), vs0 = ks_lds_f2(ssc + vs_at), vs1 = ks_lds_f2(ssc + vs_at + 32);
       const float ksc[4] = {ks0.x, ks0.y, ks1.x, ks1.y};
       float vsc[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
       const int k0 = (D.blk + j) * kKv8Block + key0;
@@ -313,7 +323,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       uint32_t vw[4][NK / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = key0 + 2 * t + (e & 1) + 8 * (e >> 1);
+        const int key = 2 * t + (e & 1) + 8 * (e >> 1);
         if constexpr (HD == 128) {
           const uint4 v = ks_lds128(sv + ks_swz<HD>(key, g));
           vw[e][0] = v.x; vw[e][1] = v.y; vw[e][2] = v.z; vw[e][3] = v.w;
