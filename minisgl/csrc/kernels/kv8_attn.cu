@@ -58,15 +58,15 @@ template <int HD, bool FP8>
 int stream_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
   using C = KsCfg<HD>;
   constexpr auto kernel = kv8_stream_kernel<HD, FP8>;
-  if (msgl_set_smem<kernel>(C::kSmem) != cudaSuccess) return 4;
+  if (msgl_set_smem<kernel>(C::kSmem, 100) != cudaSuccess) return 4;
   CUtensorMap tc, ts;
   Kv8Order order;
   if (!encode_cache(&tc, &ts, &order, p, HD)) return 2;
-  const int ctas = sm_count();
+  const int ctas = 2 * sm_count();
   const Kv8Scratch scratch = kv8_scratch<kKsRows, HD>(ws, ctas);
   if (msgl_launch(kernel, dim3(ctas), dim3(kKsThreads), C::kSmem, s, 1, tc, ts, p, order, scratch) != cudaSuccess) return 4;
   ++*launches;
-  if (msgl_launch(kv8_join_kernel<kKsRows, HD>, dim3(ctas, kKsRows / 8), dim3(256), 0, s, 1, p, scratch) != cudaSuccess) return 4;
+  if (msgl_launch(kv8_join_kernel<kKsRows, HD>, dim3(ctas, kKsRows / 4), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
   ++*launches;
   return 0;
 }
@@ -75,7 +75,8 @@ int stream_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
 
 extern "C" int64_t msgl_kv8_attention_workspace(const Kv8Attn* p, int hd, int max_q_len) {
   (void)p, (void)max_q_len;
-  return hd == 128 ? kv8_scratch_bytes<kKsRows, 128>(sm_count()) : kv8_scratch_bytes<kKsRows, 64>(sm_count());
+  const int ctas = 2 * sm_count();
+  return hd == 128 ? kv8_scratch_bytes<kKsRows, 128>(ctas) : kv8_scratch_bytes<kKsRows, 64>(ctas);
 }
 
 extern "C" int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, void* ws, int* launches, cudaStream_t s) {

@@ -2,13 +2,13 @@
 //
 // The rows of a request and kv head are its (token, head of the group) pairs, packed: row r is token r / G, head r % G,
 // so a key read once serves the whole group. A segment is a tile of R rows and the 64-key blocks that any of them
-// sees (at least one, empty or not). All segments' blocks, request by request, head by head, tile by tile, form one row
-// of units that is cut into P equal runs, one per CTA: lengths of any mixture balance without a work list from
-// the host, and a graph replays with new ones. A CTA finds its run by a scan over the requests (some 2 us). Whole
-// segments are written out at once; a run has at most one part of a segment at its start and one at its end, so there
-// are 2 P slots for parts whatever the lengths, and a second kernel joins each cut segment from its first part's header.
-// That kernel costs about 2 us; counters that let the last part's CTA do it would have to be zeroed by a launch
-// as well, or shared between calls.
+// sees (at least one, empty or not). It counts as its blocks plus COST units, what starting and ending it takes. All
+// segments' units, request by request, head by head, tile by tile, form one row that is cut into P equal runs, one per
+// CTA: lengths of any mixture balance without a work list from the host, and a graph replays with new ones. A CTA
+// finds its run by a scan over the requests. Whole segments are written out at once; a run has at most one part of a
+// segment at its start and one at its end, so there are 2 P slots for parts whatever the lengths, and a second kernel
+// joins each cut segment from its first part's header. (Counters that let the last part's CTA do that would have to be
+// zeroed by a launch as well, or shared between calls.)
 #pragma once
 #include "api.h"
 #include "common.cuh"
@@ -73,24 +73,29 @@ MSGL_DEVICE int kv8_tiles(const Kv8Req& r, int G) {
 struct Kv8Plan {
   int64_t total, u0, u1, s0;
   int ctas, b, h, t;
+  Kv8Req r;
 };
 // the CTA whose run holds unit u: runs are [total c / P, total (c + 1) / P)
-MSGL_DEVICE int kv8_cta_of(const Kv8Plan& pl, int64_t u) { return (int)(((u + 1) * pl.ctas - 1) / pl.total); }
+MSGL_DEVICE int kv8_cta_of(const Kv8Plan& pl, int64_t u) {
+  if (pl.total < (1 << 20)) return (int)(((uint32_t)(u + 1) * pl.ctas - 1) / (uint32_t)pl.total);  // (64-bit divisions are long)
+  return (int)(((u + 1) * pl.ctas - 1) / pl.total);
+}
 
 // All NT threads of the CTA; `red` holds NT / 32 words. A run has at least `least` units.
-template <int R, int NT>
+template <int R, int COST, int NT>
 MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.nq / p.nkv;
   const int rounds = (p.num_reqs + NT - 1) / NT;
   int64_t base = 0, v = 0, excl = 0, run0 = 0, run1 = 0;
+  Kv8Req r;
   // one round over the requests, NT at a time: v the units of request (round, tid), excl those before it
   auto scan = [&](int c) {
     const int b = c * NT + tid;
     v = 0;
     if (b < p.num_reqs) {
-      const Kv8Req r = kv8_request(p, b);
+      r = kv8_request(p, b);
       const int tiles = kv8_tiles<R>(r, G);
-      for (int t = 0; t < tiles; ++t) v += kv8_tile<R>(p, r, G, t).nblk;
+      for (int t = 0; t < tiles; ++t) v += kv8_tile<R>(p, r, G, t).nblk + COST;
       v *= p.nkv;
     }
     int64_t incl = v;
@@ -99,7 +104,7 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
       const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
     }
-    __syncthreads();
+    if (c > 0) __syncthreads();
     if (lane == 31) red[warp] = incl;
     __syncthreads();
     int64_t before = 0, all = 0;
@@ -113,30 +118,32 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
   };
   auto place = [&](int c) {
     if (run0 < excl || run0 >= excl + v || run0 >= run1) return;
-    const int b = c * NT + tid;
-    const Kv8Req r = kv8_request(p, b);
     const int64_t per = v / p.nkv;
     int64_t rem = run0 - excl;
-    pl->b = b;
-    pl->h = (int)(rem / per);
-    rem -= pl->h * per;
+    pl->b = c * NT + tid;
+    pl->r = r;
+    const int h = v <= UINT32_MAX ? (int)((uint32_t)rem / (uint32_t)per) : (int)(rem / per);
+    pl->h = h;
+    rem -= h * per;
     for (int t = 0;; ++t) {
-      const int nblk = kv8_tile<R>(p, r, G, t).nblk;
-      if (rem < nblk) {
+      const int units = kv8_tile<R>(p, r, G, t).nblk + COST;
+      if (rem < units) {
         pl->t = t;
         break;
       }
-      rem -= nblk;
+      rem -= units;
     }
     pl->s0 = run0 - rem;
   };
   for (int c = 0; c < rounds; ++c) scan(c);
   const int64_t total = base;
-  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, total / least));
+  int ctas = gridDim.x;
+  if (total < (int64_t)ctas * least) ctas = max(1, (int)total / least);
   const int c = blockIdx.x;
   if (c < ctas) {
-    run0 = total * c / ctas;
-    run1 = total * (c + 1) / ctas;
+    const bool small = total < (1 << 20);
+    run0 = small ? (uint32_t)total * c / ctas : total * c / ctas;
+    run1 = small ? (uint32_t)total * (c + 1) / ctas : total * (c + 1) / ctas;
   }
   if (tid == 0) {
     pl->total = total;
@@ -148,6 +155,7 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
     place(0);
   } else {
     base = 0;
+    __syncthreads();
     for (int i = 0; i < rounds; ++i) {
       scan(i);
       place(i);
@@ -200,48 +208,44 @@ MSGL_DEVICE void kv8_zero_tail(const Kv8Attn& p, int tid, int threads) {
     reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
 }
 
-// Joins cut segments: grid (ctas, rows / 8), a warp per row.
+// Joins cut segments: grid (ctas, rows / 4), a warp per row. Few registers and threads, so that its CTAs fit beside the
+// last ones of the kernel before it and only its loads are waited for.
 template <int R, int HD>
-__global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) {
+__global__ void __launch_bounds__(128) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) {
   pdl_wait();
   pdl_launch();
-  const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 4 + (threadIdx.x >> 5);
   const Kv8Part hd = s.head[c];
   if (hd.parts == 0 || i >= hd.nr) return;
   const int G = p.nq / p.nkv, r = hd.r0 + i, head = hd.h * G + r % G;
-  // part 0 ends its CTA's run, the others begin theirs
-  auto row = [&](int part) { return (int64_t)(part == 0 ? 2 * c + 1 : 2 * (c + part)) * R + i; };
-  float m = -INFINITY;
-  for (int j = lane; j < hd.parts; j += 32) m = fmaxf(m, s.ml[row(j)].x);
-  m = warp_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
+  // part 0 ends its CTA's run, the others begin theirs: slots 2 c + 1, 2 (c + 1), 2 (c + 2), ..
   constexpr int E = HD / 32;
-  float l = 0.f, acc[E];
+  float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   for (int j0 = 0; j0 < hd.parts; j0 += 32) {
-    float w = 0.f;
-    if (j0 + lane < hd.parts) {
-      const float2 ml = s.ml[row(j0 + lane)];
-      w = exp2f(ml.x - base);
-      l += w * ml.y;
-    }
-    const int n = min(32, hd.parts - j0);
+    const int n = min(32, hd.parts - j0), j = j0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) ml = s.ml[(int64_t)(j == 0 ? 2 * c + 1 : 2 * (c + j)) * R + i];
+    const float mx = fmaxf(m, warp_max(ml.x)), base = mx == -INFINITY ? 0.f : mx, f = exp2f(m - base), w = exp2f(ml.x - base);
+    m = mx;
+    l = l * f + w * ml.y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float* src = s.o + row(j0 + j) * HD + lane * E;
+    for (int k = 0; k < n; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float* src = s.o + ((int64_t)(j0 + k == 0 ? 2 * c + 1 : 2 * (c + j0 + k)) * R + i) * HD + lane * E;
       if constexpr (E == 4) {
         const float4 x = *reinterpret_cast<const float4*>(src);
-        acc[0] += wj * x.x, acc[1] += wj * x.y, acc[2] += wj * x.z, acc[3] += wj * x.w;
+        acc[0] += wk * x.x, acc[1] += wk * x.y, acc[2] += wk * x.z, acc[3] += wk * x.w;
       } else {
         const float2 x = *reinterpret_cast<const float2*>(src);
-        acc[0] += wj * x.x, acc[1] += wj * x.y;
+        acc[0] += wk * x.x, acc[1] += wk * x.y;
       }
     }
   }
-  l = warp_sum(l);
-  const float f = kv8_norm(m, l, p.sinks, head);
+  const float f = kv8_norm(m, warp_sum(l), p.sinks, head);
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.o) + ((int64_t)(hd.q0 + r / G) * p.nq + head) * (HD / 2) + lane * (E / 2);
 #pragma unroll
   for (int e = 0; e < E; e += 2) dst[e / 2] = pack_bf16(acc[e] * f, acc[e + 1] * f);

@@ -1,15 +1,16 @@
 // Attention over the 8-bit cache for few rows per request and kv head: decoded tokens, a few drafted ones.
 //
-// What bounds it is the cache's bytes, so the kernel is a stream of them: one CTA per SM, one warp that issues
-// copies of whole pages (codes swizzled by the tensor map, scales as they lie) into a ring of 64-key stages, and two
-// groups of four warps that take the stages in turn, 16 keys a warp. Codes go from shared memory to registers once,
-// 16 bytes a lane, in an order of head dims and keys that fits mma.sync without a transposition:
+// What bounds it is the cache's bytes, so the kernel is a stream of them: two CTAs per SM, each two warps that issue
+// copies of whole pages (codes swizzled by the tensor map, scales as they lie) into a ring of 64-key stages, and four
+// warps that take 16 keys each of every stage. (Two CTAs: while one starts or ends a segment the other streams.) Codes go from
+// shared memory to registers once, 16 bytes a lane, in an order of head dims and keys that fits mma.sync without a
+// transposition:
 //   S = Q K^T  (m16n8k16): lane (g, t) = (lane / 4, lane % 4) holds of key g the head dims [HD/4 t, HD/4 (t + 1)): four
 //     codes are the two registers of one step. The queries' fragments are loaded in the same order of head dims.
 //   O += P V: P's fragments are S's accumulators; lane (g, t) holds of keys 2t, 2t + 1, 2t + 8, 2t + 9 the HD / 8 head dims
 //     from HD/8 g on, and pairs of keys are made by byte permutes. So lane (g, t) ends up with HD / 4 head dims in a row.
 // Codes are exact in fp16, and the queries are, scaled by a power of two. Logits, sums and O are fp32.
-// A warp keeps its own maximum and sum; the eight are joined when a segment ends (see kv8_plan.cuh).
+// A warp keeps its own maximum and sum; the four are joined when a segment ends (see kv8_plan.cuh).
 #pragma once
 #include "kv8.cuh"
 #include "kv8_plan.cuh"
@@ -17,8 +18,9 @@
 namespace msgl {
 
 constexpr int kKsRows = 16;  // rows of a tile: M of the MMA
-constexpr int kKsWarps = 8;   // of products
-constexpr int kKsCopies = 4;  // warps that issue copies
+constexpr int kKsWarps = 4;   // of products
+constexpr int kKsCopies = 2;  // warps that issue copies
+constexpr int kKsCost = 3;    // of a segment, in blocks
 constexpr int kKsThreads = 32 * (kKsWarps + kKsCopies);
 constexpr int kKsDescs = 4;   // segments looked up ahead
 
@@ -30,12 +32,13 @@ template <int HD>
 struct KsCfg {
   static constexpr int kTile = kKv8Block * HD;
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = HD == 128 ? 8 : 16;
+  static constexpr int kStages = HD == 128 ? 4 : 8;
   static constexpr int kScales = 2 * kKv8Block * 4;  // of a stage: keys', then values'
   static constexpr int kMergeQ = HD / 4 + 4, kMergeRow = 4 * kMergeQ;  // floats of a lane's head dims and of a row (no bank conflicts)
   static constexpr int kMerge = kKsWarps * kKsRows * kMergeRow * 4 + kKsWarps * kKsRows * 8;
   static constexpr int kSmem = 1024 + kStages * (kStage + kScales) + kMerge + kKsDescs * (int)sizeof(KsDesc) + (int)sizeof(Kv8Plan) +
                                8 * (kKsThreads / 32) + 8 * (2 * kStages + 2 * kKsDescs) + 16;
+  static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 
 // byte of (row, 16-byte chunk) in a tile of HD-byte rows as the tensor map's swizzle lays it out
@@ -43,23 +46,8 @@ template <int HD>
 MSGL_DEVICE uint32_t ks_swz(int row, int chunk) {
   return HD == 128 ? (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
 }
-MSGL_DEVICE uint4 ks_lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-MSGL_DEVICE uint2 ks_lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
-MSGL_DEVICE float2 ks_lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-  return v;
-}
 MSGL_DEVICE void ks_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -91,16 +79,15 @@ MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tc, const C
 }
 
 template <int HD, bool FP8>
-__global__ void __launch_bounds__(kKsThreads, 1)
+__global__ void __maxnreg__(160)  // (two CTAs, and one of the joining kernel's that waits for them)
 kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
   using C = KsCfg<HD>;
   constexpr int NK = HD / 16;  // steps of Q K^T, and (twice as many) n-tiles of O
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem;
+  uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* scales = reinterpret_cast<float*>(ring + C::kStages * C::kStage);
-  float* merge = scales + C::kStages * (C::kScales / 4);                       // [8][16][kMergeRow]
-  float2* merge_ml = reinterpret_cast<float2*>(merge + kKsWarps * kKsRows * C::kMergeRow);  // [8][16]
+  float* merge = scales + C::kStages * (C::kScales / 4);                       // [warps][16][kMergeRow]
+  float2* merge_ml = reinterpret_cast<float2*>(merge + kKsWarps * kKsRows * C::kMergeRow);  // [warps][16]
   KsDesc* descs = reinterpret_cast<KsDesc*>(merge_ml + kKsWarps * kKsRows);
   Kv8Plan* plan = reinterpret_cast<Kv8Plan*>(descs + kKsDescs);
   int64_t* red = reinterpret_cast<int64_t*>(plan + 1);
@@ -114,7 +101,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kKsWarps / 2);
+      mbar_init(&empty[i], kKsWarps);
     }
     for (int i = 0; i < kKsDescs; ++i) {
       mbar_init(&dfull[i], 1);
@@ -128,30 +115,29 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   pdl_wait();
   pdl_launch();
   if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
-  kv8_plan<kKsRows, kKsThreads>(p, 2, plan, red);  // (its barriers order the initialisation above as well)
+  kv8_plan<kKsRows, kKsCost, kKsThreads>(p, kKsCost + 2, plan, red);  // (its barriers order the initialisation above as well)
   const Kv8Plan pl = *plan;
   const int G = p.nq / p.nkv;
   kv8_zero_tail<HD>(p, threadIdx.x, kKsThreads);
 
   if (warp >= kKsWarps) {
     // ------------------------------------------------------------------ segments and copies
-    // Every copying warp goes through the run's segments and takes every fourth block; the first one publishes them.
+    // Every copying warp goes through the run's segments and takes every second block; the first one publishes them.
     const int me = warp - kKsWarps;
     const int page = p.page, gpb = kKv8Block / page, mine = 32 / gpb;  // pages of a block, blocks whose slots the lanes hold
     int b = pl.b, h = pl.h, t = pl.t, tiles = 0;
     uint32_t seq = 0;
     int64_t u = pl.u0, s0 = pl.s0;
     bool ok = true;
-    Kv8Req r;
-    if (u < pl.u1) {
-      r = kv8_request(p, b);
-      tiles = kv8_tiles<kKsRows>(r, G);
-    }
+    Kv8Req r = pl.r;
+    if (u < pl.u1) tiles = kv8_tiles<kKsRows>(r, G);
     int i = 0, issued = 0;
     uint32_t last = 0;
     for (; ok && u < pl.u1; ++i) {
       const Kv8Tile k = kv8_tile<kKsRows>(p, r, G, t);
-      const int from = (int)(u - s0), to = (int)min((int64_t)k.nblk, pl.u1 - s0);
+      // blocks [from, to) of the segment: its first kKsCost units are none
+      const int from = (int)max(u - s0 - kKsCost, (int64_t)0), to = (int)min((int64_t)k.nblk, pl.u1 - s0 - kKsCost);
+      if (to <= 0) break;  // (the run ends before the segment's first block)
       if (me == 0) {
         const int d = i % kKsDescs;
         if (lane == 0) {
@@ -162,7 +148,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
             D.q0 = r.q0; D.h = h; D.r0 = k.r0; D.nr = k.nr; D.row = r.row; D.pos0 = k.pos0; D.pos1 = k.pos1; D.L = r.L; D.n = r.n;
             D.lo = k.lo; D.kend = k.kend; D.blk = k.blk0 + from; D.nb = to - from; D.valid = 1;
             D.slot = starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
-            const int parts = starts && !ends ? kv8_cta_of(pl, s0 + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
+            const int parts = starts && !ends ? kv8_cta_of(pl, s0 + kKsCost + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
             if (parts > 0) {  // (the run's last segment)
               Kv8Part& hd = scratch.head[blockIdx.x];
               hd.q0 = r.q0; hd.r0 = k.r0; hd.nr = k.nr; hd.h = h; hd.parts = parts;
@@ -172,8 +158,13 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
+      } else if (lane < k.nr) {  // the segment's queries are wanted when the ones before it are done
+        const int rr = k.r0 + lane, tok = rr / G;
+        const char* src = reinterpret_cast<const char*>(p.q) + 2 * ((r.q0 + tok) * p.q_row + (int64_t)(h * G + rr - tok * G) * p.q_head);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+        if (HD == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 128));
       }
-      // This warp's blocks j = j0, j0 + 4, ..: their pages' slots, a batch of `mine` blocks ahead. Looked up in one go, looked over
+      // This warp's blocks j = j0, j0 + 2, ..: their pages' slots, a batch of `mine` blocks ahead. Looked up in one go, looked over
       // when their turn comes, so that the loads' latency is not waited for.
       const int page0 = (k.blk0 + from) * gpb, pages_end = k.kend > k.lo ? (k.kend - 1) / page + 1 : 0;
       const int j0 = (int)((me - seq) & (kKsCopies - 1));
@@ -202,8 +193,8 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       if (!ok) break;
       seq += to - from;
       // the next segment
-      u = s0 + to;
-      s0 += k.nblk;
+      u = s0 + kKsCost + to;
+      s0 += kKsCost + k.nblk;
       if (u < pl.u1 && ++t == tiles) {
         t = 0;
         if (++h == p.nkv) {
@@ -232,13 +223,13 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   }
 
   // -------------------------------------------------------------------- products
-  const int g = lane >> 2, t = lane & 3, group = warp >> 2, key0 = (warp & 3) * 16;
+  const int g = lane >> 2, t = lane & 3, key0 = warp * 16;
   const int ctid = threadIdx.x;
   // this warp's keys lie in one page: [keys' page][values' page] each
   const int base = key0 + (key0 & ~(p.page - 1));
   const uint32_t k_at = (uint32_t)(base + order.codes * p.page) * HD, v_at = (uint32_t)(base + (order.codes ^ 1) * p.page) * HD;
   const uint32_t ks_at = (uint32_t)(base + order.scales * p.page + 2 * t) * 4, vs_at = (uint32_t)(base + (order.scales ^ 1) * p.page + 2 * t) * 4;
-  uint32_t seq = 0;  // stages gone through; this warp takes those of its group's parity
+  uint32_t seq = 0;  // stages gone through
   bool dead = false;
   for (int i = 0;; ++i) {
     const int d = i % kKsDescs;
@@ -292,30 +283,34 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
 #pragma unroll
     for (int j = 0; j < 2 * NK; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-    for (int j = (int)((seq ^ group) & 1); j < D.nb && !dead; j += 2) {
+    for (int j = 0; j < D.nb && !dead; ++j) {
       const uint32_t at = seq + j, stage = at % C::kStages;
       if (!kv8_wait(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
-      const uint32_t st = smem_u32(ring + stage * C::kStage), sk = st + k_at, sv = st + v_at;
-      const uint32_t ssc = smem_u32(scales + stage * (C::kScales / 4));
+      const uint8_t *sk = ring + stage * C::kStage + k_at, *sv = ring + stage * C::kStage + v_at;
+      const uint8_t* ssc = reinterpret_cast<const uint8_t*>(scales) + stage * C::kScales;
       // S: keys key0 + 8 n + g
       float s[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
+        float s2[4] = {0.f, 0.f, 0.f, 0.f};  // (two sums, so that products wait less for one another)
         s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
         uint32_t w[NK];
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c) {
-          const uint4 v = ks_lds128(sk + ks_swz<HD>(8 * n + g, t * (HD / 64) + c));
+          const uint4 v = *reinterpret_cast<const uint4*>(sk + ks_swz<HD>(8 * n + g, t * (HD / 64) + c));
           w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
         }
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
           uint32_t b0, b1;
           kv8_to_half<FP8>(w[kk], b0, b1);
-          ks_mma(s[n], qf[kk], b0, b1);
+          ks_mma(kk & 1 ? s2 : s[n], qf[kk], b0, b1);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[e];
       }
-      const float2 ks0 = ks_lds_f2(ssc + ks_at), ks1 = ks_lds_f2(ssc + ks_at + 32), vs0 = ks_lds_f2(ssc + vs_at), vs1 = ks_lds_f2(ssc + vs_at + 32);
+      const float2 ks0 = *reinterpret_cast<const float2*>(ssc + ks_at), ks1 = *reinterpret_cast<const float2*>(ssc + ks_at + 32);
+      const float2 vs0 = *reinterpret_cast<const float2*>(ssc + vs_at), vs1 = *reinterpret_cast<const float2*>(ssc + vs_at + 32);
       const float ksc[4] = {ks0.x, ks0.y, ks1.x, ks1.y};
       float vsc[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
       const int k0 = (D.blk + j) * kKv8Block + key0;
@@ -325,17 +320,17 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       for (int e = 0; e < 4; ++e) {
         const int key = 2 * t + (e & 1) + 8 * (e >> 1);
         if constexpr (HD == 128) {
-          const uint4 v = ks_lds128(sv + ks_swz<HD>(key, g));
+          const uint4 v = *reinterpret_cast<const uint4*>(sv + ks_swz<HD>(key, g));
           vw[e][0] = v.x; vw[e][1] = v.y; vw[e][2] = v.z; vw[e][3] = v.w;
         } else {
-          const uint2 v = ks_lds64(sv + ks_swz<HD>(key, g >> 1) + (g & 1) * 8);
+          const uint2 v = *reinterpret_cast<const uint2*>(sv + ks_swz<HD>(key, g >> 1) + (g & 1) * 8);
           vw[e][0] = v.x; vw[e][1] = v.y;
         }
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] *= ksc[2 * n + (e & 1)] * qs[e >> 1];
+        for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] * ksc[2 * n + (e & 1)] * qs[e >> 1];
       if (!inside) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -403,7 +398,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     }
     seq += D.nb;
 
-    // join the eight warps
+    // join the warps
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);

@@ -103,11 +103,17 @@ class Case:
         half a bf16 step of the value; half an fp16 step (2^-11) of A, for the weights p_j s^v_j; 2 d A for logits that are
         off by at most d, in the weights and in their sum: an fp32 product sum of hd terms, each addition off by at
         most 2^-23 of the terms' total, and the rounding of its scale, of the maximum taken off it and of the power of 2;
-        and 2 (L / 8 + 16) 2^-23 A for the sums over L keys, added 8 at a time at least."""
+        and 2 (L / 8 + 16) 2^-23 A for the sums over L keys, added 8 at a time at least.
+
+        Half an fp16 step of a weight is 2^-11 of it where fp16 is normal, but not less than half of the smallest step,
+        2^-25. Weights p_j s^v_j are scaled so that the largest one, M, comes to 2^14 (or a larger one, if a warp has not seen
+        it yet: then the step is a smaller part of M): each of them can be off by 2^-25 / 2^14 M, together by
+        2^-39 M sum_j |c_j|. That is what is left of a head dim in which the keys that count have codes of 0."""
         q, sinks = self.q.cpu().double(), None if self.sinks is None else self.sinks.cpu().double()
         T, nq, hd = q.shape
         c = self.cache
         kx, vx = values(c.k, c.k_scale), values(c.v, c.v_scale)
+        cx, sx = values(c.v, torch.ones_like(c.v_scale)).abs(), c.v_scale.cpu().double()
         g = nq // kx.shape[0]
         out, tol = torch.zeros_like(q), torch.zeros_like(q)
         scale = hd**-0.5 if self.scale is None else self.scale
@@ -129,7 +135,9 @@ class Case:
                 out[at + i] = (p * v).sum(1)
                 d = ((hd + 16) * big + 16) * 2.0**-23
                 A = (p * v.abs()).sum(1)
-                tol[at + i] = out[at + i].abs() * 2.0**-8 + A * (2.0**-11 + 2 * d.unsqueeze(-1) + 2 * (len(s) / 8 + 16) * 2.0**-23) + 1e-37
+                M = (p.squeeze(-1) * sx[:, s].repeat_interleave(g, 0)).amax(-1, keepdim=True)
+                least = 2.0**-39 * M * cx[:, s].repeat_interleave(g, 0).sum(1)
+                tol[at + i] = out[at + i].abs() * 2.0**-8 + A * (2.0**-11 + 2 * d.unsqueeze(-1) + 2 * (len(s) / 8 + 16) * 2.0**-23) + least + 1e-37
             at += n
         return out, tol
 
