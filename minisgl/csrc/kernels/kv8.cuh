@@ -32,6 +32,11 @@ MSGL_DEVICE bool kv8_wait(uint64_t* bar, uint32_t parity, int where) {
   }
 }
 
+// The same for a whole warp: its lanes go on or give up together.
+MSGL_DEVICE bool kv8_wait_warp(uint64_t* bar, uint32_t parity, int where) {
+  return __all_sync(0xffffffffu, kv8_wait(bar, parity, where));
+}
+
 // two values to two e4m3 codes, nearest, ties to even (the first one in the low byte)
 MSGL_DEVICE uint16_t kv8_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);

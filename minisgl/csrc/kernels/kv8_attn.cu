@@ -2,6 +2,7 @@
 //
 //   o_i = sum_j w_ij s^v_j c^v_j / sum_j w_ij,  w_ij = exp(scale s^k_j q_i . c^k_j),  over the keys j that query i sees
 #include "kv8_stream.cuh"
+#include "kv8_tiles.cuh"
 
 #include <mutex>
 
@@ -54,36 +55,71 @@ int sm_count() {
   return sms;
 }
 
-template <int HD, bool FP8>
+template <int HD, bool FP8, int NR>
 int stream_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
-  using C = KsCfg<HD>;
-  constexpr auto kernel = kv8_stream_kernel<HD, FP8>;
+  using C = KsCfg<HD, NR>;
+  constexpr auto kernel = kv8_stream_kernel<HD, FP8, NR>;
   if (msgl_set_smem<kernel>(C::kSmem, 100) != cudaSuccess) return 4;
   CUtensorMap tc, ts;
   Kv8Order order;
   if (!encode_cache(&tc, &ts, &order, p, HD)) return 2;
   const int ctas = 2 * sm_count();
-  const Kv8Scratch scratch = kv8_scratch<kKsRows, HD>(ws, ctas);
+  const Kv8Scratch scratch = kv8_scratch<C::kRows, HD>(ws, ctas);
   if (msgl_launch(kernel, dim3(ctas), dim3(kKsThreads), C::kSmem, s, 1, tc, ts, p, order, scratch) != cudaSuccess) return 4;
   ++*launches;
-  if (msgl_launch(kv8_join_kernel<kKsRows, HD>, dim3(ctas, kKsRows / 4), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
+  if (msgl_launch(kv8_join_kernel<C::kRows, HD>, dim3(ctas, C::kRows / 4), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
   ++*launches;
   return 0;
+}
+
+template <int HD, bool FP8>
+int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
+  using C = KtCfg<HD>;
+  constexpr auto kernel = kv8_tiles_kernel<HD, FP8>;
+  if (msgl_set_smem<kernel>(C::kSmem) != cudaSuccess) return 4;
+  CUtensorMap tc, ts;
+  Kv8Order order;
+  if (!encode_cache(&tc, &ts, &order, p, HD)) return 2;
+  const int ctas = sm_count();
+  const Kv8Scratch scratch = kv8_scratch<kKtRows, HD>(ws, ctas);
+  if (msgl_launch(kernel, dim3(ctas), dim3(kKtThreads), C::kSmem, s, 1, tc, ts, p, order, scratch) != cudaSuccess) return 4;
+  ++*launches;
+  if (msgl_launch(kv8_join_kernel<kKtRows, HD>, dim3(ctas, 8), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
+  ++*launches;
+  return 0;
+}
+
+// The form for what the caller has told of a request's rows: 8, 16: rows of a streaming tile, 256: tensor core tiles.
+int form_of(const Kv8Attn& p, int max_q_len) {
+  const int64_t rows = (int64_t)max_q_len * (p.nq / p.nkv);
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
+}
+
+template <int HD, bool FP8>
+int any_form(const Kv8Attn& p, int max_q_len, void* ws, int* launches, cudaStream_t s) {
+  switch (form_of(p, max_q_len)) {
+    case 8: return stream_form<HD, FP8, 1>(p, ws, launches, s);
+    case 16: return stream_form<HD, FP8, 2>(p, ws, launches, s);
+    default: return tiles_form<HD, FP8>(p, ws, launches, s);
+  }
+}
+
+template <int HD>
+int64_t workspace(int form) {
+  const int sms = sm_count();
+  return form == 8 ? kv8_scratch_bytes<8, HD>(2 * sms) : form == 16 ? kv8_scratch_bytes<16, HD>(2 * sms) : kv8_scratch_bytes<kKtRows, HD>(sms);
 }
 
 }  // namespace
 
 extern "C" int64_t msgl_kv8_attention_workspace(const Kv8Attn* p, int hd, int max_q_len) {
-  (void)p, (void)max_q_len;
-  const int ctas = 2 * sm_count();
-  return hd == 128 ? kv8_scratch_bytes<kKsRows, 128>(ctas) : kv8_scratch_bytes<kKsRows, 64>(ctas);
+  return hd == 128 ? workspace<128>(form_of(*p, max_q_len)) : workspace<64>(form_of(*p, max_q_len));
 }
 
 extern "C" int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, void* ws, int* launches, cudaStream_t s) {
-  (void)max_q_len;
   *launches = 0;
-  if (hd == 128) return fp8 ? stream_form<128, true>(*p, ws, launches, s) : stream_form<128, false>(*p, ws, launches, s);
-  if (hd == 64) return fp8 ? stream_form<64, true>(*p, ws, launches, s) : stream_form<64, false>(*p, ws, launches, s);
+  if (hd == 128) return fp8 ? any_form<128, true>(*p, max_q_len, ws, launches, s) : any_form<128, false>(*p, max_q_len, ws, launches, s);
+  if (hd == 64) return fp8 ? any_form<64, true>(*p, max_q_len, ws, launches, s) : any_form<64, false>(*p, max_q_len, ws, launches, s);
   return 3;
 }
 

@@ -11,7 +11,7 @@
 // zeroed by a launch as well, or shared between calls.)
 #pragma once
 #include "api.h"
-#include "common.cuh"
+#include "kv8.cuh"
 
 namespace msgl {
 
@@ -164,6 +164,31 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
   __syncthreads();
 }
 
+// Which of a page's two parts holds the keys' (0 or 1): the tensor maps' base is the lower of the two addresses.
+struct Kv8Order {
+  int codes, scales;
+};
+
+// The copies of one 64-key block, a page at a time: its keys' and values' codes with one instruction, its scales with
+// another (an instruction costs the warp some 100 cycles, whatever it copies). Lanes first .. first + pages - 1 hold the pages'
+// slots, -1 for a page that is not there: what lies outside the tensors is filled with zeros. A page's keys are
+// beside its values, codes and scales alike.
+template <int HD>
+MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tc, const CUtensorMap* ts, uint8_t* codes, float* scales, uint64_t* bar,
+                                int h, int slots, int first, int pages, int lane) {
+  const int page = p.page;
+  if (lane == 0) mbar_expect_tx(bar, 2 * page * pages * (HD + 4));
+  __syncwarp();
+  for (int i = 0; i < pages; ++i) {
+    int slot = __shfl_sync(0xffffffffu, slots, first + i);
+    if (lane == 0) {
+      if (slot < 0) slot = p.num_slots;
+      kv8_load_4d(codes + 2 * i * page * HD, tc, bar, 0, slot, h, 0);
+      tma_load_3d(scales + 2 * i * page, ts, bar, slot, h, 0);
+    }
+  }
+}
+
 // Scratch of one call: a header per CTA (of the segment that its run ends in, if cut there and begun in it), and per
 // slot the rows' maxima and sums (the logits' log2 domain) and their sums of values.
 struct Kv8Part {
@@ -208,16 +233,9 @@ MSGL_DEVICE void kv8_zero_tail(const Kv8Attn& p, int tid, int threads) {
     reinterpret_cast<uint4*>(p.o)[i] = make_uint4(0, 0, 0, 0);
 }
 
-// Joins cut segments: grid (ctas, rows / 4), a warp per row. Few registers and threads, so that its CTAs fit beside the
-// last ones of the kernel before it and only its loads are waited for.
 template <int R, int HD>
-__global__ void __launch_bounds__(128) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) {
-  pdl_wait();
-  pdl_launch();
-  const int c = blockIdx.x, lane = threadIdx.x & 31, i = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const Kv8Part hd = s.head[c];
-  if (hd.parts == 0 || i >= hd.nr) return;
-  const int G = p.nq / p.nkv, r = hd.r0 + i, head = hd.h * G + r % G;
+MSGL_DEVICE void kv8_join_row(const Kv8Attn& p, const Kv8Scratch& s, const Kv8Part& hd, int c, int i, int lane, int G) {
+  const int r = hd.r0 + i, head = hd.h * G + r % G;
   // part 0 ends its CTA's run, the others begin theirs: slots 2 c + 1, 2 (c + 1), 2 (c + 2), ..
   constexpr int E = HD / 32;
   float m = -INFINITY, l = 0.f, acc[E];
@@ -249,6 +267,18 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) 
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.o) + ((int64_t)(hd.q0 + r / G) * p.nq + head) * (HD / 2) + lane * (E / 2);
 #pragma unroll
   for (int e = 0; e < E; e += 2) dst[e / 2] = pack_bf16(acc[e] * f, acc[e + 1] * f);
+}
+
+// Joins cut segments: grid (ctas, groups of four rows), a warp per row. Few registers and threads, so that its CTAs fit beside the
+// last ones of the kernel before it and only its loads are waited for.
+template <int R, int HD>
+__global__ void __launch_bounds__(128) kv8_join_kernel(Kv8Attn p, Kv8Scratch s) {
+  pdl_wait();
+  pdl_launch();
+  const int c = blockIdx.x, lane = threadIdx.x & 31, G = p.nq / p.nkv;
+  const Kv8Part hd = s.head[c];
+  if (hd.parts == 0) return;
+  for (int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < hd.nr; i += gridDim.y * 4) kv8_join_row<R, HD>(p, s, hd, c, i, lane, G);
 }
 
 }  // namespace msgl

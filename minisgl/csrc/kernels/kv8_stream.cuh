@@ -5,10 +5,12 @@
 // warps that take 16 keys each of every stage. (Two CTAs: while one starts or ends a segment the other streams.) Codes go from
 // shared memory to registers once, 16 bytes a lane, in an order of head dims and keys that fits mma.sync without a
 // transposition:
-//   S = Q K^T  (m16n8k16): lane (g, t) = (lane / 4, lane % 4) holds of key g the head dims [HD/4 t, HD/4 (t + 1)): four
-//     codes are the two registers of one step. The queries' fragments are loaded in the same order of head dims.
-//   O += P V: P's fragments are S's accumulators; lane (g, t) holds of keys 2t, 2t + 1, 2t + 8, 2t + 9 the HD / 8 head dims
-//     from HD/8 g on, and pairs of keys are made by byte permutes. So lane (g, t) ends up with HD / 4 head dims in a row.
+//   S^T = K Q^T (m16n8k16, 16 keys x 8 rows): lane (g, t) = (lane / 4, lane % 4) holds of keys g and g + 8 the head dims
+//     [HD/4 t, HD/4 (t + 1)): four codes are two registers of one step. The queries' fragments are loaded in the same order.
+//   O^T += V^T P^T (16 head dims x 8 rows): lane (g, t) holds of keys 2t, 2t + 1, 2t + 8, 2t + 9 the HD / 8 head dims from
+//     HD/8 g on, and pairs of keys are made by byte permutes; P^T's fragments are S^T's, turned by movmatrix in fp16. Lane
+//     (g, t) ends up with HD / 8 head dims in a row of rows 2t and 2t + 1.
+// Keys as the 16 rows of a product, since the query rows are often 8 at most: NR = 1 takes tiles of 8 rows, NR = 2 of 16.
 // Codes are exact in fp16, and the queries are, scaled by a power of two. Logits, sums and O are fp32.
 // A warp keeps its own maximum and sum; the four are joined when a segment ends (see kv8_plan.cuh).
 #pragma once
@@ -17,7 +19,6 @@
 
 namespace msgl {
 
-constexpr int kKsRows = 16;  // rows of a tile: M of the MMA
 constexpr int kKsWarps = 4;   // of products
 constexpr int kKsCopies = 2;  // warps that issue copies
 constexpr int kKsCost = 3;    // of a segment, in blocks
@@ -28,14 +29,16 @@ struct KsDesc {
   int q0, h, r0, nr, row, pos0, pos1, L, n, lo, kend, blk, nb, slot, parts, valid;  // blocks [blk, blk + nb); slot -1: whole
 };
 
-template <int HD>
+template <int HD, int NR>
 struct KsCfg {
+  static constexpr int kRows = 8 * NR;
   static constexpr int kTile = kKv8Block * HD;
   static constexpr int kStage = 2 * kTile;
   static constexpr int kStages = HD == 128 ? 4 : 8;
   static constexpr int kScales = 2 * kKv8Block * 4;  // of a stage: keys', then values'
-  static constexpr int kMergeQ = HD / 4 + 4, kMergeRow = 4 * kMergeQ;  // floats of a lane's head dims and of a row (no bank conflicts)
-  static constexpr int kMerge = kKsWarps * kKsRows * kMergeRow * 4 + kKsWarps * kKsRows * 8;
+  // merge scratch: floats of a lane's head dims and of a row (padded, against bank conflicts)
+  static constexpr int kMergeQ = HD / 8 + 4, kMergeRow = 8 * kMergeQ + 4;
+  static constexpr int kMerge = kKsWarps * kRows * kMergeRow * 4 + kKsWarps * kRows * 8;
   static constexpr int kSmem = 1024 + kStages * (kStage + kScales) + kMerge + kKsDescs * (int)sizeof(KsDesc) + (int)sizeof(Kv8Plan) +
                                8 * (kKsThreads / 32) + 8 * (2 * kStages + 2 * kKsDescs) + 16;
   static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -53,42 +56,18 @@ MSGL_DEVICE void ks_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Which of a page's two parts holds the keys' (0 or 1): the tensor maps' base is the lower of the two addresses.
-struct Kv8Order {
-  int codes, scales;
-};
-
-// The copies of one 64-key block, a page at a time: its keys' and values' codes with one instruction, its scales with
-// another (an instruction costs the warp some 100 cycles, whatever it copies). Lanes first .. first + pages - 1 hold the pages'
-// slots, -1 for a page that is not there: what lies outside the tensors is filled with zeros. A page's keys are
-// beside its values, codes and scales alike.
-template <int HD>
-MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tc, const CUtensorMap* ts, uint8_t* codes, float* scales, uint64_t* bar,
-                                int h, int slots, int first, int pages, int lane) {
-  const int page = p.page;
-  if (lane == 0) mbar_expect_tx(bar, 2 * page * pages * (HD + 4));
-  __syncwarp();
-  for (int i = 0; i < pages; ++i) {
-    int slot = __shfl_sync(0xffffffffu, slots, first + i);
-    if (lane == 0) {
-      if (slot < 0) slot = p.num_slots;
-      kv8_load_4d(codes + 2 * i * page * HD, tc, bar, 0, slot, h, 0);
-      tma_load_3d(scales + 2 * i * page, ts, bar, slot, h, 0);
-    }
-  }
-}
-
-template <int HD, bool FP8>
-__global__ void __maxnreg__(160)  // (two CTAs, and one of the joining kernel's that waits for them)
+template <int HD, bool FP8, int NR>
+__global__ void __launch_bounds__(kKsThreads, 2)
 kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
-  using C = KsCfg<HD>;
-  constexpr int NK = HD / 16;  // steps of Q K^T, and (twice as many) n-tiles of O
+  using C = KsCfg<HD, NR>;
+  constexpr int NK = HD / 16;  // steps of K Q^T, and tiles of O^T
+  constexpr int R = C::kRows;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* scales = reinterpret_cast<float*>(ring + C::kStages * C::kStage);
   float* merge = scales + C::kStages * (C::kScales / 4);                       // [warps][16][kMergeRow]
-  float2* merge_ml = reinterpret_cast<float2*>(merge + kKsWarps * kKsRows * C::kMergeRow);  // [warps][16]
-  KsDesc* descs = reinterpret_cast<KsDesc*>(merge_ml + kKsWarps * kKsRows);
+  float2* merge_ml = reinterpret_cast<float2*>(merge + kKsWarps * R * C::kMergeRow);  // [warps][16]
+  KsDesc* descs = reinterpret_cast<KsDesc*>(merge_ml + kKsWarps * R);
   Kv8Plan* plan = reinterpret_cast<Kv8Plan*>(descs + kKsDescs);
   int64_t* red = reinterpret_cast<int64_t*>(plan + 1);
   uint64_t* full = reinterpret_cast<uint64_t*>(red + kKsThreads / 32);
@@ -115,7 +94,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   pdl_wait();
   pdl_launch();
   if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
-  kv8_plan<kKsRows, kKsCost, kKsThreads>(p, kKsCost + 2, plan, red);  // (its barriers order the initialisation above as well)
+  kv8_plan<R, kKsCost, kKsThreads>(p, kKsCost + 2, plan, red);  // (its barriers order the initialisation above as well)
   const Kv8Plan pl = *plan;
   const int G = p.nq / p.nkv;
   kv8_zero_tail<HD>(p, threadIdx.x, kKsThreads);
@@ -130,11 +109,11 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     int64_t u = pl.u0, s0 = pl.s0;
     bool ok = true;
     Kv8Req r = pl.r;
-    if (u < pl.u1) tiles = kv8_tiles<kKsRows>(r, G);
+    if (u < pl.u1) tiles = kv8_tiles<R>(r, G);
     int i = 0, issued = 0;
     uint32_t last = 0;
     for (; ok && u < pl.u1; ++i) {
-      const Kv8Tile k = kv8_tile<kKsRows>(p, r, G, t);
+      const Kv8Tile k = kv8_tile<R>(p, r, G, t);
       // blocks [from, to) of the segment: its first kKsCost units are none
       const int from = (int)max(u - s0 - kKsCost, (int64_t)0), to = (int)min((int64_t)k.nblk, pl.u1 - s0 - kKsCost);
       if (to <= 0) break;  // (the run ends before the segment's first block)
@@ -202,7 +181,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
           do {
             if (++b >= p.num_reqs) break;  // (never: units are left)
             r = kv8_request(p, b);
-            tiles = kv8_tiles<kKsRows>(r, G);
+            tiles = kv8_tiles<R>(r, G);
           } while (tiles == 0);
           if (b >= p.num_reqs) u = pl.u1;
         }
@@ -228,12 +207,12 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   // this warp's keys lie in one page: [keys' page][values' page] each
   const int base = key0 + (key0 & ~(p.page - 1));
   const uint32_t k_at = (uint32_t)(base + order.codes * p.page) * HD, v_at = (uint32_t)(base + (order.codes ^ 1) * p.page) * HD;
-  const uint32_t ks_at = (uint32_t)(base + order.scales * p.page + 2 * t) * 4, vs_at = (uint32_t)(base + (order.scales ^ 1) * p.page + 2 * t) * 4;
+  const uint32_t ks_at = (uint32_t)(base + order.scales * p.page + g) * 4, vs_at = (uint32_t)(base + (order.scales ^ 1) * p.page + g) * 4;
   uint32_t seq = 0;  // stages gone through
   bool dead = false;
   for (int i = 0;; ++i) {
     const int d = i % kKsDescs;
-    if (!dead && !kv8_wait(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
+    if (!dead && !kv8_wait_warp(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
     if (!dead && !descs[d].valid) {
       named_bar_sync(1, kKsWarps * 32);  // (pairs with the barrier below of a warp that has given up)
       break;
@@ -242,12 +221,12 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     __syncwarp();
     if (!dead && lane == 0) mbar_arrive(&dempty[d]);
 
-    // queries: rows g and g + 8 in fragments, brought to fp16's range by a power of two each
-    uint32_t qf[NK][4];
-    float qs[2];
-    int qpos[2];
+    // queries: rows g (+ 8) in fragments, brought to fp16's range by a power of two each
+    uint32_t qf[NR][NK][2];
+    float qs[NR][2];  // of rows 2 t and 2 t + 1
+    int qpos[NR][2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < NR; ++x) {
       const int rr = g + 8 * x, r = D.r0 + rr, tok = r / G;
       const bool in = !dead && rr < D.nr;
       uint4 u[HD / 32];
@@ -259,7 +238,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(src) + j);
       }
-      qpos[x] = in ? D.L - D.n + tok : -1;
+      const int pos = in ? D.L - D.n + tok : -1;
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < HD / 32; ++j)
@@ -268,152 +247,180 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const float f = kv8_q_factor(__uint_as_float(m << 16));
-      qs[x] = p.scale * kKv8Log2e * kv8_reciprocal(f);
+      const float back = p.scale * kKv8Log2e * kv8_reciprocal(f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qs[x][e] = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+        qpos[x][e] = __shfl_sync(0xffffffffu, pos, (2 * t + e) * 4);
+      }
 #pragma unroll
       for (int j = 0; j < HD / 32; ++j) {
         const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)  // dims 8 j + 2 e and the next: step 2 j + e / 2
-          qf[2 * j + (e >> 1)][x + 2 * (e & 1)] = pack_half(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
+          qf[x][2 * j + (e >> 1)][e & 1] = pack_half(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
       }
     }
 
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float o[2 * NK][4];
+    float m[NR][2], l[NR][2], o[NR][NK][4];
 #pragma unroll
-    for (int j = 0; j < 2 * NK; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int x = 0; x < NR; ++x) {
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
+    }
 
     for (int j = 0; j < D.nb && !dead; ++j) {
       const uint32_t at = seq + j, stage = at % C::kStages;
-      if (!kv8_wait(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
-      const uint8_t *sk = ring + stage * C::kStage + k_at, *sv = ring + stage * C::kStage + v_at;
-      const uint8_t* ssc = reinterpret_cast<const uint8_t*>(scales) + stage * C::kScales;
-      // S: keys key0 + 8 n + g
-      float s[2][4];
+      if (!kv8_wait_warp(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
+      const uint8_t* st = ring + stage * C::kStage;
+      const uint8_t* sc = reinterpret_cast<const uint8_t*>(scales) + stage * C::kScales;
+      // S^T of keys g and g + 8 (c = 0, 1), rows 2 t and 2 t + 1 (e): s[x][2 c + e]
+      float s[NR][4], ksc[2], vsc[2];
+      {
+        uint32_t w[2][NK];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float s2[4] = {0.f, 0.f, 0.f, 0.f};  // (two sums, so that products wait less for one another)
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        uint32_t w[NK];
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-          const uint4 v = *reinterpret_cast<const uint4*>(sk + ks_swz<HD>(8 * n + g, t * (HD / 64) + c));
-          w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+          for (int y = 0; y < HD / 64; ++y) {
+            const uint4 v = *reinterpret_cast<const uint4*>(st + k_at + ks_swz<HD>(8 * c + g, t * (HD / 64) + y));
+            w[c][4 * y] = v.x; w[c][4 * y + 1] = v.y; w[c][4 * y + 2] = v.z; w[c][4 * y + 3] = v.w;
+          }
+          ksc[c] = *reinterpret_cast<const float*>(sc + ks_at + 32 * c);
+          vsc[c] = *reinterpret_cast<const float*>(sc + vs_at + 32 * c);
         }
+        float s2[NR][4];  // (two sums each)
+#pragma unroll
+        for (int x = 0; x < NR; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
-          uint32_t b0, b1;
-          kv8_to_half<FP8>(w[kk], b0, b1);
-          ks_mma(kk & 1 ? s2 : s[n], qf[kk], b0, b1);
+          uint32_t a[4];
+          kv8_to_half<FP8>(w[0][kk], a[0], a[2]);
+          kv8_to_half<FP8>(w[1][kk], a[1], a[3]);
+#pragma unroll
+          for (int x = 0; x < NR; ++x) ks_mma(kk & 1 ? s2[x] : s[x], a, qf[x][kk][0], qf[x][kk][1]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += s2[e];
+        for (int x = 0; x < NR; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[x][e] = (s[x][e] + s2[x][e]) * ksc[e >> 1] * qs[x][e & 1];
       }
-      const float2 ks0 = *reinterpret_cast<const float2*>(ssc + ks_at), ks1 = *reinterpret_cast<const float2*>(ssc + ks_at + 32);
-      const float2 vs0 = *reinterpret_cast<const float2*>(ssc + vs_at), vs1 = *reinterpret_cast<const float2*>(ssc + vs_at + 32);
-      const float ksc[4] = {ks0.x, ks0.y, ks1.x, ks1.y};
-      float vsc[4] = {vs0.x, vs0.y, vs1.x, vs1.y};
-      const int k0 = (D.blk + j) * kKv8Block + key0;
-      const bool inside = k0 + 16 <= D.pos0 + 1 && (p.window <= 0 || k0 >= D.pos1 - p.window + 1);  // every row sees all 16
-      uint32_t vw[4][NK / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = 2 * t + (e & 1) + 8 * (e >> 1);
-        if constexpr (HD == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(sv + ks_swz<HD>(key, g));
-          vw[e][0] = v.x; vw[e][1] = v.y; vw[e][2] = v.z; vw[e][3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(sv + ks_swz<HD>(key, g >> 1) + (g & 1) * 8);
-          vw[e][0] = v.x; vw[e][1] = v.y;
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] * ksc[2 * n + (e & 1)] * qs[e >> 1];
+      const int k0 = (D.blk + j) * kKv8Block + key0, k1 = k0 + 16;
+      const bool inside = k1 <= D.pos0 + 1 && (p.window <= 0 || k0 >= D.pos1 - p.window + 1);  // every row sees every key
       if (!inside) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int c = 0; c < 2; ++c) {
+          const int kp = k0 + 8 * c + g;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int kp = k0 + 8 * n + 2 * t + e;
+          for (int x = 0; x < NR; ++x)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const bool seen = kp <= qpos[x] && (p.window <= 0 || kp > qpos[x] - p.window);
-              s[n][2 * x + e] = seen ? s[n][2 * x + e] : -INFINITY;
+            for (int e = 0; e < 2; ++e) {
+              const bool seen = kp <= qpos[x][e] && (p.window <= 0 || kp > qpos[x][e] - p.window);
+              s[x][2 * c + e] = seen ? s[x][2 * c + e] : -INFINITY;
             }
-            // a key that no row of the tile sees may be no position at all: its codes and scale can be anything
-            if (kp < D.lo || kp >= D.kend) {
-              vsc[2 * n + e] = 0.f;
+          if (kp < D.lo || kp >= D.kend) vsc[c] = 0.f;  // (it may be no position at all: its scale can be anything)
+        }
+      }
+      const float lv[2] = {kv8_log_scale(vsc[0]), kv8_log_scale(vsc[1])};
+      // running offsets and sums
+      float f[NR][2];
+      uint32_t pf[NR][2];
+      bool grown = false;
 #pragma unroll
-              for (int c = 0; c < NK / 2; ++c) vw[2 * n + e][c] = 0u;
-            }
+      for (int x = 0; x < NR; ++x) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[x][e] + lv[0], s[x][2 + e] + lv[1]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx - kKv8Top, m[x][e]);
+          const float base = mx == -INFINITY ? 0.f : mx;
+          f[x][e] = kv8_exp2(m[x][e] - base);
+          grown |= mx != m[x][e];
+          m[x][e] = mx;
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float y = s[x][2 * c + e], w = kv8_exp2(y - base);
+            sum += w;
+            s[x][2 * c + e] = y == -INFINITY ? 0.f : w * vsc[c];  // (a hidden key's weight is zero whatever its scale)
+          }
+          l[x][e] = l[x][e] * f[x][e] + sum;  // (of this lane's keys; joined over g at the end)
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[x][c]) : "r"(pack_half(s[x][2 * c], s[x][2 * c + 1])));
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int x = 0; x < NR; ++x)
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            o[x][n][0] *= f[x][0]; o[x][n][1] *= f[x][1]; o[x][n][2] *= f[x][0]; o[x][n][3] *= f[x][1];
           }
       }
-      float lv[4];
+      // O^T: tile n holds head dims HD/8 g + 2 n and the next
+      {
+        uint32_t vw[4][NK / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lv[e] = kv8_log_scale(vsc[e]);
-      float f[2];
-      uint32_t pf[4];
+        for (int e = 0; e < 4; ++e) {
+          const int key = 2 * t + (e & 1) + 8 * (e >> 1);
+          if constexpr (HD == 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(st + v_at + ks_swz<HD>(key, g));
+            vw[e][0] = v.x; vw[e][1] = v.y; vw[e][2] = v.z; vw[e][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(st + v_at + ks_swz<HD>(key, g >> 1) + (g & 1) * 8);
+            vw[e][0] = v.x; vw[e][1] = v.y;
+          }
+          const int kp = k0 + key;
+          if (!inside && (kp < D.lo || kp >= D.kend)) {  // (nor are such a key's codes any)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float mx = fmaxf(fmaxf(s[0][2 * x] + lv[0], s[0][2 * x + 1] + lv[1]), fmaxf(s[1][2 * x] + lv[2], s[1][2 * x + 1] + lv[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = fmaxf(mx - kKv8Top, m[x]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        f[x] = kv8_exp2(m[x] - base);
-        m[x] = mx;
-        float e[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) e[y] = kv8_exp2(s[y >> 1][2 * x + (y & 1)] - base);
-        l[x] = l[x] * f[x] + ((e[0] + e[1]) + (e[2] + e[3]));  // (of this lane's keys; joined over t at the end)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)  // (a hidden key's weight is zero whatever its scale)
-          e[y] = s[y >> 1][2 * x + (y & 1)] == -INFINITY ? 0.f : e[y] * vsc[y];
-        pf[x] = pack_half(e[0], e[1]);
-        pf[2 + x] = pack_half(e[2], e[3]);
-      }
-      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
-#pragma unroll
-        for (int n = 0; n < 2 * NK; ++n) {
-          o[n][0] *= f[0]; o[n][1] *= f[0]; o[n][2] *= f[1]; o[n][3] *= f[1];
-        }
-      }
-      // O: n-tile n holds head dim HD/8 g + n of every g
-#pragma unroll
-      for (int c = 0; c < NK / 2; ++c) {
-        uint32_t b[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t lo = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x5140), hi = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x7362);
-          kv8_to_half<FP8>(lo, b[x][0], b[x][1]);
-          kv8_to_half<FP8>(hi, b[x][2], b[x][3]);
+            for (int c = 0; c < NK / 2; ++c) vw[e][c] = 0u;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ks_mma(o[4 * c + e], pf, b[0][e], b[1][e]);
+        for (int c = 0; c < NK / 2; ++c) {
+          uint32_t b[2][4];  // head dims 4 c .. 4 c + 3 of keys 2 t, 2 t + 1 and of the other two
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t lo = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x5140), hi = __byte_perm(vw[2 * x][c], vw[2 * x + 1][c], 0x7362);
+            kv8_to_half<FP8>(lo, b[x][0], b[x][1]);
+            kv8_to_half<FP8>(hi, b[x][2], b[x][3]);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t a[4] = {b[0][2 * n], b[0][2 * n + 1], b[1][2 * n], b[1][2 * n + 1]};
+#pragma unroll
+            for (int x = 0; x < NR; ++x) ks_mma(o[x][2 * c + n], a, pf[x][0], pf[x][1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
     }
     seq += D.nb;
 
     // join the warps
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      const int rr = g + 8 * x;
-      if (rr < D.nr) {
-        if (t == 0) merge_ml[warp * kKsRows + rr] = make_float2(m[x], l[x]);
-        float* dst = merge + (warp * kKsRows + rr) * C::kMergeRow + t * C::kMergeQ;
+    for (int x = 0; x < NR; ++x)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)  // n-tile j, columns 2 t and 2 t + 1: head dims HD/4 t + j and HD/4 t + HD/8 + j
+      for (int e = 0; e < 2; ++e) {
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 4);
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 8);
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 16);
+        const int rr = 8 * x + 2 * t + e;
+        if (rr < D.nr) {
+          if (g == 0) merge_ml[warp * R + rr] = make_float2(m[x][e], l[x][e]);
+          float* dst = merge + (warp * R + rr) * C::kMergeRow + g * C::kMergeQ;
 #pragma unroll
-          for (int j = 0; j < HD / 8; j += 4)
-            *reinterpret_cast<float4*>(dst + n * (HD / 8) + j) = make_float4(o[j][2 * x + n], o[j + 1][2 * x + n], o[j + 2][2 * x + n], o[j + 3][2 * x + n]);
+          for (int n = 0; n < NK; n += 2)
+            *reinterpret_cast<float4*>(dst + 2 * n) = make_float4(o[x][n][e], o[x][n][2 + e], o[x][n + 1][e], o[x][n + 1][2 + e]);
+        }
       }
-    }
     named_bar_sync(1, kKsWarps * 32);
     if (*abort_flag) break;
     for (int idx = ctid; idx < D.nr * (HD / 4); idx += kKsWarps * 32) {
@@ -422,7 +429,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       float2 ml[kKsWarps];
 #pragma unroll
       for (int w = 0; w < kKsWarps; ++w) {
-        ml[w] = merge_ml[w * kKsRows + rr];
+        ml[w] = merge_ml[w * R + rr];
         mx = fmaxf(mx, ml[w].x);
       }
       const float base = mx == -INFINITY ? 0.f : mx;
@@ -432,7 +439,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       for (int w = 0; w < kKsWarps; ++w) {
         const float fw = kv8_exp2(ml[w].x - base);
         ll += fw * ml[w].y;
-        const float4 v = *reinterpret_cast<const float4*>(merge + (w * kKsRows + rr) * C::kMergeRow + c4 / (HD / 16) * C::kMergeQ + c4 % (HD / 16) * 4);
+        const float4 v = *reinterpret_cast<const float4*>(merge + (w * R + rr) * C::kMergeRow + c4 / (HD / 32) * C::kMergeQ + c4 % (HD / 32) * 4);
         acc.x += fw * v.x; acc.y += fw * v.y; acc.z += fw * v.z; acc.w += fw * v.w;
       }
       if (D.slot < 0) {
@@ -441,7 +448,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         reinterpret_cast<uint2*>(p.o)[((int64_t)(D.q0 + tok) * p.nq + head) * (HD / 4) + c4] =
             make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
       } else {
-        const int64_t row = (int64_t)D.slot * kKsRows + rr;
+        const int64_t row = (int64_t)D.slot * R + rr;
         reinterpret_cast<float4*>(scratch.o)[row * (HD / 4) + c4] = acc;
         if (c4 == 0) scratch.ml[row] = make_float2(mx, ll);
       }

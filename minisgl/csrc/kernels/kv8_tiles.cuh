@@ -1,0 +1,622 @@
+// Attention over the 8-bit cache for many rows per request and kv head: chunks of prompts, drafted tokens of wide groups.
+//
+// One CTA per SM takes segments of 256 packed rows (see kv8_plan.cuh), two tiles of 128 rows that share every key and
+// value block, 64 keys at a time, on the 5th-generation tensor core:
+//
+//   warp 0        goes through the run's segments, publishes them, copies raw pages into a ring by TMA
+//   warps 1, 2    issue the products of one tile each: S = Q K^T, then, once the weights are there, O += P V. Q and P are read
+//                 from tensor memory and K, V from shared memory, whose bandwidth is what all of this comes close to.
+//   warp 3        fetches the next segments' queries into the L2 cache
+//   warps 4 - 11  softmax, one thread per row: S out of tensor memory, weights as fp16 over S's columns, O rescaled there
+//                 when a row's offset grows by more than 2^(15 - kKtTop), O read out and written at the segment's end
+//   warps 12 - 15 convert: queries to fp16 in tensor memory at a segment's start, then codes to fp16 operand tiles (exact),
+//                 once for both tiles, and scales to what the softmax wants of them
+//
+// A tile's S and its weights share 64 columns, so its two products and its softmax run one after the other; what fills the
+// tensor core and the softmax's pipes is the other tile. Tensor memory: Q 2 x 64 columns, S / P 2 x 64, O 2 x 128.
+//
+// Numerics as in kv8_stream.cuh, with kKtTop for kKv8Top: room for offsets that are not moved at every block.
+#pragma once
+#include "kv8.cuh"
+#include "kv8_plan.cuh"
+
+namespace msgl {
+
+constexpr int kKtRows = 256;
+constexpr int kKtThreads = 512;
+constexpr int kKtCost = 2;      // of a segment, in blocks
+constexpr int kKtDescs = 4;     // segments looked up ahead
+constexpr int kKtSlots = 4;     // of scales
+constexpr float kKtTop = 10.f;
+constexpr int kKtConv = 12, kKtSoft = 4;  // first warps of the converters and of the softmax
+
+struct KtDesc {
+  int q0, h, r0, nr, L, n, lo, kend, blk, nb, slot;  // nb 0: no more
+  int pad;
+};
+struct KtScales {
+  float ks[kKv8Block], lv[kKv8Block], vs[kKv8Block];
+};
+
+template <int HD>
+struct KtCfg {
+  static constexpr int kHalf = kKv8Block * 128;      // a block's 64 head dims as an fp16 operand
+  static constexpr int kTile = kHalf * (HD / 64);
+  static constexpr int kStages = 3;                  // of K and of V operands
+  static constexpr int kRaw = HD == 128 ? 6 : 8;     // of codes
+  static constexpr int kRawStage = 2 * kKv8Block * HD;
+  static constexpr int kRawScales = 2 * kKv8Block * 4;
+  static constexpr int kOffRaw = 2 * kStages * kTile;
+  static constexpr int kOffSc = kOffRaw + kRaw * kRawStage;
+  static constexpr int kOffSlots = kOffSc + kRaw * kRawScales;
+  static constexpr int kOffQs = kOffSlots + kKtSlots * (int)sizeof(KtScales);
+  static constexpr int kOffDesc = kOffQs + kKtDescs * kKtRows * 4;
+  static constexpr int kOffPlan = kOffDesc + kKtDescs * (int)sizeof(KtDesc);
+  static constexpr int kOffRed = kOffPlan + (int)sizeof(Kv8Plan);
+  static constexpr int kOffBars = kOffRed + 8 * (kKtThreads / 32);
+  static constexpr int kBars = 4 * kStages + 2 * kRaw + kKtSlots + 3 * kKtDescs + 2 + 4 * 2;
+  static constexpr int kSmem = 1024 + kOffBars + 8 * kBars + 16;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  // tensor memory columns
+  static constexpr int kQ = 0, kS = 128, kO = 256;
+};
+
+constexpr uint32_t kt_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }  // fp16 operands, fp32 sums
+
+// pairs of fp32 in one register pair
+MSGL_DEVICE uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+MSGL_DEVICE float2 f2_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// One block of one row: S from tensor memory, the running offset and sum, and the row's weights back. Returns what the
+// row's O has to be multiplied by first.
+template <bool MASKED>
+MSGL_DEVICE float kt_softmax(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end, float& m, float& l, uint32_t (&pk)[32]) {
+  uint64_t y[32];
+  {
+    uint32_t u[64];
+    tmem_ld_32x32b_x32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&u[0]));
+    tmem_ld_32x32b_x32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&u[32]));
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 64; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(&sc.ks[j]);
+      y[j / 2] = f2_mul(f2_pack(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), f2_pack(k.x, k.y));
+      y[j / 2 + 1] = f2_mul(f2_pack(__uint_as_float(u[j + 2]), __uint_as_float(u[j + 3])), f2_pack(k.z, k.w));
+    }
+  }
+  const uint64_t q2 = f2_pack(qs, qs);
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 64; j += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(&sc.lv[j]);
+    const float2 a = f2_unpack(f2_fma(y[j / 2], q2, f2_pack(v.x, v.y))), b = f2_unpack(f2_fma(y[j / 2 + 1], q2, f2_pack(v.z, v.w)));
+    const int i = j / 4 % 2 * 2;
+    if (MASKED) {
+      if (j >= first && j < end) mx[i] = fmaxf(mx[i], a.x);
+      if (j + 1 >= first && j + 1 < end) mx[i] = fmaxf(mx[i], a.y);
+      if (j + 2 >= first && j + 2 < end) mx[i + 1] = fmaxf(mx[i + 1], b.x);
+      if (j + 3 >= first && j + 3 < end) mx[i + 1] = fmaxf(mx[i + 1], b.y);
+    } else {
+      mx[i] = fmaxf(fmaxf(mx[i], a.x), a.y);
+      mx[i + 1] = fmaxf(fmaxf(mx[i + 1], b.x), b.y);
+    }
+  }
+  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  float alpha = 1.f;
+  if (top - m > 15.f) {  // (weights are at most 2^15; the first block moves the offset up from -inf)
+    alpha = kv8_exp2(m - (top - kKtTop));
+    m = top - kKtTop;
+    l *= alpha;
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  const uint64_t b2 = f2_pack(-base, -base);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 64; j += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(&sc.vs[j]);
+    float2 e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 x = f2_unpack(f2_fma(y[j / 2 + i], q2, b2));
+      e[i] = make_float2(kv8_exp2(x.x), kv8_exp2(x.y));
+      if (MASKED) {
+        const int c = j + 2 * i;
+        if (!(c >= first && c < end)) e[i].x = 0.f;
+        if (!(c + 1 >= first && c + 1 < end)) e[i].y = 0.f;
+      }
+      const uint64_t e2 = f2_pack(e[i].x, e[i].y);
+      sum[i] = f2_add(sum[i], e2);
+      float2 w = f2_unpack(f2_mul(e2, i ? f2_pack(v.z, v.w) : f2_pack(v.x, v.y)));
+      if (MASKED) {  // (a hidden key's weight is zero whatever its scale)
+        const int c = j + 2 * i;
+        if (!(c >= first && c < end)) w.x = 0.f;
+        if (!(c + 1 >= first && c + 1 < end)) w.y = 0.f;
+      }
+      pk[j / 2 + i] = pack_half(w.x, w.y);
+    }
+  }
+  const float2 a = f2_unpack(f2_add(sum[0], sum[1]));
+  l += a.x + a.y;
+  return alpha;
+}
+
+template <int HD, bool FP8>
+__global__ void __launch_bounds__(kKtThreads, 1)
+kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
+  using C = KtCfg<HD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::kStages * C::kTile;
+  uint8_t* raw = smem + C::kOffRaw;
+  float* raw_scales = reinterpret_cast<float*>(smem + C::kOffSc);
+  KtScales* slots = reinterpret_cast<KtScales*>(smem + C::kOffSlots);
+  float* qscale = reinterpret_cast<float*>(smem + C::kOffQs);  // [kKtDescs][256]
+  KtDesc* descs = reinterpret_cast<KtDesc*>(smem + C::kOffDesc);
+  Kv8Plan* plan = reinterpret_cast<Kv8Plan*>(smem + C::kOffPlan);
+  int64_t* red = reinterpret_cast<int64_t*>(smem + C::kOffRed);
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+  uint64_t* kempty = kfull + C::kStages;
+  uint64_t* vfull = kempty + C::kStages;
+  uint64_t* vempty = vfull + C::kStages;
+  uint64_t* rfull = vempty + C::kStages;
+  uint64_t* rempty = rfull + C::kRaw;
+  uint64_t* scfull = rempty + C::kRaw;
+  uint64_t* dfull = scfull + kKtSlots;
+  uint64_t* dempty = dfull + kKtDescs;
+  uint64_t* qsfull = dempty + kKtDescs;
+  uint64_t* qfull = qsfull + kKtDescs;
+  uint64_t* qempty = qfull + 1;
+  uint64_t* sfull = qempty + 1;  // [2]: a tile's S is there
+  uint64_t* pfull = sfull + 2;   // its weights are
+  uint64_t* pvdone = pfull + 2;  // O holds them, S's columns are free
+  uint64_t* ofree = pvdone + 2;  // O has been read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofree + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < C::kStages; ++i) {
+        mbar_init(&kfull[i], 4);
+        mbar_init(&kempty[i], 2);
+        mbar_init(&vfull[i], 4);
+        mbar_init(&vempty[i], 2);
+      }
+      for (int i = 0; i < C::kRaw; ++i) {
+        mbar_init(&rfull[i], 1);
+        mbar_init(&rempty[i], 4);
+      }
+      for (int i = 0; i < kKtSlots; ++i) mbar_init(&scfull[i], 4);
+      for (int i = 0; i < kKtDescs; ++i) {
+        mbar_init(&dfull[i], 1);
+        mbar_init(&dempty[i], 2 + 1 + 8 + 4);
+        mbar_init(&qsfull[i], 4);
+      }
+      mbar_init(qfull, 4);
+      mbar_init(qempty, 2);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pfull[i], 4);
+        mbar_init(&pvdone[i], 1);
+        mbar_init(&ofree[i], 4);
+      }
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tc);
+    prefetch_tmap(&ts);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
+  if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
+  kv8_plan<kKtRows, kKtCost, kKtThreads>(p, kKtCost + 2, plan, red);
+  const Kv8Plan pl = *plan;
+  const int G = p.nq / p.nkv;
+  kv8_zero_tail<HD>(p, threadIdx.x, kKtThreads);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ segments and copies
+    const int page = p.page, gpb = kKv8Block / page, mine = 32 / gpb;  // pages of a block, blocks whose slots the lanes hold
+    int b = pl.b, h = pl.h, t = pl.t, tiles = 0, i = 0;
+    uint32_t seq = 0;
+    int64_t u = pl.u0, s0 = pl.s0;
+    bool ok = true;
+    Kv8Req r = pl.r;
+    if (u < pl.u1) tiles = kv8_tiles<kKtRows>(r, G);
+    for (; ok && u < pl.u1; ++i) {
+      const Kv8Tile k = kv8_tile<kKtRows>(p, r, G, t);
+      // blocks [from, to) of the segment: its first kKtCost units are none
+      const int from = (int)max(u - s0 - kKtCost, (int64_t)0), to = (int)min((int64_t)k.nblk, pl.u1 - s0 - kKtCost);
+      if (to <= 0) break;  // (the run ends before the segment's first block)
+      const int d = i % kKtDescs;
+      if (lane == 0) {
+        ok = kv8_wait(&dempty[d], ((i / kKtDescs) & 1) ^ 1, 720);
+        if (ok) {
+          const bool starts = from == 0, ends = to == k.nblk;
+          KtDesc& D = descs[d];
+          D.q0 = r.q0; D.h = h; D.r0 = k.r0; D.nr = k.nr; D.L = r.L; D.n = r.n; D.lo = k.lo; D.kend = k.kend;
+          D.blk = k.blk0 + from; D.nb = to - from;
+          D.slot = starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
+          const int parts = starts && !ends ? kv8_cta_of(pl, s0 + kKtCost + k.nblk - 1) - (int)blockIdx.x + 1 : 0;
+          if (parts > 0) {  // (the run's last segment)
+            Kv8Part& hd = scratch.head[blockIdx.x];
+            hd.q0 = r.q0; hd.r0 = k.r0; hd.nr = k.nr; hd.h = h; hd.parts = parts;
+          }
+          mbar_arrive(&dfull[d]);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      // the blocks' pages' slots, a batch of `mine` blocks ahead
+      const int page0 = (k.blk0 + from) * gpb, pages_end = k.kend > k.lo ? (k.kend - 1) / page + 1 : 0;
+      auto look_up = [&](int j) {
+        const int g = page0 + j * gpb + lane;
+        return g < pages_end && j + lane / gpb < to - from ? p.page_table[(int64_t)r.row * p.pt_stride + (int64_t)g * page] : -1;
+      };
+      int next = look_up(0), page_slots = -1;
+      for (int j = 0; j < to - from; ++j) {
+        if (j % mine == 0) {
+          page_slots = next;
+          if (page0 + j * gpb + lane < pages_end && j + lane / gpb < to - from) page_slots = kv8_checked(p, page_slots);
+          if (j + mine < to - from) next = look_up(j + mine);
+        }
+        const uint32_t x = seq + j, stage = x % C::kRaw;
+        if (lane == 0) ok = kv8_wait(&rempty[stage], ((x / C::kRaw) & 1) ^ 1, 721);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          seq = x;
+          break;
+        }
+        const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
+        kv8_copy_block<HD>(p, &tc, &ts, raw + stage * C::kRawStage, raw_scales + stage * (C::kRawScales / 4), &rfull[stage], h, page_slots,
+                           j % mine * gpb, pages, lane);
+      }
+      if (!ok) break;
+      seq += to - from;
+      u = s0 + kKtCost + to;
+      s0 += kKtCost + k.nblk;
+      if (u < pl.u1 && ++t == tiles) {
+        t = 0;
+        if (++h == p.nkv) {
+          h = 0;
+          do {
+            if (++b >= p.num_reqs) break;  // (never: units are left)
+            r = kv8_request(p, b);
+            tiles = kv8_tiles<kKtRows>(r, G);
+          } while (tiles == 0);
+          if (b >= p.num_reqs) u = pl.u1;
+        }
+      }
+    }
+    if (lane == 0) {
+      if (ok) {
+        if (kv8_wait(&dempty[i % kKtDescs], ((i / kKtDescs) & 1) ^ 1, 722)) {
+          descs[i % kKtDescs].nb = 0;
+          mbar_arrive(&dfull[i % kKtDescs]);
+        }
+      } else {  // given up (and recorded): the copies in flight land before the CTA's memory goes
+        for (uint32_t n = 1; n <= min(seq, (uint32_t)C::kRaw); ++n) {
+          const uint32_t x = seq - n;
+          kv8_wait(&rfull[x % C::kRaw], (x / C::kRaw) & 1, 723);
+        }
+      }
+    }
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ products of one tile
+    if (lane == 0) {
+      const int x = warp - 1;
+      const uint32_t tq = tmem + C::kQ + x * 64, tsx = tmem + C::kS + x * 64, to = tmem + C::kO + x * 128;
+      constexpr uint32_t idesc_s = kt_idesc(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
+      uint32_t g = 0, uses = 0, outs = 0;  // blocks gone through, of them this tile's, segments of this tile's
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const int d = i % kKtDescs;
+        if (!kv8_wait(&dfull[d], (i / kKtDescs) & 1, 730)) break;
+        const int nb = descs[d].nb;
+        const bool active = descs[d].nr > 128 * x;
+        if (nb == 0) break;
+        if (!(ok = kv8_wait(qfull, i & 1, 731))) break;
+        if (!active) mbar_arrive(qempty);
+        tc_fence_after();
+        for (int j = 0; j < nb; ++j, ++g) {
+          const uint32_t st = g % C::kStages, ph = (g / C::kStages) & 1;
+          if (!(ok = kv8_wait(&kfull[st], ph, 732))) break;
+          if (active) {
+            if (uses > 0 && !(ok = kv8_wait(&pvdone[x], (uses - 1) & 1, 733))) break;  // S's columns
+            tc_fence_after();
+            const uint32_t k = smem_u32(sK + st * C::kTile);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              tc_mma_f16_ts(tsx, tq + kk * 8, smem_desc_sw128(k + (kk >> 2) * C::kHalf + (kk & 3) * 32), idesc_s, kk > 0);
+            tc_commit(&kempty[st]);
+            tc_commit(&sfull[x]);
+            if (j == nb - 1) tc_commit(qempty);
+            if (!(ok = kv8_wait(&vfull[st], ph, 734))) break;
+            if (j == 0 && outs > 0 && !(ok = kv8_wait(&ofree[x], (outs - 1) & 1, 735))) break;
+            if (!(ok = kv8_wait(&pfull[x], uses & 1, 736))) break;
+            tc_fence_after();
+            const uint32_t v = smem_u32(sV + st * C::kTile);
+#pragma unroll
+            for (int kk = 0; kk < kKv8Block / 16; ++kk)
+              tc_mma_f16_ts(to, tsx + kk * 8, smem_desc_sw128_mn(v + kk * 16 * 128, C::kHalf), idesc_o, j > 0 || kk > 0);
+            tc_commit(&vempty[st]);
+            tc_commit(&pvdone[x]);
+            ++uses;
+          } else {
+            mbar_arrive(&kempty[st]);
+            if (!(ok = kv8_wait(&vfull[st], ph, 737))) break;
+            mbar_arrive(&vempty[st]);
+          }
+        }
+        if (!ok) break;
+        if (active) ++outs;
+        mbar_arrive(&dempty[d]);
+      }
+      // (on giving up, too: no product is in flight when the CTA's memories go)
+      if (!ok) kv8_wait(&sfull[x], uses & 1, 739);
+      if (uses > 0) kv8_wait(&pvdone[x], (uses - 1) & 1, 738);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ queries into the L2 cache
+    for (int i = 0;; ++i) {
+      const int d = i % kKtDescs;
+      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 740)) break;
+      const KtDesc D = descs[d];
+      if (D.nb == 0) break;
+      for (int rr = lane; rr < D.nr; rr += 32) {
+        const int r = D.r0 + rr, tok = r / G;
+        const char* src = reinterpret_cast<const char*>(p.q) + 2 * ((D.q0 + tok) * p.q_row + (int64_t)(D.h * G + r - tok * G) * p.q_head);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+        if (HD == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 128));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&dempty[d]);
+    }
+  } else if (warp < kKtConv) {
+    // ------------------------------------------------------------------ softmax
+    const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tsx = tmem + C::kS + x * 64 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
+    uint32_t g = 0, uses = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const int d = i % kKtDescs;
+      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 750)) break;
+      const KtDesc D = descs[d];
+      if (D.nb == 0) break;
+      const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
+      const bool in = rr < D.nr;
+      if (D.nr <= 128 * x) {
+        g += D.nb;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dempty[d]);
+        continue;
+      }
+      if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1, 751))) break;
+      const float qs = qscale[d * kKtRows + rr];
+      const int qpos = D.L - D.n + tok;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < D.nb; ++j, ++g) {
+        // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
+        if (!(ok = kv8_wait_warp(&sfull[x], uses & 1, 752))) break;
+        if (!(ok = kv8_wait_warp(&scfull[g % kKtSlots], (g / kKtSlots) & 1, 753))) break;
+        tc_fence_after();
+        const KtScales& sc = slots[g % kKtSlots];
+        // the keys of this block that the row sees: [first, end)
+        const int k0 = (D.blk + j) * kKv8Block;
+        const int first = p.window > 0 ? max(0, qpos - p.window + 1 - k0) : 0, end = min(qpos + 1 - k0, kKv8Block);
+        uint32_t pk[32];
+        float alpha;
+        if (__any_sync(0xffffffffu, in && (first > 0 || end < kKv8Block)))
+          alpha = kt_softmax<true>(tsx, sc, qs, in ? first : 0, in ? end : 0, m, l, pk);
+        else
+          alpha = kt_softmax<false>(tsx, sc, qs, 0, 0, m, l, pk);
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // (S of this block waited for O to hold the ones before)
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(to + c * 32, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+            tmem_st_32x32b_x32(to + c * 32, v);
+          }
+        }
+        tmem_st_32x32b_x32(tsx, pk);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[x]);
+        ++uses;
+      }
+      if (!ok) break;
+      // O out of tensor memory, 32 head dims at a time
+      if (!(ok = kv8_wait_warp(&pvdone[x], (uses - 1) & 1, 754))) break;
+      tc_fence_after();
+      const int head = D.h * G + r - tok * G;
+      const float f = D.slot < 0 ? kv8_norm(m, l, p.sinks, in ? head : 0) : 1.f;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(to + c * 32, v);
+        tc_wait_ld();
+        if (c == HD / 32 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ofree[x]);
+        }
+        if (in && D.slot < 0) {
+          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.o) + ((int64_t)(D.q0 + tok) * p.nq + head) * HD + c * 32);
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            dst[k / 8] = make_uint4(pack_bf16(__uint_as_float(v[k]) * f, __uint_as_float(v[k + 1]) * f),
+                                    pack_bf16(__uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 3]) * f),
+                                    pack_bf16(__uint_as_float(v[k + 4]) * f, __uint_as_float(v[k + 5]) * f),
+                                    pack_bf16(__uint_as_float(v[k + 6]) * f, __uint_as_float(v[k + 7]) * f));
+        } else if (in) {
+          uint4* dst = reinterpret_cast<uint4*>(scratch.o + ((int64_t)D.slot * kKtRows + rr) * HD + c * 32);
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) dst[k / 4] = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        }
+      }
+      if (in && D.slot >= 0) scratch.ml[(int64_t)D.slot * kKtRows + rr] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&dempty[d]);
+    }
+  } else {
+    // ------------------------------------------------------------------ conversions
+    const int w = warp - kKtConv, row = w * 32 + lane;
+    const uint32_t tq = tmem + C::kQ + ((uint32_t)(w * 32) << 16);
+    // Codes: a warp takes 8 keys x 64 head dims at a time, 16 a lane, so that neither its loads nor its stores of 16
+    // bytes meet in a bank: of every 8 lanes 4 have key k, the others key k ^ 5.
+    const int part = lane & 3, key8 = (lane >> 3) ^ (lane & 4 ? 5 : 0);
+    uint32_t g = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const int d = i % kKtDescs;
+      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 760)) break;
+      const KtDesc D = descs[d];
+      if (D.nb == 0) break;
+      // queries: a thread takes its row of both tiles
+      for (int x = 0; x < 2; ++x) {
+        const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
+        uint4 u[HD / 8];
+        if (rr < D.nr) {
+          const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (D.q0 + tok) * p.q_row +
+                                                            (int64_t)(D.h * G + r - tok * G) * p.q_head);
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) u[c] = __ldg(src + c);
+        } else {
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) u[c] = make_uint4(0, 0, 0, 0);
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c)
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[c].x & 0x7fff7fffu, u[c].y & 0x7fff7fffu), __vmaxu2(u[c].z & 0x7fff7fffu, u[c].w & 0x7fff7fffu)));
+        top = max(top & 0xffffu, top >> 16);
+        const float f = kv8_q_factor(__uint_as_float(top << 16));
+        qscale[d * kKtRows + rr] = p.scale * kKv8Log2e * kv8_reciprocal(f);
+        if (x == 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&qsfull[d]);
+        }
+        // Q's columns are free once the last segment's products with keys are done
+        if (x == 0 && i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1, 761))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+          uint32_t v[32];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t e[4] = {u[8 * c + k].x, u[8 * c + k].y, u[8 * c + k].z, u[8 * c + k].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[4 * k + y] = pack_half(bf16_lo(e[y]) * f, bf16_hi(e[y]) * f);
+          }
+          tmem_st_32x32b_x32(tq + x * 64 + c * 32, v);
+        }
+      }
+      if (!ok) break;
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qfull);
+
+      for (int j = 0; j < D.nb; ++j, ++g) {
+        const uint32_t rs = g % C::kRaw, st = g % C::kStages, ph = (g / C::kStages) & 1;
+        if (!(ok = kv8_wait_warp(&rfull[rs], (g / C::kRaw) & 1, 762))) break;
+        const int k0 = (D.blk + j) * kKv8Block;
+        const bool partial = k0 < D.lo || k0 + kKv8Block > D.kend;  // some of the keys may be no positions
+        const uint8_t* src = raw + rs * C::kRawStage;
+        auto convert = [&](uint8_t* dst, int which) {
+          // groups of 8 keys, w and w + 4 of them this warp's, and of 64 head dims
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int grp = w + 4 * y, key = grp * 8 + key8;
+            const int at = key + (key & ~(p.page - 1)) + which * p.page;  // row of the page's two parts
+            const bool none = partial && (k0 + key < D.lo || k0 + key >= D.kend);
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {
+              uint4 v = *reinterpret_cast<const uint4*>(src + at * HD + (HD == 128 ? ((c * 4 + part) ^ (key8 & 7)) << 4 : (part ^ ((key8 >> 1) & 3)) << 4));
+              if (none) v = make_uint4(0, 0, 0, 0);
+              uint4 a, b;
+              kv8_to_half<FP8>(v.x, a.x, a.y);
+              kv8_to_half<FP8>(v.y, a.z, a.w);
+              kv8_to_half<FP8>(v.z, b.x, b.y);
+              kv8_to_half<FP8>(v.w, b.z, b.w);
+              uint8_t* o = dst + c * C::kHalf + key * 128;
+              *reinterpret_cast<uint4*>(o + (((2 * part) ^ key8) << 4)) = a;
+              *reinterpret_cast<uint4*>(o + (((2 * part + 1) ^ key8) << 4)) = b;
+            }
+          }
+          fence_async_smem();
+        };
+        if (!(ok = kv8_wait_warp(&kempty[st], ph ^ 1, 763))) break;
+        convert(sK + st * C::kTile, order.codes);
+        // scales: what used this slot before was over when its keys' products were
+        if (row < kKv8Block) {
+          const float* sc = raw_scales + rs * (C::kRawScales / 4) + row + (row & ~(p.page - 1));
+          const bool none = partial && (k0 + row < D.lo || k0 + row >= D.kend);
+          const float ks = none ? 0.f : sc[order.scales * p.page], vs = none ? 0.f : sc[(order.scales ^ 1) * p.page];
+          KtScales& s = slots[g % kKtSlots];
+          s.ks[row] = ks;
+          s.vs[row] = vs;
+          s.lv[row] = kv8_log_scale(vs);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&kfull[st]);
+          mbar_arrive(&scfull[g % kKtSlots]);
+        }
+        if (!(ok = kv8_wait_warp(&vempty[st], ph ^ 1, 764))) break;
+        convert(sV + st * C::kTile, order.codes ^ 1);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&vfull[st]);
+          mbar_arrive(&rempty[rs]);
+        }
+      }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&dempty[d]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace msgl
