@@ -77,6 +77,12 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
   using C = KtCfg<HD>;
   constexpr auto kernel = kv8_tiles_kernel<HD, FP8>;
   if (msgl_set_smem<kernel>(C::kSmem) != cudaSuccess) return 4;
+  // (the roles' registers have to fit the launch's, or a warp would wait for more of them for good)
+  static const bool fits = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs >= kKtRegs;
+  }();
+  if (!fits) return 4;
   CUtensorMap tc, ts;
   Kv8Order order;
   if (!encode_cache(&tc, &ts, &order, p, HD)) return 2;

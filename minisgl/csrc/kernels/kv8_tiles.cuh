@@ -29,6 +29,13 @@ constexpr int kKtDescs = 4;     // segments looked up ahead
 constexpr int kKtSlots = 4;     // of scales
 constexpr float kKtTop = 10.f;
 constexpr int kKtConv = 12, kKtSoft = 4;  // first warps of the converters and of the softmax
+// registers of a thread in warps 0 - 3, the softmax and the converters: of the launch's 4 x 128 a row of warps
+constexpr int kKtRegs = 128, kKtRegsFew = 72, kKtRegsSoft = 168, kKtRegsConv = 104;
+static_assert(kKtRegsFew + 2 * kKtRegsSoft + kKtRegsConv <= 4 * kKtRegs, "more registers than the launch has");
+template <int N>
+MSGL_DEVICE void kt_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+MSGL_DEVICE void kt_more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 struct KtDesc {
   int q0, h, r0, nr, L, n, lo, kend, blk, nb, slot;  // nb 0: no more
@@ -90,76 +97,86 @@ MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// One block of one row: S from tensor memory, the running offset and sum, and the row's weights back. Returns what the
-// row's O has to be multiplied by first.
+// The offset that a row needs for one block's weights to be at most 2^kKtTop (see kKv8Top).
 template <bool MASKED>
-MSGL_DEVICE float kt_softmax(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end, float& m, float& l, uint32_t (&pk)[32]) {
-  uint64_t y[32];
-  {
-    uint32_t u[64];
-    tmem_ld_32x32b_x32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(&u[0]));
-    tmem_ld_32x32b_x32(s_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&u[32]));
+MSGL_DEVICE float kt_offset(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kKv8Block; c += 32) {
+    uint32_t u[32];
+    tmem_ld_32x32b_x32(s_tmem + c, u);
     tc_wait_ld();
 #pragma unroll
-    for (int j = 0; j < 64; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(&sc.ks[j]);
-      y[j / 2] = f2_mul(f2_pack(__uint_as_float(u[j]), __uint_as_float(u[j + 1])), f2_pack(k.x, k.y));
-      y[j / 2 + 1] = f2_mul(f2_pack(__uint_as_float(u[j + 2]), __uint_as_float(u[j + 3])), f2_pack(k.z, k.w));
-    }
+    for (int j = 0; j < 32; ++j)
+      if (!MASKED || (c + j >= first && c + j < end)) top = fmaxf(top, fmaf(__uint_as_float(u[j]) * sc.ks[c + j], qs, sc.lv[c + j]));
   }
-  const uint64_t q2 = f2_pack(qs, qs);
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int j = 0; j < 64; j += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(&sc.lv[j]);
-    const float2 a = f2_unpack(f2_fma(y[j / 2], q2, f2_pack(v.x, v.y))), b = f2_unpack(f2_fma(y[j / 2 + 1], q2, f2_pack(v.z, v.w)));
-    const int i = j / 4 % 2 * 2;
-    if (MASKED) {
-      if (j >= first && j < end) mx[i] = fmaxf(mx[i], a.x);
-      if (j + 1 >= first && j + 1 < end) mx[i] = fmaxf(mx[i], a.y);
-      if (j + 2 >= first && j + 2 < end) mx[i + 1] = fmaxf(mx[i + 1], b.x);
-      if (j + 3 >= first && j + 3 < end) mx[i + 1] = fmaxf(mx[i + 1], b.y);
-    } else {
-      mx[i] = fmaxf(fmaxf(mx[i], a.x), a.y);
-      mx[i + 1] = fmaxf(fmaxf(mx[i + 1], b.x), b.y);
-    }
-  }
-  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  float alpha = 1.f;
-  if (top - m > 15.f) {  // (weights are at most 2^15; the first block moves the offset up from -inf)
-    alpha = kv8_exp2(m - (top - kKtTop));
-    m = top - kKtTop;
-    l *= alpha;
-  }
+  return top - kKtTop;
+}
+
+// One block of one row with offset m: S from tensor memory, its weights as fp16 pairs. Returns the sum of 2^(s_j - m), and in
+// `top` the largest weight.
+template <bool MASKED>
+MSGL_DEVICE float kt_weights(uint32_t s_tmem, const KtScales& sc, float qs, float m, int first, int end, float& top, uint32_t (&pk)[32]) {
   const float base = m == -INFINITY ? 0.f : m;
-  const uint64_t b2 = f2_pack(-base, -base);
+  const uint64_t q2 = f2_pack(qs, qs), b2 = f2_pack(-base, -base);
   uint64_t sum[2] = {0, 0};
+  float mx[2] = {0.f, 0.f};
+  uint32_t u[2][32];
+  tmem_ld_32x32b_x32(s_tmem, u[0]);
+  tmem_ld_32x32b_x32(s_tmem + 32, u[1]);
+  tc_wait_ld();
 #pragma unroll
-  for (int j = 0; j < 64; j += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(&sc.vs[j]);
-    float2 e[2];
+  for (int j = 0; j < kKv8Block; j += 4) {
+    const float4 k = *reinterpret_cast<const float4*>(&sc.ks[j]), v = *reinterpret_cast<const float4*>(&sc.vs[j]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float2 x = f2_unpack(f2_fma(y[j / 2 + i], q2, b2));
-      e[i] = make_float2(kv8_exp2(x.x), kv8_exp2(x.y));
+      const int c = j + 2 * i;
+      const uint64_t y = f2_mul(f2_pack(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1])),
+                                i ? f2_pack(k.z, k.w) : f2_pack(k.x, k.y));
+      const float2 x = f2_unpack(f2_fma(y, q2, b2));
+      float2 e = make_float2(kv8_exp2(x.x), kv8_exp2(x.y));
       if (MASKED) {
-        const int c = j + 2 * i;
-        if (!(c >= first && c < end)) e[i].x = 0.f;
-        if (!(c + 1 >= first && c + 1 < end)) e[i].y = 0.f;
+        if (!(c >= first && c < end)) e.x = 0.f;
+        if (!(c + 1 >= first && c + 1 < end)) e.y = 0.f;
       }
-      const uint64_t e2 = f2_pack(e[i].x, e[i].y);
+      const uint64_t e2 = f2_pack(e.x, e.y);
       sum[i] = f2_add(sum[i], e2);
       float2 w = f2_unpack(f2_mul(e2, i ? f2_pack(v.z, v.w) : f2_pack(v.x, v.y)));
       if (MASKED) {  // (a hidden key's weight is zero whatever its scale)
-        const int c = j + 2 * i;
         if (!(c >= first && c < end)) w.x = 0.f;
         if (!(c + 1 >= first && c + 1 < end)) w.y = 0.f;
       }
-      pk[j / 2 + i] = pack_half(w.x, w.y);
+      mx[i] = fmaxf(fmaxf(mx[i], w.x), w.y);
+      pk[c / 2] = pack_half(w.x, w.y);
     }
   }
+  top = fmaxf(mx[0], mx[1]);
   const float2 a = f2_unpack(f2_add(sum[0], sum[1]));
-  l += a.x + a.y;
+  return a.x + a.y;
+}
+
+// A row's block: its weights, with a new offset first if there is none yet, or if with the old one a weight is beyond 2^15 or
+// the sum beyond 2^108 (keys whose values are nearly nothing). Few blocks need one, and the others are spared the maximum
+// of their logits. Returns what the row's O has to be multiplied by.
+template <bool MASKED>
+MSGL_DEVICE float kt_softmax(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end, float& m, float& l,
+                             uint32_t (&pk)[32]) {
+  float alpha = 1.f, sum = 0.f, top = 0.f;
+  bool move = m == -INFINITY;  // (the row has seen no key yet)
+  if (!__all_sync(0xffffffffu, move)) {
+    sum = kt_weights<MASKED>(s_tmem, sc, qs, m, first, end, top, pk);
+    move |= !(top <= 32768.f && sum <= 0x1p+108f);
+  }
+  if (__any_sync(0xffffffffu, move)) {
+    const float to = kt_offset<MASKED>(s_tmem, sc, qs, first, end);
+    if (move && to > m) {
+      alpha = kv8_exp2(m - to);
+      m = to;
+      l *= alpha;
+    }
+    sum = kt_weights<MASKED>(s_tmem, sc, qs, m, first, end, top, pk);
+  }
+  l += sum;
   return alpha;
 }
 
@@ -246,6 +263,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------------------------------------------ segments and copies
+    kt_fewer_regs<kKtRegsFew>();
     const int page = p.page, gpb = kKv8Block / page, mine = 32 / gpb;  // pages of a block, blocks whose slots the lanes hold
     int b = pl.b, h = pl.h, t = pl.t, tiles = 0, i = 0;
     uint32_t seq = 0;
@@ -333,6 +351,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     }
   } else if (warp <= 2) {
     // ------------------------------------------------------------------ products of one tile
+    kt_fewer_regs<kKtRegsFew>();
     if (lane == 0) {
       const int x = warp - 1;
       const uint32_t tq = tmem + C::kQ + x * 64, tsx = tmem + C::kS + x * 64, to = tmem + C::kO + x * 128;
@@ -354,10 +373,11 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           if (active) {
             if (uses > 0 && !(ok = kv8_wait(&pvdone[x], (uses - 1) & 1, 733))) break;  // S's columns
             tc_fence_after();
-            const uint32_t k = smem_u32(sK + st * C::kTile);
+            // (a descriptor's low bits are its address / 16)
+            const uint64_t k = smem_desc_sw128(smem_u32(sK + st * C::kTile));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
-              tc_mma_f16_ts(tsx, tq + kk * 8, smem_desc_sw128(k + (kk >> 2) * C::kHalf + (kk & 3) * 32), idesc_s, kk > 0);
+              tc_mma_f16_ts(tsx, tq + kk * 8, k + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
             tc_commit(&kempty[st]);
             tc_commit(&sfull[x]);
             if (j == nb - 1) tc_commit(qempty);
@@ -365,10 +385,10 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
             if (j == 0 && outs > 0 && !(ok = kv8_wait(&ofree[x], (outs - 1) & 1, 735))) break;
             if (!(ok = kv8_wait(&pfull[x], uses & 1, 736))) break;
             tc_fence_after();
-            const uint32_t v = smem_u32(sV + st * C::kTile);
+            const uint64_t v = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
 #pragma unroll
             for (int kk = 0; kk < kKv8Block / 16; ++kk)
-              tc_mma_f16_ts(to, tsx + kk * 8, smem_desc_sw128_mn(v + kk * 16 * 128, C::kHalf), idesc_o, j > 0 || kk > 0);
+              tc_mma_f16_ts(to, tsx + kk * 8, v + (kk * 16 * 128 >> 4), idesc_o, j > 0 || kk > 0);
             tc_commit(&vempty[st]);
             tc_commit(&pvdone[x]);
             ++uses;
@@ -388,6 +408,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------------ queries into the L2 cache
+    kt_fewer_regs<kKtRegsFew>();
     for (int i = 0;; ++i) {
       const int d = i % kKtDescs;
       if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 740)) break;
@@ -404,6 +425,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     }
   } else if (warp < kKtConv) {
     // ------------------------------------------------------------------ softmax
+    kt_more_regs<kKtRegsSoft>();
     const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tsx = tmem + C::kS + x * 64 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
@@ -425,7 +447,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1, 751))) break;
       const float qs = qscale[d * kKtRows + rr];
       const int qpos = D.L - D.n + tok;
-      float m = -INFINITY, l = 0.f;
+      float m = in ? -INFINITY : 0.f, l = 0.f;
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
         if (!(ok = kv8_wait_warp(&sfull[x], uses & 1, 752))) break;
@@ -495,6 +517,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     }
   } else {
     // ------------------------------------------------------------------ conversions
+    kt_fewer_regs<kKtRegsConv>();
     const int w = warp - kKtConv, row = w * 32 + lane;
     const uint32_t tq = tmem + C::kQ + ((uint32_t)(w * 32) << 16);
     // Codes: a warp takes 8 keys x 64 head dims at a time, 16 a lane, so that neither its loads nor its stores of 16
