@@ -7,7 +7,7 @@
 //   warps 1, 2    issue the products of one tile each: S = Q K^T, then, once the weights are there, O += P V. Q and P are read
 //                 from tensor memory and K, V from shared memory, whose bandwidth is what all of this comes close to.
 //   warp 3        fetches the next segments' queries into the L2 cache
-//   warps 4 - 11  softmax, one thread per row: S out of tensor memory, weights as fp16 over S's columns, O rescaled there
+//   warps 4 - 11  softmax, 32 rows a warp, four rows and 16 keys a lane: S out of tensor memory, weights as fp16 over S's columns, O rescaled there
 //                 when a row's offset grows by more than 2^(15 - kKtTop), O read out and written at the segment's end
 //   warps 12 - 15 convert: queries to fp16 in tensor memory at a segment's start, then codes to fp16 operand tiles (exact),
 //                 once for both tiles, and scales to what the softmax wants of them
@@ -20,6 +20,8 @@
 #include "kv8.cuh"
 #include "kv8_plan.cuh"
 
+#include <limits.h>
+
 namespace msgl {
 
 constexpr int kKtRows = 256;
@@ -30,7 +32,7 @@ constexpr int kKtSlots = 4;     // of scales
 constexpr float kKtTop = 10.f;
 constexpr int kKtConv = 12, kKtSoft = 4;  // first warps of the converters and of the softmax
 // registers of a thread in warps 0 - 3, the softmax and the converters: of the launch's 4 x 128 a row of warps
-constexpr int kKtRegs = 128, kKtRegsFew = 72, kKtRegsSoft = 168, kKtRegsConv = 104;
+constexpr int kKtRegs = 128, kKtRegsFew = 64, kKtRegsSoft = 176, kKtRegsConv = 96;
 static_assert(kKtRegsFew + 2 * kKtRegsSoft + kKtRegsConv <= 4 * kKtRegs, "more registers than the launch has");
 template <int N>
 MSGL_DEVICE void kt_fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -97,87 +99,146 @@ MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// The offset that a row needs for one block's weights to be at most 2^kKtTop (see kKv8Top).
-template <bool MASKED>
-MSGL_DEVICE float kt_offset(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end) {
-  float top = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < kKv8Block; c += 32) {
-    uint32_t u[32];
-    tmem_ld_32x32b_x32(s_tmem + c, u);
-    tc_wait_ld();
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (!MASKED || (c + j >= first && c + j < end)) top = fmaxf(top, fmaf(__uint_as_float(u[j]) * sc.ks[c + j], qs, sc.lv[c + j]));
-  }
-  return top - kKtTop;
+// 16 lanes x 64 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
+// (registers 4n, 4n + 1) and g + 8 (4n + 2, 4n + 3) the columns 8n + 2t and the next.
+MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// 16 lanes x 32 columns in the same order: lane (g, t) holds column 4n + t of rows g (register 2n) and g + 8 (2n + 1): fp16
+// pairs of those S.
+MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
-// One block of one row with offset m: S from tensor memory, its weights as fp16 pairs. Returns the sum of 2^(s_j - m), and in
-// `top` the largest weight.
+// Two of a lane's four rows (rows g and g + 8 of 16): their queries' factors, running offsets and this lane's part of their
+// sums, the keys of the block that they see, [first, end), and what their O has to be multiplied by first.
+struct KtRows {
+  float qs[2], m[2], l[2], alpha[2];
+  int first[2], end[2];
+};
+
+// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one.
 template <bool MASKED>
-MSGL_DEVICE float kt_weights(uint32_t s_tmem, const KtScales& sc, float qs, float m, int first, int end, float& top, uint32_t (&pk)[32]) {
-  const float base = m == -INFINITY ? 0.f : m;
-  const uint64_t q2 = f2_pack(qs, qs), b2 = f2_pack(-base, -base);
-  uint64_t sum[2] = {0, 0};
-  float mx[2] = {0.f, 0.f};
-  uint32_t u[2][32];
-  tmem_ld_32x32b_x32(s_tmem, u[0]);
-  tmem_ld_32x32b_x32(s_tmem + 32, u[1]);
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
+  uint32_t u[32];
+  kt_load_s(s_tmem, u);
   tc_wait_ld();
 #pragma unroll
-  for (int j = 0; j < kKv8Block; j += 4) {
-    const float4 k = *reinterpret_cast<const float4*>(&sc.ks[j]), v = *reinterpret_cast<const float4*>(&sc.vs[j]);
+  for (int k = 0; k < 2; ++k) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = j + 2 * i;
-      const uint64_t y = f2_mul(f2_pack(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1])),
-                                i ? f2_pack(k.z, k.w) : f2_pack(k.x, k.y));
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = 8 * n + 2 * t + e;
+        const float x = fmaf(__uint_as_float(u[4 * n + 2 * k + e]) * sc.ks[c], w.qs[k], sc.lv[c]);
+        if (!MASKED || (c >= w.first[k] && c < w.end[k])) top = fmaxf(top, x);
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - kKtTop;
+    if (top > w.m[k]) {
+      const float f = kv8_exp2(w.m[k] - top);
+      w.m[k] = top;
+      w.l[k] *= f;
+      w.alpha[k] *= f;
+    }
+  }
+}
+
+// A block's weights of two rows, as fp16 pairs, with the offsets as they are. `sum`: this lane's sums of 2^(s_j - m). Returns
+// whether a weight is beyond 2^15, or a sum beyond 2^108.
+template <bool MASKED>
+MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const uint64_t (&ks)[8], const uint64_t (&vs)[8], const KtRows& w, int t, float (&sum)[2],
+                            uint32_t (&pk)[16]) {
+  uint32_t u[32];
+  kt_load_s(s_tmem, u);
+  tc_wait_ld();
+  bool beyond = false;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
+    const uint64_t q2 = f2_pack(w.qs[k], w.qs[k]), b2 = f2_pack(-base, -base);
+    uint64_t total = 0;
+    float top = 0.f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int c = 8 * n + 2 * t;
+      const uint64_t y = f2_mul(f2_pack(__uint_as_float(u[4 * n + 2 * k]), __uint_as_float(u[4 * n + 2 * k + 1])), ks[n]);
       const float2 x = f2_unpack(f2_fma(y, q2, b2));
       float2 e = make_float2(kv8_exp2(x.x), kv8_exp2(x.y));
       if (MASKED) {
-        if (!(c >= first && c < end)) e.x = 0.f;
-        if (!(c + 1 >= first && c + 1 < end)) e.y = 0.f;
+        if (!(c >= w.first[k] && c < w.end[k])) e.x = 0.f;
+        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) e.y = 0.f;
       }
       const uint64_t e2 = f2_pack(e.x, e.y);
-      sum[i] = f2_add(sum[i], e2);
-      float2 w = f2_unpack(f2_mul(e2, i ? f2_pack(v.z, v.w) : f2_pack(v.x, v.y)));
+      total = f2_add(total, e2);
+      float2 v = f2_unpack(f2_mul(e2, vs[n]));
       if (MASKED) {  // (a hidden key's weight is zero whatever its scale)
-        if (!(c >= first && c < end)) w.x = 0.f;
-        if (!(c + 1 >= first && c + 1 < end)) w.y = 0.f;
+        if (!(c >= w.first[k] && c < w.end[k])) v.x = 0.f;
+        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) v.y = 0.f;
       }
-      mx[i] = fmaxf(fmaxf(mx[i], w.x), w.y);
-      pk[c / 2] = pack_half(w.x, w.y);
+      top = fmaxf(fmaxf(top, v.x), v.y);
+      pk[2 * n + k] = pack_half(v.x, v.y);
     }
+    const float2 a = f2_unpack(total);
+    sum[k] = a.x + a.y;
+    beyond |= !(top <= 32768.f && sum[k] <= 0x1p+108f);
   }
-  top = fmaxf(mx[0], mx[1]);
-  const float2 a = f2_unpack(f2_add(sum[0], sum[1]));
-  return a.x + a.y;
+  return beyond;
 }
 
-// A row's block: its weights, with a new offset first if there is none yet, or if with the old one a weight is beyond 2^15 or
-// the sum beyond 2^108 (keys whose values are nearly nothing). Few blocks need one, and the others are spared the maximum
-// of their logits. Returns what the row's O has to be multiplied by.
+// A block of the lane's rows: their weights over S's columns. New offsets first for rows that have none (they have seen no
+// key) or have weights beyond fp16, sums beyond 2^108 (keys whose values are nearly nothing): few blocks need any, and the
+// others are spared the maximum of their logits. Returns whether any of the warp's rows has a new one. (Loops that are not
+// unrolled: five roles' code has to fit the instruction cache.)
 template <bool MASKED>
-MSGL_DEVICE float kt_softmax(uint32_t s_tmem, const KtScales& sc, float qs, int first, int end, float& m, float& l,
-                             uint32_t (&pk)[32]) {
-  float alpha = 1.f, sum = 0.f, top = 0.f;
-  bool move = m == -INFINITY;  // (the row has seen no key yet)
-  if (!__all_sync(0xffffffffu, move)) {
-    sum = kt_weights<MASKED>(s_tmem, sc, qs, m, first, end, top, pk);
-    move |= !(top <= 32768.f && sum <= 0x1p+108f);
+MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& lo, KtRows& hi, int t) {
+  uint64_t ks[8], vs[8];
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    ks[n] = *reinterpret_cast<const uint64_t*>(&sc.ks[8 * n + 2 * t]);
+    vs[n] = *reinterpret_cast<const uint64_t*>(&sc.vs[8 * n + 2 * t]);
   }
-  if (__any_sync(0xffffffffu, move)) {
-    const float to = kt_offset<MASKED>(s_tmem, sc, qs, first, end);
-    if (move && to > m) {
-      alpha = kv8_exp2(m - to);
-      m = to;
-      l *= alpha;
+  bool any = false;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    float sum[2];
+    uint32_t pk[16];
+    bool moved = false;
+    lo.alpha[0] = lo.alpha[1] = 1.f;
+#pragma unroll 1
+    for (bool again = __any_sync(0xffffffffu, lo.m[0] == -INFINITY || lo.m[1] == -INFINITY);;) {
+      if (again) {
+        kt_move<MASKED>(s_tmem, sc, lo, t);
+        moved = true;
+      }
+      const bool beyond = kt_weights<MASKED>(s_tmem, ks, vs, lo, t, sum, pk);
+      again = !moved && __any_sync(0xffffffffu, beyond);
+      if (!again) break;
     }
-    sum = kt_weights<MASKED>(s_tmem, sc, qs, m, first, end, top, pk);
+    any |= moved;
+    lo.l[0] += sum[0];
+    lo.l[1] += sum[1];
+    kt_store_p(s_tmem, pk);
+    // the other two rows' turn
+    s_tmem += 16u << 16;
+    const KtRows x = lo;
+    lo = hi;
+    hi = x;
   }
-  l += sum;
-  return alpha;
+  return any;
 }
 
 template <int HD, bool FP8>
@@ -426,7 +487,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   } else if (warp < kKtConv) {
     // ------------------------------------------------------------------ softmax
     kt_more_regs<kKtRegsSoft>();
-    const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane;
+    const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane, t4 = lane & 3;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tsx = tmem + C::kS + x * 64 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
     uint32_t g = 0, uses = 0;
@@ -436,8 +497,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 750)) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
-      const bool in = rr < D.nr;
       if (D.nr <= 128 * x) {
         g += D.nb;
         __syncwarp();
@@ -445,36 +504,56 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         continue;
       }
       if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1, 751))) break;
-      const float qs = qscale[d * kKtRows + rr];
-      const int qpos = D.L - D.n + tok;
-      float m = in ? -INFINITY : 0.f, l = 0.f;
+      KtRows w[2];
+      int qpos[4];
+      int least = INT_MAX, most = 0;  // of the warp's rows' positions
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int rr = x * 128 + (warp & 3) * 32 + (lane >> 2) + 8 * k;
+        const bool in = rr < D.nr;
+        w[k >> 1].qs[k & 1] = in ? qscale[d * kKtRows + rr] : 0.f;
+        w[k >> 1].m[k & 1] = in ? -INFINITY : 0.f;
+        w[k >> 1].l[k & 1] = 0.f;
+        qpos[k] = in ? D.L - D.n + (D.r0 + rr) / G : -1;
+        if (in) least = min(least, qpos[k]), most = max(most, qpos[k]);
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      most = __reduce_max_sync(0xffffffffu, most);
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
         if (!(ok = kv8_wait_warp(&sfull[x], uses & 1, 752))) break;
         if (!(ok = kv8_wait_warp(&scfull[g % kKtSlots], (g / kKtSlots) & 1, 753))) break;
         tc_fence_after();
         const KtScales& sc = slots[g % kKtSlots];
-        // the keys of this block that the row sees: [first, end)
         const int k0 = (D.blk + j) * kKv8Block;
-        const int first = p.window > 0 ? max(0, qpos - p.window + 1 - k0) : 0, end = min(qpos + 1 - k0, kKv8Block);
-        uint32_t pk[32];
-        float alpha;
-        if (__any_sync(0xffffffffu, in && (first > 0 || end < kKv8Block)))
-          alpha = kt_softmax<true>(tsx, sc, qs, in ? first : 0, in ? end : 0, m, l, pk);
-        else
-          alpha = kt_softmax<false>(tsx, sc, qs, 0, 0, m, l, pk);
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // (S of this block waited for O to hold the ones before)
+        bool moved;
+        if (least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0)) {  // every row sees every key
+          moved = kt_softmax<false>(tsx, sc, w[0], w[1], t4);
+        } else {
 #pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            w[k >> 1].first[k & 1] = p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
+            w[k >> 1].end[k & 1] = qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
+          }
+          moved = kt_softmax<true>(tsx, sc, w[0], w[1], t4);
+        }
+        if (j > 0 && moved) {  // (S of this block waited for O to hold the ones before)
+          float f = 1.f;  // of this lane's row of O
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float y = __shfl_sync(0xffffffffu, w[k >> 1].alpha[k & 1], (lane & 7) * 4);
+            if (lane >> 3 == k) f = y;
+          }
+#pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t v[32];
             tmem_ld_32x32b_x32(to + c * 32, v);
             tc_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
             tmem_st_32x32b_x32(to + c * 32, v);
           }
         }
-        tmem_st_32x32b_x32(tsx, pk);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -482,6 +561,19 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         ++uses;
       }
       if (!ok) break;
+      // from here on a lane has one row
+      const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
+      const bool in = rr < D.nr;
+      float m = 0.f, l = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float lk = w[k >> 1].l[k & 1];
+        lk += __shfl_xor_sync(0xffffffffu, lk, 1);
+        lk += __shfl_xor_sync(0xffffffffu, lk, 2);
+        const float mk = __shfl_sync(0xffffffffu, w[k >> 1].m[k & 1], (lane & 7) * 4);
+        lk = __shfl_sync(0xffffffffu, lk, (lane & 7) * 4);
+        if (lane >> 3 == k) m = mk, l = lk;
+      }
       // O out of tensor memory, 32 head dims at a time
       if (!(ok = kv8_wait_warp(&pvdone[x], (uses - 1) & 1, 754))) break;
       tc_fence_after();
@@ -583,51 +675,56 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         const uint8_t* src = raw + rs * C::kRawStage;
         auto convert = [&](uint8_t* dst, int which) {
           // groups of 8 keys, w and w + 4 of them this warp's, and of 64 head dims
+          uint4 v[2][HD / 64];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int grp = w + 4 * y, key = grp * 8 + key8;
+            const int key = (w + 4 * y) * 8 + key8;
             const int at = key + (key & ~(p.page - 1)) + which * p.page;  // row of the page's two parts
-            const bool none = partial && (k0 + key < D.lo || k0 + key >= D.kend);
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+              v[y][c] = *reinterpret_cast<const uint4*>(src + at * HD + (HD == 128 ? ((c * 4 + part) ^ key8) << 4 : (part ^ (key8 >> 1)) << 4));
+            if (partial && (k0 + key < D.lo || k0 + key >= D.kend)) {
+#pragma unroll
+              for (int c = 0; c < HD / 64; ++c) v[y][c] = make_uint4(0, 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
-              uint4 v = *reinterpret_cast<const uint4*>(src + at * HD + (HD == 128 ? ((c * 4 + part) ^ (key8 & 7)) << 4 : (part ^ ((key8 >> 1) & 3)) << 4));
-              if (none) v = make_uint4(0, 0, 0, 0);
               uint4 a, b;
-              kv8_to_half<FP8>(v.x, a.x, a.y);
-              kv8_to_half<FP8>(v.y, a.z, a.w);
-              kv8_to_half<FP8>(v.z, b.x, b.y);
-              kv8_to_half<FP8>(v.w, b.z, b.w);
-              uint8_t* o = dst + c * C::kHalf + key * 128;
+              kv8_to_half<FP8>(v[y][c].x, a.x, a.y);
+              kv8_to_half<FP8>(v[y][c].y, a.z, a.w);
+              kv8_to_half<FP8>(v[y][c].z, b.x, b.y);
+              kv8_to_half<FP8>(v[y][c].w, b.z, b.w);
+              uint8_t* o = dst + c * C::kHalf + ((w + 4 * y) * 8 + key8) * 128;
               *reinterpret_cast<uint4*>(o + (((2 * part) ^ key8) << 4)) = a;
               *reinterpret_cast<uint4*>(o + (((2 * part + 1) ^ key8) << 4)) = b;
             }
-          }
           fence_async_smem();
         };
-        if (!(ok = kv8_wait_warp(&kempty[st], ph ^ 1, 763))) break;
-        convert(sK + st * C::kTile, order.codes);
-        // scales: what used this slot before was over when its keys' products were
-        if (row < kKv8Block) {
-          const float* sc = raw_scales + rs * (C::kRawScales / 4) + row + (row & ~(p.page - 1));
-          const bool none = partial && (k0 + row < D.lo || k0 + row >= D.kend);
-          const float ks = none ? 0.f : sc[order.scales * p.page], vs = none ? 0.f : sc[(order.scales ^ 1) * p.page];
-          KtScales& s = slots[g % kKtSlots];
-          s.ks[row] = ks;
-          s.vs[row] = vs;
-          s.lv[row] = kv8_log_scale(vs);
+        // keys, then values (one copy of the code)
+#pragma unroll 1
+        for (int y = 0; y < 2; ++y) {
+          if (!(ok = kv8_wait_warp(&(y ? vempty : kempty)[st], ph ^ 1, 763))) break;
+          convert((y ? sV : sK) + st * C::kTile, order.codes ^ y);
+          // scales: what used this slot before was over when its keys' products were
+          if (y == 0 && row < kKv8Block) {
+            const float* sc = raw_scales + rs * (C::kRawScales / 4) + row + (row & ~(p.page - 1));
+            const bool none = partial && (k0 + row < D.lo || k0 + row >= D.kend);
+            const float ks = none ? 0.f : sc[order.scales * p.page], vs = none ? 0.f : sc[(order.scales ^ 1) * p.page];
+            KtScales& s = slots[g % kKtSlots];
+            s.ks[row] = ks;
+            s.vs[row] = vs;
+            s.lv[row] = kv8_log_scale(vs);
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&(y ? vfull : kfull)[st]);
+            mbar_arrive(y ? &rempty[rs] : &scfull[g % kKtSlots]);
+          }
         }
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&kfull[st]);
-          mbar_arrive(&scfull[g % kKtSlots]);
-        }
-        if (!(ok = kv8_wait_warp(&vempty[st], ph ^ 1, 764))) break;
-        convert(sV + st * C::kTile, order.codes ^ 1);
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&vfull[st]);
-          mbar_arrive(&rempty[rs]);
-        }
+        if (!ok) break;
       }
       if (!ok) break;
       __syncwarp();
