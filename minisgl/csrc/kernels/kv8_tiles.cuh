@@ -4,16 +4,17 @@
 // value block, 64 keys at a time, on the 5th-generation tensor core:
 //
 //   warp 0        goes through the run's segments, publishes them, copies raw pages into a ring by TMA
-//   warps 1, 2    issue the products of one tile each: S = Q K^T, then, once the weights are there, O += P V. Q and P are read
-//                 from tensor memory and K, V from shared memory, whose bandwidth is what all of this comes close to.
+//   warps 1, 2    issue the products of one tile each: S = Q K^T a block ahead, and, once the weights are there, O += P V, P out
+//                 of tensor memory
 //   warp 3        fetches the next segments' queries into the L2 cache
 //   warps 4 - 11  softmax, 32 rows a warp, four rows and 16 keys a lane: S out of tensor memory, weights as fp16 over S's columns, O rescaled there
 //                 when a row's offset grows by more than 2^(15 - kKtTop), O read out and written at the segment's end
-//   warps 12 - 15 convert: queries to fp16 in tensor memory at a segment's start, then codes to fp16 operand tiles (exact),
+//   warps 12 - 15 convert: queries to fp16 at a segment's start, then codes to fp16 operand tiles (exact),
 //                 once for both tiles, and scales to what the softmax wants of them
 //
-// A tile's S and its weights share 64 columns, so its two products and its softmax run one after the other; what fills the
-// tensor core and the softmax's pipes is the other tile. Tensor memory: Q 2 x 64 columns, S / P 2 x 64, O 2 x 128.
+// A block's S and its weights share 64 columns of tensor memory, and each tile has two such: S 2 x 2 x 64 columns, O 2 x 128. (With
+// Q in tensor memory instead of shared memory there is room for one only; less shared memory is read then, but a tile's
+// softmax waits for its products some 1200 cycles every block, which the other tile does not fill.)
 //
 // Numerics as in kv8_stream.cuh, with kKtTop for kKv8Top: room for offsets that are not moved at every block.
 #pragma once
@@ -28,7 +29,7 @@ constexpr int kKtRows = 256;
 constexpr int kKtThreads = 512;
 constexpr int kKtCost = 2;      // of a segment, in blocks
 constexpr int kKtDescs = 4;     // segments looked up ahead
-constexpr int kKtSlots = 4;     // of scales
+constexpr int kKtSlots = 8;     // of scales
 constexpr float kKtTop = 10.f;
 constexpr int kKtConv = 12, kKtSoft = 4;  // first warps of the converters and of the softmax
 // registers of a thread in warps 0 - 3, the softmax and the converters: of the launch's 4 x 128 a row of warps
@@ -52,10 +53,12 @@ struct KtCfg {
   static constexpr int kHalf = kKv8Block * 128;      // a block's 64 head dims as an fp16 operand
   static constexpr int kTile = kHalf * (HD / 64);
   static constexpr int kStages = 3;                  // of K and of V operands
-  static constexpr int kRaw = HD == 128 ? 6 : 8;     // of codes
+  static constexpr int kRaw = HD == 128 ? 3 : 8;     // of codes
   static constexpr int kRawStage = 2 * kKv8Block * HD;
   static constexpr int kRawScales = 2 * kKv8Block * 4;
-  static constexpr int kOffRaw = 2 * kStages * kTile;
+  static constexpr int kQHalf = 128 * 128, kQTile = kQHalf * (HD / 64);  // a tile's queries
+  static constexpr int kOffQ = 2 * kStages * kTile;
+  static constexpr int kOffRaw = kOffQ + 2 * kQTile;
   static constexpr int kOffSc = kOffRaw + kRaw * kRawStage;
   static constexpr int kOffSlots = kOffSc + kRaw * kRawScales;
   static constexpr int kOffQs = kOffSlots + kKtSlots * (int)sizeof(KtScales);
@@ -63,11 +66,11 @@ struct KtCfg {
   static constexpr int kOffPlan = kOffDesc + kKtDescs * (int)sizeof(KtDesc);
   static constexpr int kOffRed = kOffPlan + (int)sizeof(Kv8Plan);
   static constexpr int kOffBars = kOffRed + 8 * (kKtThreads / 32);
-  static constexpr int kBars = 4 * kStages + 2 * kRaw + kKtSlots + 3 * kKtDescs + 2 + 4 * 2;
+  static constexpr int kBars = 4 * kStages + 2 * kRaw + kKtSlots + 3 * kKtDescs + 2 + 3 * 4 + 2;
   static constexpr int kSmem = 1024 + kOffBars + 8 * kBars + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
   // tensor memory columns
-  static constexpr int kQ = 0, kS = 128, kO = 256;
+  static constexpr int kS = 0, kO = 256;
 };
 
 constexpr uint32_t kt_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }  // fp16 operands, fp32 sums
@@ -268,10 +271,10 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   uint64_t* qsfull = dempty + kKtDescs;
   uint64_t* qfull = qsfull + kKtDescs;
   uint64_t* qempty = qfull + 1;
-  uint64_t* sfull = qempty + 1;  // [2]: a tile's S is there
-  uint64_t* pfull = sfull + 2;   // its weights are
-  uint64_t* pvdone = pfull + 2;  // O holds them, S's columns are free
-  uint64_t* ofree = pvdone + 2;  // O has been read
+  uint64_t* sfull = qempty + 1;  // [tile][buffer]: S is there
+  uint64_t* pfull = sfull + 4;   // its weights are
+  uint64_t* pvdone = pfull + 4;  // O holds them, S's columns are free
+  uint64_t* ofree = pvdone + 4;  // [tile]: O has been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofree + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -295,12 +298,12 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       }
       mbar_init(qfull, 4);
       mbar_init(qempty, 2);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         mbar_init(&sfull[i], 1);
         mbar_init(&pfull[i], 4);
         mbar_init(&pvdone[i], 1);
-        mbar_init(&ofree[i], 4);
       }
+      for (int i = 0; i < 2; ++i) mbar_init(&ofree[i], 4);
       fence_barrier_init();
     }
     __syncwarp();
@@ -413,59 +416,101 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   } else if (warp <= 2) {
     // ------------------------------------------------------------------ products of one tile
     kt_fewer_regs<kKtRegsFew>();
+    // Two streams, of products with keys and of products with values, each through all segments; whichever can go on does.
     if (lane == 0) {
       const int x = warp - 1;
-      const uint32_t tq = tmem + C::kQ + x * 64, tsx = tmem + C::kS + x * 64, to = tmem + C::kO + x * 128;
+      const uint32_t ts = tmem + C::kS + x * 128, to = tmem + C::kO + x * 128;
+      const uint64_t q = smem_desc_sw128(smem_u32(smem + C::kOffQ + x * C::kQTile));
       constexpr uint32_t idesc_s = kt_idesc(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
-      uint32_t g = 0, uses = 0, outs = 0;  // blocks gone through, of them this tile's, segments of this tile's
-      bool ok = true;
-      for (int i = 0; ok; ++i) {
-        const int d = i % kKtDescs;
-        if (!kv8_wait(&dfull[d], (i / kKtDescs) & 1, 730)) break;
-        const int nb = descs[d].nb;
-        const bool active = descs[d].nr > 128 * x;
-        if (nb == 0) break;
-        if (!(ok = kv8_wait(qfull, i & 1, 731))) break;
-        if (!active) mbar_arrive(qempty);
-        tc_fence_after();
-        for (int j = 0; j < nb; ++j, ++g) {
-          const uint32_t st = g % C::kStages, ph = (g / C::kStages) & 1;
-          if (!(ok = kv8_wait(&kfull[st], ph, 732))) break;
-          if (active) {
-            if (uses > 0 && !(ok = kv8_wait(&pvdone[x], (uses - 1) & 1, 733))) break;  // S's columns
+      // of a stream: segment, block in it and in all, this tile's blocks; a segment has nb blocks, and this tile rows in it or not
+      struct {
+        uint32_t i = 0, j = 0, g = 0, uses = 0;
+        int nb = 0;  // 0: none at hand, -1: no more
+        bool active = false;
+      } k, v;
+      uint32_t outs = 0;  // segments whose O has begun
+      uint64_t waiting = 0;
+      uint32_t spins = 0;
+      while (v.nb >= 0) {
+        bool went = false;
+        if (k.nb == 0 && mbar_test(&dfull[k.i % kKtDescs], (k.i / kKtDescs) & 1)) {
+          const KtDesc& D = descs[k.i % kKtDescs];
+          k.nb = D.nb > 0 ? D.nb : -1;
+          k.active = D.nr > 128 * x;
+          k.j = 0;
+        }
+        if (k.nb > 0 && (k.j > 0 || mbar_test(qfull, k.i & 1)) && mbar_test(&kfull[k.g % C::kStages], (k.g / C::kStages) & 1) &&
+            (!k.active || k.uses < 2 || mbar_test(&pvdone[2 * x + (k.uses & 1)], ((k.uses - 2) >> 1) & 1))) {
+          const uint32_t st = k.g % C::kStages;
+          if (k.active) {
             tc_fence_after();
             // (a descriptor's low bits are its address / 16)
-            const uint64_t k = smem_desc_sw128(smem_u32(sK + st * C::kTile));
+            const uint64_t b = smem_desc_sw128(smem_u32(sK + st * C::kTile));
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
-              tc_mma_f16_ts(tsx, tq + kk * 8, k + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+              tc_mma_f16(ts + (k.uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
+                         b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
             tc_commit(&kempty[st]);
-            tc_commit(&sfull[x]);
-            if (j == nb - 1) tc_commit(qempty);
-            if (!(ok = kv8_wait(&vfull[st], ph, 734))) break;
-            if (j == 0 && outs > 0 && !(ok = kv8_wait(&ofree[x], (outs - 1) & 1, 735))) break;
-            if (!(ok = kv8_wait(&pfull[x], uses & 1, 736))) break;
-            tc_fence_after();
-            const uint64_t v = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
-#pragma unroll
-            for (int kk = 0; kk < kKv8Block / 16; ++kk)
-              tc_mma_f16_ts(to, tsx + kk * 8, v + (kk * 16 * 128 >> 4), idesc_o, j > 0 || kk > 0);
-            tc_commit(&vempty[st]);
-            tc_commit(&pvdone[x]);
-            ++uses;
+            tc_commit(&sfull[2 * x + (k.uses & 1)]);
+            if ((int)k.j == k.nb - 1) tc_commit(qempty);
+            ++k.uses;
           } else {
             mbar_arrive(&kempty[st]);
-            if (!(ok = kv8_wait(&vfull[st], ph, 737))) break;
+            if ((int)k.j == k.nb - 1) mbar_arrive(qempty);
+          }
+          ++k.g;
+          if ((int)++k.j == k.nb) {
+            k.nb = 0;
+            ++k.i;
+          }
+          went = true;
+        }
+        if (v.nb == 0 && mbar_test(&dfull[v.i % kKtDescs], (v.i / kKtDescs) & 1)) {
+          const KtDesc& D = descs[v.i % kKtDescs];
+          v.nb = D.nb > 0 ? D.nb : -1;
+          v.active = D.nr > 128 * x;
+          v.j = 0;
+        }
+        if (v.nb > 0 && v.g < k.g && mbar_test(&vfull[v.g % C::kStages], (v.g / C::kStages) & 1) &&
+            (!v.active || (mbar_test(&pfull[2 * x + (v.uses & 1)], (v.uses >> 1) & 1) &&
+                           (v.j > 0 || outs == 0 || mbar_test(&ofree[x], (outs - 1) & 1))))) {
+          const uint32_t st = v.g % C::kStages;
+          if (v.active) {
+            tc_fence_after();
+            const uint64_t b = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
+#pragma unroll
+            for (int kk = 0; kk < kKv8Block / 16; ++kk)
+              tc_mma_f16_ts(to, ts + (v.uses & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, v.j > 0 || kk > 0);
+            tc_commit(&vempty[st]);
+            tc_commit(&pvdone[2 * x + (v.uses & 1)]);
+            ++v.uses;
+            if (v.j == 0) ++outs;
+          } else {
             mbar_arrive(&vempty[st]);
           }
+          ++v.g;
+          if ((int)++v.j == v.nb) {
+            mbar_arrive(&dempty[v.i % kKtDescs]);
+            v.nb = 0;
+            ++v.i;
+          }
+          went = true;
         }
-        if (!ok) break;
-        if (active) ++outs;
-        mbar_arrive(&dempty[d]);
+        if (went) {
+          waiting = 0;
+        } else if ((++spins & 255) == 0) {
+          const uint64_t now = globaltimer_ns();
+          if (waiting == 0) {
+            waiting = now;
+          } else if (now - waiting > kWaitTimeoutNs) {
+            report_error(kErrMbarTimeout, 730);
+            break;
+          }
+        }
       }
-      // (on giving up, too: no product is in flight when the CTA's memories go)
-      if (!ok) kv8_wait(&sfull[x], uses & 1, 739);
-      if (uses > 0) kv8_wait(&pvdone[x], (uses - 1) & 1, 738);
+      // no product is in flight when the CTA's memories go
+      if (k.uses > 0) kv8_wait(&sfull[2 * x + ((k.uses - 1) & 1)], ((k.uses - 1) >> 1) & 1, 738);
+      if (v.uses > 0) kv8_wait(&pvdone[2 * x + ((v.uses - 1) & 1)], ((v.uses - 1) >> 1) & 1, 739);
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------------ queries into the L2 cache
@@ -489,7 +534,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     kt_more_regs<kKtRegsSoft>();
     const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane, t4 = lane & 3;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tsx = tmem + C::kS + x * 64 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
+    const uint32_t ts = tmem + C::kS + x * 128 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
     uint32_t g = 0, uses = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -521,23 +566,25 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       most = __reduce_max_sync(0xffffffffu, most);
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
-        if (!(ok = kv8_wait_warp(&sfull[x], uses & 1, 752))) break;
+        if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1, 752))) break;
         if (!(ok = kv8_wait_warp(&scfull[g % kKtSlots], (g / kKtSlots) & 1, 753))) break;
         tc_fence_after();
         const KtScales& sc = slots[g % kKtSlots];
         const int k0 = (D.blk + j) * kKv8Block;
         bool moved;
         if (least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0)) {  // every row sees every key
-          moved = kt_softmax<false>(tsx, sc, w[0], w[1], t4);
+          moved = kt_softmax<false>(ts + (uses & 1) * 64, sc, w[0], w[1], t4);
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             w[k >> 1].first[k & 1] = p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
             w[k >> 1].end[k & 1] = qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
           }
-          moved = kt_softmax<true>(tsx, sc, w[0], w[1], t4);
+          moved = kt_softmax<true>(ts + (uses & 1) * 64, sc, w[0], w[1], t4);
         }
-        if (j > 0 && moved) {  // (S of this block waited for O to hold the ones before)
+        if (j > 0 && moved) {  // once O holds the blocks before
+          if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1, 755))) break;
+          tc_fence_after();
           float f = 1.f;  // of this lane's row of O
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -557,7 +604,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[x]);
+        if (lane == 0) mbar_arrive(&pfull[2 * x + (uses & 1)]);
         ++uses;
       }
       if (!ok) break;
@@ -575,7 +622,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         if (lane >> 3 == k) m = mk, l = lk;
       }
       // O out of tensor memory, 32 head dims at a time
-      if (!(ok = kv8_wait_warp(&pvdone[x], (uses - 1) & 1, 754))) break;
+      if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1, 754))) break;
       tc_fence_after();
       const int head = D.h * G + r - tok * G;
       const float f = D.slot < 0 ? kv8_norm(m, l, p.sinks, in ? head : 0) : 1.f;
@@ -611,7 +658,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     // ------------------------------------------------------------------ conversions
     kt_fewer_regs<kKtRegsConv>();
     const int w = warp - kKtConv, row = w * 32 + lane;
-    const uint32_t tq = tmem + C::kQ + ((uint32_t)(w * 32) << 16);
     // Codes: a warp takes 8 keys x 64 head dims at a time, 16 a lane, so that neither its loads nor its stores of 16
     // bytes meet in a bank: of every 8 lanes 4 have key k, the others key k ^ 5.
     const int part = lane & 3, key8 = (lane >> 3) ^ (lane & 4 ? 5 : 0);
@@ -646,24 +692,17 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           __syncwarp();
           if (lane == 0) mbar_arrive(&qsfull[d]);
         }
-        // Q's columns are free once the last segment's products with keys are done
+        // the queries' place is free once the last segment's products with keys are done
         if (x == 0 && i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1, 761))) break;
-        tc_fence_after();
+        uint8_t* dst = smem + C::kOffQ + x * C::kQTile + row * 128;
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-          uint32_t v[32];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t e[4] = {u[8 * c + k].x, u[8 * c + k].y, u[8 * c + k].z, u[8 * c + k].w};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) v[4 * k + y] = pack_half(bf16_lo(e[y]) * f, bf16_hi(e[y]) * f);
-          }
-          tmem_st_32x32b_x32(tq + x * 64 + c * 32, v);
-        }
+        for (int c = 0; c < HD / 8; ++c)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQHalf + (((c & 7) ^ (row & 7)) << 4)) =
+              make_uint4(pack_half(bf16_lo(u[c].x) * f, bf16_hi(u[c].x) * f), pack_half(bf16_lo(u[c].y) * f, bf16_hi(u[c].y) * f),
+                         pack_half(bf16_lo(u[c].z) * f, bf16_hi(u[c].z) * f), pack_half(bf16_lo(u[c].w) * f, bf16_hi(u[c].w) * f));
       }
       if (!ok) break;
-      tc_wait_st();
-      tc_fence_before();
+      fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(qfull);
 
