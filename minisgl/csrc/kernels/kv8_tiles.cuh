@@ -46,6 +46,7 @@ struct KtDesc {
 };
 struct KtScales {
   float ks[kKv8Block], lv[kKv8Block], vs[kKv8Block];
+  uint32_t bad[4];  // bit c % 32 of word c / 32: key c has no finite scale (0 stands in its place)
 };
 
 template <int HD>
@@ -125,123 +126,153 @@ MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
       : "memory");
 }
 
-// Two of a lane's four rows (rows g and g + 8 of 16): their queries' factors, running offsets and this lane's part of their
-// sums, the keys of the block that they see, [first, end), and what their O has to be multiplied by first.
+// The same for 8 columns of S and 4 of its weights.
+MSGL_DEVICE void kt_load_s8(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+MSGL_DEVICE void kt_store_p8(uint32_t taddr, uint32_t a, uint32_t b) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x1.b32 [%0], {%1,%2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
+}
+
+// A lane's four rows, 8 apart: their queries' factors, running offsets and this lane's part of their sums, the keys of the
+// block that they see, [first, end), and what their O has to be multiplied by first.
 struct KtRows {
-  float qs[2], m[2], l[2], alpha[2];
-  int first[2], end[2];
+  float qs[4], m[4], l[4], alpha[4];
+  int first[4], end[4];
 };
 
-// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one.
-template <bool MASKED>
+// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop,
+// like all that not every block needs: unrolled it comes out of L2, and takes ten times its time.)
 MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
-  uint32_t u[32];
-  kt_load_s(s_tmem, u);
-  tc_wait_ld();
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int n = 0; n < 8; ++n) {
+    const int c = 8 * n + 2 * t;
+    uint32_t u[2][4];
+    kt_load_s8(s_tmem + 8 * n, u[0]);
+    kt_load_s8(s_tmem + 8 * n + (16u << 16), u[1]);
+    const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), lv = *reinterpret_cast<const float2*>(&sc.lv[c]);
+    tc_wait_ld();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float top = -INFINITY;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* s = &u[k >> 1][2 * (k & 1)];
+      const float x = fmaf(__uint_as_float(s[0]) * ks.x, w.qs[k], lv.x), y = fmaf(__uint_as_float(s[1]) * ks.y, w.qs[k], lv.y);
+      if (c >= w.first[k] && c < w.end[k]) top[k] = fmaxf(top[k], x);
+      if (c + 1 >= w.first[k] && c + 1 < w.end[k]) top[k] = fmaxf(top[k], y);
+    }
+  }
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = 8 * n + 2 * t + e;
-        const float x = fmaf(__uint_as_float(u[4 * n + 2 * k + e]) * sc.ks[c], w.qs[k], sc.lv[c]);
-        if (!MASKED || (c >= w.first[k] && c < w.end[k])) top = fmaxf(top, x);
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) - kKtTop;
-    if (top > w.m[k]) {
-      const float f = kv8_exp2(w.m[k] - top);
-      w.m[k] = top;
-      w.l[k] *= f;
-      w.alpha[k] *= f;
+  for (int k = 0; k < 4; ++k) {
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2)) - kKtTop;
+    if (top[k] > w.m[k]) {
+      w.alpha[k] = kv8_exp2(w.m[k] - top[k]);
+      w.m[k] = top[k];
+      w.l[k] *= w.alpha[k];
     }
   }
 }
 
-// A block's weights of two rows, as fp16 pairs, with the offsets as they are. `sum`: this lane's sums of 2^(s_j - m). Returns
-// whether a weight is beyond 2^15, or a sum beyond 2^108.
-template <bool MASKED>
-MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const uint64_t (&ks)[8], const uint64_t (&vs)[8], const KtRows& w, int t, float (&sum)[2],
-                            uint32_t (&pk)[16]) {
-  uint32_t u[32];
-  kt_load_s(s_tmem, u);
-  tc_wait_ld();
-  bool beyond = false;
+// The weights of a block that some of the lane's rows see in part only, over S's columns.
+MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
+#pragma unroll 1
+  for (int n = 0; n < 8; ++n) {
+    const int c = 8 * n + 2 * t;
+    uint32_t u[2][4], pk[4];
+    kt_load_s8(s_tmem + 8 * n, u[0]);
+    kt_load_s8(s_tmem + 8 * n + (16u << 16), u[1]);
+    const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), vs = *reinterpret_cast<const float2*>(&sc.vs[c]);
+    tc_wait_ld();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
-    const uint64_t q2 = f2_pack(w.qs[k], w.qs[k]), b2 = f2_pack(-base, -base);
-    uint64_t total = 0;
-    float top = 0.f;
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int c = 8 * n + 2 * t;
-      const uint64_t y = f2_mul(f2_pack(__uint_as_float(u[4 * n + 2 * k]), __uint_as_float(u[4 * n + 2 * k + 1])), ks[n]);
-      const float2 x = f2_unpack(f2_fma(y, q2, b2));
-      float2 e = make_float2(kv8_exp2(x.x), kv8_exp2(x.y));
-      if (MASKED) {
-        if (!(c >= w.first[k] && c < w.end[k])) e.x = 0.f;
-        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) e.y = 0.f;
-      }
-      const uint64_t e2 = f2_pack(e.x, e.y);
-      total = f2_add(total, e2);
-      float2 v = f2_unpack(f2_mul(e2, vs[n]));
-      if (MASKED) {  // (a hidden key's weight is zero whatever its scale)
-        if (!(c >= w.first[k] && c < w.end[k])) v.x = 0.f;
-        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) v.y = 0.f;
-      }
-      top = fmaxf(fmaxf(top, v.x), v.y);
-      pk[2 * n + k] = pack_half(v.x, v.y);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* s = &u[k >> 1][2 * (k & 1)];
+      const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
+      float x = kv8_exp2(fmaf(__uint_as_float(s[0]) * ks.x, w.qs[k], -base)), y = kv8_exp2(fmaf(__uint_as_float(s[1]) * ks.y, w.qs[k], -base));
+      if (!(c >= w.first[k] && c < w.end[k])) x = 0.f;
+      if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) y = 0.f;
+      w.l[k] += x + y;
+      pk[k] = pack_half(x * vs.x, y * vs.y);
     }
-    const float2 a = f2_unpack(total);
+    // (the columns it overwrites have been read: keys 4n .. 4n + 3)
+    kt_store_p8(s_tmem + 4 * n, pk[0], pk[1]);
+    kt_store_p8(s_tmem + 4 * n + (16u << 16), pk[2], pk[3]);
+  }
+}
+
+// The weights of a block that every row sees, with the offsets as they are: fp16 pairs and this lane's sums of 2^(s_j - m).
+// Returns whether a weight is beyond 2^15, or a sum beyond 2^108.
+MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, float (&sum)[4], uint32_t (&pk)[2][16]) {
+  uint32_t u[2][32];
+  kt_load_s(s_tmem, u[0]);
+  kt_load_s(s_tmem + (16u << 16), u[1]);
+  uint64_t q2[4], b2[4], total[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
+    q2[k] = f2_pack(w.qs[k], w.qs[k]);
+    b2[k] = f2_pack(-base, -base);
+    total[k] = 0;
+  }
+  float top = 0.f;
+  tc_wait_ld();
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const int c = 8 * n + 2 * t;
+    const uint64_t ks = *reinterpret_cast<const uint64_t*>(&sc.ks[c]), vs = *reinterpret_cast<const uint64_t*>(&sc.vs[c]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
+      const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), q2[k], b2[k]));
+      const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
+      total[k] = f2_add(total[k], e2);
+      const float2 v = f2_unpack(f2_mul(e2, vs));
+      top = fmaxf(fmaxf(top, v.x), v.y);
+      pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
+    }
+  }
+  bool beyond = !(top <= 32768.f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 a = f2_unpack(total[k]);
     sum[k] = a.x + a.y;
-    beyond |= !(top <= 32768.f && sum[k] <= 0x1p+108f);
+    beyond |= !(sum[k] <= 0x1p+108f);
   }
   return beyond;
 }
 
-// A block of the lane's rows: their weights over S's columns. New offsets first for rows that have none (they have seen no
-// key) or have weights beyond fp16, sums beyond 2^108 (keys whose values are nearly nothing): few blocks need any, and the
-// others are spared the maximum of their logits. Returns whether any of the warp's rows has a new one. (Loops that are not
-// unrolled: five roles' code has to fit the instruction cache.)
-template <bool MASKED>
-MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& lo, KtRows& hi, int t) {
-  uint64_t ks[8], vs[8];
+// A block of the lane's rows, which see all of it or (`part`) not: their weights over S's columns. New offsets first where rows
+// have none (they have seen no key), or weights beyond fp16, or sums beyond 2^108 (keys whose values are nearly nothing): few
+// blocks need any, and the others are spared the maximum of their logits. Returns whether O has to be multiplied by anything.
+MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool part) {
+  float sum[4];
+  uint32_t pk[2][16];
+  bool moved = false, again = part;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    ks[n] = *reinterpret_cast<const uint64_t*>(&sc.ks[8 * n + 2 * t]);
-    vs[n] = *reinterpret_cast<const uint64_t*>(&sc.vs[8 * n + 2 * t]);
+  for (int k = 0; k < 4; ++k) {
+    w.alpha[k] = 1.f;
+    again |= w.m[k] == -INFINITY;
   }
-  bool any = false;
+  again = __any_sync(0xffffffffu, again);
 #pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    float sum[2];
-    uint32_t pk[16];
-    bool moved = false;
-    lo.alpha[0] = lo.alpha[1] = 1.f;
-#pragma unroll 1
-    for (bool again = __any_sync(0xffffffffu, lo.m[0] == -INFINITY || lo.m[1] == -INFINITY);;) {
-      if (again) {
-        kt_move<MASKED>(s_tmem, sc, lo, t);
-        moved = true;
-      }
-      const bool beyond = kt_weights<MASKED>(s_tmem, ks, vs, lo, t, sum, pk);
-      again = !moved && __any_sync(0xffffffffu, beyond);
-      if (!again) break;
+  for (;;) {
+    if (again) {
+      kt_move(s_tmem, sc, w, t);
+      moved = true;
     }
-    any |= moved;
-    lo.l[0] += sum[0];
-    lo.l[1] += sum[1];
-    kt_store_p(s_tmem, pk);
-    // the other two rows' turn
-    s_tmem += 16u << 16;
-    const KtRows x = lo;
-    lo = hi;
-    hi = x;
+    if (part) break;
+    const bool beyond = kt_weights(s_tmem, sc, w, t, sum, pk);
+    again = !moved && __any_sync(0xffffffffu, beyond);
+    if (!again) break;
   }
-  return any;
+  if (part) {
+    kt_weights_in_part(s_tmem, sc, w, t);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
+    kt_store_p(s_tmem, pk[0]);
+    kt_store_p(s_tmem + (16u << 16), pk[1]);
+  }
+  return moved && __any_sync(0xffffffffu, w.alpha[0] != 1.f || w.alpha[1] != 1.f || w.alpha[2] != 1.f || w.alpha[3] != 1.f);
 }
 
 template <int HD, bool FP8>
@@ -549,16 +580,16 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         continue;
       }
       if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1, 751))) break;
-      KtRows w[2];
+      KtRows w;
       int qpos[4];
       int least = INT_MAX, most = 0;  // of the warp's rows' positions
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int rr = x * 128 + (warp & 3) * 32 + (lane >> 2) + 8 * k;
         const bool in = rr < D.nr;
-        w[k >> 1].qs[k & 1] = in ? qscale[d * kKtRows + rr] : 0.f;
-        w[k >> 1].m[k & 1] = in ? -INFINITY : 0.f;
-        w[k >> 1].l[k & 1] = 0.f;
+        w.qs[k] = in ? qscale[d * kKtRows + rr] : 0.f;
+        w.m[k] = in ? -INFINITY : 0.f;
+        w.l[k] = 0.f;
         qpos[k] = in ? D.L - D.n + (D.r0 + rr) / G : -1;
         if (in) least = min(least, qpos[k]), most = max(most, qpos[k]);
       }
@@ -571,16 +602,23 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         tc_fence_after();
         const KtScales& sc = slots[g % kKtSlots];
         const int k0 = (D.blk + j) * kKv8Block;
-        bool moved;
-        if (least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0)) {  // every row sees every key
-          moved = kt_softmax<false>(ts + (uses & 1) * 64, sc, w[0], w[1], t4);
-        } else {
+        // does every row of the warp see every key?
+        const bool part = !(least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            w[k >> 1].first[k & 1] = p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
-            w[k >> 1].end[k & 1] = qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
-          }
-          moved = kt_softmax<true>(ts + (uses & 1) * 64, sc, w[0], w[1], t4);
+        for (int k = 0; k < 4; ++k) {
+          w.first[k] = part && p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
+          w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
+        }
+        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, t4, part);
+        if ((sc.bad[0] | sc.bad[1]) != 0) {  // a key that has no finite scale makes the rows that see it no numbers
+          const uint64_t bad = sc.bad[0] | (uint64_t)sc.bad[1] << 32;
+#pragma unroll 1
+          for (int c = 0; c < kKv8Block; ++c)
+            if (bad >> c & 1) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (c >= w.first[k] && c < w.end[k]) w.l[k] = __int_as_float(0x7fc00000);
+            }
         }
         if (j > 0 && moved) {  // once O holds the blocks before
           if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1, 755))) break;
@@ -588,7 +626,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           float f = 1.f;  // of this lane's row of O
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float y = __shfl_sync(0xffffffffu, w[k >> 1].alpha[k & 1], (lane & 7) * 4);
+            const float y = __shfl_sync(0xffffffffu, w.alpha[k], (lane & 7) * 4);
             if (lane >> 3 == k) f = y;
           }
 #pragma unroll 1
@@ -614,10 +652,10 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       float m = 0.f, l = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float lk = w[k >> 1].l[k & 1];
+        float lk = w.l[k];
         lk += __shfl_xor_sync(0xffffffffu, lk, 1);
         lk += __shfl_xor_sync(0xffffffffu, lk, 2);
-        const float mk = __shfl_sync(0xffffffffu, w[k >> 1].m[k & 1], (lane & 7) * 4);
+        const float mk = __shfl_sync(0xffffffffu, w.m[k], (lane & 7) * 4);
         lk = __shfl_sync(0xffffffffu, lk, (lane & 7) * 4);
         if (lane >> 3 == k) m = mk, l = lk;
       }
@@ -626,7 +664,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       tc_fence_after();
       const int head = D.h * G + r - tok * G;
       const float f = D.slot < 0 ? kv8_norm(m, l, p.sinks, in ? head : 0) : 1.f;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(to + c * 32, v);
@@ -668,39 +706,41 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 760)) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      // queries: a thread takes its row of both tiles
+      // Queries: a thread takes its row of both tiles, first as it is into the operand's place, which is free once the last
+      // segment's products with keys are done, then converted there.
+      if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1, 761))) break;
+#pragma unroll 1
       for (int x = 0; x < 2; ++x) {
         const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
-        uint4 u[HD / 8];
-        if (rr < D.nr) {
-          const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (D.q0 + tok) * p.q_row +
-                                                            (int64_t)(D.h * G + r - tok * G) * p.q_head);
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) u[c] = __ldg(src + c);
-        } else {
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) u[c] = make_uint4(0, 0, 0, 0);
-        }
+        const bool in = rr < D.nr;
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
+                                                          (in ? (D.q0 + tok) * p.q_row + (int64_t)(D.h * G + r - tok * G) * p.q_head : 0));
+        uint8_t* dst = smem + C::kOffQ + x * C::kQTile + row * 128;
         uint32_t top = 0;
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; ++c) {
+          uint4 u[8];
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c)
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[c].x & 0x7fff7fffu, u[c].y & 0x7fff7fffu), __vmaxu2(u[c].z & 0x7fff7fffu, u[c].w & 0x7fff7fffu)));
+          for (int y = 0; y < 8; ++y) u[y] = in ? __ldg(src + 8 * c + y) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[y].x & 0x7fff7fffu, u[y].y & 0x7fff7fffu), __vmaxu2(u[y].z & 0x7fff7fffu, u[y].w & 0x7fff7fffu)));
+            *reinterpret_cast<uint4*>(dst + c * C::kQHalf + ((y ^ (row & 7)) << 4)) = u[y];
+          }
+        }
         top = max(top & 0xffffu, top >> 16);
         const float f = kv8_q_factor(__uint_as_float(top << 16));
         qscale[d * kKtRows + rr] = p.scale * kKv8Log2e * kv8_reciprocal(f);
-        if (x == 1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&qsfull[d]);
+#pragma unroll 2
+        for (int c = 0; c < HD / 8; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQHalf + ((c & 7) << 4));  // (any order: the row is the thread's own)
+          const uint4 v = *at;
+          *at = make_uint4(pack_half(bf16_lo(v.x) * f, bf16_hi(v.x) * f), pack_half(bf16_lo(v.y) * f, bf16_hi(v.y) * f),
+                           pack_half(bf16_lo(v.z) * f, bf16_hi(v.z) * f), pack_half(bf16_lo(v.w) * f, bf16_hi(v.w) * f));
         }
-        // the queries' place is free once the last segment's products with keys are done
-        if (x == 0 && i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1, 761))) break;
-        uint8_t* dst = smem + C::kOffQ + x * C::kQTile + row * 128;
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQHalf + (((c & 7) ^ (row & 7)) << 4)) =
-              make_uint4(pack_half(bf16_lo(u[c].x) * f, bf16_hi(u[c].x) * f), pack_half(bf16_lo(u[c].y) * f, bf16_hi(u[c].y) * f),
-                         pack_half(bf16_lo(u[c].z) * f, bf16_hi(u[c].z) * f), pack_half(bf16_lo(u[c].w) * f, bf16_hi(u[c].w) * f));
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qsfull[d]);
       if (!ok) break;
       fence_async_smem();
       __syncwarp();
@@ -748,14 +788,17 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           if (!(ok = kv8_wait_warp(&(y ? vempty : kempty)[st], ph ^ 1, 763))) break;
           convert((y ? sV : sK) + st * C::kTile, order.codes ^ y);
           // scales: what used this slot before was over when its keys' products were
-          if (y == 0 && row < kKv8Block) {
+          if (y == 0 && row < kKv8Block) {  // (two whole warps)
             const float* sc = raw_scales + rs * (C::kRawScales / 4) + row + (row & ~(p.page - 1));
             const bool none = partial && (k0 + row < D.lo || k0 + row >= D.kend);
-            const float ks = none ? 0.f : sc[order.scales * p.page], vs = none ? 0.f : sc[(order.scales ^ 1) * p.page];
+            float ks = none ? 0.f : sc[order.scales * p.page], vs = none ? 0.f : sc[(order.scales ^ 1) * p.page];
+            const unsigned bad = __ballot_sync(0xffffffffu, !(fabsf(ks) < INFINITY) || !(fabsf(vs) < INFINITY));
+            if (bad >> lane & 1) ks = vs = 0.f;
             KtScales& s = slots[g % kKtSlots];
             s.ks[row] = ks;
             s.vs[row] = vs;
             s.lv[row] = kv8_log_scale(vs);
+            if (lane == 0) s.bad[w] = bad;
           }
           __syncwarp();
           if (lane == 0) {
