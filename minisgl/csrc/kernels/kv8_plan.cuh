@@ -170,22 +170,23 @@ struct Kv8Order {
 };
 
 // The copies of one 64-key block, a page at a time: its keys' and values' codes with one instruction, its scales with
-// another (an instruction costs the warp some 100 cycles, whatever it copies). Lanes first .. first + pages - 1 hold the pages'
+// another. Lanes first .. first + pages - 1 hold the pages'
 // slots, -1 for a page that is not there: what lies outside the tensors is filled with zeros. A page's keys are
 // beside its values, codes and scales alike.
 template <int HD>
 MSGL_DEVICE void kv8_copy_block(const Kv8Attn& p, const CUtensorMap* tc, const CUtensorMap* ts, uint8_t* codes, float* scales, uint64_t* bar,
-                                int h, int slots, int first, int pages, int lane) {
+                                int h, int slots, int first, int pages) {
   const int page = p.page;
-  if (lane == 0) mbar_expect_tx(bar, 2 * page * pages * (HD + 4));
+  if (elect_one()) mbar_expect_tx(bar, 2 * page * pages * (HD + 4));
   __syncwarp();
   for (int i = 0; i < pages; ++i) {
     int slot = __shfl_sync(0xffffffffu, slots, first + i);
-    if (lane == 0) {
-      if (slot < 0) slot = p.num_slots;
+    if (slot < 0) slot = p.num_slots;
+    if (elect_one()) {
       kv8_load_4d(codes + 2 * i * page * HD, tc, bar, 0, slot, h, 0);
       tma_load_3d(scales + 2 * i * page, ts, bar, slot, h, 0);
     }
+    __syncwarp();
   }
 }
 

@@ -160,12 +160,11 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
           if (j + mine * kKsCopies < to - from) next = look_up(j + mine * kKsCopies);
         }
         const uint32_t x = seq + j, stage = x % C::kStages;
-        if (lane == 0) ok = kv8_wait(&empty[stage], ((x / C::kStages) & 1) ^ 1, 701);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = kv8_wait_warp(&empty[stage], ((x / C::kStages) & 1) ^ 1, 701);
         if (!ok) break;
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
         kv8_copy_block<HD>(p, &tc, &ts, ring + stage * C::kStage, scales + stage * (C::kScales / 4), &full[stage], h, slots,
-                           at % mine * gpb, pages, lane);
+                           at % mine * gpb, pages);
         last = x;
         ++issued;
       }

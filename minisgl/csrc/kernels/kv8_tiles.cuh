@@ -76,6 +76,9 @@ struct KtCfg {
 
 constexpr uint32_t kt_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }  // fp16 operands, fp32 sums
 
+// Has this phase completed? The same answer for all of the warp.
+MSGL_DEVICE bool kt_ready(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); }
+
 // pairs of fp32 in one register pair
 MSGL_DEVICE uint64_t f2_pack(float a, float b) {
   uint64_t r;
@@ -404,15 +407,14 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           if (j + mine < to - from) next = look_up(j + mine);
         }
         const uint32_t x = seq + j, stage = x % C::kRaw;
-        if (lane == 0) ok = kv8_wait(&rempty[stage], ((x / C::kRaw) & 1) ^ 1, 721);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = kv8_wait_warp(&rempty[stage], ((x / C::kRaw) & 1) ^ 1, 721);
         if (!ok) {
           seq = x;
           break;
         }
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
         kv8_copy_block<HD>(p, &tc, &ts, raw + stage * C::kRawStage, raw_scales + stage * (C::kRawScales / 4), &rfull[stage], h, page_slots,
-                           j % mine * gpb, pages, lane);
+                           j % mine * gpb, pages);
       }
       if (!ok) break;
       seq += to - from;
@@ -448,7 +450,9 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     // ------------------------------------------------------------------ products of one tile
     kt_fewer_regs<kKtRegsFew>();
     // Two streams, of products with keys and of products with values, each through all segments; whichever can go on does.
-    if (lane == 0) {
+    // (The whole warp goes through this and one lane is elected to issue: operands are then uniform, and a product costs a few
+    // cycles to issue instead of some 100.)
+    {
       const int x = warp - 1;
       const uint32_t ts = tmem + C::kS + x * 128, to = tmem + C::kO + x * 128;
       const uint64_t q = smem_desc_sw128(smem_u32(smem + C::kOffQ + x * C::kQTile));
@@ -464,31 +468,34 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       uint32_t spins = 0;
       while (v.nb >= 0) {
         bool went = false;
-        if (k.nb == 0 && mbar_test(&dfull[k.i % kKtDescs], (k.i / kKtDescs) & 1)) {
+        if (k.nb == 0 && kt_ready(&dfull[k.i % kKtDescs], (k.i / kKtDescs) & 1)) {
           const KtDesc& D = descs[k.i % kKtDescs];
           k.nb = D.nb > 0 ? D.nb : -1;
           k.active = D.nr > 128 * x;
           k.j = 0;
         }
-        if (k.nb > 0 && (k.j > 0 || mbar_test(qfull, k.i & 1)) && mbar_test(&kfull[k.g % C::kStages], (k.g / C::kStages) & 1) &&
-            (!k.active || k.uses < 2 || mbar_test(&pvdone[2 * x + (k.uses & 1)], ((k.uses - 2) >> 1) & 1))) {
+        if (k.nb > 0 && (k.j > 0 || kt_ready(qfull, k.i & 1)) && kt_ready(&kfull[k.g % C::kStages], (k.g / C::kStages) & 1) &&
+            (!k.active || k.uses < 2 || kt_ready(&pvdone[2 * x + (k.uses & 1)], ((k.uses - 2) >> 1) & 1))) {
           const uint32_t st = k.g % C::kStages;
           if (k.active) {
             tc_fence_after();
             // (a descriptor's low bits are its address / 16)
             const uint64_t b = smem_desc_sw128(smem_u32(sK + st * C::kTile));
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              tc_mma_f16(ts + (k.uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
-                         b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
-            tc_commit(&kempty[st]);
-            tc_commit(&sfull[2 * x + (k.uses & 1)]);
-            if ((int)k.j == k.nb - 1) tc_commit(qempty);
+              for (int kk = 0; kk < HD / 16; ++kk)
+                tc_mma_f16(ts + (k.uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
+                           b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+              tc_commit(&kempty[st]);
+              tc_commit(&sfull[2 * x + (k.uses & 1)]);
+              if ((int)k.j == k.nb - 1) tc_commit(qempty);
+            }
             ++k.uses;
-          } else {
+          } else if (elect_one()) {
             mbar_arrive(&kempty[st]);
             if ((int)k.j == k.nb - 1) mbar_arrive(qempty);
           }
+          __syncwarp();
           ++k.g;
           if ((int)++k.j == k.nb) {
             k.nb = 0;
@@ -496,32 +503,35 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           }
           went = true;
         }
-        if (v.nb == 0 && mbar_test(&dfull[v.i % kKtDescs], (v.i / kKtDescs) & 1)) {
+        if (v.nb == 0 && kt_ready(&dfull[v.i % kKtDescs], (v.i / kKtDescs) & 1)) {
           const KtDesc& D = descs[v.i % kKtDescs];
           v.nb = D.nb > 0 ? D.nb : -1;
           v.active = D.nr > 128 * x;
           v.j = 0;
         }
-        if (v.nb > 0 && v.g < k.g && mbar_test(&vfull[v.g % C::kStages], (v.g / C::kStages) & 1) &&
-            (!v.active || (mbar_test(&pfull[2 * x + (v.uses & 1)], (v.uses >> 1) & 1) &&
-                           (v.j > 0 || outs == 0 || mbar_test(&ofree[x], (outs - 1) & 1))))) {
+        if (v.nb > 0 && v.g < k.g && kt_ready(&vfull[v.g % C::kStages], (v.g / C::kStages) & 1) &&
+            (!v.active || (kt_ready(&pfull[2 * x + (v.uses & 1)], (v.uses >> 1) & 1) &&
+                           (v.j > 0 || outs == 0 || kt_ready(&ofree[x], (outs - 1) & 1))))) {
           const uint32_t st = v.g % C::kStages;
           if (v.active) {
             tc_fence_after();
             const uint64_t b = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kKv8Block / 16; ++kk)
-              tc_mma_f16_ts(to, ts + (v.uses & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, v.j > 0 || kk > 0);
-            tc_commit(&vempty[st]);
-            tc_commit(&pvdone[2 * x + (v.uses & 1)]);
+              for (int kk = 0; kk < kKv8Block / 16; ++kk)
+                tc_mma_f16_ts(to, ts + (v.uses & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, v.j > 0 || kk > 0);
+              tc_commit(&vempty[st]);
+              tc_commit(&pvdone[2 * x + (v.uses & 1)]);
+            }
             ++v.uses;
             if (v.j == 0) ++outs;
-          } else {
+          } else if (elect_one()) {
             mbar_arrive(&vempty[st]);
           }
+          __syncwarp();
           ++v.g;
           if ((int)++v.j == v.nb) {
-            mbar_arrive(&dempty[v.i % kKtDescs]);
+            if (elect_one()) mbar_arrive(&dempty[v.i % kKtDescs]);
             v.nb = 0;
             ++v.i;
           }
@@ -531,9 +541,9 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           waiting = 0;
         } else if ((++spins & 255) == 0) {
           const uint64_t now = globaltimer_ns();
-          if (waiting == 0) {
+          if (__all_sync(0xffffffffu, waiting == 0)) {
             waiting = now;
-          } else if (now - waiting > kWaitTimeoutNs) {
+          } else if (__any_sync(0xffffffffu, now - waiting > kWaitTimeoutNs)) {
             report_error(kErrMbarTimeout, 730);
             break;
           }
