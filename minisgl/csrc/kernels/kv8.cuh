@@ -15,27 +15,18 @@ MSGL_DEVICE void kv8_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* b
       : "memory");
 }
 
-// mbar_wait for waits that a stream of data goes through: the clock, which takes long to read, is looked at now and then only.
-MSGL_DEVICE bool kv8_wait(uint64_t* bar, uint32_t parity, int where) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
+// mbar_wait for the roles of a stream of data: few instructions (many such waits' code has to fit the instruction cache), and no
+// look at the clock, which takes long to read. A try takes some 100 cycles, so that a wait gives up after some seconds; the role
+// then ends, and says where by kv8_gave_up.
+MSGL_DEVICE bool kv8_wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 26); ++i)
     if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 0) {
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > kWaitTimeoutNs) {
-        report_error(kErrMbarTimeout, where);
-        return false;
-      }
-    }
-  }
+  return false;
 }
-
 // The same for a whole warp: its lanes go on or give up together.
-MSGL_DEVICE bool kv8_wait_warp(uint64_t* bar, uint32_t parity, int where) {
-  return __all_sync(0xffffffffu, kv8_wait(bar, parity, where));
-}
+MSGL_DEVICE bool kv8_wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kv8_wait(bar, parity)); }
+MSGL_DEVICE void kv8_gave_up(int where) { report_error(kErrMbarTimeout, where); }
 
 // two values to two e4m3 codes, nearest, ties to even (the first one in the low byte)
 MSGL_DEVICE uint16_t kv8_e4m3x2(float lo, float hi) {

@@ -120,7 +120,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       if (me == 0) {
         const int d = i % kKsDescs;
         if (lane == 0) {
-          ok = kv8_wait(&dempty[d], ((i / kKsDescs) & 1) ^ 1, 700);
+          ok = kv8_wait(&dempty[d], ((i / kKsDescs) & 1) ^ 1);
           if (ok) {
             const bool starts = from == 0, ends = to == k.nblk;
             KsDesc& D = descs[d];
@@ -160,7 +160,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
           if (j + mine * kKsCopies < to - from) next = look_up(j + mine * kKsCopies);
         }
         const uint32_t x = seq + j, stage = x % C::kStages;
-        ok = kv8_wait_warp(&empty[stage], ((x / C::kStages) & 1) ^ 1, 701);
+        ok = kv8_wait_warp(&empty[stage], ((x / C::kStages) & 1) ^ 1);
         if (!ok) break;
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
         kv8_copy_block<HD>(p, &tc, &ts, ring + stage * C::kStage, scales + stage * (C::kScales / 4), &full[stage], h, slots,
@@ -187,14 +187,15 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       }
     }
     if (ok) {
-      if (me == 0 && lane == 0 && kv8_wait(&dempty[i % kKsDescs], ((i / kKsDescs) & 1) ^ 1, 702)) {
+      if (me == 0 && lane == 0 && kv8_wait(&dempty[i % kKsDescs], ((i / kKsDescs) & 1) ^ 1)) {
         descs[i % kKsDescs].valid = 0;
         mbar_arrive(&dfull[i % kKsDescs]);
       }
-    } else if (lane == 0) {  // given up (and recorded): this warp's copies in flight land before the CTA's memory goes
+    } else if (lane == 0) {  // given up: this warp's copies in flight land before the CTA's memory goes
+      kv8_gave_up(700);
       for (int n = 0; n < min(issued, C::kStages / kKsCopies); ++n) {
         const uint32_t x = last - n * kKsCopies;
-        kv8_wait(&full[x % C::kStages], (x / C::kStages) & 1, 703);
+        kv8_wait(&full[x % C::kStages], (x / C::kStages) & 1);
       }
     }
     return;
@@ -211,7 +212,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   bool dead = false;
   for (int i = 0;; ++i) {
     const int d = i % kKsDescs;
-    if (!dead && !kv8_wait_warp(&dfull[d], (i / kKsDescs) & 1, 710)) { dead = true; *abort_flag = 1; }
+    if (!dead && !kv8_wait_warp(&dfull[d], (i / kKsDescs) & 1)) { dead = true; *abort_flag = 1; }
     if (!dead && !descs[d].valid) {
       named_bar_sync(1, kKsWarps * 32);  // (pairs with the barrier below of a warp that has given up)
       break;
@@ -272,7 +273,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
 
     for (int j = 0; j < D.nb && !dead; ++j) {
       const uint32_t at = seq + j, stage = at % C::kStages;
-      if (!kv8_wait_warp(&full[stage], (at / C::kStages) & 1, 711)) { dead = true; *abort_flag = 1; break; }
+      if (!kv8_wait_warp(&full[stage], (at / C::kStages) & 1)) { dead = true; *abort_flag = 1; break; }
       const uint8_t* st = ring + stage * C::kStage;
       const uint8_t* sc = reinterpret_cast<const uint8_t*>(scales) + stage * C::kScales;
       // S^T of keys g and g + 8 (c = 0, 1), rows 2 t and 2 t + 1 (e): s[x][2 c + e]
@@ -421,7 +422,10 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         }
       }
     named_bar_sync(1, kKsWarps * 32);
-    if (*abort_flag) break;
+    if (*abort_flag) {
+      if (dead) kv8_gave_up(710);
+      break;
+    }
     for (int idx = ctid; idx < D.nr * (HD / 4); idx += kKsWarps * 32) {
       const int rr = idx / (HD / 4), c4 = idx % (HD / 4);
       float mx = -INFINITY;

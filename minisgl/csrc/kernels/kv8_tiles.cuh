@@ -376,7 +376,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (to <= 0) break;  // (the run ends before the segment's first block)
       const int d = i % kKtDescs;
       if (lane == 0) {
-        ok = kv8_wait(&dempty[d], ((i / kKtDescs) & 1) ^ 1, 720);
+        ok = kv8_wait(&dempty[d], ((i / kKtDescs) & 1) ^ 1);
         if (ok) {
           const bool starts = from == 0, ends = to == k.nblk;
           KtDesc& D = descs[d];
@@ -407,7 +407,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           if (j + mine < to - from) next = look_up(j + mine);
         }
         const uint32_t x = seq + j, stage = x % C::kRaw;
-        ok = kv8_wait_warp(&rempty[stage], ((x / C::kRaw) & 1) ^ 1, 721);
+        ok = kv8_wait_warp(&rempty[stage], ((x / C::kRaw) & 1) ^ 1);
         if (!ok) {
           seq = x;
           break;
@@ -435,14 +435,15 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     }
     if (lane == 0) {
       if (ok) {
-        if (kv8_wait(&dempty[i % kKtDescs], ((i / kKtDescs) & 1) ^ 1, 722)) {
+        if (kv8_wait(&dempty[i % kKtDescs], ((i / kKtDescs) & 1) ^ 1)) {
           descs[i % kKtDescs].nb = 0;
           mbar_arrive(&dfull[i % kKtDescs]);
         }
-      } else {  // given up (and recorded): the copies in flight land before the CTA's memory goes
+      } else {  // given up: the copies in flight land before the CTA's memory goes
+        kv8_gave_up(720);
         for (uint32_t n = 1; n <= min(seq, (uint32_t)C::kRaw); ++n) {
           const uint32_t x = seq - n;
-          kv8_wait(&rfull[x % C::kRaw], (x / C::kRaw) & 1, 723);
+          kv8_wait(&rfull[x % C::kRaw], (x / C::kRaw) & 1);
         }
       }
     }
@@ -464,7 +465,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         bool active = false;
       } k, v;
       uint32_t outs = 0;  // segments whose O has begun
-      uint64_t waiting = 0;
       uint32_t spins = 0;
       while (v.nb >= 0) {
         bool went = false;
@@ -538,27 +538,23 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           went = true;
         }
         if (went) {
-          waiting = 0;
-        } else if ((++spins & 255) == 0) {
-          const uint64_t now = globaltimer_ns();
-          if (__all_sync(0xffffffffu, waiting == 0)) {
-            waiting = now;
-          } else if (__any_sync(0xffffffffu, now - waiting > kWaitTimeoutNs)) {
-            report_error(kErrMbarTimeout, 730);
-            break;
-          }
+          spins = 0;
+        } else if (++spins == 1u << 26) {
+          kv8_gave_up(730);
+          break;
         }
       }
       // no product is in flight when the CTA's memories go
-      if (k.uses > 0) kv8_wait(&sfull[2 * x + ((k.uses - 1) & 1)], ((k.uses - 1) >> 1) & 1, 738);
-      if (v.uses > 0) kv8_wait(&pvdone[2 * x + ((v.uses - 1) & 1)], ((v.uses - 1) >> 1) & 1, 739);
+      if (k.uses > 0) kv8_wait(&sfull[2 * x + ((k.uses - 1) & 1)], ((k.uses - 1) >> 1) & 1);
+      if (v.uses > 0) kv8_wait(&pvdone[2 * x + ((v.uses - 1) & 1)], ((v.uses - 1) >> 1) & 1);
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------------ queries into the L2 cache
     kt_fewer_regs<kKtRegsFew>();
+    bool ok = true;
     for (int i = 0;; ++i) {
       const int d = i % kKtDescs;
-      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 740)) break;
+      if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
       for (int rr = lane; rr < D.nr; rr += 32) {
@@ -570,6 +566,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(&dempty[d]);
     }
+    if (!ok) kv8_gave_up(740);
   } else if (warp < kKtConv) {
     // ------------------------------------------------------------------ softmax
     kt_more_regs<kKtRegsSoft>();
@@ -580,7 +577,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int d = i % kKtDescs;
-      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 750)) break;
+      if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
       if (D.nr <= 128 * x) {
@@ -589,7 +586,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         if (lane == 0) mbar_arrive(&dempty[d]);
         continue;
       }
-      if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1, 751))) break;
+      if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1))) break;
       KtRows w;
       int qpos[4];
       int least = INT_MAX, most = 0;  // of the warp's rows' positions
@@ -607,8 +604,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       most = __reduce_max_sync(0xffffffffu, most);
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
-        if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1, 752))) break;
-        if (!(ok = kv8_wait_warp(&scfull[g % kKtSlots], (g / kKtSlots) & 1, 753))) break;
+        if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1))) break;
+        if (!(ok = kv8_wait_warp(&scfull[g % kKtSlots], (g / kKtSlots) & 1))) break;
         tc_fence_after();
         const KtScales& sc = slots[g % kKtSlots];
         const int k0 = (D.blk + j) * kKv8Block;
@@ -631,7 +628,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
             }
         }
         if (j > 0 && moved) {  // once O holds the blocks before
-          if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1, 755))) break;
+          if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1))) break;
           tc_fence_after();
           float f = 1.f;  // of this lane's row of O
 #pragma unroll
@@ -670,7 +667,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         if (lane >> 3 == k) m = mk, l = lk;
       }
       // O out of tensor memory, 32 head dims at a time
-      if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1, 754))) break;
+      if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1))) break;
       tc_fence_after();
       const int head = D.h * G + r - tok * G;
       const float f = D.slot < 0 ? kv8_norm(m, l, p.sinks, in ? head : 0) : 1.f;
@@ -702,6 +699,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(&dempty[d]);
     }
+    if (!ok) kv8_gave_up(750);
   } else {
     // ------------------------------------------------------------------ conversions
     kt_fewer_regs<kKtRegsConv>();
@@ -713,12 +711,12 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const int d = i % kKtDescs;
-      if (!kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1, 760)) break;
+      if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
       // Queries: a thread takes its row of both tiles, first as it is into the operand's place, which is free once the last
       // segment's products with keys are done, then converted there.
-      if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1, 761))) break;
+      if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1))) break;
 #pragma unroll 1
       for (int x = 0; x < 2; ++x) {
         const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
@@ -758,7 +756,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
 
       for (int j = 0; j < D.nb; ++j, ++g) {
         const uint32_t rs = g % C::kRaw, st = g % C::kStages, ph = (g / C::kStages) & 1;
-        if (!(ok = kv8_wait_warp(&rfull[rs], (g / C::kRaw) & 1, 762))) break;
+        if (!(ok = kv8_wait_warp(&rfull[rs], (g / C::kRaw) & 1))) break;
         const int k0 = (D.blk + j) * kKv8Block;
         const bool partial = k0 < D.lo || k0 + kKv8Block > D.kend;  // some of the keys may be no positions
         const uint8_t* src = raw + rs * C::kRawStage;
@@ -795,7 +793,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         // keys, then values (one copy of the code)
 #pragma unroll 1
         for (int y = 0; y < 2; ++y) {
-          if (!(ok = kv8_wait_warp(&(y ? vempty : kempty)[st], ph ^ 1, 763))) break;
+          if (!(ok = kv8_wait_warp(&(y ? vempty : kempty)[st], ph ^ 1))) break;
           convert((y ? sV : sK) + st * C::kTile, order.codes ^ y);
           // scales: what used this slot before was over when its keys' products were
           if (y == 0 && row < kKv8Block) {  // (two whole warps)
@@ -822,6 +820,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(&dempty[d]);
     }
+    if (!ok) kv8_gave_up(760);
   }
   tc_fence_before();
   __syncthreads();
