@@ -106,29 +106,27 @@ MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// 16 lanes x 64 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
+// 16 lanes x 32 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
 // (registers 4n, 4n + 1) and g + 8 (4n + 2, 4n + 3) the columns 8n + 2t and the next.
-MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[32]) {
+MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-        "=r"(r[30]), "=r"(r[31])
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-// 16 lanes x 32 columns in the same order: lane (g, t) holds column 4n + t of rows g (register 2n) and g + 8 (2n + 1): fp16
+// 16 lanes x 16 columns in the same order: lane (g, t) holds column 4n + t of rows g (register 2n) and g + 8 (2n + 1): fp16
 // pairs of those S.
-MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+MSGL_DEVICE void kt_load_p(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
-
+MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // The same for 8 columns of S and 4 of its weights.
 MSGL_DEVICE void kt_load_s8(uint32_t taddr, uint32_t (&r)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
@@ -144,16 +142,17 @@ struct KtRows {
   int first[4], end[4];
 };
 
-// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop,
-// like all that not every block needs: unrolled it comes out of L2, and takes ten times its time.)
-MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
-  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+// The maxima of s_j + log2 s^v_j over the keys [from, to) of a block that the lane's rows see. (A compact loop, like all that not
+// every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
+MSGL_DEVICE void kt_tops(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, int from, int to, float (&top)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top[k] = -INFINITY;
 #pragma unroll 1
-  for (int n = 0; n < 8; ++n) {
-    const int c = 8 * n + 2 * t;
+  for (int n = from; n < to; n += 8) {
+    const int c = n + 2 * t;
     uint32_t u[2][4];
-    kt_load_s8(s_tmem + 8 * n, u[0]);
-    kt_load_s8(s_tmem + 8 * n + (16u << 16), u[1]);
+    kt_load_s8(s_tmem + n, u[0]);
+    kt_load_s8(s_tmem + n + (16u << 16), u[1]);
     const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), lv = *reinterpret_cast<const float2*>(&sc.lv[c]);
     tc_wait_ld();
 #pragma unroll
@@ -167,12 +166,54 @@ MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) 
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2)) - kKtTop;
-    if (top[k] > w.m[k]) {
-      w.alpha[k] = kv8_exp2(w.m[k] - top[k]);
-      w.m[k] = top[k];
-      w.l[k] *= w.alpha[k];
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+  }
+}
+
+// Offsets with which a block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one.
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
+  float top[4];
+  kt_tops(s_tmem, sc, w, t, 0, kKv8Block, top);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (top[k] - kKtTop > w.m[k]) {
+      const float f = kv8_exp2(w.m[k] - (top[k] - kKtTop));
+      w.m[k] = top[k] - kKtTop;
+      w.l[k] *= f;
+      w.alpha[k] *= f;
     }
+}
+
+// The same in the middle of a block, of whose halves the second, or the first, has weights beyond fp16: offsets grow by whole
+// numbers, so that the first half's weights, in fp16 already, change by powers of two.
+MSGL_DEVICE void kt_raise(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, int half) {
+  float top[4], f[4];
+  kt_tops(s_tmem, sc, w, t, half * 32, half * 32 + 32, top);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float by = fmaxf(floorf(top[k] - kKtTop - w.m[k]), 0.f);  // (the largest weight is 2^kKtTop at least)
+    f[k] = kv8_exp2(-by);
+    w.m[k] += by;
+    w.l[k] *= f[k];
+    w.alpha[k] *= f[k];
+  }
+  if (half == 1) {
+    tc_wait_st();
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      uint32_t pk[8];
+      kt_load_p(s_tmem + ((uint32_t)(16 * h) << 16), pk);
+      tc_wait_ld();
+      const float a = h ? f[2] : f[0], b = h ? f[3] : f[1];  // (in fp32: fp16 has no 2^-25)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&pk[n]));
+        const float y = n & 1 ? b : a;
+        pk[n] = pack_half(x.x * y, x.y * y);
+      }
+      kt_store_p(s_tmem + ((uint32_t)(16 * h) << 16), pk);
+    }
+    tc_wait_st();
   }
 }
 
@@ -202,79 +243,82 @@ MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows&
   }
 }
 
-// The weights of a block that every row sees, with the offsets as they are: fp16 pairs and this lane's sums of 2^(s_j - m).
-// Returns whether a weight is beyond 2^15, or a sum beyond 2^108.
-MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, float (&sum)[4], uint32_t (&pk)[2][16]) {
-  uint32_t u[2][32];
+// The weights of a block that every row sees, over S's columns: 32 keys at a time, the second 32's S on the way meanwhile. The
+// maximum of the logits is spared: an offset stays until a weight is beyond 2^15, or a sum beyond 2^108 (keys whose values are
+// nearly nothing), which few blocks' are. (One loop, not unrolled: it and all that every block goes through have to fit the
+// instruction caches.)
+MSGL_DEVICE void kt_weights(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool& moved) {
+  uint32_t u[2][16], next[2][16];
   kt_load_s(s_tmem, u[0]);
   kt_load_s(s_tmem + (16u << 16), u[1]);
-  uint64_t q2[4], b2[4], total[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
-    q2[k] = f2_pack(w.qs[k], w.qs[k]);
-    b2[k] = f2_pack(-base, -base);
-    total[k] = 0;
-  }
-  float top = 0.f;
   tc_wait_ld();
+  kt_load_s(s_tmem + 32, next[0]);
+  kt_load_s(s_tmem + 32 + (16u << 16), next[1]);
+  bool raised = false;
+#pragma unroll 1
+  for (int half = 0;;) {
+    uint64_t total[4];
+    uint32_t pk[2][8];
+    float top = 0.f;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const int c = 8 * n + 2 * t;
-    const uint64_t ks = *reinterpret_cast<const uint64_t*>(&sc.ks[c]), vs = *reinterpret_cast<const uint64_t*>(&sc.vs[c]);
+    for (int k = 0; k < 4; ++k) total[k] = 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = half * 32 + 8 * n + 2 * t;
+      const uint64_t ks = *reinterpret_cast<const uint64_t*>(&sc.ks[c]), vs = *reinterpret_cast<const uint64_t*>(&sc.vs[c]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
+        const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), f2_pack(w.qs[k], w.qs[k]),
+                                          f2_pack(-w.m[k], -w.m[k])));
+        const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
+        total[k] = f2_add(total[k], e2);
+        const float2 v = f2_unpack(f2_mul(e2, vs));
+        top = fmaxf(fmaxf(top, v.x), v.y);
+        pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
+      }
+    }
+    float sum[4];
+    bool beyond = !(top <= 32768.f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
-      const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), q2[k], b2[k]));
-      const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
-      total[k] = f2_add(total[k], e2);
-      const float2 v = f2_unpack(f2_mul(e2, vs));
-      top = fmaxf(fmaxf(top, v.x), v.y);
-      pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
+      const float2 a = f2_unpack(total[k]);
+      sum[k] = a.x + a.y;
+      beyond |= !(sum[k] <= 0x1p+108f);
     }
-  }
-  bool beyond = !(top <= 32768.f);
+    if (!raised && __any_sync(0xffffffffu, beyond)) {
+      // (once: with the new offsets nothing is beyond, except in rows that are no numbers)
+      kt_raise(s_tmem, sc, w, t, half);
+      raised = moved = true;
+      continue;
+    }
+    raised = false;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 a = f2_unpack(total[k]);
-    sum[k] = a.x + a.y;
-    beyond |= !(sum[k] <= 0x1p+108f);
+    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
+    kt_store_p(s_tmem + 16 * half, pk[0]);
+    kt_store_p(s_tmem + 16 * half + (16u << 16), pk[1]);
+    if (++half == 2) break;
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[0][i] = next[0][i], u[1][i] = next[1][i];
   }
-  return beyond;
 }
 
-// A block of the lane's rows, which see all of it or (`part`) not: their weights over S's columns. New offsets first where rows
-// have none (they have seen no key), or weights beyond fp16, or sums beyond 2^108 (keys whose values are nearly nothing): few
-// blocks need any, and the others are spared the maximum of their logits. Returns whether O has to be multiplied by anything.
+// A block of the lane's rows, which see all of it or (`part`) not. New offsets first where rows have none (they have seen no key).
+// Returns whether O has to be multiplied by anything.
 MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool part) {
-  float sum[4];
-  uint32_t pk[2][16];
-  bool moved = false, again = part;
+  bool moved = part;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     w.alpha[k] = 1.f;
-    again |= w.m[k] == -INFINITY;
+    moved |= w.m[k] == -INFINITY;
   }
-  again = __any_sync(0xffffffffu, again);
-#pragma unroll 1
-  for (;;) {
-    if (again) {
-      kt_move(s_tmem, sc, w, t);
-      moved = true;
-    }
-    if (part) break;
-    const bool beyond = kt_weights(s_tmem, sc, w, t, sum, pk);
-    again = !moved && __any_sync(0xffffffffu, beyond);
-    if (!again) break;
-  }
-  if (part) {
+  moved = __any_sync(0xffffffffu, moved);
+  if (moved) kt_move(s_tmem, sc, w, t);
+  if (part)
     kt_weights_in_part(s_tmem, sc, w, t);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
-    kt_store_p(s_tmem, pk[0]);
-    kt_store_p(s_tmem + (16u << 16), pk[1]);
-  }
+  else
+    kt_weights(s_tmem, sc, w, t, moved);
   return moved && __any_sync(0xffffffffu, w.alpha[0] != 1.f || w.alpha[1] != 1.f || w.alpha[2] != 1.f || w.alpha[3] != 1.f);
 }
 
@@ -450,103 +494,88 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   } else if (warp <= 2) {
     // ------------------------------------------------------------------ products of one tile
     kt_fewer_regs<kKtRegsFew>();
-    // Two streams, of products with keys and of products with values, each through all segments; whichever can go on does.
-    // (The whole warp goes through this and one lane is elected to issue: operands are then uniform, and a product costs a few
-    // cycles to issue instead of some 100.)
-    {
-      const int x = warp - 1;
-      const uint32_t ts = tmem + C::kS + x * 128, to = tmem + C::kO + x * 128;
-      const uint64_t q = smem_desc_sw128(smem_u32(smem + C::kOffQ + x * C::kQTile));
-      constexpr uint32_t idesc_s = kt_idesc(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
-      // of a stream: segment, block in it and in all, this tile's blocks; a segment has nb blocks, and this tile rows in it or not
-      struct {
-        uint32_t i = 0, j = 0, g = 0, uses = 0;
-        int nb = 0;  // 0: none at hand, -1: no more
-        bool active = false;
-      } k, v;
-      uint32_t outs = 0;  // segments whose O has begun
-      uint32_t spins = 0;
-      while (v.nb >= 0) {
-        bool went = false;
-        if (k.nb == 0 && kt_ready(&dfull[k.i % kKtDescs], (k.i / kKtDescs) & 1)) {
-          const KtDesc& D = descs[k.i % kKtDescs];
-          k.nb = D.nb > 0 ? D.nb : -1;
-          k.active = D.nr > 128 * x;
-          k.j = 0;
-        }
-        if (k.nb > 0 && (k.j > 0 || kt_ready(qfull, k.i & 1)) && kt_ready(&kfull[k.g % C::kStages], (k.g / C::kStages) & 1) &&
-            (!k.active || k.uses < 2 || kt_ready(&pvdone[2 * x + (k.uses & 1)], ((k.uses - 2) >> 1) & 1))) {
-          const uint32_t st = k.g % C::kStages;
-          if (k.active) {
-            tc_fence_after();
+    // Block after block through all segments: S of a block before O of the one before it, so that the softmax finds the next S
+    // when it is done with one. (The whole warp goes through this, and one lane is elected to issue.)
+    const int x = warp - 1;
+    const uint32_t ts = tmem + C::kS + x * 128, to = tmem + C::kO + x * 128;
+    const uint64_t q = smem_desc_sw128(smem_u32(smem + C::kOffQ + x * C::kQTile));
+    constexpr uint32_t idesc_s = kt_idesc(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
+    uint32_t g = 0, uses = 0, outs = 0;  // blocks, of them this tile's, its segments
+    int i = 0, j = 0, nb = 0;
+    bool ok = true, active = false;
+    // the block whose O is due
+    bool due = false, due_active = false, due_first = false, due_last = false;
+#pragma unroll 1
+    for (;;) {
+      if (j == nb) {  // the next segment
+        if (!(ok = kv8_wait_warp(&dfull[i % kKtDescs], (i / kKtDescs) & 1))) break;
+        nb = descs[i % kKtDescs].nb;
+        active = descs[i % kKtDescs].nr > 128 * x;
+        j = 0;
+        if (nb > 0 && !(ok = kv8_wait_warp(qfull, i & 1))) break;
+        ++i;
+      }
+      if (nb > 0) {
+        const uint32_t st = g % C::kStages;
+        if (!(ok = kv8_wait_warp(&kfull[st], (g / C::kStages) & 1))) break;
+        const int buf = 2 * x + (uses & 1);
+        if (active) {
+          if (uses >= 2 && !(ok = kv8_wait_warp(&pvdone[buf], ((uses - 2) >> 1) & 1))) break;
+          tc_fence_after();
+          if (elect_one()) {
             // (a descriptor's low bits are its address / 16)
             const uint64_t b = smem_desc_sw128(smem_u32(sK + st * C::kTile));
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < HD / 16; ++kk)
-                tc_mma_f16(ts + (k.uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
-                           b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
-              tc_commit(&kempty[st]);
-              tc_commit(&sfull[2 * x + (k.uses & 1)]);
-              if ((int)k.j == k.nb - 1) tc_commit(qempty);
-            }
-            ++k.uses;
-          } else if (elect_one()) {
-            mbar_arrive(&kempty[st]);
-            if ((int)k.j == k.nb - 1) mbar_arrive(qempty);
+#pragma unroll 1
+            for (int kk = 0; kk < HD / 16; ++kk)
+              tc_mma_f16(ts + (uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
+                         b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+            tc_commit(&kempty[st]);
+            tc_commit(&sfull[buf]);
+            if (j == nb - 1) tc_commit(qempty);
           }
-          __syncwarp();
-          ++k.g;
-          if ((int)++k.j == k.nb) {
-            k.nb = 0;
-            ++k.i;
-          }
-          went = true;
+          ++uses;
+        } else if (elect_one()) {
+          mbar_arrive(&kempty[st]);
+          if (j == nb - 1) mbar_arrive(qempty);
         }
-        if (v.nb == 0 && kt_ready(&dfull[v.i % kKtDescs], (v.i / kKtDescs) & 1)) {
-          const KtDesc& D = descs[v.i % kKtDescs];
-          v.nb = D.nb > 0 ? D.nb : -1;
-          v.active = D.nr > 128 * x;
-          v.j = 0;
-        }
-        if (v.nb > 0 && v.g < k.g && kt_ready(&vfull[v.g % C::kStages], (v.g / C::kStages) & 1) &&
-            (!v.active || (kt_ready(&pfull[2 * x + (v.uses & 1)], (v.uses >> 1) & 1) &&
-                           (v.j > 0 || outs == 0 || kt_ready(&ofree[x], (outs - 1) & 1))))) {
-          const uint32_t st = v.g % C::kStages;
-          if (v.active) {
-            tc_fence_after();
-            const uint64_t b = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < kKv8Block / 16; ++kk)
-                tc_mma_f16_ts(to, ts + (v.uses & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, v.j > 0 || kk > 0);
-              tc_commit(&vempty[st]);
-              tc_commit(&pvdone[2 * x + (v.uses & 1)]);
-            }
-            ++v.uses;
-            if (v.j == 0) ++outs;
-          } else if (elect_one()) {
-            mbar_arrive(&vempty[st]);
-          }
-          __syncwarp();
-          ++v.g;
-          if ((int)++v.j == v.nb) {
-            if (elect_one()) mbar_arrive(&dempty[v.i % kKtDescs]);
-            v.nb = 0;
-            ++v.i;
-          }
-          went = true;
-        }
-        if (went) {
-          spins = 0;
-        } else if (++spins == 1u << 26) {
-          kv8_gave_up(730);
-          break;
-        }
+        __syncwarp();
       }
-      // no product is in flight when the CTA's memories go
-      if (k.uses > 0) kv8_wait(&sfull[2 * x + ((k.uses - 1) & 1)], ((k.uses - 1) >> 1) & 1);
-      if (v.uses > 0) kv8_wait(&pvdone[2 * x + ((v.uses - 1) & 1)], ((v.uses - 1) >> 1) & 1);
+      if (due) {  // of block g - 1
+        const uint32_t st = (g - 1) % C::kStages;
+        if (!(ok = kv8_wait_warp(&vfull[st], ((g - 1) / C::kStages) & 1))) break;
+        if (due_active) {
+          const uint32_t u = uses - 1 - (nb > 0 && active ? 1 : 0);
+          if (due_first && outs > 0 && !(ok = kv8_wait_warp(&ofree[x], (outs - 1) & 1))) break;
+          if (!(ok = kv8_wait_warp(&pfull[2 * x + (u & 1)], (u >> 1) & 1))) break;
+          outs += due_first;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t b = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
+#pragma unroll 1
+            for (int kk = 0; kk < kKv8Block / 16; ++kk)
+              tc_mma_f16_ts(to, ts + (u & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, !due_first || kk > 0);
+            tc_commit(&vempty[st]);
+            tc_commit(&pvdone[2 * x + (u & 1)]);
+          }
+        } else if (elect_one()) {
+          mbar_arrive(&vempty[st]);
+        }
+        __syncwarp();
+        // (the segment's entry: this one's, or the one before where a new segment has begun)
+        if (due_last && elect_one()) mbar_arrive(&dempty[(i - 2) % kKtDescs]);
+      }
+      if (nb == 0) break;
+      due = true;
+      due_active = active;
+      due_first = j == 0;
+      due_last = ++j == nb;
+      ++g;
+    }
+    if (!ok && lane == 0) kv8_gave_up(730);
+    // no product is in flight when the CTA's memories go
+    if (uses > 0) {
+      kv8_wait_warp(&sfull[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1);
+      kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1);
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------------ queries into the L2 cache
