@@ -16,12 +16,21 @@ MSGL_DEVICE void kv8_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* b
 }
 
 // mbar_wait for the roles of a stream of data: few instructions (many such waits' code has to fit the instruction cache), and no
-// look at the clock, which takes long to read. A try takes some 100 cycles, so that a wait gives up after some seconds; the role
+// look at the clock, which takes long to read. A try takes 0.1 to 4 us, so that a wait gives up after 0.3 to 17 s; the role
 // then ends, and says where by kv8_gave_up.
 MSGL_DEVICE bool kv8_wait(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
-  for (uint32_t i = 0; i < (1u << 26); ++i)
-    if (mbar_try_wait(bar, parity)) return true;
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(4000u)  // (suspended for up to 4 us)
+        : "memory");
+    if (ok) return true;
+  }
   return false;
 }
 // The same for a whole warp: its lanes go on or give up together.

@@ -106,26 +106,27 @@ MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// 16 lanes x 32 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
+// 16 lanes x 64 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
 // (registers 4n, 4n + 1) and g + 8 (4n + 2, 4n + 3) the columns 8n + 2t and the next.
-MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[16]) {
+MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-// 16 lanes x 16 columns in the same order: lane (g, t) holds column 4n + t of rows g (register 2n) and g + 8 (2n + 1): fp16
+// 16 lanes x 32 columns in the same order: lane (g, t) holds column 4n + t of rows g (register 2n) and g + 8 (2n + 1): fp16
 // pairs of those S.
-MSGL_DEVICE void kt_load_p(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-}
-MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 // The same for 8 columns of S and 4 of its weights.
 MSGL_DEVICE void kt_load_s8(uint32_t taddr, uint32_t (&r)[4]) {
@@ -142,13 +143,14 @@ struct KtRows {
   int first[4], end[4];
 };
 
-// The maxima of s_j + log2 s^v_j over the keys [from, to) of a block that the lane's rows see. (A compact loop, like all that not
-// every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
-MSGL_DEVICE void kt_tops(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, int from, int to, float (&top)[4]) {
+// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop,
+// like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
+  float top[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) top[k] = -INFINITY;
 #pragma unroll 1
-  for (int n = from; n < to; n += 8) {
+  for (int n = 0; n < kKv8Block; n += 8) {
     const int c = n + 2 * t;
     uint32_t u[2][4];
     kt_load_s8(s_tmem + n, u[0]);
@@ -166,54 +168,13 @@ MSGL_DEVICE void kt_tops(uint32_t s_tmem, const KtScales& sc, const KtRows& w, i
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-  }
-}
-
-// Offsets with which a block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one.
-MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
-  float top[4];
-  kt_tops(s_tmem, sc, w, t, 0, kKv8Block, top);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (top[k] - kKtTop > w.m[k]) {
-      const float f = kv8_exp2(w.m[k] - (top[k] - kKtTop));
-      w.m[k] = top[k] - kKtTop;
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2)) - kKtTop;
+    if (top[k] > w.m[k]) {
+      const float f = kv8_exp2(w.m[k] - top[k]);
+      w.m[k] = top[k];
       w.l[k] *= f;
       w.alpha[k] *= f;
     }
-}
-
-// The same in the middle of a block, of whose halves the second, or the first, has weights beyond fp16: offsets grow by whole
-// numbers, so that the first half's weights, in fp16 already, change by powers of two.
-MSGL_DEVICE void kt_raise(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, int half) {
-  float top[4], f[4];
-  kt_tops(s_tmem, sc, w, t, half * 32, half * 32 + 32, top);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float by = fmaxf(floorf(top[k] - kKtTop - w.m[k]), 0.f);  // (the largest weight is 2^kKtTop at least)
-    f[k] = kv8_exp2(-by);
-    w.m[k] += by;
-    w.l[k] *= f[k];
-    w.alpha[k] *= f[k];
-  }
-  if (half == 1) {
-    tc_wait_st();
-#pragma unroll 1
-    for (int h = 0; h < 2; ++h) {
-      uint32_t pk[8];
-      kt_load_p(s_tmem + ((uint32_t)(16 * h) << 16), pk);
-      tc_wait_ld();
-      const float a = h ? f[2] : f[0], b = h ? f[3] : f[1];  // (in fp32: fp16 has no 2^-25)
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&pk[n]));
-        const float y = n & 1 ? b : a;
-        pk[n] = pack_half(x.x * y, x.y * y);
-      }
-      kt_store_p(s_tmem + ((uint32_t)(16 * h) << 16), pk);
-    }
-    tc_wait_st();
   }
 }
 
@@ -243,83 +204,77 @@ MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows&
   }
 }
 
-// The weights of a block that every row sees, over S's columns: 32 keys at a time, the second 32's S on the way meanwhile. The
-// maximum of the logits is spared: an offset stays until a weight is beyond 2^15, or a sum beyond 2^108 (keys whose values are
-// nearly nothing), which few blocks' are. (One loop, not unrolled: it and all that every block goes through have to fit the
-// instruction caches.)
-MSGL_DEVICE void kt_weights(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool& moved) {
-  uint32_t u[2][16], next[2][16];
+// The weights of a block that every row sees, as fp16 pairs, with the offsets as they are, and this lane's sums of 2^(s_j - m).
+// Returns whether a weight is beyond 2^15, or a sum beyond 2^108 (keys whose values are nearly nothing).
+MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, float (&sum)[4], uint32_t (&pk)[2][16]) {
+  uint32_t u[2][32];
   kt_load_s(s_tmem, u[0]);
   kt_load_s(s_tmem + (16u << 16), u[1]);
-  tc_wait_ld();
-  kt_load_s(s_tmem + 32, next[0]);
-  kt_load_s(s_tmem + 32 + (16u << 16), next[1]);
-  bool raised = false;
-#pragma unroll 1
-  for (int half = 0;;) {
-    uint64_t total[4];
-    uint32_t pk[2][8];
-    float top = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) total[k] = 0;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int c = half * 32 + 8 * n + 2 * t;
-      const uint64_t ks = *reinterpret_cast<const uint64_t*>(&sc.ks[c]), vs = *reinterpret_cast<const uint64_t*>(&sc.vs[c]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
-        const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), f2_pack(w.qs[k], w.qs[k]),
-                                          f2_pack(-w.m[k], -w.m[k])));
-        const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
-        total[k] = f2_add(total[k], e2);
-        const float2 v = f2_unpack(f2_mul(e2, vs));
-        top = fmaxf(fmaxf(top, v.x), v.y);
-        pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
-      }
-    }
-    float sum[4];
-    bool beyond = !(top <= 32768.f);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 a = f2_unpack(total[k]);
-      sum[k] = a.x + a.y;
-      beyond |= !(sum[k] <= 0x1p+108f);
-    }
-    if (!raised && __any_sync(0xffffffffu, beyond)) {
-      // (once: with the new offsets nothing is beyond, except in rows that are no numbers)
-      kt_raise(s_tmem, sc, w, t, half);
-      raised = moved = true;
-      continue;
-    }
-    raised = false;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
-    kt_store_p(s_tmem + 16 * half, pk[0]);
-    kt_store_p(s_tmem + 16 * half + (16u << 16), pk[1]);
-    if (++half == 2) break;
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) u[0][i] = next[0][i], u[1][i] = next[1][i];
-  }
-}
-
-// A block of the lane's rows, which see all of it or (`part`) not. New offsets first where rows have none (they have seen no key).
-// Returns whether O has to be multiplied by anything.
-MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool part) {
-  bool moved = part;
+  uint64_t q2[4], b2[4], total[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    w.alpha[k] = 1.f;
-    moved |= w.m[k] == -INFINITY;
+    const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
+    q2[k] = f2_pack(w.qs[k], w.qs[k]);
+    b2[k] = f2_pack(-base, -base);
+    total[k] = 0;
   }
-  moved = __any_sync(0xffffffffu, moved);
-  if (moved) kt_move(s_tmem, sc, w, t);
-  if (part)
+  float top = 0.f;
+  tc_wait_ld();
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const int c = 8 * n + 2 * t;
+    const uint64_t ks = *reinterpret_cast<const uint64_t*>(&sc.ks[c]), vs = *reinterpret_cast<const uint64_t*>(&sc.vs[c]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
+      const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), q2[k], b2[k]));
+      const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
+      total[k] = f2_add(total[k], e2);
+      const float2 v = f2_unpack(f2_mul(e2, vs));
+      top = fmaxf(fmaxf(top, v.x), v.y);
+      pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
+    }
+  }
+  bool beyond = !(top <= 32768.f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 a = f2_unpack(total[k]);
+    sum[k] = a.x + a.y;
+    beyond |= !(sum[k] <= 0x1p+108f);
+  }
+  return beyond;
+}
+
+// A block of the lane's rows, which see all of it or (`part`) not: their weights over S's columns. New offsets first where rows
+// have none (`fresh`: they have seen no key yet), or weights beyond fp16: few blocks need any, and the others are spared the
+// maximum of their logits. Returns whether the rows have got factors for O.
+MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool part, bool fresh) {
+  float sum[4];
+  uint32_t pk[2][16];
+  bool moved = false;
+  // (one copy of either step, for the instruction caches)
+#pragma unroll 1
+  for (bool again = part || fresh;;) {
+    if (again) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
+      kt_move(s_tmem, sc, w, t);
+      moved = true;
+      if (part) break;
+    }
+    const bool beyond = kt_weights(s_tmem, sc, w, t, sum, pk);
+    again = !moved && __any_sync(0xffffffffu, beyond);
+    if (!again) break;
+  }
+  if (part) {
     kt_weights_in_part(s_tmem, sc, w, t);
-  else
-    kt_weights(s_tmem, sc, w, t, moved);
-  return moved && __any_sync(0xffffffffu, w.alpha[0] != 1.f || w.alpha[1] != 1.f || w.alpha[2] != 1.f || w.alpha[3] != 1.f);
+  } else {
+    kt_store_p(s_tmem, pk[0]);
+    kt_store_p(s_tmem + (16u << 16), pk[1]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
+  }
+  return moved;
 }
 
 template <int HD, bool FP8>
@@ -355,7 +310,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   uint64_t* ofree = pvdone + 4;  // [tile]: O has been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofree + 2);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (a warp's number, known as one)
   if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
@@ -394,7 +349,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
   pdl_launch();
   if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
@@ -509,8 +464,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     for (;;) {
       if (j == nb) {  // the next segment
         if (!(ok = kv8_wait_warp(&dfull[i % kKtDescs], (i / kKtDescs) & 1))) break;
-        nb = descs[i % kKtDescs].nb;
-        active = descs[i % kKtDescs].nr > 128 * x;
+        nb = __shfl_sync(0xffffffffu, descs[i % kKtDescs].nb, 0);
+        active = __shfl_sync(0xffffffffu, descs[i % kKtDescs].nr, 0) > 128 * x;
         j = 0;
         if (nb > 0 && !(ok = kv8_wait_warp(qfull, i & 1))) break;
         ++i;
@@ -525,7 +480,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           if (elect_one()) {
             // (a descriptor's low bits are its address / 16)
             const uint64_t b = smem_desc_sw128(smem_u32(sK + st * C::kTile));
-#pragma unroll 1
+#pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
               tc_mma_f16(ts + (uses & 1) * 64, q + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4),
                          b + (((kk >> 2) * C::kHalf + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
@@ -551,7 +506,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           tc_fence_after();
           if (elect_one()) {
             const uint64_t b = smem_desc_sw128_mn(smem_u32(sV + st * C::kTile), C::kHalf);
-#pragma unroll 1
+#pragma unroll
             for (int kk = 0; kk < kKv8Block / 16; ++kk)
               tc_mma_f16_ts(to, ts + (u & 1) * 64 + kk * 8, b + (kk * 16 * 128 >> 4), idesc_o, !due_first || kk > 0);
             tc_commit(&vempty[st]);
@@ -631,6 +586,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       }
       least = __reduce_min_sync(0xffffffffu, least);
       most = __reduce_max_sync(0xffffffffu, most);
+      bool fresh = true;  // rows without an offset, or limits of another block
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
         if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1))) break;
@@ -640,12 +596,19 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         const int k0 = (D.blk + j) * kKv8Block;
         // does every row of the warp see every key?
         const bool part = !(least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0));
+        if (part || fresh) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          w.first[k] = part && p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
-          w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
+          for (int k = 0; k < 4; ++k) {
+            w.first[k] = part && p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
+            w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
+          }
         }
-        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, t4, part);
+        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, t4, part, fresh);
+        // (first and end stay those of a whole block until the next one that is seen in part)
+        if (part || fresh) {
+          fresh = __any_sync(0xffffffffu, w.m[0] == -INFINITY || w.m[1] == -INFINITY || w.m[2] == -INFINITY || w.m[3] == -INFINITY);
+          if (part) fresh = true;
+        }
         if ((sc.bad[0] | sc.bad[1]) != 0) {  // a key that has no finite scale makes the rows that see it no numbers
           const uint64_t bad = sc.bad[0] | (uint64_t)sc.bad[1] << 32;
 #pragma unroll 1
@@ -656,7 +619,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
                 if (c >= w.first[k] && c < w.end[k]) w.l[k] = __int_as_float(0x7fc00000);
             }
         }
-        if (j > 0 && moved) {  // once O holds the blocks before
+        if (j > 0 && moved && __any_sync(0xffffffffu, w.alpha[0] != 1.f || w.alpha[1] != 1.f || w.alpha[2] != 1.f || w.alpha[3] != 1.f)) {
+          // once O holds the blocks before
           if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1))) break;
           tc_fence_after();
           float f = 1.f;  // of this lane's row of O
