@@ -608,11 +608,12 @@ const int32_t* kv8_ids(const at::Tensor& t, int64_t n, const at::Device& dev, co
 }
 
 // rows of heads as the kernels read them: unit inner stride, every head's row on a 16-byte boundary; else a copy
-at::Tensor kv8_rows(const at::Tensor& x, int64_t heads, int64_t hd, const at::Device& dev, const char* name) {
+// (and, for a tensor map, rows that do not overlap)
+at::Tensor kv8_rows(const at::Tensor& x, int64_t heads, int64_t hd, const at::Device& dev, const char* name, int64_t least = 0) {
   CHECK(x.scalar_type() == at::kBFloat16 && x.dim() == 3 && (heads < 0 || x.size(1) == heads) && x.size(2) == hd && x.device() == dev,
         name, " must be bf16 [tokens, heads, ", hd, "] on the cache's device, got ", x.scalar_type(), " ", x.sizes(), " on ", x.device());
-  if (x.stride(2) == 1 && (x.size(0) <= 1 || x.stride(0) % 8 == 0) && (x.size(1) <= 1 || x.stride(1) % 8 == 0) &&
-      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
+  if (x.stride(2) == 1 && (x.size(0) <= 1 || (x.stride(0) % 8 == 0 && x.stride(0) >= least)) &&
+      (x.size(1) <= 1 || (x.stride(1) % 8 == 0 && x.stride(1) >= least)) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0)
     return x;
   return x.clone(at::MemoryFormat::Contiguous);
 }
@@ -662,10 +663,10 @@ std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tenso
   const at::Device dev = ck.device();
   const int64_t nkv = ck.size(0), hd = ck.size(2), B = rows.numel();
   c10::cuda::CUDAGuard guard(dev);
-  at::Tensor qr = kv8_rows(q, -1, hd, dev, "attention_kv8: q");
+  at::Tensor qr = kv8_rows(q, -1, hd, dev, "attention_kv8: q", hd);
   const int64_t T = q.size(0), nq = q.size(1);
   CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 128, "attention_kv8: ", nq, " query heads over ", nkv, " kv heads (1 to 128 each)");
-  CHECK(T * nq < (1ll << 31) && B < (1ll << 24), "attention_kv8: too many queries for one call");
+  CHECK(T * nq < (1ll << 30) && B < (1ll << 24), "attention_kv8: too many queries for one call");
   CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt && page_table.device() == dev &&
             (page_table.numel() == 0 || page_table.stride(1) == 1 || page_table.size(1) == 1) && page_table.size(0) < (1ll << 31) &&
             page_table.size(1) < (1ll << 31),
@@ -700,7 +701,7 @@ std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tenso
     o = new_cuda({T, nq, hd}, at::kBFloat16, dev);
   }
   if (T == 0) return {o, 0};
-  p.o = o.data_ptr(); p.q = qr.data_ptr(); p.q_row = qr.stride(0); p.q_head = qr.stride(1);
+  p.o = o.data_ptr(); p.q = qr.data_ptr(); p.q_row = T > 1 ? qr.stride(0) : nq * hd; p.q_head = nq > 1 ? qr.stride(1) : hd;
   p.ck = ck.data_ptr(); p.cv = cv.data_ptr(); p.sk = sk.data_ptr<float>(); p.sv = sv.data_ptr<float>();
   p.page_table = page_table.data_ptr<int32_t>(); p.pt_stride = page_table.stride(0);
   p.pt_rows = page_table.size(0); p.pt_width = page_table.size(1); p.num_slots = ck.size(1); p.num_reqs = B; p.total_q = T;

@@ -70,6 +70,25 @@ MSGL_DEVICE void kv8_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   }
 }
 
+// The same to two bf16 pairs, exactly: every code has at most 8 significant bits.
+template <bool FP8>
+MSGL_DEVICE void kv8_to_bf16(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    uint32_t a, b;
+    kv8_to_half<true>(codes, a, b);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = pack_bf16(x.x, x.y);
+    hi = pack_bf16(y.x, y.y);
+  } else {  // 128 + the low seven bits, less 128 or, with the sign bit, 256
+    const uint32_t a = __byte_perm(codes, 0x43434343u, 0x4140), b = __byte_perm(codes, 0x43434343u, 0x4342);
+    const uint32_t x = a & 0xff7fff7fu, y = a & 0xff80ff80u, z = b & 0xff7fff7fu, w = b & 0xff80ff80u;
+    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&z), *reinterpret_cast<const __nv_bfloat162*>(&w));
+    lo = *reinterpret_cast<const uint32_t*>(&c);
+    hi = *reinterpret_cast<const uint32_t*>(&d);
+  }
+}
+
 // 2^x, to 2^-22 of it (2^-126 and below: zero)
 MSGL_DEVICE float kv8_exp2(float x) {
   float y;

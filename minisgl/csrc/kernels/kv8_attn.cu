@@ -48,6 +48,18 @@ bool encode_cache(CUtensorMap* tc, CUtensorMap* ts, Kv8Order* order, const Kv8At
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries [total_q][nq][HD] bf16 in boxes of 64 head dims of the heads of a group, of as many tokens as a tile holds.
+bool encode_queries(CUtensorMap* m, const Kv8Attn& p, int hd) {
+  const Kv8EncodeFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const int G = p.nq / p.nkv;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)p.nq, (cuuint64_t)p.total_q};
+  const cuuint64_t strides[2] = {(cuuint64_t)p.q_head * 2, (cuuint64_t)p.q_row * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)}, ones[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int sm_count() {
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
@@ -83,12 +95,12 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
     return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs >= kKtRegs;
   }();
   if (!fits) return 4;
-  CUtensorMap tc, ts;
+  CUtensorMap tc, ts, tq;
   Kv8Order order;
-  if (!encode_cache(&tc, &ts, &order, p, HD)) return 2;
+  if (!encode_cache(&tc, &ts, &order, p, HD) || !encode_queries(&tq, p, HD)) return 2;
   const int ctas = sm_count();
   const Kv8Scratch scratch = kv8_scratch<kKtRows, HD>(ws, ctas);
-  if (msgl_launch(kernel, dim3(ctas), dim3(kKtThreads), C::kSmem, s, 1, tc, ts, p, order, scratch) != cudaSuccess) return 4;
+  if (msgl_launch(kernel, dim3(ctas), dim3(kKtThreads), C::kSmem, s, 1, tc, ts, tq, p, order, scratch) != cudaSuccess) return 4;
   ++*launches;
   if (msgl_launch(kv8_join_kernel<kKtRows, HD>, dim3(ctas, 8), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
   ++*launches;

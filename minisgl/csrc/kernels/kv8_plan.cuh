@@ -51,8 +51,7 @@ MSGL_DEVICE int kv8_checked(const Kv8Attn& p, int slot) {
 struct Kv8Tile {
   int r0, nr, pos0, pos1, lo, kend, blk0, nblk;
 };
-template <int R>
-MSGL_DEVICE Kv8Tile kv8_tile(const Kv8Attn& p, const Kv8Req& r, int G, int t) {
+MSGL_DEVICE Kv8Tile kv8_tile(const Kv8Attn& p, const Kv8Req& r, int G, int R, int t) {
   Kv8Tile k;
   k.r0 = t * R;
   k.nr = min(R, r.n * G - k.r0);
@@ -64,10 +63,7 @@ MSGL_DEVICE Kv8Tile kv8_tile(const Kv8Attn& p, const Kv8Req& r, int G, int t) {
   k.nblk = max(1, (k.kend > 0 ? (k.kend - 1) / kKv8Block + 1 : 0) - k.blk0);
   return k;
 }
-template <int R>
-MSGL_DEVICE int kv8_tiles(const Kv8Req& r, int G) {
-  return (int)(((int64_t)r.n * G + R - 1) / R);
-}
+MSGL_DEVICE int kv8_tiles(const Kv8Req& r, int G, int R) { return (r.n * G - 1 + R) / R; }  // (r.n * G + 256 fits: rows are less than 2^30)
 
 // A CTA's run of units [u0, u1), and the segment that u0 is in: tile t of head h of request b, from unit s0 on.
 struct Kv8Plan {
@@ -82,8 +78,8 @@ MSGL_DEVICE int kv8_cta_of(const Kv8Plan& pl, int64_t u) {
 }
 
 // All NT threads of the CTA; `red` holds NT / 32 words. A run has at least `least` units.
-template <int R, int COST, int NT>
-MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red) {
+template <int COST, int NT>
+MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int R, int least, Kv8Plan* pl, int64_t* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.nq / p.nkv;
   const int rounds = (p.num_reqs + NT - 1) / NT;
   int64_t base = 0, v = 0, excl = 0, run0 = 0, run1 = 0;
@@ -94,8 +90,8 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
     v = 0;
     if (b < p.num_reqs) {
       r = kv8_request(p, b);
-      const int tiles = kv8_tiles<R>(r, G);
-      for (int t = 0; t < tiles; ++t) v += kv8_tile<R>(p, r, G, t).nblk + COST;
+      const int tiles = kv8_tiles(r, G, R);
+      for (int t = 0; t < tiles; ++t) v += kv8_tile(p, r, G, R, t).nblk + COST;
       v *= p.nkv;
     }
     int64_t incl = v;
@@ -126,7 +122,7 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int least, Kv8Plan* pl, int64_t* red
     pl->h = h;
     rem -= h * per;
     for (int t = 0;; ++t) {
-      const int units = kv8_tile<R>(p, r, G, t).nblk + COST;
+      const int units = kv8_tile(p, r, G, R, t).nblk + COST;
       if (rem < units) {
         pl->t = t;
         break;

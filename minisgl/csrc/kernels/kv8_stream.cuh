@@ -94,7 +94,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   pdl_wait();
   pdl_launch();
   if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
-  kv8_plan<R, kKsCost, kKsThreads>(p, kKsCost + 2, plan, red);  // (its barriers order the initialisation above as well)
+  kv8_plan<kKsCost, kKsThreads>(p, R, kKsCost + 2, plan, red);  // (its barriers order the initialisation above as well)
   const Kv8Plan pl = *plan;
   const int G = p.nq / p.nkv;
   kv8_zero_tail<HD>(p, threadIdx.x, kKsThreads);
@@ -109,11 +109,11 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     int64_t u = pl.u0, s0 = pl.s0;
     bool ok = true;
     Kv8Req r = pl.r;
-    if (u < pl.u1) tiles = kv8_tiles<R>(r, G);
+    if (u < pl.u1) tiles = kv8_tiles(r, G, R);
     int i = 0, issued = 0;
     uint32_t last = 0;
     for (; ok && u < pl.u1; ++i) {
-      const Kv8Tile k = kv8_tile<R>(p, r, G, t);
+      const Kv8Tile k = kv8_tile(p, r, G, R, t);
       // blocks [from, to) of the segment: its first kKsCost units are none
       const int from = (int)max(u - s0 - kKsCost, (int64_t)0), to = (int)min((int64_t)k.nblk, pl.u1 - s0 - kKsCost);
       if (to <= 0) break;  // (the run ends before the segment's first block)
@@ -180,7 +180,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
           do {
             if (++b >= p.num_reqs) break;  // (never: units are left)
             r = kv8_request(p, b);
-            tiles = kv8_tiles<R>(r, G);
+            tiles = kv8_tiles(r, G, R);
           } while (tiles == 0);
           if (b >= p.num_reqs) u = pl.u1;
         }

@@ -1,16 +1,16 @@
 // Attention over the 8-bit cache for many rows per request and kv head: chunks of prompts, drafted tokens of wide groups.
 //
-// One CTA per SM takes segments of 256 packed rows (see kv8_plan.cuh), two tiles of 128 rows that share every key and
-// value block, 64 keys at a time, on the 5th-generation tensor core:
+// One CTA per SM takes segments of up to 256 packed rows (see kv8_plan.cuh), two tiles of up to 128 rows, whole tokens each,
+// that share every key and value block, 64 keys at a time, on the 5th-generation tensor core:
 //
 //   warp 0        goes through the run's segments, publishes them, copies raw pages into a ring by TMA
 //   warps 1, 2    issue the products of one tile each: S = Q K^T a block ahead, and, once the weights are there, O += P V, P out
 //                 of tensor memory
-//   warp 3        fetches the next segments' queries into the L2 cache
+//   warp 3        copies the segments' queries, as they are, by TMA
 //   warps 4 - 11  softmax, 32 rows a warp, four rows and 16 keys a lane: S out of tensor memory, weights as fp16 over S's columns, O rescaled there
 //                 when a row's offset grows by more than 2^(15 - kKtTop), O read out and written at the segment's end
-//   warps 12 - 15 convert: queries to fp16 at a segment's start, then codes to fp16 operand tiles (exact),
-//                 once for both tiles, and scales to what the softmax wants of them
+//   warps 12 - 15 convert codes to operand tiles, once for both tiles of rows: keys to bf16, which is the queries' type, values to
+//                 fp16, which has the more bits for the weights (exact, both), and scales to what the softmax wants of them
 //
 // A block's S and its weights share 64 columns of tensor memory, and each tile has two such: S 2 x 2 x 64 columns, O 2 x 128. (With
 // Q in tensor memory instead of shared memory there is room for one only; less shared memory is read then, but a tile's
@@ -62,12 +62,11 @@ struct KtCfg {
   static constexpr int kOffRaw = kOffQ + 2 * kQTile;
   static constexpr int kOffSc = kOffRaw + kRaw * kRawStage;
   static constexpr int kOffSlots = kOffSc + kRaw * kRawScales;
-  static constexpr int kOffQs = kOffSlots + kKtSlots * (int)sizeof(KtScales);
-  static constexpr int kOffDesc = kOffQs + kKtDescs * kKtRows * 4;
+  static constexpr int kOffDesc = kOffSlots + kKtSlots * (int)sizeof(KtScales);
   static constexpr int kOffPlan = kOffDesc + kKtDescs * (int)sizeof(KtDesc);
   static constexpr int kOffRed = kOffPlan + (int)sizeof(Kv8Plan);
   static constexpr int kOffBars = kOffRed + 8 * (kKtThreads / 32);
-  static constexpr int kBars = 4 * kStages + 2 * kRaw + kKtSlots + 3 * kKtDescs + 2 + 3 * 4 + 2;
+  static constexpr int kBars = 4 * kStages + 2 * kRaw + kKtSlots + 2 * kKtDescs + 2 + 3 * 4 + 2;
   static constexpr int kSmem = 1024 + kOffBars + 8 * kBars + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
   // tensor memory columns
@@ -76,8 +75,10 @@ struct KtCfg {
 
 constexpr uint32_t kt_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }  // fp16 operands, fp32 sums
 
-// Has this phase completed? The same answer for all of the warp.
-MSGL_DEVICE bool kt_ready(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); }
+MSGL_DEVICE void kt_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 
 // pairs of fp32 in one register pair
 MSGL_DEVICE uint64_t f2_pack(float a, float b) {
@@ -128,41 +129,45 @@ MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// The same for 8 columns of S and 4 of its weights.
-MSGL_DEVICE void kt_load_s8(uint32_t taddr, uint32_t (&r)[4]) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+// The same for 16 columns of S and 8 of its weights.
+MSGL_DEVICE void kt_load_s16(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
-MSGL_DEVICE void kt_store_p8(uint32_t taddr, uint32_t a, uint32_t b) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x1.b32 [%0], {%1,%2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
+MSGL_DEVICE void kt_store_p8(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
 }
 
-// A lane's four rows, 8 apart: their queries' factors, running offsets and this lane's part of their sums, the keys of the
+// A lane's four rows, 8 apart: their running offsets and this lane's part of their sums, the keys of the
 // block that they see, [first, end), and what their O has to be multiplied by first.
 struct KtRows {
-  float qs[4], m[4], l[4], alpha[4];
+  float m[4], l[4], alpha[4];
   int first[4], end[4];
 };
 
 // Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop,
 // like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
-MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
-  float top[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) top[k] = -INFINITY;
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-  for (int n = 0; n < kKv8Block; n += 8) {
-    const int c = n + 2 * t;
-    uint32_t u[2][4];
-    kt_load_s8(s_tmem + n, u[0]);
-    kt_load_s8(s_tmem + n + (16u << 16), u[1]);
-    const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), lv = *reinterpret_cast<const float2*>(&sc.lv[c]);
+  for (int n = 0; n < kKv8Block; n += 16) {
+    uint32_t u[2][8];
+    kt_load_s16(s_tmem + n, u[0]);
+    kt_load_s16(s_tmem + n + (16u << 16), u[1]);
     tc_wait_ld();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t* s = &u[k >> 1][2 * (k & 1)];
-      const float x = fmaf(__uint_as_float(s[0]) * ks.x, w.qs[k], lv.x), y = fmaf(__uint_as_float(s[1]) * ks.y, w.qs[k], lv.y);
-      if (c >= w.first[k] && c < w.end[k]) top[k] = fmaxf(top[k], x);
-      if (c + 1 >= w.first[k] && c + 1 < w.end[k]) top[k] = fmaxf(top[k], y);
+    for (int y = 0; y < 2; ++y) {
+      const int c = n + 8 * y + 2 * t;
+      const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), lv = *reinterpret_cast<const float2*>(&sc.lv[c]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t* s = &u[k >> 1][4 * y + 2 * (k & 1)];
+        const float a = fmaf(__uint_as_float(s[0]) * ks.x, qs, lv.x), b = fmaf(__uint_as_float(s[1]) * ks.y, qs, lv.y);
+        if (c >= w.first[k] && c < w.end[k]) top[k] = fmaxf(top[k], a);
+        if (c + 1 >= w.first[k] && c + 1 < w.end[k]) top[k] = fmaxf(top[k], b);
+      }
     }
   }
 #pragma unroll
@@ -179,46 +184,49 @@ MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) 
 }
 
 // The weights of a block that some of the lane's rows see in part only, over S's columns.
-MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t) {
+MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t) {
 #pragma unroll 1
-  for (int n = 0; n < 8; ++n) {
-    const int c = 8 * n + 2 * t;
-    uint32_t u[2][4], pk[4];
-    kt_load_s8(s_tmem + 8 * n, u[0]);
-    kt_load_s8(s_tmem + 8 * n + (16u << 16), u[1]);
-    const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), vs = *reinterpret_cast<const float2*>(&sc.vs[c]);
+  for (int n = 0; n < kKv8Block; n += 16) {
+    uint32_t u[2][8], pk[2][4];
+    kt_load_s16(s_tmem + n, u[0]);
+    kt_load_s16(s_tmem + n + (16u << 16), u[1]);
     tc_wait_ld();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t* s = &u[k >> 1][2 * (k & 1)];
-      const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
-      float x = kv8_exp2(fmaf(__uint_as_float(s[0]) * ks.x, w.qs[k], -base)), y = kv8_exp2(fmaf(__uint_as_float(s[1]) * ks.y, w.qs[k], -base));
-      if (!(c >= w.first[k] && c < w.end[k])) x = 0.f;
-      if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) y = 0.f;
-      w.l[k] += x + y;
-      pk[k] = pack_half(x * vs.x, y * vs.y);
+    for (int y = 0; y < 2; ++y) {
+      const int c = n + 8 * y + 2 * t;
+      const float2 ks = *reinterpret_cast<const float2*>(&sc.ks[c]), vs = *reinterpret_cast<const float2*>(&sc.vs[c]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t* s = &u[k >> 1][4 * y + 2 * (k & 1)];
+        const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
+        float a = kv8_exp2(fmaf(__uint_as_float(s[0]) * ks.x, qs, -base)), b = kv8_exp2(fmaf(__uint_as_float(s[1]) * ks.y, qs, -base));
+        if (!(c >= w.first[k] && c < w.end[k])) a = 0.f;
+        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) b = 0.f;
+        w.l[k] += a + b;
+        pk[k >> 1][2 * y + (k & 1)] = pack_half(a * vs.x, b * vs.y);
+      }
     }
-    // (the columns it overwrites have been read: keys 4n .. 4n + 3)
-    kt_store_p8(s_tmem + 4 * n, pk[0], pk[1]);
-    kt_store_p8(s_tmem + 4 * n + (16u << 16), pk[2], pk[3]);
+    // (the columns it overwrites have been read: keys n / 2 .. n / 2 + 7)
+    kt_store_p8(s_tmem + n / 2, pk[0]);
+    kt_store_p8(s_tmem + n / 2 + (16u << 16), pk[1]);
   }
 }
 
 // The weights of a block that every row sees, as fp16 pairs, with the offsets as they are, and this lane's sums of 2^(s_j - m).
 // Returns whether a weight is beyond 2^15, or a sum beyond 2^108 (keys whose values are nearly nothing).
-MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w, int t, float (&sum)[4], uint32_t (&pk)[2][16]) {
+MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w, float qs, int t, float (&sum)[4], uint32_t (&pk)[2][16]) {
   uint32_t u[2][32];
   kt_load_s(s_tmem, u[0]);
   kt_load_s(s_tmem + (16u << 16), u[1]);
-  uint64_t q2[4], b2[4], total[4];
+  const uint64_t q2 = f2_pack(qs, qs);
+  uint64_t b2[4], total[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
-    q2[k] = f2_pack(w.qs[k], w.qs[k]);
     b2[k] = f2_pack(-base, -base);
     total[k] = 0;
   }
-  float top = 0.f;
+  __half2 top = __float2half2_rn(0.f);
   tc_wait_ld();
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
@@ -227,15 +235,16 @@ MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t* s = &u[k >> 1][4 * n + 2 * (k & 1)];
-      const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), q2[k], b2[k]));
+      const float2 x = f2_unpack(f2_fma(f2_mul(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), ks), q2, b2[k]));
       const uint64_t e2 = f2_pack(kv8_exp2(x.x), kv8_exp2(x.y));
       total[k] = f2_add(total[k], e2);
       const float2 v = f2_unpack(f2_mul(e2, vs));
-      top = fmaxf(fmaxf(top, v.x), v.y);
-      pk[k >> 1][2 * n + (k & 1)] = pack_half(v.x, v.y);
+      const uint32_t h = pack_half(v.x, v.y);
+      top = __hmax2(top, *reinterpret_cast<const __half2*>(&h));
+      pk[k >> 1][2 * n + (k & 1)] = h;
     }
   }
-  bool beyond = !(top <= 32768.f);
+  bool beyond = !__hble2(top, __float2half2_rn(32768.f));
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float2 a = f2_unpack(total[k]);
@@ -248,7 +257,7 @@ MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w
 // A block of the lane's rows, which see all of it or (`part`) not: their weights over S's columns. New offsets first where rows
 // have none (`fresh`: they have seen no key yet), or weights beyond fp16: few blocks need any, and the others are spared the
 // maximum of their logits. Returns whether the rows have got factors for O.
-MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int t, bool part, bool fresh) {
+MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, bool part, bool fresh) {
   float sum[4];
   uint32_t pk[2][16];
   bool moved = false;
@@ -258,16 +267,16 @@ MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int 
     if (again) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
-      kt_move(s_tmem, sc, w, t);
+      kt_move(s_tmem, sc, w, qs, t);
       moved = true;
       if (part) break;
     }
-    const bool beyond = kt_weights(s_tmem, sc, w, t, sum, pk);
+    const bool beyond = kt_weights(s_tmem, sc, w, qs, t, sum, pk);
     again = !moved && __any_sync(0xffffffffu, beyond);
     if (!again) break;
   }
   if (part) {
-    kt_weights_in_part(s_tmem, sc, w, t);
+    kt_weights_in_part(s_tmem, sc, w, qs, t);
   } else {
     kt_store_p(s_tmem, pk[0]);
     kt_store_p(s_tmem + (16u << 16), pk[1]);
@@ -279,7 +288,7 @@ MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, int 
 
 template <int HD, bool FP8>
 __global__ void __launch_bounds__(kKtThreads, 1)
-kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
+kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__ CUtensorMap ts, const __grid_constant__ CUtensorMap tq, Kv8Attn p, Kv8Order order, Kv8Scratch scratch) {
   using C = KtCfg<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -288,7 +297,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   uint8_t* raw = smem + C::kOffRaw;
   float* raw_scales = reinterpret_cast<float*>(smem + C::kOffSc);
   KtScales* slots = reinterpret_cast<KtScales*>(smem + C::kOffSlots);
-  float* qscale = reinterpret_cast<float*>(smem + C::kOffQs);  // [kKtDescs][256]
   KtDesc* descs = reinterpret_cast<KtDesc*>(smem + C::kOffDesc);
   Kv8Plan* plan = reinterpret_cast<Kv8Plan*>(smem + C::kOffPlan);
   int64_t* red = reinterpret_cast<int64_t*>(smem + C::kOffRed);
@@ -301,8 +309,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   uint64_t* scfull = rempty + C::kRaw;
   uint64_t* dfull = scfull + kKtSlots;
   uint64_t* dempty = dfull + kKtDescs;
-  uint64_t* qsfull = dempty + kKtDescs;
-  uint64_t* qfull = qsfull + kKtDescs;
+  uint64_t* qfull = dempty + kKtDescs;
   uint64_t* qempty = qfull + 1;
   uint64_t* sfull = qempty + 1;  // [tile][buffer]: S is there
   uint64_t* pfull = sfull + 4;   // its weights are
@@ -327,9 +334,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       for (int i = 0; i < kKtDescs; ++i) {
         mbar_init(&dfull[i], 1);
         mbar_init(&dempty[i], 2 + 1 + 8 + 4);
-        mbar_init(&qsfull[i], 4);
       }
-      mbar_init(qfull, 4);
+      mbar_init(qfull, 1);
       mbar_init(qempty, 2);
       for (int i = 0; i < 4; ++i) {
         mbar_init(&sfull[i], 1);
@@ -345,7 +351,14 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   } else if (warp == 0 && lane == 0) {
     prefetch_tmap(&tc);
     prefetch_tmap(&ts);
+    prefetch_tmap(&tq);
   }
+  const int G = p.nq / p.nkv, tokens = 128 / G, trows = tokens * G, R = 2 * trows;  // of a tile, of a segment
+  for (int i = threadIdx.x; i < (128 - trows) * 8 * 2 * (HD / 64); i += kKtThreads) {  // rows that no query is copied to
+    const int half = i / ((128 - trows) * 8), at = i % ((128 - trows) * 8);
+    *reinterpret_cast<uint4*>(smem + C::kOffQ + half * C::kQHalf + trows * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -353,9 +366,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   pdl_wait();
   pdl_launch();
   if (threadIdx.x == 0) scratch.head[blockIdx.x].parts = 0;
-  kv8_plan<kKtRows, kKtCost, kKtThreads>(p, kKtCost + 2, plan, red);
+  kv8_plan<kKtCost, kKtThreads>(p, R, kKtCost + 2, plan, red);
   const Kv8Plan pl = *plan;
-  const int G = p.nq / p.nkv;
   kv8_zero_tail<HD>(p, threadIdx.x, kKtThreads);
 
   if (warp == 0) {
@@ -367,9 +379,9 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     int64_t u = pl.u0, s0 = pl.s0;
     bool ok = true;
     Kv8Req r = pl.r;
-    if (u < pl.u1) tiles = kv8_tiles<kKtRows>(r, G);
+    if (u < pl.u1) tiles = kv8_tiles(r, G, R);
     for (; ok && u < pl.u1; ++i) {
-      const Kv8Tile k = kv8_tile<kKtRows>(p, r, G, t);
+      const Kv8Tile k = kv8_tile(p, r, G, R, t);
       // blocks [from, to) of the segment: its first kKtCost units are none
       const int from = (int)max(u - s0 - kKtCost, (int64_t)0), to = (int)min((int64_t)k.nblk, pl.u1 - s0 - kKtCost);
       if (to <= 0) break;  // (the run ends before the segment's first block)
@@ -426,7 +438,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           do {
             if (++b >= p.num_reqs) break;  // (never: units are left)
             r = kv8_request(p, b);
-            tiles = kv8_tiles<kKtRows>(r, G);
+            tiles = kv8_tiles(r, G, R);
           } while (tiles == 0);
           if (b >= p.num_reqs) u = pl.u1;
         }
@@ -454,7 +466,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     const int x = warp - 1;
     const uint32_t ts = tmem + C::kS + x * 128, to = tmem + C::kO + x * 128;
     const uint64_t q = smem_desc_sw128(smem_u32(smem + C::kOffQ + x * C::kQTile));
-    constexpr uint32_t idesc_s = kt_idesc(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
+    constexpr uint32_t idesc_s = idesc_bf16_f32(128, kKv8Block), idesc_o = kt_idesc(128, HD) | kIdescBMajorMN;
     uint32_t g = 0, uses = 0, outs = 0;  // blocks, of them this tile's, its segments
     int i = 0, j = 0, nb = 0;
     bool ok = true, active = false;
@@ -465,7 +477,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (j == nb) {  // the next segment
         if (!(ok = kv8_wait_warp(&dfull[i % kKtDescs], (i / kKtDescs) & 1))) break;
         nb = __shfl_sync(0xffffffffu, descs[i % kKtDescs].nb, 0);
-        active = __shfl_sync(0xffffffffu, descs[i % kKtDescs].nr, 0) > 128 * x;
+        active = __shfl_sync(0xffffffffu, descs[i % kKtDescs].nr, 0) > trows * x;
         j = 0;
         if (nb > 0 && !(ok = kv8_wait_warp(qfull, i & 1))) break;
         ++i;
@@ -533,30 +545,39 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1);
     }
   } else if (warp == 3) {
-    // ------------------------------------------------------------------ queries into the L2 cache
+    // ------------------------------------------------------------------ queries
     kt_fewer_regs<kKtRegsFew>();
     bool ok = true;
-    for (int i = 0;; ++i) {
+    int i = 0;
+#pragma unroll 1
+    for (;; ++i) {
       const int d = i % kKtDescs;
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      for (int rr = lane; rr < D.nr; rr += 32) {
-        const int r = D.r0 + rr, tok = r / G;
-        const char* src = reinterpret_cast<const char*>(p.q) + 2 * ((D.q0 + tok) * p.q_row + (int64_t)(D.h * G + r - tok * G) * p.q_head);
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
-        if (HD == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 128));
+      const int tiles = D.nr > trows ? 2 : 1, tok = D.q0 + D.r0 / G;
+      // into the L2 cache, while the last segment's are still in use
+      if (i > 0 && lane < tiles * (HD / 64)) kt_prefetch_3d(&tq, lane % (HD / 64) * 64, D.h * G, tok + lane / (HD / 64) * tokens);
+      if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1))) break;
+      if (elect_one()) {
+        mbar_expect_tx(qfull, tiles * trows * HD * 2);
+        for (int y = 0; y < tiles * (HD / 64); ++y)
+          tma_load_3d(smem + C::kOffQ + y * C::kQHalf, &tq, qfull, y % (HD / 64) * 64, D.h * G, tok + y / (HD / 64) * tokens);
+        mbar_arrive(&dempty[d]);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&dempty[d]);
     }
-    if (!ok) kv8_gave_up(740);
+    if (!ok) {  // given up: the copies in flight land before the CTA's memory goes
+      if (lane == 0) kv8_gave_up(740);
+      if (i > 0) kv8_wait_warp(qfull, (i - 1) & 1);
+    }
   } else if (warp < kKtConv) {
     // ------------------------------------------------------------------ softmax
     kt_more_regs<kKtRegsSoft>();
     const int x = (warp - kKtSoft) >> 2, row = (warp & 3) * 32 + lane, t4 = lane & 3;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + C::kS + x * 128 + lane_base, to = tmem + C::kO + x * 128 + lane_base;
+    const float qs = p.scale * kKv8Log2e;
     uint32_t g = 0, uses = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -564,28 +585,29 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      if (D.nr <= 128 * x) {
+      if (D.nr <= trows * x) {
         g += D.nb;
         __syncwarp();
         if (lane == 0) mbar_arrive(&dempty[d]);
         continue;
       }
-      if (!(ok = kv8_wait_warp(&qsfull[d], (i / kKtDescs) & 1))) break;
       KtRows w;
       int qpos[4];
       int least = INT_MAX, most = 0;  // of the warp's rows' positions
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int rr = x * 128 + (warp & 3) * 32 + (lane >> 2) + 8 * k;
-        const bool in = rr < D.nr;
-        w.qs[k] = in ? qscale[d * kKtRows + rr] : 0.f;
-        w.m[k] = in ? -INFINITY : 0.f;
+        const int rr = (warp & 3) * 32 + (lane >> 2) + 8 * k;
+        const bool in = rr < trows && x * trows + rr < D.nr;
+        w.m[k] = -INFINITY;
         w.l[k] = 0.f;
-        qpos[k] = in ? D.L - D.n + (D.r0 + rr) / G : -1;
+        qpos[k] = in ? D.L - D.n + (D.r0 + x * trows + rr) / G : INT_MIN;
         if (in) least = min(least, qpos[k]), most = max(most, qpos[k]);
       }
       least = __reduce_min_sync(0xffffffffu, least);
       most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (qpos[k] == INT_MIN) qpos[k] = most;  // (a row that is none: as the last one)
       bool fresh = true;  // rows without an offset, or limits of another block
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
@@ -603,7 +625,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
             w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
           }
         }
-        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, t4, part, fresh);
+        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, qs, t4, part, fresh);
         // (first and end stay those of a whole block until the next one that is seen in part)
         if (part || fresh) {
           fresh = __any_sync(0xffffffffu, w.m[0] == -INFINITY || w.m[1] == -INFINITY || w.m[2] == -INFINITY || w.m[3] == -INFINITY);
@@ -647,8 +669,8 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       }
       if (!ok) break;
       // from here on a lane has one row
-      const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
-      const bool in = rr < D.nr;
+      const int rr = x * trows + row, r = D.r0 + rr, tok = r / G;
+      const bool in = row < trows && rr < D.nr;
       float m = 0.f, l = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -707,53 +729,13 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      // Queries: a thread takes its row of both tiles, first as it is into the operand's place, which is free once the last
-      // segment's products with keys are done, then converted there.
-      if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1))) break;
-#pragma unroll 1
-      for (int x = 0; x < 2; ++x) {
-        const int rr = x * 128 + row, r = D.r0 + rr, tok = r / G;
-        const bool in = rr < D.nr;
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
-                                                          (in ? (D.q0 + tok) * p.q_row + (int64_t)(D.h * G + r - tok * G) * p.q_head : 0));
-        uint8_t* dst = smem + C::kOffQ + x * C::kQTile + row * 128;
-        uint32_t top = 0;
-#pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
-          uint4 u[8];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) u[y] = in ? __ldg(src + 8 * c + y) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[y].x & 0x7fff7fffu, u[y].y & 0x7fff7fffu), __vmaxu2(u[y].z & 0x7fff7fffu, u[y].w & 0x7fff7fffu)));
-            *reinterpret_cast<uint4*>(dst + c * C::kQHalf + ((y ^ (row & 7)) << 4)) = u[y];
-          }
-        }
-        top = max(top & 0xffffu, top >> 16);
-        const float f = kv8_q_factor(__uint_as_float(top << 16));
-        qscale[d * kKtRows + rr] = p.scale * kKv8Log2e * kv8_reciprocal(f);
-#pragma unroll 2
-        for (int c = 0; c < HD / 8; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(dst + (c >> 3) * C::kQHalf + ((c & 7) << 4));  // (any order: the row is the thread's own)
-          const uint4 v = *at;
-          *at = make_uint4(pack_half(bf16_lo(v.x) * f, bf16_hi(v.x) * f), pack_half(bf16_lo(v.y) * f, bf16_hi(v.y) * f),
-                           pack_half(bf16_lo(v.z) * f, bf16_hi(v.z) * f), pack_half(bf16_lo(v.w) * f, bf16_hi(v.w) * f));
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&qsfull[d]);
-      if (!ok) break;
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qfull);
-
       for (int j = 0; j < D.nb; ++j, ++g) {
         const uint32_t rs = g % C::kRaw, st = g % C::kStages, ph = (g / C::kStages) & 1;
         if (!(ok = kv8_wait_warp(&rfull[rs], (g / C::kRaw) & 1))) break;
         const int k0 = (D.blk + j) * kKv8Block;
         const bool partial = k0 < D.lo || k0 + kKv8Block > D.kend;  // some of the keys may be no positions
         const uint8_t* src = raw + rs * C::kRawStage;
-        auto convert = [&](uint8_t* dst, int which) {
+        auto convert = [&](uint8_t* dst, int which, bool values) {
           // groups of 8 keys, w and w + 4 of them this warp's, and of 64 head dims
           uint4 v[2][HD / 64];
 #pragma unroll
@@ -773,10 +755,17 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
               uint4 a, b;
-              kv8_to_half<FP8>(v[y][c].x, a.x, a.y);
-              kv8_to_half<FP8>(v[y][c].y, a.z, a.w);
-              kv8_to_half<FP8>(v[y][c].z, b.x, b.y);
-              kv8_to_half<FP8>(v[y][c].w, b.z, b.w);
+              if (values) {
+                kv8_to_half<FP8>(v[y][c].x, a.x, a.y);
+                kv8_to_half<FP8>(v[y][c].y, a.z, a.w);
+                kv8_to_half<FP8>(v[y][c].z, b.x, b.y);
+                kv8_to_half<FP8>(v[y][c].w, b.z, b.w);
+              } else {
+                kv8_to_bf16<FP8>(v[y][c].x, a.x, a.y);
+                kv8_to_bf16<FP8>(v[y][c].y, a.z, a.w);
+                kv8_to_bf16<FP8>(v[y][c].z, b.x, b.y);
+                kv8_to_bf16<FP8>(v[y][c].w, b.z, b.w);
+              }
               uint8_t* o = dst + c * C::kHalf + ((w + 4 * y) * 8 + key8) * 128;
               *reinterpret_cast<uint4*>(o + (((2 * part) ^ key8) << 4)) = a;
               *reinterpret_cast<uint4*>(o + (((2 * part + 1) ^ key8) << 4)) = b;
@@ -787,7 +776,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
 #pragma unroll 1
         for (int y = 0; y < 2; ++y) {
           if (!(ok = kv8_wait_warp(&(y ? vempty : kempty)[st], ph ^ 1))) break;
-          convert((y ? sV : sK) + st * C::kTile, order.codes ^ y);
+          convert((y ? sV : sK) + st * C::kTile, order.codes ^ y, y);
           // scales: what used this slot before was over when its keys' products were
           if (y == 0 && row < kKv8Block) {  // (two whole warps)
             const float* sc = raw_scales + rs * (C::kRawScales / 4) + row + (row & ~(p.page - 1));

@@ -171,7 +171,7 @@ def attention_kv8(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor, ro
     T, nq, hd = q.shape
     if nq < 1 or nq % cache.num_kv_heads or nq // cache.num_kv_heads > 128:
         raise ValueError(f"attention_kv8: {nq} query heads over {cache.num_kv_heads} kv heads (1 to 128 each)")
-    if T * nq >= 2**31 or B >= 2**24:
+    if T * nq >= 2**30 or B >= 2**24:
         raise ValueError("attention_kv8: too many queries for one call")
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != cache.device or (
             page_table.numel() and page_table.stride(1) != 1):
