@@ -147,12 +147,12 @@ struct KtRows {
   int first[4], end[4];
 };
 
-// Offsets with which this block's largest weight is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop,
-// like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
-MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t) {
+// Offsets with which the largest weight of this block's first `keys` is 2^kKtTop (see kKv8Top), for the rows that have a lower
+// one. (A compact loop, like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, int keys) {
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-  for (int n = 0; n < kKv8Block; n += 16) {
+  for (int n = 0; n < keys; n += 16) {
     uint32_t u[2][8];
     kt_load_s16(s_tmem + n, u[0]);
     kt_load_s16(s_tmem + n + (16u << 16), u[1]);
@@ -260,20 +260,22 @@ MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w
 MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, bool part, bool fresh) {
   float sum[4];
   uint32_t pk[2][16];
-  bool moved = false;
-  // (one copy of either step, for the instruction caches)
+  // offsets after this many keys: a row's first ones are those of 16 keys, mostly near enough
+  int keys = part ? kKv8Block : fresh ? 16 : 0, moves = 0;
 #pragma unroll 1
-  for (bool again = part || fresh;;) {
-    if (again) {
+  for (;;) {
+    if (keys > 0) {
+      if (moves == 0) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
-      kt_move(s_tmem, sc, w, qs, t);
-      moved = true;
+        for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
+      }
+      kt_move(s_tmem, sc, w, qs, t, keys);
+      ++moves;
       if (part) break;
     }
     const bool beyond = kt_weights(s_tmem, sc, w, qs, t, sum, pk);
-    again = !moved && __any_sync(0xffffffffu, beyond);
-    if (!again) break;
+    if (keys == kKv8Block || !__any_sync(0xffffffffu, beyond)) break;
+    keys = kKv8Block;
   }
   if (part) {
     kt_weights_in_part(s_tmem, sc, w, qs, t);
@@ -283,7 +285,7 @@ MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, floa
 #pragma unroll
     for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
   }
-  return moved;
+  return moves > 0;
 }
 
 template <int HD, bool FP8>
@@ -625,7 +627,16 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
             w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
           }
         }
-        const bool moved = kt_softmax(ts + (uses & 1) * 64, sc, w, qs, t4, part, fresh);
+        bool moved = false;
+        if (k0 > most || (p.window > 0 && k0 + kKv8Block - 1 <= least - p.window)) {  // no row sees a key of this block
+          uint32_t none[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) none[k] = 0;
+          kt_store_p(ts + (uses & 1) * 64, none);
+          kt_store_p(ts + (uses & 1) * 64 + (16u << 16), none);
+        } else {
+          moved = kt_softmax(ts + (uses & 1) * 64, sc, w, qs, t4, part, fresh);
+        }
         // (first and end stay those of a whole block until the next one that is seen in part)
         if (part || fresh) {
           fresh = __any_sync(0xffffffffu, w.m[0] == -INFINITY || w.m[1] == -INFINITY || w.m[2] == -INFINITY || w.m[3] == -INFINITY);
