@@ -150,6 +150,7 @@ typedef struct {
   int window;     // keys a query sees at most, -1: all up to its own
   int zero_tail;  // rows behind the last request's are set to zero
   float scale;
+  unsigned group_mul, group_shift;  // (set by the call) x / (nq / nkv) = x group_mul >> group_shift for x < 2^30
 } Kv8Attn;
 int64_t msgl_kv8_attention_workspace(const Kv8Attn* p, int hd, int max_q_len);  // bytes, written before they are read
 int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, void* workspace, int* launches, cudaStream_t s);

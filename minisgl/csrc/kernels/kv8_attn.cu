@@ -107,15 +107,19 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
   return 0;
 }
 
-// The form for what the caller has told of a request's rows: 8, 16: rows of a streaming tile, 256: tensor core tiles.
-int form_of(const Kv8Attn& p, int max_q_len) {
+// The form for what the caller has told of a request's rows: 8, 16: rows of a streaming tile, 256: tensor core tiles. A request
+// of more rows than a streaming tile has its keys streamed (out of the L2 cache) and converted once for each tile, which
+// the tensor core form does once for 256 rows, but at its own pace. Measured with 16 requests of 6000 keys, 8 kv heads, int8, us
+// by rows, tiles of 8, of 16, tensor core: head dim 128: 8: 47, 58, 131; 16: 78, 59, 134; 32: 143, 101, 136; 48: 208, 144, 145; 64: 273,
+// 187, 145; head dim 64: 8: 35, 41, 125; 16: 58, 41, 128; 48: 151, 99, 132; 64: 197, 127, 134; 96: 290, 186, 140.
+int form_of(const Kv8Attn& p, int hd, int max_q_len) {
   const int64_t rows = (int64_t)max_q_len * (p.nq / p.nkv);
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
+  return rows <= 8 ? 8 : rows <= (hd == 128 ? 48 : 64) ? 16 : 256;
 }
 
 template <int HD, bool FP8>
 int any_form(const Kv8Attn& p, int max_q_len, void* ws, int* launches, cudaStream_t s) {
-  switch (form_of(p, max_q_len)) {
+  switch (form_of(p, HD, max_q_len)) {
     case 8: return stream_form<HD, FP8, 1>(p, ws, launches, s);
     case 16: return stream_form<HD, FP8, 2>(p, ws, launches, s);
     default: return tiles_form<HD, FP8>(p, ws, launches, s);
@@ -131,13 +135,20 @@ int64_t workspace(int form) {
 }  // namespace
 
 extern "C" int64_t msgl_kv8_attention_workspace(const Kv8Attn* p, int hd, int max_q_len) {
-  return hd == 128 ? workspace<128>(form_of(*p, max_q_len)) : workspace<64>(form_of(*p, max_q_len));
+  return hd == 128 ? workspace<128>(form_of(*p, hd, max_q_len)) : workspace<64>(form_of(*p, hd, max_q_len));
 }
 
-extern "C" int msgl_kv8_attention(const Kv8Attn* p, int hd, int fp8, int max_q_len, void* ws, int* launches, cudaStream_t s) {
+extern "C" int msgl_kv8_attention(const Kv8Attn* args, int hd, int fp8, int max_q_len, void* ws, int* launches, cudaStream_t s) {
   *launches = 0;
-  if (hd == 128) return fp8 ? any_form<128, true>(*p, max_q_len, ws, launches, s) : any_form<128, false>(*p, max_q_len, ws, launches, s);
-  if (hd == 64) return fp8 ? any_form<64, true>(*p, max_q_len, ws, launches, s) : any_form<64, false>(*p, max_q_len, ws, launches, s);
+  Kv8Attn p = *args;
+  // with s = 30 + ceil(log2 G) and mul = ceil(2^s / G), x mul / 2^s is x / G and less than x / 2^s more, too little to reach
+  // the next whole number
+  const uint64_t G = p.nq / p.nkv;
+  p.group_shift = 30;
+  while ((G << 30) > (1ull << p.group_shift)) ++p.group_shift;
+  p.group_mul = (unsigned)(((1ull << p.group_shift) + G - 1) / G);
+  if (hd == 128) return fp8 ? any_form<128, true>(p, max_q_len, ws, launches, s) : any_form<128, false>(p, max_q_len, ws, launches, s);
+  if (hd == 64) return fp8 ? any_form<64, true>(p, max_q_len, ws, launches, s) : any_form<64, false>(p, max_q_len, ws, launches, s);
   return 3;
 }
 

@@ -37,6 +37,9 @@ MSGL_DEVICE Kv8Req kv8_request(const Kv8Attn& p, int b) {
   return r;
 }
 
+// Packed row x of a request: its token.
+MSGL_DEVICE int kv8_token(const Kv8Attn& p, int x) { return (int)((uint64_t)(uint32_t)x * p.group_mul >> p.group_shift); }
+
 // A page's first slot as the table has it, or -1 if there is no such page (recorded).
 MSGL_DEVICE int kv8_checked(const Kv8Attn& p, int slot) {
   if (slot < 0 || slot > p.num_slots - p.page || slot % p.page != 0) {
@@ -55,8 +58,8 @@ MSGL_DEVICE Kv8Tile kv8_tile(const Kv8Attn& p, const Kv8Req& r, int G, int R, in
   Kv8Tile k;
   k.r0 = t * R;
   k.nr = min(R, r.n * G - k.r0);
-  k.pos0 = r.L - r.n + k.r0 / G;
-  k.pos1 = r.L - r.n + (k.r0 + k.nr - 1) / G;
+  k.pos0 = r.L - r.n + kv8_token(p, k.r0);
+  k.pos1 = r.L - r.n + kv8_token(p, k.r0 + k.nr - 1);
   k.kend = max(0, k.pos1 + 1);
   k.lo = p.window > 0 ? max(0, max(k.pos0, -1) - p.window + 1) : 0;
   k.blk0 = k.lo / kKv8Block;
@@ -81,19 +84,26 @@ MSGL_DEVICE int kv8_cta_of(const Kv8Plan& pl, int64_t u) {
 template <int COST, int NT>
 MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int R, int least, Kv8Plan* pl, int64_t* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.nq / p.nkv;
-  const int rounds = (p.num_reqs + NT - 1) / NT;
+  // `per` threads for each request, a power of two: they take its tiles in turn
+  int per = 1;
+  while (per < 32 && 2 * per * (int64_t)p.num_reqs <= NT) per *= 2;
+  const int sub = lane & (per - 1), at_once = NT / per, rounds = (p.num_reqs + at_once - 1) / at_once;
   int64_t base = 0, v = 0, excl = 0, run0 = 0, run1 = 0;
+  int tiles = 0;
   Kv8Req r;
-  // one round over the requests, NT at a time: v the units of request (round, tid), excl those before it
+  // one round over the requests, `at_once` at a time: v the units of request (round, tid / per), in its first thread, excl those
+  // before it
   auto scan = [&](int c) {
-    const int b = c * NT + tid;
+    const int b = c * at_once + tid / per;
     v = 0;
+    tiles = 0;
     if (b < p.num_reqs) {
       r = kv8_request(p, b);
-      const int tiles = kv8_tiles(r, G, R);
-      for (int t = 0; t < tiles; ++t) v += kv8_tile(p, r, G, R, t).nblk + COST;
-      v *= p.nkv;
+      tiles = kv8_tiles(r, G, R);
+      for (int t = sub; t < tiles; t += per) v += kv8_tile(p, r, G, R, t).nblk + COST;
     }
+    for (int o = per / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = sub == 0 ? v * p.nkv : 0;
     int64_t incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -113,23 +123,33 @@ MSGL_DEVICE void kv8_plan(const Kv8Attn& p, int R, int least, Kv8Plan* pl, int64
     base += all;
   };
   auto place = [&](int c) {
+    v = __shfl_sync(0xffffffffu, v, lane - sub);
+    excl = __shfl_sync(0xffffffffu, excl, lane - sub);
     if (run0 < excl || run0 >= excl + v || run0 >= run1) return;
-    const int64_t per = v / p.nkv;
+    // the threads of the request that the run begins in: its head, then its tile, `per` at a time
+    const unsigned group = (per == 32 ? 0xffffffffu : (1u << per) - 1) << (lane - sub);
+    const int64_t head = v / p.nkv;
     int64_t rem = run0 - excl;
-    pl->b = c * NT + tid;
-    pl->r = r;
-    const int h = v <= UINT32_MAX ? (int)((uint32_t)rem / (uint32_t)per) : (int)(rem / per);
-    pl->h = h;
-    rem -= h * per;
-    for (int t = 0;; ++t) {
-      const int units = kv8_tile(p, r, G, R, t).nblk + COST;
-      if (rem < units) {
-        pl->t = t;
-        break;
+    const int h = v <= UINT32_MAX ? (int)((uint32_t)rem / (uint32_t)head) : (int)(rem / head);
+    rem -= h * head;
+    for (int t0 = 0; t0 < tiles; t0 += per) {
+      const int t = t0 + sub, units = t < tiles ? kv8_tile(p, r, G, R, t).nblk + COST : 0;
+      int64_t incl = units;
+      for (int o = 1; o < per; o <<= 1) {
+        const int64_t x = __shfl_up_sync(group, incl, o, per);
+        if (sub >= o) incl += x;
       }
-      rem -= units;
+      if (rem >= incl - units && rem < incl) {
+        pl->b = c * at_once + tid / per;
+        pl->r = r;
+        pl->h = h;
+        pl->t = t;
+        pl->s0 = run0 - (rem - (incl - units));
+      }
+      const int64_t sum = __shfl_sync(group, incl, per - 1, per);
+      if (rem < sum) break;
+      rem -= sum;
     }
-    pl->s0 = run0 - rem;
   };
   for (int c = 0; c < rounds; ++c) scan(c);
   const int64_t total = base;
@@ -232,7 +252,7 @@ MSGL_DEVICE void kv8_zero_tail(const Kv8Attn& p, int tid, int threads) {
 
 template <int R, int HD>
 MSGL_DEVICE void kv8_join_row(const Kv8Attn& p, const Kv8Scratch& s, const Kv8Part& hd, int c, int i, int lane, int G) {
-  const int r = hd.r0 + i, head = hd.h * G + r % G;
+  const int r = hd.r0 + i, tok = kv8_token(p, r), head = hd.h * G + r - tok * G;
   // part 0 ends its CTA's run, the others begin theirs: slots 2 c + 1, 2 (c + 1), 2 (c + 2), ..
   constexpr int E = HD / 32;
   float m = -INFINITY, l = 0.f, acc[E];
@@ -261,7 +281,7 @@ MSGL_DEVICE void kv8_join_row(const Kv8Attn& p, const Kv8Scratch& s, const Kv8Pa
     }
   }
   const float f = kv8_norm(m, warp_sum(l), p.sinks, head);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.o) + ((int64_t)(hd.q0 + r / G) * p.nq + head) * (HD / 2) + lane * (E / 2);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.o) + ((int64_t)(hd.q0 + tok) * p.nq + head) * (HD / 2) + lane * (E / 2);
 #pragma unroll
   for (int e = 0; e < E; e += 2) dst[e / 2] = pack_bf16(acc[e] * f, acc[e + 1] * f);
 }

@@ -138,7 +138,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
       } else if (lane < k.nr) {  // the segment's queries are wanted when the ones before it are done
-        const int rr = k.r0 + lane, tok = rr / G;
+        const int rr = k.r0 + lane, tok = kv8_token(p, rr);
         const char* src = reinterpret_cast<const char*>(p.q) + 2 * ((r.q0 + tok) * p.q_row + (int64_t)(h * G + rr - tok * G) * p.q_head);
         asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
         if (HD == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 128));
@@ -227,7 +227,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     int qpos[NR][2];
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
-      const int rr = g + 8 * x, r = D.r0 + rr, tok = r / G;
+      const int rr = g + 8 * x, r = D.r0 + rr, tok = kv8_token(p, r);
       const bool in = !dead && rr < D.nr;
       uint4 u[HD / 32];
 #pragma unroll
@@ -446,7 +446,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         acc.x += fw * v.x; acc.y += fw * v.y; acc.z += fw * v.z; acc.w += fw * v.w;
       }
       if (D.slot < 0) {
-        const int r = D.r0 + rr, tok = r / G, head = D.h * G + r - tok * G;
+        const int r = D.r0 + rr, tok = kv8_token(p, r), head = D.h * G + r - tok * G;
         const float f = kv8_norm(mx, ll, p.sinks, head);
         reinterpret_cast<uint2*>(p.o)[((int64_t)(D.q0 + tok) * p.nq + head) * (HD / 4) + c4] =
             make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));

@@ -557,7 +557,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
-      const int tiles = D.nr > trows ? 2 : 1, tok = D.q0 + D.r0 / G;
+      const int tiles = D.nr > trows ? 2 : 1, tok = D.q0 + kv8_token(p, D.r0);
       // into the L2 cache, while the last segment's are still in use
       if (i > 0 && lane < tiles * (HD / 64)) kt_prefetch_3d(&tq, lane % (HD / 64) * 64, D.h * G, tok + lane / (HD / 64) * tokens);
       if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1))) break;
@@ -602,7 +602,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         const bool in = rr < trows && x * trows + rr < D.nr;
         w.m[k] = -INFINITY;
         w.l[k] = 0.f;
-        qpos[k] = in ? D.L - D.n + (D.r0 + x * trows + rr) / G : INT_MIN;
+        qpos[k] = in ? D.L - D.n + kv8_token(p, D.r0 + x * trows + rr) : INT_MIN;
         if (in) least = min(least, qpos[k]), most = max(most, qpos[k]);
       }
       least = __reduce_min_sync(0xffffffffu, least);
@@ -680,7 +680,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       }
       if (!ok) break;
       // from here on a lane has one row
-      const int rr = x * trows + row, r = D.r0 + rr, tok = r / G;
+      const int rr = x * trows + row, r = D.r0 + rr, tok = kv8_token(p, r);
       const bool in = row < trows && rr < D.nr;
       float m = 0.f, l = 0.f;
 #pragma unroll

@@ -132,7 +132,7 @@ def test_nothing_to_do():
 
 # ------------------------------------------------------------------------------- attention
 # the form is chosen by max_q_len: both hold for every batch
-HINTS = [1, 1000]
+HINTS = [1, 6, 1000]
 
 
 @pytest.mark.parametrize("hint", HINTS)
