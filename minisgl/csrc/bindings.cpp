@@ -584,6 +584,19 @@ struct Kv8Tensors {
   at::Tensor k, v, k_scale, v_scale;
 };
 
+// bytes that a tensor lies in
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
+  int64_t last = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {a, a + last * t.element_size()};
+}
+
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  const auto a = span_of(x), b = span_of(y);
+  return a.first < b.second && b.first < a.second;
+}
+
 // the cache's tensors (ops.KV8Cache checks the same when it is made); returns whether the codes are e4m3
 bool kv8_check(const Kv8Tensors& c) {
   check_cuda(c.k, "cache");
@@ -598,6 +611,7 @@ bool kv8_check(const Kv8Tensors& c) {
   for (const at::Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale})
     CHECK(t->device() == c.k.device() && t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
           "8-bit cache: codes and scales must be contiguous, 16-byte aligned and on one device");
+  CHECK(!overlap(c.k, c.v) && !overlap(c.k_scale, c.v_scale), "8-bit cache: keys and values must not share memory");
   return fp8;
 }
 
@@ -647,14 +661,6 @@ std::tuple<at::Tensor, at::Tensor> load_kv8(at::Tensor ck, at::Tensor cv, at::Te
   return {k, v};
 }
 
-// bytes that a tensor lies in
-std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
-  int64_t last = 1;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  return {a, a + last * t.element_size()};
-}
-
 std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tensor cv, at::Tensor sk, at::Tensor sv,
                                           at::Tensor page_table, at::Tensor rows, at::Tensor cu_q, at::Tensor kv_lens, int64_t page,
                                           int64_t max_q_len, c10::optional<double> scale, int64_t window,
@@ -692,10 +698,7 @@ std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tenso
     CHECK(out->scalar_type() == at::kBFloat16 && out->sizes() == q.sizes() && out->is_contiguous() && out->device() == dev &&
               reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0,
           "attention_kv8: out must be contiguous bf16 ", q.sizes(), ", 16-byte aligned, on the cache's device");
-    if (T > 0) {
-      const auto a = span_of(q), b = span_of(*out);
-      CHECK(a.second <= b.first || b.second <= a.first, "attention_kv8: out must not overlap q");
-    }
+    CHECK(T == 0 || !overlap(q, *out), "attention_kv8: out must not overlap q");
     o = *out;
   } else {
     o = new_cuda({T, nq, hd}, at::kBFloat16, dev);

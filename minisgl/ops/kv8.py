@@ -59,6 +59,8 @@ class KV8Cache:
         for t in (k, self.v, self.k_scale, self.v_scale):
             if t.device != k.device or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError("8-bit cache: codes and scales must be contiguous, 16-byte aligned and on one device")
+        if _overlap(k, self.v) or _overlap(self.k_scale, self.v_scale):
+            raise ValueError("8-bit cache: keys and values must not share memory")
 
     @classmethod
     def alloc(cls, num_slots: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.int8,

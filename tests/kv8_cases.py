@@ -171,6 +171,7 @@ def bad_calls(dev):
         t = dict(dict(k=k.k, v=k.v, k_scale=k.k_scale, v_scale=k.v_scale), **kw)
         return ops.KV8Cache(t["k"], t["v"], t["k_scale"], t["v_scale"])
 
+    long = zeros(3, 16, 64, dtype=torch.int8)
     odd = zeros(2, 24, 64, dtype=torch.int8)
     wide = zeros(2, 16, 96, dtype=torch.int8)
     return [
@@ -181,6 +182,9 @@ def bad_calls(dev):
         ("scales in bf16", lambda: cache(k_scale=k.k_scale.to(bf16))),
         ("short scales", lambda: cache(v_scale=k.v_scale[:, :16].contiguous())),
         ("strided codes", lambda: cache(k=k.k.transpose(0, 1).contiguous().transpose(0, 1))),
+        ("one tensor for both codes", lambda: cache(v=k.k)),
+        ("one tensor for both scales", lambda: cache(v_scale=k.k_scale)),
+        ("codes that overlap", lambda: ops.KV8Cache(long[:2], long[1:], k.k_scale[:, :16].contiguous(), k.v_scale[:, :16].contiguous())),
         ("24 slots", lambda: ops.KV8Cache(odd, odd, zeros(2, 24), zeros(2, 24))),
         ("head dim 96", lambda: ops.KV8Cache(wide, wide, zeros(2, 16), zeros(2, 16))),
         ("a cache in bf16", lambda: ops.KV8Cache.alloc(16, 2, 64, bf16, dev)),
