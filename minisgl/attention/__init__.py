@@ -4,6 +4,8 @@ command line and all resolve to it (reference registry: python/minisgl/attention
 
 from __future__ import annotations
 
+from minisgl.core import get_global_ctx
+from minisgl.kvcache.kv8_pool import KV8Pool
 from minisgl.utils import Registry
 
 from .base import BaseAttnBackend, BaseAttnMetadata
@@ -21,9 +23,11 @@ def validate_attn_backend(name: str) -> str:
 
 
 def create_attention_backend(name: str, model_config, device) -> BaseAttnBackend:
+    """The backend for the current context's KV pool."""
     validate_attn_backend(name)
     return PagedAttentionBackend(
-        model_config.num_qo_heads, model_config.num_kv_heads, model_config.head_dim, device
+        model_config.num_qo_heads, model_config.num_kv_heads, model_config.head_dim, device,
+        kv8=isinstance(getattr(get_global_ctx(), "kv_cache", None), KV8Pool),
     )
 
 

@@ -8,6 +8,10 @@ list with the batch; CTAs stream whole pages with TMA and the last chunk of a re
 combines the partials. Other page sizes run the split-KV kernel plus a combine step. Sliding
 windows and per-head attention sinks are kernel arguments.
 
+Over an 8-bit KV pool both phases are one call of ``ops.attention_kv8``, which takes ``rows``,
+``kv_lens`` and ``cu_q`` and cuts its work on the device: nothing is planned on the host, and a
+decode graph replays with fresh lengths as it is.
+
 The metadata is small and device-resident: ``rows`` (page-table row per request), ``kv_lens``,
 ``cu_q`` and the decode work list. Decode metadata lives in static buffers so CUDA graphs replay
 with fresh lengths.
@@ -24,6 +28,7 @@ from typing import Dict, List
 import numpy as np
 import torch
 
+from minisgl import ops
 from minisgl._native import cuda as _cuda
 from minisgl.core import Batch, get_global_ctx
 from minisgl.ops import reference as ref
@@ -103,7 +108,8 @@ def decode_splits(bs: int, kv_heads: int, max_len: int, chunk: int = 256) -> int
 
 
 class PagedAttentionBackend(BaseAttnBackend):
-    def __init__(self, num_qo_heads: int, num_kv_heads: int, head_dim: int, device: torch.device):
+    def __init__(self, num_qo_heads: int, num_kv_heads: int, head_dim: int, device: torch.device,
+                 kv8: bool = False):
         from minisgl.parallel import get_tp_info
         from minisgl.utils import div_even
 
@@ -117,9 +123,10 @@ class PagedAttentionBackend(BaseAttnBackend):
         self._graph_splits: Dict[int, int] = {}
         self._ws: torch.Tensor | None = None
         # paged decode needs TMA-sized pages and a group of at most 16 query heads
+        self.kv8 = kv8
         self.page = 0
         self.num_ctas = NUM_SMS
-        if device.type == "cuda":
+        if device.type == "cuda" and not kv8:
             ps = get_global_ctx().page_size
             if ps in PAGED_DECODE_PAGES and head_dim in (64, 128) and self.nq // self.nkv <= 16:
                 self.page = ps
@@ -217,6 +224,11 @@ class PagedAttentionBackend(BaseAttnBackend):
     def forward(self, q: torch.Tensor, layer_id: int, batch: Batch, *, window: int = -1,
                 sinks: torch.Tensor | None = None) -> torch.Tensor:
         ctx = get_global_ctx()
+        if self.kv8:
+            m = batch.attn_metadata
+            o = ops.attention_kv8(q, ctx.kv_cache.layer(layer_id), ctx.page_table, m.rows, m.cu_q, m.kv_lens,
+                                  page_size=ctx.page_size, max_q_len=m.max_q_len, scale=self.scale, window=window, sinks=sinks)
+            return o.view(q.shape[0], -1)
         kc, vc = ctx.kv_cache.k_cache(layer_id), ctx.kv_cache.v_cache(layer_id)
         m: PagedMetadata = batch.attn_metadata
         if not q.is_cuda:

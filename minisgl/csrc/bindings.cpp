@@ -646,6 +646,38 @@ void store_kv8(at::Tensor k, at::Tensor v, at::Tensor ck, at::Tensor cv, at::Ten
   check_launch(msgl_kv8_store(&p, hd, fp8, stream()), "store_kv8");
 }
 
+at::Tensor qk_norm_rope_store_kv8(at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, c10::optional<at::Tensor> q_norm,
+                                  c10::optional<at::Tensor> k_norm, double eps, at::Tensor ck, at::Tensor cv, at::Tensor sk,
+                                  at::Tensor sv, at::Tensor out_loc, int64_t nq) {
+  const bool fp8 = kv8_check({ck, cv, sk, sv});
+  const at::Device dev = ck.device();
+  const int64_t nkv = ck.size(0), hd = ck.size(2), n = qkv.dim() ? qkv.size(0) : 0;
+  CHECK(nq > 0 && nq < (1 << 20) && qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * hd &&
+            qkv.is_contiguous() && qkv.device() == dev && n < (1ll << 31),
+        "qk_norm_rope_store_kv8: qkv must be contiguous bf16 [tokens, (", nq, " + 2 * ", nkv, ") * ", hd, "] on the cache's device, got ",
+        qkv.scalar_type(), " ", qkv.sizes(), " on ", qkv.device());
+  const int32_t* pos = kv8_ids(positions, n, dev, "qk_norm_rope_store_kv8: positions");
+  const int32_t* slots = kv8_ids(out_loc, n, dev, "qk_norm_rope_store_kv8: out_loc");
+  CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2 && cos_sin.size(1) == hd && cos_sin.size(0) < (1ll << 31) &&
+            cos_sin.is_contiguous() && cos_sin.device() == dev,
+        "qk_norm_rope_store_kv8: cos_sin must be contiguous fp32 [positions, ", hd, "] on the cache's device, got ",
+        cos_sin.scalar_type(), " ", cos_sin.sizes());
+  CHECK(q_norm.has_value() == k_norm.has_value(), "qk_norm_rope_store_kv8: q_norm and k_norm must both be given or both absent");
+  for (const auto* w : {&q_norm, &k_norm})
+    CHECK(!w->has_value() || ((*w)->scalar_type() == at::kBFloat16 && (*w)->dim() == 1 && (*w)->size(0) == hd &&
+                              (*w)->is_contiguous() && (*w)->device() == dev),
+          "qk_norm_rope_store_kv8: norm weights must be contiguous bf16 [", hd, "] on the cache's device");
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor q = new_cuda({n, nq, hd}, at::kBFloat16, dev);
+  if (n == 0) return q;
+  const Kv8Store p{nullptr, nullptr, 0, 0, 0, 0, ck.data_ptr(), cv.data_ptr(), sk.data_ptr<float>(), sv.data_ptr<float>(), slots,
+                   (int)n, (int)nkv, (int)ck.size(1)};
+  check_launch(msgl_qk_norm_rope_store_kv8(q.data_ptr(), qkv.data_ptr(), pos, cos_sin.data_ptr<float>(), opt_ptr(q_norm),
+                                           opt_ptr(k_norm), eps, nq, hd, cos_sin.size(0), fp8, &p, stream()),
+               "qk_norm_rope_store_kv8");
+  return q;
+}
+
 std::tuple<at::Tensor, at::Tensor> load_kv8(at::Tensor ck, at::Tensor cv, at::Tensor sk, at::Tensor sv, at::Tensor slots) {
   const bool fp8 = kv8_check({ck, cv, sk, sv});
   const at::Device dev = ck.device();
@@ -855,6 +887,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("w4_force_form", [](int halves, int splits) { msgl_w4_force_form(halves, splits); });
   m.def("experts_w4", &experts_w4);
   m.def("store_kv8", &store_kv8);
+  m.def("qk_norm_rope_store_kv8", &qk_norm_rope_store_kv8);
   m.def("load_kv8", &load_kv8);
   m.def("attention_kv8", &attention_kv8);
 

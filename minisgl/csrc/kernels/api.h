@@ -127,6 +127,10 @@ typedef struct {
   int n, nkv, num_slots;
 } Kv8Store;
 int msgl_kv8_store(const Kv8Store* p, int hd, int fp8, cudaStream_t s);
+// msgl_qk_norm_rope_store into that cache (elementwise.cu): qkv bf16 [n][nq + 2 nkv][hd]; cache's k and v are not used
+int msgl_qk_norm_rope_store_kv8(void* q_out, const void* qkv, const int32_t* positions, const float* cos_sin,
+                                const void* q_norm, const void* k_norm, float eps, int nq, int hd, int max_pos, int fp8,
+                                const Kv8Store* cache, cudaStream_t s);
 typedef struct {
   void *k, *v;  // bf16 [n][nkv][hd]
   const void *ck, *cv;

@@ -5,6 +5,7 @@
 
 #include "api.h"
 #include "common.cuh"
+#include "kv8.cuh"
 
 using namespace msgl;
 
@@ -151,6 +152,32 @@ __global__ void store_kv_kernel(const uint4* __restrict__ k, const uint4* __rest
 }
 
 // ------------------------------------------------------------------------------ qk norm + rope + store
+// A head's row through RMSNorm (with weights) and RoPE, in the lanes' order below.
+template <int E>
+MSGL_DEVICE void norm_rope(float (&a)[E], float (&b)[E], const __nv_bfloat16* nw, float eps, const float* cs, int lane) {
+  constexpr int HD = 64 * E;
+  if (nw != nullptr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
+    ss = warp_sum(ss);
+    const float inv = rsqrtf(ss / HD + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      // match the reference rounding: normalized values are rounded to bf16 before RoPE
+      a[e] = __bfloat162float(__float2bfloat16(a[e] * inv * __bfloat162float(nw[lane * E + e])));
+      b[e] = __bfloat162float(__float2bfloat16(b[e] * inv * __bfloat162float(nw[HD / 2 + lane * E + e])));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = lane * E + e;
+    const float c = cs[i], s = cs[HD / 2 + i], x = a[e], y = b[e];
+    a[e] = x * c - y * s;
+    b[e] = y * c + x * s;
+  }
+}
+
 // One warp per (token, head) over the q, k and v heads of the merged qkv row. Lane l owns
 // elements [l*E, l*E+E) of the first half and the same offsets of the second half (E = hd/64),
 // so each neox-style rotation pair (i, i + hd/2) lives in one thread.
@@ -195,32 +222,81 @@ __global__ void qk_norm_rope_store_kernel(__nv_bfloat16* __restrict__ q_out,
     return;
   }
   const bool is_q = h < nq;
-  const __nv_bfloat16* nw = is_q ? q_norm : k_norm;
-  if (nw != nullptr) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
-    ss = warp_sum(ss);
-    const float inv = rsqrtf(ss / HD + eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      // match the reference rounding: normalized values are rounded to bf16 before RoPE
-      a[e] = __bfloat162float(__float2bfloat16(a[e] * inv * __bfloat162float(nw[lane * E + e])));
-      b[e] = __bfloat162float(__float2bfloat16(b[e] * inv * __bfloat162float(nw[HD / 2 + lane * E + e])));
-    }
-  }
-  const int pos = positions[t];
-  const float* cs = cos_sin + (size_t)pos * HD;
+  norm_rope<E>(a, b, is_q ? q_norm : k_norm, eps, cos_sin + (size_t)positions[t] * HD, lane);
   __nv_bfloat16* dst;
   if (is_q) dst = q_out + ((size_t)t * nq + h) * HD;
   else dst = k_cache + (int64_t)out_loc[t] * cache_stride + (size_t)(h - nq) * HD;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int i = lane * E + e;
-    const float c = cs[i], s = cs[HD / 2 + i];
-    dst[i] = __float2bfloat16(a[e] * c - b[e] * s);
-    dst[HD / 2 + i] = __float2bfloat16(b[e] * c + a[e] * s);
+    dst[i] = __float2bfloat16(a[e]);
+    dst[HD / 2 + i] = __float2bfloat16(b[e]);
   }
+}
+
+// The same into an 8-bit cache (kv8.cu): a warp holds a whole row, so a key's or a value's codes are those of the bf16
+// row that the kernel above would store, without writing and reading that one.
+template <int E, bool FP8>
+__global__ void qk_norm_rope_store_kv8_kernel(__nv_bfloat16* __restrict__ q_out, const __nv_bfloat16* __restrict__ qkv,
+                                              const int32_t* __restrict__ positions, const float* __restrict__ cos_sin,
+                                              const __nv_bfloat16* __restrict__ q_norm,
+                                              const __nv_bfloat16* __restrict__ k_norm, float eps, int max_pos, int nq,
+                                              Kv8Store p) {
+  pdl_wait();
+  pdl_launch();
+  constexpr int HD = 64 * E;
+  const int heads = nq + 2 * p.nkv;
+  const int64_t gw = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (gw >= (int64_t)p.n * heads) return;
+  const int t = (int)(gw / heads), h = (int)(gw - (int64_t)t * heads);
+  // (warp-uniform: one warp owns one (token, head))
+  const int slot = h >= nq ? p.slots[t] : 0, pos = h < nq + p.nkv ? positions[t] : 0;
+  if (slot < 0) return;
+  if (slot >= p.num_slots || pos < 0 || pos >= max_pos) {
+    report_error(kErrBounds, slot >= p.num_slots ? kBcKvSlot : kBcRopePos);
+    return;
+  }
+  const __nv_bfloat16* src = qkv + gw * HD;
+  float a[E], b[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    a[e] = __bfloat162float(src[lane * E + e]);
+    b[e] = __bfloat162float(src[HD / 2 + lane * E + e]);
+  }
+  if (h < nq + p.nkv) {
+    norm_rope<E>(a, b, h < nq ? q_norm : k_norm, eps, cos_sin + (size_t)pos * HD, lane);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      a[e] = __bfloat162float(__float2bfloat16(a[e]));
+      b[e] = __bfloat162float(__float2bfloat16(b[e]));
+    }
+  }
+  if (h < nq) {
+    __nv_bfloat16* dst = q_out + ((int64_t)t * nq + h) * HD;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      dst[lane * E + e] = __float2bfloat16(a[e]);
+      dst[HD / 2 + lane * E + e] = __float2bfloat16(b[e]);
+    }
+    return;
+  }
+  // the largest magnitude, as fp32 patterns without their sign: those order as integers, infinities and NaN on top
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) m = max(m, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
+  m = __reduce_max_sync(0xffffffffu, m);
+  const Kv8Quant<FP8> quant(__uint_as_float(m));
+  const bool is_v = h >= nq + p.nkv;
+  const int64_t at = (int64_t)(h - nq - (is_v ? p.nkv : 0)) * p.num_slots + slot;
+  uint8_t* codes = reinterpret_cast<uint8_t*>(is_v ? p.cv : p.ck) + at * HD;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const float* x = half ? b : a;
+    if constexpr (E == 1) codes[half * HD / 2 + lane] = (uint8_t)quant.pair(x[0], 0.f);
+    else reinterpret_cast<uint16_t*>(codes + half * HD / 2)[lane] = (uint16_t)quant.pair(x[0], x[1]);
+  }
+  if (lane == 0) (is_v ? p.sv : p.sk)[at] = quant.scale;
 }
 
 // ------------------------------------------------------------------------------ argmax
@@ -367,6 +443,21 @@ extern "C" void msgl_qk_norm_rope_store(void* q_out, const void* qkv, const int3
     msgl_launch(qk_norm_rope_store_kernel<2>, grid, wpb * 32, 0, s, 1, qo, src, positions, cos_sin, qn, kn, eps, kc, vc, out_loc, n, nq, nkv, cache_stride, num_slots, max_pos);
   else
     msgl_launch(qk_norm_rope_store_kernel<4>, grid, wpb * 32, 0, s, 1, qo, src, positions, cos_sin, qn, kn, eps, kc, vc, out_loc, n, nq, nkv, cache_stride, num_slots, max_pos);
+}
+
+extern "C" int msgl_qk_norm_rope_store_kv8(void* q_out, const void* qkv, const int32_t* positions, const float* cos_sin,
+                                           const void* q_norm, const void* k_norm, float eps, int nq, int hd, int max_pos,
+                                           int fp8, const Kv8Store* cache, cudaStream_t s) {
+  const int wpb = 8;
+  const int64_t blocks = ((int64_t)cache->n * (nq + 2 * cache->nkv) + wpb - 1) / wpb;
+  if ((hd != 64 && hd != 128) || blocks > INT32_MAX) return 3;
+  if (blocks == 0) return 0;
+  auto* f = hd == 64 ? (fp8 ? qk_norm_rope_store_kv8_kernel<1, true> : qk_norm_rope_store_kv8_kernel<1, false>)
+                     : (fp8 ? qk_norm_rope_store_kv8_kernel<2, true> : qk_norm_rope_store_kv8_kernel<2, false>);
+  return msgl_launch(f, dim3((unsigned)blocks), dim3(wpb * 32), 0, s, 1, reinterpret_cast<__nv_bfloat16*>(q_out),
+                     reinterpret_cast<const __nv_bfloat16*>(qkv), positions, cos_sin,
+                     reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps,
+                     max_pos, nq, *cache) == cudaSuccess ? 0 : 4;
 }
 
 extern "C" void msgl_argmax(int32_t* out, float* out_val, const void* logits, int rows, int vocab, int64_t stride,

@@ -3,11 +3,6 @@
 // Layout (per layer): codes [kv heads][slots][HD] bytes and fp32 scales [kv heads][slots], of keys and of
 // values: a head's page is one contiguous run of codes and one of scales, so attention loads it with one
 // copy each.
-//
-// A row x has scale = max|x| / Q with Q = 127 (int8) or 448 (e4m3), and codes = nearest(x Q / max|x|), ties
-// to even. The quotient of two 16-bit values times Q has to be rounded as in exact arithmetic: it can lie on
-// a tie (x = max / 2 gives 63.5), and next to a tie it is at least 2^-18 of a step away, far more than an fp32
-// rounding. So fp32 with a quotient that is exact where it is representable suffices.
 #include "api.h"
 #include "common.cuh"
 #include "kv8.cuh"
@@ -17,45 +12,6 @@ using namespace msgl;
 namespace {
 
 constexpr int kThreads = 256;
-
-// Codes of 8 values (bf16 pairs) against the row's largest magnitude.
-template <bool FP8>
-__device__ __forceinline__ uint2 quantise8(const uint4 u, float top, float& scale) {
-  constexpr float Q = FP8 ? 448.f : 127.f;
-  scale = __fdiv_rn(top, Q);
-  uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  if (!(top > 0.f) || !(top < INFINITY)) {  // zeros; an infinity or a NaN somewhere in the row
-    if (!(top == 0.f)) scale = __int_as_float(0x7fc00000);
-    return make_uint2(0u, 0u);
-  }
-  // x Q must not overflow, and products with the remainder below not underflow: both sides of the quotient
-  // are moved to the middle of the range, by a power of two, which changes neither
-  float by = 1.f;
-  if (top > 0x1p+100f) by = 0x1p-64f;
-  if (top < 0x1p-60f) by = 0x1p+64f;
-  const float a = top * by, inv = __fdiv_rn(1.f, a);
-  float c[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = (i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1])) * by * Q;
-    // quotient by the reciprocal, then one Newton step on its remainder x - q a, which fma gives exactly:
-    // the result is the nearest fp32, exact where the quotient is representable
-    const float q = x * inv;
-    c[i] = fmaf(fmaf(-q, a, x), inv, q);
-  }
-  uint2 r;
-  if constexpr (FP8) {
-    r.x = (uint32_t)kv8_e4m3x2(c[0], c[1]) | (uint32_t)kv8_e4m3x2(c[2], c[3]) << 16;
-    r.y = (uint32_t)kv8_e4m3x2(c[4], c[5]) | (uint32_t)kv8_e4m3x2(c[6], c[7]) << 16;
-  } else {
-    uint32_t b[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = (uint32_t)__float2int_rn(c[i]) & 255u;
-    r.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-    r.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
-  }
-  return r;
-}
 
 // HD / 8 lanes per row of a token and a head, 8 values each, the key's and the value's row one after the other:
 // 16-byte loads of whole rows, 8-byte stores of whole 128- (64-) byte code rows. Bound by DRAM.
@@ -97,10 +53,13 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(Kv8Store p) {
   const int64_t at = (int64_t)h * p.num_slots + slot;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    float scale;
-    const uint2 c = quantise8<FP8>(u[i], top[i], scale);
-    reinterpret_cast<uint2*>(i ? p.cv : p.ck)[at * L + part] = c;
-    if (part == 0) (i ? p.sv : p.sk)[at] = scale;
+    const Kv8Quant<FP8> quant(top[i]);
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = quant.pair(bf16_lo(w[j]), bf16_hi(w[j]));
+    reinterpret_cast<uint2*>(i ? p.cv : p.ck)[at * L + part] = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    if (part == 0) (i ? p.sv : p.sk)[at] = quant.scale;
   }
 }
 

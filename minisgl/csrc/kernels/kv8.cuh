@@ -42,6 +42,42 @@ MSGL_DEVICE uint16_t kv8_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// A row x has scale = max|x| / Q with Q = 127 (int8) or 448 (e4m3), and codes = nearest(x Q / max|x|), ties
+// to even. The quotient has to be rounded as in exact arithmetic: it can lie on a tie (x = max / 2 gives 63.5), and
+// where it does not it is at least 2^-16 of its size away from one: x and max have 8 bits, a tie t = odd / 2 has 8 (int8; 5 in
+// e4m3, whose Q is 7 times a power of two), so 2 x Q and 2 t max are different multiples of x's unit, below 2^16 of it.
+// An fp32 quotient that is exact where it is representable suffices.
+template <bool FP8>
+struct Kv8Quant {
+  float scale, by, a, inv;
+  bool codes;  // the row has any: not one of zeros, nor one with an infinity or a NaN, whose scale is NaN
+  MSGL_DEVICE explicit Kv8Quant(float top) {
+    constexpr float Q = FP8 ? 448.f : 127.f;
+    scale = __fdiv_rn(top, Q);
+    codes = top > 0.f && top < INFINITY;
+    if (!codes && !(top == 0.f)) scale = __int_as_float(0x7fc00000);
+    // x Q must not overflow, and products with the remainder below not underflow: both sides of the quotient
+    // are moved to the middle of the range, by a power of two, which changes neither
+    by = Q;
+    a = top;
+    if (top > 0x1p+100f) by *= 0x1p-64f, a *= 0x1p-64f;
+    if (top < 0x1p-60f) by *= 0x1p+64f, a *= 0x1p+64f;
+    inv = __fdiv_rn(1.f, a);
+  }
+  // x Q / max: by the reciprocal, then one Newton step on its remainder x - q a, which fma gives exactly: the nearest
+  // fp32, exact where the quotient is representable
+  MSGL_DEVICE float quotient(float value) const {
+    const float x = value * by, q = x * inv;
+    return fmaf(fmaf(-q, a, x), inv, q);
+  }
+  // two values of the row to two codes (the first one in the low byte)
+  MSGL_DEVICE uint32_t pair(float lo, float hi) const {
+    if (!codes) return 0;
+    if constexpr (FP8) return kv8_e4m3x2(quotient(lo), quotient(hi));
+    else return ((uint32_t)__float2int_rn(quotient(lo)) & 255u) | ((uint32_t)__float2int_rn(quotient(hi)) & 255u) << 8;
+  }
+};
+
 // the two values of a pair of codes (the low 16 bits)
 template <bool FP8>
 MSGL_DEVICE float2 kv8_decode2(uint32_t pair) {

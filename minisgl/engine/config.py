@@ -27,6 +27,7 @@ class EngineConfig:
     cuda_graph_bs: List[int] | None = None
     cuda_graph_max_bs: int | None = None
     page_size: int = 1
+    kv_cache_dtype: str = "auto"  # "auto": the model's dtype; "int8" or "fp8_e4m3": 8-bit codes with a scale per row
     memory_ratio: float = 0.9
     distributed_timeout: float = 60.0
     use_dummy_weight: bool = False

@@ -25,6 +25,7 @@ from minisgl.attention.paged import PAGED_DECODE_PAGES
 from minisgl.core import Batch, Context, Req, SamplingParams, reset_global_ctx, set_global_ctx
 from minisgl.env import ENV
 from minisgl.kvcache import create_kvcache_pool
+from minisgl.kvcache.kv8_pool import KV8_DTYPES
 from minisgl.layers import set_rope_device
 from minisgl.models import create_model, load_weight
 from minisgl.parallel import destroy_distributed, set_torch_group, set_tp_info
@@ -73,6 +74,7 @@ class Engine:
             # range); float16 requests, including "auto" on float16/float32 checkpoints, run in bf16
             logger.warning_rank0("dtype float16 served as bfloat16 on CUDA")
             object.__setattr__(config, "dtype", torch.bfloat16)
+        self.kv_dtype = self._kv_dtype(config)
         torch.manual_seed(config.seed)
         if self.is_cuda:
             torch.cuda.set_device(self.device)
@@ -99,7 +101,7 @@ class Engine:
         self.num_pages = self._num_pages(free0)
         ps = config.page_size
         self.ctx.kv_cache = self.kv_cache = create_kvcache_pool(
-            self.model_config, self.num_pages + 1, ps, self.dtype, self.device
+            self.model_config, self.num_pages + 1, ps, self.kv_dtype, self.device
         )
         self.dummy_slot = self.num_pages * ps
         num_tokens = self.num_pages * ps
@@ -239,11 +241,32 @@ class Engine:
             raise RuntimeError(f"free memory differs across TP ranks: min {lo}, max {hi}")
         return lo, hi
 
+    @staticmethod
+    def _kv_dtype(config: EngineConfig) -> torch.dtype:
+        """The KV pool's type, checked before anything is loaded."""
+        name = config.kv_cache_dtype
+        if name == "auto":
+            return config.dtype
+        if name not in KV8_DTYPES:
+            raise ValueError(f"kv_cache_dtype must be auto, {' or '.join(KV8_DTYPES)}, got {name!r}")
+        mc = config.model_config
+        if config.dtype != torch.bfloat16:
+            raise ValueError(f"kv_cache_dtype {name} needs a bfloat16 model, got {config.dtype}")
+        if mc.head_dim not in (64, 128):
+            raise ValueError(f"kv_cache_dtype {name} needs head dim 64 or 128, got {mc.head_dim}")
+        if mc.num_qo_heads // div_even(mc.num_kv_heads, config.tp_info.size, allow_replicate=True) // config.tp_info.size > 128:
+            raise ValueError(f"kv_cache_dtype {name}: at most 128 query heads per kv head")
+        if config.page_size % 16:
+            logger.warning_rank0(f"page size {config.page_size} overridden to 64 (an 8-bit KV cache has pages of 16)")
+            object.__setattr__(config, "page_size", 64)
+        return KV8_DTYPES[name]
+
     def _num_pages(self, free_before: int) -> int:
         cfg = self.config
         mc = self.model_config
         kvh = div_even(mc.num_kv_heads, cfg.tp_info.size, allow_replicate=True)
-        per_page = 2 * mc.head_dim * kvh * cfg.page_size * self.dtype.itemsize * mc.num_layers
+        row = mc.head_dim * self.kv_dtype.itemsize + (4 if self.kv_dtype in KV8_DTYPES.values() else 0)
+        per_page = 2 * row * kvh * cfg.page_size * mc.num_layers
         if cfg.num_page_override is not None:
             n = cfg.num_page_override
         elif not self.is_cuda:

@@ -48,9 +48,11 @@ def create_kvcache_pool(
     dtype: "torch.dtype",
     device: "torch.device",
 ) -> BaseKVCachePool:
+    from .kv8_pool import KV8_DTYPES, KV8Pool
     from .mha_pool import MHAKVCache
 
-    return MHAKVCache(
+    pool = KV8Pool if dtype in KV8_DTYPES.values() else MHAKVCache
+    return pool(
         num_kv_heads=model_config.num_kv_heads,
         num_layers=model_config.num_layers,
         head_dim=model_config.head_dim,

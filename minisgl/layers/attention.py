@@ -7,6 +7,7 @@ import torch
 
 from minisgl import ops
 from minisgl.core import get_global_ctx
+from minisgl.kvcache.kv8_pool import KV8Pool
 from minisgl.parallel import get_tp_info
 from minisgl.utils import div_even
 
@@ -37,11 +38,14 @@ class AttentionLayer(BaseOP):
         ctx = get_global_ctx()
         batch = ctx.batch
         kv = ctx.kv_cache
-        q = ops.qk_norm_rope_store(
-            qkv, batch.positions, self._rope.cos_sin_cache,
-            self._q_norm.weight if self._q_norm is not None else None,
-            self._k_norm.weight if self._k_norm is not None else None,
-            self._eps, kv.k_cache(self._layer_id), kv.v_cache(self._layer_id), batch.out_loc,
-            self._nq, self._nkv, self._hd,
-        )
+        head = (qkv, batch.positions, self._rope.cos_sin_cache,
+                self._q_norm.weight if self._q_norm is not None else None,
+                self._k_norm.weight if self._k_norm is not None else None, self._eps)
+        if isinstance(kv, KV8Pool):
+            q = ops.qk_norm_rope_store_kv8(*head, kv.layer(self._layer_id), batch.out_loc, self._nq)
+        else:
+            q = ops.qk_norm_rope_store(
+                *head, kv.k_cache(self._layer_id), kv.v_cache(self._layer_id), batch.out_loc,
+                self._nq, self._nkv, self._hd,
+            )
         return ctx.attn_backend.forward(q, self._layer_id, batch, window=self._window, sinks=self.sinks)

@@ -12,7 +12,7 @@ import torch
 from minisgl._native import cuda as _cuda
 
 from . import reference as ref
-from .kv8 import KV8Cache, attention_kv8, load_kv8, store_kv8
+from .kv8 import KV8Cache, attention_kv8, load_kv8, qk_norm_rope_store_kv8, store_kv8
 from .moe import route_experts
 from .reference import GATE_UP_BLOCK, deinterleave_gate_up, interleave_gate_up
 from .w4 import W4Weight, experts_w4, linear_w4, quantize_w4
@@ -168,6 +168,7 @@ __all__ = [
     "KV8Cache",
     "store_kv8",
     "load_kv8",
+    "qk_norm_rope_store_kv8",
     "attention_kv8",
     "W4Weight",
     "quantize_w4",

@@ -130,6 +130,37 @@ def store_kv8(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, out_loc: torch.
     ref.store_kv8(k, v, cache, out_loc)
 
 
+def qk_norm_rope_store_kv8(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, q_norm: torch.Tensor | None,
+                           k_norm: torch.Tensor | None, eps: float, cache: KV8Cache, out_loc: torch.Tensor, nq: int) -> torch.Tensor:
+    """``qk_norm_rope_store`` into an 8-bit cache, in one kernel: splits ``qkv`` (bf16 ``[T, (nq + 2 kv heads) * head
+    dim]``) into heads, takes queries and keys through RMSNorm (with weights, bf16 ``[head dim]``) and RoPE
+    (``cos_sin`` fp32 ``[positions, head dim]``, ``positions`` int32 ``[T]``), and stores keys and values as ``store_kv8``
+    does with their bf16 rows. Returns the queries, bf16 ``[T, nq, head dim]``. A position outside ``cos_sin`` is an
+    error: the token's key is not stored, its queries are undefined."""
+    if cache.is_cuda:
+        return _cuda().qk_norm_rope_store_kv8(qkv, positions, cos_sin, q_norm, k_norm, eps, cache.k, cache.v, cache.k_scale,
+                                              cache.v_scale, out_loc, nq)
+    T, nkv, hd = qkv.shape[0] if qkv.dim() else 0, cache.num_kv_heads, cache.head_dim
+    if nq < 1:
+        raise ValueError(f"qk_norm_rope_store_kv8: {nq} query heads")
+    _check_like("qk_norm_rope_store_kv8: qkv", qkv, torch.bfloat16, (T, (nq + 2 * nkv) * hd), cache)
+    _check_ids("qk_norm_rope_store_kv8: positions", positions, T, cache)
+    _check_ids("qk_norm_rope_store_kv8: out_loc", out_loc, T, cache)
+    _check_like("qk_norm_rope_store_kv8: cos_sin", cos_sin, torch.float32, (*cos_sin.shape[:1], hd), cache)
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("qk_norm_rope_store_kv8: q_norm and k_norm must both be given or both absent")
+    for w in (q_norm, k_norm):
+        if w is not None:
+            _check_like("qk_norm_rope_store_kv8: norm weights", w, torch.bfloat16, (hd,), cache)
+    if not all(t.is_contiguous() for t in (qkv, cos_sin, q_norm, k_norm) if t is not None):
+        raise ValueError("qk_norm_rope_store_kv8: qkv, cos_sin and norm weights must be contiguous")
+    if T and not 0 <= int(positions.min()) <= int(positions.max()) < cos_sin.shape[0]:
+        raise ValueError(f"qk_norm_rope_store_kv8: a position outside the {cos_sin.shape[0]} of cos_sin")
+    if T and int(out_loc.max()) >= cache.num_slots:
+        raise ValueError(f"qk_norm_rope_store_kv8: slot {int(out_loc.max())} of {cache.num_slots}")
+    return ref.qk_norm_rope_store_kv8(qkv, positions, cos_sin, q_norm, k_norm, eps, cache, out_loc, nq)
+
+
 def load_kv8(cache: KV8Cache, slots: torch.Tensor):
     """The rows that the cache's codes at ``slots`` (int32 ``[n]``, in any order, also repeated) stand for:
     (k, v), bf16 ``[n, kv heads, head dim]``, ``code * scale`` rounded to bf16. A negative slot gives zeros, one

@@ -197,6 +197,15 @@ def store_kv8(k, v, cache, out_loc) -> None:
         scale[:, at] = s.transpose(0, 1)
 
 
+def qk_norm_rope_store_kv8(qkv, positions, cos_sin, q_norm, k_norm, eps, cache, out_loc, nq: int):
+    """Plain form of ``ops.qk_norm_rope_store_kv8``: the bf16 rows, then ``store_kv8``."""
+    t, nkv, hd = qkv.shape[0], cache.num_kv_heads, cache.head_dim
+    k, v = torch.empty(2, t, nkv, hd, dtype=qkv.dtype, device=qkv.device)
+    q = qk_norm_rope_store(qkv, positions, cos_sin, q_norm, k_norm, eps, k, v, torch.arange(t, device=qkv.device), nq, nkv, hd)
+    store_kv8(k, v, cache, out_loc)
+    return q
+
+
 def load_kv8(cache, slots):
     at = slots.long().clamp(min=0)
     keep = (slots >= 0).view(-1, 1, 1)

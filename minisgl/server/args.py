@@ -1,7 +1,7 @@
 """Command-line flags -> ``ServerArgs`` (reference: python/minisgl/server/args.py:14-268).
 
 Same flag names as the reference, plus ``--device`` (``cpu`` runs the reference-op engine),
-``--comm`` (``auto`` | ``nccl`` | ``peer``) and ``--distributed-timeout``.
+``--comm`` (``auto`` | ``nccl`` | ``peer``), ``--kv-cache-dtype`` and ``--distributed-timeout``.
 """
 
 from __future__ import annotations
@@ -70,6 +70,7 @@ def _resolve_dtype(name: str, model_path: str) -> torch.dtype:
 def build_parser() -> argparse.ArgumentParser:
     from minisgl.attention import SUPPORTED_ATTENTION_BACKENDS
     from minisgl.kvcache import SUPPORTED_CACHE_MANAGER
+    from minisgl.kvcache.kv8_pool import KV8_DTYPES
     from minisgl.moe import SUPPORTED_MOE_BACKENDS
 
     d = ServerArgs
@@ -90,6 +91,8 @@ def build_parser() -> argparse.ArgumentParser:
                    default=d.max_extend_tokens)
     p.add_argument("--num-pages", dest="num_page_override", type=int, default=d.num_page_override)
     p.add_argument("--page-size", type=int, default=d.page_size)
+    p.add_argument("--kv-cache-dtype", default=d.kv_cache_dtype, choices=["auto", *KV8_DTYPES],
+                   help="auto: the model's; int8, fp8_e4m3: 8-bit keys and values with one scale per row")
     p.add_argument("--attention-backend", "--attn", dest="attention_backend", default=d.attention_backend,
                    help=f"accepted for compatibility: {SUPPORTED_ATTENTION_BACKENDS.supported_names()} "
                         "(all run this engine's kernels)")

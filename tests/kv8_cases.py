@@ -171,6 +171,11 @@ def bad_calls(dev):
         t = dict(dict(k=k.k, v=k.v, k_scale=k.k_scale, v_scale=k.v_scale), **kw)
         return ops.KV8Cache(t["k"], t["v"], t["k_scale"], t["v_scale"])
 
+    heads = zeros(3, 8 * 64, dtype=bf16)
+
+    def fused(qkv=heads, pos=loc, cs=zeros(4, 64), qn=None, kn=None, at=loc, nq=4):
+        return ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, k, at, nq)
+
     long = zeros(3, 16, 64, dtype=torch.int8)
     odd = zeros(2, 24, 64, dtype=torch.int8)
     wide = zeros(2, 16, 96, dtype=torch.int8)
@@ -196,6 +201,18 @@ def bad_calls(dev):
         ("slots in 64 bits", lambda: ops.store_kv8(kv, kv, k, loc.long())),
         ("too few slots", lambda: ops.store_kv8(kv, kv, k, loc[:2])),
         ("strided slots", lambda: ops.store_kv8(kv, kv, k, zeros(6, dtype=i32)[::2])),
+        ("heads of 32 bits", lambda: fused(qkv=heads.float())),
+        ("heads of a cache with more", lambda: fused(nq=2)),
+        ("no query heads", lambda: fused(nq=0)),
+        ("strided heads", lambda: fused(qkv=zeros(3, 2 * 8 * 64, dtype=bf16)[:, ::2])),
+        ("positions in 64 bits", lambda: fused(pos=loc.long())),
+        ("fewer positions", lambda: fused(pos=loc[:2])),
+        ("angles in bf16", lambda: fused(cs=zeros(4, 64, dtype=bf16))),
+        ("angles of wide heads", lambda: fused(cs=zeros(4, 128))),
+        ("a norm of queries alone", lambda: fused(qn=zeros(64, dtype=bf16))),
+        ("norms in 32 bits", lambda: fused(qn=zeros(64), kn=zeros(64))),
+        ("norms of wide heads", lambda: fused(qn=zeros(128, dtype=bf16), kn=zeros(128, dtype=bf16))),
+        ("too few slots for the heads", lambda: fused(at=loc[:2])),
         ("read at 64-bit slots", lambda: ops.load_kv8(k, loc.long())),
         ("read at a table of slots", lambda: ops.load_kv8(k, loc[None])),
         ("q in 32 bits", lambda: attend(q=c.q.float())),
@@ -226,3 +243,24 @@ def bad_calls(dev):
         ("a strided out", lambda: attend(out=zeros(3, 8, 64, dtype=bf16)[:, ::2])),
         ("out over q", lambda: attend(out=c.q)),
     ]
+
+
+# ------------------------------------------------------------------------------------ engines
+# Logits of an engine with an 8-bit cache against an fp32 engine whose cache rows are rounded to the same codes. Without
+# codes a bf16 engine is within 0.06 of fp32 on the tiny models. A row that bf16 arithmetic moves by d (about 2^-9 of it)
+# changes codes where it crosses a tie: on average by sqrt(d * step), with a step of 2^-7 of the row's largest value
+# (int8), up to 2^-3 of the value itself (e4m3): 2 and 8 times a bf16 rounding of the row. A layer has some 20
+# bf16 roundings, 2 of them of cached rows; in squares (20 + 2 * 2^2) / 20 = 1.1^2 and (20 + 2 * 8^2) / 20 = 2.7^2.
+ENGINE_TOL = {"int8": 1.1 * 0.06, "fp8_e4m3": 2.7 * 0.06}
+
+
+def round_cache_rows(monkeypatch, name):
+    """Engines on the CPU store the values of 8-bit codes instead of the rows."""
+    dtype = {"int8": torch.int8, "fp8_e4m3": torch.float8_e4m3fn}[name]
+
+    def store_kv(k, v, k_cache, v_cache, out_loc):
+        for x, cache in ((k, k_cache), (v, v_cache)):
+            codes, scale = nearest(x.to(torch.bfloat16), dtype)
+            cache.view(cache.shape[0], -1)[out_loc.long()] = (codes * scale).flatten(1).to(cache.dtype)
+
+    monkeypatch.setattr(ops.ref, "store_kv", store_kv)

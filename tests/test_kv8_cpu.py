@@ -91,3 +91,30 @@ def test_tables_that_do_not_hold():
 def test_refusals(name, call):
     with pytest.raises(ValueError):
         call()
+
+
+# --------------------------------------------------------------------------------- fused store
+@pytest.mark.parametrize("dtype", FMTS)
+@pytest.mark.parametrize("norm", [True, False])
+def test_heads_to_cache(dtype, norm):
+    gen = torch.Generator().manual_seed(3)
+    T, nq, nkv, hd = 5, 6, 2, 64
+    qkv = torch.randn(T, (nq + 2 * nkv) * hd, generator=gen).to(torch.bfloat16)
+    pos = torch.tensor([3, 0, 9, 9, 1], dtype=torch.int32)
+    cs = ops.ref.rope_cos_sin(10, hd, ops.ref.default_inv_freq(hd, 1e4))
+    qn, kn = (torch.randn(2, hd, generator=gen).to(torch.bfloat16)) if norm else (None, None)
+    loc = torch.tensor([4, 17, -1, 30, 0], dtype=torch.int32)
+    cache, want = (ops.KV8Cache.alloc(32, nkv, hd, dtype, "cpu") for _ in range(2))
+    q = ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, loc, nq)
+    heads = qkv.view(T, -1, hd)
+    hq, hk = heads[:, :nq], heads[:, nq:nq + nkv]
+    if norm:
+        hq, hk = ops.ref.rmsnorm(hq, qn, 1e-6), ops.ref.rmsnorm(hk, kn, 1e-6)
+    assert torch.equal(q, ops.ref.rope(hq, pos, cs))
+    ops.store_kv8(ops.ref.rope(hk, pos, cs), heads[:, nq + nkv:], want, loc)
+    for a, b in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), (want.k, want.v, want.k_scale, want.v_scale)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope_store_kv8(qkv, pos + 1, cs, qn, kn, 1e-6, cache, loc, nq)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, loc + 2, nq)

@@ -130,6 +130,74 @@ def test_nothing_to_do():
     assert (got == 0).all()
 
 
+def heads_case(T, nq, nkv, hd, norm, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    qkv = rows_of(gen, T, nq + 2 * nkv, hd).flatten(1).cuda()
+    pos = torch.randint(0, 500, (T,), generator=gen).to(torch.int32).cuda()
+    cs = ops.ref.rope_cos_sin(500, hd, ops.ref.default_inv_freq(hd, 1e4)).cuda()
+    w = [torch.randn(hd, generator=gen).to(torch.bfloat16).cuda() for _ in range(2)] if norm else [None, None]
+    return qkv, pos, cs, *w
+
+
+def same_cache(a, b):
+    return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+               for x, y in zip((a.k, a.v, a.k_scale, a.v_scale), (b.k, b.v, b.k_scale, b.v_scale)))
+
+
+@pytest.mark.parametrize("dtype", FMTS)
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("T,nq,nkv,hd", [(1, 1, 1, 64), (5, 16, 8, 128), (130, 14, 2, 64), (33, 5, 5, 128)])
+def test_heads_to_cache(dtype, norm, T, nq, nkv, hd):
+    """The same queries and codes as storing bf16 rows first."""
+    qkv, pos, cs, qn, kn = heads_case(T, nq, nkv, hd, norm)
+    loc = torch.randperm(160)[:T].to(torch.int32).cuda()
+    loc[T // 2] = -1 if T > 1 else 3
+    cache, want = (ops.KV8Cache.alloc(160, nkv, hd, dtype) for _ in range(2))
+    q = ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, loc, nq)
+    k, v = torch.zeros(2, T, nkv, hd, dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(T, dtype=torch.int32, device="cuda")
+    assert torch.equal(q, ops.qk_norm_rope_store(qkv, pos, cs, qn, kn, 1e-6, k, v, at, nq, nkv, hd))
+    ops.store_kv8(k, v, want, loc)
+    assert same_cache(cache, want)
+
+
+def test_heads_to_cache_without_tokens_and_beyond_tables():
+    qkv, pos, cs, qn, kn = heads_case(3, 4, 2, 64, True)
+    cache, want = (ops.KV8Cache.alloc(32, 2, 64, torch.int8) for _ in range(2))
+    loc = torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    q = ops.qk_norm_rope_store_kv8(qkv[:0], pos[:0], cs, qn, kn, 1e-6, cache, loc[:0], 4)
+    assert q.shape == (0, 4, 64) and same_cache(cache, want)
+    good = ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, want, loc, 4)
+    assert error_word()[0] == 0
+    q = ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, torch.tensor([1, 32, 3], dtype=torch.int32, device="cuda"), 4)
+    assert error_word()[0] == 3 and torch.equal(q, good)
+    for t in (want.k, want.v, want.k_scale, want.v_scale):
+        t[:, 2] = 0
+    assert same_cache(cache, want)
+    bad = pos.clone()
+    bad[1] = 500
+    q = ops.qk_norm_rope_store_kv8(qkv, bad, cs, qn, kn, 1e-6, cache, loc, 4)
+    assert error_word()[0] == 3 and torch.equal(q[::2], good[::2])
+    assert torch.equal(cache.k.view(torch.uint8), want.k.view(torch.uint8))  # (the bad token's key is not stored)
+
+
+def test_heads_to_cache_captured():
+    qkv, pos, cs, qn, kn = heads_case(4, 4, 2, 128, True)
+    cache, want = (ops.KV8Cache.alloc(32, 2, 128, torch.float8_e4m3fn) for _ in range(2))
+    loc = torch.tensor([1, 2, 3, 9], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, loc, 4)
+    with torch.cuda.graph(graph):
+        q = ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, kn, 1e-6, cache, loc, 4)
+    new = heads_case(4, 4, 2, 128, True, seed=1)
+    qkv.copy_(new[0]), pos.copy_(new[1]), loc.add_(10)
+    graph.replay()
+    for at in (torch.tensor([1, 2, 3, 9], device="cuda"), loc):
+        old = heads_case(4, 4, 2, 128, True) if at is not loc else (qkv, pos, cs, qn, kn)
+        good = ops.qk_norm_rope_store_kv8(old[0], old[1], cs, qn, kn, 1e-6, want, at.to(torch.int32), 4)
+    assert torch.equal(q, good) and same_cache(cache, want)
+
+
 # ------------------------------------------------------------------------------- attention
 # the form is chosen by max_q_len: both hold for every batch
 HINTS = [1, 6, 1000]
