@@ -703,6 +703,9 @@ std::tuple<at::Tensor, int> attention_kv8(at::Tensor q, at::Tensor ck, at::Tenso
   c10::cuda::CUDAGuard guard(dev);
   at::Tensor qr = kv8_rows(q, -1, hd, dev, "attention_kv8: q", hd);
   const int64_t T = q.size(0), nq = q.size(1);
+  CHECK(std::abs((const char*)ck.data_ptr() - (const char*)cv.data_ptr()) < (1ll << 40) &&
+            std::abs((const char*)sk.data_ptr() - (const char*)sv.data_ptr()) < (1ll << 40),
+        "attention_kv8: a cache's keys and values must lie within 2^40 bytes (as KV8Cache.alloc has them)");
   CHECK(nq > 0 && nq % nkv == 0 && nq / nkv <= 128, "attention_kv8: ", nq, " query heads over ", nkv, " kv heads (1 to 128 each)");
   CHECK(T * nq < (1ll << 30) && B < (1ll << 24), "attention_kv8: too many queries for one call");
   CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt && page_table.device() == dev &&

@@ -47,34 +47,71 @@ MSGL_DEVICE uint16_t kv8_e4m3x2(float lo, float hi) {
 // where it does not it is at least 2^-16 of its size away from one: x and max have 8 bits, a tie t = odd / 2 has 8 (int8; 5 in
 // e4m3, whose Q is 7 times a power of two), so 2 x Q and 2 t max are different multiples of x's unit, below 2^16 of it.
 // An fp32 quotient that is exact where it is representable suffices.
+// pairs of fp32 in one register pair
+MSGL_DEVICE uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+MSGL_DEVICE float2 f2_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <bool FP8>
 struct Kv8Quant {
   float scale, by, a, inv;
   bool codes;  // the row has any: not one of zeros, nor one with an infinity or a NaN, whose scale is NaN
   MSGL_DEVICE explicit Kv8Quant(float top) {
     constexpr float Q = FP8 ? 448.f : 127.f;
-    scale = __fdiv_rn(top, Q);
     codes = top > 0.f && top < INFINITY;
-    if (!codes && !(top == 0.f)) scale = __int_as_float(0x7fc00000);
+    if (top > 0x1p-100f && codes) {
+      // top / Q by Q's reciprocal and one Newton step on the remainder, which fma gives exactly: within 2^-46 of the quotient,
+      // which is 2^-33 or more away from where fp32's rounding turns (8 bits over 7)
+      scale = top * (1.f / Q);
+      scale = fmaf(fmaf(-scale, Q, top), 1.f / Q, scale);
+    } else {
+      scale = top == 0.f || codes ? __fdiv_rn(top, Q) : __int_as_float(0x7fc00000);
+    }
     // x Q must not overflow, and products with the remainder below not underflow: both sides of the quotient
     // are moved to the middle of the range, by a power of two, which changes neither
     by = Q;
     a = top;
     if (top > 0x1p+100f) by *= 0x1p-64f, a *= 0x1p-64f;
     if (top < 0x1p-60f) by *= 0x1p+64f, a *= 0x1p+64f;
-    inv = __fdiv_rn(1.f, a);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(a));  // (to 1 ulp)
   }
-  // x Q / max: by the reciprocal, then one Newton step on its remainder x - q a, which fma gives exactly: the nearest
-  // fp32, exact where the quotient is representable
-  MSGL_DEVICE float quotient(float value) const {
-    const float x = value * by, q = x * inv;
-    return fmaf(fmaf(-q, a, x), inv, q);
+  // x Q / max of two values: by the reciprocal, then a Newton step on the remainder x - q a, which fma gives exactly:
+  // within 2^-45 of the quotient before its rounding to fp32, so exact where it is representable
+  MSGL_DEVICE uint64_t quotients(float lo, float hi) const {
+    const uint64_t i2 = f2_pack(inv, inv), x = f2_mul(f2_pack(lo, hi), f2_pack(by, by)), q = f2_mul(x, i2);
+    return f2_fma(f2_fma(f2_mul(q, f2_pack(-1.f, -1.f)), f2_pack(a, a), x), i2, q);
   }
-  // two values of the row to two codes (the first one in the low byte)
+  // two values of the row to two codes (the first one in the low byte; what is above them is not theirs)
   MSGL_DEVICE uint32_t pair(float lo, float hi) const {
-    if (!codes) return 0;
-    if constexpr (FP8) return kv8_e4m3x2(quotient(lo), quotient(hi));
-    else return ((uint32_t)__float2int_rn(quotient(lo)) & 255u) | ((uint32_t)__float2int_rn(quotient(hi)) & 255u) << 8;
+    if constexpr (FP8) {
+      const float2 q = f2_unpack(quotients(lo, hi));
+      return codes ? kv8_e4m3x2(q.x, q.y) : 0u;
+    } else {  // 1.5 2^23 more has the nearest whole number in its low bits
+      const float2 q = f2_unpack(f2_add(quotients(lo, hi), f2_pack(12582912.f, 12582912.f)));
+      return codes ? __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040) : 0u;
+    }
   }
 };
 

@@ -80,33 +80,6 @@ MSGL_DEVICE void kt_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
                : "memory");
 }
 
-// pairs of fp32 in one register pair
-MSGL_DEVICE uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-MSGL_DEVICE float2 f2_unpack(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-MSGL_DEVICE uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-MSGL_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-MSGL_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // 16 lanes x 64 columns of tensor memory as mma's accumulators lie: lane (g, t) = (lane / 4, lane % 4) holds of rows g
 // (registers 4n, 4n + 1) and g + 8 (4n + 2, 4n + 3) the columns 8n + 2t and the next.
 MSGL_DEVICE void kt_load_s(uint32_t taddr, uint32_t (&r)[32]) {
