@@ -30,7 +30,10 @@ constexpr int kKtThreads = 512;
 constexpr int kKtCost = 2;      // of a segment, in blocks
 constexpr int kKtDescs = 4;     // segments looked up ahead
 constexpr int kKtSlots = 8;     // of scales
-constexpr float kKtTop = 10.f;
+// Offsets are moved where a weight would pass 2^15, so 2^9 lie between the largest one seen when they were set and that. (2^5 of
+// room has a warp's 32 rows move in half of the first blocks of short prompts: 368 us instead of 320 for 28 prompts of 100 to
+// 1024 tokens. fp16 then rounds weights to 2^-31 of the largest one at worst.)
+constexpr float kKtTop = 6.f;
 constexpr int kKtConv = 12, kKtSoft = 4;  // first warps of the converters and of the softmax
 // registers of a thread in warps 0 - 3, the softmax and the converters: of the launch's 4 x 128 a row of warps
 constexpr int kKtRegs = 128, kKtRegsFew = 64, kKtRegsSoft = 176, kKtRegsConv = 96;
@@ -102,7 +105,13 @@ MSGL_DEVICE void kt_store_p(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// The same for 16 columns of S and 8 of its weights.
+// The same for 32 columns, for 16 columns of S and 8 of its weights.
+MSGL_DEVICE void kt_load_o(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
 MSGL_DEVICE void kt_load_s16(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -233,8 +242,7 @@ MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w
 MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, bool part, bool fresh) {
   float sum[4];
   uint32_t pk[2][16];
-  // offsets after this many keys: a row's first ones are those of 16 keys, mostly near enough
-  int keys = part ? kKv8Block : fresh ? 16 : 0, moves = 0;
+  int keys = part || fresh ? kKv8Block : 0, moves = 0;
 #pragma unroll 1
   for (;;) {
     if (keys > 0) {
@@ -665,33 +673,52 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         lk = __shfl_sync(0xffffffffu, lk, (lane & 7) * 4);
         if (lane >> 3 == k) m = mk, l = lk;
       }
-      // O out of tensor memory, 32 head dims at a time
+      // O out of tensor memory, 32 head dims of 16 rows at a time, in the layout of S: of a row a lane has pairs of head dims,
+      // which it trades within its four lanes for eight that follow one another. (Whole rows in a lane make stores that touch 32 lines.)
       if (!(ok = kv8_wait_warp(&pvdone[2 * x + ((uses - 1) & 1)], ((uses - 1) >> 1) & 1))) break;
       tc_fence_after();
       const int head = D.h * G + r - tok * G;
       const float f = D.slot < 0 ? kv8_norm(m, l, p.sinks, in ? head : 0) : 1.f;
+      // the row's place in the output or the scratch
+      const int64_t at = !in ? -1 : D.slot < 0 ? (int64_t)(D.q0 + tok) * p.nq + head : (int64_t)D.slot * kKtRows + rr;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(to + c * 32, v);
+      for (int c = 0; c < HD / 16; ++c) {  // head dims from 32 (c / 2) on, rows from 16 (c % 2) on
+        uint32_t v[16];
+        kt_load_o(to + c / 2 * 32 + ((uint32_t)(c & 1) << 20), v);
         tc_wait_ld();
-        if (c == HD / 32 - 1) {
+        if (c == HD / 16 - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ofree[x]);
         }
-        if (in && D.slot < 0) {
-          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.o) + ((int64_t)(D.q0 + tok) * p.nq + head) * HD + c * 32);
 #pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            dst[k / 8] = make_uint4(pack_bf16(__uint_as_float(v[k]) * f, __uint_as_float(v[k + 1]) * f),
-                                    pack_bf16(__uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 3]) * f),
-                                    pack_bf16(__uint_as_float(v[k + 4]) * f, __uint_as_float(v[k + 5]) * f),
-                                    pack_bf16(__uint_as_float(v[k + 6]) * f, __uint_as_float(v[k + 7]) * f));
-        } else if (in) {
-          uint4* dst = reinterpret_cast<uint4*>(scratch.o + ((int64_t)D.slot * kKtRows + rr) * HD + c * 32);
+        for (int k = 0; k < 2; ++k) {
+          const int src = 16 * (c & 1) + 8 * k + (lane >> 2);
+          const float fk = __shfl_sync(0xffffffffu, f, src);
+          const int64_t dst = __shfl_sync(0xffffffffu, at, src);
+          const uint32_t* o = &v[2 * k];  // head dims 8 n + 2 t4 and the next: o[4 n], o[4 n + 1]
+          if (D.slot < 0) {
+            uint32_t y[4];
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) dst[k / 4] = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+            for (int n = 0; n < 4; ++n) y[n] = pack_bf16(__uint_as_float(o[4 * n]) * fk, __uint_as_float(o[4 * n + 1]) * fk);
+#pragma unroll
+            for (int n = 0; n < 4; n += 2) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, t4 & 1 ? y[n] : y[n + 1], 1);
+              if (t4 & 1) y[n] = got;
+              else y[n + 1] = got;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, t4 & 2 ? y[n] : y[n + 2], 2);
+              if (t4 & 2) y[n] = got;
+              else y[n + 2] = got;
+            }
+            if (dst >= 0) reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.o) + dst * HD + c / 2 * 32)[t4] = make_uint4(y[0], y[1], y[2], y[3]);
+          } else if (dst >= 0) {
+            float2* to_scratch = reinterpret_cast<float2*>(scratch.o + dst * HD + c / 2 * 32) + t4;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) to_scratch[4 * n] = make_float2(__uint_as_float(o[4 * n]), __uint_as_float(o[4 * n + 1]));
+          }
         }
       }
       if (in && D.slot >= 0) scratch.ml[(int64_t)D.slot * kKtRows + rr] = make_float2(m, l);

@@ -106,9 +106,9 @@ class Case:
         and 2 (L / 8 + 16) 2^-23 A for the sums over L keys, added 8 at a time at least.
 
         Half an fp16 step of a weight is 2^-11 of it where fp16 is normal, but not less than half of the smallest step,
-        2^-25. Weights p_j s^v_j are scaled so that the largest one, M, comes to 2^10 at least (the streaming form's to 2^14;
+        2^-25. Weights p_j s^v_j are scaled so that the largest one, M, comes to 2^6 at least (the streaming form's to 2^14;
         for a warp that has not seen the largest yet the step is a smaller part of M): each of them can be off by
-        2^-25 / 2^10 M, together by 2^-35 M sum_j |c_j|. That is what is left of a head dim in which the keys that count
+        2^-25 / 2^6 M, together by 2^-31 M sum_j |c_j|. That is what is left of a head dim in which the keys that count
         have codes of 0."""
         q, sinks = self.q.cpu().double(), None if self.sinks is None else self.sinks.cpu().double()
         T, nq, hd = q.shape
@@ -137,7 +137,7 @@ class Case:
                 d = ((hd + 16) * big + 16) * 2.0**-23
                 A = (p * v.abs()).sum(1)
                 M = (p.squeeze(-1) * sx[:, s].repeat_interleave(g, 0)).amax(-1, keepdim=True)
-                least = 2.0**-35 * M * cx[:, s].repeat_interleave(g, 0).sum(1)
+                least = 2.0**-31 * M * cx[:, s].repeat_interleave(g, 0).sum(1)
                 tol[at + i] = out[at + i].abs() * 2.0**-8 + A * (2.0**-11 + 2 * d.unsqueeze(-1) + 2 * (len(s) / 8 + 16) * 2.0**-23) + least + 1e-37
             at += n
         return out, tol
