@@ -108,13 +108,14 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
 }
 
 // The form for what the caller has told of a request's rows: 8, 16: rows of a streaming tile, 256: tensor core tiles. A request
-// of more rows than a streaming tile has its keys streamed (out of the L2 cache) and converted once for each tile, which
-// the tensor core form does once for 256 rows, but at its own pace. Measured with 16 requests of 6000 keys, 8 kv heads, int8, us
-// by rows, tiles of 8, of 16, tensor core: head dim 128: 8: 47, 58, 131; 16: 78, 59, 134; 32: 143, 101, 136; 48: 208, 144, 145; 64: 273,
-// 187, 145; head dim 64: 8: 35, 41, 125; 16: 58, 41, 128; 48: 151, 99, 132; 64: 197, 127, 134; 96: 290, 186, 140.
+// of more rows than a streaming tile has its keys streamed (out of the L2 cache) and converted once for each tile,
+// which the tensor core form does once for 256 rows, but at its own pace. Measured with 16 requests of 6000 keys, 8 kv heads, int8, us
+// by rows, tiles of 8, of 16, tensor core: head dim 128: 8: 47, 58, 114; 16: 78, 59, 114; 32: 143, 101, 116; 48: 208, 144, 122;
+// 64: 273, 187, 125; head dim 64: 8: 35, 41, 110; 16: 58, 42, 109; 48: 151, 99, 115; 64: 197, 128, 114. (A single request of
+// 4000 keys takes 13 to 27 us in tiles of 16 up to 128 rows, 30 to 42 on the tensor core from 64 rows on.)
 int form_of(const Kv8Attn& p, int hd, int max_q_len) {
   const int64_t rows = (int64_t)max_q_len * (p.nq / p.nkv);
-  return rows <= 8 ? 8 : rows <= (hd == 128 ? 48 : 64) ? 16 : 256;
+  return rows <= 8 ? 8 : rows <= (hd == 128 ? 32 : 48) ? 16 : 256;
 }
 
 template <int HD, bool FP8>

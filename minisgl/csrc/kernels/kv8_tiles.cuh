@@ -27,7 +27,7 @@ namespace msgl {
 
 constexpr int kKtRows = 256;
 constexpr int kKtThreads = 512;
-constexpr int kKtCost = 2;      // of a segment, in blocks
+constexpr int kKtCost = 3;      // of a segment, in blocks
 constexpr int kKtDescs = 4;     // segments looked up ahead
 constexpr int kKtSlots = 8;     // of scales
 // Offsets are moved where a weight would pass 2^15, so 2^9 lie between the largest one seen when they were set and that. (2^5 of
