@@ -29,7 +29,7 @@ MSGL_DEVICE Kv8Req kv8_request(const Kv8Attn& p, int b) {
   r.row = p.rows[b];
   r.q0 = min(max(a, 0), p.total_q);
   r.n = min(max(e, r.q0), p.total_q) - r.q0;
-  const bool ok = r.q0 == a && r.q0 + r.n == e && r.L >= 0 && r.L <= p.pt_width && (r.L == 0 || (r.row >= 0 && r.row < p.pt_rows));
+  const bool ok = r.q0 == a && r.q0 + r.n == e && (b > 0 || a == 0) && r.L >= 0 && r.L <= p.pt_width && (r.L == 0 || (r.row >= 0 && r.row < p.pt_rows));
   if (!ok) {
     report_error(kErrBounds, kBcAttnRow);
     r.L = 0;

@@ -130,6 +130,27 @@ def test_nothing_to_do():
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("dtype", FMTS)
+@pytest.mark.parametrize("n,nkv,hd", [(20001, 2, 128), (13001, 7, 64), (5001, 16, 128)])
+def test_many_rows(dtype, n, nkv, hd):
+    """Enough rows that a lane takes two: the same as the plain forms, whose steps round as the kernels' do."""
+    gen = torch.Generator().manual_seed(n)
+    k, v = (rows_of(gen, n, nkv, hd) for _ in range(2))
+    size = n // 16 * 16 + 16
+    cache, want = (ops.KV8Cache.alloc(size, nkv, hd, dtype, device) for device in ("cuda", "cpu"))
+    loc = torch.randperm(size, generator=gen)[:n].to(torch.int32)
+    loc[5] = -1
+    ops.store_kv8(k, v, want, loc)
+    loc = loc.cuda()
+    ops.store_kv8(k.cuda(), v.cuda(), cache, loc)
+    assert all(torch.equal(a.view(torch.uint8).cpu(), b.view(torch.uint8))
+               for a, b in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), (want.k, want.v, want.k_scale, want.v_scale)))
+    for got, codes, scale in zip(ops.load_kv8(cache, loc), (cache.k, cache.v), (cache.k_scale, cache.v_scale)):
+        x = codes[:, loc.long().clamp(min=0)].float() * scale[:, loc.long().clamp(min=0), None]
+        x[:, 5] = 0
+        assert torch.equal(got, x.transpose(0, 1).to(torch.bfloat16))
+
+
 def heads_case(T, nq, nkv, hd, norm, seed=0):
     gen = torch.Generator().manual_seed(seed)
     qkv = rows_of(gen, T, nq + 2 * nkv, hd).flatten(1).cuda()
@@ -232,6 +253,13 @@ def test_long_and_many(hint, dtype, hd, reqs, nq, nkv):
 
 
 @pytest.mark.parametrize("hint", HINTS)
+@pytest.mark.parametrize("nq,nkv", [(128, 1), (130, 2), (96, 2), (64, 64)])
+def test_groups_of_any_size(hint, nq, nkv):
+    c = Case([(1, 100), (5, 77), (0, 9), (3, 2), (2, 500)], nq, nkv, 64, torch.int8, 16, sinks=True, seed=nq).to("cuda")
+    c.check(c.call(max_q_len=hint))
+
+
+@pytest.mark.parametrize("hint", HINTS)
 @pytest.mark.parametrize("dtype", FMTS)
 @pytest.mark.parametrize("window", [1, 63, 64, 65, 200, 10**6])
 def test_windows(hint, dtype, window):
@@ -318,7 +346,8 @@ def test_entries_outside_their_tables_are_recorded(hint):
     want = c.call(max_q_len=hint)
     sound = [slice(2, None), slice(0, 2)]
     for name, at, value, keep in (("rows", 0, 99, sound[0]), ("rows", 0, -1, sound[0]), ("kv_lens", 0, 10**6, sound[0]),
-                                  ("kv_lens", 0, -4, sound[0]), ("cu_q", 3, 9, slice(0, 3)), ("cu_q", 0, -2, sound[0])):
+                                  ("kv_lens", 0, -4, sound[0]), ("cu_q", 3, 9, slice(0, 3)), ("cu_q", 0, -2, sound[0]),
+                                  ("cu_q", 0, 1, sound[0])):
         c = fresh()
         getattr(c, name)[at] = value
         got = c.call(max_q_len=hint)
