@@ -358,6 +358,14 @@ def _suite(a, c) -> None:
         2 * qkv.numel() * 2)
     k = torch.randn(T, nkv * hd, device=dev, dtype=bf)
     add("store_kv", lambda: ops.store_kv(k, k, kc, vc, loc), 4 * k.numel() * 2)
+    # the same into an 8-bit cache
+    c8 = ops.KV8Cache.alloc(slots, nkv, hd, torch.int8, dev)
+    k8 = k.view(T, nkv, hd)
+    row8 = hd + 4
+    add("qk_norm_rope_store_kv8", lambda: ops.qk_norm_rope_store_kv8(qkv, pos, cs, qn, qn, 1e-6, c8, loc, nq),
+        qkv.numel() * 2 + T * nq * hd * 2 + 2 * T * nkv * row8)
+    add("store_kv8", lambda: ops.store_kv8(k8, k8, c8, loc), 2 * T * nkv * (2 * hd + row8))
+    add("load_kv8", lambda: ops.load_kv8(c8, loc), 2 * T * nkv * (2 * hd + row8))
     gu = torch.randn(T, 2 * inter, device=dev, dtype=bf)
     add("silu_and_mul", lambda: ops.silu_and_mul(gu), gu.numel() * 2 * 3 // 2)
     # GEMMs: 1-SM (16 tokens, QKV), 2-SM gated gate_up (SiLU epilogue) and down_proj

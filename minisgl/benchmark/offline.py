@@ -101,6 +101,7 @@ def main(argv=None) -> dict:
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--dummy-weight", action="store_true")
     ap.add_argument("--max-running-requests", type=int, default=256)
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "int8", "fp8_e4m3"])
     ap.add_argument("--seed", type=int, default=0)
     a = ap.parse_args(argv)
 
@@ -112,7 +113,7 @@ def main(argv=None) -> dict:
 
     rng = random.Random(a.seed)
     llm = LLM(a.model, dtype=getattr(torch, a.dtype), device=a.device, use_dummy_weight=a.dummy_weight,
-              max_running_req=a.max_running_requests)
+              max_running_req=a.max_running_requests, kv_cache_dtype=a.kv_cache_dtype)
     vocab = llm.engine.model_config.vocab_size
     if a.dataset:
         tok = load_tokenizer(a.model)
