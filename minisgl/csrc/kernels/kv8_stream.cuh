@@ -13,6 +13,11 @@
 // Keys as the 16 rows of a product, since the query rows are often 8 at most: NR = 1 takes tiles of 8 rows, NR = 2 of 16.
 // Codes are exact in fp16, and the queries are, scaled by a power of two. Logits, sums and O are fp32.
 // A warp keeps its own maximum and sum; the four are joined when a segment ends (see kv8_plan.cuh).
+//
+// Measured (8 kv heads of 128, back to back in a graph): 4 requests of 100000 keys, int8, 148 us or 5.7 TB/s; 128 of 100 to 2048, e4m3,
+// 61 us or 4.8 TB/s, of which some 8 us are the plan, the first copies and the join of cut segments (a ring of 3 stages instead
+// of 4 takes 62). Two tiles of 16 rows (25 rows of 5 drafted tokens, 16 requests of 6000) take 94 us: there it is two warps a
+// scheduler, each waiting for its own products and conversions, that bound it (52% of the issue slots used).
 #pragma once
 #include "kv8.cuh"
 #include "kv8_plan.cuh"

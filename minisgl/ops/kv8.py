@@ -8,6 +8,7 @@ At head dim 128 a token takes 132 bytes per row instead of the 256 of a bf16 cac
 
     cache = ops.KV8Cache.alloc(num_slots, num_kv_heads, head_dim, torch.int8, device)
     ops.store_kv8(k, v, cache, out_loc)                   # bf16 [T, kv heads, head dim] into slots
+    q = ops.qk_norm_rope_store_kv8(qkv, positions, cos_sin, q_norm, k_norm, eps, cache, out_loc, num_heads)  # a layer's way in
     o = ops.attention_kv8(q, cache, page_table, rows, cu_q, kv_lens, page_size=64, max_q_len=1)
     k, v = ops.load_kv8(cache, slots)                     # bf16 again
 
@@ -15,9 +16,9 @@ CUDA tensors run the sm_100a kernels, CPU tensors the plain form in ``ops.refere
 CUDA graphs (lengths, tables and slots are read on the device); they keep no state of their own, so calls on
 several streams are independent. Equal calls give equal results.
 
-What is rounded on the GPU: codes are held exactly, queries too (in fp16, scaled by a power of two, where
+What is rounded on the GPU: codes are held exactly, queries too (for few rows in fp16, scaled by a power of two, where
 values below 2^-31 of the row's largest lose bits); scores, maxima and sums are fp32; the product of a
-probability and its value's scale is rounded once to fp16. Indexes that are outside their tables are never
+probability and its value's scale is rounded once to fp16, to 2^-11 of it or 2^-31 of the row's largest such product. Indexes that are outside their tables are never
 followed: see each operator for what such an entry does; the kernels record them in the device error word
 (``minisgl._native.cuda().get_error()``), plain forms raise.
 """
