@@ -127,19 +127,29 @@ MSGL_DEVICE void kt_store_p8(uint32_t taddr, const uint32_t (&r)[4]) {
                : "memory");
 }
 
-// A lane's four rows, 8 apart: their running offsets and this lane's part of their sums, the keys of the
-// block that they see, [first, end), and what their O has to be multiplied by first.
+// A lane's four rows, 8 apart: their positions, running offsets and this lane's part of their sums, and what their O has to be
+// multiplied by first.
 struct KtRows {
+  int pos[4];
   float m[4], l[4], alpha[4];
+};
+// The keys of a block, [first, end), that they see (worked out where a block is seen in part: eight registers less for the others).
+struct KtSeen {
   int first[4], end[4];
+  MSGL_DEVICE KtSeen(const KtRows& w, int k0, int window, bool part) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      first[k] = part && window > 0 ? max(0, w.pos[k] - window + 1 - k0) : 0;
+      end[k] = !part ? kKv8Block : w.pos[k] < k0 ? 0 : min(w.pos[k] - k0, kKv8Block - 1) + 1;
+    }
+  }
 };
 
-// Offsets with which the largest weight of this block's first `keys` is 2^kKtTop (see kKv8Top), for the rows that have a lower
-// one. (A compact loop, like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
-MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, int keys) {
+// Offsets with which the largest weight of this block is 2^kKtTop (see kKv8Top), for the rows that have a lower one. (A compact loop, like all that not every block needs: unrolled it comes out of L2 each time, and takes ten times as long.)
+MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, const KtSeen& seen, float qs, int t) {
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-  for (int n = 0; n < keys; n += 16) {
+  for (int n = 0; n < kKv8Block; n += 16) {
     uint32_t u[2][8];
     kt_load_s16(s_tmem + n, u[0]);
     kt_load_s16(s_tmem + n + (16u << 16), u[1]);
@@ -152,8 +162,8 @@ MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float q
       for (int k = 0; k < 4; ++k) {
         const uint32_t* s = &u[k >> 1][4 * y + 2 * (k & 1)];
         const float a = fmaf(__uint_as_float(s[0]) * ks.x, qs, lv.x), b = fmaf(__uint_as_float(s[1]) * ks.y, qs, lv.y);
-        if (c >= w.first[k] && c < w.end[k]) top[k] = fmaxf(top[k], a);
-        if (c + 1 >= w.first[k] && c + 1 < w.end[k]) top[k] = fmaxf(top[k], b);
+        if (c >= seen.first[k] && c < seen.end[k]) top[k] = fmaxf(top[k], a);
+        if (c + 1 >= seen.first[k] && c + 1 < seen.end[k]) top[k] = fmaxf(top[k], b);
       }
     }
   }
@@ -171,7 +181,7 @@ MSGL_DEVICE void kt_move(uint32_t s_tmem, const KtScales& sc, KtRows& w, float q
 }
 
 // The weights of a block that some of the lane's rows see in part only, over S's columns.
-MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t) {
+MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows& w, const KtSeen& seen, float qs, int t) {
 #pragma unroll 1
   for (int n = 0; n < kKv8Block; n += 16) {
     uint32_t u[2][8], pk[2][4];
@@ -187,8 +197,8 @@ MSGL_DEVICE void kt_weights_in_part(uint32_t s_tmem, const KtScales& sc, KtRows&
         const uint32_t* s = &u[k >> 1][4 * y + 2 * (k & 1)];
         const float base = w.m[k] == -INFINITY ? 0.f : w.m[k];
         float a = kv8_exp2(fmaf(__uint_as_float(s[0]) * ks.x, qs, -base)), b = kv8_exp2(fmaf(__uint_as_float(s[1]) * ks.y, qs, -base));
-        if (!(c >= w.first[k] && c < w.end[k])) a = 0.f;
-        if (!(c + 1 >= w.first[k] && c + 1 < w.end[k])) b = 0.f;
+        if (!(c >= seen.first[k] && c < seen.end[k])) a = 0.f;
+        if (!(c + 1 >= seen.first[k] && c + 1 < seen.end[k])) b = 0.f;
         w.l[k] += a + b;
         pk[k >> 1][2 * y + (k & 1)] = pack_half(a * vs.x, b * vs.y);
       }
@@ -244,34 +254,32 @@ MSGL_DEVICE bool kt_weights(uint32_t s_tmem, const KtScales& sc, const KtRows& w
 // A block of the lane's rows, which see all of it or (`part`) not: their weights over S's columns. New offsets first where rows
 // have none (`fresh`: they have seen no key yet), or weights beyond fp16: few blocks need any, and the others are spared the
 // maximum of their logits. Returns whether the rows have got factors for O.
-MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, bool part, bool fresh) {
+MSGL_DEVICE bool kt_softmax(uint32_t s_tmem, const KtScales& sc, KtRows& w, float qs, int t, int k0, int window, bool part, bool fresh) {
   float sum[4];
   uint32_t pk[2][16];
-  int keys = part || fresh ? kKv8Block : 0, moves = 0;
+  bool move = part || fresh, moved = false;
 #pragma unroll 1
   for (;;) {
-    if (keys > 0) {
-      if (moves == 0) {
+    if (move) {
+      const KtSeen seen(w, k0, window, part);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
+      for (int k = 0; k < 4; ++k) w.alpha[k] = 1.f;
+      kt_move(s_tmem, sc, w, seen, qs, t);
+      moved = true;
+      if (part) {
+        kt_weights_in_part(s_tmem, sc, w, seen, qs, t);
+        return true;
       }
-      kt_move(s_tmem, sc, w, qs, t, keys);
-      ++moves;
-      if (part) break;
     }
     const bool beyond = kt_weights(s_tmem, sc, w, qs, t, sum, pk);
-    if (keys == kKv8Block || !__any_sync(0xffffffffu, beyond)) break;
-    keys = kKv8Block;
+    if (moved || !__any_sync(0xffffffffu, beyond)) break;
+    move = true;
   }
-  if (part) {
-    kt_weights_in_part(s_tmem, sc, w, qs, t);
-  } else {
-    kt_store_p(s_tmem, pk[0]);
-    kt_store_p(s_tmem + (16u << 16), pk[1]);
+  kt_store_p(s_tmem, pk[0]);
+  kt_store_p(s_tmem + (16u << 16), pk[1]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
-  }
-  return moves > 0;
+  for (int k = 0; k < 4; ++k) w.l[k] += sum[k];
+  return moved;
 }
 
 template <int HD, bool FP8>
@@ -580,7 +588,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         continue;
       }
       KtRows w;
-      int qpos[4];
       int least = INT_MAX, most = 0;  // of the warp's rows' positions
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -588,15 +595,15 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         const bool in = rr < trows && x * trows + rr < D.nr;
         w.m[k] = -INFINITY;
         w.l[k] = 0.f;
-        qpos[k] = in ? D.L - D.n + kv8_token(p, D.r0 + x * trows + rr) : INT_MIN;
-        if (in) least = min(least, qpos[k]), most = max(most, qpos[k]);
+        w.pos[k] = in ? D.L - D.n + kv8_token(p, D.r0 + x * trows + rr) : INT_MIN;
+        if (in) least = min(least, w.pos[k]), most = max(most, w.pos[k]);
       }
       least = __reduce_min_sync(0xffffffffu, least);
       most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (qpos[k] == INT_MIN) qpos[k] = most;  // (a row that is none: as the last one)
-      bool fresh = true;  // rows without an offset, or limits of another block
+        if (w.pos[k] == INT_MIN) w.pos[k] = most;  // (a row that is none: as the last one)
+      bool fresh = true;  // rows without an offset
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
         if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1))) break;
@@ -606,13 +613,6 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         const int k0 = (D.blk + j) * kKv8Block;
         // does every row of the warp see every key?
         const bool part = !(least >= k0 + kKv8Block - 1 && (p.window <= 0 || most - p.window < k0));
-        if (part || fresh) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            w.first[k] = part && p.window > 0 ? max(0, qpos[k] - p.window + 1 - k0) : 0;
-            w.end[k] = !part ? kKv8Block : qpos[k] < k0 ? 0 : min(qpos[k] - k0, kKv8Block - 1) + 1;
-          }
-        }
         bool moved = false;
         if (k0 > most || (p.window > 0 && k0 + kKv8Block - 1 <= least - p.window)) {  // no row sees a key of this block
           uint32_t none[16];
@@ -621,21 +621,18 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           kt_store_p(ts + (uses & 1) * 64, none);
           kt_store_p(ts + (uses & 1) * 64 + (16u << 16), none);
         } else {
-          moved = kt_softmax(ts + (uses & 1) * 64, sc, w, qs, t4, part, fresh);
+          moved = kt_softmax(ts + (uses & 1) * 64, sc, w, qs, t4, k0, p.window, part, fresh);
         }
-        // (first and end stay those of a whole block until the next one that is seen in part)
-        if (part || fresh) {
-          fresh = __any_sync(0xffffffffu, w.m[0] == -INFINITY || w.m[1] == -INFINITY || w.m[2] == -INFINITY || w.m[3] == -INFINITY);
-          if (part) fresh = true;
-        }
+        if (fresh) fresh = __any_sync(0xffffffffu, w.m[0] == -INFINITY || w.m[1] == -INFINITY || w.m[2] == -INFINITY || w.m[3] == -INFINITY);
         if ((sc.bad[0] | sc.bad[1]) != 0) {  // a key that has no finite scale makes the rows that see it no numbers
+          const KtSeen seen(w, k0, p.window, part);
           const uint64_t bad = sc.bad[0] | (uint64_t)sc.bad[1] << 32;
 #pragma unroll 1
           for (int c = 0; c < kKv8Block; ++c)
             if (bad >> c & 1) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                if (c >= w.first[k] && c < w.end[k]) w.l[k] = __int_as_float(0x7fc00000);
+                if (c >= seen.first[k] && c < seen.end[k]) w.l[k] = __int_as_float(0x7fc00000);
             }
         }
         if (j > 0 && moved && __any_sync(0xffffffffu, w.alpha[0] != 1.f || w.alpha[1] != 1.f || w.alpha[2] != 1.f || w.alpha[3] != 1.f)) {
