@@ -83,10 +83,12 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kKsWarps);
     }
+#pragma unroll 1
     for (int i = 0; i < kKsDescs; ++i) {
       mbar_init(&dfull[i], 1);
       mbar_init(&dempty[i], kKsWarps);
@@ -117,6 +119,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
     if (u < pl.u1) tiles = kv8_tiles(r, G, R);
     int i = 0, issued = 0;
     uint32_t last = 0;
+#pragma unroll 1
     for (; ok && u < pl.u1; ++i) {
       const Kv8Tile k = kv8_tile(p, r, G, R, t);
       // blocks [from, to) of the segment: its first kKsCost units are none
@@ -157,6 +160,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         return g < pages_end && j + lane / gpb * kKsCopies < to - from ? p.page_table[(int64_t)r.row * p.pt_stride + (int64_t)g * page] : -1;
       };
       int next = look_up(j0), slots = -1;
+#pragma unroll 1
       for (int j = j0, at = 0; j < to - from; j += kKsCopies, ++at) {
         if (at % mine == 0) {
           slots = next;
@@ -168,7 +172,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
         ok = kv8_wait_warp(&empty[stage], ((x / C::kStages) & 1) ^ 1);
         if (!ok) break;
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
-        kv8_copy_block<HD>(p, &tc, &ts, ring + stage * C::kStage, scales + stage * (C::kScales / 4), &full[stage], h, slots,
+        kv8_copy_block<HD, 4>(p, &tc, &ts, ring + stage * C::kStage, scales + stage * (C::kScales / 4), &full[stage], h, slots,
                            at % mine * gpb, pages);
         last = x;
         ++issued;
@@ -198,6 +202,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       }
     } else if (lane == 0) {  // given up: this warp's copies in flight land before the CTA's memory goes
       kv8_gave_up(700);
+#pragma unroll 1
       for (int n = 0; n < min(issued, C::kStages / kKsCopies); ++n) {
         const uint32_t x = last - n * kKsCopies;
         kv8_wait(&full[x % C::kStages], (x / C::kStages) & 1);
@@ -215,6 +220,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
   const uint32_t ks_at = (uint32_t)(base + order.scales * p.page + g) * 4, vs_at = (uint32_t)(base + (order.scales ^ 1) * p.page + g) * 4;
   uint32_t seq = 0;  // stages gone through
   bool dead = false;
+#pragma unroll 1
   for (int i = 0;; ++i) {
     const int d = i % kKsDescs;
     if (!dead && !kv8_wait_warp(&dfull[d], (i / kKsDescs) & 1)) { dead = true; *abort_flag = 1; }
@@ -276,6 +282,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       for (int j = 0; j < NK; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
     }
 
+#pragma unroll 1
     for (int j = 0; j < D.nb && !dead; ++j) {
       const uint32_t at = seq + j, stage = at % C::kStages;
       if (!kv8_wait_warp(&full[stage], (at / C::kStages) & 1)) { dead = true; *abort_flag = 1; break; }
@@ -431,6 +438,7 @@ kv8_stream_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant_
       if (dead) kv8_gave_up(710);
       break;
     }
+#pragma unroll 1
     for (int idx = ctid; idx < D.nr * (HD / 4); idx += kKsWarps * 32) {
       const int rr = idx / (HD / 4), c4 = idx % (HD / 4);
       float mx = -INFINITY;

@@ -316,28 +316,34 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (a warp's number, known as one)
   if (warp == 1) {
     if (lane == 0) {
+#pragma unroll 1
       for (int i = 0; i < C::kStages; ++i) {
         mbar_init(&kfull[i], 4);
         mbar_init(&kempty[i], 2);
         mbar_init(&vfull[i], 4);
         mbar_init(&vempty[i], 2);
       }
+#pragma unroll 1
       for (int i = 0; i < C::kRaw; ++i) {
         mbar_init(&rfull[i], 1);
         mbar_init(&rempty[i], 4);
       }
+#pragma unroll 1
       for (int i = 0; i < kKtSlots; ++i) mbar_init(&scfull[i], 4);
+#pragma unroll 1
       for (int i = 0; i < kKtDescs; ++i) {
         mbar_init(&dfull[i], 1);
         mbar_init(&dempty[i], 2 + 1 + 8 + 4);
       }
       mbar_init(qfull, 1);
       mbar_init(qempty, 2);
+#pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         mbar_init(&sfull[i], 1);
         mbar_init(&pfull[i], 4);
         mbar_init(&pvdone[i], 1);
       }
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) mbar_init(&ofree[i], 4);
       fence_barrier_init();
     }
@@ -350,6 +356,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     prefetch_tmap(&tq);
   }
   const int G = p.nq / p.nkv, tokens = 128 / G, trows = tokens * G, R = 2 * trows;  // of a tile, of a segment
+#pragma unroll 1
   for (int i = threadIdx.x; i < (128 - trows) * 8 * 2 * (HD / 64); i += kKtThreads) {  // rows that no query is copied to
     const int half = i / ((128 - trows) * 8), at = i % ((128 - trows) * 8);
     *reinterpret_cast<uint4*>(smem + C::kOffQ + half * C::kQHalf + trows * 128 + at * 16) = make_uint4(0, 0, 0, 0);
@@ -376,6 +383,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     bool ok = true;
     Kv8Req r = pl.r;
     if (u < pl.u1) tiles = kv8_tiles(r, G, R);
+#pragma unroll 1
     for (; ok && u < pl.u1; ++i) {
       const Kv8Tile k = kv8_tile(p, r, G, R, t);
       // blocks [from, to) of the segment: its first kKtCost units are none
@@ -407,6 +415,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         return g < pages_end && j + lane / gpb < to - from ? p.page_table[(int64_t)r.row * p.pt_stride + (int64_t)g * page] : -1;
       };
       int next = look_up(0), page_slots = -1;
+#pragma unroll 1
       for (int j = 0; j < to - from; ++j) {
         if (j % mine == 0) {
           page_slots = next;
@@ -420,7 +429,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
           break;
         }
         const int pages = max(0, min(gpb, pages_end - (page0 + j * gpb)));
-        kv8_copy_block<HD>(p, &tc, &ts, raw + stage * C::kRawStage, raw_scales + stage * (C::kRawScales / 4), &rfull[stage], h, page_slots,
+        kv8_copy_block<HD, 1>(p, &tc, &ts, raw + stage * C::kRawStage, raw_scales + stage * (C::kRawScales / 4), &rfull[stage], h, page_slots,
                            j % mine * gpb, pages);
       }
       if (!ok) break;
@@ -448,6 +457,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
         }
       } else {  // given up: the copies in flight land before the CTA's memory goes
         kv8_gave_up(720);
+#pragma unroll 1
         for (uint32_t n = 1; n <= min(seq, (uint32_t)C::kRaw); ++n) {
           const uint32_t x = seq - n;
           kv8_wait(&rfull[x % C::kRaw], (x / C::kRaw) & 1);
@@ -557,6 +567,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       if (i > 0 && !(ok = kv8_wait_warp(qempty, (i - 1) & 1))) break;
       if (elect_one()) {
         mbar_expect_tx(qfull, tiles * trows * HD * 2);
+#pragma unroll 1
         for (int y = 0; y < tiles * (HD / 64); ++y)
           tma_load_3d(smem + C::kOffQ + y * C::kQHalf, &tq, qfull, y % (HD / 64) * 64, D.h * G, tok + y / (HD / 64) * tokens);
         mbar_arrive(&dempty[d]);
@@ -576,6 +587,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     const float qs = p.scale * kKv8Log2e;
     uint32_t g = 0, uses = 0;
     bool ok = true;
+#pragma unroll 1
     for (int i = 0; ok; ++i) {
       const int d = i % kKtDescs;
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
@@ -604,6 +616,7 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
       for (int k = 0; k < 4; ++k)
         if (w.pos[k] == INT_MIN) w.pos[k] = most;  // (a row that is none: as the last one)
       bool fresh = true;  // rows without an offset
+#pragma unroll 1
       for (int j = 0; j < D.nb; ++j, ++g) {
         // (S first: a tile that sat out the last segments could take an earlier block's turn of the scales for its own)
         if (!(ok = kv8_wait_warp(&sfull[2 * x + (uses & 1)], (uses >> 1) & 1))) break;
@@ -737,11 +750,13 @@ kv8_tiles_kernel(const __grid_constant__ CUtensorMap tc, const __grid_constant__
     const int part = lane & 3, key8 = (lane >> 3) ^ (lane & 4 ? 5 : 0);
     uint32_t g = 0;
     bool ok = true;
+#pragma unroll 1
     for (int i = 0; ok; ++i) {
       const int d = i % kKtDescs;
       if (!(ok = kv8_wait_warp(&dfull[d], (i / kKtDescs) & 1))) break;
       const KtDesc D = descs[d];
       if (D.nb == 0) break;
+#pragma unroll 1
       for (int j = 0; j < D.nb; ++j, ++g) {
         const uint32_t rs = g % C::kRaw, st = g % C::kStages, ph = (g / C::kStages) & 1;
         if (!(ok = kv8_wait_warp(&rfull[rs], (g / C::kRaw) & 1))) break;
