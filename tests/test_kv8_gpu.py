@@ -419,6 +419,28 @@ def test_calls_on_several_streams():
             assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
+@pytest.mark.parametrize("hint", HINTS)
+def test_cache_beyond_32_bits(hint):
+    """4.6 GB of codes each: the last pages give what the same rows give in a small cache."""
+    nq, nkv, hd, n, slots = 32, 16, 128, 300, 2_240_000
+    gen = torch.Generator().manual_seed(5)
+    k, v = (rows_of(gen, n, nkv, hd).cuda() for _ in range(2))
+    q = torch.randn(2, nq, hd, generator=gen).to(torch.bfloat16).cuda()
+    rows, ends, lens = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0], [0, 2], [n]))
+    got = []
+    for size in (512, slots):
+        cache = ops.KV8Cache.alloc(size, nkv, hd, torch.int8)
+        at = torch.arange(size - 512, size, dtype=torch.int32, device="cuda").view(-1, 64)[torch.arange(7, -1, -1, device="cuda")].flatten()
+        ops.store_kv8(k, v, cache, at[:n].contiguous())
+        back = ops.load_kv8(cache, at[:n].contiguous())
+        got.append((ops.attention_kv8(q, cache, at[None], rows, ends, lens, page_size=64, max_q_len=hint), *back))
+        assert not cache.k[0, : size - 512].any()
+        del cache
+    assert got[0][0].isfinite().all() and got[0][0].any()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_as_a_model_uses_them():
     """A prompt in two chunks, then single tokens: every step's rows are stored, then attended to."""
     torch.manual_seed(0)
