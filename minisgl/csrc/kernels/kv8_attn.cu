@@ -102,7 +102,7 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
   const Kv8Scratch scratch = kv8_scratch<kKtRows, HD>(ws, ctas);
   if (msgl_launch(kernel, dim3(ctas), dim3(kKtThreads), C::kSmem, s, 1, tc, ts, tq, p, order, scratch) != cudaSuccess) return 4;
   ++*launches;
-  if (msgl_launch(kv8_join_kernel<kKtRows, HD>, dim3(ctas, 8), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
+  if (msgl_launch(kv8_join_kernel<kKtRows, HD>, dim3(ctas, 32), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
   ++*launches;
   return 0;
 }
