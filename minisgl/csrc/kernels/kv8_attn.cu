@@ -102,6 +102,7 @@ int tiles_form(const Kv8Attn& p, void* ws, int* launches, cudaStream_t s) {
   const Kv8Scratch scratch = kv8_scratch<kKtRows, HD>(ws, ctas);
   if (msgl_launch(kernel, dim3(ctas), dim3(kKtThreads), C::kSmem, s, 1, tc, ts, tq, p, order, scratch) != cudaSuccess) return 4;
   ++*launches;
+  // (32: two rows a warp; 8 take 7 us longer after short prompts, 64 start too many blocks where few are cut)
   if (msgl_launch(kv8_join_kernel<kKtRows, HD>, dim3(ctas, 32), dim3(128), 0, s, 1, p, scratch) != cudaSuccess) return 4;
   ++*launches;
   return 0;

@@ -19,7 +19,7 @@
 // Numerics as in kv8_stream.cuh, with kKtTop for kKv8Top: room for offsets that are not moved at every block.
 //
 // Measured (40 heads over 8 of 128): a chunk of 2048 tokens after 30000 cached ones takes 1520 us in int8, 856 TFLOP/s, before the
-// power limit lowers the clock; 28 prompts of 100 to 1024 tokens 308 us in e4m3. A block of 256 x 64 takes some 2700 cycles, of which the tensor core is busy for 40%; the
+// power limit lowers the clock; 28 prompts of 100 to 1024 tokens 302 us in e4m3. A block of 256 x 64 takes some 2700 cycles, of which the tensor core is busy for 40%; the
 // softmax has 2100 of work (half of it waits for the 2^x units and issue slots that two of its warps share with a converting one), and
 // the rest is its wait for S. Code that few blocks run costs its way from the L2 cache each time, hence the loops in it.
 #pragma once

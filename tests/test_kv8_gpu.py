@@ -253,6 +253,22 @@ def test_long_and_many(hint, dtype, hd, reqs, nq, nkv):
 
 
 @pytest.mark.parametrize("hint", HINTS)
+@pytest.mark.parametrize("B,longest,tokens,nkv,window", [
+    (300, 300, 1, 2, -1), (700, 200, 2, 3, -1), (150, 320, 9, 4, -1), (90, 510, 130, 4, -1), (60, 900, 200, 3, 100), (513, 64, 1, 8, 20),
+])
+def test_many_short_requests(hint, B, longest, tokens, nkv, window):
+    """More requests than a CTA has threads, more segments than there are CTAs."""
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(1, longest + 1, (B,), generator=gen).tolist()
+    reqs = [(min(1 + (7 * i) % tokens, n), n) for i, n in enumerate(lens)]
+    reqs[3], reqs[B // 2] = (0, 10), (1, 0)
+    c = Case(reqs, 4 * nkv, nkv, 64, torch.int8, 16, window, seed=B).to("cuda")
+    got = c.call(max_q_len=hint)
+    c.check(got)
+    assert torch.equal(c.call(max_q_len=hint), got)
+
+
+@pytest.mark.parametrize("hint", HINTS)
 @pytest.mark.parametrize("nq,nkv", [(128, 1), (130, 2), (96, 2), (64, 64)])
 def test_groups_of_any_size(hint, nq, nkv):
     c = Case([(1, 100), (5, 77), (0, 9), (3, 2), (2, 500)], nq, nkv, 64, torch.int8, 16, sinks=True, seed=nq).to("cuda")
