@@ -152,32 +152,6 @@ __global__ void store_kv_kernel(const uint4* __restrict__ k, const uint4* __rest
 }
 
 // ------------------------------------------------------------------------------ qk norm + rope + store
-// A head's row through RMSNorm (with weights) and RoPE, in the lanes' order below.
-template <int E>
-MSGL_DEVICE void norm_rope(float (&a)[E], float (&b)[E], const __nv_bfloat16* nw, float eps, const float* cs, int lane) {
-  constexpr int HD = 64 * E;
-  if (nw != nullptr) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
-    ss = warp_sum(ss);
-    const float inv = rsqrtf(ss / HD + eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      // match the reference rounding: normalized values are rounded to bf16 before RoPE
-      a[e] = __bfloat162float(__float2bfloat16(a[e] * inv * __bfloat162float(nw[lane * E + e])));
-      b[e] = __bfloat162float(__float2bfloat16(b[e] * inv * __bfloat162float(nw[HD / 2 + lane * E + e])));
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = lane * E + e;
-    const float c = cs[i], s = cs[HD / 2 + i], x = a[e], y = b[e];
-    a[e] = x * c - y * s;
-    b[e] = y * c + x * s;
-  }
-}
-
 // One warp per (token, head) over the q, k and v heads of the merged qkv row. Lane l owns
 // elements [l*E, l*E+E) of the first half and the same offsets of the second half (E = hd/64),
 // so each neox-style rotation pair (i, i + hd/2) lives in one thread.
@@ -222,15 +196,58 @@ __global__ void qk_norm_rope_store_kernel(__nv_bfloat16* __restrict__ q_out,
     return;
   }
   const bool is_q = h < nq;
-  norm_rope<E>(a, b, is_q ? q_norm : k_norm, eps, cos_sin + (size_t)positions[t] * HD, lane);
+  const __nv_bfloat16* nw = is_q ? q_norm : k_norm;
+  if (nw != nullptr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
+    ss = warp_sum(ss);
+    const float inv = rsqrtf(ss / HD + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      // match the reference rounding: normalized values are rounded to bf16 before RoPE
+      a[e] = __bfloat162float(__float2bfloat16(a[e] * inv * __bfloat162float(nw[lane * E + e])));
+      b[e] = __bfloat162float(__float2bfloat16(b[e] * inv * __bfloat162float(nw[HD / 2 + lane * E + e])));
+    }
+  }
+  const int pos = positions[t];
+  const float* cs = cos_sin + (size_t)pos * HD;
   __nv_bfloat16* dst;
   if (is_q) dst = q_out + ((size_t)t * nq + h) * HD;
   else dst = k_cache + (int64_t)out_loc[t] * cache_stride + (size_t)(h - nq) * HD;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int i = lane * E + e;
-    dst[i] = __float2bfloat16(a[e]);
-    dst[HD / 2 + i] = __float2bfloat16(b[e]);
+    const float c = cs[i], s = cs[HD / 2 + i];
+    dst[i] = __float2bfloat16(a[e] * c - b[e] * s);
+    dst[HD / 2 + i] = __float2bfloat16(b[e] * c + a[e] * s);
+  }
+}
+
+// A head's row through RMSNorm (with weights) and RoPE, in the same order of lanes and with the roundings that the kernel above has
+// (its products and sums as the compiler joins them, written out).
+template <int E>
+MSGL_DEVICE void norm_rope(float (&a)[E], float (&b)[E], const __nv_bfloat16* nw, float eps, const float* cs, int lane) {
+  constexpr int HD = 64 * E;
+  if (nw != nullptr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ss += a[e] * a[e] + b[e] * b[e];
+    ss = warp_sum(ss);
+    const float inv = rsqrtf(ss / HD + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      // match the reference rounding: normalized values are rounded to bf16 before RoPE
+      a[e] = __bfloat162float(__float2bfloat16(a[e] * inv * __bfloat162float(nw[lane * E + e])));
+      b[e] = __bfloat162float(__float2bfloat16(b[e] * inv * __bfloat162float(nw[HD / 2 + lane * E + e])));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = lane * E + e;
+    const float c = cs[i], s = cs[HD / 2 + i], x = a[e], y = b[e];
+    a[e] = fmaf(x, c, -__fmul_rn(y, s));
+    b[e] = fmaf(y, c, __fmul_rn(x, s));
   }
 }
 
