@@ -4,8 +4,6 @@ command line and all resolve to it (reference registry: python/minisgl/attention
 
 from __future__ import annotations
 
-from minisgl.core import get_global_ctx
-from minisgl.kvcache.kv8_pool import KV8Pool
 from minisgl.utils import Registry
 
 from .base import BaseAttnBackend, BaseAttnMetadata
@@ -22,12 +20,11 @@ def validate_attn_backend(name: str) -> str:
     return name
 
 
-def create_attention_backend(name: str, model_config, device) -> BaseAttnBackend:
-    """The backend for the current context's KV pool."""
+def create_attention_backend(name: str, model_config, device, kv8: bool = False) -> BaseAttnBackend:
+    """``kv8``: the KV pool is an 8-bit one (``kvcache.kv8_pool.KV8Pool``)."""
     validate_attn_backend(name)
     return PagedAttentionBackend(
-        model_config.num_qo_heads, model_config.num_kv_heads, model_config.head_dim, device,
-        kv8=isinstance(getattr(get_global_ctx(), "kv_cache", None), KV8Pool),
+        model_config.num_qo_heads, model_config.num_kv_heads, model_config.head_dim, device, kv8
     )
 
 

@@ -117,7 +117,7 @@ class Engine:
 
         # ----------------------------------------------------------------- backends
         self.ctx.attn_backend = self.attn_backend = create_attention_backend(
-            config.attention_backend, self.model_config, self.device
+            config.attention_backend, self.model_config, self.device, kv8=self.kv_dtype in KV8_DTYPES.values()
         )
         if self.model_config.is_moe:
             from minisgl.moe import create_moe_backend
